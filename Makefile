@@ -17,7 +17,7 @@ ARCH := -gencode arch=compute_100a,code=sm_100a
 NVFLAGS := -std=c++20 -O3 $(ARCH) -lineinfo -Xcompiler -fPIC -Xcompiler -Wall \
            --expt-relaxed-constexpr -Iinclude -I$(CSRC)
 CU_SRCS := $(CSRC)/decode.cu $(CSRC)/decode_bf16.cu $(CSRC)/prefill.cu $(CSRC)/forward.cu $(CSRC)/gemm.cu \
-           $(CSRC)/abi.cu
+           $(CSRC)/chunk.cu $(CSRC)/logits.cu $(CSRC)/abi.cu
 HOST_SRCS := $(HOST)/ops_gpu.cpp
 CU_OBJS := $(patsubst $(CSRC)/%.cu,_build/%.o,$(CU_SRCS))
 HOST_OBJS := $(patsubst $(HOST)/%.cpp,_build/host_%.o,$(HOST_SRCS))

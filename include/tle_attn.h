@@ -319,6 +319,97 @@ int tle_prefill(float* out, const float* q, const float* k, const float* v, floa
                 float* value_cache, int layer, int pos0, int n_tokens, int n_ctx,
                 const tle_shape_t* shape, void* workspace, size_t workspace_bytes, void* stream);
 
+/* ---- chunks of new tokens over a paged KV cache ----
+ * No counterpart in the reference (it feeds a prompt token by token into one
+ * contiguous cache, generate.cpp:52-59).  A batch holds one chunk of
+ * n_tokens >= 0 new tokens per sequence, behind pos cached rows: 1 token is a
+ * decode step, a few are a guess to be checked, many a prompt or a piece of
+ * one.  The tokens of all chunks are packed in sequence order: token i of the
+ * batch is row i of q, k, v and out.  A step is, per layer,
+ *   tle_append_paged / tle_append_bf16_paged   (rope q and k, store k and v),
+ *   tle_prefill_bf16_paged                     (attention over bf16 pools).
+ * Any n_head that is a multiple of n_head_kv (at most 128 query heads per KV
+ * head), head_dim 64.  Activations (q, k, v, out) are fp32 or bf16. */
+enum {
+    TLE_ACT_F32 = 0,
+    TLE_ACT_BF16 = 1
+};
+
+/* One sequence's chunk: token t of the chunk is appended at row pos + t. */
+typedef struct {
+    const int32_t* pages; /* DEVICE int32 [n_pages]: page ids in [0, pool n_pages)      */
+    int32_t n_pages;      /* entries in pages; need n_pages * page_rows >= pos + n_tokens */
+    int32_t pos;          /* rows already in the cache, >= 0                            */
+    int32_t n_tokens;     /* new tokens, >= 0                                           */
+    int32_t reserved;     /* 0                                                          */
+} tle_paged_chunk_t;
+
+/* What tle_chunk_desc_paged found out about a batch; the calls below take it
+ * beside the device copy of the descriptor it belongs to. */
+typedef struct {
+    int32_t n_seqs, n_tokens;      /* sequences; tokens of all chunks                  */
+    int32_t n_head, n_head_kv;     /* the shape that the descriptor was made for       */
+    int32_t page_rows;
+    int32_t n_ctas, n_segs;        /* attention: CTAs, and their pieces of work        */
+    int32_t n_merge, merge_rows;   /* row blocks split over pieces; rows of the largest */
+    int32_t reserved;
+    int64_t part_rows;             /* partial result rows in the workspace             */
+} tle_chunk_plan_t;
+
+/* Bytes that suffice for the descriptor of such a batch (0: bad arguments,
+ * see tle_last_error). */
+size_t tle_chunk_desc_bytes(const tle_shape_t* shape, const tle_paged_chunk_t* chunks, int n_seqs,
+                            int max_ctas);
+
+/* Builds the descriptor in HOST memory from host-side chunk records (the page
+ * tables stay on the device): the place of every token, and the attention's
+ * work split evenly over about one CTA per SM (max_ctas > 0: at most that
+ * many).  The caller copies desc_host to device memory unchanged (16-byte
+ * aligned).  At most 2^31 - 1 rows of q heads per chunk and tokens in all. */
+int tle_chunk_desc_paged(const tle_shape_t* shape, int page_rows, const tle_paged_chunk_t* chunks,
+                         int n_seqs, int max_ctas, void* desc_host, size_t desc_bytes,
+                         tle_chunk_plan_t* plan);
+
+/* For every token i of the batch, at position p: if flags & TLE_DECODE_ROTATE,
+ * rope(q_i, k_i, p) with the decode's angles; q_out_i = q_i in the type of q
+ * (fp32 or bf16); row p of its sequence in layer `layer` of the pools = k_i,
+ * v_i, rounded once to the pool's type.  q and q_out may both be NULL (k and
+ * v only) and may be the same buffer.  Row i of q is at q + i * q_stride
+ * elements, likewise k and v; strides are multiples of 8, at least the row's
+ * n_head * 64 (n_head_kv * 64) elements; q_out is packed.  Two tokens of a
+ * batch must not share a row of the pools.  A page id outside the pool is not
+ * dereferenced (0x105, its rows are not stored); a batch without tokens does
+ * nothing.  Other flag bits are rejected with TLE_ERR_INVALID. */
+int tle_append_paged(const tle_shape_t* shape, const tle_page_pool_t* pool, const tle_chunk_plan_t* plan,
+                     const void* desc_dev, const void* q, int64_t q_stride, const void* k,
+                     int64_t k_stride, const void* v, int64_t v_stride, void* q_out, int act_type,
+                     int layer, int flags, void* stream);
+int tle_append_bf16_paged(const tle_shape_t* shape, const tle_page_pool_bf16_t* pool,
+                          const tle_chunk_plan_t* plan, const void* desc_dev, const void* q,
+                          int64_t q_stride, const void* k, int64_t k_stride, const void* v,
+                          int64_t v_stride, void* q_out, int act_type, int layer, int flags,
+                          void* stream);
+
+/* Scratch of tle_prefill_bf16_paged for this plan (partial results of row
+ * blocks that several CTAs share; may be 0). */
+size_t tle_prefill_bf16_paged_workspace_bytes(const tle_chunk_plan_t* plan);
+
+/* Causal attention of the chunks over the bf16 pools: token t of a chunk
+ * attends to rows 0 .. pos + t of its sequence, its own chunk's rows (stored
+ * before by tle_append_bf16_paged) among them; q already rotated.  Row i of
+ * out at out + i * out_stride elements, in the type of q; strides as above.
+ * With bf16 activations the softmax weights enter the tensor cores as bf16
+ * (bf16 precision); with fp32 activations q and the weights enter as sums of
+ * three bf16 numbers each, so the result is that of 32-bit arithmetic on the
+ * bf16 rows.  Rows of the pools that no token attends to are never part of a
+ * result, whatever they hold.  A page id outside the pool is not dereferenced
+ * (0x105, its rows count as zeros).  out rows behind the last token are left
+ * as they are.  Calls that share a workspace must not overlap on the GPU. */
+int tle_prefill_bf16_paged(const tle_shape_t* shape, const tle_page_pool_bf16_t* pool,
+                           const tle_chunk_plan_t* plan, const void* desc_dev, const void* q,
+                           int64_t q_stride, void* out, int64_t out_stride, int act_type, int layer,
+                           void* workspace, size_t workspace_bytes, void* stream);
+
 /* ---- multi-GPU sequence partition ---- */
 
 /* Greedy longest-processing-time assignment of sequences to n_ranks GPUs,

@@ -79,6 +79,44 @@ int tle_sample_temperature(float* logits, int n_vocab, float temperature, float 
 int tle_sample_top_p(float* logits, int n_vocab, float temperature, float top_p, float r,
                      int32_t* token, void* stream);
 
+/* The rules that tle_logits_adjust applies to each row of a batch of logits
+ * (no reference counterpart: its samplers take the raw logits).  Device
+ * pointers; a group whose first pointer is NULL is left out. */
+typedef struct {
+    /* The tokens of row r so far: tokens[token_start[r] .. token_start[r + 1]),
+     * the first n_prompt[r] of them given and the rest made (n_prompt NULL:
+     * none given). */
+    const int32_t* tokens;      /* [n_tokens] */
+    const int32_t* token_start; /* [n_rows + 1] */
+    const int32_t* n_prompt;    /* [n_rows] or NULL */
+    /* [n_rows] each, or NULL: no such penalty. */
+    const float* repetition;    /* tokens so far: x > 0 ? x / repetition : x * repetition */
+    const float* frequency;     /* made tokens:   x - frequency * (times made)            */
+    const float* presence;      /* made tokens:   x - presence                            */
+    /* Biases of row r: x + bias_values[i] for the token bias_tokens[i], i in
+     * [bias_start[r], bias_start[r + 1]); a token listed several times gets
+     * their sum, added in the list's order. */
+    const int32_t* bias_tokens; /* [n_biases] */
+    const float* bias_values;   /* [n_biases] */
+    const int32_t* bias_start;  /* [n_rows + 1] */
+    /* Token t of row r may be sampled if bit t % 32 of
+     * allowed[r * allowed_stride + t / 32] is set; otherwise its logit
+     * becomes -inf, whatever it was. */
+    const uint32_t* allowed;
+    int64_t allowed_stride;     /* words, >= ceil(n_vocab / 32) */
+    int32_t n_tokens, n_biases; /* entries of the two lists: starts and ends are cut to them */
+} tle_logit_rules_t;
+
+/* out[r][t] = logits[r][t] under row r's rules, in the order repetition,
+ * frequency, presence, biases, mask; n_rows rows of n_vocab logits, row r at
+ * r * out_stride (r * logits_stride) elements, what lies between the rows is
+ * left as it is.  out may be logits, with the same stride.  Ids outside
+ * [0, n_vocab) are skipped and reported through tle_device_error (0x106); a list whose
+ * start lies behind its end counts as empty.  A row whose mask allows nothing
+ * is all -inf.  Run it before tle_sample_*. */
+int tle_logits_adjust(float* out, int64_t out_stride, const float* logits, int64_t logits_stride,
+                      int n_rows, int n_vocab, const tle_logit_rules_t* rules, void* stream);
+
 /* ---- forward() ---- */
 
 typedef struct {

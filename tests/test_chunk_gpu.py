@@ -1,0 +1,507 @@
+"""Chunks of new tokens over a paged cache (tle_append_paged,
+tle_append_bf16_paged, tle_prefill_bf16_paged) against the formulas in 64 bits.
+
+Tolerances, per value (u = half a step of a type, relative: bf16 2^-8, fp32
+2^-24):
+* append: the angle is the 32-bit number fl32(pos * f_i) by definition; sine
+  and cosine are off by 2 ulp (2^-23) at most, the two products and their sum
+  by a rounding each, so a rotated element is within (|a| + |b|) 2^-22 of the
+  formula, plus u of the stored type.
+* attend: a score is a sum of 64 products in 32 bits: off by at most
+  ds = 2^-17 sum|q k| / 8 with the tensor cores' truncating sums; a weight is
+  then off by 2 (ds + |s| 2^-23 + 2^-22) relative (numerator and sum), and the
+  sum over rows adds (rows / 16 + 16) 2^-23; with bf16 activations a weight is
+  rounded to bf16 (2^-8) after an exponential good to 2^-13.  All of it times
+  sum w |v|; the result is rounded once to the type of q.
+"""
+import os
+import sys
+
+import numpy as np
+import pytest
+
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+sys.path.insert(0, os.path.join(ROOT, "tinyllama-engine_b200"))
+
+pytestmark = pytest.mark.gpu
+
+HD, BASE = 64, 10000.0
+U = {"f32": 2.0 ** -24, "bf16": 2.0 ** -8}
+
+
+def dtype(name):
+    import torch
+    return {"f32": torch.float32, "bf16": torch.bfloat16}[name]
+
+
+class Case:
+    """A paged cache of random rows and a batch over it, on the GPU."""
+
+    def __init__(self, pos, new, heads=(32, 4), page=64, act="f32", pool="bf16", layers=2, seed=0, spare=3,
+                 pad=0, max_ctas=0, scale=1.0):
+        import torch
+        import tle
+        self.pos, self.new, self.heads, self.page, self.act = list(pos), list(new), heads, page, act
+        self.H, self.KH = heads
+        self.layers, self.layer = layers, layers - 1
+        g = torch.Generator(device="cuda").manual_seed(seed)
+        need = [-(-(p + m) // page) for p, m in zip(pos, new)]
+        n_pages = sum(need) + spare
+        ids = torch.randperm(n_pages, generator=g, device="cuda").to(torch.int32)
+        self.tables, at = [], 0
+        for k in need:
+            self.tables.append(ids[at:at + k].clone())
+            at += k
+        self.free = ids[at:]
+        shape = tle.Shape(layers, self.H, self.KH, HD, BASE)
+        self.cache = tle.PagedKVCache(n_pages, page, shape, dtype=dtype(pool))
+        self.cache.key_pool.copy_(torch.randn(self.cache.key_pool.shape, generator=g, device="cuda"))
+        self.cache.value_pool.copy_(torch.randn(self.cache.value_pool.shape, generator=g, device="cuda"))
+        T = sum(new)
+        rnd = lambda w: torch.randn(T + pad, w * HD, generator=g, device="cuda").to(dtype(act))  # noqa: E731
+        self.T = T
+        self.q, self.k, self.v = rnd(self.H) * scale, rnd(self.KH), rnd(self.KH)
+        self.out = torch.full_like(self.q, 7.0)
+        self.batch = tle.PagedChunkBatch(self.cache, self.tables, pos, new, max_ctas=max_ctas)
+
+    def positions(self):
+        return np.concatenate([np.arange(p, p + m) for p, m in zip(self.pos, self.new)] or [[]]).astype(np.int64)
+
+    def flat_rows(self, s, rows):
+        """Rows of sequence s as rows of a layer's flattened pool."""
+        t = self.tables[s].cpu().numpy().astype(np.int64)
+        return t[rows // self.page] * self.page + rows % self.page
+
+
+def angles(positions):
+    f = (np.float32(1) / np.power(BASE, np.arange(0, HD, 2) / HD).astype(np.float32)).astype(np.float32)
+    return (positions.astype(np.float32)[:, None] * f).astype(np.float64)
+
+
+def rotated(x, positions):
+    """64-bit rotation of x [tokens][heads * 64], and |a| + |b| of each element's pair."""
+    y = x.double().cpu().numpy().reshape(len(positions), -1, HD // 2, 2)
+    a = angles(positions)[:, None, :]
+    z = np.stack([y[..., 0] * np.cos(a) - y[..., 1] * np.sin(a), y[..., 0] * np.sin(a) + y[..., 1] * np.cos(a)], -1)
+    size = np.repeat(np.abs(y).sum(-1, keepdims=True), 2, -1)
+    return z.reshape(x.shape), size.reshape(x.shape)
+
+
+def attention64(c, q):
+    """The formula in 64 bits: results and tolerances [T][H * 64]."""
+    import torch
+    out = torch.zeros(c.T, c.H * HD, dtype=torch.float64, device="cuda")
+    tol = torch.zeros_like(out)
+    G = c.H // c.KH
+    t0 = 0
+    for s, (p, m) in enumerate(zip(c.pos, c.new)):
+        if m == 0:
+            continue
+        rows = torch.from_numpy(c.flat_rows(s, np.arange(p + m))).cuda()
+        for h in range(c.H):
+            sl = slice((h // G) * HD, (h // G + 1) * HD)
+            k = c.cache.key_pool[c.layer].view(-1, c.KH * HD)[rows, sl].double()
+            v = c.cache.value_pool[c.layer].view(-1, c.KH * HD)[rows, sl].double()
+            qq = q[t0:t0 + m, h * HD:(h + 1) * HD].double()
+            e = qq @ k.T / 8
+            hide = torch.arange(p + m, device="cuda")[None, :] > p + torch.arange(m, device="cuda")[:, None]
+            big = (qq.abs() @ k.abs().T / 8).masked_fill(hide, 0).amax(1, keepdim=True)
+            top = e.abs().masked_fill(hide, 0).amax(1, keepdim=True)
+            w = torch.softmax(e.masked_fill(hide, -float("inf")), 1)
+            o = w @ torch.where(hide.all(0)[:, None], torch.zeros_like(v), v)
+            size = w @ v.abs()
+            rel = 2 * (big * 2.0 ** -17 + top * 2.0 ** -23 + 2.0 ** -22) + ((p + m) / 16 + 16) * 2.0 ** -23
+            if c.act == "bf16":
+                rel = rel + 2.0 ** -8 + 2.0 ** -12
+            out[t0:t0 + m, h * HD:(h + 1) * HD] = o
+            tol[t0:t0 + m, h * HD:(h + 1) * HD] = rel * size + U[c.act] * (o.abs() + rel * size)
+        t0 += m
+    return out, tol
+
+
+def check_attend(c, q=None, out=None):
+    import torch
+    import tle
+    q = c.q if q is None else q
+    out = c.out if out is None else out
+    c.batch.attend(q, out, c.layer)
+    torch.cuda.synchronize()
+    want, tol = attention64(c, q)
+    d = (out[:c.T].double() - want).abs()
+    assert bool((d <= tol).all()), float((d / tol).max())
+    assert tle.device_error() == 0
+
+
+CASES = [
+    dict(pos=[0], new=[1]),                                             # one token, one row
+    dict(pos=[0], new=[129]),
+    dict(pos=[126, 127, 128, 129], new=[1, 1, 1, 1]),                   # around a tile's edge
+    dict(pos=[63, 64, 0, 500], new=[1, 2, 3, 0]),                       # a sequence without tokens
+    dict(pos=[0, 0, 7], new=[0, 0, 5]),
+    dict(pos=[300], new=[16]), dict(pos=[300], new=[17]),               # around the row tiles (8 heads a token)
+    dict(pos=[300], new=[32]), dict(pos=[300], new=[33]),
+    dict(pos=[1000, 3, 250], new=[40, 257, 1], page=128),
+    dict(pos=[2000, 1029, 1500, 2040], new=[1, 1, 1, 1], page=1024),
+    dict(pos=[5000], new=[3]),                                          # one sequence over many CTAs
+    dict(pos=[70, 131], new=[45, 130], heads=(8, 8)),                   # one query head per KV head
+    dict(pos=[70, 131], new=[45, 130], heads=(12, 4)),                  # groups of 3, of 5, of 7
+    dict(pos=[70, 131], new=[45, 130], heads=(20, 4), page=256),
+    dict(pos=[70, 0], new=[1, 300], heads=(7, 1)),
+    dict(pos=[64], new=[3], heads=(128, 1)),                            # a token fills a row tile
+    dict(pos=list(range(0, 1600, 25)), new=[1 + i % 5 for i in range(64)]),
+    dict(pos=[900, 10, 400], new=[100, 200, 300], max_ctas=3),          # several items per CTA
+    dict(pos=[900, 10, 400], new=[100, 200, 300], max_ctas=1),
+]
+
+
+@pytest.mark.parametrize("act", ["f32", "bf16"])
+@pytest.mark.parametrize("i", range(len(CASES)))
+def test_attend_matches_the_formula(cuda, i, act):
+    check_attend(Case(**CASES[i], act=act, seed=i))
+
+
+@pytest.mark.parametrize("act", ["f32", "bf16"])
+def test_attend_large_scores(cuda, act):
+    """Weights concentrated on a few rows (scores up to about +-100)."""
+    check_attend(Case([700, 130], [20, 1], act=act, scale=25.0, seed=3))
+
+
+@pytest.mark.parametrize("act", ["f32", "bf16"])
+def test_attend_falling_and_rising_scores(cuda, act):
+    """Scores that grow along the rows (every tile moves the running maximum)
+    and that fall (none after the first does)."""
+    import torch
+    for sign in (1.0, -1.0):
+        c = Case([900], [2], act=act, seed=4)
+        ramp = torch.linspace(-1, 1, 902, device="cuda") * sign
+        rows = torch.from_numpy(c.flat_rows(0, np.arange(902))).cuda()
+        kp = c.cache.key_pool[c.layer].view(-1, 256)
+        c.q.abs_().mul_(3)
+        kp[rows] = (ramp[:, None] * 6).expand(-1, 256).to(kp.dtype)
+        check_attend(c)
+
+
+@pytest.mark.parametrize("act", ["f32", "bf16"])
+@pytest.mark.parametrize("pos,new", [([200], [3]), ([0, 60], [70, 1]), ([120], [150])])
+@pytest.mark.parametrize("bad", ["nan", "inf", "-inf"])
+def test_rows_nobody_attends_to_do_not_matter(cuda, act, pos, new, bad):
+    """NaN and infinities behind a sequence's last row, in other pages, other
+    layers: the results are those of finite rows, bit for bit."""
+    import torch
+    c = Case(pos, new, act=act, seed=5)
+    c.batch.attend(c.q, c.out, c.layer)
+    first = c.out.clone()
+    for pool in (c.cache.key_pool, c.cache.value_pool):
+        keep = torch.zeros(pool.shape[1] * pool.shape[2], dtype=torch.bool, device="cuda")
+        for s, (p, m) in enumerate(zip(pos, new)):
+            keep[torch.from_numpy(c.flat_rows(s, np.arange(p + m))).cuda()] = True
+        pool[c.layer].view(-1, 256)[~keep] = float(bad)
+        pool[:c.layer] = float(bad)
+    check_attend(c)
+    assert torch.equal(first, c.out)
+
+
+@pytest.mark.parametrize("act", ["f32", "bf16"])
+@pytest.mark.parametrize("pos,new,at", [([200], [3], 201), ([0], [70], 40), ([100], [300], 260), ([5], [1], 2),
+                                        ([1000], [40], 1039), ([1000], [1], 1000), ([130], [33], 3)])
+@pytest.mark.parametrize("bad", ["nan", "inf"])
+@pytest.mark.parametrize("where", ["k", "v"])
+def test_a_bad_row_reaches_only_the_tokens_that_attend_to_it(cuda, act, pos, new, at, bad, where):
+    import torch
+    import tle
+    c = Case(pos, new, act=act, seed=6)
+    c.batch.attend(c.q, c.out, c.layer)
+    first = c.out.clone()
+    want, tol = attention64(c, c.q)
+    row = int(c.flat_rows(0, np.array([at]))[0])
+    pool = c.cache.key_pool if where == "k" else c.cache.value_pool
+    pool[c.layer].view(-1, 256)[row, 64:128] = float(bad)      # KV head 1: query heads 8 .. 15
+    c.batch.attend(c.q, c.out, c.layer)
+    torch.cuda.synchronize()
+    sees = torch.arange(new[0], device="cuda") + pos[0] >= at
+    mine = slice(8 * HD, 16 * HD)
+    assert bool(((c.out.double() - want).abs() <= tol)[~sees].all())
+    assert torch.equal(c.out[:, :8 * HD], first[:, :8 * HD]) and torch.equal(c.out[:, 16 * HD:], first[:, 16 * HD:])
+    hit = c.out[sees, mine]
+    if where == "v":
+        assert bool((~torch.isfinite(hit)).all())
+    elif bad == "nan":
+        assert bool(torch.isnan(hit).all())
+    else:                       # a score of +-inf (or NaN): the row alone, or no weight at all
+        now, _ = attention64(c, c.q)
+        fine = torch.isfinite(now[sees, mine])
+        assert bool(torch.isnan(hit[~fine]).all()) or bool((~torch.isfinite(hit[~fine])).all())
+    assert tle.device_error() == 0
+
+
+def test_attend_leaves_rows_behind_the_last_token(cuda):
+    import torch
+    c = Case([100, 20], [3, 4], pad=5)
+    check_attend(c)
+    assert bool((c.out[7:] == 7.0).all())
+
+
+@pytest.mark.parametrize("act", ["f32", "bf16"])
+def test_attend_row_strides(cuda, act):
+    """q inside a fused q/k/v buffer, out inside a wider one."""
+    import torch
+    c = Case([90, 300], [33, 2], act=act, seed=8)
+    qkv = torch.randn(c.T, 40 * HD, device="cuda").to(c.q.dtype)
+    wide = torch.full((c.T, 32 * HD + 24), 7.0, device="cuda", dtype=c.q.dtype)
+    check_attend(c, q=qkv[:, :32 * HD], out=wide[:, 16:16 + 32 * HD])
+    assert bool((wide[:, :16] == 7).all()) and bool((wide[:, 16 + 32 * HD:] == 7).all())
+
+
+@pytest.mark.parametrize("act", ["f32", "bf16"])
+def test_attend_is_reproducible_and_replays(cuda, act):
+    """Same bits in a second call, on another stream, and from a captured
+    graph after the inputs changed in place."""
+    import torch
+    c = Case([700, 50, 1300], [40, 9, 1], act=act, seed=9)
+    c.batch.attend(c.q, c.out, c.layer)
+    first = c.out.clone()
+    c.out.fill_(0)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    c.batch.attend(c.q, c.out, c.layer, stream=side)
+    torch.cuda.current_stream().wait_stream(side)
+    assert torch.equal(first, c.out)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        c.batch.run(c.q, c.k, c.v, c.out, c.layer)
+    for seed in (1, 2):
+        g = torch.Generator(device="cuda").manual_seed(seed)
+        for t in (c.q, c.k, c.v):
+            t.copy_(torch.randn(t.shape, generator=g, device="cuda"))
+        graph.replay()
+        torch.cuda.synchronize()
+        got = c.out.clone()
+        c.batch.run(c.q, c.k, c.v, c.out, c.layer)
+        torch.cuda.synchronize()
+        assert torch.equal(got, c.out)
+
+
+def test_set_positions_replans(cuda):
+    """The same batch object over growing contexts and other chunk lengths."""
+    c = Case([900, 60, 3000], [300, 200, 400], seed=10)
+    for pos, new in (([0, 0, 0], [5, 1, 0]), ([5, 1, 0], [1, 1, 1]), ([6, 2, 1], [200, 0, 300]), ([900, 60, 3000], [300, 200, 400])):
+        c.pos, c.new, c.T = pos, new, sum(new)
+        c.batch.set_positions(pos, new)
+        check_attend(c)
+
+
+def test_two_batches_in_flight(cuda):
+    """Two batches (own workspaces) over one cache on two streams at once."""
+    import torch
+    import tle
+    a = Case([2500, 100], [30, 1], seed=11)
+    other = tle.PagedChunkBatch(a.cache, a.tables, a.pos, a.new)
+    a.batch.attend(a.q, a.out, a.layer)
+    torch.cuda.synchronize()
+    want = a.out.clone()
+    outs = [torch.zeros_like(a.out) for _ in range(2)]
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    torch.cuda.synchronize()
+    for _ in range(5):
+        for b, s, o in zip((a.batch, other), streams, outs):
+            b.attend(a.q, o, a.layer, stream=s)
+    torch.cuda.synchronize()
+    assert torch.equal(outs[0], want) and torch.equal(outs[1], want)
+
+
+@pytest.mark.parametrize("act", ["f32", "bf16"])
+def test_bad_page_ids_are_reported_not_read(cuda, act):
+    """An id outside the pool: its rows count as zeros and 0x105 is recorded;
+    append stores nothing there."""
+    import torch
+    import tle
+    c = Case([130], [6], act=act, seed=12)
+    good = c.tables[0].clone()
+    for bad in (c.cache.n_pages, -1, 1 << 30):
+        c.tables[0].copy_(good)
+        c.tables[0][1] = bad
+        c.batch.attend(c.q, c.out, c.layer)
+        torch.cuda.synchronize()
+        assert tle.device_error() == 0x105
+        c.tables[0].copy_(good)
+        kp, vp = c.cache.key_pool.clone(), c.cache.value_pool.clone()
+        page = int(good[1])
+        c.cache.key_pool[c.layer, page] = 0
+        c.cache.value_pool[c.layer, page] = 0
+        got = c.out.clone()
+        check_attend(c)
+        assert torch.equal(got, c.out)
+        c.cache.key_pool.copy_(kp)
+        c.cache.value_pool.copy_(vp)
+    c.tables[0][2] = c.cache.n_pages          # rows 128 .. 191 hold the six new ones
+    before = (c.cache.key_pool.clone(), c.cache.value_pool.clone())
+    c.batch.append(None, c.k, c.v, c.layer)
+    torch.cuda.synchronize()
+    assert tle.device_error() == 0x105
+    assert torch.equal(before[0], c.cache.key_pool) and torch.equal(before[1], c.cache.value_pool)
+
+
+def test_offsets_past_32_bits(cuda):
+    """Pages whose rows lie more than 2^32 bytes and 2^31 elements into the pools."""
+    import torch
+    import tle
+    page, n_pages = 65536, 140                                   # 9.2 M rows, 4.7 GB a pool
+    shape = tle.Shape(1, 32, 4, HD, BASE)
+    dims = (1, n_pages, page, 256)
+    kp, vp = (torch.empty(dims, dtype=torch.bfloat16, device="cuda") for _ in range(2))
+    cache = tle.PagedKVCache(n_pages, page, shape, dtype=torch.bfloat16, pools=(kp, vp))
+    c = Case([10], [3], seed=13, layers=1)
+    c.cache, c.page = cache, page
+    c.pos, c.new, c.T = [300, 70], [5, 1], 6
+    c.tables = [torch.tensor([139], dtype=torch.int32, device="cuda"), torch.tensor([131], dtype=torch.int32, device="cuda")]
+    g = torch.Generator(device="cuda").manual_seed(13)
+    for t in c.tables:
+        for pool in (kp, vp):
+            pool[0, int(t[0]), :400] = torch.randn(400, 256, generator=g, device="cuda").to(torch.bfloat16)
+    c.q = torch.randn(6, 2048, generator=g, device="cuda")
+    c.k, c.v = (torch.randn(6, 256, generator=g, device="cuda") for _ in range(2))
+    c.out = torch.zeros_like(c.q)
+    c.batch = tle.PagedChunkBatch(cache, c.tables, c.pos, c.new)
+    c.batch.append(None, c.k, c.v, 0)
+    want, size = rotated(c.k, c.positions())
+    rows = np.concatenate([c.flat_rows(s, np.arange(p, p + m)) for s, (p, m) in enumerate(zip(c.pos, c.new))])
+    got = kp[0].view(-1, 256)[torch.from_numpy(rows).cuda()].double().cpu().numpy()
+    assert np.all(np.abs(got - want) <= np.abs(want) * 2.0 ** -8 + size * 2.0 ** -21)
+    check_attend(c)
+
+
+# ------------------------------------------------------------------- append
+@pytest.mark.parametrize("act,pool", [("f32", "f32"), ("f32", "bf16"), ("bf16", "f32"), ("bf16", "bf16")])
+@pytest.mark.parametrize("kw", [
+    dict(pos=[0], new=[1]), dict(pos=[63, 0, 200], new=[2, 0, 65]), dict(pos=[3000, 17], new=[33, 1], page=256),
+    dict(pos=[40], new=[9], heads=(7, 1)), dict(pos=[70, 131], new=[45, 130], heads=(20, 4)),
+    dict(pos=[5], new=[3], heads=(8, 8)), dict(pos=[100000], new=[2], page=1024)])
+def test_append_matches_the_formula(cuda, act, pool, kw):
+    import torch
+    import tle
+    c = Case(**kw, act=act, pool=pool, seed=20, pad=2)
+    p = c.positions()
+    before = (c.cache.key_pool.clone(), c.cache.value_pool.clone())
+    q0, k0 = c.q.clone(), c.k.clone()
+    c.batch.append(c.q, c.k, c.v, c.layer, q_out=c.out)
+    torch.cuda.synchronize()
+    assert torch.equal(q0, c.q) and torch.equal(k0, c.k)
+    want, size = rotated(c.q[:c.T], p)
+    got = c.out[:c.T].double().cpu().numpy()
+    assert np.all(np.abs(got - want) <= np.abs(want) * U[act] + size * 2.0 ** -21)
+    assert bool((c.out[c.T:] == 7.0).all())
+    rows = np.concatenate([c.flat_rows(s, np.arange(a, a + m)) for s, (a, m) in enumerate(zip(c.pos, c.new))])
+    at = torch.from_numpy(rows).cuda()
+    want, size = rotated(c.k[:c.T], p)
+    got = c.cache.key_pool[c.layer].view(-1, c.KH * HD)[at].double().cpu().numpy()
+    assert np.all(np.abs(got - want) <= np.abs(want) * U[pool] + size * 2.0 ** -21)
+    got = c.cache.value_pool[c.layer].view(-1, c.KH * HD)[at]
+    assert torch.equal(got, c.v[:c.T].to(got.dtype))
+    for new, old in zip((c.cache.key_pool, c.cache.value_pool), before):   # nothing else is written
+        old[c.layer].view(-1, c.KH * HD)[at] = new[c.layer].view(-1, c.KH * HD)[at]
+        assert torch.equal(new, old)
+    assert tle.device_error() == 0
+
+
+def test_append_in_place_strided_and_unrotated(cuda):
+    import torch
+    c = Case([90, 300], [33, 2], seed=21)
+    qkv = torch.randn(c.T, 40 * HD, device="cuda")
+    q, k, v = qkv[:, :32 * HD], qkv[:, 32 * HD:36 * HD], qkv[:, 36 * HD:]
+    c.batch.append(q, k, v, c.layer, q_out=c.out)
+    a = (c.out.clone(), c.cache.key_pool.clone(), c.cache.value_pool.clone())
+    qq = q.contiguous()
+    c.batch.append(qq, k.contiguous(), v.contiguous(), c.layer, q_out=qq)      # q in place
+    torch.cuda.synchronize()
+    assert torch.equal(qq, a[0]) and torch.equal(c.cache.key_pool, a[1]) and torch.equal(c.cache.value_pool, a[2])
+    c.batch.append(q, k, v, c.layer, rotate=False, q_out=c.out)
+    torch.cuda.synchronize()
+    assert torch.equal(c.out, q)
+    rows = np.concatenate([c.flat_rows(s, np.arange(p, p + m)) for s, (p, m) in enumerate(zip(c.pos, c.new))])
+    assert torch.equal(c.cache.key_pool[c.layer].view(-1, 256)[torch.from_numpy(rows).cuda()], k.to(torch.bfloat16))
+
+
+# ---------------------------------------------------------- used together
+def test_pieces_of_a_prompt_equal_the_whole_and_decode_goes_on(cuda):
+    """A prompt appended and attended in pieces gives the rows and results of
+    the whole prompt at once; the framework's paged decode of the next token
+    agrees with a chunk of one (bf16 precision, its contract)."""
+    import torch
+    import tle
+    n = 333
+    whole = Case([0], [n], page=64, seed=30)
+    whole.batch.run(whole.q, whole.k, whole.v, whole.out, 1)
+    parts = Case([0], [n], page=64, seed=30)
+    at = 0
+    for m in (1, 63, 64, 100, 1, 104):
+        b = tle.PagedChunkBatch(parts.cache, parts.tables, [at], [m])
+        s = slice(at, at + m)
+        b.run(parts.q[s], parts.k[s], parts.v[s], parts.out[s], 1)
+        at += m
+    torch.cuda.synchronize()
+    assert torch.equal(whole.cache.key_pool, parts.cache.key_pool)
+    assert torch.equal(whole.cache.value_pool, parts.cache.value_pool)
+    turned = torch.empty_like(whole.q)
+    whole.batch.append(whole.q, whole.k, whole.v, 1, q_out=turned)
+    want, tol = attention64(whole, turned)
+    for c in (whole, parts):
+        assert bool(((c.out.double() - want).abs() <= tol).all())
+    # the next token: framework decode, then the chunk of one on the same cache
+    pos = n - 1                                  # decode the last token again
+    dec = tle.PagedDecodeBatchBf16(whole.cache, [whole.tables[0]], [pos])
+    one = tle.PagedChunkBatch(whole.cache, [whole.tables[0]], [pos], [1])
+    q, k, v = whole.q[pos:], whole.k[pos:], whole.v[pos:]
+    a, b = torch.zeros(1, 2048, device="cuda"), torch.zeros(1, 2048, device="cuda")
+    dec.run(q, k, v, a, 1)
+    rows = whole.cache.key_pool.clone()
+    one.run(q, k, v, b, 1)
+    torch.cuda.synchronize()
+    assert float((a - b).abs().max()) <= 2e-2
+    near = (rows.float() - whole.cache.key_pool.float()).abs() <= rows.float().abs() * 2.0 ** -7 + 1e-30
+    assert bool(near.all())
+    assert tle.device_error() == 0
+
+
+def test_prompt_into_an_fp32_cache_then_the_framework_decode(cuda):
+    """append into fp32 pools holds what the paged fp32 decode expects: its
+    result over those rows is the formula's (decode contract, 1e-4)."""
+    import torch
+    import tle
+    c = Case([0, 0], [130, 40], page=16, pool="f32", seed=31)
+    c.batch.append(c.q, c.k, c.v, c.layer, q_out=c.out)
+    dec = tle.PagedDecodeBatch(c.cache, c.tables, [129, 39])
+    last = torch.tensor([129, 169], device="cuda")
+    out = torch.zeros(2, 2048, device="cuda")
+    dec.run(c.q[last], c.k[last], c.v[last], out, c.layer)
+    torch.cuda.synchronize()
+    want, _ = attention64(c, c.out)
+    assert float((out.double() - want[last]).abs().max()) <= 1e-4
+
+
+def test_a_serving_step_with_sampling(cuda):
+    """Prompt pieces, one decode step, logits under rules, a token: each
+    stage through its public call, the token the 64-bit formula's."""
+    import torch
+    import tle
+    V = 1000
+    c = Case([0, 64, 500], [70, 1, 3], act="bf16", seed=32)
+    c.batch.run(c.q, c.k, c.v, c.out, c.layer)
+    last = torch.tensor([69, 70, 73], device="cuda")
+    W = torch.randn(2048, V, device="cuda", generator=torch.Generator(device="cuda").manual_seed(1)) / 45
+    logits = c.out[last].float() @ W
+    hist = torch.tensor([5, 5, 9, 11, 5], dtype=torch.int32, device="cuda")
+    start = torch.tensor([0, 3, 3, 5], dtype=torch.int32, device="cuda")
+    allowed = torch.full((3, -(-V // 32)), -1, dtype=torch.int32, device="cuda")
+    top = int(logits[1].argmax())
+    allowed[1, top // 32] &= ~(1 << (top % 32)) if top % 32 < 31 else 0x7FFFFFFF
+    f = lambda *x: torch.tensor(x, dtype=torch.float32, device="cuda")  # noqa: E731
+    rules = tle.LogitRules(3, V, tokens=hist, token_start=start, repetition=f(1.5, 2, 1.1), frequency=f(.5, .1, .2),
+                           presence=f(.2, .3, .1), allowed=allowed)
+    adj = torch.empty_like(logits)
+    tle.logits_adjust(adj, logits, rules)
+    tok = torch.zeros(3, dtype=torch.int32, device="cuda")
+    for r in range(3):
+        tle.sample_argmax(adj[r], tok[r:r + 1])
+    torch.cuda.synchronize()
+    assert torch.equal(tok.long(), adj.argmax(1)) and int(tok[1]) != top
+    assert tle.device_error() == 0

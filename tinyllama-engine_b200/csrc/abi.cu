@@ -1396,3 +1396,451 @@ int tle_prompt_forward(const tle_model_t* m, const void* packed, const tle_state
 }
 
 }  // extern "C"
+
+// ===================== chunks over a paged cache (tle_attn.h) =====================
+
+namespace {
+
+int check_chunk_shape(const tle_shape_t* s) {
+    if (!s) return set_error(TLE_ERR_INVALID, "shape is NULL");
+    if (s->n_layers <= 0 || s->n_head <= 0 || s->n_head_kv <= 0)
+        return set_error(TLE_ERR_INVALID, "bad shape: n_layers %d, n_head %d, n_head_kv %d", s->n_layers, s->n_head,
+                         s->n_head_kv);
+    if (s->head_dim != tle::kHeadDim || s->n_head % s->n_head_kv != 0 || s->n_head / s->n_head_kv > tle::kChunkRows ||
+        s->n_head > 65535)
+        return set_error(TLE_ERR_UNSUPPORTED,
+                         "chunk kernels need head_dim 64 and n_head a multiple (at most %d) of n_head_kv (got %d, %d, %d)",
+                         tle::kChunkRows, s->head_dim, s->n_head, s->n_head_kv);
+    if (!(s->rope_freq_base > 0.f)) return set_error(TLE_ERR_INVALID, "rope_freq_base must be > 0");
+    return 0;
+}
+
+int check_chunks(const tle_shape_t* shape, int page_rows, const tle_paged_chunk_t* chunks, int n_seqs) {
+    if (int rc = check_chunk_shape(shape)) return rc;
+    if (n_seqs <= 0 || !chunks) return set_error(TLE_ERR_INVALID, "need n_seqs > 0 and non-null chunks");
+    const int64_t g = shape->n_head / shape->n_head_kv;
+    int64_t tokens = 0;
+    for (int s = 0; s < n_seqs; ++s) {
+        const tle_paged_chunk_t& c = chunks[s];
+        if (c.pos < 0 || c.n_tokens < 0 || c.n_pages < 0)
+            return set_error(TLE_ERR_INVALID, "sequence %d: pos %d, n_tokens %d, n_pages %d must be >= 0", s, c.pos,
+                             c.n_tokens, c.n_pages);
+        if (c.n_tokens == 0) continue;
+        if (!c.pages || (reinterpret_cast<uintptr_t>(c.pages) & 3u) != 0)
+            return set_error(TLE_ERR_INVALID, "sequence %d: page table must be non-null and 4-byte aligned", s);
+        const int64_t end = static_cast<int64_t>(c.pos) + c.n_tokens;
+        if (page_rows > 0 && static_cast<int64_t>(c.n_pages) * page_rows < end)
+            return set_error(TLE_ERR_INVALID,
+                             "sequence %d: need pos + n_tokens <= n_pages * page_rows (pos=%d, n_tokens=%d, n_pages=%d)", s,
+                             c.pos, c.n_tokens, c.n_pages);
+        if (end > INT32_MAX - tle::kChunkTile || c.n_tokens * g > INT32_MAX - tle::kChunkItemRows)
+            return set_error(TLE_ERR_UNSUPPORTED, "sequence %d: pos %d + n_tokens %d too long", s, c.pos, c.n_tokens);
+        tokens += c.n_tokens;
+    }
+    if (tokens > INT32_MAX / 2) return set_error(TLE_ERR_UNSUPPORTED, "%lld tokens in all", static_cast<long long>(tokens));
+    return 0;
+}
+
+// The attention's work plan.  Costs are in half steps: a step of the kernel
+// takes one K/V tile for both row tiles of an item of more than kChunkRows
+// rows ("dual"), or two tiles for a smaller item, so a tile costs 2 or 1;
+// kSegUnits is the fixed cost of a segment (Q load, epilogue).
+constexpr int64_t kSegUnits = 4;
+constexpr int64_t kMinPieceUnits = 4;   // smallest piece of an item worth a CTA of its own
+
+struct ChunkPlanner {
+    const tle_shape_t* shape;
+    const tle_paged_chunk_t* chunks;
+    int n_seqs;
+    int max_ctas;
+    int64_t n_items = 0, units = 0;
+
+    struct Item {
+        int seq, kvh, row0, n_rows, tiles;
+        int unit() const { return n_rows > tle::kChunkRows ? 2 : 1; }   // cost of a tile
+        int step() const { return n_rows > tle::kChunkRows ? 1 : 2; }   // tiles of a step
+        int64_t cost() const { return static_cast<int64_t>(tiles) * unit(); }
+        int parts(int t) const { return n_rows > tle::kChunkRows ? 1 : std::min(2, t); }
+    };
+
+    template <class F>
+    void each_item(F&& f) const {
+        const int g = shape->n_head / shape->n_head_kv;
+        for (int s = 0; s < n_seqs; ++s)
+            for (int h = 0; h < shape->n_head_kv; ++h) {
+                const int rows = chunks[s].n_tokens * g;
+                for (int r = 0; r < rows; r += tle::kChunkItemRows) {
+                    Item it{s, h, r, std::min(tle::kChunkItemRows, rows - r), 0};
+                    it.tiles = (chunks[s].pos + (r + it.n_rows - 1) / g) / tle::kChunkTile + 1;
+                    f(it);
+                }
+            }
+    }
+
+    // Calls seg(cta, item, t0, t1, parts of the item, parts before) and
+    // merge(item, parts) in order; returns the CTA count.
+    template <class S, class M>
+    int run(S&& seg, M&& merge) {
+        n_items = units = 0;
+        each_item([&](const Item& it) {
+            ++n_items;
+            units += it.cost();
+        });
+        const int G = max_ctas;
+        if (n_items <= G) {
+            // few items: every item in equal pieces, one piece per CTA, the
+            // smallest piece for which the CTAs suffice
+            int64_t piece = std::max(kMinPieceUnits, (units + G - 1) / G);
+            for (;;) {
+                int64_t n = 0;
+                each_item([&](const Item& it) { n += (it.cost() + piece - 1) / piece; });
+                if (n <= G) break;
+                piece += std::max<int64_t>(1, piece / 16);
+            }
+            int cta = 0;
+            each_item([&](const Item& it) {
+                const int64_t k = (it.cost() + piece - 1) / piece;
+                auto cut = [&](int64_t j) {
+                    const int64_t t = j * it.tiles / k;
+                    return j >= k ? it.tiles : static_cast<int>((t + it.step() - 1) / it.step() * it.step());
+                };
+                int parts = 0;
+                for (int64_t j = 0; j < k; ++j) parts += it.parts(std::max(0, cut(j + 1) - cut(j)));
+                int before = 0;
+                for (int64_t j = 0; j < k; ++j) {
+                    const int a = cut(j), b = cut(j + 1);
+                    if (b <= a) continue;
+                    seg(cta++, it, a, b, parts, before);
+                    before += it.parts(b - a);
+                }
+                if (parts > 1) merge(it, parts);
+            });
+            return cta;
+        }
+        // many items: the concatenated cost of all items cut into G equal
+        // ranges, each boundary on a step of the item it falls into
+        const int64_t total = units + n_items * kSegUnits;
+        int64_t X = 0;
+        int c = 0;
+        each_item([&](const Item& it) {
+            const int64_t end = X + kSegUnits + it.cost();
+            auto walk = [&](int c0, auto&& f) {   // f(cta, t0, t1); returns the CTA that goes on
+                int t = 0;
+                while (t < it.tiles) {
+                    const int64_t x = c0 >= G - 1 ? end : (c0 + 1) * total / G;
+                    int to = it.tiles;
+                    if (x < end) {
+                        const int64_t r = std::max<int64_t>(0, x - X - kSegUnits) / it.unit();
+                        to = static_cast<int>(r / it.step() * it.step());
+                        if (it.tiles - to < it.step()) to = it.tiles;
+                    }
+                    if (to > t) f(c0, t, to);
+                    t = std::max(t, to);
+                    if (x <= end && c0 < G - 1) ++c0;
+                }
+                return c0;
+            };
+            int parts = 0, before = 0;
+            walk(c, [&](int, int a, int b) { parts += it.parts(b - a); });
+            c = walk(c, [&](int cta, int a, int b) {
+                seg(cta, it, a, b, parts, before);
+                before += it.parts(b - a);
+            });
+            if (parts > 1) merge(it, parts);
+            X = end;
+        });
+        return G;
+    }
+};
+
+int chunk_ctas(int max_ctas) {
+    if (max_ctas <= 0) max_ctas = sm_count();
+    return std::min(max_ctas, tle::kMaxCtas);
+}
+
+// The checks shared by the calls on a descriptor.
+int check_chunk_call(const tle_shape_t* shape, const tle_chunk_plan_t* plan, const void* desc_dev, int act_type, int layer) {
+    if (int rc = check_chunk_shape(shape)) return rc;
+    if (!plan || !desc_dev) return set_error(TLE_ERR_INVALID, "plan and descriptor must be non-null");
+    if (!aligned16(desc_dev)) return set_error(TLE_ERR_INVALID, "the descriptor must be 16-byte aligned");
+    if (plan->n_head != shape->n_head || plan->n_head_kv != shape->n_head_kv)
+        return set_error(TLE_ERR_INVALID, "the plan was made for %d/%d heads, not %d/%d", plan->n_head, plan->n_head_kv,
+                         shape->n_head, shape->n_head_kv);
+    if (act_type != TLE_ACT_F32 && act_type != TLE_ACT_BF16)
+        return set_error(TLE_ERR_UNSUPPORTED, "activation type %d", act_type);
+    if (layer < 0 || layer >= shape->n_layers)
+        return set_error(TLE_ERR_INVALID, "layer %d outside [0, %d)", layer, shape->n_layers);
+    return 0;
+}
+
+int check_rows(const void* p, int64_t stride, int heads, const char* what) {
+    if (!p) return set_error(TLE_ERR_INVALID, "%s is NULL", what);
+    if (!aligned16(p)) return set_error(TLE_ERR_INVALID, "%s must be 16-byte aligned", what);
+    if (stride < static_cast<int64_t>(heads) * tle::kHeadDim || stride % 8 != 0)
+        return set_error(TLE_ERR_INVALID, "%s: stride %lld must be a multiple of 8 and at least %d", what,
+                         static_cast<long long>(stride), heads * tle::kHeadDim);
+    return 0;
+}
+
+// Checks a pool; fills *shift.  min_page: the smallest page of this pool type.
+int check_chunk_pool(const tle_shape_t* shape, const tle_chunk_plan_t* plan, const void* kp, const void* vp, int n_pages,
+                     int page_rows, int min_page, int* shift) {
+    if (!kp || !vp) return set_error(TLE_ERR_INVALID, "page pool and both pools must be non-null");
+    if (!aligned16(kp) || !aligned16(vp)) return set_error(TLE_ERR_INVALID, "page pools must be 16-byte aligned");
+    if (page_rows < min_page || page_rows > 65536 || (page_rows & (page_rows - 1)) != 0)
+        return set_error(TLE_ERR_INVALID, "page_rows %d is not a power of two in [%d, 65536]", page_rows, min_page);
+    if (page_rows != plan->page_rows)
+        return set_error(TLE_ERR_INVALID, "the plan was made for pages of %d rows, not %d", plan->page_rows, page_rows);
+    if (n_pages <= 0) return set_error(TLE_ERR_INVALID, "pool n_pages %d <= 0", n_pages);
+    const double rows = static_cast<double>(n_pages) * page_rows;
+    if (rows >= 2147483648.0 || rows * shape->n_layers * shape->n_head_kv * tle::kHeadDim > 4.0e18)
+        return set_error(TLE_ERR_INVALID, "page pool too large");
+    int sh = 0;
+    while ((1 << sh) < page_rows) ++sh;
+    *shift = sh;
+    return 0;
+}
+
+int append_common(const tle_shape_t* shape, const tle_chunk_plan_t* plan, const void* desc_dev, const void* q,
+                  int64_t q_stride, const void* k, int64_t k_stride, const void* v, int64_t v_stride, void* q_out,
+                  int act_type, int layer, int flags, void* key_pool, void* value_pool, int n_pages, int page_rows,
+                  bool pool_bf16, void* stream) {
+    if (int rc = check_chunk_call(shape, plan, desc_dev, act_type, layer)) return rc;
+    int shift = 0;
+    if (int rc = check_chunk_pool(shape, plan, key_pool, value_pool, n_pages, page_rows, pool_bf16 ? 64 : 16, &shift))
+        return rc;
+    if (flags & ~TLE_DECODE_ROTATE) return set_error(TLE_ERR_INVALID, "unknown flags 0x%x", flags);
+    if (plan->n_tokens == 0) return ok();
+    if ((q == nullptr) != (q_out == nullptr)) return set_error(TLE_ERR_INVALID, "q and q_out go together");
+    if (q) {
+        if (int rc = check_rows(q, q_stride, shape->n_head, "q")) return rc;
+        if (!aligned16(q_out)) return set_error(TLE_ERR_INVALID, "q_out must be 16-byte aligned");
+        if (q == q_out && q_stride != static_cast<int64_t>(shape->n_head) * tle::kHeadDim)
+            return set_error(TLE_ERR_INVALID, "q_out is packed: it can be q only where q is");
+    }
+    if (int rc = check_rows(k, k_stride, shape->n_head_kv, "k")) return rc;
+    if (int rc = check_rows(v, v_stride, shape->n_head_kv, "v")) return rc;
+    tle::AppendArgs a{};
+    a.d = tle::chunk_desc(desc_dev, plan->n_seqs, plan->n_segs, plan->n_merge, plan->n_tokens);
+    a.n_tokens = plan->n_tokens;
+    a.q = q;
+    a.k = k;
+    a.v = v;
+    a.q_out = q_out;
+    a.q_stride = q_stride;
+    a.k_stride = k_stride;
+    a.v_stride = v_stride;
+    const size_t layer_bytes = static_cast<size_t>(n_pages) * page_rows * shape->n_head_kv * tle::kHeadDim * (pool_bf16 ? 2 : 4);
+    a.key_pool = static_cast<unsigned char*>(key_pool) + layer_bytes * layer;
+    a.value_pool = static_cast<unsigned char*>(value_pool) + layer_bytes * layer;
+    a.pool_pages = n_pages;
+    a.page_shift = shift;
+    a.n_head = q ? shape->n_head : 0;
+    a.n_head_kv = shape->n_head_kv;
+    a.rotate = (flags & TLE_DECODE_ROTATE) ? 1 : 0;
+    fill_inv_freq(a.inv_freq, tle::kHeadDim / 2, shape->rope_freq_base);
+    cudaError_t e = tle::error_word(&a.err);
+    if (e != cudaSuccess) return cuda_error(e, "device error word");
+    e = tle::launch_append(a, act_type == TLE_ACT_BF16, pool_bf16, static_cast<cudaStream_t>(stream));
+    if (e != cudaSuccess) return cuda_error(e, "append launch");
+    return ok();
+}
+
+}  // namespace
+
+extern "C" {
+
+size_t tle_chunk_desc_bytes(const tle_shape_t* shape, const tle_paged_chunk_t* chunks, int n_seqs, int max_ctas) {
+    if (check_chunks(shape, 0, chunks, n_seqs)) return 0;
+    ChunkPlanner p{shape, chunks, n_seqs, chunk_ctas(max_ctas)};
+    size_t segs = 0, merges = 0, tokens = 0;
+    const int G = p.run([&](int, const ChunkPlanner::Item&, int, int, int, int) { ++segs; },
+                        [&](const ChunkPlanner::Item&, int) { ++merges; });
+    for (int s = 0; s < n_seqs; ++s) tokens += static_cast<size_t>(chunks[s].n_tokens);
+    return tle::chunk_desc_bytes(n_seqs, segs, merges, tokens, G);
+}
+
+int tle_chunk_desc_paged(const tle_shape_t* shape, int page_rows, const tle_paged_chunk_t* chunks, int n_seqs,
+                         int max_ctas, void* desc_host, size_t desc_bytes, tle_chunk_plan_t* plan) {
+    if (!desc_host || !plan) return set_error(TLE_ERR_INVALID, "desc_host and plan must be non-null");
+    if (page_rows < 16 || page_rows > 65536 || (page_rows & (page_rows - 1)) != 0)
+        return set_error(TLE_ERR_INVALID, "page_rows %d is not a power of two in [16, 65536]", page_rows);
+    if (int rc = check_chunks(shape, page_rows, chunks, n_seqs)) return rc;
+    ChunkPlanner p{shape, chunks, n_seqs, chunk_ctas(max_ctas)};
+    tle_chunk_plan_t out{};
+    int64_t segs = 0, merges = 0, part_rows = 0;
+    int merge_rows = 0;
+    const int G = p.run([&](int, const ChunkPlanner::Item&, int, int, int, int) { ++segs; },
+                        [&](const ChunkPlanner::Item& it, int parts) {
+                            ++merges;
+                            part_rows += static_cast<int64_t>(parts) * it.n_rows;
+                            merge_rows = std::max(merge_rows, it.n_rows);
+                        });
+    int64_t tokens = 0;
+    for (int s = 0; s < n_seqs; ++s) tokens += chunks[s].n_tokens;
+    if (segs > INT32_MAX / 2 || part_rows > INT32_MAX / 2)
+        return set_error(TLE_ERR_UNSUPPORTED, "batch too large (%lld pieces)", static_cast<long long>(segs));
+    out.n_seqs = n_seqs;
+    out.n_tokens = static_cast<int32_t>(tokens);
+    out.n_head = shape->n_head;
+    out.n_head_kv = shape->n_head_kv;
+    out.page_rows = page_rows;
+    out.n_ctas = G;
+    out.n_segs = static_cast<int32_t>(segs);
+    out.n_merge = static_cast<int32_t>(merges);
+    out.merge_rows = merge_rows;
+    out.part_rows = part_rows;
+    const size_t need = tle::chunk_desc_bytes(n_seqs, segs, merges, tokens, G);
+    if (desc_bytes < need)
+        return set_error(TLE_ERR_INVALID, "descriptor buffer %zu bytes < %zu needed", desc_bytes, need);
+    if ((reinterpret_cast<uintptr_t>(desc_host) & 7u) != 0)
+        return set_error(TLE_ERR_INVALID, "desc_host must be 8-byte aligned");
+    auto* hdr = static_cast<tle::ChunkHeader*>(desc_host);
+    *hdr = tle::ChunkHeader{tle::kChunkMagic, n_seqs, out.n_tokens, G, out.n_segs, out.n_merge, {0, 0}};
+    const tle::ChunkDesc d = tle::chunk_desc(desc_host, n_seqs, segs, merges, tokens);
+    auto* seq = const_cast<tle::ChunkSeq*>(d.seqs);
+    auto* seg = const_cast<tle::ChunkSeg*>(d.segs);
+    auto* mrg = const_cast<tle::ChunkMerge*>(d.merges);
+    auto* tok = const_cast<tle::ChunkTok*>(d.toks);
+    auto* start = const_cast<int32_t*>(d.cta_start);
+    int32_t first = 0;
+    for (int s = 0; s < n_seqs; ++s) {
+        const tle_paged_chunk_t& c = chunks[s];
+        seq[s] = tle::ChunkSeq{c.pages, c.n_pages, c.pos, c.n_tokens, first};
+        for (int t = 0; t < c.n_tokens; ++t) tok[first + t] = tle::ChunkTok{s, c.pos + t};
+        first += c.n_tokens;
+    }
+    int32_t part = 0, at = 0;
+    int cta_seen = 0;   // CTAs whose start is written
+    p.run(
+        [&](int cta, const ChunkPlanner::Item& it, int t0, int t1, int parts, int before) {
+            while (cta_seen <= cta) start[cta_seen++] = at;
+            seg[at++] = tle::ChunkSeg{it.seq, it.kvh, it.row0, it.n_rows, t0, t1,
+                                      parts > 1 ? part + before * it.n_rows : -1, 0};
+        },
+        [&](const ChunkPlanner::Item& it, int parts) {
+            *mrg++ = tle::ChunkMerge{it.seq, it.kvh, it.row0, it.n_rows, part, parts};
+            part += parts * it.n_rows;
+        });
+    while (cta_seen <= G) start[cta_seen++] = at;
+    *plan = out;
+    return ok();
+}
+
+int tle_append_paged(const tle_shape_t* shape, const tle_page_pool_t* pool, const tle_chunk_plan_t* plan,
+                     const void* desc_dev, const void* q, int64_t q_stride, const void* k, int64_t k_stride,
+                     const void* v, int64_t v_stride, void* q_out, int act_type, int layer, int flags, void* stream) {
+    if (!pool) return set_error(TLE_ERR_INVALID, "page pool and both pools must be non-null");
+    return append_common(shape, plan, desc_dev, q, q_stride, k, k_stride, v, v_stride, q_out, act_type, layer, flags,
+                         pool->key_pool, pool->value_pool, pool->n_pages, pool->page_rows, false, stream);
+}
+
+int tle_append_bf16_paged(const tle_shape_t* shape, const tle_page_pool_bf16_t* pool, const tle_chunk_plan_t* plan,
+                          const void* desc_dev, const void* q, int64_t q_stride, const void* k, int64_t k_stride,
+                          const void* v, int64_t v_stride, void* q_out, int act_type, int layer, int flags,
+                          void* stream) {
+    if (!pool) return set_error(TLE_ERR_INVALID, "page pool and both pools must be non-null");
+    return append_common(shape, plan, desc_dev, q, q_stride, k, k_stride, v, v_stride, q_out, act_type, layer, flags,
+                         pool->key_pool, pool->value_pool, pool->n_pages, pool->page_rows, true, stream);
+}
+
+size_t tle_prefill_bf16_paged_workspace_bytes(const tle_chunk_plan_t* plan) {
+    if (!plan || plan->part_rows <= 0) return 0;
+    return static_cast<size_t>(plan->part_rows) * (tle::kHeadDim + 1) * sizeof(float);
+}
+
+int tle_prefill_bf16_paged(const tle_shape_t* shape, const tle_page_pool_bf16_t* pool, const tle_chunk_plan_t* plan,
+                           const void* desc_dev, const void* q, int64_t q_stride, void* out, int64_t out_stride,
+                           int act_type, int layer, void* workspace, size_t workspace_bytes, void* stream) {
+    if (int rc = check_chunk_call(shape, plan, desc_dev, act_type, layer)) return rc;
+    if (!pool) return set_error(TLE_ERR_INVALID, "page pool and both pools must be non-null");
+    int shift = 0;
+    if (int rc = check_chunk_pool(shape, plan, pool->key_pool, pool->value_pool, pool->n_pages, pool->page_rows, 64, &shift))
+        return rc;
+    if (plan->n_tokens == 0) return ok();
+    if (int rc = check_rows(q, q_stride, shape->n_head, "q")) return rc;
+    if (int rc = check_rows(out, out_stride, shape->n_head, "out")) return rc;
+    const size_t need = tle_prefill_bf16_paged_workspace_bytes(plan);
+    if (need && (!workspace || workspace_bytes < need))
+        return set_error(TLE_ERR_WORKSPACE, "workspace %zu bytes < %zu needed", workspace_bytes, need);
+    if (need && !aligned16(workspace)) return set_error(TLE_ERR_INVALID, "workspace must be 16-byte aligned");
+    tle::ChunkArgs a{};
+    a.d = tle::chunk_desc(desc_dev, plan->n_seqs, plan->n_segs, plan->n_merge, plan->n_tokens);
+    a.n_tokens = plan->n_tokens;
+    a.n_ctas = plan->n_ctas;
+    a.n_segs = plan->n_segs;
+    a.n_merge = plan->n_merge;
+    a.merge_rows = plan->merge_rows;
+    a.q = q;
+    a.out = out;
+    a.q_stride = q_stride;
+    a.out_stride = out_stride;
+    const size_t layer_halfs = static_cast<size_t>(pool->n_pages) * pool->page_rows * shape->n_head_kv * tle::kHeadDim;
+    a.key_pool = static_cast<const uint16_t*>(pool->key_pool) + layer_halfs * layer;
+    a.value_pool = static_cast<const uint16_t*>(pool->value_pool) + layer_halfs * layer;
+    a.pool_pages = pool->n_pages;
+    a.page_shift = shift;
+    a.n_head = shape->n_head;
+    a.n_head_kv = shape->n_head_kv;
+    a.part_o = static_cast<float*>(workspace);
+    a.part_lse = need ? a.part_o + static_cast<size_t>(plan->part_rows) * tle::kHeadDim : nullptr;
+    cudaError_t e = tle::error_word(&a.err);
+    if (e != cudaSuccess) return cuda_error(e, "device error word");
+    e = tle::launch_chunk_attention(a, act_type == TLE_ACT_BF16, static_cast<cudaStream_t>(stream));
+    if (e != cudaSuccess) return cuda_error(e, "chunk attention launch");
+    return ok();
+}
+
+// ===================== logit rules (tle_forward.h) =====================
+
+int tle_logits_adjust(float* out, int64_t out_stride, const float* logits, int64_t logits_stride, int n_rows,
+                      int n_vocab, const tle_logit_rules_t* rules, void* stream) {
+    if (!out || !logits || !rules) return set_error(TLE_ERR_INVALID, "null pointer argument");
+    if (n_rows <= 0 || n_rows > 65535 || n_vocab <= 0 || n_vocab > (1 << 30))
+        return set_error(TLE_ERR_INVALID, "n_rows %d outside [1, 65535] or n_vocab %d outside [1, 2^30]", n_rows, n_vocab);
+    if (out_stride < n_vocab || logits_stride < n_vocab)
+        return set_error(TLE_ERR_INVALID, "out_stride %lld or logits_stride %lld < n_vocab", static_cast<long long>(out_stride),
+                         static_cast<long long>(logits_stride));
+    if (out == logits && out_stride != logits_stride)
+        return set_error(TLE_ERR_INVALID, "out is logits, with another stride");
+    const tle_logit_rules_t& r = *rules;
+    if (r.tokens && !r.token_start) return set_error(TLE_ERR_INVALID, "tokens without token_start");
+    if (!r.tokens && (r.repetition || r.frequency || r.presence))
+        return set_error(TLE_ERR_INVALID, "penalties without tokens");
+    if (r.bias_tokens && (!r.bias_values || !r.bias_start))
+        return set_error(TLE_ERR_INVALID, "bias_tokens without bias_values or bias_start");
+    if (r.n_tokens < 0 || r.n_biases < 0) return set_error(TLE_ERR_INVALID, "negative list length");
+    if (r.allowed && r.allowed_stride < (n_vocab + 31) / 32)
+        return set_error(TLE_ERR_INVALID, "allowed_stride %lld < %d words", static_cast<long long>(r.allowed_stride),
+                         (n_vocab + 31) / 32);
+    tle::LogitArgs a{};
+    a.logits = logits;
+    a.out = out;
+    a.n_vocab = n_vocab;
+    a.out_stride = out_stride;
+    a.logits_stride = logits_stride;
+    a.n_list_tokens = r.n_tokens;
+    a.n_list_biases = r.n_biases;
+    if (r.tokens && (r.repetition || r.frequency || r.presence)) {
+        a.tokens = r.tokens;
+        a.token_start = r.token_start;
+        a.n_prompt = r.n_prompt;
+        a.repetition = r.repetition;
+        a.frequency = r.frequency;
+        a.presence = r.presence;
+    }
+    if (r.bias_tokens) {
+        a.bias_tokens = r.bias_tokens;
+        a.bias_values = r.bias_values;
+        a.bias_start = r.bias_start;
+    }
+    a.allowed = r.allowed;
+    a.allowed_stride = r.allowed_stride;
+    cudaError_t e = tle::error_word(&a.err);
+    if (e != cudaSuccess) return cuda_error(e, "device error word");
+    e = tle::launch_logits_adjust(a, n_rows, static_cast<cudaStream_t>(stream));
+    if (e != cudaSuccess) return cuda_error(e, "logit rules launch");
+    return ok();
+}
+
+}  // extern "C"

@@ -338,6 +338,117 @@ cudaError_t launch_to_f16(uint16_t* out, const float* x, size_t n, uint32_t* err
 cudaError_t launch_embed_rows(int type, float* x, const void* table, const int32_t* tokens, int n_tokens,
                              int n_vocab, int n_embd, uint32_t* err, cudaStream_t stream);
 
+// ---- chunks of new tokens over a paged cache (chunk.cu) ----
+// Descriptor (built on the host by tle_chunk_desc_paged):
+//   ChunkHeader | ChunkSeq[n_seqs] | ChunkSeg[n_segs] | ChunkMerge[n_merge]
+//   | ChunkTok[n_tokens] | int32 cta_start[n_ctas + 1]
+// The attention works on rows: row t * g + h of a chunk and KV head is query
+// head h of the group (g = n_head / n_head_kv) of token t, so that a K/V tile
+// serves all the heads that share it.  An item is a block of kChunkItemRows
+// rows of one (chunk, KV head); a segment a range of kChunkTile-row K/V tiles
+// of one item, done by one CTA.
+constexpr int kChunkTile = 128;       // K/V rows per tile
+constexpr int kChunkRows = 128;       // rows per tensor-core tile
+constexpr int kChunkItemRows = 2 * kChunkRows;
+constexpr int32_t kChunkMagic = 0x544c4543;  // "TLEC"
+struct ChunkHeader {
+    int32_t magic, n_seqs, n_tokens, n_ctas, n_segs, n_merge;
+    int32_t reserved[2];
+};
+struct ChunkSeq {
+    const int32_t* pages;
+    int32_t n_pages, pos, n_tokens, first;   // first: batch index of its first token
+};
+struct ChunkSeg {
+    int32_t seq, kvh;
+    int32_t row0, n_rows;    // the item's rows (n_rows <= kChunkItemRows)
+    int32_t t0, t1;          // K/V tiles [t0, t1)
+    int32_t part;            // first row of this segment's partial results; -1: it writes out itself
+    int32_t reserved;
+};
+struct ChunkMerge {          // an item whose results are in n_parts blocks of n_rows partial rows
+    int32_t seq, kvh, row0, n_rows, part, n_parts;
+};
+struct ChunkTok {
+    int32_t seq, pos;
+};
+static_assert(sizeof(ChunkHeader) == 32 && sizeof(ChunkSeq) == 24 && sizeof(ChunkSeg) == 32 &&
+                  sizeof(ChunkMerge) == 24 && sizeof(ChunkTok) == 8,
+              "chunk descriptor records");
+struct ChunkDesc {           // device pointers into one descriptor
+    const ChunkSeq* seqs;
+    const ChunkSeg* segs;
+    const ChunkMerge* merges;
+    const ChunkTok* toks;
+    const int32_t* cta_start;
+};
+inline size_t chunk_desc_bytes(size_t n_seqs, size_t n_segs, size_t n_merge, size_t n_tokens, size_t n_ctas) {
+    return sizeof(ChunkHeader) + n_seqs * sizeof(ChunkSeq) + n_segs * sizeof(ChunkSeg) + n_merge * sizeof(ChunkMerge) +
+           n_tokens * sizeof(ChunkTok) + (n_ctas + 1) * sizeof(int32_t);
+}
+inline ChunkDesc chunk_desc(const void* base, size_t n_seqs, size_t n_segs, size_t n_merge, size_t n_tokens) {
+    const unsigned char* p = static_cast<const unsigned char*>(base) + sizeof(ChunkHeader);
+    ChunkDesc d;
+    d.seqs = reinterpret_cast<const ChunkSeq*>(p);
+    d.segs = reinterpret_cast<const ChunkSeg*>(d.seqs + n_seqs);
+    d.merges = reinterpret_cast<const ChunkMerge*>(d.segs + n_segs);
+    d.toks = reinterpret_cast<const ChunkTok*>(d.merges + n_merge);
+    d.cta_start = reinterpret_cast<const int32_t*>(d.toks + n_tokens);
+    return d;
+}
+struct AppendArgs {
+    ChunkDesc d;
+    int n_tokens;
+    const void* q;           // activations: fp32 or bf16
+    const void* k;
+    const void* v;
+    void* q_out;
+    int64_t q_stride, k_stride, v_stride;   // elements
+    void* key_pool;          // the layer's pages: [pool_pages][1 << page_shift][n_head_kv * 64]
+    void* value_pool;
+    int pool_pages, page_shift;
+    int n_head, n_head_kv;   // n_head 0: no q
+    int rotate;
+    uint32_t* err;
+    float inv_freq[kHeadDim / 2];
+};
+cudaError_t launch_append(const AppendArgs& a, bool act_bf16, bool pool_bf16, cudaStream_t stream);
+struct ChunkArgs {
+    ChunkDesc d;
+    int n_tokens, n_ctas, n_segs, n_merge, merge_rows;
+    const void* q;           // rotated; fp32 or bf16
+    void* out;
+    int64_t q_stride, out_stride;
+    const uint16_t* key_pool;     // the layer's pages, bf16
+    const uint16_t* value_pool;
+    int pool_pages, page_shift;
+    int n_head, n_head_kv;
+    float* part_o;           // [part_rows][64] normalised partial results
+    float* part_lse;         // [part_rows] log2 of the sum of exponentials; -inf: no row attended
+    uint32_t* err;
+};
+cudaError_t launch_chunk_attention(const ChunkArgs& a, bool act_bf16, cudaStream_t stream);
+// Logit rules (logits.cu): rules as in tle_forward.h, checked by the caller.
+struct LogitArgs {
+    const float* logits;
+    float* out;
+    int n_vocab, n_list_tokens, n_list_biases;
+    int64_t out_stride, logits_stride;
+    const int32_t* tokens;
+    const int32_t* token_start;
+    const int32_t* n_prompt;
+    const float* repetition;
+    const float* frequency;
+    const float* presence;
+    const int32_t* bias_tokens;
+    const float* bias_values;
+    const int32_t* bias_start;
+    const uint32_t* allowed;
+    int64_t allowed_stride;
+    uint32_t* err;
+};
+cudaError_t launch_logits_adjust(const LogitArgs& a, int n_rows, cudaStream_t stream);
+
 constexpr int kMaxDevices = 64;
 struct PerDeviceOnce {
     std::atomic<bool> done[kMaxDevices] = {};

@@ -47,6 +47,9 @@ EXPORTED = (
     "tle_forward_workspace_bytes", "tle_forward", "tle_forward_layers_one_launch", "tle_sample_temperature", "tle_sample_top_p",
     "tle_prompt_weights_bytes", "tle_prompt_pack_weights", "tle_prompt_scratch_bytes",
     "tle_prompt_forward",
+    # chunks over a paged cache, logit rules
+    "tle_chunk_desc_bytes", "tle_chunk_desc_paged", "tle_append_paged", "tle_append_bf16_paged",
+    "tle_prefill_bf16_paged_workspace_bytes", "tle_prefill_bf16_paged", "tle_logits_adjust",
 )
 
 
@@ -97,6 +100,28 @@ class PagePool(ctypes.Structure):
 class PagedSeq(ctypes.Structure):
     """tle_paged_seq_t: one sequence's device page table and decode position."""
     _fields_ = [("pages", ctypes.c_void_p), ("n_pages", ctypes.c_int32), ("pos", ctypes.c_int32)]
+
+
+class PagedChunk(ctypes.Structure):
+    """tle_paged_chunk_t: one sequence's device page table, cached rows and new tokens."""
+    _fields_ = [("pages", ctypes.c_void_p), ("n_pages", ctypes.c_int32), ("pos", ctypes.c_int32),
+                ("n_tokens", ctypes.c_int32), ("reserved", ctypes.c_int32)]
+
+
+class ChunkPlan(ctypes.Structure):
+    """tle_chunk_plan_t: what tle_chunk_desc_paged found out about a batch."""
+    _fields_ = [(n, ctypes.c_int32) for n in ("n_seqs", "n_tokens", "n_head", "n_head_kv", "page_rows",
+                                               "n_ctas", "n_segs", "n_merge", "merge_rows", "reserved")] + \
+               [("part_rows", ctypes.c_int64)]
+
+
+class LogitRulesDesc(ctypes.Structure):
+    """tle_logit_rules_t: the rules of tle_logits_adjust (device pointers)."""
+    _fields_ = [(n, ctypes.c_void_p) for n in ("tokens", "token_start", "n_prompt", "repetition",
+                                                "frequency", "presence", "bias_tokens", "bias_values",
+                                                "bias_start", "allowed")] + \
+               [("allowed_stride", ctypes.c_int64), ("n_tokens", ctypes.c_int32),
+                ("n_biases", ctypes.c_int32)]
 
 
 class Weight(ctypes.Structure):
@@ -192,6 +217,18 @@ def lib() -> ctypes.CDLL:
         L.tle_prompt_scratch_bytes.argtypes = [P(Model), i, i]
         L.tle_prompt_scratch_bytes.restype = sz
         L.tle_prompt_forward.argtypes = [P(Model), vp, P(State), vp, i, i, vp, sz, vp]
+        i64 = ctypes.c_int64
+        L.tle_chunk_desc_bytes.argtypes = [P(Shape), P(PagedChunk), i, i]
+        L.tle_chunk_desc_bytes.restype = sz
+        L.tle_chunk_desc_paged.argtypes = [P(Shape), i, P(PagedChunk), i, i, vp, sz, P(ChunkPlan)]
+        for name in ("tle_append_paged", "tle_append_bf16_paged"):
+            getattr(L, name).argtypes = [P(Shape), vp, P(ChunkPlan), vp, vp, i64, vp, i64, vp, i64, vp, i,
+                                         i, i, vp]
+        L.tle_prefill_bf16_paged_workspace_bytes.argtypes = [P(ChunkPlan)]
+        L.tle_prefill_bf16_paged_workspace_bytes.restype = sz
+        L.tle_prefill_bf16_paged.argtypes = [P(Shape), vp, P(ChunkPlan), vp, vp, i64, vp, i64, i, i, vp, sz,
+                                             vp]
+        L.tle_logits_adjust.argtypes = [vp, i64, vp, i64, i, i, P(LogitRulesDesc), vp]
         _lib = L
     return _lib
 
@@ -476,23 +513,31 @@ class DecodeBatch:
 class PagedKVCache:
     """Key/value page pools shared by a batch of sequences.
 
-    The pools are [n_layers][n_pages][page_rows][256] fp32; a sequence's row
-    r lives in row r % page_rows of page ``table[r // page_rows]``.  Page ids
+    The pools are [n_layers][n_pages][page_rows][256] fp32 (256 = n_head_kv *
+    head_dim of the shape), made here or given as ``pools`` = (keys, values);
+    a sequence's row r lives in row r % page_rows of page ``table[r // page_rows]``.  Page ids
     are handed out from a free list (``alloc`` / ``free``); the page tables
     are int32 CUDA tensors the caller keeps per sequence.  The reference keeps
     one contiguous [n_layers][n_ctx][256] cache per sequence (run_state.h:20-25).
     """
 
     def __init__(self, n_pages: int, page_rows: int = 256, shape: Optional[Shape] = None,
-                 device="cuda", dtype=None):
+                 device="cuda", dtype=None, pools=None):
         import torch
         self.shape = shape or tinyllama_shape()
         self.n_pages = int(n_pages)
         self.page_rows = int(page_rows)
         self.dtype = dtype or torch.float32   # torch.bfloat16: pools for PagedDecodeBatchBf16
-        dims = (self.shape.n_layers, self.n_pages, self.page_rows, 256)
-        self.key_pool = torch.zeros(dims, dtype=self.dtype, device=device)
-        self.value_pool = torch.zeros(dims, dtype=self.dtype, device=device)
+        dims = (self.shape.n_layers, self.n_pages, self.page_rows, self.shape.n_head_kv * self.shape.head_dim)
+        if pools is not None:
+            self.key_pool, self.value_pool = pools
+            for t in pools:
+                if tuple(t.shape) != dims or t.dtype != self.dtype or not t.is_contiguous() or \
+                        t.device != pools[0].device:
+                    raise ValueError(f"pools: need two contiguous {self.dtype} tensors of shape {dims}")
+        else:
+            self.key_pool = torch.zeros(dims, dtype=self.dtype, device=device)
+            self.value_pool = torch.zeros(dims, dtype=self.dtype, device=device)
         self._free = list(range(self.n_pages - 1, -1, -1))
 
     def pool(self):
@@ -576,6 +621,159 @@ class PagedDecodeBatch:
                                             _ptr(k), _ptr(v), _ptr(out), layer,
                                             _decode_flags(rotate, kv_ready), _ptr(self.workspace),
                                             self.workspace.numel() * 4, _stream(stream)))
+
+
+# ------------------------------------------------- chunks over a paged cache
+class PagedChunkBatch:
+    """One chunk of new tokens per sequence over a PagedKVCache: ``lengths[s]``
+    tokens (>= 0; 1 is a decode step) behind ``positions[s]`` cached rows,
+    through the int32 CUDA page table ``tables[s]``.
+
+    The tokens of all chunks are packed in sequence order: q and out
+    [tokens][n_head*64], k and v [tokens][n_head_kv*64], all float32 or all
+    bfloat16, rows contiguous and any row stride that is a multiple of 8.
+    ``append`` rotates q and k and stores k and v (fp32 or bf16 cache),
+    ``attend`` is the causal attention over a bf16 cache, ``run`` does both.
+    ``set_positions`` re-plans on the host and uploads the descriptor (one H2D
+    copy), once per step of all layers.  Calls of one batch share its
+    workspace: they must not overlap on the GPU.
+    """
+
+    def __init__(self, cache: PagedKVCache, tables: Sequence, positions: Sequence[int],
+                 lengths: Sequence[int], max_ctas: int = 0, stream=None):
+        import torch
+        self.cache = cache
+        self.shape = cache.shape
+        self.device = cache.key_pool.device
+        self.max_ctas = max_ctas
+        self.tables = list(tables)
+        self.n = len(self.tables)
+        for i, t in enumerate(self.tables):
+            if t.dtype != torch.int32 or t.device != self.device or not t.is_cuda or not t.is_contiguous():
+                raise ValueError(f"tables[{i}]: need a contiguous int32 tensor on {self.device}")
+        self.plan = ChunkPlan()
+        self._desc_dev = self.workspace = None
+        self._q = {}
+        self.set_positions(positions, lengths, stream)
+
+    def build_host(self, positions: Sequence[int], lengths: Sequence[int]):
+        """The descriptor in a new pinned host buffer (self.plan is set)."""
+        import torch
+        if len(positions) != self.n or len(lengths) != self.n:
+            raise ValueError("one position and one length per sequence")
+        chunks = (PagedChunk * max(self.n, 1))()
+        for i, t in enumerate(self.tables):
+            chunks[i] = PagedChunk(_ptr(t), int(t.numel()), int(positions[i]), int(lengths[i]), 0)
+        L = lib()
+        nbytes = L.tle_chunk_desc_bytes(ctypes.byref(self.shape), chunks, self.n, self.max_ctas)
+        if nbytes == 0:
+            _check(TLE_ERR_INVALID)
+        host = torch.empty(nbytes, dtype=torch.uint8, pin_memory=True)
+        plan = ChunkPlan()
+        _check(L.tle_chunk_desc_paged(ctypes.byref(self.shape), self.cache.page_rows, chunks, self.n,
+                                      self.max_ctas, host.data_ptr(), nbytes, ctypes.byref(plan)))
+        self.plan = plan
+        return host
+
+    def set_positions(self, positions: Sequence[int], lengths: Sequence[int], stream=None) -> None:
+        import torch
+        with torch.cuda.device(self.device):
+            host = self.build_host(positions, lengths)   # a new one: the last upload may be pending
+            s = stream or torch.cuda.current_stream()
+            with torch.cuda.stream(s):
+                if self._desc_dev is None or self._desc_dev.numel() < host.numel():
+                    self._desc_dev = torch.empty(host.numel(), dtype=torch.uint8, device=self.device)
+                self._desc_dev[:host.numel()].copy_(host, non_blocking=True)
+                nbytes = lib().tle_prefill_bf16_paged_workspace_bytes(ctypes.byref(self.plan))
+                if self.workspace is None or self.workspace.numel() * 4 < nbytes:
+                    self.workspace = torch.empty(max(nbytes // 4, 4), dtype=torch.float32, device=self.device)
+        self.positions = [int(p) for p in positions]
+        self.lengths = [int(x) for x in lengths]
+
+    def _rows(self, t, heads: int, name: str, dtype):
+        """Pointer and row stride of an activation tensor."""
+        import torch
+        if t.dtype not in (torch.float32, torch.bfloat16) or (dtype is not None and t.dtype != dtype):
+            raise ValueError(f"{name}: activations are all float32 or all bfloat16, got {t.dtype}")
+        if t.device != self.device:
+            raise ValueError(f"{name}: is on {t.device}, the cache on {self.device}")
+        w = heads * self.shape.head_dim
+        if t.dim() != 2 or t.shape[1] != w or t.shape[0] < self.plan.n_tokens or t.stride(1) != 1:
+            raise ValueError(f"{name}: need [{self.plan.n_tokens}][{w}] with contiguous rows, got "
+                             f"{tuple(t.shape)} with strides {t.stride()}")
+        return t.data_ptr(), (t.stride(0) if t.shape[0] > 1 else w)
+
+    def _on(self, stream):
+        """(stream handle, the tensors' device made current)."""
+        import torch
+        if stream is None:
+            return torch.cuda.current_stream(self.device).cuda_stream
+        if stream.device != self.device:
+            raise ValueError(f"stream of {stream.device}, tensors on {self.device}")
+        for t in (self._desc_dev, self.workspace):
+            t.record_stream(stream)
+        return stream.cuda_stream
+
+    def append(self, q, k, v, layer: int, rotate: bool = True, q_out=None, stream=None) -> None:
+        """rope(q, k) at each token's position (rotate), k and v stored in
+        their rows of the cache, q written to q_out (contiguous, the type of
+        q; may be q; q and q_out both None: keys and values only)."""
+        import torch
+        dt = k.dtype
+        kp, ks = self._rows(k, self.shape.n_head_kv, "k", None)
+        vp, vs = self._rows(v, self.shape.n_head_kv, "v", dt)
+        qp = qs = qo = None
+        if q is not None:
+            if q_out is None:
+                raise ValueError("q_out: where the rotated q goes")
+            qp, qs = self._rows(q, self.shape.n_head, "q", dt)
+            qo, os = self._rows(q_out, self.shape.n_head, "q_out", dt)
+            if os != self.shape.n_head * self.shape.head_dim:
+                raise ValueError("q_out: need a contiguous tensor")
+        elif q_out is not None:
+            raise ValueError("q_out without q")
+        L = lib()
+        fn = L.tle_append_paged if self.cache.dtype == torch.float32 else L.tle_append_bf16_paged
+        pool = self.cache.pool()
+        st = self._on(stream)
+        with torch.cuda.device(self.device):
+            _check(fn(ctypes.byref(self.shape), ctypes.addressof(pool), ctypes.byref(self.plan),
+                      self._desc_dev.data_ptr(), qp, qs or 0, kp, ks, vp, vs, qo, int(dt == torch.bfloat16),
+                      layer, TLE_DECODE_ROTATE if rotate else 0, st))
+
+    def attend(self, q, out, layer: int, stream=None) -> None:
+        """Causal attention of the chunks (q already rotated) over a bf16
+        cache; rows of out behind the last token are left as they are."""
+        import torch
+        if self.cache.dtype != torch.bfloat16:
+            raise ValueError("attend: a bfloat16 PagedKVCache expected")
+        qp, qs = self._rows(q, self.shape.n_head, "q", None)
+        op, os = self._rows(out, self.shape.n_head, "out", q.dtype)
+        pool = self.cache.pool()
+        st = self._on(stream)
+        with torch.cuda.device(self.device):
+            _check(lib().tle_prefill_bf16_paged(ctypes.byref(self.shape), ctypes.addressof(pool),
+                                                ctypes.byref(self.plan), self._desc_dev.data_ptr(), qp, qs,
+                                                op, os, int(q.dtype == torch.bfloat16), layer,
+                                                self.workspace.data_ptr(), self.workspace.numel() * 4, st))
+
+    def run(self, q, k, v, out, layer: int, rotate: bool = True, stream=None) -> None:
+        """append, then attend: the attention block of one layer for every
+        chunk.  q is left as it is (the rotated q goes through a buffer of
+        the batch)."""
+        import torch
+        if not rotate:
+            self.append(None, k, v, layer, rotate=False, stream=stream)
+            self.attend(q, out, layer, stream=stream)
+            return
+        buf = self._q.get(q.dtype)
+        if buf is None or buf.shape[0] < self.plan.n_tokens:
+            buf = self._q[q.dtype] = torch.empty((self.plan.n_tokens, self.shape.n_head * self.shape.head_dim),
+                                                 dtype=q.dtype, device=self.device)
+        if stream is not None:
+            buf.record_stream(stream)
+        self.append(q, k, v, layer, rotate=True, q_out=buf, stream=stream)
+        self.attend(buf, out, layer, stream=stream)
 
 
 # ------------------------------------------------- decode without allocation
@@ -701,6 +899,98 @@ def sample_top_p(logits, token_out, temperature: float, top_p: float, r: float, 
     _want(logits, 1, "logits")
     _check(lib().tle_sample_top_p(_ptr(logits), logits.numel(), temperature, top_p, r,
                                   _ptr(token_out), _stream(stream)))
+
+
+class LogitRules:
+    """The rules of logits_adjust for ``n_rows`` rows of ``n_vocab`` logits
+    (tle_logit_rules_t); every argument is a CUDA tensor, contiguous unless
+    said otherwise, and a group that is None is left out:
+
+    tokens, token_start  int32: the tokens of row r so far are
+        tokens[token_start[r]:token_start[r + 1]], the first n_prompt[r]
+        (int32, None: 0) of them given, the rest made;
+    repetition           float32 [n_rows]: tokens so far, x / rep where x > 0,
+        x * rep elsewhere;
+    frequency, presence  float32 [n_rows]: made tokens, - freq * times, - pres;
+    bias_tokens, bias_values, bias_start  int32, float32, int32: + the values
+        of bias_tokens[bias_start[r]:bias_start[r + 1]];
+    allowed              int32 [n_rows][>= ceil(n_vocab / 32)], any row stride:
+        bit t % 32 of word t / 32 clear: token t gets -inf.
+    """
+
+    _GROUPS = (("tokens", "int32"), ("token_start", "int32"), ("n_prompt", "int32"), ("repetition", "float32"),
+               ("frequency", "float32"), ("presence", "float32"), ("bias_tokens", "int32"),
+               ("bias_values", "float32"), ("bias_start", "int32"))
+
+    def __init__(self, n_rows: int, n_vocab: int, tokens=None, token_start=None, n_prompt=None,
+                 repetition=None, frequency=None, presence=None, bias_tokens=None, bias_values=None,
+                 bias_start=None, allowed=None):
+        import torch
+        given = {"tokens": tokens, "token_start": token_start, "n_prompt": n_prompt, "repetition": repetition,
+                 "frequency": frequency, "presence": presence, "bias_tokens": bias_tokens,
+                 "bias_values": bias_values, "bias_start": bias_start}
+        sizes = {"token_start": n_rows + 1, "bias_start": n_rows + 1, "n_prompt": n_rows, "repetition": n_rows,
+                 "frequency": n_rows, "presence": n_rows}
+        self.n_rows, self.n_vocab = int(n_rows), int(n_vocab)
+        self.device = None
+        for name, dt in self._GROUPS:
+            t = given[name]
+            if t is None:
+                continue
+            if t.dtype != getattr(torch, dt) or not t.is_cuda or not t.is_contiguous() or \
+                    t.numel() != sizes.get(name, t.numel()):
+                raise ValueError(f"{name}: need a contiguous {dt} CUDA tensor" +
+                                 (f" of {sizes[name]}" if name in sizes else ""))
+            self._same(t, name)
+        if tokens is None and any(given[x] is not None for x in ("token_start", "n_prompt", "repetition",
+                                                                 "frequency", "presence")):
+            raise ValueError("penalties need tokens and token_start")
+        if tokens is not None and token_start is None:
+            raise ValueError("tokens without token_start")
+        n_bias = sum(x is not None for x in (bias_tokens, bias_values, bias_start))
+        if n_bias not in (0, 3) or (n_bias and bias_tokens.numel() != bias_values.numel()):
+            raise ValueError("bias_tokens, bias_values and bias_start go together, one value per token")
+        stride = 0
+        if allowed is not None:
+            if allowed.dtype != torch.int32 or not allowed.is_cuda or allowed.dim() != 2 or \
+                    allowed.shape[0] != n_rows or allowed.shape[1] < -(-self.n_vocab // 32) or \
+                    (allowed.shape[1] > 1 and allowed.stride(1) != 1):
+                raise ValueError("allowed: need int32 CUDA words [n_rows][>= n_vocab / 32], rows contiguous")
+            self._same(allowed, "allowed")
+            stride = allowed.stride(0) if n_rows > 1 else allowed.shape[1]
+        self.keep = [*given.values(), allowed]
+        one = lambda t: None if t is None else (t.data_ptr() or None)  # noqa: E731
+        self.desc = LogitRulesDesc(*[one(given[n]) for n, _ in self._GROUPS], one(allowed), stride,
+                                   0 if tokens is None else tokens.numel(),
+                                   0 if bias_tokens is None else bias_tokens.numel())
+        if tokens is not None and tokens.numel() == 0:          # an empty list: no penalties
+            for n in ("tokens", "repetition", "frequency", "presence"):
+                setattr(self.desc, n, None)
+
+    def _same(self, t, name):
+        self.device = self.device or t.device
+        if t.device != self.device:
+            raise ValueError(f"{name}: is on {t.device}, the other rules on {self.device}")
+
+
+def logits_adjust(out, logits, rules: LogitRules, stream=None) -> None:
+    """out[r][t] = logits[r][t] under row r's rules (tle_logits_adjust), for
+    float32 CUDA tensors [n_rows][n_vocab] with contiguous rows and any row
+    stride; out may be logits.  Before sample_argmax / sample_temperature /
+    sample_top_p."""
+    import torch
+    for t, name in ((out, "out"), (logits, "logits")):
+        if t.dtype != torch.float32 or not t.is_cuda or tuple(t.shape) != (rules.n_rows, rules.n_vocab) or \
+                (rules.n_vocab > 1 and t.stride(1) != 1):
+            raise ValueError(f"{name}: need float32 CUDA [{rules.n_rows}][{rules.n_vocab}], rows contiguous")
+        if t.device != (rules.device or logits.device):
+            raise ValueError(f"{name}: is on {t.device}, the rules on {rules.device or logits.device}")
+    if stream is not None and stream.device != logits.device:
+        raise ValueError(f"stream of {stream.device}, tensors on {logits.device}")
+    rows = lambda t: t.stride(0) if rules.n_rows > 1 else rules.n_vocab  # noqa: E731
+    with torch.cuda.device(logits.device):
+        _check(lib().tle_logits_adjust(out.data_ptr(), rows(out), logits.data_ptr(), rows(logits), rules.n_rows,
+                                       rules.n_vocab, ctypes.byref(rules.desc), _stream(stream)))
 
 
 class DeviceModel:
