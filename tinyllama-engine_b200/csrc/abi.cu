@@ -1782,6 +1782,7 @@ int tle_prefill_bf16_paged(const tle_shape_t* shape, const tle_page_pool_bf16_t*
     a.page_shift = shift;
     a.n_head = shape->n_head;
     a.n_head_kv = shape->n_head_kv;
+    a.group = shape->n_head / shape->n_head_kv;
     a.part_o = static_cast<float*>(workspace);
     a.part_lse = need ? a.part_o + static_cast<size_t>(plan->part_rows) * tle::kHeadDim : nullptr;
     cudaError_t e = tle::error_word(&a.err);

@@ -422,7 +422,7 @@ struct ChunkArgs {
     const uint16_t* key_pool;     // the layer's pages, bf16
     const uint16_t* value_pool;
     int pool_pages, page_shift;
-    int n_head, n_head_kv;
+    int n_head, n_head_kv, group;   // group = n_head / n_head_kv
     float* part_o;           // [part_rows][64] normalised partial results
     float* part_lse;         // [part_rows] log2 of the sum of exponentials; -inf: no row attended
     uint32_t* err;
