@@ -131,18 +131,49 @@ __global__ void __launch_bounds__(kAppendThreads) append_kernel(const __grid_con
 // and if a row that only some of the item's tokens attend to is not finite,
 // the segment's rows are computed again one by one from global memory
 // (chunk_row_exact), which reads nothing but the attended rows.
-constexpr int CT_THREADS = 384;
+constexpr int CT_THREADS = 512;
 constexpr int CT_STAGES = 4;
 constexpr int kTile = kChunkTile;            // 128
 constexpr int kBox = 64;                     // rows per TMA box: the smallest bf16 page
 constexpr int kTileHalfs = kTile * HD;       // elements of a K or V tile (16 KB)
-constexpr int kRegsControl = 88, kRegsSoftmax = 208, kRegsLaunch = 168;
-static_assert(128 * kRegsControl + 256 * kRegsSoftmax <= CT_THREADS * kRegsLaunch,
+constexpr int kRegsControl = 56, kRegsLoader = 56, kRegsSoftmax = 200, kRegsLaunch = 128;
+static_assert(128 * (kRegsControl + kRegsLoader) + 256 * kRegsSoftmax <= CT_THREADS * kRegsLaunch,
               "setmaxnreg split exceeds the launch register budget");
 constexpr float kExpScale = kScale * kLog2e;
 // The reference maximum moves only when the row's maximum grows by more than
 // 8 (log2 units), so O is rescaled rarely; P <= 2^8.
 constexpr float kMoveThreshold = 8.0f;
+
+// A segment as the kernel's roles see it.
+struct Work {
+    const int32_t* pages;
+    int kvh, row0, n_rows, t0, t1, part;
+    int pos, first;
+    int pos_min, kv_len;   // position of the item's first token; rows of its last token
+    bool dual;
+    __device__ __forceinline__ bool edge(int n) const { return n * kTile + kTile - 1 > pos_min; }
+};
+__device__ __forceinline__ Work work_at(const ChunkArgs& A, int i) {
+    const ChunkSeg sg = A.d.segs[i];
+    const ChunkSeq sq = A.d.seqs[sg.seq];
+    Work w;
+    w.pages = sq.pages;
+    w.kvh = sg.kvh;
+    w.row0 = sg.row0;
+    w.n_rows = sg.n_rows;
+    w.t0 = sg.t0;
+    w.t1 = sg.t1;
+    w.part = sg.part;
+    w.pos = sq.pos;
+    w.first = sq.first;
+    const int g = A.group;
+    w.pos_min = sq.pos + sg.row0 / g;
+    w.kv_len = sq.pos + (sg.row0 + sg.n_rows - 1) / g + 1;
+    w.dual = sg.n_rows > kChunkRows;
+    return w;
+}
+
+constexpr int kWorkCache = 20;
 
 template <bool F32>
 struct ChunkSmem {
@@ -159,6 +190,7 @@ struct ChunkSmem {
     uint64_t scanned[2];                            // warp 3 is done with a segment's edge tiles
     uint64_t s_full[2], s_free[2], p_full[2], p_free[2];
     int bad[2];                                     // the segment has a non-finite masked V row
+    Work work[kWorkCache];                          // the CTA's first segments
     uint32_t tmem_base;
 };
 
@@ -266,35 +298,6 @@ struct ChunkTma {
     CUtensorMap k, v;   // the layer's pools as [pool rows][n_head_kv * 64] bf16, box {64, 64}
 };
 
-// A segment as the kernel's roles see it.
-struct Work {
-    const int32_t* pages;
-    int kvh, row0, n_rows, t0, t1, part;
-    int pos, first;
-    int pos_min, kv_len;   // position of the item's first token; rows of its last token
-    bool dual;
-    __device__ __forceinline__ bool edge(int n) const { return n * kTile + kTile - 1 > pos_min; }
-};
-__device__ __forceinline__ Work work_at(const ChunkArgs& A, int i) {
-    const ChunkSeg sg = A.d.segs[i];
-    const ChunkSeq sq = A.d.seqs[sg.seq];
-    Work w;
-    w.pages = sq.pages;
-    w.kvh = sg.kvh;
-    w.row0 = sg.row0;
-    w.n_rows = sg.n_rows;
-    w.t0 = sg.t0;
-    w.t1 = sg.t1;
-    w.part = sg.part;
-    w.pos = sq.pos;
-    w.first = sq.first;
-    const int g = A.group;
-    w.pos_min = sq.pos + sg.row0 / g;
-    w.kv_len = sq.pos + (sg.row0 + sg.n_rows - 1) / g + 1;
-    w.dual = sg.n_rows > kChunkRows;
-    return w;
-}
-
 // Where a row's result goes: 64 values in the type of q, or a partial row.
 template <class Act>
 struct RowOut {
@@ -388,11 +391,12 @@ __device__ __noinline__ void chunk_row_exact(const ChunkArgs& A, const Work& w, 
     }
 }
 
-// Warp roles (384 threads, one CTA per SM):
+// Warp roles (512 threads, one CTA per SM):
 //   warp 0      TMA producer of K/V tiles, all segments in order;
 //   warps 1, 2  MMA issuers of softmax warpgroup 1 / 2;
-//   warp 3      Q rows into shared memory (bf16 terms, swizzled), V of edge tiles;
-//   warps 4-11  softmax, one TMEM lane (= row) per thread.
+//   warp 3      V of the edge tiles;
+//   warps 4-11  softmax, one TMEM lane (= row) per thread;
+//   warps 12-15 Q rows into shared memory (bf16 terms, swizzled).
 template <bool F32>
 __global__ void __launch_bounds__(CT_THREADS, 1)
     chunk_attn_kernel(const __grid_constant__ ChunkArgs A, const __grid_constant__ ChunkTma M) {
@@ -410,7 +414,7 @@ __global__ void __launch_bounds__(CT_THREADS, 1)
             mbar_init(&S.v_ok[i], 1);
         }
         for (int i = 0; i < 2; ++i) {
-            mbar_init(&S.q_full[i], 1);
+            mbar_init(&S.q_full[i], 4);   // one arrival per loader warp
             mbar_init(&S.q_free[i], 2 + 8);
             mbar_init(&S.scanned[i], 1);
             mbar_init(&S.s_full[i], 1);
@@ -433,6 +437,9 @@ __global__ void __launch_bounds__(CT_THREADS, 1)
     // everything below reads what earlier kernels on the stream wrote
     asm volatile("griddepcontrol.wait;" ::: "memory");
     const int seg0 = A.d.cta_start[blockIdx.x], seg1 = A.d.cta_start[blockIdx.x + 1];
+    if (tid < kWorkCache && seg0 + tid < seg1) S.work[tid] = work_at(A, seg0 + tid);
+    __syncthreads();
+    auto work_of = [&](int i) { return i - seg0 < kWorkCache ? S.work[i - seg0] : work_at(A, i); };
     bool failed = false;
 
     if (wg == 0) {
@@ -441,7 +448,7 @@ __global__ void __launch_bounds__(CT_THREADS, 1)
             // ------------------------------ TMA producer ------------------------------
             int ring = 0;
             for (int i = seg0; i < seg1; ++i) {
-                const Work w = work_at(A, i);
+                const Work w = work_of(i);
                 const int pool_rows = A.pool_pages << A.page_shift;   // a box from here on is all zeros
                 // lane l holds where box b0 + l starts
                 int b0 = 2 * w.t0, y = 0;
@@ -480,53 +487,15 @@ __global__ void __launch_bounds__(CT_THREADS, 1)
             for (int u = ring > CT_STAGES ? ring - CT_STAGES : 0; u < ring && !failed; ++u)
                 wait_or_flag(&S.kv_full[u % CT_STAGES], (u / CT_STAGES) & 1, A.err, kErrDrain, failed);
         } else if (warp == 3) {
-            // -------------------- Q rows, and V of the edge tiles ----------------------
-            auto load_q = [&](int i, int k) {   // segment i, the k-th of this CTA
-                const Work w = work_at(A, i);
-                const int b = k % kQBufs;
-                if (k >= kQBufs) wait_or_flag(&S.q_free[b], ((k / kQBufs) - 1) & 1, A.err, kErrWaitEmpty, failed);
-                const int n_tiles = w.dual ? 2 : 1;
-                for (int e = lane; e < n_tiles * kChunkRows * (HD / 8); e += 32) {
-                    const int r = e >> 3, ch = e & 7;
-                    const int row = w.row0 + r, t = row / A.group, h = row - t * A.group;
-                    const Act* src = static_cast<const Act*>(A.q) + static_cast<int64_t>(w.first + t) * A.q_stride +
-                                     (w.kvh * A.group + h) * HD + ch * 8;
-                    const int off = (r & (kChunkRows - 1)) * HD + ((ch ^ (r & 7)) << 3);
-                    const bool ok = r < w.n_rows;
-                    if constexpr (!F32) {
-                        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(
-                                         smem_u32(&S.q[b][r >> 7][0][off])),
-                                     "l"(ok ? src : static_cast<const Act*>(A.q)), "r"(ok ? 16 : 0)
-                                     : "memory");
-                    } else {
-                        float x[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-                        if (ok) {
-                            const float4 a = reinterpret_cast<const float4*>(src)[0], c = reinterpret_cast<const float4*>(src)[1];
-                            x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w;
-                            x[4] = c.x; x[5] = c.y; x[6] = c.z; x[7] = c.w;
-                        }
-#pragma unroll
-                        for (int term = 0; term < kTerms; ++term) {
-                            *reinterpret_cast<uint4*>(&S.q[b][r >> 7][term][off]) =
-                                make_uint4(top_pair(x[0], x[1]), top_pair(x[2], x[3]), top_pair(x[4], x[5]), top_pair(x[6], x[7]));
-#pragma unroll
-                            for (int c2 = 0; c2 < 4; ++c2) f2_split(rest_pair(x[2 * c2], x[2 * c2 + 1]), x[2 * c2], x[2 * c2 + 1]);
-                        }
-                    }
-                }
-                if constexpr (!F32) cp_async_wait_all();
-                if (lane == 0) S.bad[k & 1] = 0;
-                fence_proxy_async_smem();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(&S.q_full[b]);
-            };
+            // -------------------------- V of the edge tiles ----------------------------
             int ring = 0;
-            if (kQBufs == 2 && seg0 < seg1) load_q(seg0, 0);
             for (int i = seg0; i < seg1; ++i) {
                 const int k = i - seg0;
-                if (kQBufs == 1) load_q(i, k);
-                else if (i + 1 < seg1) load_q(i + 1, k + 1);
-                const Work w = work_at(A, i);
+                const Work w = work_of(i);
+                // the Q of this segment is loaded only after the softmax is done with
+                // the segment that used this flag before
+                wait_or_flag(&S.q_full[k % kQBufs], (k / kQBufs) & 1, A.err, kErrWaitFull, failed);
+                if (lane == 0) S.bad[k & 1] = 0;
                 for (int n = w.t0; n < w.t1; ++n, ++ring) {
                     const int st = ring % CT_STAGES;
                     wait_or_flag(&S.kv_full[st], (ring / CT_STAGES) & 1, A.err, kErrWaitFull, failed);
@@ -567,7 +536,7 @@ __global__ void __launch_bounds__(CT_THREADS, 1)
             int seg = seg0, k = 0, n = 0;
             Work w{};
             if (seg < seg1) {
-                w = work_at(A, seg);
+                w = work_of(seg);
                 n = w.t0;
             }
             struct Own {
@@ -588,7 +557,7 @@ __global__ void __launch_bounds__(CT_THREADS, 1)
                         ++seg;
                         ++k;
                         if (seg == seg1) return false;
-                        w = work_at(A, seg);
+                        w = work_of(seg);
                         n = w.t0;
                         continue;
                     }
@@ -673,6 +642,70 @@ __global__ void __launch_bounds__(CT_THREADS, 1)
             }
             if (a > 0) wait_or_flag(&S.p_free[i], (a - 1) & 1, A.err, kErrDrain, failed);   // MMAs done before TMEM is freed
         }
+    } else if (wg == 3) {
+        // ------------------------------ Q loader -----------------------------------
+        regs_dealloc<kRegsLoader>();
+        const int lw = warp - 12;
+        for (int i = seg0; i < seg1; ++i) {
+            const int k = i - seg0, b = k % kQBufs;
+            const Work w = work_of(i);
+            if (k >= kQBufs) wait_or_flag(&S.q_free[b], ((k / kQBufs) - 1) & 1, A.err, kErrWaitEmpty, failed);
+            // 8 lanes per row, 4 rows per step, a quarter of each row tile per warp
+            const int ch = lane & 7;
+            for (int m = 0; m < (w.dual ? 2 : 1); ++m) {
+                auto source = [&](int r, bool& ok) {
+                    const int row = w.row0 + m * kChunkRows + r, t = row / A.group, h = row - t * A.group;
+                    ok = m * kChunkRows + r < w.n_rows;
+                    return ok ? static_cast<const Act*>(A.q) + static_cast<int64_t>(w.first + t) * A.q_stride +
+                                    (w.kvh * A.group + h) * HD + ch * 8
+                              : static_cast<const Act*>(A.q);
+                };
+                if constexpr (!F32) {
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) {
+                        const int r = lw * 32 + 4 * j + (lane >> 3);
+                        bool ok;
+                        const Act* src = source(r, ok);
+                        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(
+                                         smem_u32(&S.q[b][m][0][r * HD + ((ch ^ (r & 7)) << 3)])),
+                                     "l"(src), "r"(ok ? 16 : 0)
+                                     : "memory");
+                    }
+                } else {
+#pragma unroll
+                    for (int j0 = 0; j0 < 8; j0 += 4) {
+                        float4 x[4][2];
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) {
+                            bool ok;
+                            const float4* src = reinterpret_cast<const float4*>(source(lw * 32 + 4 * (j0 + j) + (lane >> 3), ok));
+                            x[j][0] = x[j][1] = make_float4(0.f, 0.f, 0.f, 0.f);
+                            if (ok) {
+                                x[j][0] = src[0];
+                                x[j][1] = src[1];
+                            }
+                        }
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) {
+                            const int r = lw * 32 + 4 * (j0 + j) + (lane >> 3);
+                            float* f = reinterpret_cast<float*>(x[j]);
+#pragma unroll
+                            for (int term = 0; term < kTerms; ++term) {
+                                *reinterpret_cast<uint4*>(&S.q[b][m][term][r * HD + ((ch ^ (r & 7)) << 3)]) =
+                                    make_uint4(top_pair(f[0], f[1]), top_pair(f[2], f[3]), top_pair(f[4], f[5]),
+                                               top_pair(f[6], f[7]));
+#pragma unroll
+                                for (int c = 0; c < 4; ++c) f2_split(rest_pair(f[2 * c], f[2 * c + 1]), f[2 * c], f[2 * c + 1]);
+                            }
+                        }
+                    }
+                }
+            }
+            if constexpr (!F32) cp_async_wait_all();
+            fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&S.q_full[b]);
+        }
     } else {
         // ------------------------------ softmax ------------------------------------
         regs_alloc<kRegsSoftmax>();
@@ -683,7 +716,7 @@ __global__ void __launch_bounds__(CT_THREADS, 1)
         int a = 0;   // own tiles so far (barrier phases)
         for (int sgi = seg0; sgi < seg1; ++sgi) {
             const int k = sgi - seg0;
-            const Work w = work_at(A, sgi);
+            const Work w = work_of(sgi);
             const int step = w.dual ? 1 : 2;
             const int n0 = w.dual ? w.t0 : w.t0 + i;
             if (n0 >= w.t1) {   // no tile of this segment is ours
