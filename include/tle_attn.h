@@ -350,9 +350,9 @@ typedef struct {
     int32_t n_seqs, n_tokens;      /* sequences; tokens of all chunks                  */
     int32_t n_head, n_head_kv;     /* the shape that the descriptor was made for       */
     int32_t page_rows;
-    int32_t n_ctas, n_segs;        /* attention: CTAs, and their pieces of work        */
+    int32_t n_ctas, n_few_ctas;    /* attention: CTAs of its two kernels (many and few rows) */
+    int32_t n_segs;                /* their pieces of work                             */
     int32_t n_merge, merge_rows;   /* row blocks split over pieces; rows of the largest */
-    int32_t reserved;
     int64_t part_rows;             /* partial result rows in the workspace             */
 } tle_chunk_plan_t;
 

@@ -9,7 +9,7 @@ import pytest
 
 import tle
 
-TILE, ITEM, ROWS = 128, 256, 128
+TILE, ITEM, FEW = 128, 256, 64
 P = 0x400000
 
 
@@ -41,9 +41,9 @@ def parse(buf, plan):
     segs = take(plan.n_segs, 32)
     merges = take(plan.n_merge, 24)
     toks = take(plan.n_tokens, 8)
-    start = take(plan.n_ctas + 1, 4)[:, 0]
+    start, few = take(plan.n_ctas + 1, 4)[:, 0], take(plan.n_few_ctas + 1, 4)[:, 0]
     assert at == len(b)
-    return seqs, segs, merges, toks, start
+    return seqs, segs, merges, toks, start, few
 
 
 @pytest.mark.parametrize("seed", range(12))
@@ -57,13 +57,15 @@ def test_plan_covers_every_tile_once(seed):
     rc, buf, plan = describe(pos, new, heads, max_ctas=max_ctas)
     assert rc == 0, tle.lib().tle_last_error()
     g = heads[0] // heads[1]
-    seqs, segs, merges, toks, start = parse(buf, plan)
+    seqs, segs, merges, toks, start, few = parse(buf, plan)
     assert plan.n_tokens == sum(new) and plan.n_seqs == n
     assert [tuple(x) for x in toks] == [(s, pos[s] + t) for s in range(n) for t in range(new[s])]
     first = np.cumsum([0] + new)[:-1]
     assert np.array_equal(seqs[:, 3], pos) and np.array_equal(seqs[:, 4], new) and np.array_equal(seqs[:, 5], first)
-    assert plan.n_ctas <= (max_ctas or 148)
-    assert start[0] == 0 and start[-1] == plan.n_segs and np.all(np.diff(start) >= 0)
+    assert max(plan.n_ctas, plan.n_few_ctas) <= (max_ctas or 148)
+    assert start[0] == 0 and start[-1] == few[0] and few[-1] == plan.n_segs
+    assert np.all(np.diff(start) >= 0) and np.all(np.diff(few) >= 0)
+    assert np.all(segs[:few[0], 3] > FEW) and np.all(segs[few[0]:, 3] <= FEW)   # many rows, then few
     items = {(s, h, r0): min(ITEM, new[s] * g - r0) for s in range(n) for h in range(heads[1])
              for r0 in range(0, new[s] * g, ITEM)}
     seen, parts = {k: [] for k in items}, {}
@@ -71,17 +73,15 @@ def test_plan_covers_every_tile_once(seed):
     for s, h, r0, rows, t0, t1, part, _ in segs:
         assert items[(s, h, r0)] == rows and t0 < t1
         seen[(s, h, r0)].append((t0, t1))
-        k = 1 if rows > ROWS else min(2, t1 - t0)
-        if part < 0:
-            assert k == 1
-        else:
-            used[part:part + k * rows] += 1
-            parts.setdefault((s, h, r0), []).append((part, k))
+        if part >= 0:
+            used[part:part + rows] += 1
+            parts.setdefault((s, h, r0), []).append(part)
     for (s, h, r0), rows in items.items():
         tiles = (pos[s] + (r0 + rows - 1) // g) // TILE + 1
         cuts = seen[(s, h, r0)]
         assert cuts[0][0] == 0 and cuts[-1][1] == tiles                # in order, without gaps
         assert all(a[1] == b[0] for a, b in zip(cuts, cuts[1:]))
+        assert len(cuts) == 1 or (s, h, r0) in parts                   # alone: it writes the result itself
     assert np.all(used == 1)
     merged = {}
     for s, h, r0, rows, part, k in merges:
@@ -90,11 +90,7 @@ def test_plan_covers_every_tile_once(seed):
     assert set(merged) == set(parts)
     for key, lst in parts.items():                                     # a block of partial rows per part, in order
         part, k = merged[key]
-        assert sum(x for _, x in lst) == k
-        at = part
-        for p, x in lst:
-            assert p == at
-            at += x * items[key]
+        assert lst == [part + j * items[key] for j in range(k)] and k == len(seen[key])
 
 
 def test_plan_balances_long_work():
@@ -102,7 +98,7 @@ def test_plan_balances_long_work():
     tiles above the even share."""
     rc, buf, plan = describe([30000], [2048])
     assert rc == 0
-    _, segs, _, _, start = parse(buf, plan)
+    _, segs, _, _, start, _ = parse(buf, plan)
     cost = [sum(2 * (x[5] - x[4]) for x in segs[a:b]) for a, b in zip(start, start[1:])]
     assert plan.n_ctas == 148 and max(cost) <= sum(cost) / 148 + 16
 

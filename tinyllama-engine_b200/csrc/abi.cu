@@ -1441,30 +1441,29 @@ int check_chunks(const tle_shape_t* shape, int page_rows, const tle_paged_chunk_
     return 0;
 }
 
-// The attention's work plan.  Costs are in half steps: a step of the kernel
-// takes one K/V tile for both row tiles of an item of more than kChunkRows
-// rows ("dual"), or two tiles for a smaller item, so a tile costs 2 or 1;
-// kSegUnits is the fixed cost of a segment (Q load, epilogue).
-constexpr int64_t kSegUnits = 4;
-constexpr int64_t kMinPieceUnits = 4;   // smallest piece of an item worth a CTA of its own
+// The attention's work plan, made apart for the items of either kernel: those
+// of at most kChunkFewRows rows, and the others.  Costs in units: a K/V tile
+// costs 1 for the few rows; 2 for an item of more than kChunkRows rows (both
+// chains do the whole tile) and 1 for one in between (each does half of it).
+// A segment has a fixed cost (Q load, joining and storing the result).
+constexpr int64_t kSegUnits = 4, kFewSegUnits = 2;
+constexpr int64_t kMinPieceUnits = 4, kFewMinPieceUnits = 2;   // smallest piece of an item worth a CTA of its own
 
 struct ChunkPlanner {
     const tle_shape_t* shape;
     const tle_paged_chunk_t* chunks;
     int n_seqs;
     int max_ctas;
-    int64_t n_items = 0, units = 0;
 
     struct Item {
         int seq, kvh, row0, n_rows, tiles;
+        bool few() const { return n_rows <= tle::kChunkFewRows; }
         int unit() const { return n_rows > tle::kChunkRows ? 2 : 1; }   // cost of a tile
-        int step() const { return n_rows > tle::kChunkRows ? 1 : 2; }   // tiles of a step
         int64_t cost() const { return static_cast<int64_t>(tiles) * unit(); }
-        int parts(int t) const { return n_rows > tle::kChunkRows ? 1 : std::min(2, t); }
     };
 
     template <class F>
-    void each_item(F&& f) const {
+    void each_item(bool few, F&& f) const {
         const int g = shape->n_head / shape->n_head_kv;
         for (int s = 0; s < n_seqs; ++s)
             for (int h = 0; h < shape->n_head_kv; ++h) {
@@ -1472,7 +1471,7 @@ struct ChunkPlanner {
                 for (int r = 0; r < rows; r += tle::kChunkItemRows) {
                     Item it{s, h, r, std::min(tle::kChunkItemRows, rows - r), 0};
                     it.tiles = (chunks[s].pos + (r + it.n_rows - 1) / g) / tle::kChunkTile + 1;
-                    f(it);
+                    if (it.few() == few) f(it);
                 }
             }
     }
@@ -1480,60 +1479,53 @@ struct ChunkPlanner {
     // Calls seg(cta, item, t0, t1, parts of the item, parts before) and
     // merge(item, parts) in order; returns the CTA count.
     template <class S, class M>
-    int run(S&& seg, M&& merge) {
-        n_items = units = 0;
-        each_item([&](const Item& it) {
+    int run(bool few, S&& seg, M&& merge) const {
+        const int64_t seg_units = few ? kFewSegUnits : kSegUnits, min_piece = few ? kFewMinPieceUnits : kMinPieceUnits;
+        int64_t n_items = 0, units = 0;
+        each_item(few, [&](const Item& it) {
             ++n_items;
             units += it.cost();
         });
+        if (n_items == 0) return 0;
         const int G = max_ctas;
+        // Few items: every item in equal pieces, one piece per CTA, the smallest
+        // piece for which the CTAs suffice -- unless cutting the items' concatenated
+        // costs evenly (below) leaves less for the longest CTA.
+        int64_t piece = std::max(min_piece, (units + G - 1) / G);
         if (n_items <= G) {
-            // few items: every item in equal pieces, one piece per CTA, the
-            // smallest piece for which the CTAs suffice
-            int64_t piece = std::max(kMinPieceUnits, (units + G - 1) / G);
             for (;;) {
                 int64_t n = 0;
-                each_item([&](const Item& it) { n += (it.cost() + piece - 1) / piece; });
+                each_item(few, [&](const Item& it) { n += (it.cost() + piece - 1) / piece; });
                 if (n <= G) break;
                 piece += std::max<int64_t>(1, piece / 16);
             }
+        }
+        const int64_t total = units + n_items * seg_units;
+        if (n_items <= G && piece + seg_units <= (total + G - 1) / G + 2 * seg_units) {
             int cta = 0;
-            each_item([&](const Item& it) {
+            each_item(few, [&](const Item& it) {
                 const int64_t k = (it.cost() + piece - 1) / piece;
-                auto cut = [&](int64_t j) {
-                    const int64_t t = j * it.tiles / k;
-                    return j >= k ? it.tiles : static_cast<int>((t + it.step() - 1) / it.step() * it.step());
-                };
-                int parts = 0;
-                for (int64_t j = 0; j < k; ++j) parts += it.parts(std::max(0, cut(j + 1) - cut(j)));
-                int before = 0;
-                for (int64_t j = 0; j < k; ++j) {
-                    const int a = cut(j), b = cut(j + 1);
-                    if (b <= a) continue;
-                    seg(cta++, it, a, b, parts, before);
-                    before += it.parts(b - a);
-                }
+                auto cut = [&](int64_t j) { return static_cast<int>(j * it.tiles / k); };
+                int parts = 0, before = 0;
+                for (int64_t j = 0; j < k; ++j) parts += cut(j + 1) > cut(j);
+                for (int64_t j = 0; j < k; ++j)
+                    if (cut(j + 1) > cut(j)) seg(cta++, it, cut(j), cut(j + 1), parts, before++);
                 if (parts > 1) merge(it, parts);
             });
             return cta;
         }
-        // many items: the concatenated cost of all items cut into G equal
-        // ranges, each boundary on a step of the item it falls into
-        const int64_t total = units + n_items * kSegUnits;
+        // the concatenated cost of all items cut into G equal ranges, each boundary
+        // on a tile of the item it falls into
         int64_t X = 0;
         int c = 0;
-        each_item([&](const Item& it) {
-            const int64_t end = X + kSegUnits + it.cost();
+        each_item(few, [&](const Item& it) {
+            const int64_t end = X + seg_units + it.cost();
             auto walk = [&](int c0, auto&& f) {   // f(cta, t0, t1); returns the CTA that goes on
                 int t = 0;
                 while (t < it.tiles) {
                     const int64_t x = c0 >= G - 1 ? end : (c0 + 1) * total / G;
                     int to = it.tiles;
-                    if (x < end) {
-                        const int64_t r = std::max<int64_t>(0, x - X - kSegUnits) / it.unit();
-                        to = static_cast<int>(r / it.step() * it.step());
-                        if (it.tiles - to < it.step()) to = it.tiles;
-                    }
+                    if (x < end) to = static_cast<int>(std::max<int64_t>(0, x - X - seg_units) / it.unit());
                     if (to > t) f(c0, t, to);
                     t = std::max(t, to);
                     if (x <= end && c0 < G - 1) ++c0;
@@ -1541,11 +1533,8 @@ struct ChunkPlanner {
                 return c0;
             };
             int parts = 0, before = 0;
-            walk(c, [&](int, int a, int b) { parts += it.parts(b - a); });
-            c = walk(c, [&](int cta, int a, int b) {
-                seg(cta, it, a, b, parts, before);
-                before += it.parts(b - a);
-            });
+            walk(c, [&](int, int, int) { ++parts; });
+            c = walk(c, [&](int cta, int a, int b) { seg(cta, it, a, b, parts, before++); });
             if (parts > 1) merge(it, parts);
             X = end;
         });
@@ -1621,7 +1610,7 @@ int append_common(const tle_shape_t* shape, const tle_chunk_plan_t* plan, const 
     if (int rc = check_rows(k, k_stride, shape->n_head_kv, "k")) return rc;
     if (int rc = check_rows(v, v_stride, shape->n_head_kv, "v")) return rc;
     tle::AppendArgs a{};
-    a.d = tle::chunk_desc(desc_dev, plan->n_seqs, plan->n_segs, plan->n_merge, plan->n_tokens);
+    a.d = tle::chunk_desc(desc_dev, plan->n_seqs, plan->n_segs, plan->n_merge, plan->n_tokens, plan->n_ctas);
     a.n_tokens = plan->n_tokens;
     a.q = q;
     a.k = k;
@@ -1652,12 +1641,13 @@ extern "C" {
 
 size_t tle_chunk_desc_bytes(const tle_shape_t* shape, const tle_paged_chunk_t* chunks, int n_seqs, int max_ctas) {
     if (check_chunks(shape, 0, chunks, n_seqs)) return 0;
-    ChunkPlanner p{shape, chunks, n_seqs, chunk_ctas(max_ctas)};
-    size_t segs = 0, merges = 0, tokens = 0;
-    const int G = p.run([&](int, const ChunkPlanner::Item&, int, int, int, int) { ++segs; },
-                        [&](const ChunkPlanner::Item&, int) { ++merges; });
+    const ChunkPlanner p{shape, chunks, n_seqs, chunk_ctas(max_ctas)};
+    size_t segs = 0, merges = 0, tokens = 0, ctas[2];
+    for (int few = 0; few < 2; ++few)
+        ctas[few] = p.run(few, [&](int, const ChunkPlanner::Item&, int, int, int, int) { ++segs; },
+                          [&](const ChunkPlanner::Item&, int) { ++merges; });
     for (int s = 0; s < n_seqs; ++s) tokens += static_cast<size_t>(chunks[s].n_tokens);
-    return tle::chunk_desc_bytes(n_seqs, segs, merges, tokens, G);
+    return tle::chunk_desc_bytes(n_seqs, segs, merges, tokens, ctas[0], ctas[1]);
 }
 
 int tle_chunk_desc_paged(const tle_shape_t* shape, int page_rows, const tle_paged_chunk_t* chunks, int n_seqs,
@@ -1666,16 +1656,17 @@ int tle_chunk_desc_paged(const tle_shape_t* shape, int page_rows, const tle_page
     if (page_rows < 16 || page_rows > 65536 || (page_rows & (page_rows - 1)) != 0)
         return set_error(TLE_ERR_INVALID, "page_rows %d is not a power of two in [16, 65536]", page_rows);
     if (int rc = check_chunks(shape, page_rows, chunks, n_seqs)) return rc;
-    ChunkPlanner p{shape, chunks, n_seqs, chunk_ctas(max_ctas)};
+    const ChunkPlanner p{shape, chunks, n_seqs, chunk_ctas(max_ctas)};
     tle_chunk_plan_t out{};
     int64_t segs = 0, merges = 0, part_rows = 0;
-    int merge_rows = 0;
-    const int G = p.run([&](int, const ChunkPlanner::Item&, int, int, int, int) { ++segs; },
-                        [&](const ChunkPlanner::Item& it, int parts) {
-                            ++merges;
-                            part_rows += static_cast<int64_t>(parts) * it.n_rows;
-                            merge_rows = std::max(merge_rows, it.n_rows);
-                        });
+    int merge_rows = 0, ctas[2];
+    for (int few = 0; few < 2; ++few)
+        ctas[few] = p.run(few, [&](int, const ChunkPlanner::Item&, int, int, int, int) { ++segs; },
+                          [&](const ChunkPlanner::Item& it, int parts) {
+                              ++merges;
+                              part_rows += static_cast<int64_t>(parts) * it.n_rows;
+                              merge_rows = std::max(merge_rows, it.n_rows);
+                          });
     int64_t tokens = 0;
     for (int s = 0; s < n_seqs; ++s) tokens += chunks[s].n_tokens;
     if (segs > INT32_MAX / 2 || part_rows > INT32_MAX / 2)
@@ -1685,24 +1676,24 @@ int tle_chunk_desc_paged(const tle_shape_t* shape, int page_rows, const tle_page
     out.n_head = shape->n_head;
     out.n_head_kv = shape->n_head_kv;
     out.page_rows = page_rows;
-    out.n_ctas = G;
+    out.n_ctas = ctas[0];
+    out.n_few_ctas = ctas[1];
     out.n_segs = static_cast<int32_t>(segs);
     out.n_merge = static_cast<int32_t>(merges);
     out.merge_rows = merge_rows;
     out.part_rows = part_rows;
-    const size_t need = tle::chunk_desc_bytes(n_seqs, segs, merges, tokens, G);
+    const size_t need = tle::chunk_desc_bytes(n_seqs, segs, merges, tokens, ctas[0], ctas[1]);
     if (desc_bytes < need)
         return set_error(TLE_ERR_INVALID, "descriptor buffer %zu bytes < %zu needed", desc_bytes, need);
     if ((reinterpret_cast<uintptr_t>(desc_host) & 7u) != 0)
         return set_error(TLE_ERR_INVALID, "desc_host must be 8-byte aligned");
     auto* hdr = static_cast<tle::ChunkHeader*>(desc_host);
-    *hdr = tle::ChunkHeader{tle::kChunkMagic, n_seqs, out.n_tokens, G, out.n_segs, out.n_merge, {0, 0}};
-    const tle::ChunkDesc d = tle::chunk_desc(desc_host, n_seqs, segs, merges, tokens);
+    *hdr = tle::ChunkHeader{tle::kChunkMagic, n_seqs, out.n_tokens, out.n_ctas, out.n_segs, out.n_merge, out.n_few_ctas, 0};
+    const tle::ChunkDesc d = tle::chunk_desc(desc_host, n_seqs, segs, merges, tokens, ctas[0]);
     auto* seq = const_cast<tle::ChunkSeq*>(d.seqs);
     auto* seg = const_cast<tle::ChunkSeg*>(d.segs);
     auto* mrg = const_cast<tle::ChunkMerge*>(d.merges);
     auto* tok = const_cast<tle::ChunkTok*>(d.toks);
-    auto* start = const_cast<int32_t*>(d.cta_start);
     int32_t first = 0;
     for (int s = 0; s < n_seqs; ++s) {
         const tle_paged_chunk_t& c = chunks[s];
@@ -1711,18 +1702,22 @@ int tle_chunk_desc_paged(const tle_shape_t* shape, int page_rows, const tle_page
         first += c.n_tokens;
     }
     int32_t part = 0, at = 0;
-    int cta_seen = 0;   // CTAs whose start is written
-    p.run(
-        [&](int cta, const ChunkPlanner::Item& it, int t0, int t1, int parts, int before) {
-            while (cta_seen <= cta) start[cta_seen++] = at;
-            seg[at++] = tle::ChunkSeg{it.seq, it.kvh, it.row0, it.n_rows, t0, t1,
-                                      parts > 1 ? part + before * it.n_rows : -1, 0};
-        },
-        [&](const ChunkPlanner::Item& it, int parts) {
-            *mrg++ = tle::ChunkMerge{it.seq, it.kvh, it.row0, it.n_rows, part, parts};
-            part += parts * it.n_rows;
-        });
-    while (cta_seen <= G) start[cta_seen++] = at;
+    for (int few = 0; few < 2; ++few) {
+        auto* start = const_cast<int32_t*>(few ? d.few_start : d.cta_start);
+        int seen = 0;   // CTAs whose start is written
+        p.run(
+            few,
+            [&](int cta, const ChunkPlanner::Item& it, int t0, int t1, int parts, int before) {
+                while (seen <= cta) start[seen++] = at;
+                seg[at++] = tle::ChunkSeg{it.seq, it.kvh, it.row0, it.n_rows, t0, t1,
+                                          parts > 1 ? part + before * it.n_rows : -1, 0};
+            },
+            [&](const ChunkPlanner::Item& it, int parts) {
+                *mrg++ = tle::ChunkMerge{it.seq, it.kvh, it.row0, it.n_rows, part, parts};
+                part += parts * it.n_rows;
+            });
+        while (seen <= ctas[few]) start[seen++] = at;
+    }
     *plan = out;
     return ok();
 }
@@ -1765,10 +1760,10 @@ int tle_prefill_bf16_paged(const tle_shape_t* shape, const tle_page_pool_bf16_t*
         return set_error(TLE_ERR_WORKSPACE, "workspace %zu bytes < %zu needed", workspace_bytes, need);
     if (need && !aligned16(workspace)) return set_error(TLE_ERR_INVALID, "workspace must be 16-byte aligned");
     tle::ChunkArgs a{};
-    a.d = tle::chunk_desc(desc_dev, plan->n_seqs, plan->n_segs, plan->n_merge, plan->n_tokens);
+    a.d = tle::chunk_desc(desc_dev, plan->n_seqs, plan->n_segs, plan->n_merge, plan->n_tokens, plan->n_ctas);
     a.n_tokens = plan->n_tokens;
     a.n_ctas = plan->n_ctas;
-    a.n_segs = plan->n_segs;
+    a.n_few_ctas = plan->n_few_ctas;
     a.n_merge = plan->n_merge;
     a.merge_rows = plan->merge_rows;
     a.q = q;

@@ -107,17 +107,22 @@ __global__ void __launch_bounds__(kAppendThreads) append_kernel(const __grid_con
 // item is up to 256 rows; a segment is a range of 128-row K/V tiles of an
 // item, and a CTA walks the segments that the plan gave it (ChunkPlanner in
 // abi.cu: the batch's tiles cut evenly over the SMs, so ragged batches, long
-// contexts with few tokens and whole prompts all fill the GPU).  An item of
-// more than 128 rows ("dual") has its two row tiles in the two softmax
-// warpgroups, which share each K/V tile; a smaller one has the same rows in
-// both, and they take the tiles alternately, so the tensor cores and the
-// exponentials of two tiles are in flight either way.
+// contexts with few tokens and whole prompts all fill the GPU).
 //
-// Per tile (M = 128 rows, N = 128 keys): S = Q K^T into TMEM, softmax by one
-// thread per row with a lazily moved reference maximum, P back into TMEM as
-// the A operand of O += P V.  K and V tiles come by TMA (two 64-row boxes,
-// each inside a page, 128-byte swizzle): K is K-major, V is read MN-major, so
-// nothing is transposed or copied beforehand.
+// Two chains per CTA, each a softmax warpgroup with its own scores S, running
+// maximum, sum and output O in tensor memory.  In an item of more than 128
+// rows ("dual") each chain has a row tile and they share every K/V tile; of a
+// smaller item both have the same rows and take its blocks of keys
+// alternately, and at the segment's end each joins the two results for half
+// of the columns.  A chain goes through its blocks (a tile; with fp32
+// activations half of one): S = Q K^T, softmax by one thread per row with a
+// lazily moved reference maximum, P into TMEM as the A operand of O += P V.
+// The next S is there before this block is done.  The two warps of a
+// scheduler, one of each chain, take turns at their exponentials, so that one
+// is at the exponential unit while the other loads, masks and packs.
+// K and V tiles come by TMA (two 64-row boxes, each inside a page, 128-byte
+// swizzle): K is K-major, V is read MN-major, so nothing is transposed or
+// copied beforehand.
 //
 // Precision: bf16 activations: P rounded to bf16 (its sum is not), fp32
 // accumulation.  fp32 activations: q and P are cut into three bf16 numbers of
@@ -127,17 +132,22 @@ __global__ void __launch_bounds__(kAppendThreads) append_kernel(const __grid_con
 // Rows beyond what a token attends to: a score is masked by selection, but
 // P = 0 does not silence a NaN or infinity in V.  Tiles that hold such rows
 // for any row of the item ("edge" tiles, the last one or two) therefore pass
-// through warp 3 first: rows behind the last one are zeroed in shared memory,
-// and if a row that only some of the item's tokens attend to is not finite,
-// the segment's rows are computed again one by one from global memory
+// through one warp first: rows behind the last one are zeroed in shared
+// memory, and if a row that only some of the item's tokens attend to is not
+// finite, the segment's rows are computed again one by one from global memory
 // (chunk_row_exact), which reads nothing but the attended rows.
 constexpr int CT_THREADS = 512;
+constexpr int kChains = 2;
 constexpr int CT_STAGES = 4;
 constexpr int kTile = kChunkTile;            // 128
 constexpr int kBox = 64;                     // rows per TMA box: the smallest bf16 page
 constexpr int kTileHalfs = kTile * HD;       // elements of a K or V tile (16 KB)
-constexpr int kRegsControl = 56, kRegsLoader = 56, kRegsSoftmax = 200, kRegsLaunch = 128;
-static_assert(128 * (kRegsControl + kRegsLoader) + 256 * kRegsSoftmax <= CT_THREADS * kRegsLaunch,
+template <bool F32>
+constexpr int kKeysOf = F32 ? 64 : 128;      // keys of a block
+template <bool F32>
+constexpr int kBufsOf = F32 ? 2 : 1;         // S and P buffers of a chain
+constexpr int kRegsControl = 56, kRegsSoftmax = 200, kRegsLaunch = 128;
+static_assert(256 * kRegsControl + 256 * kRegsSoftmax <= CT_THREADS * kRegsLaunch,
               "setmaxnreg split exceeds the launch register budget");
 constexpr float kExpScale = kScale * kLog2e;
 // The reference maximum moves only when the row's maximum grows by more than
@@ -183,25 +193,27 @@ struct ChunkSmem {
     uint16_t k[CT_STAGES][kTileHalfs];
     uint16_t v[CT_STAGES][kTileHalfs];
     uint64_t kv_full[CT_STAGES];
-    uint64_t kv_empty[CT_STAGES];                   // both MMA warps and warp 3
-    uint64_t v_ok[CT_STAGES];                       // edge tiles: V checked by warp 3
-    uint64_t q_full[2];
-    uint64_t q_free[2];                             // both MMA warps' last S and the 8 softmax warps
-    uint64_t scanned[2];                            // warp 3 is done with a segment's edge tiles
-    uint64_t s_full[2], s_free[2], p_full[2], p_free[2];
+    uint64_t kv_empty[CT_STAGES];                   // the PV issuers and the edge warp
+    uint64_t v_ok[CT_STAGES];                       // edge tiles: V checked
+    uint64_t q_full[2], q_free[2];
+    uint64_t scanned[2];                            // the segment's edge tiles are checked
+    uint64_t seg_end[2];                            // the softmax is done with the segment
+    uint64_t joined, read;                          // smaller items: both results there; both read
+    uint64_t s_full[kChains][2], s_free[kChains][2], p_full[kChains][2], p_free[kChains][2];
+    uint64_t turn[kChains][4];                      // a warp's turn at the exponentials
     int bad[2];                                     // the segment has a non-finite masked V row
-    Work work[kWorkCache];                          // the CTA's first segments
     uint32_t tmem_base;
+    Work work[kWorkCache];                          // the CTA's first segments
 };
 
-// TMEM columns (all 512).  bf16: S 128, P 64 and O 64 per warpgroup.  fp32:
-// the first two terms of P lie on S (read before they are written, and the
-// next S waits for the PV that reads them), the third beside it.
-constexpr uint32_t col_s(int i) { return 128u * i; }
-constexpr uint32_t col_p(int i) { return 256u + 64u * i; }
-constexpr uint32_t col_o(int i) { return 384u + 64u * i; }
+// TMEM columns (all 512): per chain S 128, P 64 and O 64.  fp32: two buffers
+// of 64 keys; the first two terms of P lie on the block's S (whose buffer is
+// free again after the PV that reads them), the third where bf16 has P.  At
+// the end of a smaller item's segment P's columns hold the row's maximum and sum.
+constexpr uint32_t col_s(int c, int h) { return 128u * c + 64u * h; }
+constexpr uint32_t col_p(int c, int h) { return 256u + 64u * c + 32u * h; }
+constexpr uint32_t col_o(int c) { return 384u + 64u * c; }
 
-constexpr uint32_t kIdS = idesc_bf16_f32(kChunkRows, kTile);
 constexpr uint32_t kIdO = idesc_bf16_f32(kChunkRows, HD) | (1u << 16);   // B (= V) MN-major
 
 // Shared-memory descriptor of 16 rows of V as an MN-major B operand: rows of
@@ -242,6 +254,8 @@ __device__ __forceinline__ float fmax3(float a, float b, float c) {
     asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
     return r;
 }
+// Which of 16 pairs take the way below: the rest go to the exponential unit.
+constexpr uint32_t kPolyPairs = (1u << 2) | (1u << 5) | (1u << 7) | (1u << 10) | (1u << 13);
 // 2^x for a pair on the FMA and ALU pipes: x = n + f with n the nearest
 // integer (the 1.5 2^23 shifter), 2^f by a cubic on [-1/2, 1/2] (relative
 // error 7.5e-5, a fiftieth of the bf16 rounding of P), n added to the
@@ -284,14 +298,55 @@ __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&r)[16
         : "memory");
 }
 
+__device__ __forceinline__ void tmem_ld16(uint32_t taddr, float (&v)[16]) {
+    uint32_t r[16];
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+          "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+        : "r"(taddr));
+#pragma unroll
+    for (int i = 0; i < 16; ++i) v[i] = __uint_as_float(r[i]);
+}
+
 // Bounded wait; after the first expiry in a thread its later waits return at
-// once, so a broken pipeline unwinds in about one timeout.
+// once, so a broken pipeline unwinds in about one timeout.  The timer is read
+// only after 256 probes: a wait here is short.
 __device__ __forceinline__ void wait_or_flag(uint64_t* bar, uint32_t parity, uint32_t* err, uint32_t code, bool& failed) {
-    if (failed) return;
-    if (!mbar_wait(bar, parity)) {
-        record_error(err, code);
-        failed = true;
+    if (failed || mbar_test_wait(bar, parity)) return;
+    uint64_t t0 = 0;
+    for (;;) {
+#pragma unroll 1
+        for (int i = 0; i < 256; ++i)
+            if (mbar_try_wait(bar, parity)) return;
+        const uint64_t t = globaltimer();
+        if (t0 == 0) t0 = t;
+        if (t - t0 > kWaitTimeoutNs) break;
     }
+    record_error(err, code);
+    failed = true;
+}
+
+// A value that all lanes have, in a form that the compiler knows to be uniform
+// (a warp reduction's result): what feeds an MMA's descriptors and the loops
+// around it must not go through per-lane registers, or every MMA waits for
+// half a dozen of them to be moved over.
+__device__ __forceinline__ int uniform(int x) { return __reduce_max_sync(0xffffffffu, x); }
+__device__ __forceinline__ uint32_t uniform(uint32_t x) { return __reduce_max_sync(0xffffffffu, x); }
+// wait_or_flag for a converged warp, with uniform branches.
+__device__ __forceinline__ void wait_uniform(uint64_t* bar, uint32_t parity, uint32_t* err, uint32_t code, bool& failed) {
+    if (failed || __all_sync(0xffffffffu, mbar_test_wait(bar, parity))) return;
+    uint64_t t0 = 0;
+    for (;;) {
+#pragma unroll 1
+        for (int i = 0; i < 256; ++i)
+            if (__all_sync(0xffffffffu, mbar_try_wait(bar, parity))) return;
+        const uint64_t t = globaltimer();
+        if (t0 == 0) t0 = t;
+        if (__any_sync(0xffffffffu, t - t0 > kWaitTimeoutNs)) break;
+    }
+    record_error(err, code);
+    failed = true;
 }
 
 struct ChunkTma {
@@ -305,17 +360,16 @@ struct RowOut {
     float* part;
     float* lse;
 };
-// r: the row's index in the item; block: which of the item's partial blocks
-// after the segment's first (0 or 1).
+// r: the row's index in the item.
 template <class Act>
-__device__ __forceinline__ RowOut<Act> row_out(const ChunkArgs& A, const Work& w, int r, int block) {
+__device__ __forceinline__ RowOut<Act> row_out(const ChunkArgs& A, const Work& w, int r) {
     RowOut<Act> o{};
     if (w.part < 0) {
         const int row = w.row0 + r, t = row / A.group, h = row - t * A.group;
         o.out = static_cast<Act*>(A.out) + static_cast<int64_t>(w.first + t) * A.out_stride +
                 (w.kvh * A.group + h) * HD;
     } else {
-        const size_t at = static_cast<size_t>(w.part) + static_cast<size_t>(block) * w.n_rows + r;
+        const size_t at = static_cast<size_t>(w.part) + r;
         o.part = A.part_o + at * HD;
         o.lse = A.part_lse + at;
     }
@@ -339,10 +393,16 @@ __device__ __forceinline__ void bf16x8(const uint4 w, float (&f)[8]) {
     }
 }
 
+// Whether any of 8 bf16 numbers has an exponent of all ones.
+__device__ __forceinline__ bool not_finite(const uint4 x) {
+    auto full = [](uint32_t u) { return ((u & 0x7f807f80u) + 0x00800080u) & 0x80008000u; };
+    return (full(x.x) | full(x.y) | full(x.z) | full(x.w)) != 0;
+}
+
 // One row of a segment from global memory, attended rows only: the way taken
-// when a masked row of V is not finite (see above); tiles t, t + step, ...
+// when a masked row of V is not finite (see above).
 template <class Act>
-__device__ __noinline__ void chunk_row_exact(const ChunkArgs& A, const Work& w, int r, int t, int step, RowOut<Act> dst) {
+__device__ __noinline__ void chunk_row_exact(const ChunkArgs& A, const Work& w, int r, RowOut<Act> dst) {
     const int row = w.row0 + r, tok = row / A.group, h = w.kvh * A.group + row - tok * A.group;
     const int pos = w.pos + tok;
     const Act* qp = static_cast<const Act*>(A.q) + static_cast<int64_t>(w.first + tok) * A.q_stride + h * HD;
@@ -355,9 +415,9 @@ __device__ __noinline__ void chunk_row_exact(const ChunkArgs& A, const Work& w, 
     }
     float m = -INFINITY, l = 0.f;
     const size_t rs = static_cast<size_t>(A.n_head_kv) * HD;
-    for (; t < w.t1; t += step) {
-        const int end = min((t + 1) * kTile, pos + 1);
-        for (int j = t * kTile; j < end; ++j) {
+    {
+        const int end = min(w.t1 * kTile, pos + 1);
+        for (int j = w.t0 * kTile; j < end; ++j) {
             const int id = w.pages[j >> A.page_shift];
             const bool ok = static_cast<unsigned>(id) < static_cast<unsigned>(A.pool_pages);
             const size_t at = ok ? (static_cast<size_t>(id) << A.page_shift) | (j & ((1 << A.page_shift) - 1)) : 0;
@@ -391,18 +451,70 @@ __device__ __noinline__ void chunk_row_exact(const ChunkArgs& A, const Work& w, 
     }
 }
 
+// A producer warp: the K/V tiles of segments [seg0, seg1) in order into a ring
+// of stages; a box (64 rows, within a page) by TMA each.
+template <int STAGES>
+__device__ __forceinline__ void produce_tiles(const ChunkArgs& A, const ChunkTma& M, int seg0, int seg1,
+                                              uint16_t (*k)[kTileHalfs], uint16_t (*v)[kTileHalfs], uint64_t* full,
+                                              uint64_t* empty, bool& failed) {
+    const int lane = threadIdx.x & 31;
+    const int pool_rows = A.pool_pages << A.page_shift;   // a box from here on is all zeros
+    int ring = 0;
+    for (int sg = seg0; sg < seg1; ++sg) {
+        const Work w = work_at(A, sg);
+        // lane l holds where box b0 + l starts
+        int b0 = 2 * w.t0, y = 0;
+        auto refill = [&]() {
+            const int r = (b0 + lane) * kBox;
+            y = pool_rows;
+            if (r < w.kv_len && b0 + lane < 2 * w.t1) {
+                const int id = w.pages[r >> A.page_shift];
+                if (static_cast<unsigned>(id) < static_cast<unsigned>(A.pool_pages))
+                    y = (id << A.page_shift) + (r & ((1 << A.page_shift) - 1));
+                else
+                    record_error(A.err, kErrBadPage);
+            }
+        };
+        refill();
+        for (int n = w.t0; n < w.t1; ++n, ++ring) {
+            if (2 * n - b0 >= 32) {
+                b0 = 2 * n;
+                refill();
+            }
+            const int st = ring % STAGES;
+            const int y0 = __shfl_sync(0xffffffffu, y, 2 * n - b0);
+            const int y1 = __shfl_sync(0xffffffffu, y, 2 * n - b0 + 1);
+            wait_or_flag(&empty[st], ((ring / STAGES) & 1) ^ 1, A.err, kErrWaitEmpty, failed);
+            if (lane == 0 && !failed) {
+                mbar_arrive_expect_tx(&full[st], 2 * kTileHalfs * 2);
+                tma_load_2d(k[st], &M.k, w.kvh * HD, y0, &full[st]);
+                tma_load_2d(k[st] + kBox * HD, &M.k, w.kvh * HD, y1, &full[st]);
+                tma_load_2d(v[st], &M.v, w.kvh * HD, y0, &full[st]);
+                tma_load_2d(v[st] + kBox * HD, &M.v, w.kvh * HD, y1, &full[st]);
+            }
+            __syncwarp();
+        }
+    }
+    // no copy may still be in flight when the CTA leaves
+    for (int u = ring > STAGES ? ring - STAGES : 0; u < ring && !failed; ++u)
+        wait_or_flag(&full[u % STAGES], (u / STAGES) & 1, A.err, kErrDrain, failed);
+}
+
 // Warp roles (512 threads, one CTA per SM):
-//   warp 0      TMA producer of K/V tiles, all segments in order;
-//   warps 1, 2  MMA issuers of softmax warpgroup 1 / 2;
-//   warp 3      V of the edge tiles;
-//   warps 4-11  softmax, one TMEM lane (= row) per thread;
-//   warps 12-15 Q rows into shared memory (bf16 terms, swizzled).
+//   warps 0, 1  issue S of chain 0, 1; warps 2, 3 issue PV (apart, so that
+//               neither stream waits for the other's operands);
+//   warps 4-11  softmax, a warpgroup per chain, one TMEM lane (= row) per thread;
+//   warp 12     TMA producer of K/V tiles, all segments in order;
+//   warp 13     V of the edge tiles;
+//   warps 14-15 Q rows into shared memory (bf16 terms, swizzled).
 template <bool F32>
 __global__ void __launch_bounds__(CT_THREADS, 1)
     chunk_attn_kernel(const __grid_constant__ ChunkArgs A, const __grid_constant__ ChunkTma M) {
     using Smem = ChunkSmem<F32>;
     using Act = std::conditional_t<F32, float, __nv_bfloat16>;
-    constexpr int kTerms = Smem::kTerms, kQBufs = Smem::kQBufs;
+    constexpr int kTerms = Smem::kTerms, kQBufs = Smem::kQBufs, kKeys = kKeysOf<F32>, kBufs = kBufsOf<F32>;
+    constexpr int kBlocks = kTile / kKeys;   // of a tile
+    constexpr uint32_t kIdS = idesc_bf16_f32(kChunkRows, kKeys);
     extern __shared__ __align__(1024) unsigned char smem_raw[];
     Smem& S = *reinterpret_cast<Smem*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, wg = warp >> 2;
@@ -410,18 +522,26 @@ __global__ void __launch_bounds__(CT_THREADS, 1)
     if (tid == 0) {
         for (int i = 0; i < CT_STAGES; ++i) {
             mbar_init(&S.kv_full[i], 1);
-            mbar_init(&S.kv_empty[i], 3);
+            mbar_init(&S.kv_empty[i], kChains + 1);
             mbar_init(&S.v_ok[i], 1);
         }
         for (int i = 0; i < 2; ++i) {
-            mbar_init(&S.q_full[i], 4);   // one arrival per loader warp
-            mbar_init(&S.q_free[i], 2 + 8);
+            mbar_init(&S.q_full[i], 2);          // one arrival per loader warp
+            mbar_init(&S.q_free[i], kChains);
             mbar_init(&S.scanned[i], 1);
-            mbar_init(&S.s_full[i], 1);
-            mbar_init(&S.s_free[i], 4);
-            mbar_init(&S.p_full[i], 4);
-            mbar_init(&S.p_free[i], 1);
+            mbar_init(&S.seg_end[i], 4 * kChains);   // one per softmax warp
         }
+        mbar_init(&S.joined, 4 * kChains);
+        mbar_init(&S.read, 4 * kChains);
+        for (int c = 0; c < kChains; ++c)
+            for (int q = 0; q < 4; ++q) mbar_init(&S.turn[c][q], 1);
+        for (int c = 0; c < kChains; ++c)
+            for (int h = 0; h < 2; ++h) {
+                mbar_init(&S.s_full[c][h], 1);
+                mbar_init(&S.s_free[c][h], 4);
+                mbar_init(&S.p_full[c][h], 4);
+                mbar_init(&S.p_free[c][h], 1);
+            }
         fence_barrier_init();
         prefetch_tmap(&M.k);
         prefetch_tmap(&M.v);
@@ -430,227 +550,165 @@ __global__ void __launch_bounds__(CT_THREADS, 1)
         tmem_alloc(&S.tmem_base, 512);
         tmem_relinquish();
     }
-    tc_fence_before();
-    __syncthreads();
-    tc_fence_after();
-    const uint32_t tmem = S.tmem_base;
     // everything below reads what earlier kernels on the stream wrote
     asm volatile("griddepcontrol.wait;" ::: "memory");
     const int seg0 = A.d.cta_start[blockIdx.x], seg1 = A.d.cta_start[blockIdx.x + 1];
     if (tid < kWorkCache && seg0 + tid < seg1) S.work[tid] = work_at(A, seg0 + tid);
+    tc_fence_before();
     __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = S.tmem_base;
     auto work_of = [&](int i) { return i - seg0 < kWorkCache ? S.work[i - seg0] : work_at(A, i); };
     bool failed = false;
 
     if (wg == 0) {
         regs_dealloc<kRegsControl>();
-        if (warp == 0) {
-            // ------------------------------ TMA producer ------------------------------
-            int ring = 0;
-            for (int i = seg0; i < seg1; ++i) {
-                const Work w = work_of(i);
-                const int pool_rows = A.pool_pages << A.page_shift;   // a box from here on is all zeros
-                // lane l holds where box b0 + l starts
-                int b0 = 2 * w.t0, y = 0;
-                auto refill = [&]() {
-                    const int r = (b0 + lane) * kBox;
-                    y = pool_rows;
-                    if (r < w.kv_len) {
-                        const int id = w.pages[r >> A.page_shift];
-                        if (static_cast<unsigned>(id) < static_cast<unsigned>(A.pool_pages))
-                            y = (id << A.page_shift) + (r & ((1 << A.page_shift) - 1));
-                        else if (b0 + lane < 2 * w.t1)
-                            record_error(A.err, kErrBadPage);
-                    }
-                };
-                refill();
-                for (int n = w.t0; n < w.t1; ++n, ++ring) {
-                    if (2 * n - b0 >= 32) {
-                        b0 = 2 * n;
-                        refill();
-                    }
+        const int c = uniform(warp & 1);   // the chain
+        const uint32_t tm = uniform(tmem);
+        int ring = 0, x = 0;   // K/V tiles and own blocks so far
+        const int n_seg = uniform(seg1 - seg0);
+        const uint32_t k0 = uniform(smem_u32(S.k[0])), v0 = uniform(smem_u32(S.v[0])), q0 = uniform(smem_u32(S.q[0][0][0]));
+        if (uniform(warp) < 2) {
+            // ------------------------------ S = Q K^T ------------------------------
+            for (int k = 0; k < n_seg; ++k) {
+                const int b = k % kQBufs;
+                const Work w = work_of(seg0 + k);
+                const int t0 = uniform(w.t0), t1 = uniform(w.t1), kv_len = uniform(w.kv_len);
+                const int dual = uniform(static_cast<int>(w.dual));
+                const uint32_t qa = q0 + (b * 2 + (dual ? c : 0)) * (kTerms * kTileHalfs * 2);
+                wait_uniform(&S.q_full[b], (k / kQBufs) & 1, A.err, kErrWaitFull, failed);
+                bool any = false;
+                for (int n = t0; n < t1; ++n, ++ring) {
                     const int st = ring % CT_STAGES;
-                    const int y0 = __shfl_sync(0xffffffffu, y, 2 * n - b0);
-                    const int y1 = __shfl_sync(0xffffffffu, y, 2 * n - b0 + 1);
-                    wait_or_flag(&S.kv_empty[st], ((ring / CT_STAGES) & 1) ^ 1, A.err, kErrWaitEmpty, failed);
-                    if (lane == 0 && !failed) {
-                        mbar_arrive_expect_tx(&S.kv_full[st], 2 * kTileHalfs * 2);
-                        tma_load_2d(S.k[st], &M.k, w.kvh * HD, y0, &S.kv_full[st]);
-                        tma_load_2d(S.k[st] + kBox * HD, &M.k, w.kvh * HD, y1, &S.kv_full[st]);
-                        tma_load_2d(S.v[st], &M.v, w.kvh * HD, y0, &S.kv_full[st]);
-                        tma_load_2d(S.v[st] + kBox * HD, &M.v, w.kvh * HD, y1, &S.kv_full[st]);
-                    }
-                    __syncwarp();
-                }
-            }
-            // no copy may still be in flight when the CTA leaves
-            for (int u = ring > CT_STAGES ? ring - CT_STAGES : 0; u < ring && !failed; ++u)
-                wait_or_flag(&S.kv_full[u % CT_STAGES], (u / CT_STAGES) & 1, A.err, kErrDrain, failed);
-        } else if (warp == 3) {
-            // -------------------------- V of the edge tiles ----------------------------
-            int ring = 0;
-            for (int i = seg0; i < seg1; ++i) {
-                const int k = i - seg0;
-                const Work w = work_of(i);
-                // the Q of this segment is loaded only after the softmax is done with
-                // the segment that used this flag before
-                wait_or_flag(&S.q_full[k % kQBufs], (k / kQBufs) & 1, A.err, kErrWaitFull, failed);
-                if (lane == 0) S.bad[k & 1] = 0;
-                for (int n = w.t0; n < w.t1; ++n, ++ring) {
-                    const int st = ring % CT_STAGES;
-                    wait_or_flag(&S.kv_full[st], (ring / CT_STAGES) & 1, A.err, kErrWaitFull, failed);
-                    if (w.edge(n)) {
-                        bool bad = false;
-                        const int some = max(0, w.pos_min + 1 - n * kTile);   // from here on not for every row
-                        const int none = w.kv_len - n * kTile;                // from here on for none
-                        uint4* v = reinterpret_cast<uint4*>(S.v[st]);
-                        for (int e = (some & ~3) * 8 + lane; e < kTile * 8; e += 32) {
-                            const int jl = e >> 3;
-                            if (jl >= none) v[e] = make_uint4(0, 0, 0, 0);
-                            else if (jl >= some) {
-                                const uint4 x = v[e];
-                                auto full = [](uint32_t u) { return ((u & 0x7f807f80u) + 0x00800080u) & 0x80008000u; };
-                                bad |= (full(x.x) | full(x.y) | full(x.z) | full(x.w)) != 0;   // exponent all ones
-                            }
+                    wait_uniform(&S.kv_full[st], (ring / CT_STAGES) & 1, A.err, kErrWaitFull, failed);
+                    for (int u = 0; u < kBlocks && n * kTile + u * kKeys < kv_len; ++u) {
+                        if (!dual && (((n - t0) * kBlocks + u) & 1) != c) continue;
+                        const int h = x % kBufs;
+                        // the buffer: its last scores read (bf16), its last P multiplied (fp32)
+                        if (x >= kBufs)
+                            wait_uniform(F32 ? &S.p_free[c][h] : &S.s_free[c][h], (x / kBufs - 1) & 1, A.err, kErrWaitMma, failed);
+                        tc_fence_after();
+                        const uint64_t dk = sw128_desc(k0 + (st * kTileHalfs + u * kKeys * HD) * 2), dq = sw128_desc(qa);
+                        const uint32_t tS = tm + col_s(c, h);
+                        if (elect_one()) {
+#pragma unroll
+                            for (int term = kTerms - 1; term >= 0; --term)   // the smallest first
+#pragma unroll
+                                for (int kk = 0; kk < HD / 16; ++kk)
+                                    umma_bf16(tS, dq + term * ((kTileHalfs * 2) >> 4) + 2 * kk, dk + 2 * kk, kIdS,
+                                              term < kTerms - 1 || kk > 0);
+                            umma_commit(&S.s_full[c][h]);
                         }
-                        if (__any_sync(0xffffffffu, bad) && lane == 0) S.bad[k & 1] = 1;
-                        fence_proxy_async_smem();
                         __syncwarp();
-                        if (lane == 0) mbar_arrive(&S.v_ok[st]);
+                        ++x;
+                        any = true;
                     }
-                    __syncwarp();
-                    if (lane == 0) mbar_arrive(&S.kv_empty[st]);
                 }
-                if (lane == 0) mbar_arrive(&S.scanned[k & 1]);
+                // Q may be replaced once these MMAs are done
+                if (any) {
+                    if (elect_one()) umma_commit(&S.q_free[b]);
+                } else if (lane == 0) {
+                    mbar_arrive(&S.q_free[b]);
+                }
+                __syncwarp();
             }
         } else {
-            // ------------------------------ MMA issuers --------------------------------
-            // Warp 1 + i serves softmax warpgroup i.  It walks every tile: its
-            // own ones get S = Q K^T (as soon as the softmax has read the last
-            // S, ahead of the last tile's PV) and O += P V, the others are
-            // released at once.
-            const int i = warp - 1;
-            const uint32_t tS = tmem + col_s(i), tP = tmem + col_p(i), tO = tmem + col_o(i);
-            int ring = 0;          // the tile the walk stands on
-            uint32_t v_par = 0;    // parity of the next v_ok of each stage
-            int seg = seg0, k = 0, n = 0;
-            Work w{};
-            if (seg < seg1) {
-                w = work_of(seg);
-                n = w.t0;
-            }
-            struct Own {
-                int ring, k;
-                bool first, edge;
-                uint32_t v_parity;
-            };
-            // The next own tile, the walk left behind it; false at the end.
-            auto next_own = [&](Own& o) {
-                while (seg < seg1) {
-                    if (n == w.t1) {
-                        const bool none = !w.dual && w.t0 + i >= w.t1;
-                        if (none) {   // no tile of this segment is ours: q_full first, so that the
-                                      // arrival belongs to this segment's phase
-                            wait_or_flag(&S.q_full[k % kQBufs], (k / kQBufs) & 1, A.err, kErrWaitFull, failed);
-                            if (lane == 0) mbar_arrive(&S.q_free[k % kQBufs]);
-                        }
-                        ++seg;
-                        ++k;
-                        if (seg == seg1) return false;
-                        w = work_of(seg);
-                        n = w.t0;
-                        continue;
-                    }
+            // ------------------------------ O += P V -------------------------------
+            uint32_t v_par = 0;   // parity of the next v_ok of each stage
+            for (int k = 0; k < n_seg; ++k) {
+                const Work w = work_of(seg0 + k);
+                const int t0 = uniform(w.t0), t1 = uniform(w.t1), kv_len = uniform(w.kv_len), pos_min = uniform(w.pos_min);
+                const int dual = uniform(static_cast<int>(w.dual));
+                uint32_t acc = 0;   // the segment's first block overwrites O
+                for (int n = t0; n < t1; ++n, ++ring) {
                     const int st = ring % CT_STAGES;
-                    const bool edge = w.edge(n);
-                    const bool mine = w.dual || ((n - w.t0) & 1) == i;
+                    const bool edge = n * kTile + kTile - 1 > pos_min;
                     const uint32_t par = (v_par >> st) & 1;
                     if (edge) v_par ^= 1u << st;
-                    if (mine) {
-                        o = Own{ring, k, n - w.t0 < (w.dual ? 1 : 2), edge, par};
-                        ++n;
-                        ++ring;
-                        return true;
+                    // our blocks of this tile: u0, u0 + du, ..., below u1
+                    const int u0 = dual ? 0 : (c + (n - t0) * kBlocks) & 1, du = dual ? 1 : 2;
+                    const int u1 = min(kBlocks, (kv_len - n * kTile + kKeys - 1) / kKeys);
+                    if (u0 >= u1) {
+                        wait_uniform(&S.kv_full[st], (ring / CT_STAGES) & 1, A.err, kErrWaitFull, failed);
+                        if (lane == 0) mbar_arrive(&S.kv_empty[st]);
+                        __syncwarp();
+                        continue;
                     }
-                    wait_or_flag(&S.kv_full[st], (ring / CT_STAGES) & 1, A.err, kErrWaitFull, failed);
-                    if (lane == 0) mbar_arrive(&S.kv_empty[st]);
-                    __syncwarp();
-                    ++n;
-                    ++ring;
-                }
-                return false;
-            };
-            // Whether the own tile just returned is the segment's last own one.
-            auto last_own = [&]() { return w.dual ? n == w.t1 : n + 1 >= w.t1; };
-            auto issue_s = [&](const Own& o, int a, bool last) {   // a: own tiles before this one
-                const int st = o.ring % CT_STAGES, b = o.k % kQBufs;
-                if (o.first) wait_or_flag(&S.q_full[b], (o.k / kQBufs) & 1, A.err, kErrWaitFull, failed);
-                wait_or_flag(&S.kv_full[st], (o.ring / CT_STAGES) & 1, A.err, kErrWaitFull, failed);
-                if (a > 0) wait_or_flag(F32 ? &S.p_free[i] : &S.s_free[i], (a - 1) & 1, A.err, kErrWaitMma, failed);
-                tc_fence_after();
-                if (elect_one()) {
-                    const int m = w.dual ? i : 0;
-                    const uint64_t dk = sw128_desc(smem_u32(S.k[st]));
+                    if (edge) wait_uniform(&S.v_ok[st], par, A.err, kErrWaitFull, failed);
+                    for (int u = u0; u < u1; u += du, ++x) {
+                        const int h = x % kBufs;
+                        wait_uniform(&S.p_full[c][h], (x / kBufs) & 1, A.err, kErrWaitMma, failed);
+                        tc_fence_after();
+                        const uint64_t dv = v_desc(v0 + (st * kTileHalfs + u * kKeys * HD) * 2);
+                        const uint32_t tP = tm + col_p(c, h), tS = tm + col_s(c, h), tO = tm + col_o(c);
+                        if (elect_one()) {
 #pragma unroll
-                    for (int term = kTerms - 1; term >= 0; --term) {   // the smallest first
-                        const uint64_t dq = sw128_desc(smem_u32(S.q[b][m][term]));
+                            for (int term = kTerms - 1; term >= 0; --term) {
+                                const uint32_t tp = term == kTerms - 1 ? tP : tS + 32u * term;
 #pragma unroll
-                        for (int kk = 0; kk < HD / 16; ++kk)
-                            umma_bf16(tS, dq + 2 * kk, dk + 2 * kk, kIdS, term < kTerms - 1 || kk > 0);
+                                for (int kk = 0; kk < kKeys / 16; ++kk)
+                                    umma_bf16_tmem_a(tO, tp + 8 * kk, dv + (2048 >> 4) * kk, kIdO,
+                                                     term < kTerms - 1 || kk > 0 ? 1u : acc);
+                            }
+                            umma_commit(&S.p_free[c][h]);
+                            if (u + du >= u1) umma_commit(&S.kv_empty[st]);
+                        }
+                        __syncwarp();
+                        acc = 1;
                     }
-                    umma_commit(&S.s_full[i]);
-                    if (last) umma_commit(&S.q_free[b]);
                 }
-                __syncwarp();
-            };
-            auto issue_pv = [&](const Own& o, int a) {
-                const int st = o.ring % CT_STAGES;
-                if (o.edge) wait_or_flag(&S.v_ok[st], o.v_parity, A.err, kErrWaitFull, failed);
-                wait_or_flag(&S.p_full[i], a & 1, A.err, kErrWaitMma, failed);
-                tc_fence_after();
-                if (elect_one()) {
-                    const uint64_t dv = v_desc(smem_u32(S.v[st]));
-#pragma unroll
-                    for (int term = kTerms - 1; term >= 0; --term) {
-                        const uint32_t tp = term == kTerms - 1 ? tP : tS + 64 * term;
-#pragma unroll
-                        for (int kk = 0; kk < kTile / 16; ++kk)
-                            umma_bf16_tmem_a(tO, tp + 8 * kk, dv + (2048 >> 4) * kk, kIdO,
-                                             (!o.first || term < kTerms - 1 || kk > 0) ? 1u : 0u);
-                    }
-                    umma_commit(&S.p_free[i]);
-                    umma_commit(&S.kv_empty[st]);
-                }
-                __syncwarp();
-            };
-            Own cur{}, nxt{};
-            int a = 0;
-            bool have = next_own(cur);
-            if (have) issue_s(cur, 0, last_own());
-            while (have) {
-                if constexpr (F32) {
-                    issue_pv(cur, a);
-                    have = next_own(nxt);
-                    if (have) issue_s(nxt, a + 1, last_own());
-                } else {
-                    have = next_own(nxt);
-                    if (have) issue_s(nxt, a + 1, last_own());
-                    issue_pv(cur, a);
-                }
-                cur = nxt;
-                ++a;
             }
-            if (a > 0) wait_or_flag(&S.p_free[i], (a - 1) & 1, A.err, kErrDrain, failed);   // MMAs done before TMEM is freed
+            for (int y = max(0, x - kBufs); y < x; ++y)   // MMAs done before TMEM is freed
+                wait_uniform(&S.p_free[c][y % kBufs], (y / kBufs) & 1, A.err, kErrDrain, failed);
+        }
+    } else if (warp == 12) {
+        regs_dealloc<kRegsControl>();
+        produce_tiles<CT_STAGES>(A, M, seg0, seg1, S.k, S.v, S.kv_full, S.kv_empty, failed);
+    } else if (warp == 13) {
+        // -------------------------- V of the edge tiles ----------------------------
+        regs_dealloc<kRegsControl>();
+        int ring = 0;
+        for (int sg = seg0; sg < seg1; ++sg) {
+            const int k = sg - seg0;
+            const Work w = work_of(sg);
+            // the flag was last read by the segment before the last one
+            if (k >= 2) wait_or_flag(&S.seg_end[k & 1], ((k - 2) >> 1) & 1, A.err, kErrWaitMma, failed);
+            if (lane == 0) S.bad[k & 1] = 0;
+            __syncwarp();
+            for (int n = w.t0; n < w.t1; ++n, ++ring) {
+                const int st = ring % CT_STAGES;
+                wait_or_flag(&S.kv_full[st], (ring / CT_STAGES) & 1, A.err, kErrWaitFull, failed);
+                if (w.edge(n)) {
+                    bool bad = false;
+                    const int some = max(0, w.pos_min + 1 - n * kTile);   // from here on not for every row
+                    const int none = w.kv_len - n * kTile;                // from here on for none
+                    uint4* v = reinterpret_cast<uint4*>(S.v[st]);
+                    for (int e = (some & ~3) * 8 + lane; e < kTile * 8; e += 32) {
+                        const int jl = e >> 3;
+                        if (jl >= none) v[e] = make_uint4(0, 0, 0, 0);
+                        else if (jl >= some) {
+                            bad |= not_finite(v[e]);
+                        }
+                    }
+                    if (__any_sync(0xffffffffu, bad) && lane == 0) S.bad[k & 1] = 1;
+                    fence_proxy_async_smem();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&S.v_ok[st]);
+                }
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&S.kv_empty[st]);
+            }
+            if (lane == 0) mbar_arrive(&S.scanned[k & 1]);
         }
     } else if (wg == 3) {
-        // ------------------------------ Q loader -----------------------------------
-        regs_dealloc<kRegsLoader>();
-        const int lw = warp - 12;
-        for (int i = seg0; i < seg1; ++i) {
-            const int k = i - seg0, b = k % kQBufs;
-            const Work w = work_of(i);
+        // ------------------------------ Q loaders ----------------------------------
+        regs_dealloc<kRegsControl>();
+        const int lw = warp - 14;
+        for (int sg = seg0; sg < seg1; ++sg) {
+            const int k = sg - seg0, b = k % kQBufs;
+            const Work w = work_of(sg);
             if (k >= kQBufs) wait_or_flag(&S.q_free[b], ((k / kQBufs) - 1) & 1, A.err, kErrWaitEmpty, failed);
-            // 8 lanes per row, 4 rows per step, a quarter of each row tile per warp
+            // 8 lanes per row, 4 rows per step, half of each row tile per warp
             const int ch = lane & 7;
             for (int m = 0; m < (w.dual ? 2 : 1); ++m) {
                 auto source = [&](int r, bool& ok) {
@@ -661,9 +719,9 @@ __global__ void __launch_bounds__(CT_THREADS, 1)
                               : static_cast<const Act*>(A.q);
                 };
                 if constexpr (!F32) {
-#pragma unroll
-                    for (int j = 0; j < 8; ++j) {
-                        const int r = lw * 32 + 4 * j + (lane >> 3);
+#pragma unroll 4
+                    for (int j = 0; j < 16; ++j) {
+                        const int r = lw * 64 + 4 * j + (lane >> 3);
                         bool ok;
                         const Act* src = source(r, ok);
                         asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(
@@ -672,13 +730,13 @@ __global__ void __launch_bounds__(CT_THREADS, 1)
                                      : "memory");
                     }
                 } else {
-#pragma unroll
-                    for (int j0 = 0; j0 < 8; j0 += 4) {
+#pragma unroll 1
+                    for (int j0 = 0; j0 < 16; j0 += 4) {
                         float4 x[4][2];
 #pragma unroll
                         for (int j = 0; j < 4; ++j) {
                             bool ok;
-                            const float4* src = reinterpret_cast<const float4*>(source(lw * 32 + 4 * (j0 + j) + (lane >> 3), ok));
+                            const float4* src = reinterpret_cast<const float4*>(source(lw * 64 + 4 * (j0 + j) + (lane >> 3), ok));
                             x[j][0] = x[j][1] = make_float4(0.f, 0.f, 0.f, 0.f);
                             if (ok) {
                                 x[j][0] = src[0];
@@ -687,7 +745,7 @@ __global__ void __launch_bounds__(CT_THREADS, 1)
                         }
 #pragma unroll
                         for (int j = 0; j < 4; ++j) {
-                            const int r = lw * 32 + 4 * (j0 + j) + (lane >> 3);
+                            const int r = lw * 64 + 4 * (j0 + j) + (lane >> 3);
                             float* f = reinterpret_cast<float*>(x[j]);
 #pragma unroll
                             for (int term = 0; term < kTerms; ++term) {
@@ -709,60 +767,63 @@ __global__ void __launch_bounds__(CT_THREADS, 1)
     } else {
         // ------------------------------ softmax ------------------------------------
         regs_alloc<kRegsSoftmax>();
-        const int i = wg - 1;
-        const int lr = tid - 128 * wg;                 // TMEM lane
-        const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
-        const uint32_t tS = tmem + lanes + col_s(i), tP = tmem + lanes + col_p(i), tO = tmem + lanes + col_o(i);
-        int a = 0;   // own tiles so far (barrier phases)
-        for (int sgi = seg0; sgi < seg1; ++sgi) {
-            const int k = sgi - seg0;
-            const Work w = work_of(sgi);
-            const int step = w.dual ? 1 : 2;
-            const int n0 = w.dual ? w.t0 : w.t0 + i;
-            if (n0 >= w.t1) {   // no tile of this segment is ours
-                wait_or_flag(&S.q_full[k % kQBufs], (k / kQBufs) & 1, A.err, kErrWaitFull, failed);
-                __syncwarp();
-                if (lane == 0) mbar_arrive(&S.q_free[k % kQBufs]);
-                continue;
-            }
-            const int r = w.dual ? 128 * i + lr : lr;  // row of the item
+        const int c = wg - 1;
+        const int lr = tid & 127;                      // TMEM lane
+        const uint32_t tL = tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16);
+        const uint32_t tO = tL + col_o(c);
+        int x = 0;        // own blocks so far (barrier phases)
+        int n_joins = 0;  // segments of smaller items so far
+        int turns = 0;    // turns taken: chain 0 first, then alternately
+        auto take_turn = [&]() {
+            if (c == 1 || turns > 0)
+                wait_or_flag(&S.turn[c][warp & 3], (c == 1 ? turns : turns - 1) & 1, A.err, kErrWaitMma, failed);
+            ++turns;
+        };
+        auto pass_turn = [&]() {
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&S.turn[1 - c][warp & 3]);
+        };
+        for (int sg = seg0; sg < seg1; ++sg) {
+            const int k = sg - seg0;
+            const Work w = work_of(sg);
+            const int r = w.dual ? kChunkRows * c + lr : lr;   // row of the item
             const int my_pos = w.pos + (w.row0 + min(r, w.n_rows - 1)) / A.group;
             float m_ref = -INFINITY;                   // reference maximum, log2 units
             float l_run = 0.f;
-            for (int n = n0; n < w.t1; n += step, ++a) {
-                wait_or_flag(&S.s_full[i], a & 1, A.err, kErrWaitMma, failed);
+            const int x0 = x;
+            const int key0 = w.t0 * kTile, key_end = min(w.t1 * kTile, w.kv_len);
+            for (int key = key0 + (w.dual ? 0 : c * kKeys); key < key_end; key += w.dual ? kKeys : 2 * kKeys, ++x) {
+                const int h = x % kBufs;
+                const uint32_t tS = tL + col_s(c, 0) + 64u * h, tP = tL + col_p(c, 0) + 32u * h;
+                wait_or_flag(&S.s_full[c][h], (x / kBufs) & 1, A.err, kErrWaitMma, failed);
                 tc_fence_after();
-                float s[kTile];
+                float s[kKeys];
 #pragma unroll
-                for (int c = 0; c < kTile / 32; ++c) {
-                    float tmp[32];
-                    tmem_ld32(tS + 32 * c, tmp);
-#pragma unroll
-                    for (int e = 0; e < 32; ++e) s[32 * c + e] = tmp[e];
-                }
+                for (int q = 0; q < kKeys / 32; ++q) tmem_ld32(tS + 32 * q, *reinterpret_cast<float(*)[32]>(&s[32 * q]));
                 tmem_wait_ld();
                 if constexpr (!F32) {
                     tc_fence_before();
                     __syncwarp();
-                    if (lane == 0) mbar_arrive(&S.s_free[i]);   // the MMA may overwrite S
+                    if (lane == 0) mbar_arrive(&S.s_free[c][h]);   // the MMA may overwrite S
                 }
-                const int left = my_pos - n * kTile;   // the last attended key of this tile
-                if (left < kTile - 1) {
+                const int left = my_pos - key;   // the block's last attended key
+                if (left < kKeys - 1) {
 #pragma unroll
-                    for (int e = 0; e < kTile; ++e)
+                    for (int e = 0; e < kKeys; ++e)
                         if (e > left) s[e] = -INFINITY;
                 }
-                float mc[16];
+                float mc[kKeys / 8];
 #pragma unroll
-                for (int c = 0; c < 16; ++c) {
-                    float m = fmax3(s[8 * c], s[8 * c + 1], s[8 * c + 2]);
-                    m = fmax3(m, s[8 * c + 3], s[8 * c + 4]);
-                    m = fmax3(m, s[8 * c + 5], s[8 * c + 6]);
-                    mc[c] = fmax3(m, s[8 * c + 7], m);
+                for (int q = 0; q < kKeys / 8; ++q) {
+                    float m = fmax3(s[8 * q], s[8 * q + 1], s[8 * q + 2]);
+                    m = fmax3(m, s[8 * q + 3], s[8 * q + 4]);
+                    m = fmax3(m, s[8 * q + 5], s[8 * q + 6]);
+                    mc[q] = fmax3(m, s[8 * q + 7], m);
                 }
-#pragma unroll
-                for (int c = 0; c < 5; ++c) mc[c] = fmax3(mc[3 * c], mc[3 * c + 1], mc[3 * c + 2]);
-                const float mt = fmax3(fmax3(mc[0], mc[1], mc[2]), fmax3(mc[3], mc[4], mc[15]), -INFINITY) * kExpScale;
+                float mt = fmax3(fmax3(mc[0], mc[1], mc[2]), fmax3(mc[3], mc[4], mc[5]), fmax3(mc[6], mc[7], mc[7]));
+                if constexpr (kKeys == 128)
+                    mt = fmax3(mt, fmax3(fmax3(mc[8], mc[9], mc[10]), mc[11], mc[12]), fmax3(mc[13], mc[14], mc[15]));
+                mt *= kExpScale;
                 float alpha = 1.f;
                 const bool move = m_ref == m_ref && !(mt <= m_ref + kMoveThreshold);   // to a NaN too, never from one
                 if (move) {
@@ -771,77 +832,59 @@ __global__ void __launch_bounds__(CT_THREADS, 1)
                 }
                 const float m_use = m_ref == -INFINITY ? 0.f : m_ref;   // nothing attended so far: weights 0
                 const uint64_t sc2 = f2(kExpScale, kExpScale), negm2 = f2(-m_use, -m_use);
-                // P and O may be touched once the previous PV is done
-                auto settle = [&]() {
-                    if (n > n0) {
-                        wait_or_flag(&S.p_free[i], (a - 1) & 1, A.err, kErrWaitMma, failed);
-                        tc_fence_after();
-                        if (__any_sync(0xffffffffu, move)) {
 #pragma unroll
-                            for (int c = 0; c < HD / 32; ++c) {
-                                float o[32];
-                                tmem_ld32(tO + 32 * c, o);
-                                tmem_wait_ld();
-                                uint32_t ob[32];
+                for (int e = 0; e < kKeys / 2; ++e)
+                    f2_split(ffma2(f2(s[2 * e], s[2 * e + 1]), sc2, negm2), s[2 * e], s[2 * e + 1]);
+                take_turn();
 #pragma unroll
-                                for (int e = 0; e < 32; ++e) ob[e] = __float_as_uint(o[e] * alpha);
-                                tmem_st32(tO + 32 * c, ob);
-                            }
-                        }
+                for (int e = 0; e < kKeys / 2; ++e) {
+                    // bf16: some of the pairs on the FMA pipe, the rest on the SFU
+                    if (!F32 && ((kPolyPairs >> (e & 15)) & 1)) {
+                        ex2_poly2(s[2 * e], s[2 * e + 1], s[2 * e], s[2 * e + 1]);
+                    } else {
+                        s[2 * e] = ex2_sfu(s[2 * e]);
+                        s[2 * e + 1] = ex2_sfu(s[2 * e + 1]);
                     }
-                };
+                }
+                pass_turn();
+                if (!F32 && left < kKeys - 1) {   // the cubic leaves 1e-38 at masked keys
+#pragma unroll
+                    for (int e = 0; e < kKeys; ++e)
+                        if (e > left) s[e] = 0.f;
+                }
+                // P and O may be touched once the last PV is done (fp32: P lies where only
+                // an earlier PV could be reading, and S was issued after that)
+                if (x > 0 && !F32) wait_or_flag(&S.p_free[c][0], (x - 1) & 1, A.err, kErrWaitMma, failed);
+                if (x > x0 && __any_sync(0xffffffffu, move)) {
+                    if (F32) wait_or_flag(&S.p_free[c][(x - 1) % kBufs], ((x - 1) / kBufs) & 1, A.err, kErrWaitMma, failed);
+                    tc_fence_after();
+#pragma unroll
+                    for (int q = 0; q < HD / 16; ++q) {
+                        float o[16];
+                        tmem_ld16(tO + 16 * q, o);
+                        tmem_wait_ld();
+                        uint32_t ob[16];
+#pragma unroll
+                        for (int e = 0; e < 16; ++e) ob[e] = __float_as_uint(o[e] * alpha);
+                        tmem_st16(tO + 16 * q, ob);
+                    }
+                }
                 uint64_t lsum2[4] = {f2(0.f, 0.f), f2(0.f, 0.f), f2(0.f, 0.f), f2(0.f, 0.f)};
-                if constexpr (!F32) {
-                    uint32_t pk[kTile / 2];
 #pragma unroll
-                    for (int e = 0; e < kTile / 2; ++e)
-                        f2_split(ffma2(f2(s[2 * e], s[2 * e + 1]), sc2, negm2), s[2 * e], s[2 * e + 1]);
+                for (int e = 0; e < kKeys / 2; ++e) lsum2[e & 3] = fadd2(lsum2[e & 3], f2(s[2 * e], s[2 * e + 1]));
 #pragma unroll
-                    for (int e = 0; e < kTile / 2; ++e) {   // 5 pairs in 16 on the FMA pipe, the rest on the SFU
-                        float p0, p1;
-                        if ((e & 15) == 2 || (e & 15) == 5 || (e & 15) == 7 || (e & 15) == 10 || (e & 15) == 13) {
-                            ex2_poly2(s[2 * e], s[2 * e + 1], p0, p1);
-                        } else {
-                            p0 = ex2_sfu(s[2 * e]);
-                            p1 = ex2_sfu(s[2 * e + 1]);
-                        }
-                        s[2 * e] = p0;
-                        s[2 * e + 1] = p1;
-                    }
-                    if (left < kTile - 1) {   // the cubic leaves 1e-38 at masked keys
+                for (int q = 0; q < kKeys / 32; ++q) {   // 32 keys: 16 columns of each term
+                    uint32_t pk[16];
 #pragma unroll
-                        for (int e = 0; e < kTile; ++e)
-                            if (e > left) s[e] = 0.f;
-                    }
-#pragma unroll
-                    for (int e = 0; e < kTile / 2; ++e) {
-                        lsum2[e & 3] = fadd2(lsum2[e & 3], f2(s[2 * e], s[2 * e + 1]));
-                        pk[e] = pack_bf16(s[2 * e], s[2 * e + 1]);
-                    }
-                    settle();
-                    tmem_st32(tP, *reinterpret_cast<const uint32_t(*)[32]>(&pk[0]));
-                    tmem_st32(tP + 32, *reinterpret_cast<const uint32_t(*)[32]>(&pk[32]));
-                } else {
-                    settle();
-#pragma unroll
-                    for (int c = 0; c < kTile / 32; ++c) {   // 32 keys: 16 columns of each term
-                        uint32_t t0[16], t1[16], t2[16];
+                    for (int term = 0; term < kTerms; ++term) {
 #pragma unroll
                         for (int e = 0; e < 16; ++e) {
-                            float x0, x1;
-                            f2_split(ffma2(f2(s[32 * c + 2 * e], s[32 * c + 2 * e + 1]), sc2, negm2), x0, x1);
-                            x0 = ex2_sfu(x0);
-                            x1 = ex2_sfu(x1);
-                            lsum2[e & 3] = fadd2(lsum2[e & 3], f2(x0, x1));
-                            t0[e] = top_pair(x0, x1);
-                            f2_split(rest_pair(x0, x1), x0, x1);
-                            t1[e] = top_pair(x0, x1);
-                            f2_split(rest_pair(x0, x1), x0, x1);
-                            t2[e] = top_pair(x0, x1);
+                            float& x0 = s[32 * q + 2 * e];
+                            float& x1 = s[32 * q + 2 * e + 1];
+                            pk[e] = F32 ? top_pair(x0, x1) : pack_bf16(x0, x1);
+                            if (F32 && term + 1 < kTerms) f2_split(rest_pair(x0, x1), x0, x1);
                         }
-                        tmem_st16(tS + 16 * c, t0);
-                        tmem_st16(tS + 64 + 16 * c, t1);
-                        tmem_st16(tP + 16 * c, t2);
+                        tmem_st16((term == kTerms - 1 ? tP : tS + 32 * term) + 16 * q, pk);
                     }
                 }
                 float lsum0, lsum1;
@@ -850,40 +893,89 @@ __global__ void __launch_bounds__(CT_THREADS, 1)
                 tmem_wait_st();
                 tc_fence_before();
                 __syncwarp();
-                if (lane == 0) mbar_arrive(&S.p_full[i]);
+                if (lane == 0) mbar_arrive(&S.p_full[c][h]);
             }
-            // ---- epilogue ----
-            wait_or_flag(&S.p_free[i], (a - 1) & 1, A.err, kErrWaitMma, failed);
+            if (c == 1 && !w.dual && ((key_end - key0 + kKeys - 1) / kKeys) % 2 == 1) {   // chain 0 had a block more
+                take_turn();
+                pass_turn();
+            }
+            // ---- the segment's result ----
+            for (int y = max(x0, x - kBufs); y < x; ++y)
+                wait_or_flag(&S.p_free[c][y % kBufs], (y / kBufs) & 1, A.err, kErrWaitMma, failed);
             wait_or_flag(&S.scanned[k & 1], (k >> 1) & 1, A.err, kErrWaitMma, failed);
             tc_fence_after();
             const bool mine = r < w.n_rows;
-            const RowOut<Act> dst = row_out<Act>(A, w, mine ? r : 0, w.dual ? 0 : i);
-            if (S.bad[k & 1]) {
-                if (mine) chunk_row_exact<Act>(A, w, r, n0, step, dst);
-                __syncwarp();
-            } else {
-                const bool empty = m_ref == -INFINITY;
-                const float inv = empty ? 0.f : 1.0f / l_run;
-#pragma unroll
-                for (int c = 0; c < HD / 32; ++c) {
-                    float o[32];
-                    tmem_ld32(tO + 32 * c, o);
+            const RowOut<Act> dst = row_out<Act>(A, w, mine ? r : 0);
+            // columns [col0, col1) of the row from up to two chains with weights f0, f1
+            // (a chain without weight may hold anything)
+            auto put = [&](int col0, int col1, uint32_t t0, float f0, uint32_t t1, float f1, bool two) {
+                for (int col = col0; col < col1; col += 16) {
+                    float o[16];
+                    tmem_ld16(t0 + col, o);
                     tmem_wait_ld();
 #pragma unroll
-                    for (int e = 0; e < 32; ++e) o[e] = empty ? 0.f : o[e] * inv;
+                    for (int e = 0; e < 16; ++e) o[e] = f0 != 0.f ? o[e] * f0 : 0.f;
+                    if (two) {
+                        float y[16];
+                        tmem_ld16(t1 + col, y);
+                        tmem_wait_ld();
+#pragma unroll
+                        for (int e = 0; e < 16; ++e) o[e] = f1 != 0.f ? fmaf(f1, y[e], o[e]) : o[e];
+                    }
                     if (mine) {
 #pragma unroll
-                        for (int e = 0; e < 32; e += 8) {
-                            if (dst.out) store8(dst.out + 32 * c + e, o + e);
-                            else store8(dst.part + 32 * c + e, o + e);
+                        for (int e = 0; e < 16; e += 8) {
+                            if (dst.out) store8(dst.out + col + e, o + e);
+                            else store8(dst.part + col + e, o + e);
                         }
                     }
                 }
-                if (mine && dst.lse) *dst.lse = empty ? -INFINITY : m_ref + log2f(l_run);
+            };
+            if (w.dual) {
+                if (S.bad[k & 1]) {
+                    const Work cold = w;   // a copy, so that w itself stays in registers
+                    if (mine) chunk_row_exact<Act>(A, cold, r, dst);
+                    __syncwarp();
+                } else {
+                    const bool empty = m_ref == -INFINITY;
+                    put(0, HD, tO, empty ? 0.f : 1.0f / l_run, 0u, 0.f, false);
+                    if (mine && dst.lse) *dst.lse = empty ? -INFINITY : m_ref + log2f(l_run);
+                }
+                tc_fence_before();
+            } else {
+                tmem_st2(tL + col_p(c, 0), m_ref, l_run);
+                tmem_wait_st();
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&S.joined);
+                wait_or_flag(&S.joined, n_joins & 1, A.err, kErrWaitMma, failed);
+                tc_fence_after();
+                if (S.bad[k & 1]) {
+                    const Work cold = w;
+                    if (mine && c == 0) chunk_row_exact<Act>(A, cold, r, dst);
+                    __syncwarp();
+                } else {
+                    float m0, l0, m1, l1;
+                    tmem_ld2(tL + col_p(0, 0), m0, l0);
+                    tmem_ld2(tL + col_p(1, 0), m1, l1);
+                    tmem_wait_ld();
+                    const float m_all = fmaxf(m0, m1);
+                    const float w0 = m0 != -INFINITY ? exp2f(m0 - m_all) : 0.f, w1 = m1 != -INFINITY ? exp2f(m1 - m_all) : 0.f;
+                    const float l_all = (w0 != 0.f ? w0 * l0 : 0.f) + (w1 != 0.f ? w1 * l1 : 0.f);
+                    const bool empty = l_all == 0.f;
+                    const float inv = empty ? 0.f : 1.0f / l_all;
+                    put(32 * c, 32 * c + 32, tL + col_o(0), w0 * inv, tL + col_o(1), w1 * inv, true);
+                    if (mine && dst.lse && c == 0) *dst.lse = empty ? -INFINITY : m_all + log2f(l_all);
+                }
+                // both have read before either's O or P columns are written again
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&S.read);
+                wait_or_flag(&S.read, n_joins & 1, A.err, kErrWaitMma, failed);
+                ++n_joins;
             }
-            tc_fence_before();
             __syncwarp();
-            if (lane == 0) mbar_arrive(&S.q_free[k % kQBufs]);
+            if (lane == 0) mbar_arrive(&S.seg_end[k & 1]);
         }
     }
     tc_fence_before();
@@ -891,6 +983,270 @@ __global__ void __launch_bounds__(CT_THREADS, 1)
     if (warp == 0) {
         tc_fence_after();
         tmem_dealloc(tmem, 512);
+    }
+}
+
+// ---- few rows --------------------------------------------------------------------
+// Items of at most kChunkFewRows rows (decode steps, a few guessed tokens) are
+// bound by the K/V bytes, and a 128-row tensor-core tile would be mostly empty:
+// here eight warps with 16-row mma.sync tiles (m16n8k16) share a tile, as row
+// groups of 16 rows times key groups of 128 / (16 groups) keys, each warp with its own running
+// maximum, sum and output in registers; the key groups of a row are joined in
+// shared memory at the segment's end.  K and V come through a ring of TMA
+// tiles as above, kept full across segments by a producer warp.  Precision
+// and the treatment of rows that not every token attends to as above.
+constexpr int FW_WARPS = 8;
+constexpr int FW_THREADS = 32 * (FW_WARPS + 1);
+constexpr int FW_STAGES = 5;
+struct FewSmem {
+    uint16_t k[FW_STAGES][kTileHalfs];
+    uint16_t v[FW_STAGES][kTileHalfs];
+    float o[FW_WARPS][16][HD + 4];      // a warp's result, and its rows' maximum and sum
+    float2 ml[FW_WARPS][16];
+    uint64_t full[FW_STAGES], empty[FW_STAGES];
+    int bad;                            // the segment has a non-finite V row that not every row attends to
+};
+
+__device__ __forceinline__ void ldsm4(uint32_t addr, uint32_t (&r)[4]) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+                 : "r"(addr)
+                 : "memory");
+}
+__device__ __forceinline__ void ldsm4_t(uint32_t addr, uint32_t (&r)[4]) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+                 : "r"(addr)
+                 : "memory");
+}
+__device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+        "{%0, %1, %2, %3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+template <bool F32>
+__global__ void __launch_bounds__(FW_THREADS, 1)
+    chunk_few_kernel(const __grid_constant__ ChunkArgs A, const __grid_constant__ ChunkTma M) {
+    using Act = std::conditional_t<F32, float, __nv_bfloat16>;
+    constexpr int kTerms = F32 ? 3 : 1;
+    extern __shared__ __align__(1024) unsigned char smem_raw[];
+    FewSmem& S = *reinterpret_cast<FewSmem*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    if (tid == 0) {
+        for (int i = 0; i < FW_STAGES; ++i) {
+            mbar_init(&S.full[i], 1);
+            mbar_init(&S.empty[i], FW_WARPS);
+        }
+        S.bad = 0;
+        fence_barrier_init();
+        prefetch_tmap(&M.k);
+        prefetch_tmap(&M.v);
+    }
+    __syncthreads();
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    const int seg0 = A.d.few_start[blockIdx.x], seg1 = A.d.few_start[blockIdx.x + 1];
+    bool failed = false;
+    if (warp == FW_WARPS) {
+        produce_tiles<FW_STAGES>(A, M, seg0, seg1, S.k, S.v, S.full, S.empty, failed);
+        return;
+    }
+    const int gid = lane >> 2, tg = lane & 3;     // fragment row and column pair
+    const int mi = lane >> 3, li = lane & 7;      // ldmatrix: matrix and row of this lane's address
+    int ring = 0;
+    for (int sg = seg0; sg < seg1; ++sg) {
+        const Work w = work_at(A, sg);
+        const int rgroups = (w.n_rows + 15) >> 4 <= 1 ? 1 : (w.n_rows + 15) >> 4 <= 2 ? 2 : 4;
+        const int keys = 16 * rgroups;            // of a tile, per warp
+        const int rg = warp % rgroups, kg = warp / rgroups;
+        // this lane's rows gid and gid + 8 of the row group, as A fragments of Q
+        int pos_r[2];
+        uint32_t qf[kTerms][HD / 16][4];
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+            const int r = rg * 16 + gid + 8 * e;
+            const bool ok = r < w.n_rows;
+            const int row = w.row0 + (ok ? r : 0), t = row / A.group, h = row - t * A.group;
+            pos_r[e] = w.pos + t;
+            const Act* src = static_cast<const Act*>(A.q) + static_cast<int64_t>(w.first + t) * A.q_stride +
+                             (w.kvh * A.group + h) * HD + 2 * tg;
+#pragma unroll
+            for (int ks = 0; ks < HD / 16; ++ks)
+#pragma unroll
+                for (int half = 0; half < 2; ++half) {
+                    if constexpr (F32) {
+                        float2 x = ok ? load_pair(src + 16 * ks + 8 * half) : make_float2(0.f, 0.f);
+#pragma unroll
+                        for (int term = 0; term < kTerms; ++term) {
+                            qf[term][ks][2 * half + e] = top_pair(x.x, x.y);
+                            f2_split(rest_pair(x.x, x.y), x.x, x.y);
+                        }
+                    } else {
+                        qf[0][ks][2 * half + e] = ok ? *reinterpret_cast<const uint32_t*>(src + 16 * ks + 8 * half) : 0u;
+                    }
+                }
+        }
+        float m_ref[2] = {-INFINITY, -INFINITY}, l_run[2] = {0.f, 0.f};
+        float o[HD / 8][4];
+#pragma unroll
+        for (int i = 0; i < HD / 8; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
+        for (int n = w.t0; n < w.t1; ++n, ++ring) {
+            const int st = ring % FW_STAGES;
+            wait_or_flag(&S.full[st], (ring / FW_STAGES) & 1, A.err, kErrWaitFull, failed);
+            const uint32_t kb = smem_u32(S.k[st]), vb = smem_u32(S.v[st]);
+            const bool edge = w.edge(n);
+            for (int j0 = kg * keys; j0 < (kg + 1) * keys; j0 += 16) {   // 16 keys
+                const int key0 = n * kTile + j0;
+                if (key0 >= w.kv_len) break;
+                if (edge) {
+                    // V rows behind the last one: zero; rows only some attend to: finite?
+                    bool bad = false;
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const int jl = 4 * e + (lane >> 3), key = key0 + jl;
+                        uint4* p = reinterpret_cast<uint4*>(S.v[st] + (j0 + jl) * HD) + (lane & 7);
+                        if (key >= w.kv_len) *p = make_uint4(0, 0, 0, 0);
+                        else if (key > w.pos_min) bad |= not_finite(*p);
+                    }
+                    if (__any_sync(0xffffffffu, bad) && lane == 0) S.bad = 1;
+                    __syncwarp();
+                }
+                float s[2][4];   // keys key0 + 8 b + 2 tg (+1): rows gid (0, 1), gid + 8 (2, 3)
+#pragma unroll
+                for (int b = 0; b < 2; ++b) s[b][0] = s[b][1] = s[b][2] = s[b][3] = 0.f;
+#pragma unroll
+                for (int ks = 0; ks < HD / 16; ++ks) {
+                    const int r = j0 + li + 8 * (mi >> 1), ch = 2 * ks + (mi & 1);
+                    uint32_t kf[4];
+                    ldsm4(kb + r * (HD * 2) + ((ch ^ (r & 7)) << 4), kf);
+#pragma unroll
+                    for (int term = kTerms - 1; term >= 0; --term) {
+                        mma16816(s[0], qf[term][ks], kf[0], kf[1]);
+                        mma16816(s[1], qf[term][ks], kf[2], kf[3]);
+                    }
+                }
+                if (edge) {
+#pragma unroll
+                    for (int b = 0; b < 2; ++b)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e)
+                            if (key0 + 8 * b + 2 * tg + (e & 1) > pos_r[e >> 1]) s[b][e] = -INFINITY;
+                }
+                float mt[2];
+#pragma unroll
+                for (int e = 0; e < 2; ++e)
+                    mt[e] = fmax3(fmax3(s[0][2 * e], s[0][2 * e + 1], s[1][2 * e]), s[1][2 * e + 1], -INFINITY) * kExpScale;
+                // m_ref is the same in the four lanes of a row
+                auto grows = [&](int e) { return m_ref[e] == m_ref[e] && !(mt[e] <= m_ref[e] + kMoveThreshold); };
+                if (__any_sync(0xffffffffu, grows(0) || grows(1))) {
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        float m = fmax3(mt[e], __shfl_xor_sync(0xffffffffu, mt[e], 1), -INFINITY);
+                        m = fmax3(m, __shfl_xor_sync(0xffffffffu, m, 2), -INFINITY);
+                        if (m_ref[e] == m_ref[e] && !(m <= m_ref[e] + kMoveThreshold)) {
+                            const float alpha = m_ref[e] == -INFINITY ? 0.f : exp2f(m_ref[e] - m);
+                            m_ref[e] = m;
+                            l_run[e] *= alpha;
+#pragma unroll
+                            for (int i = 0; i < HD / 8; ++i) {
+                                o[i][2 * e] *= alpha;
+                                o[i][2 * e + 1] *= alpha;
+                            }
+                        }
+                    }
+                }
+                const float m_use[2] = {m_ref[0] == -INFINITY ? 0.f : m_ref[0], m_ref[1] == -INFINITY ? 0.f : m_ref[1]};
+#pragma unroll
+                for (int b = 0; b < 2; ++b)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        s[b][e] = ex2_sfu(fmaf(s[b][e], kExpScale, -m_use[e >> 1]));
+                        l_run[e >> 1] += s[b][e];
+                    }
+                uint32_t pf[kTerms][4];   // A fragment of P: keys 2 tg (+1), then + 8
+                if constexpr (F32) {
+#pragma unroll
+                    for (int term = 0; term < kTerms; ++term)
+#pragma unroll
+                        for (int b = 0; b < 2; ++b)
+#pragma unroll
+                            for (int e = 0; e < 2; ++e) {
+                                pf[term][2 * b + e] = top_pair(s[b][2 * e], s[b][2 * e + 1]);
+                                f2_split(rest_pair(s[b][2 * e], s[b][2 * e + 1]), s[b][2 * e], s[b][2 * e + 1]);
+                            }
+                } else {
+#pragma unroll
+                    for (int b = 0; b < 2; ++b)
+#pragma unroll
+                        for (int e = 0; e < 2; ++e) pf[0][2 * b + e] = pack_bf16(s[b][2 * e], s[b][2 * e + 1]);
+                }
+#pragma unroll
+                for (int dp = 0; dp < HD / 16; ++dp) {
+                    const int r = j0 + li + 8 * (mi & 1), ch = 2 * dp + (mi >> 1);
+                    uint32_t vf[4];
+                    ldsm4_t(vb + r * (HD * 2) + ((ch ^ (r & 7)) << 4), vf);
+#pragma unroll
+                    for (int term = kTerms - 1; term >= 0; --term) {
+                        mma16816(o[2 * dp], pf[term], vf[0], vf[1]);
+                        mma16816(o[2 * dp + 1], pf[term], vf[2], vf[3]);
+                    }
+                }
+            }
+            if (edge) fence_proxy_async_smem();   // zeroed rows: before the stage's next TMA load
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&S.empty[st]);
+        }
+        // ---- join the key groups ----
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+            l_run[e] += __shfl_xor_sync(0xffffffffu, l_run[e], 1);
+            l_run[e] += __shfl_xor_sync(0xffffffffu, l_run[e], 2);
+            if (tg == 0) S.ml[warp][gid + 8 * e] = make_float2(m_ref[e], l_run[e]);
+#pragma unroll
+            for (int i = 0; i < HD / 8; ++i)
+                *reinterpret_cast<float2*>(&S.o[warp][gid + 8 * e][8 * i + 2 * tg]) = make_float2(o[i][2 * e], o[i][2 * e + 1]);
+        }
+        named_bar_sync(1, 32 * FW_WARPS);
+        if (S.bad) {
+            if (tid < w.n_rows) chunk_row_exact<Act>(A, w, tid, row_out<Act>(A, w, tid));
+        } else {
+            const int kgroups = FW_WARPS / rgroups;
+            for (int e = tid; e < w.n_rows * (HD / 8); e += 32 * FW_WARPS) {
+                const int r = e >> 3, c8 = (e & 7) * 8, w0 = r >> 4, rr = r & 15;
+                float m_all = -INFINITY;
+                for (int q = 0; q < kgroups; ++q) m_all = fmaxf(m_all, S.ml[w0 + q * rgroups][rr].x);
+                float acc[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f}, l_all = 0.f;
+                for (int q = 0; q < kgroups; ++q) {
+                    const float2 ml = S.ml[w0 + q * rgroups][rr];
+                    const float f = ml.x == -INFINITY ? 0.f : exp2f(ml.x - m_all);
+                    l_all = fmaf(f, ml.y, l_all);
+                    const float4* src = reinterpret_cast<const float4*>(&S.o[w0 + q * rgroups][rr][c8]);
+                    const float4 x = src[0], y = src[1];
+                    acc[0] = fmaf(f, x.x, acc[0]);
+                    acc[1] = fmaf(f, x.y, acc[1]);
+                    acc[2] = fmaf(f, x.z, acc[2]);
+                    acc[3] = fmaf(f, x.w, acc[3]);
+                    acc[4] = fmaf(f, y.x, acc[4]);
+                    acc[5] = fmaf(f, y.y, acc[5]);
+                    acc[6] = fmaf(f, y.z, acc[6]);
+                    acc[7] = fmaf(f, y.w, acc[7]);
+                }
+                const bool empty = l_all == 0.f;   // no row of this segment is attended to
+                const float inv = empty ? 0.f : 1.0f / l_all;
+#pragma unroll
+                for (int i = 0; i < 8; ++i) acc[i] = empty ? 0.f : acc[i] * inv;
+                const RowOut<Act> dst = row_out<Act>(A, w, r);
+                if (dst.out) store8(dst.out + c8, acc);
+                else store8(dst.part + c8, acc);
+                if (dst.lse && c8 == 0) *dst.lse = empty ? -INFINITY : m_all + log2f(l_all);
+            }
+        }
+        named_bar_sync(1, 32 * FW_WARPS);
+        if (tid == 0) S.bad = 0;   // next written after the next tile, read after the next barrier
+        named_bar_sync(1, 32 * FW_WARPS);
     }
 }
 
@@ -984,6 +1340,19 @@ cudaError_t launch_chunk_attn(const ChunkArgs& a, const ChunkTma& m, cudaStream_
     return cudaLaunchKernelEx(&L.cfg, chunk_attn_kernel<F32>, a, m);
 }
 
+template <bool F32>
+cudaError_t launch_chunk_few(const ChunkArgs& a, const ChunkTma& m, cudaStream_t stream) {
+    constexpr size_t smem = sizeof(FewSmem) + 1024;
+    static_assert(smem <= 232448, "shared memory of one SM");
+    static PerDeviceOnce once;
+    cudaError_t e = once.run([&](int) {
+        return cudaFuncSetAttribute(chunk_few_kernel<F32>, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
+    });
+    if (e != cudaSuccess) return e;
+    Launch L(dim3(a.n_few_ctas), FW_THREADS, smem, stream);
+    return cudaLaunchKernelEx(&L.cfg, chunk_few_kernel<F32>, a, m);
+}
+
 cudaError_t launch_chunk_attention(const ChunkArgs& a, bool act_bf16, cudaStream_t stream) {
     ChunkTma m;
     const uint64_t cols = static_cast<uint64_t>(a.n_head_kv) * HD, rows = static_cast<uint64_t>(a.pool_pages) << a.page_shift;
@@ -991,8 +1360,15 @@ cudaError_t launch_chunk_attention(const ChunkArgs& a, bool act_bf16, cudaStream
     if (e != cudaSuccess) return e;
     e = make_tmap_16b(&m.v, const_cast<uint16_t*>(a.value_pool), cols, rows, kBox, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16);
     if (e != cudaSuccess) return e;
-    e = act_bf16 ? launch_chunk_attn<false>(a, m, stream) : launch_chunk_attn<true>(a, m, stream);
-    if (e != cudaSuccess || a.n_merge == 0) return e;
+    if (a.n_few_ctas > 0) {
+        e = act_bf16 ? launch_chunk_few<false>(a, m, stream) : launch_chunk_few<true>(a, m, stream);
+        if (e != cudaSuccess) return e;
+    }
+    if (a.n_ctas > 0) {
+        e = act_bf16 ? launch_chunk_attn<false>(a, m, stream) : launch_chunk_attn<true>(a, m, stream);
+        if (e != cudaSuccess) return e;
+    }
+    if (a.n_merge == 0) return cudaSuccess;
     constexpr int warps = kMergeThreads / 32;
     Launch L(dim3(a.n_merge, (a.merge_rows + warps - 1) / warps), kMergeThreads, 0, stream);
     return act_bf16 ? cudaLaunchKernelEx(&L.cfg, chunk_merge_kernel<__nv_bfloat16>, a)

@@ -341,19 +341,20 @@ cudaError_t launch_embed_rows(int type, float* x, const void* table, const int32
 // ---- chunks of new tokens over a paged cache (chunk.cu) ----
 // Descriptor (built on the host by tle_chunk_desc_paged):
 //   ChunkHeader | ChunkSeq[n_seqs] | ChunkSeg[n_segs] | ChunkMerge[n_merge]
-//   | ChunkTok[n_tokens] | int32 cta_start[n_ctas + 1]
+//   | ChunkTok[n_tokens] | int32 cta_start[n_ctas + 1] | int32 few_start[n_few_ctas + 1]
 // The attention works on rows: row t * g + h of a chunk and KV head is query
 // head h of the group (g = n_head / n_head_kv) of token t, so that a K/V tile
 // serves all the heads that share it.  An item is a block of kChunkItemRows
 // rows of one (chunk, KV head); a segment a range of kChunkTile-row K/V tiles
-// of one item, done by one CTA.
+// of one item, done by one CTA; the segments of items of at most kChunkFewRows
+// rows come last (few_start), for a kernel of their own.
 constexpr int kChunkTile = 128;       // K/V rows per tile
 constexpr int kChunkRows = 128;       // rows per tensor-core tile
 constexpr int kChunkItemRows = 2 * kChunkRows;
+constexpr int kChunkFewRows = 64;
 constexpr int32_t kChunkMagic = 0x544c4543;  // "TLEC"
 struct ChunkHeader {
-    int32_t magic, n_seqs, n_tokens, n_ctas, n_segs, n_merge;
-    int32_t reserved[2];
+    int32_t magic, n_seqs, n_tokens, n_ctas, n_segs, n_merge, n_few_ctas, reserved;
 };
 struct ChunkSeq {
     const int32_t* pages;
@@ -381,12 +382,13 @@ struct ChunkDesc {           // device pointers into one descriptor
     const ChunkMerge* merges;
     const ChunkTok* toks;
     const int32_t* cta_start;
+    const int32_t* few_start;
 };
-inline size_t chunk_desc_bytes(size_t n_seqs, size_t n_segs, size_t n_merge, size_t n_tokens, size_t n_ctas) {
+inline size_t chunk_desc_bytes(size_t n_seqs, size_t n_segs, size_t n_merge, size_t n_tokens, size_t n_ctas, size_t n_few) {
     return sizeof(ChunkHeader) + n_seqs * sizeof(ChunkSeq) + n_segs * sizeof(ChunkSeg) + n_merge * sizeof(ChunkMerge) +
-           n_tokens * sizeof(ChunkTok) + (n_ctas + 1) * sizeof(int32_t);
+           n_tokens * sizeof(ChunkTok) + (n_ctas + n_few + 2) * sizeof(int32_t);
 }
-inline ChunkDesc chunk_desc(const void* base, size_t n_seqs, size_t n_segs, size_t n_merge, size_t n_tokens) {
+inline ChunkDesc chunk_desc(const void* base, size_t n_seqs, size_t n_segs, size_t n_merge, size_t n_tokens, size_t n_ctas) {
     const unsigned char* p = static_cast<const unsigned char*>(base) + sizeof(ChunkHeader);
     ChunkDesc d;
     d.seqs = reinterpret_cast<const ChunkSeq*>(p);
@@ -394,6 +396,7 @@ inline ChunkDesc chunk_desc(const void* base, size_t n_seqs, size_t n_segs, size
     d.merges = reinterpret_cast<const ChunkMerge*>(d.segs + n_segs);
     d.toks = reinterpret_cast<const ChunkTok*>(d.merges + n_merge);
     d.cta_start = reinterpret_cast<const int32_t*>(d.toks + n_tokens);
+    d.few_start = d.cta_start + n_ctas + 1;
     return d;
 }
 struct AppendArgs {
@@ -415,7 +418,7 @@ struct AppendArgs {
 cudaError_t launch_append(const AppendArgs& a, bool act_bf16, bool pool_bf16, cudaStream_t stream);
 struct ChunkArgs {
     ChunkDesc d;
-    int n_tokens, n_ctas, n_segs, n_merge, merge_rows;
+    int n_tokens, n_ctas, n_few_ctas, n_merge, merge_rows;
     const void* q;           // rotated; fp32 or bf16
     void* out;
     int64_t q_stride, out_stride;

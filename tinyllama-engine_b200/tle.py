@@ -111,7 +111,7 @@ class PagedChunk(ctypes.Structure):
 class ChunkPlan(ctypes.Structure):
     """tle_chunk_plan_t: what tle_chunk_desc_paged found out about a batch."""
     _fields_ = [(n, ctypes.c_int32) for n in ("n_seqs", "n_tokens", "n_head", "n_head_kv", "page_rows",
-                                               "n_ctas", "n_segs", "n_merge", "merge_rows", "reserved")] + \
+                                               "n_ctas", "n_few_ctas", "n_segs", "n_merge", "merge_rows")] + \
                [("part_rows", ctypes.c_int64)]
 
 
