@@ -117,9 +117,11 @@ __global__ void __launch_bounds__(kAppendThreads) append_kernel(const __grid_con
 // of the columns.  A chain goes through its blocks (a tile; with fp32
 // activations half of one): S = Q K^T, softmax by one thread per row with a
 // lazily moved reference maximum, P into TMEM as the A operand of O += P V.
-// The next S is there before this block is done.  The two warps of a
-// scheduler, one of each chain, take turns at their exponentials, so that one
-// is at the exponential unit while the other loads, masks and packs.
+// The next S is there before this block is done.  A scheduler has two softmax
+// warps, so what a warp waits for costs time: barriers are probed ahead of
+// their use, and between the scores' load and the first store of P there is
+// no branch, so that the compiler can overlap maximum, exponentials, sums and
+// packing.
 // K and V tiles come by TMA (two 64-row boxes, each inside a page, 128-byte
 // swizzle): K is K-major, V is read MN-major, so nothing is transposed or
 // copied beforehand.
@@ -200,7 +202,6 @@ struct ChunkSmem {
     uint64_t seg_end[2];                            // the softmax is done with the segment
     uint64_t joined, read;                          // smaller items: both results there; both read
     uint64_t s_full[kChains][2], s_free[kChains][2], p_full[kChains][2], p_free[kChains][2];
-    uint64_t turn[kChains][4];                      // a warp's turn at the exponentials
     int bad[2];                                     // the segment has a non-finite masked V row
     uint32_t tmem_base;
     Work work[kWorkCache];                          // the CTA's first segments
@@ -253,28 +254,6 @@ __device__ __forceinline__ float fmax3(float a, float b, float c) {
     float r;
     asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
     return r;
-}
-// Which of 16 pairs take the way below: the rest go to the exponential unit.
-constexpr uint32_t kPolyPairs = (1u << 2) | (1u << 5) | (1u << 7) | (1u << 10) | (1u << 13);
-// 2^x for a pair on the FMA and ALU pipes: x = n + f with n the nearest
-// integer (the 1.5 2^23 shifter), 2^f by a cubic on [-1/2, 1/2] (relative
-// error 7.5e-5, a fiftieth of the bf16 rounding of P), n added to the
-// exponent field.  x is clamped at -126, so a masked score gives 1e-38.
-__device__ __forceinline__ void ex2_poly2(float x0, float x1, float& r0, float& r1) {
-    const uint64_t x2 = f2(fmaxf(x0, -126.0f), fmaxf(x1, -126.0f));
-    const uint64_t sh = f2(12582912.0f, 12582912.0f);
-    const uint64_t t = fadd2(x2, sh);
-    const uint64_t n = fadd2(t, f2(-12582912.0f, -12582912.0f));
-    const uint64_t f = ffma2(n, f2(-1.0f, -1.0f), x2);
-    uint64_t p = ffma2(f2(0.0551716648f, 0.0551716648f), f, f2(0.2426111251f, 0.2426111251f));
-    p = ffma2(p, f, f2(0.6932609677f, 0.6932609677f));
-    p = ffma2(p, f, f2(0.9999280572f, 0.9999280572f));
-    float t0, t1, p0, p1;
-    f2_split(t, t0, t1);
-    f2_split(p, p0, p1);
-    const int kSh = __float_as_int(12582912.0f);
-    r0 = __int_as_float(__float_as_int(p0) + ((__float_as_int(t0) - kSh) << 23));
-    r1 = __int_as_float(__float_as_int(p1) + ((__float_as_int(t1) - kSh) << 23));
 }
 __device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
     uint32_t r;
@@ -534,8 +513,6 @@ __global__ void __launch_bounds__(CT_THREADS, 1)
         mbar_init(&S.joined, 4 * kChains);
         mbar_init(&S.read, 4 * kChains);
         for (int c = 0; c < kChains; ++c)
-            for (int q = 0; q < 4; ++q) mbar_init(&S.turn[c][q], 1);
-        for (int c = 0; c < kChains; ++c)
             for (int h = 0; h < 2; ++h) {
                 mbar_init(&S.s_full[c][h], 1);
                 mbar_init(&S.s_free[c][h], 4);
@@ -773,16 +750,7 @@ __global__ void __launch_bounds__(CT_THREADS, 1)
         const uint32_t tO = tL + col_o(c);
         int x = 0;        // own blocks so far (barrier phases)
         int n_joins = 0;  // segments of smaller items so far
-        int turns = 0;    // turns taken: chain 0 first, then alternately
-        auto take_turn = [&]() {
-            if (c == 1 || turns > 0)
-                wait_or_flag(&S.turn[c][warp & 3], (c == 1 ? turns : turns - 1) & 1, A.err, kErrWaitMma, failed);
-            ++turns;
-        };
-        auto pass_turn = [&]() {
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&S.turn[1 - c][warp & 3]);
-        };
+        bool s_ready = false;   // S of block x is there
         for (int sg = seg0; sg < seg1; ++sg) {
             const int k = sg - seg0;
             const Work w = work_of(sg);
@@ -792,10 +760,12 @@ __global__ void __launch_bounds__(CT_THREADS, 1)
             float l_run = 0.f;
             const int x0 = x;
             const int key0 = w.t0 * kTile, key_end = min(w.t1 * kTile, w.kv_len);
-            for (int key = key0 + (w.dual ? 0 : c * kKeys); key < key_end; key += w.dual ? kKeys : 2 * kKeys, ++x) {
+            // Block x from key on; EDGE: some of its keys are masked for some row.
+            auto block = [&]<bool EDGE>(int key) {
                 const int h = x % kBufs;
                 const uint32_t tS = tL + col_s(c, 0) + 64u * h, tP = tL + col_p(c, 0) + 32u * h;
-                wait_or_flag(&S.s_full[c][h], (x / kBufs) & 1, A.err, kErrWaitMma, failed);
+                if (!s_ready) wait_or_flag(&S.s_full[c][h], (x / kBufs) & 1, A.err, kErrWaitMma, failed);
+                __syncwarp();
                 tc_fence_after();
                 float s[kKeys];
 #pragma unroll
@@ -806,8 +776,8 @@ __global__ void __launch_bounds__(CT_THREADS, 1)
                     __syncwarp();
                     if (lane == 0) mbar_arrive(&S.s_free[c][h]);   // the MMA may overwrite S
                 }
-                const int left = my_pos - key;   // the block's last attended key
-                if (left < kKeys - 1) {
+                if constexpr (EDGE) {
+                    const int left = my_pos - key;   // the block's last attended key
 #pragma unroll
                     for (int e = 0; e < kKeys; ++e)
                         if (e > left) s[e] = -INFINITY;
@@ -824,39 +794,37 @@ __global__ void __launch_bounds__(CT_THREADS, 1)
                 if constexpr (kKeys == 128)
                     mt = fmax3(mt, fmax3(fmax3(mc[8], mc[9], mc[10]), mc[11], mc[12]), fmax3(mc[13], mc[14], mc[15]));
                 mt *= kExpScale;
-                float alpha = 1.f;
                 const bool move = m_ref == m_ref && !(mt <= m_ref + kMoveThreshold);   // to a NaN too, never from one
-                if (move) {
-                    alpha = (m_ref == -INFINITY) ? 0.f : exp2f(m_ref - mt);
-                    m_ref = mt;
-                }
+                const float alpha = move ? ex2_sfu(m_ref - mt) : 1.f;                  // 0 from -inf
+                m_ref = move ? mt : m_ref;
+                const bool any_move = __any_sync(0xffffffffu, move);
                 const float m_use = m_ref == -INFINITY ? 0.f : m_ref;   // nothing attended so far: weights 0
                 const uint64_t sc2 = f2(kExpScale, kExpScale), negm2 = f2(-m_use, -m_use);
+                // probed now, needed further down: the last PV, and the next block's S
+                const bool p_done = F32 || x == 0 || mbar_test_wait(&S.p_free[c][0], (x - 1) & 1);
+                s_ready = mbar_test_wait(&S.s_full[c][(x + 1) % kBufs], ((x + 1) / kBufs) & 1);
 #pragma unroll
                 for (int e = 0; e < kKeys / 2; ++e)
                     f2_split(ffma2(f2(s[2 * e], s[2 * e + 1]), sc2, negm2), s[2 * e], s[2 * e + 1]);
-                take_turn();
 #pragma unroll
-                for (int e = 0; e < kKeys / 2; ++e) {
-                    // bf16: some of the pairs on the FMA pipe, the rest on the SFU
-                    if (!F32 && ((kPolyPairs >> (e & 15)) & 1)) {
-                        ex2_poly2(s[2 * e], s[2 * e + 1], s[2 * e], s[2 * e + 1]);
-                    } else {
-                        s[2 * e] = ex2_sfu(s[2 * e]);
-                        s[2 * e + 1] = ex2_sfu(s[2 * e + 1]);
-                    }
-                }
-                pass_turn();
-                if (!F32 && left < kKeys - 1) {   // the cubic leaves 1e-38 at masked keys
+                for (int e = 0; e < kKeys; ++e) s[e] = ex2_sfu(s[e]);
+                uint64_t lsum2[4] = {f2(0.f, 0.f), f2(0.f, 0.f), f2(0.f, 0.f), f2(0.f, 0.f)};
 #pragma unroll
-                    for (int e = 0; e < kKeys; ++e)
-                        if (e > left) s[e] = 0.f;
+                for (int e = 0; e < kKeys / 2; ++e) lsum2[e & 3] = fadd2(lsum2[e & 3], f2(s[2 * e], s[2 * e + 1]));
+                float lsum0, lsum1;
+                f2_split(fadd2(fadd2(lsum2[0], lsum2[1]), fadd2(lsum2[2], lsum2[3])), lsum0, lsum1);
+                l_run = l_run * alpha + (lsum0 + lsum1);
+                [[maybe_unused]] uint32_t pk[kKeys / 2];
+                if constexpr (!F32) {
+#pragma unroll
+                    for (int e = 0; e < kKeys / 2; ++e) pk[e] = pack_bf16(s[2 * e], s[2 * e + 1]);
                 }
                 // P and O may be touched once the last PV is done (fp32: P lies where only
                 // an earlier PV could be reading, and S was issued after that)
-                if (x > 0 && !F32) wait_or_flag(&S.p_free[c][0], (x - 1) & 1, A.err, kErrWaitMma, failed);
-                if (x > x0 && __any_sync(0xffffffffu, move)) {
-                    if (F32) wait_or_flag(&S.p_free[c][(x - 1) % kBufs], ((x - 1) / kBufs) & 1, A.err, kErrWaitMma, failed);
+                if (!p_done) wait_or_flag(&S.p_free[c][0], (x - 1) & 1, A.err, kErrWaitMma, failed);
+                __syncwarp();
+                if (any_move && x > x0) {
+                    if (F32) wait_uniform(&S.p_free[c][(x - 1) % kBufs], ((x - 1) / kBufs) & 1, A.err, kErrWaitMma, failed);
                     tc_fence_after();
 #pragma unroll
                     for (int q = 0; q < HD / 16; ++q) {
@@ -869,35 +837,36 @@ __global__ void __launch_bounds__(CT_THREADS, 1)
                         tmem_st16(tO + 16 * q, ob);
                     }
                 }
-                uint64_t lsum2[4] = {f2(0.f, 0.f), f2(0.f, 0.f), f2(0.f, 0.f), f2(0.f, 0.f)};
+                if constexpr (!F32) {
+                    tc_fence_after();
+                    tmem_st32(tP, *reinterpret_cast<const uint32_t(*)[32]>(&pk[0]));
+                    tmem_st32(tP + 32, *reinterpret_cast<const uint32_t(*)[32]>(&pk[32]));
+                } else {
 #pragma unroll
-                for (int e = 0; e < kKeys / 2; ++e) lsum2[e & 3] = fadd2(lsum2[e & 3], f2(s[2 * e], s[2 * e + 1]));
+                    for (int q = 0; q < kKeys / 32; ++q) {   // 32 keys: 16 columns of each term
 #pragma unroll
-                for (int q = 0; q < kKeys / 32; ++q) {   // 32 keys: 16 columns of each term
-                    uint32_t pk[16];
+                        for (int term = 0; term < kTerms; ++term) {
+                            uint32_t t[16];
 #pragma unroll
-                    for (int term = 0; term < kTerms; ++term) {
-#pragma unroll
-                        for (int e = 0; e < 16; ++e) {
-                            float& x0 = s[32 * q + 2 * e];
-                            float& x1 = s[32 * q + 2 * e + 1];
-                            pk[e] = F32 ? top_pair(x0, x1) : pack_bf16(x0, x1);
-                            if (F32 && term + 1 < kTerms) f2_split(rest_pair(x0, x1), x0, x1);
+                            for (int e = 0; e < 16; ++e) {
+                                float& x0 = s[32 * q + 2 * e];
+                                float& x1 = s[32 * q + 2 * e + 1];
+                                t[e] = top_pair(x0, x1);
+                                if (term + 1 < kTerms) f2_split(rest_pair(x0, x1), x0, x1);
+                            }
+                            tmem_st16((term == kTerms - 1 ? tP : tS + 32 * term) + 16 * q, t);
                         }
-                        tmem_st16((term == kTerms - 1 ? tP : tS + 32 * term) + 16 * q, pk);
                     }
                 }
-                float lsum0, lsum1;
-                f2_split(fadd2(fadd2(lsum2[0], lsum2[1]), fadd2(lsum2[2], lsum2[3])), lsum0, lsum1);
-                l_run = l_run * alpha + (lsum0 + lsum1);
                 tmem_wait_st();
                 tc_fence_before();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&S.p_full[c][h]);
-            }
-            if (c == 1 && !w.dual && ((key_end - key0 + kKeys - 1) / kKeys) % 2 == 1) {   // chain 0 had a block more
-                take_turn();
-                pass_turn();
+                ++x;
+            };
+            for (int key = key0 + (w.dual ? 0 : c * kKeys); key < key_end; key += w.dual ? kKeys : 2 * kKeys) {
+                if (key + kKeys - 1 > w.pos_min) block.template operator()<true>(key);
+                else block.template operator()<false>(key);
             }
             // ---- the segment's result ----
             for (int y = max(x0, x - kBufs); y < x; ++y)
