@@ -140,7 +140,6 @@ __global__ void __launch_bounds__(kAppendThreads) append_kernel(const __grid_con
 // (chunk_row_exact), which reads nothing but the attended rows.
 constexpr int CT_THREADS = 512;
 constexpr int kChains = 2;
-constexpr int CT_STAGES = 4;
 constexpr int kTile = kChunkTile;            // 128
 constexpr int kBox = 64;                     // rows per TMA box: the smallest bf16 page
 constexpr int kTileHalfs = kTile * HD;       // elements of a K or V tile (16 KB)
@@ -189,14 +188,16 @@ constexpr int kWorkCache = 20;
 
 template <bool F32>
 struct ChunkSmem {
+    static constexpr int kStages = F32 ? 3 : 4;     // K/V tiles
     static constexpr int kTerms = F32 ? 3 : 1;      // bf16 terms of q and P
     static constexpr int kQBufs = F32 ? 1 : 2;      // Q buffers (segments in flight)
     uint16_t q[kQBufs][2][kTerms][kTileHalfs];      // 16 KB each, SW128 K-major
-    uint16_t k[CT_STAGES][kTileHalfs];
-    uint16_t v[CT_STAGES][kTileHalfs];
-    uint64_t kv_full[CT_STAGES];
-    uint64_t kv_empty[CT_STAGES];                   // the PV issuers and the edge warp
-    uint64_t v_ok[CT_STAGES];                       // edge tiles: V checked
+    uint16_t k[kStages][kTileHalfs];
+    uint16_t v[kStages][kTileHalfs];
+    uint4 stage[8][256];                            // a softmax warp's results on their way out
+    uint64_t kv_full[kStages];
+    uint64_t kv_empty[kStages];                   // the PV issuers and the edge warp
+    uint64_t v_ok[kStages];                       // edge tiles: V checked
     uint64_t q_full[2], q_free[2];
     uint64_t scanned[2];                            // the segment's edge tiles are checked
     uint64_t seg_end[2];                            // the softmax is done with the segment
@@ -330,6 +331,17 @@ __device__ __forceinline__ void wait_uniform(uint64_t* bar, uint32_t parity, uin
 
 struct ChunkTma {
     CUtensorMap k, v;   // the layer's pools as [pool rows][n_head_kv * 64] bf16, box {64, 64}
+};
+
+// A row of a (chunk, KV head) as token and head of the group, moved on without
+// a division per step.
+struct RowWalk {
+    int64_t t;
+    int h;
+    __device__ __forceinline__ RowWalk(int row, int group) : t(row / group), h(row - row / group * group) {}
+    __device__ __forceinline__ void step(int rows, int group) {
+        for (h += rows; h >= group; h -= group) ++t;
+    }
 };
 
 // Where a row's result goes: 64 values in the type of q, or a partial row.
@@ -491,7 +503,7 @@ __global__ void __launch_bounds__(CT_THREADS, 1)
     chunk_attn_kernel(const __grid_constant__ ChunkArgs A, const __grid_constant__ ChunkTma M) {
     using Smem = ChunkSmem<F32>;
     using Act = std::conditional_t<F32, float, __nv_bfloat16>;
-    constexpr int kTerms = Smem::kTerms, kQBufs = Smem::kQBufs, kKeys = kKeysOf<F32>, kBufs = kBufsOf<F32>;
+    constexpr int CT_STAGES = Smem::kStages, kTerms = Smem::kTerms, kQBufs = Smem::kQBufs, kKeys = kKeysOf<F32>, kBufs = kBufsOf<F32>;
     constexpr int kBlocks = kTile / kKeys;   // of a tile
     constexpr uint32_t kIdS = idesc_bf16_f32(kChunkRows, kKeys);
     extern __shared__ __align__(1024) unsigned char smem_raw[];
@@ -688,23 +700,20 @@ __global__ void __launch_bounds__(CT_THREADS, 1)
             // 8 lanes per row, 4 rows per step, half of each row tile per warp
             const int ch = lane & 7;
             for (int m = 0; m < (w.dual ? 2 : 1); ++m) {
-                auto source = [&](int r, bool& ok) {
-                    const int row = w.row0 + m * kChunkRows + r, t = row / A.group, h = row - t * A.group;
-                    ok = m * kChunkRows + r < w.n_rows;
-                    return ok ? static_cast<const Act*>(A.q) + static_cast<int64_t>(w.first + t) * A.q_stride +
-                                    (w.kvh * A.group + h) * HD + ch * 8
-                              : static_cast<const Act*>(A.q);
-                };
+                const int r0 = lw * 64 + (lane >> 3);   // row of the tile
+                RowWalk at(w.row0 + m * kChunkRows + r0, A.group);
+                const Act* base = static_cast<const Act*>(A.q) + static_cast<int64_t>(w.first) * A.q_stride +
+                                  w.kvh * A.group * HD + ch * 8;
                 if constexpr (!F32) {
 #pragma unroll 4
                     for (int j = 0; j < 16; ++j) {
-                        const int r = lw * 64 + 4 * j + (lane >> 3);
-                        bool ok;
-                        const Act* src = source(r, ok);
+                        const int r = r0 + 4 * j;
+                        const bool ok = m * kChunkRows + r < w.n_rows;
                         asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(
                                          smem_u32(&S.q[b][m][0][r * HD + ((ch ^ (r & 7)) << 3)])),
-                                     "l"(src), "r"(ok ? 16 : 0)
+                                     "l"(ok ? base + at.t * A.q_stride + at.h * HD : base), "r"(ok ? 16 : 0)
                                      : "memory");
+                        at.step(4, A.group);
                     }
                 } else {
 #pragma unroll 1
@@ -712,17 +721,17 @@ __global__ void __launch_bounds__(CT_THREADS, 1)
                         float4 x[4][2];
 #pragma unroll
                         for (int j = 0; j < 4; ++j) {
-                            bool ok;
-                            const float4* src = reinterpret_cast<const float4*>(source(lw * 64 + 4 * (j0 + j) + (lane >> 3), ok));
+                            const float4* src = reinterpret_cast<const float4*>(base + at.t * A.q_stride + at.h * HD);
                             x[j][0] = x[j][1] = make_float4(0.f, 0.f, 0.f, 0.f);
-                            if (ok) {
+                            if (m * kChunkRows + r0 + 4 * (j0 + j) < w.n_rows) {
                                 x[j][0] = src[0];
                                 x[j][1] = src[1];
                             }
+                            at.step(4, A.group);
                         }
 #pragma unroll
                         for (int j = 0; j < 4; ++j) {
-                            const int r = lw * 64 + 4 * (j0 + j) + (lane >> 3);
+                            const int r = r0 + 4 * (j0 + j);
                             float* f = reinterpret_cast<float*>(x[j]);
 #pragma unroll
                             for (int term = 0; term < kTerms; ++term) {
@@ -874,41 +883,82 @@ __global__ void __launch_bounds__(CT_THREADS, 1)
             wait_or_flag(&S.scanned[k & 1], (k >> 1) & 1, A.err, kErrWaitMma, failed);
             tc_fence_after();
             const bool mine = r < w.n_rows;
-            const RowOut<Act> dst = row_out<Act>(A, w, mine ? r : 0);
-            // columns [col0, col1) of the row from up to two chains with weights f0, f1
-            // (a chain without weight may hold anything)
-            auto put = [&](int col0, int col1, uint32_t t0, float f0, uint32_t t1, float f1, bool two) {
-                for (int col = col0; col < col1; col += 16) {
-                    float o[16];
-                    tmem_ld16(t0 + col, o);
+            // COLS columns from col0 on of every row of the warp, from one chain or two with
+            // weights f0, f1 (a chain without weight may hold anything).  Through shared
+            // memory, 16-byte chunk j of row r at j ^ (r & 7), so that the lanes of a store
+            // write whole rows.
+            uint4* stage = S.stage[4 * c + (warp & 3)];
+            const int row_base = (w.dual ? kChunkRows * c : 0) + 32 * (warp & 3);   // the warp's rows in the item
+            auto fetch = [&](float (&o)[32], int col, uint32_t t0, float f0, uint32_t t1, float f1, bool two) {
+                tmem_ld32(t0 + col, o);
+                tmem_wait_ld();
+#pragma unroll
+                for (int e = 0; e < 32; ++e) o[e] = f0 != 0.f ? o[e] * f0 : 0.f;
+                if (two) {
+                    float y[32];
+                    tmem_ld32(t1 + col, y);
                     tmem_wait_ld();
 #pragma unroll
-                    for (int e = 0; e < 16; ++e) o[e] = f0 != 0.f ? o[e] * f0 : 0.f;
-                    if (two) {
-                        float y[16];
-                        tmem_ld16(t1 + col, y);
-                        tmem_wait_ld();
-#pragma unroll
-                        for (int e = 0; e < 16; ++e) o[e] = f1 != 0.f ? fmaf(f1, y[e], o[e]) : o[e];
-                    }
-                    if (mine) {
-#pragma unroll
-                        for (int e = 0; e < 16; e += 8) {
-                            if (dst.out) store8(dst.out + col + e, o + e);
-                            else store8(dst.part + col + e, o + e);
-                        }
-                    }
+                    for (int e = 0; e < 32; ++e) o[e] = f1 != 0.f ? fmaf(f1, y[e], o[e]) : o[e];
                 }
             };
+            // the staged rows, CHUNKS chunks each, to their places; dst(at) is a row's first byte
+            auto flush = [&]<int CHUNKS>(auto&& dst) {
+                constexpr int kRowsPerStep = 32 / CHUNKS;
+                __syncwarp();
+                const int ch = lane % CHUNKS;
+                int rr = lane / CHUNKS;
+                RowWalk at(w.row0 + row_base + rr, A.group);
+#pragma unroll
+                for (int q = 0; q < CHUNKS; ++q, rr += kRowsPerStep) {
+                    if (row_base + rr < w.n_rows)
+                        reinterpret_cast<uint4*>(dst(at, row_base + rr))[ch] = stage[rr * CHUNKS + (ch ^ (rr & (CHUNKS - 1)))];
+                    at.step(kRowsPerStep, A.group);
+                }
+                __syncwarp();
+            };
+            auto put = [&]<int COLS>(int col0, uint32_t t0, float f0, uint32_t t1, float f1, bool two) {
+                auto out_row = [&](const RowWalk& at, int) {
+                    return static_cast<Act*>(A.out) + (w.first + at.t) * A.out_stride + (w.kvh * A.group + at.h) * HD;
+                };
+                auto part_row = [&](const RowWalk&, int ri) { return A.part_o + (static_cast<size_t>(w.part) + ri) * HD; };
+                if (F32 || w.part >= 0) {
+                    for (int col = col0; col < col0 + COLS; col += 32) {
+                        float o[32];
+                        fetch(o, col, t0, f0, t1, f1, two);
+#pragma unroll
+                        for (int j = 0; j < 8; ++j)
+                            stage[lane * 8 + (j ^ (lane & 7))] =
+                                make_uint4(__float_as_uint(o[4 * j]), __float_as_uint(o[4 * j + 1]),
+                                           __float_as_uint(o[4 * j + 2]), __float_as_uint(o[4 * j + 3]));
+                        if (w.part >= 0) flush.template operator()<8>([&](const RowWalk& at, int ri) { return part_row(at, ri) + col; });
+                        else flush.template operator()<8>([&](const RowWalk& at, int ri) { return out_row(at, ri) + col; });
+                    }
+                } else {
+                    constexpr int kChunks = COLS / 8;
+#pragma unroll
+                    for (int p = 0; p < COLS / 32; ++p) {
+                        float o[32];
+                        fetch(o, col0 + 32 * p, t0, f0, t1, f1, two);
+#pragma unroll
+                        for (int j = 0; j < 4; ++j)
+                            stage[lane * kChunks + ((4 * p + j) ^ (lane & (kChunks - 1)))] =
+                                make_uint4(pack_bf16(o[8 * j], o[8 * j + 1]), pack_bf16(o[8 * j + 2], o[8 * j + 3]),
+                                           pack_bf16(o[8 * j + 4], o[8 * j + 5]), pack_bf16(o[8 * j + 6], o[8 * j + 7]));
+                    }
+                    flush.template operator()<kChunks>([&](const RowWalk& at, int ri) { return out_row(at, ri) + col0; });
+                }
+            };
+            float* lse = mine && w.part >= 0 ? A.part_lse + w.part + r : nullptr;
             if (w.dual) {
                 if (S.bad[k & 1]) {
                     const Work cold = w;   // a copy, so that w itself stays in registers
-                    if (mine) chunk_row_exact<Act>(A, cold, r, dst);
+                    if (mine) chunk_row_exact<Act>(A, cold, r, row_out<Act>(A, cold, r));
                     __syncwarp();
                 } else {
                     const bool empty = m_ref == -INFINITY;
-                    put(0, HD, tO, empty ? 0.f : 1.0f / l_run, 0u, 0.f, false);
-                    if (mine && dst.lse) *dst.lse = empty ? -INFINITY : m_ref + log2f(l_run);
+                    put.template operator()<HD>(0, tO, empty ? 0.f : 1.0f / l_run, 0u, 0.f, false);
+                    if (lse) *lse = empty ? -INFINITY : m_ref + log2f(l_run);
                 }
                 tc_fence_before();
             } else {
@@ -921,7 +971,7 @@ __global__ void __launch_bounds__(CT_THREADS, 1)
                 tc_fence_after();
                 if (S.bad[k & 1]) {
                     const Work cold = w;
-                    if (mine && c == 0) chunk_row_exact<Act>(A, cold, r, dst);
+                    if (mine && c == 0) chunk_row_exact<Act>(A, cold, r, row_out<Act>(A, cold, r));
                     __syncwarp();
                 } else {
                     float m0, l0, m1, l1;
@@ -933,8 +983,8 @@ __global__ void __launch_bounds__(CT_THREADS, 1)
                     const float l_all = (w0 != 0.f ? w0 * l0 : 0.f) + (w1 != 0.f ? w1 * l1 : 0.f);
                     const bool empty = l_all == 0.f;
                     const float inv = empty ? 0.f : 1.0f / l_all;
-                    put(32 * c, 32 * c + 32, tL + col_o(0), w0 * inv, tL + col_o(1), w1 * inv, true);
-                    if (mine && dst.lse && c == 0) *dst.lse = empty ? -INFINITY : m_all + log2f(l_all);
+                    put.template operator()<HD / 2>(32 * c, tL + col_o(0), w0 * inv, tL + col_o(1), w1 * inv, true);
+                    if (lse && c == 0) *lse = empty ? -INFINITY : m_all + log2f(l_all);
                 }
                 // both have read before either's O or P columns are written again
                 tc_fence_before();
@@ -1232,22 +1282,31 @@ __global__ void __launch_bounds__(kMergeThreads) chunk_merge_kernel(const __grid
     if (r >= m.n_rows) return;
     const float* lse = A.part_lse + m.part + r;
     const float* po = A.part_o + (static_cast<size_t>(m.part) + r) * HD + 2 * lane;
-    float mx = -INFINITY;
-    for (int b = lane; b < m.n_parts; b += 32) mx = fmaxf(mx, lse[static_cast<size_t>(b) * m.n_rows]);
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+    // four blocks at a time, all of their loads in flight
     float2 acc = make_float2(0.f, 0.f);
-    float sum = 0.f;
-    for (int b0 = 0; b0 < m.n_parts; b0 += 32) {
-        const int nb = min(32, m.n_parts - b0);
-        float w = lane < nb ? exp2f(lse[static_cast<size_t>(b0 + lane) * m.n_rows] - mx) : 0.f;
-#pragma unroll 8
-        for (int b = 0; b < nb; ++b) {
-            const float wb = __shfl_sync(0xffffffffu, w, b);
-            const float2 x = *reinterpret_cast<const float2*>(po + static_cast<size_t>(b0 + b) * m.n_rows * HD);
-            sum += wb;
-            acc.x = fmaf(wb, x.x, acc.x);
-            acc.y = fmaf(wb, x.y, acc.y);
+    float mx = -INFINITY, sum = 0.f;
+    for (int b0 = 0; b0 < m.n_parts; b0 += 4) {
+        float l[4];
+        float2 x[4];
+#pragma unroll
+        for (int b = 0; b < 4; ++b) {
+            const bool in = b0 + b < m.n_parts;
+            const size_t at = static_cast<size_t>(in ? b0 + b : b0) * m.n_rows;
+            l[b] = in ? lse[at] : -INFINITY;
+            x[b] = *reinterpret_cast<const float2*>(po + at * HD);
+        }
+        const float top = fmaxf(fmaxf(fmaxf(l[0], l[1]), fmaxf(l[2], l[3])), mx);
+        const float keep = mx == -INFINITY ? 0.f : exp2f(mx - top);
+        sum *= keep;
+        acc.x *= keep;
+        acc.y *= keep;
+        mx = top;
+#pragma unroll
+        for (int b = 0; b < 4; ++b) {
+            const float w = l[b] == -INFINITY ? 0.f : exp2f(l[b] - mx);
+            sum += w;
+            acc.x = fmaf(w, x[b].x, acc.x);
+            acc.y = fmaf(w, x[b].y, acc.y);
         }
     }
     const ChunkSeq sq = A.d.seqs[m.seq];
