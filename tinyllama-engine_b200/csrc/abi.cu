@@ -3,10 +3,13 @@
 // every entry point returns a TLE_* status and records a message for
 // tle_last_error().
 #include <algorithm>
+#include <functional>
+#include <utility>
 #include <cmath>
 #include <cstdarg>
 #include <cstdio>
 #include <cstring>
+#include <exception>
 #include <mutex>
 #include <numeric>
 #include <string>
@@ -1442,11 +1445,13 @@ int check_chunks(const tle_shape_t* shape, int page_rows, const tle_paged_chunk_
 }
 
 // The attention's work plan, made apart for the items of either kernel: those
-// of at most kChunkFewRows rows, and the others.  Costs in units: a K/V tile
+// of chunks of at most kChunkFewRows rows, and the others.  Costs in units: a K/V tile
 // costs 1 for the few rows; 2 for an item of more than kChunkRows rows (both
 // chains do the whole tile) and 1 for one in between (each does half of it).
 // A segment has a fixed cost (Q load, joining and storing the result).
 constexpr int64_t kSegUnits = 4, kFewSegUnits = 2;
+constexpr int64_t kJoinUnits = 8;             // partial results of cut items, and the launch that joins them
+constexpr int64_t kMaxWholeItems = 4096;    // sorted on the host, a few tenths of a millisecond
 constexpr int64_t kMinPieceUnits = 4, kFewMinPieceUnits = 2;   // smallest piece of an item worth a CTA of its own
 
 struct ChunkPlanner {
@@ -1457,7 +1462,6 @@ struct ChunkPlanner {
 
     struct Item {
         int seq, kvh, row0, n_rows, tiles;
-        bool few() const { return n_rows <= tle::kChunkFewRows; }
         int unit() const { return n_rows > tle::kChunkRows ? 2 : 1; }   // cost of a tile
         int64_t cost() const { return static_cast<int64_t>(tiles) * unit(); }
     };
@@ -1471,9 +1475,36 @@ struct ChunkPlanner {
                 for (int r = 0; r < rows; r += tle::kChunkItemRows) {
                     Item it{s, h, r, std::min(tle::kChunkItemRows, rows - r), 0};
                     it.tiles = (chunks[s].pos + (r + it.n_rows - 1) / g) / tle::kChunkTile + 1;
-                    if (it.few() == few) f(it);
+                    if ((rows <= tle::kChunkFewRows) == few) f(it);
                 }
             }
+    }
+
+    // Whole items, longest first (see run); false if they do not balance.
+    template <class S>
+    bool whole(bool few, int64_t n_items, int64_t total, int64_t seg_units, S&& seg) const {
+        std::vector<Item> items;
+        items.reserve(static_cast<size_t>(n_items));
+        each_item(few, [&](const Item& it) { items.push_back(it); });
+        std::stable_sort(items.begin(), items.end(), [](const Item& a, const Item& b) { return a.cost() > b.cost(); });
+        const int G = max_ctas;
+        std::vector<std::pair<int64_t, int>> heap;   // (cost so far, CTA), the least on top
+        for (int c = 0; c < G; ++c) heap.emplace_back(0, c);
+        std::vector<std::pair<int, int>> owner;      // (CTA, item)
+        owner.reserve(items.size());
+        int64_t most = 0;
+        for (size_t i = 0; i < items.size(); ++i) {
+            std::pop_heap(heap.begin(), heap.end(), std::greater<>());
+            auto& h = heap.back();
+            owner.emplace_back(h.second, static_cast<int>(i));
+            h.first += items[i].cost() + seg_units;
+            most = std::max(most, h.first);
+            std::push_heap(heap.begin(), heap.end(), std::greater<>());
+        }
+        if (most > total / G + kJoinUnits) return false;
+        std::sort(owner.begin(), owner.end());
+        for (const auto& o : owner) seg(o.first, items[o.second], 0, items[o.second].tiles, 1, 0);
+        return true;
     }
 
     // Calls seg(cta, item, t0, t1, parts of the item, parts before) and
@@ -1488,6 +1519,10 @@ struct ChunkPlanner {
         });
         if (n_items == 0) return 0;
         const int G = max_ctas;
+        // Many items of different cost, few enough to sort: whole items, the longest
+        // first to the CTA with the least so far, unless that leaves a CTA with more
+        // than cutting them (below) and joining the pieces would cost.
+        if (n_items > G / 2 && n_items <= kMaxWholeItems && whole(few, n_items, units + n_items * seg_units, seg_units, seg)) return G;
         // Few items: every item in equal pieces, one piece per CTA, the smallest
         // piece for which the CTAs suffice -- unless cutting the items' concatenated
         // costs evenly (below) leaves less for the longest CTA.
@@ -1639,7 +1674,7 @@ int append_common(const tle_shape_t* shape, const tle_chunk_plan_t* plan, const 
 
 extern "C" {
 
-size_t tle_chunk_desc_bytes(const tle_shape_t* shape, const tle_paged_chunk_t* chunks, int n_seqs, int max_ctas) {
+size_t tle_chunk_desc_bytes(const tle_shape_t* shape, const tle_paged_chunk_t* chunks, int n_seqs, int max_ctas) try {
     if (check_chunks(shape, 0, chunks, n_seqs)) return 0;
     const ChunkPlanner p{shape, chunks, n_seqs, chunk_ctas(max_ctas)};
     size_t segs = 0, merges = 0, tokens = 0, ctas[2];
@@ -1648,10 +1683,13 @@ size_t tle_chunk_desc_bytes(const tle_shape_t* shape, const tle_paged_chunk_t* c
                           [&](const ChunkPlanner::Item&, int) { ++merges; });
     for (int s = 0; s < n_seqs; ++s) tokens += static_cast<size_t>(chunks[s].n_tokens);
     return tle::chunk_desc_bytes(n_seqs, segs, merges, tokens, ctas[0], ctas[1]);
+} catch (const std::exception& e) {   // the planner's lists: out of host memory
+    set_error(TLE_ERR_INVALID, "chunk plan: %s", e.what());
+    return 0;
 }
 
 int tle_chunk_desc_paged(const tle_shape_t* shape, int page_rows, const tle_paged_chunk_t* chunks, int n_seqs,
-                         int max_ctas, void* desc_host, size_t desc_bytes, tle_chunk_plan_t* plan) {
+                         int max_ctas, void* desc_host, size_t desc_bytes, tle_chunk_plan_t* plan) try {
     if (!desc_host || !plan) return set_error(TLE_ERR_INVALID, "desc_host and plan must be non-null");
     if (page_rows < 16 || page_rows > 65536 || (page_rows & (page_rows - 1)) != 0)
         return set_error(TLE_ERR_INVALID, "page_rows %d is not a power of two in [16, 65536]", page_rows);
@@ -1720,6 +1758,8 @@ int tle_chunk_desc_paged(const tle_shape_t* shape, int page_rows, const tle_page
     }
     *plan = out;
     return ok();
+} catch (const std::exception& e) {
+    return set_error(TLE_ERR_INVALID, "chunk plan: %s", e.what());
 }
 
 int tle_append_paged(const tle_shape_t* shape, const tle_page_pool_t* pool, const tle_chunk_plan_t* plan,
@@ -1778,6 +1818,13 @@ int tle_prefill_bf16_paged(const tle_shape_t* shape, const tle_page_pool_bf16_t*
     a.n_head = shape->n_head;
     a.n_head_kv = shape->n_head_kv;
     a.group = shape->n_head / shape->n_head_kv;
+    if (a.group > 1) {
+        int bits = 1;
+        while ((1 << bits) < a.group) ++bits;
+        const uint64_t one = 1ull << (31 + bits);
+        a.group_mul = static_cast<uint32_t>((one + a.group - 1) / a.group);
+        a.group_shift = static_cast<uint32_t>(bits - 1);
+    }
     a.part_o = static_cast<float*>(workspace);
     a.part_lse = need ? a.part_o + static_cast<size_t>(plan->part_rows) * tle::kHeadDim : nullptr;
     cudaError_t e = tle::error_word(&a.err);

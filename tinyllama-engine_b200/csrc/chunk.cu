@@ -155,6 +155,12 @@ constexpr float kExpScale = kScale * kLog2e;
 // 8 (log2 units), so O is rescaled rarely; P <= 2^8.
 constexpr float kMoveThreshold = 8.0f;
 
+// The token of row `row` of a (chunk, KV head): row / group by a multiplication
+// (group_mul = ceil(2^(31 + L) / group) with L = ceil(log2 group), exact for rows
+// below 2^31; 0 for a group of one).
+__device__ __forceinline__ int row_token(const ChunkArgs& A, int row) {
+    return A.group_mul ? static_cast<int>(__umulhi(static_cast<uint32_t>(row), A.group_mul) >> A.group_shift) : row;
+}
 // A segment as the kernel's roles see it.
 struct Work {
     const int32_t* pages;
@@ -177,9 +183,8 @@ __device__ __forceinline__ Work work_at(const ChunkArgs& A, int i) {
     w.part = sg.part;
     w.pos = sq.pos;
     w.first = sq.first;
-    const int g = A.group;
-    w.pos_min = sq.pos + sg.row0 / g;
-    w.kv_len = sq.pos + (sg.row0 + sg.n_rows - 1) / g + 1;
+    w.pos_min = sq.pos + row_token(A, sg.row0);
+    w.kv_len = sq.pos + row_token(A, sg.row0 + sg.n_rows - 1) + 1;
     w.dual = sg.n_rows > kChunkRows;
     return w;
 }
@@ -333,14 +338,23 @@ struct ChunkTma {
     CUtensorMap k, v;   // the layer's pools as [pool rows][n_head_kv * 64] bf16, box {64, 64}
 };
 
-// A row of a (chunk, KV head) as token and head of the group, moved on without
-// a division per step.
+// Element pointer of a row's head in an array of token rows, moved on from row
+// to row without a division: `p` at token t0, head h0 of the group.
+template <class T>
 struct RowWalk {
-    int64_t t;
+    T* p;
     int h;
-    __device__ __forceinline__ RowWalk(int row, int group) : t(row / group), h(row - row / group * group) {}
-    __device__ __forceinline__ void step(int rows, int group) {
-        for (h += rows; h >= group; h -= group) ++t;
+    int64_t wrap;   // from behind a token's last head of the group to the next one's first
+    __device__ __forceinline__ RowWalk(const ChunkArgs& A, T* base, int64_t stride, int first, int kvh, int row) {
+        const int t = row_token(A, row);
+        h = row - t * A.group;
+        p = base + static_cast<int64_t>(first + t) * stride + (kvh * A.group + h) * HD;
+        wrap = stride - A.group * HD;
+    }
+    template <int ROWS>
+    __device__ __forceinline__ void step(const ChunkArgs& A) {
+        p += ROWS * HD;
+        for (h += ROWS; h >= A.group; h -= A.group) p += wrap;
     }
 };
 
@@ -356,7 +370,7 @@ template <class Act>
 __device__ __forceinline__ RowOut<Act> row_out(const ChunkArgs& A, const Work& w, int r) {
     RowOut<Act> o{};
     if (w.part < 0) {
-        const int row = w.row0 + r, t = row / A.group, h = row - t * A.group;
+        const int row = w.row0 + r, t = row_token(A, row), h = row - t * A.group;
         o.out = static_cast<Act*>(A.out) + static_cast<int64_t>(w.first + t) * A.out_stride +
                 (w.kvh * A.group + h) * HD;
     } else {
@@ -394,7 +408,7 @@ __device__ __forceinline__ bool not_finite(const uint4 x) {
 // when a masked row of V is not finite (see above).
 template <class Act>
 __device__ __noinline__ void chunk_row_exact(const ChunkArgs& A, const Work& w, int r, RowOut<Act> dst) {
-    const int row = w.row0 + r, tok = row / A.group, h = w.kvh * A.group + row - tok * A.group;
+    const int row = w.row0 + r, tok = row_token(A, row), h = w.kvh * A.group + row - tok * A.group;
     const int pos = w.pos + tok;
     const Act* qp = static_cast<const Act*>(A.q) + static_cast<int64_t>(w.first + tok) * A.q_stride + h * HD;
     float q[HD], o[HD];
@@ -701,19 +715,20 @@ __global__ void __launch_bounds__(CT_THREADS, 1)
             const int ch = lane & 7;
             for (int m = 0; m < (w.dual ? 2 : 1); ++m) {
                 const int r0 = lw * 64 + (lane >> 3);   // row of the tile
-                RowWalk at(w.row0 + m * kChunkRows + r0, A.group);
-                const Act* base = static_cast<const Act*>(A.q) + static_cast<int64_t>(w.first) * A.q_stride +
-                                  w.kvh * A.group * HD + ch * 8;
+                RowWalk<const Act> at(A, static_cast<const Act*>(A.q) + ch * 8, A.q_stride, w.first, w.kvh,
+                                      w.row0 + m * kChunkRows + r0);
+                const int left = w.n_rows - m * kChunkRows - r0;   // steps of 4 rows while below
+                // rows r0 and r0 + 4 and their chunk's place; further rows keep one of the two
+                const int off[2] = {r0 * HD + ((ch ^ (r0 & 7)) << 3), (r0 + 4) * HD + ((ch ^ ((r0 + 4) & 7)) << 3)};
                 if constexpr (!F32) {
 #pragma unroll 4
                     for (int j = 0; j < 16; ++j) {
-                        const int r = r0 + 4 * j;
-                        const bool ok = m * kChunkRows + r < w.n_rows;
+                        const bool ok = 4 * j < left;
                         asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(
-                                         smem_u32(&S.q[b][m][0][r * HD + ((ch ^ (r & 7)) << 3)])),
-                                     "l"(ok ? base + at.t * A.q_stride + at.h * HD : base), "r"(ok ? 16 : 0)
+                                         smem_u32(&S.q[b][m][0][off[j & 1] + (j >> 1) * 8 * HD])),
+                                     "l"(ok ? at.p : static_cast<const Act*>(A.q)), "r"(ok ? 16 : 0)
                                      : "memory");
-                        at.step(4, A.group);
+                        at.template step<4>(A);
                     }
                 } else {
 #pragma unroll 1
@@ -721,21 +736,21 @@ __global__ void __launch_bounds__(CT_THREADS, 1)
                         float4 x[4][2];
 #pragma unroll
                         for (int j = 0; j < 4; ++j) {
-                            const float4* src = reinterpret_cast<const float4*>(base + at.t * A.q_stride + at.h * HD);
+                            const float4* src = reinterpret_cast<const float4*>(at.p);
                             x[j][0] = x[j][1] = make_float4(0.f, 0.f, 0.f, 0.f);
-                            if (m * kChunkRows + r0 + 4 * (j0 + j) < w.n_rows) {
+                            if (4 * (j0 + j) < left) {
                                 x[j][0] = src[0];
                                 x[j][1] = src[1];
                             }
-                            at.step(4, A.group);
+                            at.template step<4>(A);
                         }
 #pragma unroll
                         for (int j = 0; j < 4; ++j) {
-                            const int r = r0 + 4 * (j0 + j);
+                            const int at_q = off[j & 1] + ((j0 + j) >> 1) * 8 * HD;
                             float* f = reinterpret_cast<float*>(x[j]);
 #pragma unroll
                             for (int term = 0; term < kTerms; ++term) {
-                                *reinterpret_cast<uint4*>(&S.q[b][m][term][r * HD + ((ch ^ (r & 7)) << 3)]) =
+                                *reinterpret_cast<uint4*>(&S.q[b][m][term][at_q]) =
                                     make_uint4(top_pair(f[0], f[1]), top_pair(f[2], f[3]), top_pair(f[4], f[5]),
                                                top_pair(f[6], f[7]));
 #pragma unroll
@@ -764,7 +779,7 @@ __global__ void __launch_bounds__(CT_THREADS, 1)
             const int k = sg - seg0;
             const Work w = work_of(sg);
             const int r = w.dual ? kChunkRows * c + lr : lr;   // row of the item
-            const int my_pos = w.pos + (w.row0 + min(r, w.n_rows - 1)) / A.group;
+            const int my_pos = w.pos + row_token(A, w.row0 + min(r, w.n_rows - 1));
             float m_ref = -INFINITY;                   // reference maximum, log2 units
             float l_run = 0.f;
             const int x0 = x;
@@ -902,26 +917,26 @@ __global__ void __launch_bounds__(CT_THREADS, 1)
                     for (int e = 0; e < 32; ++e) o[e] = f1 != 0.f ? fmaf(f1, y[e], o[e]) : o[e];
                 }
             };
-            // the staged rows, CHUNKS chunks each, to their places; dst(at) is a row's first byte
-            auto flush = [&]<int CHUNKS>(auto&& dst) {
+            // the staged rows, CHUNKS chunks each, to their places
+            auto flush = [&]<int CHUNKS, class T>(T* base, int64_t stride) {   // stride 0: partial rows
                 constexpr int kRowsPerStep = 32 / CHUNKS;
                 __syncwarp();
                 const int ch = lane % CHUNKS;
                 int rr = lane / CHUNKS;
-                RowWalk at(w.row0 + row_base + rr, A.group);
+                RowWalk<T> at(A, base, stride, w.first, w.kvh, w.row0 + row_base + rr);
+                if (stride == 0) {
+                    at.p = base + static_cast<int64_t>(w.part + row_base + rr) * HD;
+                    at.wrap = 0;
+                }
 #pragma unroll
                 for (int q = 0; q < CHUNKS; ++q, rr += kRowsPerStep) {
                     if (row_base + rr < w.n_rows)
-                        reinterpret_cast<uint4*>(dst(at, row_base + rr))[ch] = stage[rr * CHUNKS + (ch ^ (rr & (CHUNKS - 1)))];
-                    at.step(kRowsPerStep, A.group);
+                        reinterpret_cast<uint4*>(at.p)[ch] = stage[rr * CHUNKS + (ch ^ (rr & (CHUNKS - 1)))];
+                    at.template step<kRowsPerStep>(A);
                 }
                 __syncwarp();
             };
             auto put = [&]<int COLS>(int col0, uint32_t t0, float f0, uint32_t t1, float f1, bool two) {
-                auto out_row = [&](const RowWalk& at, int) {
-                    return static_cast<Act*>(A.out) + (w.first + at.t) * A.out_stride + (w.kvh * A.group + at.h) * HD;
-                };
-                auto part_row = [&](const RowWalk&, int ri) { return A.part_o + (static_cast<size_t>(w.part) + ri) * HD; };
                 if (F32 || w.part >= 0) {
                     for (int col = col0; col < col0 + COLS; col += 32) {
                         float o[32];
@@ -931,8 +946,8 @@ __global__ void __launch_bounds__(CT_THREADS, 1)
                             stage[lane * 8 + (j ^ (lane & 7))] =
                                 make_uint4(__float_as_uint(o[4 * j]), __float_as_uint(o[4 * j + 1]),
                                            __float_as_uint(o[4 * j + 2]), __float_as_uint(o[4 * j + 3]));
-                        if (w.part >= 0) flush.template operator()<8>([&](const RowWalk& at, int ri) { return part_row(at, ri) + col; });
-                        else flush.template operator()<8>([&](const RowWalk& at, int ri) { return out_row(at, ri) + col; });
+                        flush.template operator()<8>(w.part >= 0 ? A.part_o + col : static_cast<float*>(A.out) + col,
+                                                     w.part >= 0 ? 0 : A.out_stride);
                     }
                 } else {
                     constexpr int kChunks = COLS / 8;
@@ -946,7 +961,7 @@ __global__ void __launch_bounds__(CT_THREADS, 1)
                                 make_uint4(pack_bf16(o[8 * j], o[8 * j + 1]), pack_bf16(o[8 * j + 2], o[8 * j + 3]),
                                            pack_bf16(o[8 * j + 4], o[8 * j + 5]), pack_bf16(o[8 * j + 6], o[8 * j + 7]));
                     }
-                    flush.template operator()<kChunks>([&](const RowWalk& at, int ri) { return out_row(at, ri) + col0; });
+                    flush.template operator()<kChunks>(static_cast<Act*>(A.out) + col0, A.out_stride);
                 }
             };
             float* lse = mine && w.part >= 0 ? A.part_lse + w.part + r : nullptr;
@@ -1006,7 +1021,7 @@ __global__ void __launch_bounds__(CT_THREADS, 1)
 }
 
 // ---- few rows --------------------------------------------------------------------
-// Items of at most kChunkFewRows rows (decode steps, a few guessed tokens) are
+// Chunks of at most kChunkFewRows rows (decode steps, a few guessed tokens) are
 // bound by the K/V bytes, and a 128-row tensor-core tile would be mostly empty:
 // here eight warps with 16-row mma.sync tiles (m16n8k16) share a tile, as row
 // groups of 16 rows times key groups of 128 / (16 groups) keys, each warp with its own running
@@ -1088,7 +1103,7 @@ __global__ void __launch_bounds__(FW_THREADS, 1)
         for (int e = 0; e < 2; ++e) {
             const int r = rg * 16 + gid + 8 * e;
             const bool ok = r < w.n_rows;
-            const int row = w.row0 + (ok ? r : 0), t = row / A.group, h = row - t * A.group;
+            const int row = w.row0 + (ok ? r : 0), t = row_token(A, row), h = row - t * A.group;
             pos_r[e] = w.pos + t;
             const Act* src = static_cast<const Act*>(A.q) + static_cast<int64_t>(w.first + t) * A.q_stride +
                              (w.kvh * A.group + h) * HD + 2 * tg;
@@ -1310,7 +1325,7 @@ __global__ void __launch_bounds__(kMergeThreads) chunk_merge_kernel(const __grid
         }
     }
     const ChunkSeq sq = A.d.seqs[m.seq];
-    const int row = m.row0 + r, t = row / A.group, h = row - t * A.group;
+    const int row = m.row0 + r, t = row_token(A, row), h = row - t * A.group;
     const float inv = 1.0f / sum;
     Act* out = static_cast<Act*>(A.out) + static_cast<int64_t>(sq.first + t) * A.out_stride +
                (m.kvh * A.group + h) * HD + 2 * lane;

@@ -346,7 +346,7 @@ cudaError_t launch_embed_rows(int type, float* x, const void* table, const int32
 // head h of the group (g = n_head / n_head_kv) of token t, so that a K/V tile
 // serves all the heads that share it.  An item is a block of kChunkItemRows
 // rows of one (chunk, KV head); a segment a range of kChunkTile-row K/V tiles
-// of one item, done by one CTA; the segments of items of at most kChunkFewRows
+// of one item, done by one CTA; the segments of chunks of at most kChunkFewRows
 // rows come last (few_start), for a kernel of their own.
 constexpr int kChunkTile = 128;       // K/V rows per tile
 constexpr int kChunkRows = 128;       // rows per tensor-core tile
@@ -426,6 +426,7 @@ struct ChunkArgs {
     const uint16_t* value_pool;
     int pool_pages, page_shift;
     int n_head, n_head_kv, group;   // group = n_head / n_head_kv
+    uint32_t group_mul, group_shift;   // row / group by multiplication (row_token)
     float* part_o;           // [part_rows][64] normalised partial results
     float* part_lse;         // [part_rows] log2 of the sum of exponentials; -inf: no row attended
     uint32_t* err;
