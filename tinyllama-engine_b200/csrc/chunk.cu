@@ -1038,7 +1038,8 @@ struct FewSmem {
     float o[FW_WARPS][16][HD + 4];      // a warp's result, and its rows' maximum and sum
     float2 ml[FW_WARPS][16];
     uint64_t full[FW_STAGES], empty[FW_STAGES];
-    int bad;                            // the segment has a non-finite V row that not every row attends to
+    int bad[2];                         // the segment has a non-finite V row that not every row attends to
+    Work work[kWorkCache];              // the CTA's first segments
 };
 
 __device__ __forceinline__ void ldsm4(uint32_t addr, uint32_t (&r)[4]) {
@@ -1075,14 +1076,16 @@ __global__ void __launch_bounds__(FW_THREADS, 1)
             mbar_init(&S.full[i], 1);
             mbar_init(&S.empty[i], FW_WARPS);
         }
-        S.bad = 0;
+        S.bad[0] = S.bad[1] = 0;
         fence_barrier_init();
         prefetch_tmap(&M.k);
         prefetch_tmap(&M.v);
     }
-    __syncthreads();
     asm volatile("griddepcontrol.wait;" ::: "memory");
     const int seg0 = A.d.few_start[blockIdx.x], seg1 = A.d.few_start[blockIdx.x + 1];
+    if (tid < kWorkCache && seg0 + tid < seg1) S.work[tid] = work_at(A, seg0 + tid);
+    __syncthreads();
+    auto work_of = [&](int i) { return i - seg0 < kWorkCache ? S.work[i - seg0] : work_at(A, i); };
     bool failed = false;
     if (warp == FW_WARPS) {
         produce_tiles<FW_STAGES>(A, M, seg0, seg1, S.k, S.v, S.full, S.empty, failed);
@@ -1090,46 +1093,71 @@ __global__ void __launch_bounds__(FW_THREADS, 1)
     }
     const int gid = lane >> 2, tg = lane & 3;     // fragment row and column pair
     const int mi = lane >> 3, li = lane & 7;      // ldmatrix: matrix and row of this lane's address
-    int ring = 0;
-    for (int sg = seg0; sg < seg1; ++sg) {
-        const Work w = work_at(A, sg);
-        const int rgroups = (w.n_rows + 15) >> 4 <= 1 ? 1 : (w.n_rows + 15) >> 4 <= 2 ? 2 : 4;
-        const int keys = 16 * rgroups;            // of a tile, per warp
-        const int rg = warp % rgroups, kg = warp / rgroups;
-        // this lane's rows gid and gid + 8 of the row group, as A fragments of Q
-        int pos_r[2];
-        uint32_t qf[kTerms][HD / 16][4];
+    auto row_groups = [](int n_rows) { return n_rows <= 16 ? 1 : n_rows <= 32 ? 2 : 4; };
+    // This lane's rows gid and gid + 8 of the row group, two columns of each 8:
+    // loaded ahead of the segment that needs them.
+    using Raw = std::conditional_t<F32, float2, uint32_t>;
+    Raw raw[2][HD / 8];
+    auto load_q = [&](const Work& w) {
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-            const int r = rg * 16 + gid + 8 * e;
+            const int r = warp % row_groups(w.n_rows) * 16 + gid + 8 * e;
             const bool ok = r < w.n_rows;
             const int row = w.row0 + (ok ? r : 0), t = row_token(A, row), h = row - t * A.group;
-            pos_r[e] = w.pos + t;
-            const Act* src = static_cast<const Act*>(A.q) + static_cast<int64_t>(w.first + t) * A.q_stride +
-                             (w.kvh * A.group + h) * HD + 2 * tg;
+            const Raw* src = reinterpret_cast<const Raw*>(static_cast<const Act*>(A.q) +
+                                                          static_cast<int64_t>(w.first + t) * A.q_stride +
+                                                          (w.kvh * A.group + h) * HD) + tg;
 #pragma unroll
-            for (int ks = 0; ks < HD / 16; ++ks)
-#pragma unroll
-                for (int half = 0; half < 2; ++half) {
-                    if constexpr (F32) {
-                        float2 x = ok ? load_pair(src + 16 * ks + 8 * half) : make_float2(0.f, 0.f);
-#pragma unroll
-                        for (int term = 0; term < kTerms; ++term) {
-                            qf[term][ks][2 * half + e] = top_pair(x.x, x.y);
-                            f2_split(rest_pair(x.x, x.y), x.x, x.y);
-                        }
-                    } else {
-                        qf[0][ks][2 * half + e] = ok ? *reinterpret_cast<const uint32_t*>(src + 16 * ks + 8 * half) : 0u;
-                    }
-                }
+            for (int i = 0; i < HD / 8; ++i) raw[e][i] = ok ? src[4 * i] : Raw{};
         }
-        float m_ref[2] = {-INFINITY, -INFINITY}, l_run[2] = {0.f, 0.f};
+    };
+    int ring = 0;
+    // The tiles of one segment; leaves the warp's maxima, sums and outputs in S.
+    // HALF (at most 8 rows): with fp32 the upper 8 rows of the A fragments hold the
+    // second term of the same rows, so two MMAs do for three terms.
+    auto segment = [&]<bool HALF>(const Work& w, int k) {
+        constexpr int kRows = HALF ? 1 : 2;       // rows of a lane: gid (, gid + 8)
+        constexpr int kFrags = !F32 ? 1 : HALF ? 2 : 3;
+        const int rgroups = row_groups(w.n_rows);
+        const int keys = 16 * rgroups;            // of a tile, per warp
+        const int rg = warp % rgroups, kg = warp / rgroups;
+        int pos_r[kRows];
+        uint32_t qf[kFrags][HD / 16][4];          // A fragments of Q
+#pragma unroll
+        for (int f = 0; f < kFrags; ++f)
+#pragma unroll
+            for (int ks = 0; ks < HD / 16; ++ks) qf[f][ks][0] = qf[f][ks][1] = qf[f][ks][2] = qf[f][ks][3] = 0u;
+#pragma unroll
+        for (int e = 0; e < kRows; ++e) {
+            pos_r[e] = w.pos + row_token(A, w.row0 + min(rg * 16 + gid + 8 * e, w.n_rows - 1));
+#pragma unroll
+            for (int i = 0; i < HD / 8; ++i) {
+                if constexpr (F32) {
+                    float2 x = raw[e][i];
+#pragma unroll
+                    for (int term = 0; term < kTerms; ++term) {
+                        if (HALF) qf[term >> 1][i >> 1][2 * (i & 1) + (term & 1)] = top_pair(x.x, x.y);
+                        else qf[term][i >> 1][2 * (i & 1) + e] = top_pair(x.x, x.y);
+                        f2_split(rest_pair(x.x, x.y), x.x, x.y);
+                    }
+                } else {
+                    qf[0][i >> 1][2 * (i & 1) + e] = raw[e][i];
+                }
+            }
+        }
+        float m_ref[kRows], l_run[kRows];
+#pragma unroll
+        for (int e = 0; e < kRows; ++e) {
+            m_ref[e] = -INFINITY;
+            l_run[e] = 0.f;
+        }
         float o[HD / 8][4];
 #pragma unroll
         for (int i = 0; i < HD / 8; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
         for (int n = w.t0; n < w.t1; ++n, ++ring) {
             const int st = ring % FW_STAGES;
             wait_or_flag(&S.full[st], (ring / FW_STAGES) & 1, A.err, kErrWaitFull, failed);
+            __syncwarp();
             const uint32_t kb = smem_u32(S.k[st]), vb = smem_u32(S.v[st]);
             const bool edge = w.edge(n);
             for (int j0 = kg * keys; j0 < (kg + 1) * keys; j0 += 16) {   // 16 keys
@@ -1145,141 +1173,168 @@ __global__ void __launch_bounds__(FW_THREADS, 1)
                         if (key >= w.kv_len) *p = make_uint4(0, 0, 0, 0);
                         else if (key > w.pos_min) bad |= not_finite(*p);
                     }
-                    if (__any_sync(0xffffffffu, bad) && lane == 0) S.bad = 1;
+                    if (__any_sync(0xffffffffu, bad) && lane == 0) S.bad[k & 1] = 1;
                     __syncwarp();
                 }
-                float s[2][4];   // keys key0 + 8 b + 2 tg (+1): rows gid (0, 1), gid + 8 (2, 3)
+                // S: one accumulator per fragment and 8 keys, so that the MMAs of a
+                // fragment only wait for each other
+                float sf[kFrags][2][4];
 #pragma unroll
-                for (int b = 0; b < 2; ++b) s[b][0] = s[b][1] = s[b][2] = s[b][3] = 0.f;
+                for (int f = 0; f < kFrags; ++f)
+#pragma unroll
+                    for (int b = 0; b < 2; ++b) sf[f][b][0] = sf[f][b][1] = sf[f][b][2] = sf[f][b][3] = 0.f;
+                uint32_t kf[HD / 16][4];
 #pragma unroll
                 for (int ks = 0; ks < HD / 16; ++ks) {
                     const int r = j0 + li + 8 * (mi >> 1), ch = 2 * ks + (mi & 1);
-                    uint32_t kf[4];
-                    ldsm4(kb + r * (HD * 2) + ((ch ^ (r & 7)) << 4), kf);
+                    ldsm4(kb + r * (HD * 2) + ((ch ^ (r & 7)) << 4), kf[ks]);
+                }
 #pragma unroll
-                    for (int term = kTerms - 1; term >= 0; --term) {
-                        mma16816(s[0], qf[term][ks], kf[0], kf[1]);
-                        mma16816(s[1], qf[term][ks], kf[2], kf[3]);
+                for (int ks = 0; ks < HD / 16; ++ks)
+#pragma unroll
+                    for (int f = 0; f < kFrags; ++f) {
+                        mma16816(sf[f][0], qf[f][ks], kf[ks][0], kf[ks][1]);
+                        mma16816(sf[f][1], qf[f][ks], kf[ks][2], kf[ks][3]);
                     }
+                uint32_t vf[HD / 16][4];
+#pragma unroll
+                for (int dp = 0; dp < HD / 16; ++dp) {
+                    const int r = j0 + li + 8 * (mi & 1), ch = 2 * dp + (mi >> 1);
+                    ldsm4_t(vb + r * (HD * 2) + ((ch ^ (r & 7)) << 4), vf[dp]);
                 }
-                if (edge) {
+                float s[kRows][4];   // row, keys key0 + 2 tg (+1), key0 + 8 + 2 tg (+1)
 #pragma unroll
-                    for (int b = 0; b < 2; ++b)
+                for (int e = 0; e < kRows; ++e)
 #pragma unroll
-                        for (int e = 0; e < 4; ++e)
-                            if (key0 + 8 * b + 2 * tg + (e & 1) > pos_r[e >> 1]) s[b][e] = -INFINITY;
+                    for (int q = 0; q < 4; ++q) {
+                        const int b = q >> 1, i = 2 * e + (q & 1);
+                        if (!F32) s[e][q] = sf[0][b][i];
+                        else if (HALF) s[e][q] = sf[0][b][i] + (sf[0][b][i + 2] + sf[kFrags - 1][b][i]);
+                        else s[e][q] = sf[0][b][i] + (sf[kFrags > 1 ? 1 : 0][b][i] + sf[kFrags - 1][b][i]);
+                        if (edge && key0 + 8 * b + 2 * tg + (q & 1) > pos_r[e]) s[e][q] = -INFINITY;
+                    }
+                float mt[kRows];
+                bool grow = false;   // m_ref is the same in the four lanes of a row
+#pragma unroll
+                for (int e = 0; e < kRows; ++e) {
+                    mt[e] = fmax3(fmax3(s[e][0], s[e][1], s[e][2]), s[e][3], s[e][3]) * kExpScale;
+                    grow |= m_ref[e] == m_ref[e] && !(mt[e] <= m_ref[e] + kMoveThreshold);
                 }
-                float mt[2];
+                if (__any_sync(0xffffffffu, grow)) {
 #pragma unroll
-                for (int e = 0; e < 2; ++e)
-                    mt[e] = fmax3(fmax3(s[0][2 * e], s[0][2 * e + 1], s[1][2 * e]), s[1][2 * e + 1], -INFINITY) * kExpScale;
-                // m_ref is the same in the four lanes of a row
-                auto grows = [&](int e) { return m_ref[e] == m_ref[e] && !(mt[e] <= m_ref[e] + kMoveThreshold); };
-                if (__any_sync(0xffffffffu, grows(0) || grows(1))) {
-#pragma unroll
-                    for (int e = 0; e < 2; ++e) {
+                    for (int e = 0; e < kRows; ++e) {
                         float m = fmax3(mt[e], __shfl_xor_sync(0xffffffffu, mt[e], 1), -INFINITY);
                         m = fmax3(m, __shfl_xor_sync(0xffffffffu, m, 2), -INFINITY);
                         if (m_ref[e] == m_ref[e] && !(m <= m_ref[e] + kMoveThreshold)) {
-                            const float alpha = m_ref[e] == -INFINITY ? 0.f : exp2f(m_ref[e] - m);
+                            const float alpha = ex2_sfu(m_ref[e] - m);   // 0 from -inf
                             m_ref[e] = m;
                             l_run[e] *= alpha;
 #pragma unroll
                             for (int i = 0; i < HD / 8; ++i) {
                                 o[i][2 * e] *= alpha;
                                 o[i][2 * e + 1] *= alpha;
+                                if (HALF) {
+                                    o[i][2] *= alpha;
+                                    o[i][3] *= alpha;
+                                }
                             }
                         }
                     }
                 }
-                const float m_use[2] = {m_ref[0] == -INFINITY ? 0.f : m_ref[0], m_ref[1] == -INFINITY ? 0.f : m_ref[1]};
+                uint32_t pf[kFrags][4];   // A fragments of P: keys 2 tg (+1), then + 8
 #pragma unroll
-                for (int b = 0; b < 2; ++b)
+                for (int f = 0; f < kFrags; ++f) pf[f][0] = pf[f][1] = pf[f][2] = pf[f][3] = 0u;
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        s[b][e] = ex2_sfu(fmaf(s[b][e], kExpScale, -m_use[e >> 1]));
-                        l_run[e >> 1] += s[b][e];
-                    }
-                uint32_t pf[kTerms][4];   // A fragment of P: keys 2 tg (+1), then + 8
-                if constexpr (F32) {
+                for (int e = 0; e < kRows; ++e) {
+                    const float m_use = m_ref[e] == -INFINITY ? 0.f : m_ref[e];
 #pragma unroll
-                    for (int term = 0; term < kTerms; ++term)
+                    for (int q = 0; q < 4; ++q) s[e][q] = ex2_sfu(fmaf(s[e][q], kExpScale, -m_use));
+                    l_run[e] += (s[e][0] + s[e][1]) + (s[e][2] + s[e][3]);
 #pragma unroll
-                        for (int b = 0; b < 2; ++b)
+                    for (int b = 0; b < 2; ++b) {
+                        float x0 = s[e][2 * b], x1 = s[e][2 * b + 1];
+                        if constexpr (F32) {
 #pragma unroll
-                            for (int e = 0; e < 2; ++e) {
-                                pf[term][2 * b + e] = top_pair(s[b][2 * e], s[b][2 * e + 1]);
-                                f2_split(rest_pair(s[b][2 * e], s[b][2 * e + 1]), s[b][2 * e], s[b][2 * e + 1]);
+                            for (int term = 0; term < kTerms; ++term) {
+                                if (HALF) pf[term >> 1][2 * b + (term & 1)] = top_pair(x0, x1);
+                                else pf[term][2 * b + e] = top_pair(x0, x1);
+                                f2_split(rest_pair(x0, x1), x0, x1);
                             }
-                } else {
-#pragma unroll
-                    for (int b = 0; b < 2; ++b)
-#pragma unroll
-                        for (int e = 0; e < 2; ++e) pf[0][2 * b + e] = pack_bf16(s[b][2 * e], s[b][2 * e + 1]);
-                }
-#pragma unroll
-                for (int dp = 0; dp < HD / 16; ++dp) {
-                    const int r = j0 + li + 8 * (mi & 1), ch = 2 * dp + (mi >> 1);
-                    uint32_t vf[4];
-                    ldsm4_t(vb + r * (HD * 2) + ((ch ^ (r & 7)) << 4), vf);
-#pragma unroll
-                    for (int term = kTerms - 1; term >= 0; --term) {
-                        mma16816(o[2 * dp], pf[term], vf[0], vf[1]);
-                        mma16816(o[2 * dp + 1], pf[term], vf[2], vf[3]);
+                        } else {
+                            pf[0][2 * b + e] = pack_bf16(x0, x1);
+                        }
                     }
                 }
+#pragma unroll
+                for (int f = kFrags - 1; f >= 0; --f)
+#pragma unroll
+                    for (int dp = 0; dp < HD / 16; ++dp) {
+                        mma16816(o[2 * dp], pf[f], vf[dp][0], vf[dp][1]);
+                        mma16816(o[2 * dp + 1], pf[f], vf[dp][2], vf[dp][3]);
+                    }
             }
             if (edge) fence_proxy_async_smem();   // zeroed rows: before the stage's next TMA load
             __syncwarp();
             if (lane == 0) mbar_arrive(&S.empty[st]);
         }
-        // ---- join the key groups ----
 #pragma unroll
-        for (int e = 0; e < 2; ++e) {
+        for (int e = 0; e < kRows; ++e) {
             l_run[e] += __shfl_xor_sync(0xffffffffu, l_run[e], 1);
             l_run[e] += __shfl_xor_sync(0xffffffffu, l_run[e], 2);
             if (tg == 0) S.ml[warp][gid + 8 * e] = make_float2(m_ref[e], l_run[e]);
 #pragma unroll
             for (int i = 0; i < HD / 8; ++i)
-                *reinterpret_cast<float2*>(&S.o[warp][gid + 8 * e][8 * i + 2 * tg]) = make_float2(o[i][2 * e], o[i][2 * e + 1]);
+                *reinterpret_cast<float2*>(&S.o[warp][gid + 8 * e][8 * i + 2 * tg]) =
+                    HALF ? make_float2(o[i][0] + o[i][2], o[i][1] + o[i][3]) : make_float2(o[i][2 * e], o[i][2 * e + 1]);
         }
+    };
+    if (seg0 < seg1) load_q(work_of(seg0));
+    for (int sg = seg0; sg < seg1; ++sg) {
+        const int k = sg - seg0;
+        const Work w = work_of(sg);
+        const int rgroups = row_groups(w.n_rows);
+        if (w.n_rows <= 8) segment.template operator()<true>(w, k);
+        else segment.template operator()<false>(w, k);
+        // ---- join the key groups ----
+        if (sg + 1 < seg1) load_q(work_of(sg + 1));
         named_bar_sync(1, 32 * FW_WARPS);
-        if (S.bad) {
-            if (tid < w.n_rows) chunk_row_exact<Act>(A, w, tid, row_out<Act>(A, w, tid));
+        if (tid == 0) S.bad[(k + 1) & 1] = 0;   // of the next segment: nobody is there before the barrier below
+        if (S.bad[k & 1]) {
+            const Work cold = w;
+            if (tid < w.n_rows) chunk_row_exact<Act>(A, cold, tid, row_out<Act>(A, cold, tid));
         } else {
+            // a row per warp, two columns per lane; lane q has the weight of key group q
             const int kgroups = FW_WARPS / rgroups;
-            for (int e = tid; e < w.n_rows * (HD / 8); e += 32 * FW_WARPS) {
-                const int r = e >> 3, c8 = (e & 7) * 8, w0 = r >> 4, rr = r & 15;
-                float m_all = -INFINITY;
-                for (int q = 0; q < kgroups; ++q) m_all = fmaxf(m_all, S.ml[w0 + q * rgroups][rr].x);
-                float acc[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f}, l_all = 0.f;
-                for (int q = 0; q < kgroups; ++q) {
-                    const float2 ml = S.ml[w0 + q * rgroups][rr];
-                    const float f = ml.x == -INFINITY ? 0.f : exp2f(ml.x - m_all);
-                    l_all = fmaf(f, ml.y, l_all);
-                    const float4* src = reinterpret_cast<const float4*>(&S.o[w0 + q * rgroups][rr][c8]);
-                    const float4 x = src[0], y = src[1];
-                    acc[0] = fmaf(f, x.x, acc[0]);
-                    acc[1] = fmaf(f, x.y, acc[1]);
-                    acc[2] = fmaf(f, x.z, acc[2]);
-                    acc[3] = fmaf(f, x.w, acc[3]);
-                    acc[4] = fmaf(f, y.x, acc[4]);
-                    acc[5] = fmaf(f, y.y, acc[5]);
-                    acc[6] = fmaf(f, y.z, acc[6]);
-                    acc[7] = fmaf(f, y.w, acc[7]);
-                }
-                const bool empty = l_all == 0.f;   // no row of this segment is attended to
-                const float inv = empty ? 0.f : 1.0f / l_all;
+            for (int r = warp; r < w.n_rows; r += FW_WARPS) {
+                const int w0 = r >> 4, rr = r & 15;
+                const float2 ml = lane < kgroups ? S.ml[w0 + lane * rgroups][rr] : make_float2(-INFINITY, 0.f);
+                float m_all = ml.x;
 #pragma unroll
-                for (int i = 0; i < 8; ++i) acc[i] = empty ? 0.f : acc[i] * inv;
+                for (int d = 1; d < FW_WARPS; d *= 2) m_all = fmaxf(m_all, __shfl_xor_sync(0xffffffffu, m_all, d));
+                const float f = ml.x == -INFINITY ? 0.f : ex2_sfu(ml.x - m_all);
+                float l_all = f == 0.f ? 0.f : f * ml.y;
+#pragma unroll
+                for (int d = 1; d < FW_WARPS; d *= 2) l_all += __shfl_xor_sync(0xffffffffu, l_all, d);
+                float2 acc = make_float2(0.f, 0.f);
+#pragma unroll
+                for (int q = 0; q < FW_WARPS; ++q) {
+                    const float fq = __shfl_sync(0xffffffffu, f, q);
+                    if (q < kgroups) {
+                        const float2 x = *reinterpret_cast<const float2*>(&S.o[w0 + q * rgroups][rr][2 * lane]);
+                        acc.x = fmaf(fq, x.x, acc.x);
+                        acc.y = fmaf(fq, x.y, acc.y);
+                    }
+                }
+                const float l_row = __shfl_sync(0xffffffffu, l_all, 0), m_row = __shfl_sync(0xffffffffu, m_all, 0);
+                const bool empty = l_row == 0.f;   // no row of this segment is attended to
+                const float inv = empty ? 0.f : 1.0f / l_row;
+                acc = empty ? make_float2(0.f, 0.f) : make_float2(acc.x * inv, acc.y * inv);
                 const RowOut<Act> dst = row_out<Act>(A, w, r);
-                if (dst.out) store8(dst.out + c8, acc);
-                else store8(dst.part + c8, acc);
-                if (dst.lse && c8 == 0) *dst.lse = empty ? -INFINITY : m_all + log2f(l_all);
+                if (dst.out) store_pair(dst.out + 2 * lane, acc);
+                else store_pair(dst.part + 2 * lane, acc);
+                if (dst.lse && lane == 0) *dst.lse = empty ? -INFINITY : m_row + log2f(l_row);
             }
         }
-        named_bar_sync(1, 32 * FW_WARPS);
-        if (tid == 0) S.bad = 0;   // next written after the next tile, read after the next barrier
         named_bar_sync(1, 32 * FW_WARPS);
     }
 }
