@@ -95,7 +95,7 @@ typedef struct {
     const float* presence;      /* made tokens:   x - presence                            */
     /* Biases of row r: x + bias_values[i] for the token bias_tokens[i], i in
      * [bias_start[r], bias_start[r + 1]); a token listed several times gets
-     * their sum, added in the list's order. */
+     * all of them, in the list's order. */
     const int32_t* bias_tokens; /* [n_biases] */
     const float* bias_values;   /* [n_biases] */
     const int32_t* bias_start;  /* [n_rows + 1] */
