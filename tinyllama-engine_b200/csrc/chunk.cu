@@ -190,7 +190,10 @@ __global__ void __launch_bounds__(kAppendThreads) append_kernel(const __grid_con
 // Precision: bf16 activations: P rounded to bf16 (its sum is not), fp32
 // accumulation.  fp32 activations: q and P are cut into three bf16 numbers of
 // 8 bits each whose sum is the 24-bit value exactly, so S and O are 32-bit
-// sums of exact products; the cost is three times the MMAs.
+// sums of exact products; the cost is three times the MMAs.  The tensor cores
+// cut their running sums off instead of rounding them (over 16000 rows O came
+// out 3e-5 too small), so with fp32 activations O is summed there over
+// kFlushBlocks blocks only and from there on in registers.
 //
 // Rows beyond what a token attends to: a score is masked by selection, but
 // P = 0 does not silence a NaN or infinity in V.  Tiles that hold such rows
@@ -208,6 +211,7 @@ template <bool F32>
 constexpr int kKeysOf = F32 ? 64 : 128;      // keys of a block
 template <bool F32>
 constexpr int kBufsOf = F32 ? 2 : 1;         // S and P buffers of a chain
+constexpr int kFlushBlocks = 4;              // fp32: blocks whose PV are summed in tensor memory (48 MMAs)
 constexpr int kRegsControl = 56, kRegsSoftmax = 200, kRegsLaunch = 128;
 static_assert(256 * kRegsControl + 256 * kRegsSoftmax <= CT_THREADS * kRegsLaunch,
               "setmaxnreg split exceeds the launch register budget");
@@ -660,7 +664,8 @@ __global__ void __launch_bounds__(CT_THREADS, 1)
                 const Work w = work_of(seg0 + k);
                 const int t0 = uniform(w.t0), t1 = uniform(w.t1), kv_len = uniform(w.kv_len), pos_min = uniform(w.pos_min);
                 const int dual = uniform(static_cast<int>(w.dual));
-                uint32_t acc = 0;   // the segment's first block overwrites O
+                uint32_t acc = 0;   // the segment's first block overwrites O, fp32: every kFlushBlocks-th
+                const int x_first = x;
                 for (int n = t0; n < t1; ++n, ++ring) {
                     const int st = ring % CT_STAGES;
                     const bool edge = n * kTile + kTile - 1 > pos_min;
@@ -678,6 +683,7 @@ __global__ void __launch_bounds__(CT_THREADS, 1)
                     if (edge) wait_uniform(&S.v_ok[st], par, A.err, kErrWaitFull, failed);
                     for (int u = u0; u < u1; u += du, ++x) {
                         const int h = x % kBufs;
+                        if (F32 && (x - x_first) % kFlushBlocks == 0) acc = 0;
                         wait_uniform(&S.p_full[c][h], (x / kBufs) & 1, A.err, kErrWaitMma, failed);
                         tc_fence_after();
                         const uint64_t dv = v_desc(v0 + (st * kTileHalfs + u * kKeys * HD) * 2);
@@ -813,6 +819,16 @@ __global__ void __launch_bounds__(CT_THREADS, 1)
         int x = 0;        // own blocks so far (barrier phases)
         int n_joins = 0;  // segments of smaller items so far
         bool s_ready = false;   // S of block x is there
+        auto add_o = [&](auto& sum) {
+#pragma unroll
+            for (int q = 0; q < HD / 32; ++q) {
+                float o[32];
+                tmem_ld32(tO + 32 * q, o);
+                tmem_wait_ld();
+#pragma unroll
+                for (int e = 0; e < 32; ++e) sum[32 * q + e] += o[e];
+            }
+        };
         for (int sg = seg0; sg < seg1; ++sg) {
             const int k = sg - seg0;
             const Work w = work_of(sg);
@@ -820,6 +836,11 @@ __global__ void __launch_bounds__(CT_THREADS, 1)
             const int my_pos = w.pos + row_token(A, w.row0 + min(r, w.n_rows - 1));
             float m_ref = -INFINITY;                   // reference maximum, log2 units
             float l_run = 0.f;
+            [[maybe_unused]] float o_sum[F32 ? HD : 1];   // O of the blocks before the last flush
+            if constexpr (F32) {
+#pragma unroll
+                for (int e = 0; e < HD; ++e) o_sum[e] = 0.f;
+            }
             const int x0 = x;
             const int key0 = w.t0 * kTile, key_end = min(w.t1 * kTile, w.kv_len);
             // Block x from key on; EDGE: some of its keys are masked for some row.
@@ -885,7 +906,19 @@ __global__ void __launch_bounds__(CT_THREADS, 1)
                 // an earlier PV could be reading, and S was issued after that)
                 if (!p_done) wait_or_flag(&S.p_free[c][0], (x - 1) & 1, A.err, kErrWaitMma, failed);
                 __syncwarp();
-                if (any_move && x > x0) {
+                if constexpr (F32) {
+                    if (x > x0 && (x - x0) % kFlushBlocks == 0) {   // the next PV starts anew
+                        wait_or_flag(&S.p_free[c][(x - 1) % kBufs], ((x - 1) / kBufs) & 1, A.err, kErrWaitMma, failed);
+                        __syncwarp();
+                        tc_fence_after();
+                        add_o(o_sum);
+                    }
+                    if (any_move && x > x0) {
+#pragma unroll
+                        for (int e = 0; e < HD; ++e) o_sum[e] *= alpha;
+                    }
+                }
+                if (any_move && x > x0 && (!F32 || (x - x0) % kFlushBlocks != 0)) {
                     if (F32) wait_uniform(&S.p_free[c][(x - 1) % kBufs], ((x - 1) / kBufs) & 1, A.err, kErrWaitMma, failed);
                     tc_fence_after();
 #pragma unroll
@@ -934,7 +967,16 @@ __global__ void __launch_bounds__(CT_THREADS, 1)
             for (int y = max(x0, x - kBufs); y < x; ++y)
                 wait_or_flag(&S.p_free[c][y % kBufs], (y / kBufs) & 1, A.err, kErrWaitMma, failed);
             wait_or_flag(&S.scanned[k & 1], (k >> 1) & 1, A.err, kErrWaitMma, failed);
+            __syncwarp();
             tc_fence_after();
+            if constexpr (F32) {
+                if (x - x0 > kFlushBlocks) {   // O whole again, in its place
+                    add_o(o_sum);
+#pragma unroll
+                    for (int q = 0; q < HD / 32; ++q) tmem_st32(tO + 32 * q, *reinterpret_cast<const uint32_t(*)[32]>(&o_sum[32 * q]));
+                    tmem_wait_st();
+                }
+            }
             const bool mine = r < w.n_rows;
             // COLS columns from col0 on of every row of the warp, from one chain or two with
             // weights f0, f1 (a chain without weight may hold anything).  Through shared
@@ -1070,6 +1112,7 @@ __global__ void __launch_bounds__(CT_THREADS, 1)
 constexpr int FW_WARPS = 8;
 constexpr int FW_THREADS = 32 * (FW_WARPS + 1);
 constexpr int FW_STAGES = 5;
+constexpr int kFewFlush = 8;        // fp32: tiles (of one row group) whose MMAs are summed in a row
 struct FewSmem {
     uint16_t k[FW_STAGES][kTileHalfs];
     uint16_t v[FW_STAGES][kTileHalfs];
@@ -1192,7 +1235,29 @@ __global__ void __launch_bounds__(FW_THREADS, 1)
         float o[HD / 8][4];
 #pragma unroll
         for (int i = 0; i < HD / 8; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
+        // fp32: o is summed by MMAs over kFewFlush tiles only and from there on in S
+        // (the tensor cores cut their sums off)
+        int since = 0;
+        bool flushed = false;
+        auto held = [&](int e, int i) -> float2& {
+            return *reinterpret_cast<float2*>(&S.o[warp][gid + 8 * e][8 * i + 2 * tg]);
+        };
+        auto flush = [&]() {
+#pragma unroll
+            for (int e = 0; e < kRows; ++e)
+#pragma unroll
+                for (int i = 0; i < HD / 8; ++i) {
+                    float2 y = HALF ? make_float2(o[i][0] + o[i][2], o[i][1] + o[i][3]) : make_float2(o[i][2 * e], o[i][2 * e + 1]);
+                    if (flushed) y = make_float2(held(e, i).x + y.x, held(e, i).y + y.y);
+                    held(e, i) = y;
+                }
+#pragma unroll
+            for (int i = 0; i < HD / 8; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
+            flushed = true;
+            since = 0;
+        };
         for (int n = w.t0; n < w.t1; ++n, ++ring) {
+            if (F32 && ++since > kFewFlush / rgroups) flush();
             const int st = ring % FW_STAGES;
             wait_or_flag(&S.full[st], (ring / FW_STAGES) & 1, A.err, kErrWaitFull, failed);
             __syncwarp();
@@ -1275,6 +1340,7 @@ __global__ void __launch_bounds__(FW_THREADS, 1)
                                     o[i][2] *= alpha;
                                     o[i][3] *= alpha;
                                 }
+                                if (F32 && flushed) held(e, i) = make_float2(held(e, i).x * alpha, held(e, i).y * alpha);
                             }
                         }
                     }
@@ -1320,11 +1386,8 @@ __global__ void __launch_bounds__(FW_THREADS, 1)
             l_run[e] += __shfl_xor_sync(0xffffffffu, l_run[e], 1);
             l_run[e] += __shfl_xor_sync(0xffffffffu, l_run[e], 2);
             if (tg == 0) S.ml[warp][gid + 8 * e] = make_float2(m_ref[e], l_run[e]);
-#pragma unroll
-            for (int i = 0; i < HD / 8; ++i)
-                *reinterpret_cast<float2*>(&S.o[warp][gid + 8 * e][8 * i + 2 * tg]) =
-                    HALF ? make_float2(o[i][0] + o[i][2], o[i][1] + o[i][3]) : make_float2(o[i][2 * e], o[i][2 * e + 1]);
         }
+        flush();
     };
     if (seg0 < seg1) load_q(work_of(seg0));
     for (int sg = seg0; sg < seg1; ++sg) {
