@@ -249,6 +249,31 @@ def _stream(stream) -> int:
     return int(stream.cuda_stream)
 
 
+def _raw_stream(stream, index: int) -> int:
+    """Handle of `stream`, or of the current stream of device `index`, which
+    becomes the current device of a call made under _on_device."""
+    import torch
+    if stream is None:
+        # the handle without a Stream object around it, 1.5 us less, where torch offers it
+        raw = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+        return raw(index) if raw else torch.cuda.current_stream(index).cuda_stream
+    if stream.device.index != index:
+        raise ValueError(f"stream of {stream.device}, tensors on cuda:{index}")
+    return stream.cuda_stream
+
+
+def _on_device(index: int, fn, *args) -> None:
+    """fn(*args), checked, with device `index` current."""
+    import torch
+    if torch.cuda.current_device() == index:
+        rc = fn(*args)
+    else:
+        with torch.cuda.device(index):
+            rc = fn(*args)
+    if rc != TLE_OK:
+        raise TleError(rc, lib().tle_last_error().decode())
+
+
 def _want(t, numel: int, name: str):
     import torch
     if t.dtype != torch.float32 or not t.is_cuda or not t.is_contiguous():
@@ -541,7 +566,8 @@ class PagedKVCache:
         self._free = list(range(self.n_pages - 1, -1, -1))
 
     def pool(self):
-        if self.dtype != __import__("torch").float32:
+        import torch
+        if self.dtype != torch.float32:
             return PagePoolBf16(_ptr(self.key_pool), _ptr(self.value_pool), self.n_pages, self.page_rows)
         return PagePool(_ptr(self.key_pool), _ptr(self.value_pool), self.n_pages, self.page_rows)
 
@@ -645,6 +671,14 @@ class PagedChunkBatch:
         self.cache = cache
         self.shape = cache.shape
         self.device = cache.key_pool.device
+        if self.device.type != "cuda":
+            raise ValueError("a PagedKVCache on a CUDA device expected")
+        self._index = self.device.index
+        self._shape_ref = ctypes.byref(self.shape)
+        self._widths = (self.shape.n_head * self.shape.head_dim, self.shape.n_head_kv * self.shape.head_dim)
+        self._bf16 = cache.dtype == torch.bfloat16
+        if not self._bf16 and cache.dtype != torch.float32:
+            raise ValueError(f"a float32 or bfloat16 PagedKVCache expected, got {cache.dtype}")
         self.max_ctas = max_ctas
         self.tables = list(tables)
         self.n = len(self.tables)
@@ -690,72 +724,70 @@ class PagedChunkBatch:
         self.positions = [int(p) for p in positions]
         self.lengths = [int(x) for x in lengths]
 
-    def _rows(self, t, heads: int, name: str, dtype):
-        """Pointer and row stride of an activation tensor."""
-        import torch
-        if t.dtype not in (torch.float32, torch.bfloat16) or (dtype is not None and t.dtype != dtype):
+    def _rows(self, t, w: int, name: str, dtype):
+        """Pointer and row stride of an activation tensor of rows of w."""
+        shape, strides = t.shape, t.stride()
+        if t.dtype is not dtype:
             raise ValueError(f"{name}: activations are all float32 or all bfloat16, got {t.dtype}")
-        if t.device != self.device:
+        if t.get_device() != self._index:
             raise ValueError(f"{name}: is on {t.device}, the cache on {self.device}")
-        w = heads * self.shape.head_dim
-        if t.dim() != 2 or t.shape[1] != w or t.shape[0] < self.plan.n_tokens or t.stride(1) != 1:
+        if len(shape) != 2 or shape[1] != w or shape[0] < self.plan.n_tokens or strides[1] != 1:
             raise ValueError(f"{name}: need [{self.plan.n_tokens}][{w}] with contiguous rows, got "
-                             f"{tuple(t.shape)} with strides {t.stride()}")
-        return t.data_ptr(), (t.stride(0) if t.shape[0] > 1 else w)
+                             f"{tuple(shape)} with strides {strides}")
+        return t.data_ptr(), (strides[0] if shape[0] > 1 else w)
 
-    def _on(self, stream):
-        """(stream handle, the tensors' device made current)."""
+    def _act(self, t, name: str) -> int:
+        """TLE_ACT_* of an activation tensor."""
         import torch
-        if stream is None:
-            return torch.cuda.current_stream(self.device).cuda_stream
-        if stream.device != self.device:
-            raise ValueError(f"stream of {stream.device}, tensors on {self.device}")
-        for t in (self._desc_dev, self.workspace):
-            t.record_stream(stream)
-        return stream.cuda_stream
+        if t.dtype is torch.bfloat16:
+            return 1
+        if t.dtype is torch.float32:
+            return 0
+        raise ValueError(f"{name}: activations are all float32 or all bfloat16, got {t.dtype}")
+
+    def _on(self, stream) -> int:
+        if stream is not None:
+            for t in (self._desc_dev, self.workspace):
+                t.record_stream(stream)
+        return _raw_stream(stream, self._index)
 
     def append(self, q, k, v, layer: int, rotate: bool = True, q_out=None, stream=None) -> None:
         """rope(q, k) at each token's position (rotate), k and v stored in
         their rows of the cache, q written to q_out (contiguous, the type of
         q; may be q; q and q_out both None: keys and values only)."""
-        import torch
-        dt = k.dtype
-        kp, ks = self._rows(k, self.shape.n_head_kv, "k", None)
-        vp, vs = self._rows(v, self.shape.n_head_kv, "v", dt)
-        qp = qs = qo = None
+        act, dt = self._act(k, "k"), k.dtype
+        wq, wkv = self._widths
+        kp, ks = self._rows(k, wkv, "k", dt)
+        vp, vs = self._rows(v, wkv, "v", dt)
+        qp = qo = None
+        qs = 0
         if q is not None:
             if q_out is None:
                 raise ValueError("q_out: where the rotated q goes")
-            qp, qs = self._rows(q, self.shape.n_head, "q", dt)
-            qo, os = self._rows(q_out, self.shape.n_head, "q_out", dt)
-            if os != self.shape.n_head * self.shape.head_dim:
+            qp, qs = self._rows(q, wq, "q", dt)
+            qo, os = self._rows(q_out, wq, "q_out", dt)
+            if os != wq:
                 raise ValueError("q_out: need a contiguous tensor")
         elif q_out is not None:
             raise ValueError("q_out without q")
         L = lib()
-        fn = L.tle_append_paged if self.cache.dtype == torch.float32 else L.tle_append_bf16_paged
         pool = self.cache.pool()
-        st = self._on(stream)
-        with torch.cuda.device(self.device):
-            _check(fn(ctypes.byref(self.shape), ctypes.addressof(pool), ctypes.byref(self.plan),
-                      self._desc_dev.data_ptr(), qp, qs or 0, kp, ks, vp, vs, qo, int(dt == torch.bfloat16),
-                      layer, TLE_DECODE_ROTATE if rotate else 0, st))
+        _on_device(self._index, L.tle_append_bf16_paged if self._bf16 else L.tle_append_paged, self._shape_ref,
+                   ctypes.addressof(pool), ctypes.byref(self.plan), self._desc_dev.data_ptr(), qp, qs, kp, ks, vp, vs,
+                   qo, act, layer, TLE_DECODE_ROTATE if rotate else 0, self._on(stream))
 
     def attend(self, q, out, layer: int, stream=None) -> None:
         """Causal attention of the chunks (q already rotated) over a bf16
         cache; rows of out behind the last token are left as they are."""
-        import torch
-        if self.cache.dtype != torch.bfloat16:
+        if not self._bf16:
             raise ValueError("attend: a bfloat16 PagedKVCache expected")
-        qp, qs = self._rows(q, self.shape.n_head, "q", None)
-        op, os = self._rows(out, self.shape.n_head, "out", q.dtype)
+        act = self._act(q, "q")
+        qp, qs = self._rows(q, self._widths[0], "q", q.dtype)
+        op, os = self._rows(out, self._widths[0], "out", q.dtype)
         pool = self.cache.pool()
-        st = self._on(stream)
-        with torch.cuda.device(self.device):
-            _check(lib().tle_prefill_bf16_paged(ctypes.byref(self.shape), ctypes.addressof(pool),
-                                                ctypes.byref(self.plan), self._desc_dev.data_ptr(), qp, qs,
-                                                op, os, int(q.dtype == torch.bfloat16), layer,
-                                                self.workspace.data_ptr(), self.workspace.numel() * 4, st))
+        _on_device(self._index, lib().tle_prefill_bf16_paged, self._shape_ref, ctypes.addressof(pool),
+                   ctypes.byref(self.plan), self._desc_dev.data_ptr(), qp, qs, op, os, act, layer,
+                   self.workspace.data_ptr(), self.workspace.numel() * 4, self._on(stream))
 
     def run(self, q, k, v, out, layer: int, rotate: bool = True, stream=None) -> None:
         """append, then attend: the attention block of one layer for every
@@ -958,11 +990,13 @@ class LogitRules:
                 raise ValueError("allowed: need int32 CUDA words [n_rows][>= n_vocab / 32], rows contiguous")
             self._same(allowed, "allowed")
             stride = allowed.stride(0) if n_rows > 1 else allowed.shape[1]
+        self.index = None if self.device is None else self.device.index
         self.keep = [*given.values(), allowed]
         one = lambda t: None if t is None else (t.data_ptr() or None)  # noqa: E731
         self.desc = LogitRulesDesc(*[one(given[n]) for n, _ in self._GROUPS], one(allowed), stride,
                                    0 if tokens is None else tokens.numel(),
                                    0 if bias_tokens is None else bias_tokens.numel())
+        self.desc_ref = ctypes.byref(self.desc)
         if tokens is not None and tokens.numel() == 0:          # an empty list: no penalties
             for n in ("tokens", "repetition", "frequency", "presence"):
                 setattr(self.desc, n, None)
@@ -979,18 +1013,18 @@ def logits_adjust(out, logits, rules: LogitRules, stream=None) -> None:
     stride; out may be logits.  Before sample_argmax / sample_temperature /
     sample_top_p."""
     import torch
+    n, v = rules.n_rows, rules.n_vocab
+    index = rules.index if rules.index is not None else logits.get_device()
+    at = []
     for t, name in ((out, "out"), (logits, "logits")):
-        if t.dtype != torch.float32 or not t.is_cuda or tuple(t.shape) != (rules.n_rows, rules.n_vocab) or \
-                (rules.n_vocab > 1 and t.stride(1) != 1):
-            raise ValueError(f"{name}: need float32 CUDA [{rules.n_rows}][{rules.n_vocab}], rows contiguous")
-        if t.device != (rules.device or logits.device):
-            raise ValueError(f"{name}: is on {t.device}, the rules on {rules.device or logits.device}")
-    if stream is not None and stream.device != logits.device:
-        raise ValueError(f"stream of {stream.device}, tensors on {logits.device}")
-    rows = lambda t: t.stride(0) if rules.n_rows > 1 else rules.n_vocab  # noqa: E731
-    with torch.cuda.device(logits.device):
-        _check(lib().tle_logits_adjust(out.data_ptr(), rows(out), logits.data_ptr(), rows(logits), rules.n_rows,
-                                       rules.n_vocab, ctypes.byref(rules.desc), _stream(stream)))
+        shape, strides = t.shape, t.stride()
+        if t.dtype is not torch.float32 or not t.is_cuda or len(shape) != 2 or shape[0] != n or shape[1] != v or \
+                (v > 1 and strides[1] != 1):
+            raise ValueError(f"{name}: need float32 CUDA [{n}][{v}], rows contiguous")
+        if t.get_device() != index:
+            raise ValueError(f"{name}: is on {t.device}, the rules on cuda:{index}")
+        at += [t.data_ptr(), strides[0] if n > 1 else v]
+    _on_device(index, lib().tle_logits_adjust, *at, n, v, rules.desc_ref, _raw_stream(stream, index))
 
 
 class DeviceModel:
