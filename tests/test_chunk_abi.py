@@ -9,7 +9,7 @@ import pytest
 
 import tle
 
-TILE, ITEM, FEW = 128, 256, 64
+TILE, ITEM, FEW = 128, 256, 32
 P = 0x400000
 
 

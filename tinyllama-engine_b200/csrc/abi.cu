@@ -1450,9 +1450,9 @@ int check_chunks(const tle_shape_t* shape, int page_rows, const tle_paged_chunk_
 // chains do the whole tile) and 1 for one in between (each does half of it).
 // A segment has a fixed cost (Q load, joining and storing the result).
 constexpr int64_t kSegUnits = 4, kFewSegUnits = 2;
-constexpr int64_t kJoinUnits = 8;             // partial results of cut items, and the launch that joins them
+constexpr int64_t kJoinUnits = 16;            // partial results of cut items, and the launch that joins them
 constexpr int64_t kMaxWholeItems = 4096;    // sorted on the host, a few tenths of a millisecond
-constexpr int64_t kMinPieceUnits = 4, kFewMinPieceUnits = 2;   // smallest piece of an item worth a CTA of its own
+constexpr int64_t kMinPieceUnits = 2, kFewMinPieceUnits = 1;   // smallest piece of an item worth a CTA of its own
 
 struct ChunkPlanner {
     const tle_shape_t* shape;

@@ -1111,7 +1111,7 @@ __global__ void __launch_bounds__(CT_THREADS, 1)
 // and the treatment of rows that not every token attends to as above.
 constexpr int FW_WARPS = 8;
 constexpr int FW_THREADS = 32 * (FW_WARPS + 1);
-constexpr int FW_STAGES = 5;
+constexpr int FW_STAGES = 4;
 constexpr int kFewFlush = 8;        // fp32: tiles (of one row group) whose MMAs are summed in a row
 struct FewSmem {
     uint16_t k[FW_STAGES][kTileHalfs];

@@ -351,7 +351,7 @@ cudaError_t launch_embed_rows(int type, float* x, const void* table, const int32
 constexpr int kChunkTile = 128;       // K/V rows per tile
 constexpr int kChunkRows = 128;       // rows per tensor-core tile
 constexpr int kChunkItemRows = 2 * kChunkRows;
-constexpr int kChunkFewRows = 64;
+constexpr int kChunkFewRows = 32;
 constexpr int32_t kChunkMagic = 0x544c4543;  // "TLEC"
 struct ChunkHeader {
     int32_t magic, n_seqs, n_tokens, n_ctas, n_segs, n_merge, n_few_ctas, reserved;
