@@ -354,29 +354,37 @@ typedef struct {
     int32_t n_segs;                /* their pieces of work                             */
     int32_t n_merge, merge_rows;   /* row blocks split over pieces; rows of the largest */
     int64_t part_rows;             /* partial result rows in the workspace             */
+    int64_t desc_bytes;            /* bytes of the descriptor                          */
 } tle_chunk_plan_t;
 
-/* Bytes that suffice for the descriptor of such a batch (0: bad arguments,
- * see tle_last_error). */
+/* Bytes that suffice for the descriptor of such a batch, at any positions (0:
+ * bad arguments, see tle_last_error). */
 size_t tle_chunk_desc_bytes(const tle_shape_t* shape, const tle_paged_chunk_t* chunks, int n_seqs,
                             int max_ctas);
 
 /* Builds the descriptor in HOST memory from host-side chunk records (the page
  * tables stay on the device): the place of every token, and the attention's
  * work split evenly over about one CTA per SM (max_ctas > 0: at most that
- * many).  The caller copies desc_host to device memory unchanged (16-byte
- * aligned).  At most 2^31 - 1 rows of q heads per chunk and tokens in all. */
+ * many).  desc_host is 8-byte aligned; the caller copies its first
+ * plan->desc_bytes bytes to device memory (16-byte aligned) unchanged.
+ *
+ * The calls below check on the device that the descriptor is the one of their
+ * plan; otherwise they do nothing and 0x10b is reported.  So a captured call
+ * may be replayed after the descriptor was replaced only if the new plan has
+ * the same numbers (the pages, and positions that leave the split as it was,
+ * may differ). */
 int tle_chunk_desc_paged(const tle_shape_t* shape, int page_rows, const tle_paged_chunk_t* chunks,
                          int n_seqs, int max_ctas, void* desc_host, size_t desc_bytes,
                          tle_chunk_plan_t* plan);
 
 /* For every token i of the batch, at position p: if flags & TLE_DECODE_ROTATE,
  * rope(q_i, k_i, p) with the decode's angles; q_out_i = q_i in the type of q
- * (fp32 or bf16); row p of its sequence in layer `layer` of the pools = k_i,
+ * (act_type, TLE_ACT_*); row p of its sequence in layer `layer` of the pools = k_i,
  * v_i, rounded once to the pool's type.  q and q_out may both be NULL (k and
  * v only) and may be the same buffer.  Row i of q is at q + i * q_stride
  * elements, likewise k and v; strides are multiples of 8, at least the row's
- * n_head * 64 (n_head_kv * 64) elements; q_out is packed.  Two tokens of a
+ * n_head * 64 (n_head_kv * 64) elements; q_out is packed; all pointers are
+ * 16-byte aligned.  Two tokens of a
  * batch must not share a row of the pools.  A page id outside the pool is not
  * dereferenced (0x105, its rows are not stored); a batch without tokens does
  * nothing.  Other flag bits are rejected with TLE_ERR_INVALID. */
@@ -404,7 +412,7 @@ size_t tle_prefill_bf16_paged_workspace_bytes(const tle_chunk_plan_t* plan);
  * bf16 rows.  Rows of the pools that no token attends to are never part of a
  * result, whatever they hold.  A page id outside the pool is not dereferenced
  * (0x105, its rows count as zeros).  out rows behind the last token are left
- * as they are.  Calls that share a workspace must not overlap on the GPU. */
+ * as they are.  out may be q, with the same stride.  Calls that share a workspace must not overlap on the GPU. */
 int tle_prefill_bf16_paged(const tle_shape_t* shape, const tle_page_pool_bf16_t* pool,
                            const tle_chunk_plan_t* plan, const void* desc_dev, const void* q,
                            int64_t q_stride, void* out, int64_t out_stride, int act_type, int layer,
@@ -423,11 +431,12 @@ int tle_partition_lpt(const int32_t* lengths, int n_seqs, int n_ranks, int32_t* 
 /* Reads (and clears if clear != 0) the device error word that kernels set;
  * 0 = no error.  Codes: 0x101-0x104 a bounded wait expired (0x101 a stage
  * never filled, 0x102 never drained, 0x103 a tensor-core commit never
- * arrived, 0x104 the exit-time drain), 0x105 a paged decode met a page id
+ * arrived, 0x104 the exit-time drain), 0x105 a paged call met a page id
  * outside the pool, 0x106 a token id outside the vocabulary, 0x108 a grid
  * barrier wait of the one-launch forward expired, 0x109 a finite activation
  * of the batched prompt overflowed fp16, 0x10a a bf16 or short-batch decode
- * record outside its cache or max_rows, 0x1ff the self-test below.  The first code recorded
+ * record outside its cache or max_rows, 0x10b a chunk call met the descriptor of
+ * another plan than its own (it did nothing), 0x1ff the self-test below.  The first code recorded
  * stays until cleared.  Synchronises the device. */
 int tle_device_error(int clear, uint32_t* code);
 

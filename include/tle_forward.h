@@ -103,8 +103,8 @@ typedef struct {
      * allowed[r * allowed_stride + t / 32] is set; otherwise its logit
      * becomes -inf, whatever it was. */
     const uint32_t* allowed;
-    int64_t allowed_stride;     /* words, >= ceil(n_vocab / 32) */
-    int32_t n_tokens, n_biases; /* entries of the two lists: starts and ends are cut to them */
+    int64_t allowed_stride;     /* words, >= ceil(n_vocab / 32), or 0: one mask for all rows */
+    int32_t n_tokens, n_biases; /* entries of the two lists, <= 2^30: starts and ends are cut to them */
 } tle_logit_rules_t;
 
 /* out[r][t] = logits[r][t] under row r's rules, in the order repetition,

@@ -26,7 +26,8 @@ def describe(pos, new, heads=(32, 4), page=64, max_ctas=0, n_pages=None, table=l
     buf = np.zeros((nbytes + 7) // 8, np.int64)
     rc = tle.lib().tle_chunk_desc_paged(ctypes.byref(shape), page, c, n, max_ctas, buf.ctypes.data, nbytes,
                                         ctypes.byref(plan))
-    return rc, buf.view(np.uint8)[:nbytes], plan
+    assert rc != 0 or plan.desc_bytes <= nbytes
+    return rc, buf.view(np.uint8)[:plan.desc_bytes], plan
 
 
 def parse(buf, plan):
@@ -103,6 +104,24 @@ def test_plan_balances_long_work():
     _, segs, _, _, start, _ = parse(buf, plan)
     cost = [sum(2 * (x[5] - x[4]) for x in segs[a:b]) for a, b in zip(start, start[1:])]
     assert plan.n_ctas == 148 and max(cost) <= sum(cost) / 148 + 16
+
+
+def test_desc_buffer_size_and_plan_number():
+    """A buffer of the stated size does at any positions, a smaller one than
+    needed is refused; the number that the calls check differs between plans."""
+    shape = tle.Shape(2, 32, 4, 64, 10000.0)
+    c, plan, numbers = (tle.PagedChunk * 3)(), tle.ChunkPlan(), set()
+    for pos in ([0, 0, 0], [5000, 1, 300], [5001, 1, 300], [9000, 9000, 9000]):
+        for i, new in enumerate((300, 1, 20)):
+            c[i] = tle.PagedChunk(0x4000, 500, pos[i], new, 0)
+        nbytes = tle.lib().tle_chunk_desc_bytes(ctypes.byref(shape), c, 3, 0)
+        buf = np.zeros(nbytes // 8 + 1, np.int64)
+        go = lambda size, at=0: tle.lib().tle_chunk_desc_paged(  # noqa: E731
+            ctypes.byref(shape), 64, c, 3, 0, buf.ctypes.data + at, size, ctypes.byref(plan))
+        assert go(nbytes) == tle.TLE_OK and go(plan.desc_bytes) == tle.TLE_OK
+        numbers.add((int(buf[0]), plan.n_segs, plan.n_merge, plan.part_rows, plan.n_ctas, plan.n_few_ctas))
+        assert go(plan.desc_bytes - 1) == tle.TLE_ERR_INVALID and go(plan.desc_bytes, 4) == tle.TLE_ERR_INVALID
+    assert len({x[0] for x in numbers}) == len({x[1:] for x in numbers}) > 1
 
 
 def test_empty_batches():
@@ -195,6 +214,9 @@ def test_logit_rules_refuse_bad_arguments():
     assert go(os=99) == bad and go(xs=99) == bad and go(os=104) == bad
     assert go(tokens=P) == bad and go(repetition=P) == bad and go(presence=P, token_start=P) == bad
     assert go(bias_tokens=P) == bad and go(bias_tokens=P, bias_values=P) == bad
-    assert go(allowed=P, allowed_stride=3) == bad
+    assert go(allowed=P, allowed_stride=3) == bad and go(allowed=P, allowed_stride=-4) == bad
+    assert go(out=P + 2) == bad and go(x=P + 1) == bad and go(tokens=P + 2, token_start=P, frequency=P) == bad
+    assert go(tokens=P, token_start=P, frequency=P + 2) == bad and go(allowed=P + 2, allowed_stride=4) == bad
+    assert go(tokens=P, token_start=P, n_tokens=(1 << 30) + 1) == bad
     assert go(tokens=P, token_start=P, n_tokens=-1) == bad
     assert L.tle_logits_adjust(P, 100, P, 100, 2, 100, None, None) == bad

@@ -281,6 +281,155 @@ def test_attend_is_reproducible_and_replays(cuda, act):
         assert torch.equal(got, c.out)
 
 
+@pytest.mark.parametrize("pos,new", [([700, 50, 1300], [40, 9, 1]), ([5000, 20], [70, 2])])
+def test_a_replay_under_another_plan_does_nothing(cuda, pos, new):
+    """A captured call whose descriptor was replaced: 0x10b, and neither pools
+    nor results change; under a plan with the same numbers it is right."""
+    import torch
+    import tle
+    c = Case(pos, new, seed=13)
+    c.batch.run(c.q, c.k, c.v, c.out, c.layer)          # the buffer of the rotated q
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        c.batch.run(c.q, c.k, c.v, c.out, c.layer)
+    plan = bytes(c.batch.plan)
+    c.batch.set_positions([p - 1 for p in pos], new)
+    assert bytes(c.batch.plan) == plan
+    graph.replay()
+    torch.cuda.synchronize()
+    got = c.out.clone()
+    c.out.fill_(3)
+    c.batch.run(c.q, c.k, c.v, c.out, c.layer)
+    torch.cuda.synchronize()
+    assert torch.equal(got, c.out) and tle.device_error() == 0
+    refused = 0
+    for other in ([0] * len(pos), [p // 3 for p in pos]):
+        c.batch.set_positions(other, new)
+        pools = (c.cache.key_pool.clone(), c.cache.value_pool.clone())
+        c.out.fill_(3)
+        graph.replay()
+        torch.cuda.synchronize()
+        if bytes(c.batch.plan) == plan:                 # the split may be the same there too
+            got = c.out.clone()
+            c.batch.run(c.q, c.k, c.v, c.out, c.layer)
+            torch.cuda.synchronize()
+            assert torch.equal(got, c.out) and tle.device_error() == 0
+            continue
+        refused += 1
+        assert tle.device_error() == 0x10b
+        assert bool((c.out == 3).all())
+        assert torch.equal(pools[0], c.cache.key_pool) and torch.equal(pools[1], c.cache.value_pool)
+    assert refused
+    c.out.fill_(3)
+    c.batch.set_positions(pos, [1] * len(pos))          # fewer tokens
+    graph.replay()
+    torch.cuda.synchronize()
+    assert tle.device_error() == 0x10b and bool((c.out == 3).all())
+
+
+@pytest.mark.parametrize("act", ["f32", "bf16"])
+@pytest.mark.parametrize("pos,new,bad", [([700, 50, 1300], [40, 9, 1], None), ([9000], [100], None), ([0, 4000], [600, 3], None),
+                                         ([120, 40], [150, 3], 200)])
+def test_attend_in_place(cuda, act, pos, new, bad):
+    """out is q, with items cut over several CTAs and rows computed again."""
+    import torch
+    c = Case(pos, new, act=act, seed=14)
+    if bad is not None:
+        c.cache.value_pool.view(c.layers, -1, c.KH * HD)[c.layer, int(c.flat_rows(0, np.array([bad]))[0])] = float("inf")
+    c.batch.attend(c.q, c.out, c.layer)
+    c.batch.attend(c.q, c.q, c.layer)
+    torch.cuda.synchronize()
+    assert torch.equal(c.q.nan_to_num(9.0), c.out.nan_to_num(9.0))
+
+
+@pytest.mark.parametrize("new", [1, 4, 64])
+def test_long_fp32_sums_do_not_drift(cuda, new):
+    """All rows of V positive, so that sums that are cut off instead of rounded
+    drift.  Each of at most 48 MMAs between two rounded sums loses up to 2^-23
+    of the sum, the 16000 / 256 rounded ones (16 pieces and 16 joins more) up to
+    2^-24 each; a score is 12 MMAs' sum of |q k| / 8 off by 2^-23 each, its
+    weight and their sum by that and by 2^-22 and |s| 2^-23."""
+    import torch
+    c = Case([16000], [new], heads=(8, 2), seed=15, scale=0.1)
+    c.cache.value_pool.abs_()
+    c.batch.attend(c.q, c.out, c.layer)
+    want = torch.empty(new, c.H * HD, dtype=torch.float64, device="cuda")
+    rows = torch.from_numpy(c.flat_rows(0, np.arange(16000 + new))).cuda()
+    size = 0.0
+    for h in range(c.H):
+        sl = slice(h // 4 * HD, (h // 4 + 1) * HD)
+        k = c.cache.key_pool[c.layer].view(-1, c.KH * HD)[rows, sl].double()
+        v = c.cache.value_pool[c.layer].view(-1, c.KH * HD)[rows, sl].double()
+        q = c.q[:, h * HD:(h + 1) * HD].double()
+        hide = torch.arange(16000 + new, device="cuda")[None, :] > 16000 + torch.arange(new, device="cuda")[:, None]
+        w = torch.softmax((q @ k.T / 8).masked_fill(hide, -float("inf")), 1)
+        want[:, h * HD:(h + 1) * HD] = w @ v
+        size = max(size, float((q.abs() @ k.abs().T / 8).max()))
+    tol = 48 * 2.0 ** -23 + (16000 / 256 + 32) * 2.0 ** -24 + 2 * (12 * size * 2.0 ** -23 + 2.0 ** -22 + size * 2.0 ** -23)
+    assert float(((c.out.double() - want).abs() / want).max()) <= tol
+
+
+def test_tensors_are_checked(cuda):
+    import torch
+    import tle
+    c = Case([100, 20], [3, 4])
+    b, T = c.batch, c.T
+    f = lambda *s, dt=torch.float32: torch.zeros(s, dtype=dt, device="cuda")  # noqa: E731
+    bf = torch.bfloat16
+    for q, out in ((c.q.cpu(), c.out), (c.q, c.out.cpu()), (c.q.to(bf), c.out), (c.q, c.out.to(bf)), (c.q.double(), c.out.double()),
+                   (c.q[:T - 1], c.out), (c.q, c.out[:T - 1]), (c.q[:, :-64], c.out), (f(2048, T).T, c.out), (c.q.flatten(), c.out)):
+        with pytest.raises(ValueError):
+            b.attend(q, out, 0)
+    for q, out, layer in ((f(T, 2052)[:, :2048], c.out, 0), (c.q, f(1, 2048).expand(T, 2048), 0), (c.q, c.out, 2), (c.q, c.out, -1),
+                          (f(T * 2048 + 2)[2:].view(T, 2048), c.out, 0), (c.q, f(T * 2048 + 1)[1:].view(T, 2048), 0)):
+        with pytest.raises(tle.TleError):
+            b.attend(q, out, layer)
+    for q, k, v, qo in ((c.q, c.k, c.v, None), (None, c.k, c.v, c.q), (c.q, c.k, c.v.to(bf), c.q), (c.q, c.k[:, :-64], c.v, c.q),
+                        (c.q, c.k, c.v, f(T, 2112)[:, :2048]), (c.q.to(bf), c.k, c.v, c.q)):
+        with pytest.raises(ValueError):
+            b.append(q, k, v, 0, q_out=qo)
+    plain = tle.PagedKVCache(8, 64, c.cache.shape)
+    with pytest.raises(ValueError):
+        tle.PagedChunkBatch(plain, c.tables, [0, 0], [1, 1]).attend(c.q, c.out, 0)
+    with pytest.raises(ValueError):
+        tle.PagedChunkBatch(plain, [t.long() for t in c.tables], [0, 0], [1, 1])
+    with pytest.raises(ValueError):
+        tle.PagedChunkBatch(plain, [t.cpu() for t in c.tables], [0, 0], [1, 1])
+    with pytest.raises(ValueError):
+        tle.PagedChunkBatch(plain, c.tables, [0], [1, 1])
+    with pytest.raises(tle.TleError):
+        tle.PagedChunkBatch(c.cache, c.tables, [1000, 0], [1, 1])
+    with pytest.raises(ValueError):
+        tle.PagedKVCache(8, 64, c.cache.shape, pools=(plain.key_pool, plain.value_pool[:, :4]))
+    with pytest.raises(ValueError):
+        tle.PagedKVCache(8, 64, c.cache.shape, dtype=bf, pools=(plain.key_pool, plain.value_pool))
+    given = tle.PagedKVCache(8, 64, c.cache.shape, pools=(plain.key_pool, plain.value_pool))
+    assert given.key_pool.data_ptr() == plain.key_pool.data_ptr()
+
+
+def test_buffers_outlive_work_on_another_stream(cuda):
+    """A batch that is dropped while its call waits on a stream of its own:
+    what the allocator hands out next does not reach that call."""
+    import torch
+    import tle
+    c = Case([3000, 40], [60, 2], seed=16)
+    want = torch.zeros_like(c.out)
+    c.batch.attend(c.q, want, c.layer)
+    side = torch.cuda.Stream()
+    gate = torch.randn(4096, 4096, device="cuda")
+    torch.cuda.synchronize()
+    with torch.cuda.stream(side):
+        for _ in range(40):
+            gate = gate @ gate * 1e-2          # keeps the stream busy
+        c.batch.attend(c.q, c.out, c.layer)
+    sizes = [(t.numel(), t.dtype) for t in (c.batch._desc_dev, c.batch.workspace)]
+    c.batch = None
+    for n, dt in sizes * 4:
+        torch.full((n,), 77, dtype=dt, device="cuda")
+    torch.cuda.synchronize()
+    assert torch.equal(c.out, want) and tle.device_error() == 0
+
+
 def test_set_positions_replans(cuda):
     """The same batch object over growing contexts and other chunk lengths."""
     c = Case([900, 60, 3000], [300, 200, 400], seed=10)

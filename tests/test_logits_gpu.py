@@ -177,6 +177,59 @@ def test_non_finite_logits_and_a_row_that_allows_nothing(cuda):
     assert bool((out[2][bits == 0] == -float("inf")).all())
 
 
+@pytest.mark.parametrize("biases", [3, 200])
+def test_a_bias_does_not_lift_the_mask(cuda, biases):
+    """-inf where the mask says so, under an infinite or NaN bias too."""
+    import torch
+    import tle
+    V = 90
+    ids = np.arange(biases, dtype=np.int32) % V
+    b = np.resize(np.array([np.inf, np.nan, -np.inf], np.float32), biases)
+    words = np.full((1, 3), 0b1000, np.int32)          # every 32nd token from 3 on
+    R = tle.LogitRules(1, V, bias_tokens=dev(ids), bias_values=dev(b), bias_start=dev(np.array([0, biases], np.int32)),
+                       allowed=dev(words))
+    out = torch.zeros(1, V, device="cuda")
+    tle.logits_adjust(out, torch.ones(1, V, device="cuda"), R)
+    ok = torch.arange(V, device="cuda") % 32 == 3
+    assert bool((out[0][~ok] == -float("inf")).all())
+    assert not bool((out[0][ok] == -float("inf")).all())
+
+
+def test_one_mask_for_all_rows(cuda):
+    import torch
+    import tle
+    c = make(5, 700, 60, seed=11, biases=8, mask=True)
+    shared = dev(c["allowed"][:1])
+    R = tle.LogitRules(5, 700, **{k: dev(c[k]) for k in KEYS if k in c and k != "allowed"}, allowed=shared.expand(5, -1))
+    out = torch.empty(5, 700, device="cuda")
+    tle.logits_adjust(out, dev(c["x"]), R)
+    c["allowed"] = np.repeat(c["allowed"][:1], 5, 0)
+    check(c, out)
+
+
+def test_rules_and_tensors_are_checked(cuda):
+    import torch
+    import tle
+    i32 = lambda *x: torch.tensor(x, dtype=torch.int32, device="cuda")  # noqa: E731
+    f32 = lambda *x: torch.tensor(x, dtype=torch.float32, device="cuda")  # noqa: E731
+    ok = dict(tokens=i32(1, 2, 3), token_start=i32(0, 1, 3), repetition=f32(1, 2))
+    tle.LogitRules(2, 50, **ok)
+    for bad in (dict(tokens=ok["tokens"].long()), dict(tokens=ok["tokens"].cpu()), dict(token_start=i32(0, 3)),
+                dict(token_start=None), dict(tokens=None), dict(repetition=f32(1)), dict(repetition=f32(1, 2).double()),
+                dict(tokens=i32(1, 2, 3, 4)[::2]), dict(n_prompt=i32(1, 2, 3)), dict(bias_tokens=i32(1)),
+                dict(bias_tokens=i32(1), bias_values=f32(1, 2), bias_start=i32(0, 1, 1)),
+                dict(allowed=i32(1, 2)), dict(allowed=torch.zeros(2, 1, dtype=torch.int32, device="cuda")),
+                dict(allowed=torch.zeros(2, 4, dtype=torch.int32, device="cuda")[:, ::2])):
+        with pytest.raises(ValueError):
+            tle.LogitRules(2, 50, **{**ok, **bad})
+    R = tle.LogitRules(2, 50, **ok)
+    x = torch.zeros(2, 50, device="cuda")
+    for a, b in ((x[:1], x), (x, x[:, :49]), (x.double(), x), (x, x.cpu()), (torch.zeros(50, 2, device="cuda").T, x),
+                 (torch.zeros(1, 50, device="cuda").expand(2, 50), x)):
+        with pytest.raises((ValueError, tle.TleError)):
+            tle.logits_adjust(a, b, R)
+
+
 def test_bad_ids_are_skipped_and_reported(cuda):
     import torch
     import tle

@@ -1448,11 +1448,19 @@ int check_chunks(const tle_shape_t* shape, int page_rows, const tle_paged_chunk_
 // of chunks of at most kChunkFewRows rows, and the others.  Costs in units: a K/V tile
 // costs 1 for the few rows; 2 for an item of more than kChunkRows rows (both
 // chains do the whole tile) and 1 for one in between (each does half of it).
-// A segment has a fixed cost (Q load, joining and storing the result).
+// A segment has a fixed cost (Q load, joining and storing the result).  Times
+// below: 32 query on 4 KV heads, 148 CTAs.
 constexpr int64_t kSegUnits = 4, kFewSegUnits = 2;
-constexpr int64_t kJoinUnits = 16;            // partial results of cut items, and the launch that joins them
+// How far above the even share the longest CTA may be before items are cut:
+// what the partial results and the launch that joins them cost.  6 x 509 tokens
+// behind 1999 rows, bf16: 67.2 us with 16, 73.7 us with 8 (cut); 3 x 300 tokens
+// behind 4000 rows, fp32: 79 us with 16 (cut), 93 us with 32.
+constexpr int64_t kJoinUnits = 16;
 constexpr int64_t kMaxWholeItems = 4096;    // sorted on the host, a few tenths of a millisecond
-constexpr int64_t kMinPieceUnits = 2, kFewMinPieceUnits = 1;   // smallest piece of an item worth a CTA of its own
+// Smallest piece of an item worth a CTA of its own.  5 tokens behind 2000 rows
+// (40 rows per KV head): bf16 9.5 us with 2, 10.9 us with 4; fp32 13.2 and 14.4 us.
+// Few rows, 5 tokens of 4 rows each behind 700 rows: 12.7 us with 1, 14.4 us with 2.
+constexpr int64_t kMinPieceUnits = 2, kFewMinPieceUnits = 1;
 
 struct ChunkPlanner {
     const tle_shape_t* shape;
@@ -1646,6 +1654,7 @@ int append_common(const tle_shape_t* shape, const tle_chunk_plan_t* plan, const 
     if (int rc = check_rows(v, v_stride, shape->n_head_kv, "v")) return rc;
     tle::AppendArgs a{};
     a.d = tle::chunk_desc(desc_dev, plan->n_seqs, plan->n_segs, plan->n_merge, plan->n_tokens, plan->n_ctas);
+    a.plan_id = tle::chunk_plan_id(*plan);
     a.n_tokens = plan->n_tokens;
     a.q = q;
     a.k = k;
@@ -1674,63 +1683,71 @@ int append_common(const tle_shape_t* shape, const tle_chunk_plan_t* plan, const 
 
 extern "C" {
 
-size_t tle_chunk_desc_bytes(const tle_shape_t* shape, const tle_paged_chunk_t* chunks, int n_seqs, int max_ctas) try {
+size_t tle_chunk_desc_bytes(const tle_shape_t* shape, const tle_paged_chunk_t* chunks, int n_seqs, int max_ctas) {
     if (check_chunks(shape, 0, chunks, n_seqs)) return 0;
-    const ChunkPlanner p{shape, chunks, n_seqs, chunk_ctas(max_ctas)};
-    size_t segs = 0, merges = 0, tokens = 0, ctas[2];
-    for (int few = 0; few < 2; ++few)
-        ctas[few] = p.run(few, [&](int, const ChunkPlanner::Item&, int, int, int, int) { ++segs; },
-                          [&](const ChunkPlanner::Item&, int) { ++merges; });
-    for (int s = 0; s < n_seqs; ++s) tokens += static_cast<size_t>(chunks[s].n_tokens);
-    return tle::chunk_desc_bytes(n_seqs, segs, merges, tokens, ctas[0], ctas[1]);
-} catch (const std::exception& e) {   // the planner's lists: out of host memory
-    set_error(TLE_ERR_INVALID, "chunk plan: %s", e.what());
-    return 0;
+    // a bound that needs no plan: cuts add at most a piece per CTA to an item each
+    const size_t g = static_cast<size_t>(shape->n_head / shape->n_head_kv), G = static_cast<size_t>(chunk_ctas(max_ctas));
+    size_t tokens = 0, items = 0;
+    for (int s = 0; s < n_seqs; ++s) {
+        tokens += static_cast<size_t>(chunks[s].n_tokens);
+        items += (chunks[s].n_tokens * g + tle::kChunkItemRows - 1) / tle::kChunkItemRows;
+    }
+    return tle::chunk_desc_bytes(n_seqs, items * shape->n_head_kv + 2 * G, 2 * G, tokens, G, G);
 }
 
 int tle_chunk_desc_paged(const tle_shape_t* shape, int page_rows, const tle_paged_chunk_t* chunks, int n_seqs,
                          int max_ctas, void* desc_host, size_t desc_bytes, tle_chunk_plan_t* plan) try {
     if (!desc_host || !plan) return set_error(TLE_ERR_INVALID, "desc_host and plan must be non-null");
+    if ((reinterpret_cast<uintptr_t>(desc_host) & 7u) != 0)
+        return set_error(TLE_ERR_INVALID, "desc_host must be 8-byte aligned");
     if (page_rows < 16 || page_rows > 65536 || (page_rows & (page_rows - 1)) != 0)
         return set_error(TLE_ERR_INVALID, "page_rows %d is not a power of two in [16, 65536]", page_rows);
     if (int rc = check_chunks(shape, page_rows, chunks, n_seqs)) return rc;
     const ChunkPlanner p{shape, chunks, n_seqs, chunk_ctas(max_ctas)};
+    std::vector<tle::ChunkSeg> segs;
+    std::vector<tle::ChunkMerge> merges;
+    std::vector<int32_t> start[2];   // first piece of each CTA of the two kernels
+    int64_t part = 0;
+    int merge_rows = 0;
+    for (int few = 0; few < 2; ++few) {
+        const int n = p.run(
+            few,
+            [&](int cta, const ChunkPlanner::Item& it, int t0, int t1, int parts, int before) {
+                start[few].resize(std::max<size_t>(start[few].size(), cta + 1), static_cast<int32_t>(segs.size()));
+                segs.push_back(tle::ChunkSeg{it.seq, it.kvh, it.row0, it.n_rows, t0, t1,
+                                             parts > 1 ? static_cast<int32_t>(part + before * it.n_rows) : -1, 0});
+            },
+            [&](const ChunkPlanner::Item& it, int parts) {
+                merges.push_back(tle::ChunkMerge{it.seq, it.kvh, it.row0, it.n_rows, static_cast<int32_t>(part), parts});
+                part += static_cast<int64_t>(parts) * it.n_rows;
+                merge_rows = std::max(merge_rows, it.n_rows);
+            });
+        start[few].resize(n + 1, static_cast<int32_t>(segs.size()));
+    }
+    if (segs.size() > INT32_MAX / 2 || part > INT32_MAX / 2)
+        return set_error(TLE_ERR_UNSUPPORTED, "batch too large (%zu pieces)", segs.size());
     tle_chunk_plan_t out{};
-    int64_t segs = 0, merges = 0, part_rows = 0;
-    int merge_rows = 0, ctas[2];
-    for (int few = 0; few < 2; ++few)
-        ctas[few] = p.run(few, [&](int, const ChunkPlanner::Item&, int, int, int, int) { ++segs; },
-                          [&](const ChunkPlanner::Item& it, int parts) {
-                              ++merges;
-                              part_rows += static_cast<int64_t>(parts) * it.n_rows;
-                              merge_rows = std::max(merge_rows, it.n_rows);
-                          });
     int64_t tokens = 0;
     for (int s = 0; s < n_seqs; ++s) tokens += chunks[s].n_tokens;
-    if (segs > INT32_MAX / 2 || part_rows > INT32_MAX / 2)
-        return set_error(TLE_ERR_UNSUPPORTED, "batch too large (%lld pieces)", static_cast<long long>(segs));
     out.n_seqs = n_seqs;
     out.n_tokens = static_cast<int32_t>(tokens);
     out.n_head = shape->n_head;
     out.n_head_kv = shape->n_head_kv;
     out.page_rows = page_rows;
-    out.n_ctas = ctas[0];
-    out.n_few_ctas = ctas[1];
-    out.n_segs = static_cast<int32_t>(segs);
-    out.n_merge = static_cast<int32_t>(merges);
+    out.n_ctas = static_cast<int32_t>(start[0].size()) - 1;
+    out.n_few_ctas = static_cast<int32_t>(start[1].size()) - 1;
+    out.n_segs = static_cast<int32_t>(segs.size());
+    out.n_merge = static_cast<int32_t>(merges.size());
     out.merge_rows = merge_rows;
-    out.part_rows = part_rows;
-    const size_t need = tle::chunk_desc_bytes(n_seqs, segs, merges, tokens, ctas[0], ctas[1]);
+    out.part_rows = part;
+    const size_t need = tle::chunk_desc_bytes(n_seqs, segs.size(), merges.size(), tokens, out.n_ctas, out.n_few_ctas);
+    out.desc_bytes = static_cast<int64_t>(need);
     if (desc_bytes < need)
         return set_error(TLE_ERR_INVALID, "descriptor buffer %zu bytes < %zu needed", desc_bytes, need);
-    if ((reinterpret_cast<uintptr_t>(desc_host) & 7u) != 0)
-        return set_error(TLE_ERR_INVALID, "desc_host must be 8-byte aligned");
     auto* hdr = static_cast<tle::ChunkHeader*>(desc_host);
-    *hdr = tle::ChunkHeader{tle::kChunkMagic, n_seqs, out.n_tokens, out.n_ctas, out.n_segs, out.n_merge, out.n_few_ctas, 0};
-    const tle::ChunkDesc d = tle::chunk_desc(desc_host, n_seqs, segs, merges, tokens, ctas[0]);
+    *hdr = tle::ChunkHeader{tle::chunk_plan_id(out), n_seqs, out.n_tokens, out.n_ctas, out.n_few_ctas, out.n_segs, out.n_merge};
+    const tle::ChunkDesc d = tle::chunk_desc(desc_host, n_seqs, segs.size(), merges.size(), tokens, out.n_ctas);
     auto* seq = const_cast<tle::ChunkSeq*>(d.seqs);
-    auto* seg = const_cast<tle::ChunkSeg*>(d.segs);
-    auto* mrg = const_cast<tle::ChunkMerge*>(d.merges);
     auto* tok = const_cast<tle::ChunkTok*>(d.toks);
     int32_t first = 0;
     for (int s = 0; s < n_seqs; ++s) {
@@ -1739,26 +1756,13 @@ int tle_chunk_desc_paged(const tle_shape_t* shape, int page_rows, const tle_page
         for (int t = 0; t < c.n_tokens; ++t) tok[first + t] = tle::ChunkTok{s, c.pos + t};
         first += c.n_tokens;
     }
-    int32_t part = 0, at = 0;
-    for (int few = 0; few < 2; ++few) {
-        auto* start = const_cast<int32_t*>(few ? d.few_start : d.cta_start);
-        int seen = 0;   // CTAs whose start is written
-        p.run(
-            few,
-            [&](int cta, const ChunkPlanner::Item& it, int t0, int t1, int parts, int before) {
-                while (seen <= cta) start[seen++] = at;
-                seg[at++] = tle::ChunkSeg{it.seq, it.kvh, it.row0, it.n_rows, t0, t1,
-                                          parts > 1 ? part + before * it.n_rows : -1, 0};
-            },
-            [&](const ChunkPlanner::Item& it, int parts) {
-                *mrg++ = tle::ChunkMerge{it.seq, it.kvh, it.row0, it.n_rows, part, parts};
-                part += parts * it.n_rows;
-            });
-        while (seen <= ctas[few]) start[seen++] = at;
-    }
+    std::copy(segs.begin(), segs.end(), const_cast<tle::ChunkSeg*>(d.segs));
+    std::copy(merges.begin(), merges.end(), const_cast<tle::ChunkMerge*>(d.merges));
+    std::copy(start[0].begin(), start[0].end(), const_cast<int32_t*>(d.cta_start));
+    std::copy(start[1].begin(), start[1].end(), const_cast<int32_t*>(d.few_start));
     *plan = out;
     return ok();
-} catch (const std::exception& e) {
+} catch (const std::exception& e) {   // the planner's lists: out of host memory
     return set_error(TLE_ERR_INVALID, "chunk plan: %s", e.what());
 }
 
@@ -1801,7 +1805,7 @@ int tle_prefill_bf16_paged(const tle_shape_t* shape, const tle_page_pool_bf16_t*
     if (need && !aligned16(workspace)) return set_error(TLE_ERR_INVALID, "workspace must be 16-byte aligned");
     tle::ChunkArgs a{};
     a.d = tle::chunk_desc(desc_dev, plan->n_seqs, plan->n_segs, plan->n_merge, plan->n_tokens, plan->n_ctas);
-    a.n_tokens = plan->n_tokens;
+    a.plan_id = tle::chunk_plan_id(*plan);
     a.n_ctas = plan->n_ctas;
     a.n_few_ctas = plan->n_few_ctas;
     a.n_merge = plan->n_merge;
@@ -1847,14 +1851,22 @@ int tle_logits_adjust(float* out, int64_t out_stride, const float* logits, int64
     if (out == logits && out_stride != logits_stride)
         return set_error(TLE_ERR_INVALID, "out is logits, with another stride");
     const tle_logit_rules_t& r = *rules;
+    for (const void* p : {static_cast<const void*>(out), static_cast<const void*>(logits), static_cast<const void*>(r.tokens),
+                          static_cast<const void*>(r.token_start), static_cast<const void*>(r.n_prompt),
+                          static_cast<const void*>(r.repetition), static_cast<const void*>(r.frequency),
+                          static_cast<const void*>(r.presence), static_cast<const void*>(r.bias_tokens),
+                          static_cast<const void*>(r.bias_values), static_cast<const void*>(r.bias_start),
+                          static_cast<const void*>(r.allowed)})
+        if ((reinterpret_cast<uintptr_t>(p) & 3u) != 0) return set_error(TLE_ERR_INVALID, "pointers must be 4-byte aligned");
     if (r.tokens && !r.token_start) return set_error(TLE_ERR_INVALID, "tokens without token_start");
     if (!r.tokens && (r.repetition || r.frequency || r.presence))
         return set_error(TLE_ERR_INVALID, "penalties without tokens");
     if (r.bias_tokens && (!r.bias_values || !r.bias_start))
         return set_error(TLE_ERR_INVALID, "bias_tokens without bias_values or bias_start");
-    if (r.n_tokens < 0 || r.n_biases < 0) return set_error(TLE_ERR_INVALID, "negative list length");
-    if (r.allowed && r.allowed_stride < (n_vocab + 31) / 32)
-        return set_error(TLE_ERR_INVALID, "allowed_stride %lld < %d words", static_cast<long long>(r.allowed_stride),
+    if (r.n_tokens < 0 || r.n_biases < 0 || r.n_tokens > (1 << 30) || r.n_biases > (1 << 30))
+        return set_error(TLE_ERR_INVALID, "list length %d or %d outside [0, 2^30]", r.n_tokens, r.n_biases);
+    if (r.allowed && r.allowed_stride != 0 && r.allowed_stride < (n_vocab + 31) / 32)
+        return set_error(TLE_ERR_INVALID, "allowed_stride %lld is neither 0 nor >= %d words", static_cast<long long>(r.allowed_stride),
                          (n_vocab + 31) / 32);
     tle::LogitArgs a{};
     a.logits = logits;

@@ -98,7 +98,12 @@ __global__ void __launch_bounds__(kAppendThreads) append_kernel(const __grid_con
     const int units = A.n_head + 2 * A.n_head_kv, kv0 = A.n_head, v0 = A.n_head + A.n_head_kv;
     const int pieces = (units + HPW - 1) / HPW;
     const int j_end = static_cast<int>(static_cast<int64_t>(part + 1) * pieces / parts);
+    const uint64_t desc_id = A.d.hdr->id;
     const ChunkTok tk = A.d.toks[tok];
+    if (desc_id != A.plan_id) {
+        if (lane == 0) record_error(A.err, kErrBadDesc);
+        return;
+    }
     const int d0 = lane % LPH * VE;             // this lane's elements of a head
     const Act* q = static_cast<const Act*>(A.q) + tok * A.q_stride + d0;
     const Act* k = static_cast<const Act*>(A.k) + tok * A.k_stride + d0;
@@ -225,6 +230,16 @@ constexpr float kMoveThreshold = 8.0f;
 // below 2^31; 0 for a group of one).
 __device__ __forceinline__ int row_token(const ChunkArgs& A, int row) {
     return A.group_mul ? static_cast<int>(__umulhi(static_cast<uint32_t>(row), A.group_mul) >> A.group_shift) : row;
+}
+// Segments [seg0, seg1) of this CTA; none if the descriptor is not the launch's.
+__device__ __forceinline__ void my_segments(const ChunkArgs& A, const int32_t* start, int& seg0, int& seg1) {
+    const uint64_t id = A.d.hdr->id;
+    seg0 = start[blockIdx.x];
+    seg1 = start[blockIdx.x + 1];
+    if (id != A.plan_id) {
+        seg0 = seg1 = 0;
+        if (threadIdx.x == 0) record_error(A.err, kErrBadDesc);
+    }
 }
 // A segment as the kernel's roles see it.
 struct Work {
@@ -597,7 +612,8 @@ __global__ void __launch_bounds__(CT_THREADS, 1)
     }
     // everything below reads what earlier kernels on the stream wrote
     asm volatile("griddepcontrol.wait;" ::: "memory");
-    const int seg0 = A.d.cta_start[blockIdx.x], seg1 = A.d.cta_start[blockIdx.x + 1];
+    int seg0, seg1;
+    my_segments(A, A.d.cta_start, seg0, seg1);
     if (tid < kWorkCache && seg0 + tid < seg1) S.work[tid] = work_at(A, seg0 + tid);
     tc_fence_before();
     __syncthreads();
@@ -708,106 +724,106 @@ __global__ void __launch_bounds__(CT_THREADS, 1)
             for (int y = max(0, x - kBufs); y < x; ++y)   // MMAs done before TMEM is freed
                 wait_uniform(&S.p_free[c][y % kBufs], (y / kBufs) & 1, A.err, kErrDrain, failed);
         }
-    } else if (warp == 12) {
-        regs_dealloc<kRegsControl>();
-        produce_tiles<CT_STAGES>(A, M, seg0, seg1, S.k, S.v, S.kv_full, S.kv_empty, failed);
-    } else if (warp == 13) {
-        // -------------------------- V of the edge tiles ----------------------------
-        regs_dealloc<kRegsControl>();
-        int ring = 0;
-        for (int sg = seg0; sg < seg1; ++sg) {
-            const int k = sg - seg0;
-            const Work w = work_of(sg);
-            // the flag was last read by the segment before the last one
-            if (k >= 2) wait_or_flag(&S.seg_end[k & 1], ((k - 2) >> 1) & 1, A.err, kErrWaitMma, failed);
-            if (lane == 0) S.bad[k & 1] = 0;
-            __syncwarp();
-            for (int n = w.t0; n < w.t1; ++n, ++ring) {
-                const int st = ring % CT_STAGES;
-                wait_or_flag(&S.kv_full[st], (ring / CT_STAGES) & 1, A.err, kErrWaitFull, failed);
-                if (w.edge(n)) {
-                    bool bad = false;
-                    const int some = max(0, w.pos_min + 1 - n * kTile);   // from here on not for every row
-                    const int none = w.kv_len - n * kTile;                // from here on for none
-                    uint4* v = reinterpret_cast<uint4*>(S.v[st]);
-                    for (int e = (some & ~3) * 8 + lane; e < kTile * 8; e += 32) {
-                        const int jl = e >> 3;
-                        if (jl >= none) v[e] = make_uint4(0, 0, 0, 0);
-                        else if (jl >= some) {
-                            bad |= not_finite(v[e]);
-                        }
-                    }
-                    if (__any_sync(0xffffffffu, bad) && lane == 0) S.bad[k & 1] = 1;
-                    fence_proxy_async_smem();
-                    __syncwarp();
-                    if (lane == 0) mbar_arrive(&S.v_ok[st]);
-                }
-                __syncwarp();
-                if (lane == 0) mbar_arrive(&S.kv_empty[st]);
-            }
-            if (lane == 0) mbar_arrive(&S.scanned[k & 1]);
-        }
     } else if (wg == 3) {
-        // ------------------------------ Q loaders ----------------------------------
         regs_dealloc<kRegsControl>();
-        const int lw = warp - 14;
-        for (int sg = seg0; sg < seg1; ++sg) {
-            const int k = sg - seg0, b = k % kQBufs;
-            const Work w = work_of(sg);
-            if (k >= kQBufs) wait_or_flag(&S.q_free[b], ((k / kQBufs) - 1) & 1, A.err, kErrWaitEmpty, failed);
-            // 8 lanes per row, 4 rows per step, half of each row tile per warp
-            const int ch = lane & 7;
-            for (int m = 0; m < (w.dual ? 2 : 1); ++m) {
-                const int r0 = lw * 64 + (lane >> 3);   // row of the tile
-                RowWalk<const Act> at(A, static_cast<const Act*>(A.q) + ch * 8, A.q_stride, w.first, w.kvh,
-                                      w.row0 + m * kChunkRows + r0);
-                const int left = w.n_rows - m * kChunkRows - r0;   // steps of 4 rows while below
-                // rows r0 and r0 + 4 and their chunk's place; further rows keep one of the two
-                const int off[2] = {r0 * HD + ((ch ^ (r0 & 7)) << 3), (r0 + 4) * HD + ((ch ^ ((r0 + 4) & 7)) << 3)};
-                if constexpr (!F32) {
-#pragma unroll 4
-                    for (int j = 0; j < 16; ++j) {
-                        const bool ok = 4 * j < left;
-                        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(
-                                         smem_u32(&S.q[b][m][0][off[j & 1] + (j >> 1) * 8 * HD])),
-                                     "l"(ok ? at.p : static_cast<const Act*>(A.q)), "r"(ok ? 16 : 0)
-                                     : "memory");
-                        at.template step<4>(A);
-                    }
-                } else {
-#pragma unroll 1
-                    for (int j0 = 0; j0 < 16; j0 += 4) {
-                        float4 x[4][2];
-#pragma unroll
-                        for (int j = 0; j < 4; ++j) {
-                            const float4* src = reinterpret_cast<const float4*>(at.p);
-                            x[j][0] = x[j][1] = make_float4(0.f, 0.f, 0.f, 0.f);
-                            if (4 * (j0 + j) < left) {
-                                x[j][0] = src[0];
-                                x[j][1] = src[1];
+        if (warp == 12) {
+            produce_tiles<CT_STAGES>(A, M, seg0, seg1, S.k, S.v, S.kv_full, S.kv_empty, failed);
+        } else if (warp == 13) {
+            // -------------------------- V of the edge tiles ----------------------------
+            int ring = 0;
+            for (int sg = seg0; sg < seg1; ++sg) {
+                const int k = sg - seg0;
+                const Work w = work_of(sg);
+                // the flag was last read by the segment before the last one
+                if (k >= 2) wait_or_flag(&S.seg_end[k & 1], ((k - 2) >> 1) & 1, A.err, kErrWaitMma, failed);
+                if (lane == 0) S.bad[k & 1] = 0;
+                __syncwarp();
+                for (int n = w.t0; n < w.t1; ++n, ++ring) {
+                    const int st = ring % CT_STAGES;
+                    wait_or_flag(&S.kv_full[st], (ring / CT_STAGES) & 1, A.err, kErrWaitFull, failed);
+                    if (w.edge(n)) {
+                        bool bad = false;
+                        const int some = max(0, w.pos_min + 1 - n * kTile);   // from here on not for every row
+                        const int none = w.kv_len - n * kTile;                // from here on for none
+                        uint4* v = reinterpret_cast<uint4*>(S.v[st]);
+                        for (int e = (some & ~3) * 8 + lane; e < kTile * 8; e += 32) {
+                            const int jl = e >> 3;
+                            if (jl >= none) v[e] = make_uint4(0, 0, 0, 0);
+                            else if (jl >= some) {
+                                bad |= not_finite(v[e]);
                             }
+                        }
+                        if (__any_sync(0xffffffffu, bad) && lane == 0) S.bad[k & 1] = 1;
+                        fence_proxy_async_smem();
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive(&S.v_ok[st]);
+                    }
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&S.kv_empty[st]);
+                }
+                if (lane == 0) mbar_arrive(&S.scanned[k & 1]);
+            }
+        } else {
+            // ------------------------------ Q loaders ----------------------------------
+            const int lw = warp - 14;
+            for (int sg = seg0; sg < seg1; ++sg) {
+                const int k = sg - seg0, b = k % kQBufs;
+                const Work w = work_of(sg);
+                if (k >= kQBufs) wait_or_flag(&S.q_free[b], ((k / kQBufs) - 1) & 1, A.err, kErrWaitEmpty, failed);
+                // 8 lanes per row, 4 rows per step, half of each row tile per warp
+                const int ch = lane & 7;
+                for (int m = 0; m < (w.dual ? 2 : 1); ++m) {
+                    const int r0 = lw * 64 + (lane >> 3);   // row of the tile
+                    RowWalk<const Act> at(A, static_cast<const Act*>(A.q) + ch * 8, A.q_stride, w.first, w.kvh,
+                                          w.row0 + m * kChunkRows + r0);
+                    const int left = w.n_rows - m * kChunkRows - r0;   // steps of 4 rows while below
+                    // rows r0 and r0 + 4 and their chunk's place; further rows keep one of the two
+                    const int off[2] = {r0 * HD + ((ch ^ (r0 & 7)) << 3), (r0 + 4) * HD + ((ch ^ ((r0 + 4) & 7)) << 3)};
+                    if constexpr (!F32) {
+#pragma unroll 4
+                        for (int j = 0; j < 16; ++j) {
+                            const bool ok = 4 * j < left;
+                            asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(
+                                             smem_u32(&S.q[b][m][0][off[j & 1] + (j >> 1) * 8 * HD])),
+                                         "l"(ok ? at.p : static_cast<const Act*>(A.q)), "r"(ok ? 16 : 0)
+                                         : "memory");
                             at.template step<4>(A);
                         }
+                    } else {
+#pragma unroll 1
+                        for (int j0 = 0; j0 < 16; j0 += 4) {
+                            float4 x[4][2];
 #pragma unroll
-                        for (int j = 0; j < 4; ++j) {
-                            const int at_q = off[j & 1] + ((j0 + j) >> 1) * 8 * HD;
-                            float* f = reinterpret_cast<float*>(x[j]);
+                            for (int j = 0; j < 4; ++j) {
+                                const float4* src = reinterpret_cast<const float4*>(at.p);
+                                x[j][0] = x[j][1] = make_float4(0.f, 0.f, 0.f, 0.f);
+                                if (4 * (j0 + j) < left) {
+                                    x[j][0] = src[0];
+                                    x[j][1] = src[1];
+                                }
+                                at.template step<4>(A);
+                            }
 #pragma unroll
-                            for (int term = 0; term < kTerms; ++term) {
-                                *reinterpret_cast<uint4*>(&S.q[b][m][term][at_q]) =
-                                    make_uint4(top_pair(f[0], f[1]), top_pair(f[2], f[3]), top_pair(f[4], f[5]),
-                                               top_pair(f[6], f[7]));
+                            for (int j = 0; j < 4; ++j) {
+                                const int at_q = off[j & 1] + ((j0 + j) >> 1) * 8 * HD;
+                                float* f = reinterpret_cast<float*>(x[j]);
 #pragma unroll
-                                for (int c = 0; c < 4; ++c) f2_split(rest_pair(f[2 * c], f[2 * c + 1]), f[2 * c], f[2 * c + 1]);
+                                for (int term = 0; term < kTerms; ++term) {
+                                    *reinterpret_cast<uint4*>(&S.q[b][m][term][at_q]) =
+                                        make_uint4(top_pair(f[0], f[1]), top_pair(f[2], f[3]), top_pair(f[4], f[5]),
+                                                   top_pair(f[6], f[7]));
+#pragma unroll
+                                    for (int c = 0; c < 4; ++c) f2_split(rest_pair(f[2 * c], f[2 * c + 1]), f[2 * c], f[2 * c + 1]);
+                                }
                             }
                         }
                     }
                 }
+                if constexpr (!F32) cp_async_wait_all();
+                fence_proxy_async_smem();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&S.q_full[b]);
             }
-            if constexpr (!F32) cp_async_wait_all();
-            fence_proxy_async_smem();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&S.q_full[b]);
         }
     } else {
         // ------------------------------ softmax ------------------------------------
@@ -1163,7 +1179,8 @@ __global__ void __launch_bounds__(FW_THREADS, 1)
         prefetch_tmap(&M.v);
     }
     asm volatile("griddepcontrol.wait;" ::: "memory");
-    const int seg0 = A.d.few_start[blockIdx.x], seg1 = A.d.few_start[blockIdx.x + 1];
+    int seg0, seg1;
+    my_segments(A, A.d.few_start, seg0, seg1);
     if (tid < kWorkCache && seg0 + tid < seg1) S.work[tid] = work_at(A, seg0 + tid);
     __syncthreads();
     auto work_of = [&](int i) { return i - seg0 < kWorkCache ? S.work[i - seg0] : work_at(A, i); };
@@ -1174,7 +1191,8 @@ __global__ void __launch_bounds__(FW_THREADS, 1)
     }
     const int gid = lane >> 2, tg = lane & 3;     // fragment row and column pair
     const int mi = lane >> 3, li = lane & 7;      // ldmatrix: matrix and row of this lane's address
-    auto row_groups = [](int n_rows) { return n_rows <= 16 ? 1 : n_rows <= 32 ? 2 : 4; };
+    static_assert(kChunkFewRows <= 32, "two row groups at most");
+    auto row_groups = [](int n_rows) { return n_rows <= 16 ? 1 : 2; };
     // This lane's rows gid and gid + 8 of the row group, two columns of each 8:
     // loaded ahead of the segment that needs them.
     using Raw = std::conditional_t<F32, float2, uint32_t>;
@@ -1448,7 +1466,12 @@ __global__ void __launch_bounds__(kMergeThreads) chunk_merge_kernel(const __grid
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     asm volatile("griddepcontrol.wait;" ::: "memory");
     const int lane = threadIdx.x & 31;
+    const uint64_t id = A.d.hdr->id;
     const ChunkMerge m = A.d.merges[blockIdx.x];
+    if (id != A.plan_id) {
+        if (threadIdx.x == 0) record_error(A.err, kErrBadDesc);
+        return;
+    }
     const int r = blockIdx.y * (kMergeThreads / 32) + (threadIdx.x >> 5);
     if (r >= m.n_rows) return;
     const float* lse = A.part_lse + m.part + r;

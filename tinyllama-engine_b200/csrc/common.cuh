@@ -22,6 +22,7 @@ enum : uint32_t {
     kErrGridWait = 0x108,   // persistent forward: a grid barrier wait gave up
     kErrF16Range = 0x109,   // batched prompt: a finite value beyond fp16's range became inf
     kErrBadSeq = 0x10a,     // bf16 decode: a sequence record outside its cache or max_rows (skipped)
+    kErrBadDesc = 0x10b,    // chunk calls: a descriptor of another plan than the launch (nothing done)
     kErrSelfTest = 0x1ff,   // tle_selftest_wait_timeout: the planted wait expired
 };
 

@@ -351,11 +351,28 @@ cudaError_t launch_embed_rows(int type, float* x, const void* table, const int32
 constexpr int kChunkTile = 128;       // K/V rows per tile
 constexpr int kChunkRows = 128;       // rows per tensor-core tile
 constexpr int kChunkItemRows = 2 * kChunkRows;
+// The kernel for few rows pays while a 128-row tensor-core tile is mostly empty.
+// 32 sequences behind 2000 rows: 32 rows 22.4 us (bf16) and 35.3 us (fp32),
+// against 24.2 and 37.4 us by the other kernel; 64 rows 34.1 and 57.0 against
+// 25.0 and 38.7 us.
 constexpr int kChunkFewRows = 32;
-constexpr int32_t kChunkMagic = 0x544c4543;  // "TLEC"
 struct ChunkHeader {
-    int32_t magic, n_seqs, n_tokens, n_ctas, n_segs, n_merge, n_few_ctas, reserved;
+    uint64_t id;             // chunk_plan_id of the plan
+    int32_t n_seqs, n_tokens, n_ctas, n_few_ctas, n_segs, n_merge;
 };
+// A number for everything in a plan that a launch depends on (FNV-1a over its
+// fields).  A kernel does nothing (kErrBadDesc) unless the descriptor carries
+// the number of the plan that it was launched with: a captured launch that is
+// replayed after the descriptor was replaced would walk the new one with the
+// old one's offsets.
+inline uint64_t chunk_plan_id(const tle_chunk_plan_t& p) {
+    const int64_t fields[] = {p.n_seqs, p.n_tokens, p.n_head, p.n_head_kv, p.page_rows, p.n_ctas,
+                              p.n_few_ctas, p.n_segs, p.n_merge, p.merge_rows, p.part_rows};
+    uint64_t h = 0xcbf29ce484222325ull;
+    for (int64_t f : fields)
+        for (int b = 0; b < 64; b += 8) h = (h ^ ((static_cast<uint64_t>(f) >> b) & 0xffu)) * 0x100000001b3ull;
+    return h;
+}
 struct ChunkSeq {
     const int32_t* pages;
     int32_t n_pages, pos, n_tokens, first;   // first: batch index of its first token
@@ -377,6 +394,7 @@ static_assert(sizeof(ChunkHeader) == 32 && sizeof(ChunkSeq) == 24 && sizeof(Chun
                   sizeof(ChunkMerge) == 24 && sizeof(ChunkTok) == 8,
               "chunk descriptor records");
 struct ChunkDesc {           // device pointers into one descriptor
+    const ChunkHeader* hdr;
     const ChunkSeq* seqs;
     const ChunkSeg* segs;
     const ChunkMerge* merges;
@@ -391,6 +409,7 @@ inline size_t chunk_desc_bytes(size_t n_seqs, size_t n_segs, size_t n_merge, siz
 inline ChunkDesc chunk_desc(const void* base, size_t n_seqs, size_t n_segs, size_t n_merge, size_t n_tokens, size_t n_ctas) {
     const unsigned char* p = static_cast<const unsigned char*>(base) + sizeof(ChunkHeader);
     ChunkDesc d;
+    d.hdr = static_cast<const ChunkHeader*>(base);
     d.seqs = reinterpret_cast<const ChunkSeq*>(p);
     d.segs = reinterpret_cast<const ChunkSeg*>(d.seqs + n_seqs);
     d.merges = reinterpret_cast<const ChunkMerge*>(d.segs + n_segs);
@@ -401,6 +420,7 @@ inline ChunkDesc chunk_desc(const void* base, size_t n_seqs, size_t n_segs, size
 }
 struct AppendArgs {
     ChunkDesc d;
+    uint64_t plan_id;
     int n_tokens;
     const void* q;           // activations: fp32 or bf16
     const void* k;
@@ -418,7 +438,8 @@ struct AppendArgs {
 cudaError_t launch_append(const AppendArgs& a, bool act_bf16, bool pool_bf16, cudaStream_t stream);
 struct ChunkArgs {
     ChunkDesc d;
-    int n_tokens, n_ctas, n_few_ctas, n_merge, merge_rows;
+    uint64_t plan_id;
+    int n_ctas, n_few_ctas, n_merge, merge_rows;
     const void* q;           // rotated; fp32 or bf16
     void* out;
     int64_t q_stride, out_stride;

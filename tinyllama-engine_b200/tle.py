@@ -112,7 +112,7 @@ class ChunkPlan(ctypes.Structure):
     """tle_chunk_plan_t: what tle_chunk_desc_paged found out about a batch."""
     _fields_ = [(n, ctypes.c_int32) for n in ("n_seqs", "n_tokens", "n_head", "n_head_kv", "page_rows",
                                                "n_ctas", "n_few_ctas", "n_segs", "n_merge", "merge_rows")] + \
-               [("part_rows", ctypes.c_int64)]
+               [("part_rows", ctypes.c_int64), ("desc_bytes", ctypes.c_int64)]
 
 
 class LogitRulesDesc(ctypes.Structure):
@@ -662,7 +662,10 @@ class PagedChunkBatch:
     ``attend`` is the causal attention over a bf16 cache, ``run`` does both.
     ``set_positions`` re-plans on the host and uploads the descriptor (one H2D
     copy), once per step of all layers.  Calls of one batch share its
-    workspace: they must not overlap on the GPU.
+    descriptor and workspace: they must not overlap on the GPU, nor
+    ``set_positions`` with a call that still runs on another stream.  A
+    captured call belongs to its plan: replayed after ``set_positions`` made
+    another one it does nothing and tle_device_error reports 0x10b.
     """
 
     def __init__(self, cache: PagedKVCache, tables: Sequence, positions: Sequence[int],
@@ -688,6 +691,7 @@ class PagedChunkBatch:
         self.plan = ChunkPlan()
         self._desc_dev = self.workspace = None
         self._q = {}
+        self._streams = set()   # handles of the streams that the buffers below are known to be used on
         self.set_positions(positions, lengths, stream)
 
     def build_host(self, positions: Sequence[int], lengths: Sequence[int]):
@@ -707,20 +711,25 @@ class PagedChunkBatch:
         _check(L.tle_chunk_desc_paged(ctypes.byref(self.shape), self.cache.page_rows, chunks, self.n,
                                       self.max_ctas, host.data_ptr(), nbytes, ctypes.byref(plan)))
         self.plan = plan
-        return host
+        return host[:plan.desc_bytes]
 
     def set_positions(self, positions: Sequence[int], lengths: Sequence[int], stream=None) -> None:
         import torch
+        if stream is not None and stream.device != self.device:
+            raise ValueError(f"stream of {stream.device}, cache on {self.device}")
         with torch.cuda.device(self.device):
             host = self.build_host(positions, lengths)   # a new one: the last upload may be pending
-            s = stream or torch.cuda.current_stream()
-            with torch.cuda.stream(s):
+            with torch.cuda.stream(stream or torch.cuda.current_stream()):
                 if self._desc_dev is None or self._desc_dev.numel() < host.numel():
-                    self._desc_dev = torch.empty(host.numel(), dtype=torch.uint8, device=self.device)
-                self._desc_dev[:host.numel()].copy_(host, non_blocking=True)
+                    # with room for the plans of later positions
+                    self._desc_dev = torch.empty(host.numel() * 5 // 4 + 4096, dtype=torch.uint8, device=self.device)
+                    self._streams.clear()
                 nbytes = lib().tle_prefill_bf16_paged_workspace_bytes(ctypes.byref(self.plan))
                 if self.workspace is None or self.workspace.numel() * 4 < nbytes:
                     self.workspace = torch.empty(max(nbytes // 4, 4), dtype=torch.float32, device=self.device)
+                    self._streams.clear()
+                self._on(stream)
+                self._desc_dev[:host.numel()].copy_(host, non_blocking=True)
         self.positions = [int(p) for p in positions]
         self.lengths = [int(x) for x in lengths]
 
@@ -746,10 +755,16 @@ class PagedChunkBatch:
         raise ValueError(f"{name}: activations are all float32 or all bfloat16, got {t.dtype}")
 
     def _on(self, stream) -> int:
-        if stream is not None:
-            for t in (self._desc_dev, self.workspace):
-                t.record_stream(stream)
-        return _raw_stream(stream, self._index)
+        """Handle of the stream; the batch's buffers are kept from reuse until
+        what it ran there is done."""
+        raw = _raw_stream(stream, self._index)
+        if raw not in self._streams:
+            import torch
+            s = stream or torch.cuda.current_stream(self._index)
+            for t in (self._desc_dev, self.workspace, *self._q.values()):
+                t.record_stream(s)
+            self._streams.add(raw)
+        return raw
 
     def append(self, q, k, v, layer: int, rotate: bool = True, q_out=None, stream=None) -> None:
         """rope(q, k) at each token's position (rotate), k and v stored in
@@ -778,7 +793,8 @@ class PagedChunkBatch:
 
     def attend(self, q, out, layer: int, stream=None) -> None:
         """Causal attention of the chunks (q already rotated) over a bf16
-        cache; rows of out behind the last token are left as they are."""
+        cache; rows of out behind the last token are left as they are.  out
+        may be q."""
         if not self._bf16:
             raise ValueError("attend: a bfloat16 PagedKVCache expected")
         act = self._act(q, "q")
@@ -802,8 +818,7 @@ class PagedChunkBatch:
         if buf is None or buf.shape[0] < self.plan.n_tokens:
             buf = self._q[q.dtype] = torch.empty((self.plan.n_tokens, self.shape.n_head * self.shape.head_dim),
                                                  dtype=q.dtype, device=self.device)
-        if stream is not None:
-            buf.record_stream(stream)
+            self._streams.clear()
         self.append(q, k, v, layer, rotate=True, q_out=buf, stream=stream)
         self.attend(buf, out, layer, stream=stream)
 
@@ -946,8 +961,8 @@ class LogitRules:
     frequency, presence  float32 [n_rows]: made tokens, - freq * times, - pres;
     bias_tokens, bias_values, bias_start  int32, float32, int32: + the values
         of bias_tokens[bias_start[r]:bias_start[r + 1]];
-    allowed              int32 [n_rows][>= ceil(n_vocab / 32)], any row stride:
-        bit t % 32 of word t / 32 clear: token t gets -inf.
+    allowed              int32 [n_rows][>= ceil(n_vocab / 32)], any row stride (0:
+        one mask for all rows): bit t % 32 of word t / 32 clear: token t gets -inf.
     """
 
     _GROUPS = (("tokens", "int32"), ("token_start", "int32"), ("n_prompt", "int32"), ("repetition", "float32"),
