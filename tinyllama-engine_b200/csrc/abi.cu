@@ -1671,7 +1671,15 @@ int append_common(const tle_shape_t* shape, const tle_chunk_plan_t* plan, const 
     a.n_head = q ? shape->n_head : 0;
     a.n_head_kv = shape->n_head_kv;
     a.rotate = (flags & TLE_DECODE_ROTATE) ? 1 : 0;
-    fill_inv_freq(a.inv_freq, tle::kHeadDim / 2, shape->rope_freq_base);
+    if (a.rotate) {
+        // 32 powers, half a microsecond: kept for the thread's last base
+        thread_local float base = 0.f, table[tle::kHeadDim / 2];
+        if (base != shape->rope_freq_base) {
+            base = shape->rope_freq_base;
+            fill_inv_freq(table, tle::kHeadDim / 2, base);
+        }
+        std::copy(std::begin(table), std::end(table), a.inv_freq);
+    }
     cudaError_t e = tle::error_word(&a.err);
     if (e != cudaSuccess) return cuda_error(e, "device error word");
     e = tle::launch_append(a, act_type == TLE_ACT_BF16, pool_bf16, static_cast<cudaStream_t>(stream));

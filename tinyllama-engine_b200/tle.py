@@ -27,6 +27,7 @@ TLE_ERR_CUDA = 4
 TLE_ERR_DEVICE = 5
 
 TLE_DECODE_ROTATE = 1
+TLE_ACT_F32, TLE_ACT_BF16 = 0, 1
 TLE_DECODE_KV_READY = 2
 
 
@@ -680,6 +681,7 @@ class PagedChunkBatch:
         self._shape_ref = ctypes.byref(self.shape)
         self._widths = (self.shape.n_head * self.shape.head_dim, self.shape.n_head_kv * self.shape.head_dim)
         self._bf16 = cache.dtype == torch.bfloat16
+        self._acts = {torch.float32: TLE_ACT_F32, torch.bfloat16: TLE_ACT_BF16}
         if not self._bf16 and cache.dtype != torch.float32:
             raise ValueError(f"a float32 or bfloat16 PagedKVCache expected, got {cache.dtype}")
         self.max_ctas = max_ctas
@@ -689,7 +691,7 @@ class PagedChunkBatch:
             if t.dtype != torch.int32 or t.device != self.device or not t.is_cuda or not t.is_contiguous():
                 raise ValueError(f"tables[{i}]: need a contiguous int32 tensor on {self.device}")
         self.plan = ChunkPlan()
-        self._desc_dev = self.workspace = None
+        self._desc_dev = self.workspace = self._pool_made = None
         self._q = {}
         self._streams = set()   # handles of the streams that the buffers below are known to be used on
         self.set_positions(positions, lengths, stream)
@@ -747,12 +749,17 @@ class PagedChunkBatch:
 
     def _act(self, t, name: str) -> int:
         """TLE_ACT_* of an activation tensor."""
-        import torch
-        if t.dtype is torch.bfloat16:
-            return 1
-        if t.dtype is torch.float32:
-            return 0
-        raise ValueError(f"{name}: activations are all float32 or all bfloat16, got {t.dtype}")
+        act = self._acts.get(t.dtype)
+        if act is None:
+            raise ValueError(f"{name}: activations are all float32 or all bfloat16, got {t.dtype}")
+        return act
+
+    def _pool(self):
+        """The cache's tle_page_pool_t, made again only when it has other tensors."""
+        c, made = self.cache, self._pool_made
+        if made is None or made[0] is not c.key_pool or made[1] is not c.value_pool:
+            made = self._pool_made = (c.key_pool, c.value_pool, c.pool())
+        return made[2]
 
     def _on(self, stream) -> int:
         """Handle of the stream; the batch's buffers are kept from reuse until
@@ -786,7 +793,7 @@ class PagedChunkBatch:
         elif q_out is not None:
             raise ValueError("q_out without q")
         L = lib()
-        pool = self.cache.pool()
+        pool = self._pool()
         _on_device(self._index, L.tle_append_bf16_paged if self._bf16 else L.tle_append_paged, self._shape_ref,
                    ctypes.addressof(pool), ctypes.byref(self.plan), self._desc_dev.data_ptr(), qp, qs, kp, ks, vp, vs,
                    qo, act, layer, TLE_DECODE_ROTATE if rotate else 0, self._on(stream))
@@ -800,7 +807,7 @@ class PagedChunkBatch:
         act = self._act(q, "q")
         qp, qs = self._rows(q, self._widths[0], "q", q.dtype)
         op, os = self._rows(out, self._widths[0], "out", q.dtype)
-        pool = self.cache.pool()
+        pool = self._pool()
         _on_device(self._index, lib().tle_prefill_bf16_paged, self._shape_ref, ctypes.addressof(pool),
                    ctypes.byref(self.plan), self._desc_dev.data_ptr(), qp, qs, op, os, act, layer,
                    self.workspace.data_ptr(), self.workspace.numel() * 4, self._on(stream))
