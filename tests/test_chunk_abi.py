@@ -38,13 +38,16 @@ def parse(buf, plan):
         a = np.frombuffer(b[at:at + count * width], dtype).reshape(count, width // 4)
         at += count * width
         return a
+    cta = take(plan.n_ctas + plan.n_few_ctas, 64)
+    segs = take(plan.n_segs, 64)
     seqs = take(plan.n_seqs, 24)
-    segs = take(plan.n_segs, 32)
     merges = take(plan.n_merge, 24)
     toks = take(plan.n_tokens, 8)
-    start, few = take(plan.n_ctas + 1, 4)[:, 0], take(plan.n_few_ctas + 1, 4)[:, 0]
     assert at == len(b)
-    return seqs, segs, merges, toks, start, few
+    return seqs, segs, merges, toks, cta
+
+
+PAGES, POS, FIRST, KVH, ROW0, ROWS, T0, T1, PART, POS_MIN, KV_LEN, SEG0, SEG1, SEQ = 0, 2, 3, 4, 5, 6, 7, 8, 9, 10, 11, 12, 13, 14
 
 
 @pytest.mark.parametrize("seed", range(12))
@@ -58,21 +61,28 @@ def test_plan_covers_every_tile_once(seed):
     rc, buf, plan = describe(pos, new, heads, max_ctas=max_ctas)
     assert rc == 0, tle.lib().tle_last_error()
     g = heads[0] // heads[1]
-    seqs, segs, merges, toks, start, few = parse(buf, plan)
+    seqs, segs, merges, toks, cta = parse(buf, plan)
     assert plan.n_tokens == sum(new) and plan.n_seqs == n
     assert [tuple(x) for x in toks] == [(s, pos[s] + t) for s in range(n) for t in range(new[s])]
     first = np.cumsum([0] + new)[:-1]
     assert np.array_equal(seqs[:, 3], pos) and np.array_equal(seqs[:, 4], new) and np.array_equal(seqs[:, 5], first)
     assert max(plan.n_ctas, plan.n_few_ctas) <= (max_ctas or 148)
-    assert start[0] == 0 and start[-1] == few[0] and few[-1] == plan.n_segs
-    assert np.all(np.diff(start) >= 0) and np.all(np.diff(few) >= 0)
-    chunk_rows = np.array(new)[segs[:, 0]] * g                         # chunks of many rows, then of few
-    assert np.all(chunk_rows[:few[0]] > FEW) and np.all(chunk_rows[few[0]:] <= FEW)
+    assert cta.shape[0] == 0 or (cta[0, SEG0] == 0 and cta[-1, SEG1] == plan.n_segs)
+    assert np.array_equal(cta[1:, SEG0], cta[:-1, SEG1]) and np.all(cta[:, SEG0] <= cta[:, SEG1])
+    for x in cta[cta[:, SEG0] < cta[:, SEG1]]:                         # a copy of the CTA's first piece
+        assert np.array_equal(np.delete(x, [SEG0, SEG1]), np.delete(segs[x[SEG0]], [SEG0, SEG1]))
+    few0 = cta[plan.n_ctas, SEG0] if plan.n_few_ctas else plan.n_segs
+    chunk_rows = np.array(new)[segs[:, SEQ]] * g                       # chunks of many rows, then of few
+    assert np.all(chunk_rows[:few0] > FEW) and np.all(chunk_rows[few0:] <= FEW)
+    assert np.array_equal(segs[:, POS], np.array(pos)[segs[:, SEQ]]) and np.array_equal(segs[:, FIRST], first[segs[:, SEQ]])
+    assert np.array_equal(segs[:, PAGES], 0x4000 * (segs[:, SEQ] + 1))
+    assert np.array_equal(segs[:, POS_MIN], segs[:, POS] + segs[:, ROW0] // g)
+    assert np.array_equal(segs[:, KV_LEN], segs[:, POS] + (segs[:, ROW0] + segs[:, ROWS] - 1) // g + 1)
     items = {(s, h, r0): min(ITEM, new[s] * g - r0) for s in range(n) for h in range(heads[1])
              for r0 in range(0, new[s] * g, ITEM)}
     seen, parts = {k: [] for k in items}, {}
     used = np.zeros(plan.part_rows, int)
-    for s, h, r0, rows, t0, t1, part, _ in segs:
+    for s, h, r0, rows, t0, t1, part in segs[:, [SEQ, KVH, ROW0, ROWS, T0, T1, PART]]:
         assert items[(s, h, r0)] == rows and t0 < t1
         seen[(s, h, r0)].append((t0, t1))
         if part >= 0:
@@ -101,8 +111,8 @@ def test_plan_balances_long_work():
     tiles above the even share."""
     rc, buf, plan = describe([30000], [2048])
     assert rc == 0
-    _, segs, _, _, start, _ = parse(buf, plan)
-    cost = [sum(2 * (x[5] - x[4]) for x in segs[a:b]) for a, b in zip(start, start[1:])]
+    _, segs, _, _, cta = parse(buf, plan)
+    cost = [sum(2 * (x[T1] - x[T0]) for x in segs[a:b]) for a, b in cta[:, [SEG0, SEG1]]]
     assert plan.n_ctas == 148 and max(cost) <= sum(cost) / 148 + 16
 
 

@@ -1653,7 +1653,8 @@ int append_common(const tle_shape_t* shape, const tle_chunk_plan_t* plan, const 
     if (int rc = check_rows(k, k_stride, shape->n_head_kv, "k")) return rc;
     if (int rc = check_rows(v, v_stride, shape->n_head_kv, "v")) return rc;
     tle::AppendArgs a{};
-    a.d = tle::chunk_desc(desc_dev, plan->n_seqs, plan->n_segs, plan->n_merge, plan->n_tokens, plan->n_ctas);
+    a.d = tle::chunk_desc(desc_dev, plan->n_seqs, plan->n_segs, plan->n_merge,
+                          static_cast<size_t>(plan->n_ctas) + plan->n_few_ctas);
     a.plan_id = tle::chunk_plan_id(*plan);
     a.n_tokens = plan->n_tokens;
     a.q = q;
@@ -1700,7 +1701,7 @@ size_t tle_chunk_desc_bytes(const tle_shape_t* shape, const tle_paged_chunk_t* c
         tokens += static_cast<size_t>(chunks[s].n_tokens);
         items += (chunks[s].n_tokens * g + tle::kChunkItemRows - 1) / tle::kChunkItemRows;
     }
-    return tle::chunk_desc_bytes(n_seqs, items * shape->n_head_kv + 2 * G, 2 * G, tokens, G, G);
+    return tle::chunk_desc_bytes(n_seqs, items * shape->n_head_kv + 2 * G, 2 * G, tokens, 2 * G);
 }
 
 int tle_chunk_desc_paged(const tle_shape_t* shape, int page_rows, const tle_paged_chunk_t* chunks, int n_seqs,
@@ -1715,15 +1716,25 @@ int tle_chunk_desc_paged(const tle_shape_t* shape, int page_rows, const tle_page
     std::vector<tle::ChunkSeg> segs;
     std::vector<tle::ChunkMerge> merges;
     std::vector<int32_t> start[2];   // first piece of each CTA of the two kernels
-    int64_t part = 0;
+    const int g = shape->n_head / shape->n_head_kv;
+    std::vector<int32_t> first(n_seqs);
+    int64_t tokens = 0, part = 0;
     int merge_rows = 0;
+    for (int s = 0; s < n_seqs; ++s) {
+        first[s] = static_cast<int32_t>(tokens);
+        tokens += chunks[s].n_tokens;
+    }
     for (int few = 0; few < 2; ++few) {
         const int n = p.run(
             few,
             [&](int cta, const ChunkPlanner::Item& it, int t0, int t1, int parts, int before) {
                 start[few].resize(std::max<size_t>(start[few].size(), cta + 1), static_cast<int32_t>(segs.size()));
-                segs.push_back(tle::ChunkSeg{it.seq, it.kvh, it.row0, it.n_rows, t0, t1,
-                                             parts > 1 ? static_cast<int32_t>(part + before * it.n_rows) : -1, 0});
+                const tle_paged_chunk_t& c = chunks[it.seq];
+                tle::ChunkSeg sg{c.pages, c.pos, first[it.seq], it.kvh, it.row0, it.n_rows, t0, t1, -1, 0, 0, 0, 0, it.seq, 0};
+                if (parts > 1) sg.part = static_cast<int32_t>(part + before * it.n_rows);
+                sg.pos_min = c.pos + it.row0 / g;
+                sg.kv_len = c.pos + (it.row0 + it.n_rows - 1) / g + 1;
+                segs.push_back(sg);
             },
             [&](const ChunkPlanner::Item& it, int parts) {
                 merges.push_back(tle::ChunkMerge{it.seq, it.kvh, it.row0, it.n_rows, static_cast<int32_t>(part), parts});
@@ -1735,8 +1746,6 @@ int tle_chunk_desc_paged(const tle_shape_t* shape, int page_rows, const tle_page
     if (segs.size() > INT32_MAX / 2 || part > INT32_MAX / 2)
         return set_error(TLE_ERR_UNSUPPORTED, "batch too large (%zu pieces)", segs.size());
     tle_chunk_plan_t out{};
-    int64_t tokens = 0;
-    for (int s = 0; s < n_seqs; ++s) tokens += chunks[s].n_tokens;
     out.n_seqs = n_seqs;
     out.n_tokens = static_cast<int32_t>(tokens);
     out.n_head = shape->n_head;
@@ -1748,26 +1757,30 @@ int tle_chunk_desc_paged(const tle_shape_t* shape, int page_rows, const tle_page
     out.n_merge = static_cast<int32_t>(merges.size());
     out.merge_rows = merge_rows;
     out.part_rows = part;
-    const size_t need = tle::chunk_desc_bytes(n_seqs, segs.size(), merges.size(), tokens, out.n_ctas, out.n_few_ctas);
+    const size_t n_ctas = static_cast<size_t>(out.n_ctas) + out.n_few_ctas;
+    const size_t need = tle::chunk_desc_bytes(n_seqs, segs.size(), merges.size(), tokens, n_ctas);
     out.desc_bytes = static_cast<int64_t>(need);
     if (desc_bytes < need)
         return set_error(TLE_ERR_INVALID, "descriptor buffer %zu bytes < %zu needed", desc_bytes, need);
     auto* hdr = static_cast<tle::ChunkHeader*>(desc_host);
     *hdr = tle::ChunkHeader{tle::chunk_plan_id(out), n_seqs, out.n_tokens, out.n_ctas, out.n_few_ctas, out.n_segs, out.n_merge};
-    const tle::ChunkDesc d = tle::chunk_desc(desc_host, n_seqs, segs.size(), merges.size(), tokens, out.n_ctas);
+    const tle::ChunkDesc d = tle::chunk_desc(desc_host, n_seqs, segs.size(), merges.size(), n_ctas);
     auto* seq = const_cast<tle::ChunkSeq*>(d.seqs);
     auto* tok = const_cast<tle::ChunkTok*>(d.toks);
-    int32_t first = 0;
     for (int s = 0; s < n_seqs; ++s) {
         const tle_paged_chunk_t& c = chunks[s];
-        seq[s] = tle::ChunkSeq{c.pages, c.n_pages, c.pos, c.n_tokens, first};
-        for (int t = 0; t < c.n_tokens; ++t) tok[first + t] = tle::ChunkTok{s, c.pos + t};
-        first += c.n_tokens;
+        seq[s] = tle::ChunkSeq{c.pages, c.n_pages, c.pos, c.n_tokens, first[s]};
+        for (int t = 0; t < c.n_tokens; ++t) *tok++ = tle::ChunkTok{s, c.pos + t};
     }
+    auto* cta = const_cast<tle::ChunkSeg*>(d.cta);
+    for (const auto& st : start)
+        for (size_t c = 0; c + 1 < st.size(); ++c, ++cta) {
+            *cta = st[c] < st[c + 1] ? segs[st[c]] : tle::ChunkSeg{};
+            cta->seg0 = st[c];
+            cta->seg1 = st[c + 1];
+        }
     std::copy(segs.begin(), segs.end(), const_cast<tle::ChunkSeg*>(d.segs));
     std::copy(merges.begin(), merges.end(), const_cast<tle::ChunkMerge*>(d.merges));
-    std::copy(start[0].begin(), start[0].end(), const_cast<int32_t*>(d.cta_start));
-    std::copy(start[1].begin(), start[1].end(), const_cast<int32_t*>(d.few_start));
     *plan = out;
     return ok();
 } catch (const std::exception& e) {   // the planner's lists: out of host memory
@@ -1812,7 +1825,8 @@ int tle_prefill_bf16_paged(const tle_shape_t* shape, const tle_page_pool_bf16_t*
         return set_error(TLE_ERR_WORKSPACE, "workspace %zu bytes < %zu needed", workspace_bytes, need);
     if (need && !aligned16(workspace)) return set_error(TLE_ERR_INVALID, "workspace must be 16-byte aligned");
     tle::ChunkArgs a{};
-    a.d = tle::chunk_desc(desc_dev, plan->n_seqs, plan->n_segs, plan->n_merge, plan->n_tokens, plan->n_ctas);
+    a.d = tle::chunk_desc(desc_dev, plan->n_seqs, plan->n_segs, plan->n_merge,
+                          static_cast<size_t>(plan->n_ctas) + plan->n_few_ctas);
     a.plan_id = tle::chunk_plan_id(*plan);
     a.n_ctas = plan->n_ctas;
     a.n_few_ctas = plan->n_few_ctas;

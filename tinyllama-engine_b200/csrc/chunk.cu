@@ -217,9 +217,14 @@ constexpr int kKeysOf = F32 ? 64 : 128;      // keys of a block
 template <bool F32>
 constexpr int kBufsOf = F32 ? 2 : 1;         // S and P buffers of a chain
 constexpr int kFlushBlocks = 4;              // fp32: blocks whose PV are summed in tensor memory (48 MMAs)
-constexpr int kRegsControl = 56, kRegsSoftmax = 200, kRegsLaunch = 128;
-static_assert(256 * kRegsControl + 256 * kRegsSoftmax <= CT_THREADS * kRegsLaunch,
-              "setmaxnreg split exceeds the launch register budget");
+constexpr int kRegsLaunch = 128;
+// fp32: the Q loaders hold more (777 tokens behind 16000 rows: 276 us with 72,
+// 291 us with 56, 287 us with 80).
+template <bool F32>
+constexpr int kRegsControl = F32 ? 72 : 56;
+template <bool F32>
+constexpr int kRegsSoftmax = 2 * kRegsLaunch - kRegsControl<F32>;
+static_assert(CT_THREADS == 512, "two warpgroups of either kind: the split uses the launch's registers up");
 constexpr float kExpScale = kScale * kLog2e;
 // The reference maximum moves only when the row's maximum grows by more than
 // 8 (log2 units), so O is rescaled rarely; P <= 2^8.
@@ -231,45 +236,31 @@ constexpr float kMoveThreshold = 8.0f;
 __device__ __forceinline__ int row_token(const ChunkArgs& A, int row) {
     return A.group_mul ? static_cast<int>(__umulhi(static_cast<uint32_t>(row), A.group_mul) >> A.group_shift) : row;
 }
-// Segments [seg0, seg1) of this CTA; none if the descriptor is not the launch's.
-__device__ __forceinline__ void my_segments(const ChunkArgs& A, const int32_t* start, int& seg0, int& seg1) {
-    const uint64_t id = A.d.hdr->id;
-    seg0 = start[blockIdx.x];
-    seg1 = start[blockIdx.x + 1];
-    if (id != A.plan_id) {
-        seg0 = seg1 = 0;
-        if (threadIdx.x == 0) record_error(A.err, kErrBadDesc);
-    }
-}
 // A segment as the kernel's roles see it.
-struct Work {
-    const int32_t* pages;
-    int kvh, row0, n_rows, t0, t1, part;
-    int pos, first;
-    int pos_min, kv_len;   // position of the item's first token; rows of its last token
-    bool dual;
+struct Work : ChunkSeg {
+    __device__ __forceinline__ bool dual() const { return n_rows > kChunkRows; }
     __device__ __forceinline__ bool edge(int n) const { return n * kTile + kTile - 1 > pos_min; }
 };
-__device__ __forceinline__ Work work_at(const ChunkArgs& A, int i) {
-    const ChunkSeg sg = A.d.segs[i];
-    const ChunkSeq sq = A.d.seqs[sg.seq];
-    Work w;
-    w.pages = sq.pages;
-    w.kvh = sg.kvh;
-    w.row0 = sg.row0;
-    w.n_rows = sg.n_rows;
-    w.t0 = sg.t0;
-    w.t1 = sg.t1;
-    w.part = sg.part;
-    w.pos = sq.pos;
-    w.first = sq.first;
-    w.pos_min = sq.pos + row_token(A, sg.row0);
-    w.kv_len = sq.pos + row_token(A, sg.row0 + sg.n_rows - 1) + 1;
-    w.dual = sg.n_rows > kChunkRows;
-    return w;
+// The CTA's record `cta` (its first segment, and the range of all) into shared
+// memory, by one thread; an empty range if the descriptor is not the launch's.
+__device__ __forceinline__ void fetch_first(const ChunkArgs& A, int cta, Work* to) {
+    const uint64_t id = A.d.hdr->id;
+    Work w = *static_cast<const Work*>(A.d.cta + cta);
+    if (id != A.plan_id) {
+        w.seg0 = w.seg1 = 0;
+        record_error(A.err, kErrBadDesc);
+    }
+    *to = w;
 }
-
-constexpr int kWorkCache = 20;
+constexpr int kWorkCache = 20;   // segments of a CTA that are held in shared memory
+// Those behind the first, by a warp that has nothing to do yet.
+__device__ __forceinline__ void fetch_work(const ChunkArgs& A, int seg0, int seg1, Work* to, uint64_t* full) {
+    const int lane = threadIdx.x & 31;
+    for (int i = 4 + lane; i < 4 * kWorkCache; i += 32)
+        if (seg0 + i / 4 < seg1) reinterpret_cast<uint4*>(to)[i] = reinterpret_cast<const uint4*>(A.d.segs + seg0)[i];
+    __syncwarp();
+    if (lane == 0) mbar_arrive(full);
+}
 
 template <bool F32>
 struct ChunkSmem {
@@ -290,6 +281,7 @@ struct ChunkSmem {
     uint64_t s_full[kChains][2], s_free[kChains][2], p_full[kChains][2], p_free[kChains][2];
     int bad[2];                                     // the segment has a non-finite masked V row
     uint32_t tmem_base;
+    uint64_t work_full;
     Work work[kWorkCache];                          // the CTA's first segments
 };
 
@@ -515,15 +507,15 @@ __device__ __noinline__ void chunk_row_exact(const ChunkArgs& A, const Work& w, 
 
 // A producer warp: the K/V tiles of segments [seg0, seg1) in order into a ring
 // of stages; a box (64 rows, within a page) by TMA each.
-template <int STAGES>
-__device__ __forceinline__ void produce_tiles(const ChunkArgs& A, const ChunkTma& M, int seg0, int seg1,
+template <int STAGES, class F>
+__device__ __forceinline__ void produce_tiles(const ChunkArgs& A, const ChunkTma& M, int seg0, int seg1, F&& work_of,
                                               uint16_t (*k)[kTileHalfs], uint16_t (*v)[kTileHalfs], uint64_t* full,
                                               uint64_t* empty, bool& failed) {
     const int lane = threadIdx.x & 31;
     const int pool_rows = A.pool_pages << A.page_shift;   // a box from here on is all zeros
     int ring = 0;
     for (int sg = seg0; sg < seg1; ++sg) {
-        const Work w = work_at(A, sg);
+        const Work w = work_of(sg);
         // lane l holds where box b0 + l starts
         int b0 = 2 * w.t0, y = 0;
         auto refill = [&]() {
@@ -577,6 +569,7 @@ __global__ void __launch_bounds__(CT_THREADS, 1)
     constexpr int CT_STAGES = Smem::kStages, kTerms = Smem::kTerms, kQBufs = Smem::kQBufs, kKeys = kKeysOf<F32>, kBufs = kBufsOf<F32>;
     constexpr int kBlocks = kTile / kKeys;   // of a tile
     constexpr uint32_t kIdS = idesc_bf16_f32(kChunkRows, kKeys);
+    constexpr int kRegsC = kRegsControl<F32>, kRegsS = kRegsSoftmax<F32>;
     extern __shared__ __align__(1024) unsigned char smem_raw[];
     Smem& S = *reinterpret_cast<Smem*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, wg = warp >> 2;
@@ -593,6 +586,7 @@ __global__ void __launch_bounds__(CT_THREADS, 1)
             mbar_init(&S.scanned[i], 1);
             mbar_init(&S.seg_end[i], 4 * kChains);   // one per softmax warp
         }
+        mbar_init(&S.work_full, 1);
         mbar_init(&S.joined, 4 * kChains);
         mbar_init(&S.read, 4 * kChains);
         for (int c = 0; c < kChains; ++c)
@@ -612,18 +606,20 @@ __global__ void __launch_bounds__(CT_THREADS, 1)
     }
     // everything below reads what earlier kernels on the stream wrote
     asm volatile("griddepcontrol.wait;" ::: "memory");
-    int seg0, seg1;
-    my_segments(A, A.d.cta_start, seg0, seg1);
-    if (tid < kWorkCache && seg0 + tid < seg1) S.work[tid] = work_at(A, seg0 + tid);
+    if (tid == 0) fetch_first(A, blockIdx.x, &S.work[0]);
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
+    const int seg0 = S.work[0].seg0, seg1 = S.work[0].seg1;
     const uint32_t tmem = S.tmem_base;
-    auto work_of = [&](int i) { return i - seg0 < kWorkCache ? S.work[i - seg0] : work_at(A, i); };
     bool failed = false;
+    auto work_of = [&](int i) -> const Work& {
+        if (i == seg0 + 1) wait_or_flag(&S.work_full, 0, A.err, kErrWaitFull, failed);
+        return i - seg0 < kWorkCache ? S.work[i - seg0] : *static_cast<const Work*>(A.d.segs + i);
+    };
 
     if (wg == 0) {
-        regs_dealloc<kRegsControl>();
+        regs_dealloc<kRegsC>();
         const int c = uniform(warp & 1);   // the chain
         const uint32_t tm = uniform(tmem);
         int ring = 0, x = 0;   // K/V tiles and own blocks so far
@@ -635,7 +631,7 @@ __global__ void __launch_bounds__(CT_THREADS, 1)
                 const int b = k % kQBufs;
                 const Work w = work_of(seg0 + k);
                 const int t0 = uniform(w.t0), t1 = uniform(w.t1), kv_len = uniform(w.kv_len);
-                const int dual = uniform(static_cast<int>(w.dual));
+                const int dual = uniform(static_cast<int>(w.dual()));
                 const uint32_t qa = q0 + (b * 2 + (dual ? c : 0)) * (kTerms * kTileHalfs * 2);
                 wait_uniform(&S.q_full[b], (k / kQBufs) & 1, A.err, kErrWaitFull, failed);
                 bool any = false;
@@ -679,7 +675,7 @@ __global__ void __launch_bounds__(CT_THREADS, 1)
             for (int k = 0; k < n_seg; ++k) {
                 const Work w = work_of(seg0 + k);
                 const int t0 = uniform(w.t0), t1 = uniform(w.t1), kv_len = uniform(w.kv_len), pos_min = uniform(w.pos_min);
-                const int dual = uniform(static_cast<int>(w.dual));
+                const int dual = uniform(static_cast<int>(w.dual()));
                 uint32_t acc = 0;   // the segment's first block overwrites O, fp32: every kFlushBlocks-th
                 const int x_first = x;
                 for (int n = t0; n < t1; ++n, ++ring) {
@@ -725,11 +721,12 @@ __global__ void __launch_bounds__(CT_THREADS, 1)
                 wait_uniform(&S.p_free[c][y % kBufs], (y / kBufs) & 1, A.err, kErrDrain, failed);
         }
     } else if (wg == 3) {
-        regs_dealloc<kRegsControl>();
+        regs_dealloc<kRegsC>();
         if (warp == 12) {
-            produce_tiles<CT_STAGES>(A, M, seg0, seg1, S.k, S.v, S.kv_full, S.kv_empty, failed);
+            produce_tiles<CT_STAGES>(A, M, seg0, seg1, work_of, S.k, S.v, S.kv_full, S.kv_empty, failed);
         } else if (warp == 13) {
             // -------------------------- V of the edge tiles ----------------------------
+            fetch_work(A, seg0, seg1, S.work, &S.work_full);
             int ring = 0;
             for (int sg = seg0; sg < seg1; ++sg) {
                 const int k = sg - seg0;
@@ -770,42 +767,42 @@ __global__ void __launch_bounds__(CT_THREADS, 1)
                 const int k = sg - seg0, b = k % kQBufs;
                 const Work w = work_of(sg);
                 if (k >= kQBufs) wait_or_flag(&S.q_free[b], ((k / kQBufs) - 1) & 1, A.err, kErrWaitEmpty, failed);
-                // 8 lanes per row, 4 rows per step, half of each row tile per warp
-                const int ch = lane & 7;
-                for (int m = 0; m < (w.dual ? 2 : 1); ++m) {
-                    const int r0 = lw * 64 + (lane >> 3);   // row of the tile
+                // 8 lanes per row, 4 rows per step, the warps alternate; rows behind the
+                // last one stay as they are: nobody looks at their scores
+                const int ch = lane & 7, r0 = 4 * lw + (lane >> 3);
+                for (int m = 0; m < (w.dual() ? 2 : 1); ++m) {
                     RowWalk<const Act> at(A, static_cast<const Act*>(A.q) + ch * 8, A.q_stride, w.first, w.kvh,
                                           w.row0 + m * kChunkRows + r0);
-                    const int left = w.n_rows - m * kChunkRows - r0;   // steps of 4 rows while below
-                    // rows r0 and r0 + 4 and their chunk's place; further rows keep one of the two
-                    const int off[2] = {r0 * HD + ((ch ^ (r0 & 7)) << 3), (r0 + 4) * HD + ((ch ^ ((r0 + 4) & 7)) << 3)};
+                    const int left = w.n_rows - m * kChunkRows - r0;   // steps of 8 rows while below
+                    const int off = r0 * HD + ((ch ^ r0) << 3);        // the chunk's place; 8 rows on it is the same
+                    const int steps = min(16, (w.n_rows - m * kChunkRows + 7) / 8);
                     if constexpr (!F32) {
 #pragma unroll 4
-                        for (int j = 0; j < 16; ++j) {
-                            const bool ok = 4 * j < left;
-                            asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(
-                                             smem_u32(&S.q[b][m][0][off[j & 1] + (j >> 1) * 8 * HD])),
-                                         "l"(ok ? at.p : static_cast<const Act*>(A.q)), "r"(ok ? 16 : 0)
-                                         : "memory");
-                            at.template step<4>(A);
+                        for (int j = 0; j < steps; ++j) {
+                            if (8 * j < left)
+                                asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(
+                                                 smem_u32(&S.q[b][m][0][off + j * 8 * HD])),
+                                             "l"(at.p)
+                                             : "memory");
+                            at.template step<8>(A);
                         }
                     } else {
 #pragma unroll 1
-                        for (int j0 = 0; j0 < 16; j0 += 4) {
+                        for (int j0 = 0; j0 < steps; j0 += 4) {
                             float4 x[4][2];
 #pragma unroll
                             for (int j = 0; j < 4; ++j) {
                                 const float4* src = reinterpret_cast<const float4*>(at.p);
                                 x[j][0] = x[j][1] = make_float4(0.f, 0.f, 0.f, 0.f);
-                                if (4 * (j0 + j) < left) {
+                                if (8 * (j0 + j) < left) {
                                     x[j][0] = src[0];
                                     x[j][1] = src[1];
                                 }
-                                at.template step<4>(A);
+                                at.template step<8>(A);
                             }
 #pragma unroll
                             for (int j = 0; j < 4; ++j) {
-                                const int at_q = off[j & 1] + ((j0 + j) >> 1) * 8 * HD;
+                                const int at_q = off + (j0 + j) * 8 * HD;
                                 float* f = reinterpret_cast<float*>(x[j]);
 #pragma unroll
                                 for (int term = 0; term < kTerms; ++term) {
@@ -827,7 +824,7 @@ __global__ void __launch_bounds__(CT_THREADS, 1)
         }
     } else {
         // ------------------------------ softmax ------------------------------------
-        regs_alloc<kRegsSoftmax>();
+        regs_alloc<kRegsS>();
         const int c = wg - 1;
         const int lr = tid & 127;                      // TMEM lane
         const uint32_t tL = tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16);
@@ -847,8 +844,10 @@ __global__ void __launch_bounds__(CT_THREADS, 1)
         };
         for (int sg = seg0; sg < seg1; ++sg) {
             const int k = sg - seg0;
-            const Work w = work_of(sg);
-            const int r = w.dual ? kChunkRows * c + lr : lr;   // row of the item
+            const Work& w = work_of(sg);   // read again where needed: registers are short here
+            const bool dual = w.dual();
+            const int pos_min = w.pos_min;
+            const int r = dual ? kChunkRows * c + lr : lr;   // row of the item
             const int my_pos = w.pos + row_token(A, w.row0 + min(r, w.n_rows - 1));
             float m_ref = -INFINITY;                   // reference maximum, log2 units
             float l_run = 0.f;
@@ -975,8 +974,8 @@ __global__ void __launch_bounds__(CT_THREADS, 1)
                 if (lane == 0) mbar_arrive(&S.p_full[c][h]);
                 ++x;
             };
-            for (int key = key0 + (w.dual ? 0 : c * kKeys); key < key_end; key += w.dual ? kKeys : 2 * kKeys) {
-                if (key + kKeys - 1 > w.pos_min) block.template operator()<true>(key);
+            for (int key = key0 + (dual ? 0 : c * kKeys); key < key_end; key += dual ? kKeys : 2 * kKeys) {
+                if (key + kKeys - 1 > pos_min) block.template operator()<true>(key);
                 else block.template operator()<false>(key);
             }
             // ---- the segment's result ----
@@ -999,7 +998,7 @@ __global__ void __launch_bounds__(CT_THREADS, 1)
             // memory, 16-byte chunk j of row r at j ^ (r & 7), so that the lanes of a store
             // write whole rows.
             uint4* stage = S.stage[4 * c + (warp & 3)];
-            const int row_base = (w.dual ? kChunkRows * c : 0) + 32 * (warp & 3);   // the warp's rows in the item
+            const int row_base = (dual ? kChunkRows * c : 0) + 32 * (warp & 3);   // the warp's rows in the item
             auto fetch = [&](float (&o)[32], int col, uint32_t t0, float f0, uint32_t t1, float f1, bool two) {
                 tmem_ld32(t0 + col, o);
                 tmem_wait_ld();
@@ -1061,7 +1060,7 @@ __global__ void __launch_bounds__(CT_THREADS, 1)
                 }
             };
             float* lse = mine && w.part >= 0 ? A.part_lse + w.part + r : nullptr;
-            if (w.dual) {
+            if (dual) {
                 if (S.bad[k & 1]) {
                     const Work cold = w;   // a copy, so that w itself stays in registers
                     if (mine) chunk_row_exact<Act>(A, cold, r, row_out<Act>(A, cold, r));
@@ -1134,7 +1133,7 @@ struct FewSmem {
     uint16_t v[FW_STAGES][kTileHalfs];
     float o[FW_WARPS][16][HD + 4];      // a warp's result, and its rows' maximum and sum
     float2 ml[FW_WARPS][16];
-    uint64_t full[FW_STAGES], empty[FW_STAGES];
+    uint64_t full[FW_STAGES], empty[FW_STAGES], work_full;
     int bad[2];                         // the segment has a non-finite V row that not every row attends to
     Work work[kWorkCache];              // the CTA's first segments
 };
@@ -1173,20 +1172,23 @@ __global__ void __launch_bounds__(FW_THREADS, 1)
             mbar_init(&S.full[i], 1);
             mbar_init(&S.empty[i], FW_WARPS);
         }
+        mbar_init(&S.work_full, 1);
         S.bad[0] = S.bad[1] = 0;
         fence_barrier_init();
         prefetch_tmap(&M.k);
         prefetch_tmap(&M.v);
     }
     asm volatile("griddepcontrol.wait;" ::: "memory");
-    int seg0, seg1;
-    my_segments(A, A.d.few_start, seg0, seg1);
-    if (tid < kWorkCache && seg0 + tid < seg1) S.work[tid] = work_at(A, seg0 + tid);
+    if (tid == 0) fetch_first(A, A.n_ctas + blockIdx.x, &S.work[0]);
     __syncthreads();
-    auto work_of = [&](int i) { return i - seg0 < kWorkCache ? S.work[i - seg0] : work_at(A, i); };
+    const int seg0 = S.work[0].seg0, seg1 = S.work[0].seg1;
     bool failed = false;
+    auto work_of = [&](int i) -> const Work& {
+        if (i == seg0 + 1) wait_or_flag(&S.work_full, 0, A.err, kErrWaitFull, failed);
+        return i - seg0 < kWorkCache ? S.work[i - seg0] : *static_cast<const Work*>(A.d.segs + i);
+    };
     if (warp == FW_WARPS) {
-        produce_tiles<FW_STAGES>(A, M, seg0, seg1, S.k, S.v, S.full, S.empty, failed);
+        produce_tiles<FW_STAGES>(A, M, seg0, seg1, work_of, S.k, S.v, S.full, S.empty, failed);
         return;
     }
     const int gid = lane >> 2, tg = lane & 3;     // fragment row and column pair
@@ -1407,7 +1409,8 @@ __global__ void __launch_bounds__(FW_THREADS, 1)
         }
         flush();
     };
-    if (seg0 < seg1) load_q(work_of(seg0));
+    if (seg0 < seg1) load_q(S.work[0]);
+    if (warp == FW_WARPS - 1) fetch_work(A, seg0, seg1, S.work, &S.work_full);
     for (int sg = seg0; sg < seg1; ++sg) {
         const int k = sg - seg0;
         const Work w = work_of(sg);

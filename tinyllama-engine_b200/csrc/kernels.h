@@ -340,14 +340,17 @@ cudaError_t launch_embed_rows(int type, float* x, const void* table, const int32
 
 // ---- chunks of new tokens over a paged cache (chunk.cu) ----
 // Descriptor (built on the host by tle_chunk_desc_paged):
-//   ChunkHeader | ChunkSeq[n_seqs] | ChunkSeg[n_segs] | ChunkMerge[n_merge]
-//   | ChunkTok[n_tokens] | int32 cta_start[n_ctas + 1] | int32 few_start[n_few_ctas + 1]
+//   ChunkHeader | ChunkSeg cta[n_ctas + n_few_ctas] | ChunkSeg[n_segs]
+//   | ChunkSeq[n_seqs] | ChunkMerge[n_merge] | ChunkTok[n_tokens]
 // The attention works on rows: row t * g + h of a chunk and KV head is query
 // head h of the group (g = n_head / n_head_kv) of token t, so that a K/V tile
 // serves all the heads that share it.  An item is a block of kChunkItemRows
 // rows of one (chunk, KV head); a segment a range of kChunkTile-row K/V tiles
 // of one item, done by one CTA; the segments of chunks of at most kChunkFewRows
-// rows come last (few_start), for a kernel of their own.
+// rows come last, for a kernel of their own (the last n_few_ctas of cta).  A
+// CTA's record in cta is a copy of its first segment with the range of its
+// segments, and a segment holds all that its CTA needs, so that between the
+// launch and the first page id there is one load instead of three in a row.
 constexpr int kChunkTile = 128;       // K/V rows per tile
 constexpr int kChunkRows = 128;       // rows per tensor-core tile
 constexpr int kChunkItemRows = 2 * kChunkRows;
@@ -377,12 +380,15 @@ struct ChunkSeq {
     const int32_t* pages;
     int32_t n_pages, pos, n_tokens, first;   // first: batch index of its first token
 };
-struct ChunkSeg {
-    int32_t seq, kvh;
-    int32_t row0, n_rows;    // the item's rows (n_rows <= kChunkItemRows)
-    int32_t t0, t1;          // K/V tiles [t0, t1)
-    int32_t part;            // first row of this segment's partial results; -1: it writes out itself
-    int32_t reserved;
+struct alignas(16) ChunkSeg {
+    const int32_t* pages;
+    int32_t pos, first;        // of the chunk, as in ChunkSeq
+    int32_t kvh, row0, n_rows; // the item's rows (n_rows <= kChunkItemRows)
+    int32_t t0, t1;            // K/V tiles [t0, t1)
+    int32_t part;              // first row of this segment's partial results; -1: it writes out itself
+    int32_t pos_min, kv_len;   // position of the item's first token; rows of its last token
+    int32_t seg0, seg1;        // in cta: the CTA's segments [seg0, seg1)
+    int32_t seq, reserved;
 };
 struct ChunkMerge {          // an item whose results are in n_parts blocks of n_rows partial rows
     int32_t seq, kvh, row0, n_rows, part, n_parts;
@@ -390,32 +396,30 @@ struct ChunkMerge {          // an item whose results are in n_parts blocks of n
 struct ChunkTok {
     int32_t seq, pos;
 };
-static_assert(sizeof(ChunkHeader) == 32 && sizeof(ChunkSeq) == 24 && sizeof(ChunkSeg) == 32 &&
+static_assert(sizeof(ChunkHeader) == 32 && sizeof(ChunkSeq) == 24 && sizeof(ChunkSeg) == 64 &&
                   sizeof(ChunkMerge) == 24 && sizeof(ChunkTok) == 8,
               "chunk descriptor records");
 struct ChunkDesc {           // device pointers into one descriptor
     const ChunkHeader* hdr;
-    const ChunkSeq* seqs;
+    const ChunkSeg* cta;
     const ChunkSeg* segs;
+    const ChunkSeq* seqs;
     const ChunkMerge* merges;
     const ChunkTok* toks;
-    const int32_t* cta_start;
-    const int32_t* few_start;
 };
-inline size_t chunk_desc_bytes(size_t n_seqs, size_t n_segs, size_t n_merge, size_t n_tokens, size_t n_ctas, size_t n_few) {
-    return sizeof(ChunkHeader) + n_seqs * sizeof(ChunkSeq) + n_segs * sizeof(ChunkSeg) + n_merge * sizeof(ChunkMerge) +
-           n_tokens * sizeof(ChunkTok) + (n_ctas + n_few + 2) * sizeof(int32_t);
+inline size_t chunk_desc_bytes(size_t n_seqs, size_t n_segs, size_t n_merge, size_t n_tokens, size_t n_ctas) {
+    return sizeof(ChunkHeader) + (n_ctas + n_segs) * sizeof(ChunkSeg) + n_seqs * sizeof(ChunkSeq) +
+           n_merge * sizeof(ChunkMerge) + n_tokens * sizeof(ChunkTok);
 }
-inline ChunkDesc chunk_desc(const void* base, size_t n_seqs, size_t n_segs, size_t n_merge, size_t n_tokens, size_t n_ctas) {
-    const unsigned char* p = static_cast<const unsigned char*>(base) + sizeof(ChunkHeader);
+// n_ctas: of both kernels
+inline ChunkDesc chunk_desc(const void* base, size_t n_seqs, size_t n_segs, size_t n_merge, size_t n_ctas) {
     ChunkDesc d;
     d.hdr = static_cast<const ChunkHeader*>(base);
-    d.seqs = reinterpret_cast<const ChunkSeq*>(p);
-    d.segs = reinterpret_cast<const ChunkSeg*>(d.seqs + n_seqs);
-    d.merges = reinterpret_cast<const ChunkMerge*>(d.segs + n_segs);
+    d.cta = reinterpret_cast<const ChunkSeg*>(d.hdr + 1);
+    d.segs = d.cta + n_ctas;
+    d.seqs = reinterpret_cast<const ChunkSeq*>(d.segs + n_segs);
+    d.merges = reinterpret_cast<const ChunkMerge*>(d.seqs + n_seqs);
     d.toks = reinterpret_cast<const ChunkTok*>(d.merges + n_merge);
-    d.cta_start = reinterpret_cast<const int32_t*>(d.toks + n_tokens);
-    d.few_start = d.cta_start + n_ctas + 1;
     return d;
 }
 struct AppendArgs {
