@@ -77,7 +77,9 @@ __device__ __forceinline__ void store_n(T* p, const float (&x)[N]) {
 // pairs and fetches those of its own elements from the lanes that have them,
 // once for all units.  HBM-bound: each element is read once and written once;
 // kAppendBatch pieces per lane are in flight (fp32: 2048 tokens 7.8 us with 10, 10.6 us
-// with 4; bf16: 18 k tokens 33 us with 4, 41 us with 8).
+// with 4; bf16: 18 k tokens 33 us with 4, 41 us with 8).  19 600 tokens bf16: 160.6 MB
+// in 32.8 us, 4.9 TB/s; 64 single tokens 3.6 us, the launch and one dependent
+// load after another.
 constexpr int kAppendThreads = 256;
 constexpr int kAppendPart = 4;             // pieces of the smallest part of a token
 constexpr int kAppendWarps = 148 * 16;   // below so many tokens their heads are spread over several warps
@@ -191,6 +193,16 @@ __global__ void __launch_bounds__(kAppendThreads) append_kernel(const __grid_con
 // K and V tiles come by TMA (two 64-row boxes, each inside a page, 128-byte
 // swizzle): K is K-major, V is read MN-major, so nothing is transposed or
 // copied beforehand.
+//
+// What bounds it: with 64 columns a score costs 256 tensor-core operations and
+// one exponential, and the exponential unit (16 a cycle and SM) is the slower of
+// the two: 2048 cycles for 256 x 128 scores; a block takes about 2650 (bf16).
+// 2048 tokens behind 30000 rows, 32 query on 4 KV heads: 660 us, 789 TFLOP/s; ncu:
+// exponential unit 76 % busy, tensor cores 38 %.  Exponentials by polynomial on
+// the FMA units, for a part of the scores: 774 us where this took 669.  Four
+// softmax warpgroups of 64 rows, or two blocks of 64 keys in flight per chain:
+// 881 to 1340 us where this took 700, for registers.  fp32: 777 tokens behind 16000
+// rows 276 us, 378 TFLOP/s of three products each, tensor cores 58 % busy.
 //
 // Precision: bf16 activations: P rounded to bf16 (its sum is not), fp32
 // accumulation.  fp32 activations: q and P are cut into three bf16 numbers of
@@ -1124,9 +1136,11 @@ __global__ void __launch_bounds__(CT_THREADS, 1)
 // shared memory at the segment's end.  K and V come through a ring of TMA
 // tiles as above, kept full across segments by a producer warp.  Precision
 // and the treatment of rows that not every token attends to as above.
+// 64 decode steps of 32 query heads: behind 2047 rows 25.3 us (98.6 MB, 3.9 TB/s;
+// 256 items on 148 CTAs, two at most), behind 8000 rows 67 us (6.1 TB/s).
 constexpr int FW_WARPS = 8;
 constexpr int FW_THREADS = 32 * (FW_WARPS + 1);
-constexpr int FW_STAGES = 4;
+constexpr int FW_STAGES = 4;       // 64 x 1 behind 2047 rows: 25.6 us, with 5 27.4 us
 constexpr int kFewFlush = 8;        // fp32: tiles (of one row group) whose MMAs are summed in a row
 struct FewSmem {
     uint16_t k[FW_STAGES][kTileHalfs];
@@ -1462,7 +1476,8 @@ __global__ void __launch_bounds__(FW_THREADS, 1)
 }
 
 // Items in several partial blocks: out = sum_b w_b o_b / sum_b w_b, w_b =
-// 2^(lse_b - max), in block order.  A warp per row, lane = two columns.
+// 2^(lse_b - max), in block order.  A warp per row, lane = two columns.  About
+// 2.5 us with its launch, which is why the plan cuts items only where that pays.
 constexpr int kMergeThreads = 256;
 template <class Act>
 __global__ void __launch_bounds__(kMergeThreads) chunk_merge_kernel(const __grid_constant__ ChunkArgs A) {
