@@ -23,8 +23,9 @@
 // The slice: 8192 tokens, so that a row's lists are read few times (256 rows of
 // 100003 with lists of 4000 tokens: 63 us, with 4096 tokens 71 us), or 2048 where
 // that would leave SMs idle (one row of 32000: 3.3 us against 5.0 us).  Of the 63 us
-// the 205 MB of logits are 31 us at the copy rate; the rest is counting, of which
-// a row's list is gone through by each of its 13 slices.
+// the 205 MB of logits are 31 us at the copy rate; the rest is the chain of row
+// scalars, lists, counts and results, with three CTAs per SM (74 registers) to hide
+// it.  Held to 64 or 48 registers it spills (67, 92 us); 512 threads a CTA: 71 us.
 #include <math.h>
 #include <stdint.h>
 

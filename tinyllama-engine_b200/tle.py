@@ -9,6 +9,9 @@ exception is raised.
 Names follow the reference: ``rope`` (ops.h:175), ``attention`` (ops.h:204),
 ``rope_attention`` (forward.cpp:192-208 fused), ``DecodeBatch`` (attention()
 for many sequences), ``prefill`` (generate.cpp:56-59 as one causal kernel).
+Without a counterpart there: ``PagedChunkBatch`` (chunks of new tokens over a
+paged cache) and ``logits_adjust`` (penalties, biases and masks before a
+sampler).
 """
 from __future__ import annotations
 
