@@ -57,7 +57,20 @@ def test_plan_covers_every_tile_once(seed):
     pos = [int(x) for x in r.integers(0, 5000, n)]
     new = [int(x) for x in r.integers(0, [2, 40, 700][seed % 3], n)]
     heads = [(32, 4), (8, 8), (20, 4), (7, 1)][seed % 4]
-    max_ctas = [0, 1, 3, 148][int(r.integers(0, 4))]
+    check_plan(pos, new, heads, [0, 1, 3, 148][int(r.integers(0, 4))])
+
+
+@pytest.mark.parametrize("pos,new,heads", [
+    ([0, 9], [40000, 5], (32, 4)),                       # more items than are sorted
+    ([500] * 300, [1] * 300, (32, 32)),                  # the same of few rows
+    ([1 << 20, 5], [1, 300], (32, 4)),                   # one item far longer than the others
+])
+def test_plan_of_many_or_uneven_items(pos, new, heads):
+    check_plan(pos, new, heads, 0)
+
+
+def check_plan(pos, new, heads, max_ctas):
+    n = len(pos)
     rc, buf, plan = describe(pos, new, heads, max_ctas=max_ctas)
     assert rc == 0, tle.lib().tle_last_error()
     g = heads[0] // heads[1]

@@ -77,10 +77,11 @@ __device__ __forceinline__ void store_n(T* p, const float (&x)[N]) {
 // pairs and fetches those of its own elements from the lanes that have them,
 // once for all units.  HBM-bound: each element is read once and written once;
 // kAppendBatch pieces per lane are in flight (fp32: 2048 tokens 7.8 us with 10, 10.6 us
-// with 4; bf16: 18 k tokens 33 us with 4, 41 us with 8).  19 600 tokens bf16: 160.6 MB
-// in 32.8 us, 4.9 TB/s; 64 single tokens 3.6 us, the launch and one dependent
+// with 4; bf16: 18 k tokens 33 us with 4, 41 us with 8).  18 k tokens bf16: 160.6 MB
+// in 31.7 us, 5.1 TB/s (small blocks leave their places to the next ones soon: 256
+// threads 33.0 us); 64 single tokens 3.6 us, the launch and one dependent
 // load after another.
-constexpr int kAppendThreads = 256;
+constexpr int kAppendThreads = 64;
 constexpr int kAppendPart = 4;             // pieces of the smallest part of a token
 constexpr int kAppendWarps = 148 * 16;   // below so many tokens their heads are spread over several warps
 
