@@ -91,8 +91,13 @@ def check_plan(pos, new, heads, max_ctas):
     assert np.array_equal(segs[:, PAGES], 0x4000 * (segs[:, SEQ] + 1))
     assert np.array_equal(segs[:, POS_MIN], segs[:, POS] + segs[:, ROW0] // g)
     assert np.array_equal(segs[:, KV_LEN], segs[:, POS] + (segs[:, ROW0] + segs[:, ROWS] - 1) // g + 1)
-    items = {(s, h, r0): min(ITEM, new[s] * g - r0) for s in range(n) for h in range(heads[1])
-             for r0 in range(0, new[s] * g, ITEM)}
+    items = {(s, h, r0): rows for s, h, r0, rows in segs[:, [SEQ, KVH, ROW0, ROWS]]}
+    starts = {}                                                        # blocks of rows, each row in one
+    for s, h, r0 in sorted(items):
+        at = starts.get((s, h), 0)
+        assert r0 == at and r0 % (ITEM // 2) == 0 and 0 < items[(s, h, r0)] <= ITEM
+        starts[(s, h)] = at + items[(s, h, r0)]
+    assert starts == {(s, h): new[s] * g for s in range(n) for h in range(heads[1]) if new[s]}
     seen, parts = {k: [] for k in items}, {}
     used = np.zeros(plan.part_rows, int)
     for s, h, r0, rows, t0, t1, part in segs[:, [SEQ, KVH, ROW0, ROWS, T0, T1, PART]]:

@@ -4,6 +4,7 @@
 // tle_last_error().
 #include <algorithm>
 #include <functional>
+#include <tuple>
 #include <utility>
 #include <cmath>
 #include <cstdarg>
@@ -1453,7 +1454,7 @@ int check_chunks(const tle_shape_t* shape, int page_rows, const tle_paged_chunk_
 constexpr int64_t kSegUnits = 4, kFewSegUnits = 2;
 // How far above the even share the longest CTA may be before items are cut:
 // what the partial results and the launch that joins them cost.  6 x 509 tokens
-// behind 1999 rows, bf16: 67.2 us with 16, 73.7 us with 8 (cut); 3 x 300 tokens
+// behind 1999 rows, bf16: 67.2 us with 16, 73.7 us with 8 (cut), both without halves; 3 x 300 tokens
 // behind 4000 rows, fp32: 79 us with 16 (cut), 93 us with 32.
 constexpr int64_t kJoinUnits = 16;
 constexpr int64_t kMaxWholeItems = 4096;    // sorted on the host, a few tenths of a millisecond
@@ -1474,44 +1475,77 @@ struct ChunkPlanner {
         int64_t cost() const { return static_cast<int64_t>(tiles) * unit(); }
     };
 
+    Item item(int seq, int kvh, int row0, int n_rows) const {
+        const int g = shape->n_head / shape->n_head_kv;
+        return Item{seq, kvh, row0, n_rows, (chunks[seq].pos + (row0 + n_rows - 1) / g) / tle::kChunkTile + 1};
+    }
+
     template <class F>
     void each_item(bool few, F&& f) const {
         const int g = shape->n_head / shape->n_head_kv;
         for (int s = 0; s < n_seqs; ++s)
             for (int h = 0; h < shape->n_head_kv; ++h) {
                 const int rows = chunks[s].n_tokens * g;
-                for (int r = 0; r < rows; r += tle::kChunkItemRows) {
-                    Item it{s, h, r, std::min(tle::kChunkItemRows, rows - r), 0};
-                    it.tiles = (chunks[s].pos + (r + it.n_rows - 1) / g) / tle::kChunkTile + 1;
-                    if ((rows <= tle::kChunkFewRows) == few) f(it);
-                }
+                if ((rows <= tle::kChunkFewRows) != few) continue;
+                for (int r = 0; r < rows; r += tle::kChunkItemRows) f(item(s, h, r, std::min(tle::kChunkItemRows, rows - r)));
             }
     }
 
-    // Whole items, longest first (see run); false if they do not balance.
+    // Whole items, longest first, each to the CTA with the least so far; returns
+    // the cost of the longest CTA.  halves: an item of more than kChunkRows rows
+    // that would leave its CTA above the even share is taken as two instead.
+    int64_t deal(std::vector<Item> items, bool halves, int64_t share, int64_t seg_units,
+                 std::vector<std::pair<int, Item>>& owner) const {
+        auto less = [](const Item& a, const Item& b) {   // a total order: the plan is the same every time
+            return std::make_tuple(a.cost(), b.seq, b.kvh, b.row0) < std::make_tuple(b.cost(), a.seq, a.kvh, a.row0);
+        };
+        std::make_heap(items.begin(), items.end(), less);
+        std::vector<std::pair<int64_t, int>> load;   // (cost so far, CTA), the least on top
+        for (int c = 0; c < max_ctas; ++c) load.emplace_back(0, c);
+        int64_t most = 0;
+        while (!items.empty()) {
+            std::pop_heap(items.begin(), items.end(), less);
+            const Item it = items.back();
+            items.pop_back();
+            if (halves && it.n_rows > tle::kChunkRows && load.front().first + it.cost() + seg_units > share) {
+                for (int r = 0; r < it.n_rows; r += tle::kChunkRows) {
+                    items.push_back(item(it.seq, it.kvh, it.row0 + r, std::min(tle::kChunkRows, it.n_rows - r)));
+                    std::push_heap(items.begin(), items.end(), less);
+                }
+                continue;
+            }
+            std::pop_heap(load.begin(), load.end(), std::greater<>());
+            auto& h = load.back();
+            owner.emplace_back(h.second, it);
+            h.first += it.cost() + seg_units;
+            most = std::max(most, h.first);
+            std::push_heap(load.begin(), load.end(), std::greater<>());
+        }
+        return most;
+    }
+
+    // Every item, or its halves, by one CTA (see run); false if that does not balance.
     template <class S>
     bool whole(bool few, int64_t n_items, int64_t total, int64_t seg_units, S&& seg) const {
         std::vector<Item> items;
-        items.reserve(static_cast<size_t>(n_items));
+        items.reserve(static_cast<size_t>(n_items) * 2);
         each_item(few, [&](const Item& it) { items.push_back(it); });
-        std::stable_sort(items.begin(), items.end(), [](const Item& a, const Item& b) { return a.cost() > b.cost(); });
-        const int G = max_ctas;
-        std::vector<std::pair<int64_t, int>> heap;   // (cost so far, CTA), the least on top
-        for (int c = 0; c < G; ++c) heap.emplace_back(0, c);
-        std::vector<std::pair<int, int>> owner;      // (CTA, item)
-        owner.reserve(items.size());
-        int64_t most = 0;
-        for (size_t i = 0; i < items.size(); ++i) {
-            std::pop_heap(heap.begin(), heap.end(), std::greater<>());
-            auto& h = heap.back();
-            owner.emplace_back(h.second, static_cast<int>(i));
-            h.first += items[i].cost() + seg_units;
-            most = std::max(most, h.first);
-            std::push_heap(heap.begin(), heap.end(), std::greater<>());
+        std::vector<std::pair<int, Item>> owner, owner2;   // CTA, item
+        const int64_t share = (total + max_ctas - 1) / max_ctas;
+        int64_t most = deal(items, false, share, seg_units, owner);
+        if (!few && most > share) {
+            // halves read K and V twice, but need no joining: 20 ragged chunks of up to
+            // 100 tokens behind up to 2000 rows, bf16, 47.1 us, whole 49.9 us; 40 of 40
+            // behind 1000, fp32, 51.7 and 57.6 us; 6 of 509 behind 1999, bf16, 63.2 and 65.4 us
+            const int64_t most2 = deal(items, true, share, seg_units, owner2);
+            if (most2 < most) {
+                most = most2;
+                owner.swap(owner2);
+            }
         }
-        if (most > total / G + kJoinUnits) return false;
-        std::sort(owner.begin(), owner.end());
-        for (const auto& o : owner) seg(o.first, items[o.second], 0, items[o.second].tiles, 1, 0);
+        if (most > total / max_ctas + kJoinUnits) return false;
+        std::stable_sort(owner.begin(), owner.end(), [](const auto& a, const auto& b) { return a.first < b.first; });
+        for (const auto& o : owner) seg(o.first, o.second, 0, o.second.tiles, 1, 0);
         return true;
     }
 
@@ -1694,14 +1728,14 @@ extern "C" {
 
 size_t tle_chunk_desc_bytes(const tle_shape_t* shape, const tle_paged_chunk_t* chunks, int n_seqs, int max_ctas) {
     if (check_chunks(shape, 0, chunks, n_seqs)) return 0;
-    // a bound that needs no plan: cuts add at most a piece per CTA to an item each
+    // a bound that needs no plan: two halves of every item, or cuts, at most one per CTA
     const size_t g = static_cast<size_t>(shape->n_head / shape->n_head_kv), G = static_cast<size_t>(chunk_ctas(max_ctas));
     size_t tokens = 0, items = 0;
     for (int s = 0; s < n_seqs; ++s) {
         tokens += static_cast<size_t>(chunks[s].n_tokens);
         items += (chunks[s].n_tokens * g + tle::kChunkItemRows - 1) / tle::kChunkItemRows;
     }
-    return tle::chunk_desc_bytes(n_seqs, items * shape->n_head_kv + 2 * G, 2 * G, tokens, 2 * G);
+    return tle::chunk_desc_bytes(n_seqs, 2 * items * shape->n_head_kv + 2 * G, 2 * G, tokens, 2 * G);
 }
 
 int tle_chunk_desc_paged(const tle_shape_t* shape, int page_rows, const tle_paged_chunk_t* chunks, int n_seqs,

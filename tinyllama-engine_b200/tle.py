@@ -253,14 +253,20 @@ def _stream(stream) -> int:
     return int(stream.cuda_stream)
 
 
+_current_stream = _current_device = None   # torch's functions, looked up at the first call
+
+
 def _raw_stream(stream, index: int) -> int:
     """Handle of `stream`, or of the current stream of device `index`, which
     becomes the current device of a call made under _on_device."""
-    import torch
+    global _current_stream
     if stream is None:
-        # the handle without a Stream object around it, 1.5 us less, where torch offers it
-        raw = getattr(torch._C, "_cuda_getCurrentRawStream", None)
-        return raw(index) if raw else torch.cuda.current_stream(index).cuda_stream
+        if _current_stream is None:
+            import torch
+            # the handle without a Stream object around it, 1.5 us less, where torch offers it
+            _current_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or \
+                (lambda i: torch.cuda.current_stream(i).cuda_stream)
+        return _current_stream(index)
     if stream.device.index != index:
         raise ValueError(f"stream of {stream.device}, tensors on cuda:{index}")
     return stream.cuda_stream
@@ -268,10 +274,14 @@ def _raw_stream(stream, index: int) -> int:
 
 def _on_device(index: int, fn, *args) -> None:
     """fn(*args), checked, with device `index` current."""
-    import torch
-    if torch.cuda.current_device() == index:
+    global _current_device
+    if _current_device is None:
+        import torch
+        _current_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
+    if _current_device() == index:
         rc = fn(*args)
     else:
+        import torch
         with torch.cuda.device(index):
             rc = fn(*args)
     if rc != TLE_OK:
@@ -989,6 +999,7 @@ class LogitRules:
         sizes = {"token_start": n_rows + 1, "bias_start": n_rows + 1, "n_prompt": n_rows, "repetition": n_rows,
                  "frequency": n_rows, "presence": n_rows}
         self.n_rows, self.n_vocab = int(n_rows), int(n_vocab)
+        self._f32 = torch.float32
         self.device = None
         for name, dt in self._GROUPS:
             t = given[name]
@@ -1026,6 +1037,16 @@ class LogitRules:
             for n in ("tokens", "repetition", "frequency", "presence"):
                 setattr(self.desc, n, None)
 
+    def _rows(self, t, index: int, name: str):
+        """Pointer and row stride of the logits that the rules are for."""
+        n, v = self.n_rows, self.n_vocab
+        strides = t.stride()
+        if t.dtype is not self._f32 or tuple(t.shape) != (n, v) or (v > 1 and strides[1] != 1):
+            raise ValueError(f"{name}: need float32 CUDA [{n}][{v}], rows contiguous")
+        if index < 0 or t.get_device() != index:
+            raise ValueError(f"{name}: is on {t.device}, need " + (f"cuda:{index}" if index >= 0 else "a CUDA device"))
+        return t.data_ptr(), (strides[0] if n > 1 else v)
+
     def _same(self, t, name):
         self.device = self.device or t.device
         if t.device != self.device:
@@ -1037,19 +1058,11 @@ def logits_adjust(out, logits, rules: LogitRules, stream=None) -> None:
     float32 CUDA tensors [n_rows][n_vocab] with contiguous rows and any row
     stride; out may be logits.  Before sample_argmax / sample_temperature /
     sample_top_p."""
-    import torch
-    n, v = rules.n_rows, rules.n_vocab
     index = rules.index if rules.index is not None else logits.get_device()
-    at = []
-    for t, name in ((out, "out"), (logits, "logits")):
-        shape, strides = t.shape, t.stride()
-        if t.dtype is not torch.float32 or not t.is_cuda or len(shape) != 2 or shape[0] != n or shape[1] != v or \
-                (v > 1 and strides[1] != 1):
-            raise ValueError(f"{name}: need float32 CUDA [{n}][{v}], rows contiguous")
-        if t.get_device() != index:
-            raise ValueError(f"{name}: is on {t.device}, the rules on cuda:{index}")
-        at += [t.data_ptr(), strides[0] if n > 1 else v]
-    _on_device(index, lib().tle_logits_adjust, *at, n, v, rules.desc_ref, _raw_stream(stream, index))
+    op, os = rules._rows(out, index, "out")
+    lp, ls = rules._rows(logits, index, "logits")
+    _on_device(index, lib().tle_logits_adjust, op, os, lp, ls, rules.n_rows, rules.n_vocab, rules.desc_ref,
+               _raw_stream(stream, index))
 
 
 class DeviceModel:
