@@ -369,6 +369,35 @@ def test_long_fp32_sums_do_not_drift(cuda, new):
     assert float(((c.out.double() - want).abs() / want).max()) <= tol
 
 
+@pytest.mark.parametrize("act", ["f32", "bf16"])
+def test_a_long_prompt_at_some_tokens(cuda, act):
+    """20000 tokens at once (more blocks of rows than the plan sorts), some
+    tokens of it against the formula; tolerance as above."""
+    import torch
+    import tle
+    c = Case([37], [20000], act=act, seed=17, layers=1)
+    c.batch.attend(c.q, c.out, c.layer)
+    torch.cuda.synchronize()
+    rows = torch.from_numpy(c.flat_rows(0, np.arange(20037))).cuda()
+    at = torch.tensor([0, 1, 90, 91, 127, 128, 4095, 9999, 15000, 19998, 19999], device="cuda")
+    hide = torch.arange(20037, device="cuda")[None, :] > 37 + at[:, None]
+    u = U["bf16" if act == "bf16" else "f32"]
+    for h in range(0, c.H, 5):
+        sl = slice(h // 8 * HD, (h // 8 + 1) * HD)
+        k = c.cache.key_pool[0].view(-1, c.KH * HD)[rows, sl].double()
+        v = c.cache.value_pool[0].view(-1, c.KH * HD)[rows, sl].double()
+        q = c.q[at, h * HD:(h + 1) * HD].double()
+        e = (q @ k.T / 8).masked_fill(hide, -float("inf"))
+        w = torch.softmax(e, 1)
+        ds = 2.0 ** -17 * float((q.abs() @ k.abs().T / 8).max())
+        rel = 2 * (ds + float(e[~hide].abs().max()) * 2.0 ** -23 + 2.0 ** -22) + (20037 / 16 + 16) * 2.0 ** -23
+        rel += 2.0 ** -8 + 2.0 ** -13 if act == "bf16" else 0.0
+        want = w @ v
+        tol = rel * (w @ v.abs()) + u * (want.abs() + rel * (w @ v.abs()))
+        assert bool(((c.out[at, h * HD:(h + 1) * HD].double() - want).abs() <= tol).all())
+    assert tle.device_error() == 0
+
+
 def test_tensors_are_checked(cuda):
     import torch
     import tle

@@ -195,6 +195,26 @@ def test_a_bias_does_not_lift_the_mask(cuda, biases):
     assert not bool((out[0][ok] == -float("inf")).all())
 
 
+def test_the_most_rows(cuda):
+    """65535 rows, each with a token list of its own."""
+    import torch
+    import tle
+    n, V = 65535, 37
+    g = torch.Generator(device="cuda").manual_seed(12)
+    x = torch.randn(n, V, generator=g, device="cuda")
+    ids = torch.randint(0, V, (n, 2), generator=g, device="cuda", dtype=torch.int32)
+    rep = 1 + torch.rand(n, generator=g, device="cuda")
+    R = tle.LogitRules(n, V, tokens=ids.flatten(), token_start=torch.arange(0, 2 * n + 1, 2, dtype=torch.int32, device="cuda"),
+                       repetition=rep)
+    out = torch.empty_like(x)
+    tle.logits_adjust(out, x, R)
+    seen = torch.zeros(n, V, dtype=torch.bool, device="cuda").scatter_(1, ids.long(), True)
+    want = torch.where(seen, torch.where(x > 0, x.double() / rep.double()[:, None], x.double() * rep.double()[:, None]), x.double())
+    assert bool(((out.double() - want).abs() <= 2.0 ** -23 * want.abs()).all())
+    with pytest.raises(tle.TleError):
+        tle.logits_adjust(torch.empty(n + 1, 1, device="cuda"), torch.empty(n + 1, 1, device="cuda"), tle.LogitRules(n + 1, 1))
+
+
 def test_one_mask_for_all_rows(cuda):
     import torch
     import tle
