@@ -1291,17 +1291,17 @@ __global__ void __launch_bounds__(FW_THREADS, 1)
             flushed = true;
             since = 0;
         };
-        for (int n = w.t0; n < w.t1; ++n, ++ring) {
+        // Tile n; EDGE: some row does not attend to all of it.
+        auto tile = [&]<bool EDGE>(int n) {
             if (F32 && ++since > kFewFlush / rgroups) flush();
             const int st = ring % FW_STAGES;
             wait_or_flag(&S.full[st], (ring / FW_STAGES) & 1, A.err, kErrWaitFull, failed);
             __syncwarp();
             const uint32_t kb = smem_u32(S.k[st]), vb = smem_u32(S.v[st]);
-            const bool edge = w.edge(n);
             for (int j0 = kg * keys; j0 < (kg + 1) * keys; j0 += 16) {   // 16 keys
                 const int key0 = n * kTile + j0;
-                if (key0 >= w.kv_len) break;
-                if (edge) {
+                if (EDGE && key0 >= w.kv_len) break;
+                if constexpr (EDGE) {
                     // V rows behind the last one: zero; rows only some attend to: finite?
                     bool bad = false;
 #pragma unroll
@@ -1341,20 +1341,18 @@ __global__ void __launch_bounds__(FW_THREADS, 1)
                     ldsm4_t(vb + r * (HD * 2) + ((ch ^ (r & 7)) << 4), vf[dp]);
                 }
                 float s[kRows][4];   // row, keys key0 + 2 tg (+1), key0 + 8 + 2 tg (+1)
+                float mt[kRows];
+                bool grow = false;   // m_ref is the same in the four lanes of a row
 #pragma unroll
-                for (int e = 0; e < kRows; ++e)
+                for (int e = 0; e < kRows; ++e) {
 #pragma unroll
                     for (int q = 0; q < 4; ++q) {
                         const int b = q >> 1, i = 2 * e + (q & 1);
                         if (!F32) s[e][q] = sf[0][b][i];
                         else if (HALF) s[e][q] = sf[0][b][i] + (sf[0][b][i + 2] + sf[kFrags - 1][b][i]);
                         else s[e][q] = sf[0][b][i] + (sf[kFrags > 1 ? 1 : 0][b][i] + sf[kFrags - 1][b][i]);
-                        if (edge && key0 + 8 * b + 2 * tg + (q & 1) > pos_r[e]) s[e][q] = -INFINITY;
+                        if (EDGE && key0 + 8 * b + 2 * tg + (q & 1) > pos_r[e]) s[e][q] = -INFINITY;
                     }
-                float mt[kRows];
-                bool grow = false;   // m_ref is the same in the four lanes of a row
-#pragma unroll
-                for (int e = 0; e < kRows; ++e) {
                     mt[e] = fmax3(fmax3(s[e][0], s[e][1], s[e][2]), s[e][3], s[e][3]) * kExpScale;
                     grow |= m_ref[e] == m_ref[e] && !(mt[e] <= m_ref[e] + kMoveThreshold);
                 }
@@ -1412,9 +1410,13 @@ __global__ void __launch_bounds__(FW_THREADS, 1)
                         mma16816(o[2 * dp + 1], pf[f], vf[dp][2], vf[dp][3]);
                     }
             }
-            if (edge) fence_proxy_async_smem();   // zeroed rows: before the stage's next TMA load
+            if (EDGE) fence_proxy_async_smem();   // zeroed rows: before the stage's next TMA load
             __syncwarp();
             if (lane == 0) mbar_arrive(&S.empty[st]);
+        };
+        for (int n = w.t0; n < w.t1; ++n, ++ring) {
+            if (w.edge(n)) tile.template operator()<true>(n);
+            else tile.template operator()<false>(n);
         }
 #pragma unroll
         for (int e = 0; e < kRows; ++e) {
