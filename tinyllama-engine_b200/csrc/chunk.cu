@@ -1137,11 +1137,13 @@ __global__ void __launch_bounds__(CT_THREADS, 1)
 // shared memory at the segment's end.  K and V come through a ring of TMA
 // tiles as above, kept full across segments by a producer warp.  Precision
 // and the treatment of rows that not every token attends to as above.
-// 64 decode steps of 32 query heads: behind 2047 rows 25.3 us (98.6 MB, 3.9 TB/s;
-// 256 items on 148 CTAs, two at most), behind 8000 rows 67 us (6.1 TB/s).
+// 64 decode steps of 32 query heads: behind 1024 to 2047 rows 24.6 us (fp32; 98.6 MB,
+// 4.0 TB/s, of which launch, start and end are 8 us), behind 8000 rows 84.8 us (bf16;
+// 525 MB, 6.2 TB/s).  Tiles that every row attends to have code of their own: 24.8
+// us, with one code for both 25.7; two such tiles side by side per warp 25.4.
 constexpr int FW_WARPS = 8;
 constexpr int FW_THREADS = 32 * (FW_WARPS + 1);
-constexpr int FW_STAGES = 4;       // 64 x 1 behind 2047 rows: 25.6 us, with 5 27.4 us
+constexpr int FW_STAGES = 4;       // 64 x 1 behind 2047 rows: 25.8 us, with 3 the same, with 5 28.4 us
 constexpr int kFewFlush = 8;        // fp32: tiles (of one row group) whose MMAs are summed in a row
 struct FewSmem {
     uint16_t k[FW_STAGES][kTileHalfs];

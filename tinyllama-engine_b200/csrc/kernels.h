@@ -355,9 +355,9 @@ constexpr int kChunkTile = 128;       // K/V rows per tile
 constexpr int kChunkRows = 128;       // rows per tensor-core tile
 constexpr int kChunkItemRows = 2 * kChunkRows;
 // The kernel for few rows pays while a 128-row tensor-core tile is mostly empty.
-// 32 sequences behind 2000 rows: 32 rows 22.4 us (bf16) and 35.3 us (fp32),
-// against 24.2 and 37.4 us by the other kernel; 64 rows 34.1 and 57.0 against
-// 25.0 and 38.7 us.
+// 32 sequences behind 2000 rows: 32 rows 19.9 us (bf16) and 31.8 us (fp32),
+// against 22.5 and 39.8 us by the other kernel; 64 rows, while this kernel took
+// them, 34.1 and 57.0 against 25.0 and 38.7 us.
 constexpr int kChunkFewRows = 32;
 struct ChunkHeader {
     uint64_t id;             // chunk_plan_id of the plan
