@@ -683,3 +683,70 @@ def test_a_serving_step_with_sampling(cuda):
     torch.cuda.synchronize()
     assert torch.equal(tok.long(), adj.argmax(1)) and int(tok[1]) != top
     assert tle.device_error() == 0
+
+
+# ------------------------------------------- captured calls and larger plans
+def grown(c, pos, new, room):
+    """c's batch over tables for `room` rows per sequence, planned for pos, new."""
+    import torch
+    import tle
+    c.page = 64
+    c.cache = tle.PagedKVCache(len(pos) * (room // 64) + 1, 64, c.cache.shape, dtype=torch.bfloat16)
+    g = torch.Generator(device="cuda").manual_seed(77)
+    for pool in (c.cache.key_pool, c.cache.value_pool):
+        pool.copy_(torch.randn(pool.shape, generator=g, device="cuda"))
+    c.tables = [c.cache.table(c.cache.alloc(room // 64)) for _ in pos]
+    c.batch = tle.PagedChunkBatch(c.cache, c.tables, pos, new)
+
+
+@pytest.mark.parametrize("pos,new,large", [
+    ([700], [1], ([5000], [1])),                        # the same tokens, more pieces: a larger workspace
+    ([700], [1], ([6000], [300])),                      # more tokens: descriptor and q buffer too
+    ([700, 3], [5, 40], ([4000, 5000], [60, 200])),
+])
+def test_a_replay_after_a_larger_plan_uses_no_freed_buffer(cuda, pos, new, large):
+    """Captured under a small plan, replayed after a larger one replaced the
+    batch's buffers: 0x10b and nothing is written, neither pools nor results
+    nor memory that was handed out since; right again under the small plan."""
+    import torch
+    import tle
+    c = Case(pos, new, seed=40)
+    grown(c, pos, new, 6400)
+    c.batch.run(c.q, c.k, c.v, c.out, c.layer)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        c.batch.run(c.q, c.k, c.v, c.out, c.layer)
+    graph.replay()
+    torch.cuda.synchronize()
+    want, plan = c.out.clone(), bytes(c.batch.plan)
+    held = [t for t in (c.batch._desc_dev, c.batch.workspace, c.batch._q[c.q.dtype])]
+    places = [(t.data_ptr(), t.numel() * t.element_size()) for t in held]
+    sizes = [(t.numel(), t.dtype) for t in held]
+    del held
+    big = Case(large[0], large[1], seed=41)
+    c.batch.set_positions(*large)
+    assert bytes(c.batch.plan) != plan
+    c.batch.run(big.q, big.k, big.v, big.out, c.layer)
+    torch.cuda.synchronize()
+    others = [torch.full((n * 4 if dt == torch.uint8 else n,), 77, dtype=dt, device="cuda") for n, dt in sizes for _ in range(8)]
+    for t in others:                                    # what the graph uses is nobody else's
+        a, n = t.data_ptr(), t.numel() * t.element_size()
+        assert all(a + n <= p or p + m <= a for p, m in places)
+    pools = (c.cache.key_pool.clone(), c.cache.value_pool.clone())
+    c.out.fill_(3)
+    graph.replay()
+    torch.cuda.synchronize()
+    assert tle.device_error() == 0x10b
+    assert bool((c.out == 3).all())
+    assert torch.equal(pools[0], c.cache.key_pool) and torch.equal(pools[1], c.cache.value_pool)
+    c.batch.set_positions(pos, new)
+    assert bytes(c.batch.plan) == plan
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(c.out, want) and tle.device_error() == 0
+    c.out.fill_(3)
+    c.batch.run(c.q, c.k, c.v, c.out, c.layer)
+    torch.cuda.synchronize()
+    assert torch.equal(c.out, want)
+    assert all(bool((t == 77).all()) for t in others)

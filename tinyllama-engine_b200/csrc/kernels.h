@@ -364,7 +364,7 @@ struct ChunkHeader {
     int32_t n_seqs, n_tokens, n_ctas, n_few_ctas, n_segs, n_merge;
 };
 // A number for everything in a plan that a launch depends on (FNV-1a over its
-// fields).  A kernel does nothing (kErrBadDesc) unless the descriptor carries
+// fields; never 0, which marks a descriptor of no plan).  A kernel does nothing (kErrBadDesc) unless the descriptor carries
 // the number of the plan that it was launched with: a captured launch that is
 // replayed after the descriptor was replaced would walk the new one with the
 // old one's offsets.
@@ -374,7 +374,7 @@ inline uint64_t chunk_plan_id(const tle_chunk_plan_t& p) {
     uint64_t h = 0xcbf29ce484222325ull;
     for (int64_t f : fields)
         for (int b = 0; b < 64; b += 8) h = (h ^ ((static_cast<uint64_t>(f) >> b) & 0xffu)) * 0x100000001b3ull;
-    return h;
+    return h ? h : 1;
 }
 struct ChunkSeq {
     const int32_t* pages;

@@ -679,7 +679,10 @@ class PagedChunkBatch:
     descriptor and workspace: they must not overlap on the GPU, nor
     ``set_positions`` with a call that still runs on another stream.  A
     captured call belongs to its plan: replayed after ``set_positions`` made
-    another one it does nothing and tle_device_error reports 0x10b.
+    another one it does nothing and tle_device_error reports 0x10b, under a
+    plan with the same numbers it is right.  Buffers that a larger plan
+    replaced stay with the batch for such calls, so the batch has to live as
+    long as a graph that holds a call of it.
     """
 
     def __init__(self, cache: PagedKVCache, tables: Sequence, positions: Sequence[int],
@@ -706,6 +709,8 @@ class PagedChunkBatch:
         self.plan = ChunkPlan()
         self._desc_dev = self.workspace = self._pool_made = None
         self._q = {}
+        self._descs = []        # every descriptor buffer so far, _desc_dev the last
+        self._old = []          # workspaces and q buffers that larger ones replaced
         self._streams = set()   # handles of the streams that the buffers below are known to be used on
         self.set_positions(positions, lengths, stream)
 
@@ -735,18 +740,31 @@ class PagedChunkBatch:
         with torch.cuda.device(self.device):
             host = self.build_host(positions, lengths)   # a new one: the last upload may be pending
             with torch.cuda.stream(stream or torch.cuda.current_stream()):
-                if self._desc_dev is None or self._desc_dev.numel() < host.numel():
-                    # with room for the plans of later positions
-                    self._desc_dev = torch.empty(host.numel() * 5 // 4 + 4096, dtype=torch.uint8, device=self.device)
-                    self._streams.clear()
                 nbytes = lib().tle_prefill_bf16_paged_workspace_bytes(ctypes.byref(self.plan))
                 if self.workspace is None or self.workspace.numel() * 4 < nbytes:
-                    self.workspace = torch.empty(max(nbytes // 4, 4), dtype=torch.float32, device=self.device)
+                    # as far above the old one, so that few are ever kept
+                    room = max(nbytes // 4, 4) if self.workspace is None else max(nbytes // 4, self.workspace.numel() * 5 // 4)
+                    self._keep(self.workspace)
+                    self.workspace = torch.empty(room, dtype=torch.float32, device=self.device)
+                    self._streams.clear()
+                if self._desc_dev is None or self._desc_dev.numel() < host.numel():
+                    # with room for the plans of later positions; the old one may be in a graph
+                    self._desc_dev = torch.empty(host.numel() * 5 // 4 + 4096, dtype=torch.uint8, device=self.device)
+                    self._descs.append(self._desc_dev)
                     self._streams.clear()
                 self._on(stream)
-                self._desc_dev[:host.numel()].copy_(host, non_blocking=True)
+                for d in self._descs:
+                    if d.numel() >= host.numel():
+                        d[:host.numel()].copy_(host, non_blocking=True)
+                    else:
+                        d[:8].zero_()   # the number of no plan: a captured call does nothing
         self.positions = [int(p) for p in positions]
         self.lengths = [int(x) for x in lengths]
+
+    def _keep(self, t) -> None:
+        """Keeps a buffer that a larger one replaces: a captured call may refer to it."""
+        if t is not None:
+            self._old.append(t)
 
     def _rows(self, t, w: int, name: str, dtype):
         """Pointer and row stride of an activation tensor of rows of w."""
@@ -781,7 +799,7 @@ class PagedChunkBatch:
         if raw not in self._streams:
             import torch
             s = stream or torch.cuda.current_stream(self._index)
-            for t in (self._desc_dev, self.workspace, *self._q.values()):
+            for t in (*self._descs, *self._old, self.workspace, *self._q.values()):
                 t.record_stream(s)
             self._streams.add(raw)
         return raw
@@ -836,6 +854,7 @@ class PagedChunkBatch:
             return
         buf = self._q.get(q.dtype)
         if buf is None or buf.shape[0] < self.plan.n_tokens:
+            self._keep(buf)
             buf = self._q[q.dtype] = torch.empty((self.plan.n_tokens, self.shape.n_head * self.shape.head_dim),
                                                  dtype=q.dtype, device=self.device)
             self._streams.clear()
