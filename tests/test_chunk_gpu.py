@@ -750,3 +750,31 @@ def test_a_replay_after_a_larger_plan_uses_no_freed_buffer(cuda, pos, new, large
     torch.cuda.synchronize()
     assert torch.equal(c.out, want)
     assert all(bool((t == 77).all()) for t in others)
+
+
+@pytest.mark.parametrize("act", ["f32", "bf16"])
+def test_a_shorter_descriptor_of_another_plan_does_nothing(cuda, act):
+    """Calls with a plan whose records would lie behind the end of the
+    descriptor that they are given: 0x10b, nothing is written."""
+    import ctypes
+    import torch
+    import tle
+    c = Case([3000, 40, 20], [100, 1, 300], act=act, seed=42)
+    small = tle.PagedChunkBatch(c.cache, c.tables[:1], [0], [1])
+    n = small.plan.desc_bytes
+    desc = small._desc_dev[:n].clone()
+    assert n < c.batch.plan.desc_bytes / 10 and c.batch.plan.n_merge > 0
+    pools = (c.cache.key_pool.clone(), c.cache.value_pool.clone())
+    L, pool, plan, code = tle.lib(), c.cache.pool(), c.batch.plan, [tle.TLE_ACT_F32, tle.TLE_ACT_BF16][act == "bf16"]
+    stream = torch.cuda.current_stream().cuda_stream
+    c.out.fill_(3)
+    rc = L.tle_append_bf16_paged(ctypes.byref(c.cache.shape), ctypes.addressof(pool), ctypes.byref(plan), desc.data_ptr(),
+                                 c.q.data_ptr(), 2048, c.k.data_ptr(), 256, c.v.data_ptr(), 256, c.out.data_ptr(), code, 0, 1,
+                                 stream)
+    assert rc == tle.TLE_OK and tle.device_error() == 0x10b
+    rc = L.tle_prefill_bf16_paged(ctypes.byref(c.cache.shape), ctypes.addressof(pool), ctypes.byref(plan), desc.data_ptr(),
+                                  c.q.data_ptr(), 2048, c.out.data_ptr(), 2048, code, 0, c.batch.workspace.data_ptr(),
+                                  c.batch.workspace.numel() * 4, stream)
+    assert rc == tle.TLE_OK and tle.device_error() == 0x10b
+    assert bool((c.out == 3).all())
+    assert torch.equal(pools[0], c.cache.key_pool) and torch.equal(pools[1], c.cache.value_pool)

@@ -101,12 +101,12 @@ __global__ void __launch_bounds__(kAppendThreads) append_kernel(const __grid_con
     const int units = A.n_head + 2 * A.n_head_kv, kv0 = A.n_head, v0 = A.n_head + A.n_head_kv;
     const int pieces = (units + HPW - 1) / HPW;
     const int j_end = static_cast<int>(static_cast<int64_t>(part + 1) * pieces / parts);
-    const uint64_t desc_id = A.d.hdr->id;
-    const ChunkTok tk = A.d.toks[tok];
-    if (desc_id != A.plan_id) {
+    // before its records: another plan's descriptor may end before this one's do
+    if (A.d.hdr->id != A.plan_id) {
         if (lane == 0) record_error(A.err, kErrBadDesc);
         return;
     }
+    const ChunkTok tk = A.d.toks[tok];
     const int d0 = lane % LPH * VE;             // this lane's elements of a head
     const Act* q = static_cast<const Act*>(A.q) + tok * A.q_stride + d0;
     const Act* k = static_cast<const Act*>(A.k) + tok * A.k_stride + d0;
@@ -255,15 +255,15 @@ struct Work : ChunkSeg {
     __device__ __forceinline__ bool edge(int n) const { return n * kTile + kTile - 1 > pos_min; }
 };
 // The CTA's record `cta` (its first segment, and the range of all) into shared
-// memory, by one thread; an empty range if the descriptor is not the launch's.
+// memory, by one thread; an empty range if the descriptor is not the launch's,
+// of which nothing but the number is read then: it may end before this record.
 __device__ __forceinline__ void fetch_first(const ChunkArgs& A, int cta, Work* to) {
-    const uint64_t id = A.d.hdr->id;
-    Work w = *static_cast<const Work*>(A.d.cta + cta);
-    if (id != A.plan_id) {
-        w.seg0 = w.seg1 = 0;
+    if (A.d.hdr->id == A.plan_id) {
+        *to = *static_cast<const Work*>(A.d.cta + cta);
+    } else {
+        to->seg0 = to->seg1 = 0;
         record_error(A.err, kErrBadDesc);
     }
-    *to = w;
 }
 constexpr int kWorkCache = 20;   // segments of a CTA that are held in shared memory
 // Those behind the first, by a warp that has nothing to do yet.
@@ -1489,12 +1489,11 @@ __global__ void __launch_bounds__(kMergeThreads) chunk_merge_kernel(const __grid
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     asm volatile("griddepcontrol.wait;" ::: "memory");
     const int lane = threadIdx.x & 31;
-    const uint64_t id = A.d.hdr->id;
-    const ChunkMerge m = A.d.merges[blockIdx.x];
-    if (id != A.plan_id) {
+    if (A.d.hdr->id != A.plan_id) {
         if (threadIdx.x == 0) record_error(A.err, kErrBadDesc);
         return;
     }
+    const ChunkMerge m = A.d.merges[blockIdx.x];
     const int r = blockIdx.y * (kMergeThreads / 32) + (threadIdx.x >> 5);
     if (r >= m.n_rows) return;
     const float* lse = A.part_lse + m.part + r;

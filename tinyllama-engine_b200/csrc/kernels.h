@@ -350,7 +350,9 @@ cudaError_t launch_embed_rows(int type, float* x, const void* table, const int32
 // rows come last, for a kernel of their own (the last n_few_ctas of cta).  A
 // CTA's record in cta is a copy of its first segment with the range of its
 // segments, and a segment holds all that its CTA needs, so that between the
-// launch and the first page id there is one load instead of three in a row.
+// launch and the first page id there are two loads (the number, which has to
+// be the launch's before anything behind it is read, and the record) instead
+// of four in a row.
 constexpr int kChunkTile = 128;       // K/V rows per tile
 constexpr int kChunkRows = 128;       // rows per tensor-core tile
 constexpr int kChunkItemRows = 2 * kChunkRows;
