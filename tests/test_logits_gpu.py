@@ -305,3 +305,35 @@ def test_strides_stream_and_replay(cuda):
     c["x"] = c["x"] * np.float32(-0.5)
     graph.replay()
     check(c, dst[:, 7:1010])
+
+
+@pytest.mark.parametrize("far", [2 ** 31 - 1, 2 ** 31 - 2, 2 ** 31 - 3, 2 ** 31 - 200, 2 ** 30 + 1, -2 ** 31])
+def test_starts_far_outside_the_list(cuda, far):
+    """Starts and ends next to the largest and smallest 32-bit numbers: both
+    ends are cut to the list, whatever its alignment."""
+    import torch
+    import tle
+    c = make(4, 300, 40, seed=13, biases=10)
+    nt, nb = c["tokens"].size, c["bias_tokens"].size
+    starts, ends = ("token_start", "bias_start"), (nt, nb)
+    for at in range(5):                                  # which start is the far one
+        given = {k: np.linspace(0, n, 5).astype(np.int32) for k, n in zip(starts, ends)}
+        cut = {}
+        for k, n in zip(starts, ends):
+            given[k][at] = far
+            cut[k] = np.clip(given[k], 0, n)
+        for shift in range(4):
+            room = dev(np.concatenate([np.full(shift, 7, np.int32), c["tokens"]]))
+            R = tle.LogitRules(4, 300, **{k: dev(c[k]) for k in KEYS if k in c and k not in starts + ("tokens",)},
+                               tokens=room[shift:], **{k: dev(given[k]) for k in starts})
+            out = torch.empty(4, 300, device="cuda")
+            tle.logits_adjust(out, dev(c["x"]), R)
+            # the rows' own lists, one behind the other (a start behind its end: none)
+            rows = {}
+            for k, lst in zip(starts, (("tokens",), ("bias_tokens", "bias_values"))):
+                parts = [slice(cut[k][r], max(cut[k][r], cut[k][r + 1])) for r in range(4)]
+                for name in lst:
+                    rows[name] = np.concatenate([c[name][p] for p in parts])
+                rows[k] = np.concatenate([[0], np.cumsum([p.stop - p.start for p in parts])]).astype(np.int32)
+            check({**c, **rows}, out)
+    assert tle.device_error() == 0

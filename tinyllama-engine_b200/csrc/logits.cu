@@ -91,9 +91,11 @@ __global__ void __launch_bounds__(kThreads) logits_kernel(const __grid_constant_
     for (int q = 0; q < kPieces; ++q)
         if (tid + q * kThreads < body) x[q] = *reinterpret_cast<const float4*>(src + head + 4 * (tid + q * kThreads));
     if constexpr (PEN) __syncthreads();
-    lo = max(lo, 0);
-    hi = min(hi, A.n_list_tokens);
-    bias_hi = min(bias_hi, A.n_list_biases);
+    // cut to the lists, which end at 2^30, so that no sum below overflows
+    hi = max(min(hi, A.n_list_tokens), 0);
+    lo = min(max(lo, 0), hi);
+    bias_hi = max(min(bias_hi, A.n_list_biases), 0);
+    bias_lo = min(max(bias_lo, 0), bias_hi);
     // The last warp gathers the slice's biases from entry i0 of the list on, until
     // the list ends or kBiasList are there.
     auto gather = [&](int i0) {
@@ -137,7 +139,7 @@ __global__ void __launch_bounds__(kThreads) logits_kernel(const __grid_constant_
     int my_t = -1 - lane;
     float my_b = 0.f, my_x = 0.f;
     if (lister) {
-        gather(max(bias_lo, 0));
+        gather(bias_lo);
         __syncwarp();
         const int nb = bias_n;
         in_lanes = nb <= 32 && bias_next >= bias_hi;
