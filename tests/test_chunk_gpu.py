@@ -778,3 +778,29 @@ def test_a_shorter_descriptor_of_another_plan_does_nothing(cuda, act):
     assert rc == tle.TLE_OK and tle.device_error() == 0x10b
     assert bool((c.out == 3).all())
     assert torch.equal(pools[0], c.cache.key_pool) and torch.equal(pools[1], c.cache.value_pool)
+
+
+def test_run_on_a_stream_takes_memory_of_that_stream(cuda):
+    """The buffer of the rotated q is not one that work still pending on
+    another stream writes to."""
+    import torch
+    c = Case([900, 40], [200, 57], seed=43)
+    want = torch.empty_like(c.out)
+    c.batch.run(c.q, c.k, c.v, want, c.layer)
+    torch.cuda.synchronize()
+    c.batch._q.clear()
+    del c.batch._old[:]
+    torch.cuda.empty_cache()
+    side = torch.cuda.Stream()
+    pending = torch.empty_like(c.q)
+    at = pending.data_ptr()
+    gate = torch.randn(4096, 4096, device="cuda")
+    torch.cuda.synchronize()
+    for _ in range(20):
+        gate = gate @ gate * 1e-2
+    pending.fill_(77.0)
+    del pending                                          # free for this stream, not for others
+    c.batch.run(c.q, c.k, c.v, c.out, c.layer, stream=side)
+    assert c.batch._q[c.q.dtype].data_ptr() != at
+    torch.cuda.synchronize()
+    assert torch.equal(c.out, want)

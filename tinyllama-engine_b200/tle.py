@@ -855,8 +855,8 @@ class PagedChunkBatch:
         buf = self._q.get(q.dtype)
         if buf is None or buf.shape[0] < self.plan.n_tokens:
             self._keep(buf)
-            buf = self._q[q.dtype] = torch.empty((self.plan.n_tokens, self.shape.n_head * self.shape.head_dim),
-                                                 dtype=q.dtype, device=self.device)
+            with torch.cuda.device(self.device), torch.cuda.stream(stream):   # memory that this stream may use at once
+                buf = self._q[q.dtype] = torch.empty((self.plan.n_tokens, self._widths[0]), dtype=q.dtype, device=self.device)
             self._streams.clear()
         self.append(q, k, v, layer, rotate=True, q_out=buf, stream=stream)
         self.attend(buf, out, layer, stream=stream)
