@@ -804,3 +804,23 @@ def test_run_on_a_stream_takes_memory_of_that_stream(cuda):
     assert c.batch._q[c.q.dtype].data_ptr() != at
     torch.cuda.synchronize()
     assert torch.equal(c.out, want)
+
+
+def test_plans_are_not_made_in_a_capture(cuda):
+    """set_positions uploads from a host buffer that it gives back: recorded in
+    a graph, a replay would upload whatever is there then.  Refused."""
+    import torch
+    import tle
+    c = Case([100, 20], [3, 4], seed=44)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        with pytest.raises(RuntimeError):
+            c.batch.set_positions([101, 21], [3, 4])
+        with pytest.raises(RuntimeError):
+            tle.PagedChunkBatch(c.cache, c.tables, [100, 20], [3, 4])
+        c.batch.attend(c.q, c.out, c.layer)
+    graph.replay()
+    torch.cuda.synchronize()
+    want, tol = attention64(c, c.q)
+    assert bool(((c.out.double() - want).abs() <= tol).all())
+    assert tle.device_error() == 0

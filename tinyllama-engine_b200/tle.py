@@ -675,7 +675,7 @@ class PagedChunkBatch:
     ``append`` rotates q and k and stores k and v (fp32 or bf16 cache),
     ``attend`` is the causal attention over a bf16 cache, ``run`` does both.
     ``set_positions`` re-plans on the host and uploads the descriptor (one H2D
-    copy), once per step of all layers.  Calls of one batch share its
+    copy), once per step of all layers, not in a graph capture.  Calls of one batch share its
     descriptor and workspace: they must not overlap on the GPU, nor
     ``set_positions`` with a call that still runs on another stream.  A
     captured call belongs to its plan: replayed after ``set_positions`` made
@@ -738,8 +738,11 @@ class PagedChunkBatch:
         if stream is not None and stream.device != self.device:
             raise ValueError(f"stream of {stream.device}, cache on {self.device}")
         with torch.cuda.device(self.device):
-            host = self.build_host(positions, lengths)   # a new one: the last upload may be pending
             with torch.cuda.stream(stream or torch.cuda.current_stream()):
+                if torch.cuda.is_current_stream_capturing():
+                    raise RuntimeError("a plan is made and uploaded outside of a graph capture: a replay would upload "
+                                       "from a host buffer that is long given back")
+                host = self.build_host(positions, lengths)   # a new one: the last upload may be pending
                 nbytes = lib().tle_prefill_bf16_paged_workspace_bytes(ctypes.byref(self.plan))
                 if self.workspace is None or self.workspace.numel() * 4 < nbytes:
                     # as far above the old one, so that few are ever kept
