@@ -824,3 +824,73 @@ def test_plans_are_not_made_in_a_capture(cuda):
     want, tol = attention64(c, c.q)
     assert bool(((c.out.double() - want).abs() <= tol).all())
     assert tle.device_error() == 0
+
+
+# ------------------------------------------------- infinities in attended rows
+def infinite_keys(c, rows):
+    """Scores of -inf at these rows of sequence 0 for every head: an infinity in
+    one column of K against q of one sign there."""
+    c.q.view(c.q.shape[0], c.H, HD)[:, :, 5] = c.q.view(c.q.shape[0], c.H, HD)[:, :, 5].abs() + 0.1
+    import torch
+    at = torch.from_numpy(c.flat_rows(0, np.array(rows))).cuda()
+    c.cache.key_pool[c.layer].view(-1, c.KH, HD)[at, :, 5] = -float("inf")
+
+
+def attention64_without(c, rows):
+    """attention64 of c (one sequence), the rows' weights 0; NaN where a token
+    attends to nothing else."""
+    import torch
+    p, m, G = c.pos[0], c.new[0], c.H // c.KH
+    out = torch.zeros(m, c.H * HD, dtype=torch.float64, device="cuda")
+    tol = torch.zeros_like(out)
+    at = torch.from_numpy(c.flat_rows(0, np.arange(p + m))).cuda()
+    hide = torch.arange(p + m, device="cuda")[None, :] > p + torch.arange(m, device="cuda")[:, None]
+    gone = torch.zeros(p + m, dtype=torch.bool, device="cuda")
+    gone[torch.tensor(rows, device="cuda")] = True
+    hide = hide | gone
+    for h in range(c.H):
+        sl = slice((h // G) * HD, (h // G + 1) * HD)
+        k = c.cache.key_pool[c.layer].view(-1, c.KH * HD)[at, sl].double()
+        v = c.cache.value_pool[c.layer].view(-1, c.KH * HD)[at, sl].double()
+        k[gone] = 0
+        qq = c.q[:m, h * HD:(h + 1) * HD].double()
+        e = qq @ k.T / 8
+        big = (qq.abs() @ k.abs().T / 8).masked_fill(hide, 0).amax(1, keepdim=True)
+        top = e.abs().masked_fill(hide, 0).amax(1, keepdim=True)
+        w = torch.softmax(e.masked_fill(hide, -float("inf")), 1)
+        vv = torch.where(torch.isfinite(v), v, torch.zeros_like(v))
+        o, size = w @ vv, w @ vv.abs()
+        rel = 2 * (big * 2.0 ** -17 + top * 2.0 ** -23 + 2.0 ** -22) + ((p + m) / 16 + 16) * 2.0 ** -23
+        if c.act == "bf16":
+            rel = rel + 2.0 ** -8 + 2.0 ** -12
+        out[:, h * HD:(h + 1) * HD] = o
+        tol[:, h * HD:(h + 1) * HD] = rel * size + U[c.act] * (o.abs() + rel * size)
+    return out, tol
+
+
+def check_keys_of_no_weight(c, keys, bad=None):
+    import torch
+    import tle
+    infinite_keys(c, keys)
+    sees = torch.zeros(c.T, dtype=torch.bool, device="cuda")
+    if bad is not None:
+        row = int(c.flat_rows(0, np.array([bad]))[0])
+        c.cache.value_pool[c.layer].view(-1, c.KH * HD)[row] = float("nan")
+        sees = torch.arange(c.T, device="cuda") + c.pos[0] >= bad
+    c.batch.attend(c.q, c.out, c.layer)
+    torch.cuda.synchronize()
+    want, tol = attention64_without(c, keys)
+    some = torch.isfinite(want).all(1) & ~sees
+    assert bool(some.any()) and bool(((c.out.double() - want).abs() <= tol)[some].all())
+    assert bool((~torch.isfinite(c.out[sees])).all())
+    assert tle.device_error() == 0
+
+
+@pytest.mark.parametrize("act", ["f32", "bf16"])
+@pytest.mark.parametrize("pos,new,keys,bad", [([200], [3], [0], 201), ([1000], [20], list(range(140)), 1019),
+                                              ([130], [2], list(range(128)), 131)])
+def test_keys_of_no_weight_beside_a_bad_row(cuda, act, pos, new, keys, bad):
+    """Rows whose score is -inf come first, a NaN in V behind some tokens of the
+    same block: the tokens that do not attend to it have the formula's finite
+    results."""
+    check_keys_of_no_weight(Case(pos, new, act=act, seed=50, max_ctas=1), keys, bad)

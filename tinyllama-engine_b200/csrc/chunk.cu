@@ -497,6 +497,7 @@ __device__ __noinline__ void chunk_row_exact(const ChunkArgs& A, const Work& w, 
                 for (int e = 0; e < 8; ++e) s = fmaf(q[8 * c + e], f[e], s);
             }
             const float mn = s > m || s != s ? s : m;   // keeps a NaN
+            if (mn == -INFINITY) continue;              // nothing has a weight so far
             const float al = (m == mn) ? 1.f : exp2f(m - mn);
             const float p = exp2f(s - mn);
             m = mn;
