@@ -894,3 +894,34 @@ def test_keys_of_no_weight_beside_a_bad_row(cuda, act, pos, new, keys, bad):
     same block: the tokens that do not attend to it have the formula's finite
     results."""
     check_keys_of_no_weight(Case(pos, new, act=act, seed=50, max_ctas=1), keys, bad)
+
+
+@pytest.mark.parametrize("act", ["f32", "bf16"])
+@pytest.mark.parametrize("pos,new,keys,bad", [
+    ([200], [3], [0], None), ([200], [1], [0, 150], None), ([3000], [2], [1, 700, 2999], None),       # few rows
+    ([0], [70], [1], 40), ([100], [300], [0, 1, 2, 50], 260), ([5000], [20], [17, 4000], None),       # many, in pieces
+    ([1000], [40], list(range(140)), None), ([130], [16], list(range(128)), None)])
+@pytest.mark.parametrize("values", ["full", "halves"])
+def test_keys_of_no_weight(cuda, act, pos, new, keys, bad, values):
+    """An infinity in K whose scores are -inf takes its row out and leaves the
+    results finite, for q of 24 bits and for q that a bf16 number holds (whose
+    lower terms are zero)."""
+    import torch
+    c = Case(pos, new, act=act, seed=51)
+    if values == "halves":
+        c.q = c.q.to(torch.bfloat16).to(c.q.dtype)
+        c.q[:, 5::64] = 0.4                              # + 0.1: 0.5 in the column with the infinity
+    check_keys_of_no_weight(c, keys, bad)
+
+
+@pytest.mark.parametrize("act", ["f32", "bf16"])
+@pytest.mark.parametrize("pos,new", [([900], [70]), ([900], [2])])
+def test_keys_of_no_weight_in_place(cuda, act, pos, new):
+    """The same with out = q: rows computed again read their q first."""
+    import torch
+    c = Case(pos, new, act=act, seed=52)
+    infinite_keys(c, [3, 400])
+    c.batch.attend(c.q, c.out, c.layer)
+    c.batch.attend(c.q, c.q, c.layer)
+    torch.cuda.synchronize()
+    assert bool(torch.isfinite(c.out).all()) and torch.equal(c.q, c.out)

@@ -219,7 +219,9 @@ __global__ void __launch_bounds__(kAppendThreads) append_kernel(const __grid_con
 // through one warp first: rows behind the last one are zeroed in shared
 // memory, and if a row that only some of the item's tokens attend to is not
 // finite, the segment's rows are computed again one by one from global memory
-// (chunk_row_exact), which reads nothing but the attended rows.
+// (chunk_row_exact), which reads nothing but the attended rows.  fp32: so are
+// rows that came out NaN, since an infinity in K times a zero term of q is NaN
+// where 32-bit arithmetic has a score of -inf.
 constexpr int CT_THREADS = 512;
 constexpr int kChains = 2;
 constexpr int kTile = kChunkTile;            // 128
@@ -467,7 +469,7 @@ __device__ __forceinline__ bool not_finite(const uint4 x) {
 }
 
 // One row of a segment from global memory, attended rows only: the way taken
-// when a masked row of V is not finite (see above).
+// when a masked row of V is not finite, or the row's weights are not (see above).
 template <class Act>
 __device__ __noinline__ void chunk_row_exact(const ChunkArgs& A, const Work& w, int r, RowOut<Act> dst) {
     const int row = w.row0 + r, tok = row_token(A, row), h = w.kvh * A.group + row - tok * A.group;
@@ -1074,8 +1076,9 @@ __global__ void __launch_bounds__(CT_THREADS, 1)
                 }
             };
             float* lse = mine && w.part >= 0 ? A.part_lse + w.part + r : nullptr;
+            // fp32: a NaN may come from a zero term of q against an infinity in K
             if (dual) {
-                if (S.bad[k & 1]) {
+                if (S.bad[k & 1] || (F32 && __any_sync(0xffffffffu, mine && l_run != l_run))) {
                     const Work cold = w;   // a copy, so that w itself stays in registers
                     if (mine) chunk_row_exact<Act>(A, cold, r, row_out<Act>(A, cold, r));
                     __syncwarp();
@@ -1093,18 +1096,18 @@ __global__ void __launch_bounds__(CT_THREADS, 1)
                 if (lane == 0) mbar_arrive(&S.joined);
                 wait_or_flag(&S.joined, n_joins & 1, A.err, kErrWaitMma, failed);
                 tc_fence_after();
-                if (S.bad[k & 1]) {
+                float m0, l0, m1, l1;   // the same in both chains
+                tmem_ld2(tL + col_p(0, 0), m0, l0);
+                tmem_ld2(tL + col_p(1, 0), m1, l1);
+                tmem_wait_ld();
+                const float m_all = fmaxf(m0, m1);
+                const float w0 = m0 != -INFINITY ? exp2f(m0 - m_all) : 0.f, w1 = m1 != -INFINITY ? exp2f(m1 - m_all) : 0.f;
+                const float l_all = (w0 != 0.f ? w0 * l0 : 0.f) + (w1 != 0.f ? w1 * l1 : 0.f);
+                if (S.bad[k & 1] || (F32 && __any_sync(0xffffffffu, mine && l_all != l_all))) {
                     const Work cold = w;
                     if (mine && c == 0) chunk_row_exact<Act>(A, cold, r, row_out<Act>(A, cold, r));
                     __syncwarp();
                 } else {
-                    float m0, l0, m1, l1;
-                    tmem_ld2(tL + col_p(0, 0), m0, l0);
-                    tmem_ld2(tL + col_p(1, 0), m1, l1);
-                    tmem_wait_ld();
-                    const float m_all = fmaxf(m0, m1);
-                    const float w0 = m0 != -INFINITY ? exp2f(m0 - m_all) : 0.f, w1 = m1 != -INFINITY ? exp2f(m1 - m_all) : 0.f;
-                    const float l_all = (w0 != 0.f ? w0 * l0 : 0.f) + (w1 != 0.f ? w1 * l1 : 0.f);
                     const bool empty = l_all == 0.f;
                     const float inv = empty ? 0.f : 1.0f / l_all;
                     put.template operator()<HD / 2>(32 * c, tL + col_o(0), w0 * inv, tL + col_o(1), w1 * inv, true);
@@ -1426,6 +1429,8 @@ __global__ void __launch_bounds__(FW_THREADS, 1)
             l_run[e] += __shfl_xor_sync(0xffffffffu, l_run[e], 1);
             l_run[e] += __shfl_xor_sync(0xffffffffu, l_run[e], 2);
             if (tg == 0) S.ml[warp][gid + 8 * e] = make_float2(m_ref[e], l_run[e]);
+            // fp32: a NaN may come from a zero term of q against an infinity in K
+            if (F32 && rg * 16 + gid + 8 * e < w.n_rows && l_run[e] != l_run[e]) S.bad[k & 1] = 1;
         }
         flush();
     };
