@@ -832,7 +832,7 @@ def infinite_keys(c, rows):
     one column of K against q of one sign there."""
     c.q.view(c.q.shape[0], c.H, HD)[:, :, 5] = c.q.view(c.q.shape[0], c.H, HD)[:, :, 5].abs() + 0.1
     import torch
-    at = torch.from_numpy(c.flat_rows(0, np.array(rows))).cuda()
+    at = torch.from_numpy(c.flat_rows(0, np.array(rows, np.int64))).cuda()
     c.cache.key_pool[c.layer].view(-1, c.KH, HD)[at, :, 5] = -float("inf")
 
 
@@ -925,3 +925,27 @@ def test_keys_of_no_weight_in_place(cuda, act, pos, new):
     c.batch.attend(c.q, c.q, c.layer)
     torch.cuda.synchronize()
     assert bool(torch.isfinite(c.out).all()) and torch.equal(c.q, c.out)
+
+
+@pytest.mark.parametrize("act", ["f32", "bf16"])
+@pytest.mark.parametrize("pos,new,max_ctas", [([0], [1], 0), ([0], [40], 1), ([90], [3], 1), ([300], [20], 1), ([300], [60], 1),
+                                              ([900], [3], 0), ([5000], [20], 0), ([5000], [70], 0)])
+def test_rows_without_any_weight(cuda, act, pos, new, max_ctas):
+    """Scores of -inf only: 0/0, whether the plan cuts the item or not; the
+    tokens that see one other row have that row of V."""
+    import torch
+    import tle
+    c = Case(pos, new, act=act, seed=53, max_ctas=max_ctas)
+    last = pos[0] + new[0] - 1
+    infinite_keys(c, list(range(last)))
+    c.batch.attend(c.q, c.out, c.layer)
+    torch.cuda.synchronize()
+    assert bool(torch.isnan(c.out[:-1]).all())
+    if last:
+        v = c.cache.value_pool[c.layer].view(-1, c.KH, HD)[int(c.flat_rows(0, np.array([last]))[0])]
+        got = c.out[-1].view(c.KH, -1, HD).double()
+        assert bool(((got - v[:, None].double()).abs() <= 2.0 ** -21 * v[:, None].abs()).all())
+    infinite_keys(c, [last])
+    c.batch.attend(c.q, c.out, c.layer)
+    torch.cuda.synchronize()
+    assert bool(torch.isnan(c.out).all()) and tle.device_error() == 0

@@ -462,6 +462,10 @@ __device__ __forceinline__ RowOut<Act> row_out(const ChunkArgs& A, const Work& w
     }
     return o;
 }
+// Factor of the results of rows without any weight: a piece of an item counts
+// for nothing when the pieces are joined; a whole row with scores of -inf only
+// is 0/0.
+__device__ __forceinline__ float no_weight(const Work& w) { return w.part < 0 ? NAN : 0.f; }
 // Whether any of 8 bf16 numbers has an exponent of all ones.
 __device__ __forceinline__ bool not_finite(const uint4 x) {
     auto full = [](uint32_t u) { return ((u & 0x7f807f80u) + 0x00800080u) & 0x80008000u; };
@@ -470,6 +474,8 @@ __device__ __forceinline__ bool not_finite(const uint4 x) {
 
 // One row of a segment from global memory, attended rows only: the way taken
 // when a masked row of V is not finite, or the row's weights are not (see above).
+// About 1.5 us a key (777 tokens behind 16000 rows 25 ms): a segment of more than
+// a million keys would outlast the other warps' waits, which is reported.
 template <class Act>
 __device__ __noinline__ void chunk_row_exact(const ChunkArgs& A, const Work& w, int r, RowOut<Act> dst) {
     const int row = w.row0 + r, tok = row_token(A, row), h = w.kvh * A.group + row - tok * A.group;
@@ -511,7 +517,7 @@ __device__ __noinline__ void chunk_row_exact(const ChunkArgs& A, const Work& w, 
             }
         }
     }
-    const float inv = m == -INFINITY ? 0.f : 1.0f / l;
+    const float inv = m == -INFINITY ? no_weight(w) : 1.0f / l;
     if (dst.lse) *dst.lse = m == -INFINITY ? -INFINITY : m + log2f(l);
     for (int d = 0; d < HD; d += 8) {
         float x[8];
@@ -1084,7 +1090,7 @@ __global__ void __launch_bounds__(CT_THREADS, 1)
                     __syncwarp();
                 } else {
                     const bool empty = m_ref == -INFINITY;
-                    put.template operator()<HD>(0, tO, empty ? 0.f : 1.0f / l_run, 0u, 0.f, false);
+                    put.template operator()<HD>(0, tO, empty ? no_weight(w) : 1.0f / l_run, 0u, 0.f, false);
                     if (lse) *lse = empty ? -INFINITY : m_ref + log2f(l_run);
                 }
                 tc_fence_before();
@@ -1109,7 +1115,7 @@ __global__ void __launch_bounds__(CT_THREADS, 1)
                     __syncwarp();
                 } else {
                     const bool empty = l_all == 0.f;
-                    const float inv = empty ? 0.f : 1.0f / l_all;
+                    const float inv = empty ? no_weight(w) : 1.0f / l_all;
                     put.template operator()<HD / 2>(32 * c, tL + col_o(0), w0 * inv, tL + col_o(1), w1 * inv, true);
                     if (lse && c == 0) *lse = empty ? -INFINITY : m_all + log2f(l_all);
                 }
@@ -1473,9 +1479,9 @@ __global__ void __launch_bounds__(FW_THREADS, 1)
                     }
                 }
                 const float l_row = __shfl_sync(0xffffffffu, l_all, 0), m_row = __shfl_sync(0xffffffffu, m_all, 0);
-                const bool empty = l_row == 0.f;   // no row of this segment is attended to
+                const bool empty = l_row == 0.f;   // no row of this segment has a weight
                 const float inv = empty ? 0.f : 1.0f / l_row;
-                acc = empty ? make_float2(0.f, 0.f) : make_float2(acc.x * inv, acc.y * inv);
+                acc = empty ? make_float2(no_weight(w), no_weight(w)) : make_float2(acc.x * inv, acc.y * inv);
                 const RowOut<Act> dst = row_out<Act>(A, w, r);
                 if (dst.out) store_pair(dst.out + 2 * lane, acc);
                 else store_pair(dst.part + 2 * lane, acc);
