@@ -248,3 +248,12 @@ def test_logit_rules_refuse_bad_arguments():
     assert go(tokens=P, token_start=P, n_tokens=(1 << 30) + 1) == bad
     assert go(tokens=P, token_start=P, n_tokens=-1) == bad
     assert L.tle_logits_adjust(P, 100, P, 100, 2, 100, None, None) == bad
+
+
+def test_attention_in_place_wants_one_stride():
+    """out = q with another stride would overwrite rows of q that other CTAs
+    still read: refused before any launch."""
+    _, _, plan = describe([3000], [40])
+    assert call("tle_prefill_bf16_paged", plan, os=2056) == tle.TLE_ERR_INVALID
+    assert "stride" in tle.lib().tle_last_error().decode()
+    assert call("tle_prefill_bf16_paged", plan, qs=4096) == tle.TLE_ERR_INVALID

@@ -1854,6 +1854,7 @@ int tle_prefill_bf16_paged(const tle_shape_t* shape, const tle_page_pool_bf16_t*
     if (plan->n_tokens == 0) return ok();
     if (int rc = check_rows(q, q_stride, shape->n_head, "q")) return rc;
     if (int rc = check_rows(out, out_stride, shape->n_head, "out")) return rc;
+    if (out == q && out_stride != q_stride && plan->n_tokens > 1) return set_error(TLE_ERR_INVALID, "out is q, with another stride");
     const size_t need = tle_prefill_bf16_paged_workspace_bytes(plan);
     if (need && (!workspace || workspace_bytes < need))
         return set_error(TLE_ERR_WORKSPACE, "workspace %zu bytes < %zu needed", workspace_bytes, need);
