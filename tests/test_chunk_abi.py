@@ -257,3 +257,21 @@ def test_attention_in_place_wants_one_stride():
     assert call("tle_prefill_bf16_paged", plan, os=2056) == tle.TLE_ERR_INVALID
     assert "stride" in tle.lib().tle_last_error().decode()
     assert call("tle_prefill_bf16_paged", plan, qs=4096) == tle.TLE_ERR_INVALID
+
+
+@pytest.mark.parametrize("pos,new", [([3000, 10, 5], [40, 1, 300]), ([0], [1]), ([20], [0])])
+def test_descriptor_at_any_8_byte_boundary(pos, new):
+    """The records are stored without alignment beyond the buffer's 8 bytes:
+    the same bytes at 0 and at 8 modulo 16."""
+    shape, n = tle.Shape(2, 32, 4, 64, 10000.0), len(pos)
+    c = (tle.PagedChunk * n)(*[tle.PagedChunk(0x4000, 500, p, m, 0) for p, m in zip(pos, new)])
+    nbytes = tle.lib().tle_chunk_desc_bytes(ctypes.byref(shape), c, n, 0)
+    got = []
+    for off in (0, 8):
+        raw = np.full(nbytes + 64, 0xAB, np.uint8)
+        at = (-raw.ctypes.data) % 16 + off
+        plan = tle.ChunkPlan()
+        assert tle.lib().tle_chunk_desc_paged(ctypes.byref(shape), 64, c, n, 0, raw.ctypes.data + at, nbytes, ctypes.byref(plan)) == 0
+        assert np.all(raw[:at] == 0xAB) and np.all(raw[at + plan.desc_bytes:] == 0xAB)
+        got.append(raw[at:at + plan.desc_bytes].copy())
+    assert np.array_equal(got[0], got[1])

@@ -1796,25 +1796,33 @@ int tle_chunk_desc_paged(const tle_shape_t* shape, int page_rows, const tle_page
     out.desc_bytes = static_cast<int64_t>(need);
     if (desc_bytes < need)
         return set_error(TLE_ERR_INVALID, "descriptor buffer %zu bytes < %zu needed", desc_bytes, need);
-    auto* hdr = static_cast<tle::ChunkHeader*>(desc_host);
-    *hdr = tle::ChunkHeader{tle::chunk_plan_id(out), n_seqs, out.n_tokens, out.n_ctas, out.n_few_ctas, out.n_segs, out.n_merge};
-    const tle::ChunkDesc d = tle::chunk_desc(desc_host, n_seqs, segs.size(), merges.size(), n_ctas);
-    auto* seq = const_cast<tle::ChunkSeq*>(d.seqs);
-    auto* tok = const_cast<tle::ChunkTok*>(d.toks);
+    // record by record, as chunk_desc has them; desc_host need not be aligned for all
+    auto* at = static_cast<unsigned char*>(desc_host);
+    auto put = [&at](const void* p, size_t bytes) {
+        if (bytes) std::memcpy(at, p, bytes);
+        at += bytes;
+    };
+    const tle::ChunkHeader hdr{tle::chunk_plan_id(out), n_seqs, out.n_tokens, out.n_ctas, out.n_few_ctas, out.n_segs, out.n_merge};
+    put(&hdr, sizeof hdr);
+    for (const auto& st : start)
+        for (size_t c = 0; c + 1 < st.size(); ++c) {
+            tle::ChunkSeg cta = st[c] < st[c + 1] ? segs[st[c]] : tle::ChunkSeg{};
+            cta.seg0 = st[c];
+            cta.seg1 = st[c + 1];
+            put(&cta, sizeof cta);
+        }
+    put(segs.data(), segs.size() * sizeof(tle::ChunkSeg));
     for (int s = 0; s < n_seqs; ++s) {
         const tle_paged_chunk_t& c = chunks[s];
-        seq[s] = tle::ChunkSeq{c.pages, c.n_pages, c.pos, c.n_tokens, first[s]};
-        for (int t = 0; t < c.n_tokens; ++t) *tok++ = tle::ChunkTok{s, c.pos + t};
+        const tle::ChunkSeq seq{c.pages, c.n_pages, c.pos, c.n_tokens, first[s]};
+        put(&seq, sizeof seq);
     }
-    auto* cta = const_cast<tle::ChunkSeg*>(d.cta);
-    for (const auto& st : start)
-        for (size_t c = 0; c + 1 < st.size(); ++c, ++cta) {
-            *cta = st[c] < st[c + 1] ? segs[st[c]] : tle::ChunkSeg{};
-            cta->seg0 = st[c];
-            cta->seg1 = st[c + 1];
+    put(merges.data(), merges.size() * sizeof(tle::ChunkMerge));
+    for (int s = 0; s < n_seqs; ++s)
+        for (int t = 0; t < chunks[s].n_tokens; ++t) {
+            const tle::ChunkTok tok{s, chunks[s].pos + t};
+            put(&tok, sizeof tok);
         }
-    std::copy(segs.begin(), segs.end(), const_cast<tle::ChunkSeg*>(d.segs));
-    std::copy(merges.begin(), merges.end(), const_cast<tle::ChunkMerge*>(d.merges));
     *plan = out;
     return ok();
 } catch (const std::exception& e) {   // the planner's lists: out of host memory
