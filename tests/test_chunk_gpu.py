@@ -949,3 +949,27 @@ def test_rows_without_any_weight(cuda, act, pos, new, max_ctas):
     c.batch.attend(c.q, c.out, c.layer)
     torch.cuda.synchronize()
     assert bool(torch.isnan(c.out).all()) and tle.device_error() == 0
+
+
+@pytest.mark.parametrize("pool", ["f32", "bf16"])
+def test_calls_follow_the_cache_to_other_memory(cuda, pool):
+    """Pools whose storage was exchanged under the same tensor objects: the
+    next call reads and writes the new one."""
+    import torch
+    import tle
+    c = Case([90, 30], [20, 3], pool=pool, seed=54)
+    other = Case([90, 30], [20, 3], pool=pool, seed=55)      # tables of the same sizes
+    c.batch.append(c.q, c.k, c.v, c.layer, q_out=c.out)
+    torch.cuda.synchronize()
+    old = (c.cache.key_pool.detach(), c.cache.value_pool.detach())   # the storage itself
+    before = tuple(t.clone() for t in old)
+    c.cache.key_pool.data, c.cache.value_pool.data = (t.clone() for t in (other.cache.key_pool, other.cache.value_pool))
+    c.batch.append(c.q * 2, c.k * 2, c.v * 2, c.layer, q_out=c.out)
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(old, before))
+    rows = np.concatenate([c.flat_rows(s, np.arange(p, p + m)) for s, (p, m) in enumerate(zip(c.pos, c.new))])
+    got = c.cache.value_pool[c.layer].view(-1, 256)[torch.from_numpy(rows).cuda()]
+    assert torch.equal(got, (c.v * 2).to(got.dtype))
+    if pool == "bf16":
+        check_attend(c)
+    assert tle.device_error() == 0

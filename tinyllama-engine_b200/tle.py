@@ -789,11 +789,14 @@ class PagedChunkBatch:
         return act
 
     def _pool(self):
-        """The cache's tle_page_pool_t, made again only when it has other tensors."""
-        c, made = self.cache, self._pool_made
-        if made is None or made[0] is not c.key_pool or made[1] is not c.value_pool:
-            made = self._pool_made = (c.key_pool, c.value_pool, c.pool())
-        return made[2]
+        """The cache's tle_page_pool_t, one structure for all calls, with the
+        pools' places as they are now."""
+        c, pool = self.cache, self._pool_made
+        if pool is None:
+            pool = self._pool_made = c.pool()
+        pool.key_pool = c.key_pool.data_ptr()
+        pool.value_pool = c.value_pool.data_ptr()
+        return pool
 
     def _on(self, stream) -> int:
         """Handle of the stream; the batch's buffers are kept from reuse until
