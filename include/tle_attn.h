@@ -369,10 +369,12 @@ size_t tle_chunk_desc_bytes(const tle_shape_t* shape, const tle_paged_chunk_t* c
  * plan->desc_bytes bytes to device memory (16-byte aligned) unchanged.
  *
  * The calls below check on the device that the descriptor is the one of their
- * plan; otherwise they do nothing and 0x10b is reported.  So a captured call
- * may be replayed after the descriptor was replaced only if the new plan has
- * the same numbers (the pages, and positions that leave the split as it was,
- * may differ). */
+ * plan; otherwise they do nothing (only its first 8 bytes are read) and 0x10b
+ * is reported.  So a captured call may be replayed after the descriptor was
+ * replaced only if the new plan has the same numbers (the pages, and positions
+ * that leave the split as it was, may differ).  The descriptor and workspace
+ * of a captured call have to stay allocated as long as it may be replayed;
+ * 8 bytes of zeros at its start make a descriptor that of no plan. */
 int tle_chunk_desc_paged(const tle_shape_t* shape, int page_rows, const tle_paged_chunk_t* chunks,
                          int n_seqs, int max_ctas, void* desc_host, size_t desc_bytes,
                          tle_chunk_plan_t* plan);
@@ -410,9 +412,12 @@ size_t tle_prefill_bf16_paged_workspace_bytes(const tle_chunk_plan_t* plan);
  * (bf16 precision); with fp32 activations q and the weights enter as sums of
  * three bf16 numbers each, so the result is that of 32-bit arithmetic on the
  * bf16 rows.  Rows of the pools that no token attends to are never part of a
- * result, whatever they hold.  A page id outside the pool is not dereferenced
- * (0x105, its rows count as zeros).  out rows behind the last token are left
- * as they are.  out may be q, with the same stride.  Calls that share a workspace must not overlap on the GPU. */
+ * result, whatever they hold; infinities and NaN in rows that it attends to act
+ * as in the formula (a row of V may make NaN of an infinity in its column; a
+ * token whose scores are all -inf has NaN).  A page id outside the pool is not
+ * dereferenced (0x105, its rows count as zeros).  out rows behind the last
+ * token are left as they are.  out may be q, with the same stride.  Calls that
+ * share a workspace must not overlap on the GPU. */
 int tle_prefill_bf16_paged(const tle_shape_t* shape, const tle_page_pool_bf16_t* pool,
                            const tle_chunk_plan_t* plan, const void* desc_dev, const void* q,
                            int64_t q_stride, void* out, int64_t out_stride, int act_type, int layer,

@@ -1455,7 +1455,11 @@ constexpr int64_t kSegUnits = 4, kFewSegUnits = 2;
 // How far above the even share the longest CTA may be before items are cut:
 // what the partial results and the launch that joins them cost.  6 x 509 tokens
 // behind 1999 rows, bf16: 67.2 us with 16, 73.7 us with 8 (cut), both without halves; 3 x 300 tokens
-// behind 4000 rows, fp32: 79 us with 16 (cut), 93 us with 32.
+// behind 4000 rows, fp32: 79 us with 16 (cut), 93 us with 32.  Measured on many
+// rows; for few rows, where a whole item of 2000 rows costs 18, it is wide: nearly
+// one item more than the even share passes.  One token behind 2000 rows, bf16: 18
+// sequences (cut) 11.6 us, 19 (whole, on 76 CTAs) 12.1, 32 12.5, 38 (cut) 17.8, 48
+// (whole, two items on some CTAs) 23.8, 64 26.8, 80 37.6 us.
 constexpr int64_t kJoinUnits = 16;
 constexpr int64_t kMaxWholeItems = 4096;    // sorted on the host, a few tenths of a millisecond
 // Smallest piece of an item worth a CTA of its own.  5 tokens behind 2000 rows

@@ -79,7 +79,7 @@ __device__ __forceinline__ void store_n(T* p, const float (&x)[N]) {
 // kAppendBatch pieces per lane are in flight (fp32: 2048 tokens 7.8 us with 10, 10.6 us
 // with 4; bf16: 18 k tokens 33 us with 4, 41 us with 8).  18 k tokens bf16: 160.6 MB
 // in 31.7 us, 5.1 TB/s (small blocks leave their places to the next ones soon: 256
-// threads 33.0 us); 64 single tokens 3.6 us, the launch and one dependent
+// threads 33.0 us); 64 single tokens 3.7 us, the launch and one dependent
 // load after another.
 constexpr int kAppendThreads = 64;
 constexpr int kAppendPart = 4;             // pieces of the smallest part of a token
@@ -198,12 +198,12 @@ __global__ void __launch_bounds__(kAppendThreads) append_kernel(const __grid_con
 // What bounds it: with 64 columns a score costs 256 tensor-core operations and
 // one exponential, and the exponential unit (16 a cycle and SM) is the slower of
 // the two: 2048 cycles for 256 x 128 scores; a block takes about 2650 (bf16).
-// 2048 tokens behind 30000 rows, 32 query on 4 KV heads: 660 us, 789 TFLOP/s; ncu:
+// 2048 tokens behind 30000 rows, 32 query on 4 KV heads: 650 us, 800 TFLOP/s; ncu:
 // exponential unit 76 % busy, tensor cores 38 %.  Exponentials by polynomial on
 // the FMA units, for a part of the scores: 774 us where this took 669.  Four
 // softmax warpgroups of 64 rows, or two blocks of 64 keys in flight per chain:
 // 881 to 1340 us where this took 700, for registers.  fp32: 777 tokens behind 16000
-// rows 276 us, 378 TFLOP/s of three products each, tensor cores 58 % busy.
+// rows 279 us, 374 TFLOP/s of three products each, tensor cores 57 % busy.
 //
 // Precision: bf16 activations: P rounded to bf16 (its sum is not), fp32
 // accumulation.  fp32 activations: q and P are cut into three bf16 numbers of
@@ -1147,10 +1147,10 @@ __global__ void __launch_bounds__(CT_THREADS, 1)
 // shared memory at the segment's end.  K and V come through a ring of TMA
 // tiles as above, kept full across segments by a producer warp.  Precision
 // and the treatment of rows that not every token attends to as above.
-// 64 decode steps of 32 query heads: behind 1024 to 2047 rows 24.6 us (fp32; 98.6 MB,
-// 4.0 TB/s, of which launch, start and end are 8 us), behind 8000 rows 84.8 us (bf16;
-// 525 MB, 6.2 TB/s).  Tiles that every row attends to have code of their own: 24.8
-// us, with one code for both 25.7; two such tiles side by side per warp 25.4.
+// 64 decode steps of 32 query heads: behind 1024 to 2047 rows 25.3 us (fp32; 98.6 MB,
+// 3.9 TB/s, of which launch, start and end are 8 us), behind 8000 rows 86.0 us (bf16;
+// 525 MB, 6.1 TB/s).  Tiles that every row attends to have code of their own: 0.9 us
+// less than with one code for both; two such tiles side by side per warp: 0.6 us more.
 constexpr int FW_WARPS = 8;
 constexpr int FW_THREADS = 32 * (FW_WARPS + 1);
 constexpr int FW_STAGES = 4;       // 64 x 1 behind 2047 rows: 25.8 us, with 3 the same, with 5 28.4 us
