@@ -973,3 +973,21 @@ def test_calls_follow_the_cache_to_other_memory(cuda, pool):
     if pool == "bf16":
         check_attend(c)
     assert tle.device_error() == 0
+
+
+def test_what_a_batch_keeps_is_bounded(cuda):
+    """Batches that grow by a token at a time: all the buffers ever kept are at
+    most three times the newest ones."""
+    import torch
+    c = Case([0, 900], [200, 200], page=64, seed=56, layers=1)
+    for n in range(20, 200):
+        c.batch.set_positions([0, 5 * n], [n, 1])
+        c.batch.run(c.q, c.k, c.v, c.out, 0)
+    torch.cuda.synchronize()
+    b = c.batch
+    size = lambda ts: sum(t.numel() * t.element_size() for t in ts)  # noqa: E731
+    newest = size([b._desc_dev, b.workspace, *b._q.values()])
+    assert size([*b._descs, b.workspace, *b._q.values(), *b._old]) <= 3 * newest
+    assert b._q[c.q.dtype].shape[0] < 2 * 200
+    b.set_positions(c.pos, c.new)
+    check_attend(c)

@@ -745,14 +745,12 @@ class PagedChunkBatch:
                 host = self.build_host(positions, lengths)   # a new one: the last upload may be pending
                 nbytes = lib().tle_prefill_bf16_paged_workspace_bytes(ctypes.byref(self.plan))
                 if self.workspace is None or self.workspace.numel() * 4 < nbytes:
-                    # as far above the old one, so that few are ever kept
-                    room = max(nbytes // 4, 4) if self.workspace is None else max(nbytes // 4, self.workspace.numel() * 5 // 4)
-                    self._keep(self.workspace)
-                    self.workspace = torch.empty(room, dtype=torch.float32, device=self.device)
+                    self.workspace = torch.empty(self._room(max(nbytes // 4, 4), self.workspace), dtype=torch.float32,
+                                                 device=self.device)
                     self._streams.clear()
                 if self._desc_dev is None or self._desc_dev.numel() < host.numel():
                     # with room for the plans of later positions; the old one may be in a graph
-                    self._desc_dev = torch.empty(host.numel() * 5 // 4 + 4096, dtype=torch.uint8, device=self.device)
+                    self._desc_dev = torch.empty(host.numel() * 3 // 2 + 4096, dtype=torch.uint8, device=self.device)
                     self._descs.append(self._desc_dev)
                     self._streams.clear()
                 self._on(stream)
@@ -764,10 +762,14 @@ class PagedChunkBatch:
         self.positions = [int(p) for p in positions]
         self.lengths = [int(x) for x in lengths]
 
-    def _keep(self, t) -> None:
-        """Keeps a buffer that a larger one replaces: a captured call may refer to it."""
-        if t is not None:
-            self._old.append(t)
+    def _room(self, n: int, old) -> int:
+        """Rows of the buffer that replaces `old` where n are needed: half as much
+        again as it had at least, so that all that is kept for captured calls
+        stays below twice the newest."""
+        if old is None:
+            return n
+        self._old.append(old)
+        return max(n, old.shape[0] * 3 // 2)
 
     def _rows(self, t, w: int, name: str, dtype):
         """Pointer and row stride of an activation tensor of rows of w."""
@@ -860,9 +862,9 @@ class PagedChunkBatch:
             return
         buf = self._q.get(q.dtype)
         if buf is None or buf.shape[0] < self.plan.n_tokens:
-            self._keep(buf)
             with torch.cuda.device(self.device), torch.cuda.stream(stream):   # memory that this stream may use at once
-                buf = self._q[q.dtype] = torch.empty((self.plan.n_tokens, self._widths[0]), dtype=q.dtype, device=self.device)
+                buf = self._q[q.dtype] = torch.empty((self._room(self.plan.n_tokens, buf), self._widths[0]), dtype=q.dtype,
+                                                     device=self.device)
             self._streams.clear()
         self.append(q, k, v, layer, rotate=True, q_out=buf, stream=stream)
         self.attend(buf, out, layer, stream=stream)
