@@ -414,10 +414,11 @@ size_t tle_prefill_bf16_paged_workspace_bytes(const tle_chunk_plan_t* plan);
  * bf16 rows.  Rows of the pools that no token attends to are never part of a
  * result, whatever they hold; infinities and NaN in rows that it attends to act
  * as in the formula (a row of V may make NaN of an infinity in its column; a
- * token whose scores are all -inf has NaN).  A page id outside the pool is not
- * dereferenced (0x105, its rows count as zeros).  out rows behind the last
- * token are left as they are.  out may be q, with the same stride.  Calls that
- * share a workspace must not overlap on the GPU. */
+ * token whose scores are all -inf has NaN).  Weighted sums are divided at the end:
+ * |v| times the rows that a token attends to has to stay below 2^120.  A page
+ * id outside the pool is not dereferenced (0x105, its rows count as zeros).
+ * out rows behind the last token are left as they are.  out may be q, with the
+ * same stride.  Calls that share a workspace must not overlap on the GPU. */
 int tle_prefill_bf16_paged(const tle_shape_t* shape, const tle_page_pool_bf16_t* pool,
                            const tle_chunk_plan_t* plan, const void* desc_dev, const void* q,
                            int64_t q_stride, void* out, int64_t out_stride, int act_type, int layer,
