@@ -212,18 +212,28 @@ def prepare(case, seed):
     return st
 
 
+def _power32(e):
+    """2^e of whole numbers -126 <= e <= 127, in 32 bits and exact (many rows have numbers half-way between two codes)."""
+    return ((e.to(torch.int32) + 127) << 23).view(torch.float32)
+
+
+def _power64(e):
+    """2^e of whole numbers, in 64 bits and exact."""
+    return ((e.to(torch.int64) + 1023) << 52).view(torch.float64)
+
+
 def _to_8_bits(x):
     """Whole numbers (int8) and the byte of the power of two (uint8) of rows of finite numbers."""
     most = x.abs().amax(-1)
     # 127 * 2^e as a number of 32 bits is exact, so that the comparison is
     e = torch.frexp(most)[1] - 7                           # most < 2^(e + 7): e or e + 1
-    e = torch.where(most > 127.0 * torch.exp2(e.float()), e + 1, e).clamp_(min=-126)
-    codes = torch.round(x * torch.exp2(-e.float())[..., None])
+    e = torch.where(most > 127.0 * _power32(e), e + 1, e).clamp_(min=-126)
+    codes = torch.round(x * _power32(-e)[..., None])
     return codes.to(torch.int8), (e + 127).to(torch.uint8)
 
 
-def _from_8_bits(codes, scale, dtype=torch.float32):
-    return (codes.to(dtype) * torch.exp2(scale.to(dtype) - 127.0)[..., None])
+def _from_8_bits(codes, scale):
+    return codes.float() * _power32(scale.int() - 127)[..., None]
 
 
 def _prepare_sample(case, g, dev):
@@ -432,7 +442,7 @@ def exact(case, seed):
         """Head h of sequence s's first rows in the 8-bit pool: [end][64]."""
         at = flat(s, 0, end)
         codes, b = (st[x + y][layer, :, h].reshape(-1, *d)[at] for y, d in (("_codes", (HD,)), ("_scale", ())))
-        return codes.double() * torch.pow(2.0, b.double() - 127)[:, None]
+        return codes.double() * _power64(b.long() - 127)[:, None]
 
     if case["op"] == "read":
         got = {x: torch.cat([torch.cat([stored(x, s, h, p + m) for h in range(KH)], 1) for s, (p, m) in enumerate(zip(pos, new))])
@@ -476,7 +486,11 @@ def exact(case, seed):
         return {"q": q.flatten(1), "k_pool": kp, "v_pool": vp}
 
     def rounded(x):
-        step = torch.pow(2.0, torch.ceil(torch.log2(x.abs().amax(-1, keepdim=True) / 127)).clamp(min=-126))
+        most = x.abs().amax(-1, keepdim=True)
+        e = torch.floor(torch.log2(most.clamp(min=2.0 ** -120))).long() - 8     # from below, up to the first that is enough
+        for _ in range(4):
+            e = torch.where(127 * _power64(e) < most, e + 1, e)
+        step = _power64(e.clamp(min=-126))
         return (torch.round(x / step) * step).flatten(1)
 
     return {"q": q.flatten(1), "k": rounded(k), "v": rounded(v)}
