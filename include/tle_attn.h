@@ -424,6 +424,104 @@ int tle_prefill_bf16_paged(const tle_shape_t* shape, const tle_page_pool_bf16_t*
                            int64_t q_stride, void* out, int64_t out_stride, int act_type, int layer,
                            void* workspace, size_t workspace_bytes, void* stream);
 
+/* ---- rules of an append: rope layouts, scaled positions, norms ----
+ * No counterpart in the reference, whose rope() turns the pairs (2i, 2i+1) of
+ * whole heads (ops.cpp:1223-1281) and which has no norms of heads. */
+#define TLE_ROPE_INTERLEAVED 0   /* pairs (2i, 2i + 1), as tle_rope            */
+#define TLE_ROPE_HALF 1          /* pairs (i, i + rotary_dim / 2)              */
+typedef struct {
+    int32_t layout;         /* TLE_ROPE_*                                                       */
+    int32_t rotary_dim;     /* elements of a head that are rotated: 16, 32, 48 or 64; the others
+                               stay as they are                                                 */
+    const float* inv_freq;  /* HOST [rotary_dim / 2], read during the call; NULL: the shape's
+                               1 / rope_freq_base^(2i / rotary_dim)                             */
+    float rope_factor;      /* on sine and cosine (1: none)                                     */
+    float norm_eps;         /* >= 0                                                             */
+    const float* q_norm;    /* device [64] or NULL (no norm): q heads become
+                               x / sqrt(mean(x^2) + norm_eps) * q_norm before they are rotated  */
+    const float* k_norm;    /* the same for k heads                                             */
+} tle_append_rules_t;
+
+/* Frequencies for contexts `factor` times as long as the original_ctx rows that
+ * a model was trained on; HOST only.  inv_freq [rotary_dim / 2] and
+ * *rope_factor go into tle_append_rules_t.  With f_i = base^(-2i / rotary_dim):
+ *   TLE_ROPE_SCALE_NONE    f_i
+ *   TLE_ROPE_SCALE_LINEAR  f_i / factor
+ *   TLE_ROPE_SCALE_NTK     f_i with the base base * factor^(rotary_dim / (rotary_dim - 2))
+ *   TLE_ROPE_SCALE_YARN    f_i where a pair turns more than 32 times within
+ *                          original_ctx, f_i / factor where less than once, and
+ *                          a linear ramp over the pairs in between;
+ *                          *rope_factor = 1 + 0.1 ln(factor), otherwise 1. */
+enum { TLE_ROPE_SCALE_NONE = 0, TLE_ROPE_SCALE_LINEAR = 1, TLE_ROPE_SCALE_NTK = 2, TLE_ROPE_SCALE_YARN = 3 };
+int tle_rope_frequencies(int kind, float base, int rotary_dim, float factor, int original_ctx,
+                         float* inv_freq, float* rope_factor);
+
+/* tle_append_paged / tle_append_bf16_paged by rules: q and k heads are normed,
+ * then (flags & TLE_DECODE_ROTATE) rotated by angle fl32(p * inv_freq[i]), v is
+ * stored as it is.  Everything in 32 bits, rounded once. */
+int tle_append_rules_paged(const tle_shape_t* shape, const tle_page_pool_t* pool, const tle_chunk_plan_t* plan,
+                           const void* desc_dev, const void* q, int64_t q_stride, const void* k,
+                           int64_t k_stride, const void* v, int64_t v_stride, void* q_out, int act_type,
+                           int layer, int flags, const tle_append_rules_t* rules, void* stream);
+int tle_append_rules_bf16_paged(const tle_shape_t* shape, const tle_page_pool_bf16_t* pool,
+                                const tle_chunk_plan_t* plan, const void* desc_dev, const void* q,
+                                int64_t q_stride, const void* k, int64_t k_stride, const void* v,
+                                int64_t v_stride, void* q_out, int act_type, int layer, int flags,
+                                const tle_append_rules_t* rules, void* stream);
+
+/* ---- pages of 8 bits ----
+ * No counterpart in the reference.  A head's row x[0..63] is 64 whole numbers c
+ * in -127..127 and a byte b, standing for c * 2^(b - 127): 2^(b - 127) is the
+ * smallest power of two for which no |x| / 2^(b - 127) is above 127 (1 <= b <=
+ * 248: numbers above 127 * 2^121 become that), c the nearest whole number
+ * (ties to even).  Such values are bf16 numbers
+ * exactly.  A row with an infinity or NaN gets b = 255 and zeros, and counts as
+ * 64 NaN.  Half the bytes of bf16 pages (65 instead of 128 a head's row), off
+ * by at most 2^(b - 128), that is max|x| / 127 where bf16 has |x| / 256. */
+typedef struct {
+    int8_t* key_codes;     /* device [n_layers][n_pages][n_head_kv][page_rows][64] */
+    int8_t* value_codes;
+    uint8_t* key_scale;    /* device [n_layers][n_pages][n_head_kv][page_rows]     */
+    uint8_t* value_scale;
+    int32_t n_pages;
+    int32_t page_rows;     /* a power of two, 64 .. 65536; pointers 16-byte aligned */
+} tle_page_pool_q8_t;
+
+/* tle_append_rules_paged into 8-bit pages (rules NULL: the shape's rope, no
+ * norms). */
+int tle_append_q8_paged(const tle_shape_t* shape, const tle_page_pool_q8_t* pool, const tle_chunk_plan_t* plan,
+                        const void* desc_dev, const void* q, int64_t q_stride, const void* k,
+                        int64_t k_stride, const void* v, int64_t v_stride, void* q_out, int act_type,
+                        int layer, int flags, const tle_append_rules_t* rules, void* stream);
+
+/* The stored values as numbers of out_type (TLE_ACT_*; exact in either): the
+ * rows 0 .. pos + n_tokens - 1 of every sequence with new tokens, one sequence
+ * after another, n_rows in all; with TLE_READ_NEW in flags the rows of the new
+ * tokens only (n_rows = the plan's n_tokens), in the order of the batch.  Row i
+ * of k_out at k_out + i * k_stride elements, n_head_kv * 64 of them; strides as
+ * for tle_append_paged; k_out or v_out may be NULL.  Rows behind n_rows are
+ * not written and reported (0x10c).  A page id outside the pool: 0x105, its
+ * rows are zeros. */
+#define TLE_READ_NEW 1
+int tle_read_q8_paged(const tle_shape_t* shape, const tle_page_pool_q8_t* pool, const tle_chunk_plan_t* plan,
+                      const void* desc_dev, void* k_out, int64_t k_stride, void* v_out, int64_t v_stride,
+                      int64_t n_rows, int out_type, int layer, int flags, void* stream);
+
+/* tle_prefill_bf16_paged over 8-bit pages, with the same descriptor and the
+ * same contract; q and the softmax weights enter as sums of two fp16 numbers
+ * (24 bits) where a chunk has at most 32 rows per KV head, and as for bf16 pages
+ * otherwise.  Chunks of more rows are attended to over a bf16 copy of their
+ * sequences' rows in the workspace, which nothing is rounded for. */
+size_t tle_prefill_q8_paged_workspace_bytes(const tle_shape_t* shape, const tle_paged_chunk_t* chunks, int n_seqs,
+                                            const tle_chunk_plan_t* plan);
+/* workspace: 16-byte aligned, at least that many bytes.  Where a captured call
+ * is replayed under a plan of the same numbers whose chunks of many rows have
+ * more rows than the workspace has room for, it reports 0x10c, and what it
+ * leaves in those chunks' rows of out is of no use. */
+int tle_prefill_q8_paged(const tle_shape_t* shape, const tle_page_pool_q8_t* pool, const tle_chunk_plan_t* plan,
+                         const void* desc_dev, const void* q, int64_t q_stride, void* out, int64_t out_stride,
+                         int act_type, int layer, void* workspace, size_t workspace_bytes, void* stream);
+
 /* ---- multi-GPU sequence partition ---- */
 
 /* Greedy longest-processing-time assignment of sequences to n_ranks GPUs,
@@ -442,7 +540,8 @@ int tle_partition_lpt(const int32_t* lengths, int n_seqs, int n_ranks, int32_t* 
  * barrier wait of the one-launch forward expired, 0x109 a finite activation
  * of the batched prompt overflowed fp16, 0x10a a bf16 or short-batch decode
  * record outside its cache or max_rows, 0x10b a chunk call met the descriptor of
- * another plan than its own (it did nothing), 0x1ff the self-test below.  The first code recorded
+ * another plan than its own (it did nothing), 0x10c an 8-bit cache call met more rows
+ * than its buffer has room for, 0x1ff the self-test below.  The first code recorded
  * stays until cleared.  Synchronises the device. */
 int tle_device_error(int clear, uint32_t* code);
 

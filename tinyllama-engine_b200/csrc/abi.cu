@@ -1671,16 +1671,18 @@ int check_chunk_pool(const tle_shape_t* shape, const tle_chunk_plan_t* plan, con
     return 0;
 }
 
-int append_common(const tle_shape_t* shape, const tle_chunk_plan_t* plan, const void* desc_dev, const void* q,
-                  int64_t q_stride, const void* k, int64_t k_stride, const void* v, int64_t v_stride, void* q_out,
-                  int act_type, int layer, int flags, void* key_pool, void* value_pool, int n_pages, int page_rows,
-                  bool pool_bf16, void* stream) {
+// The checks and arguments that appends into any pool share, but for the pool's
+// places; a.n_tokens 0: nothing to do.
+int append_args(const tle_shape_t* shape, const tle_chunk_plan_t* plan, const void* desc_dev, const void* q,
+                int64_t q_stride, const void* k, int64_t k_stride, const void* v, int64_t v_stride, void* q_out,
+                int act_type, int layer, int flags, const void* key_pool, const void* value_pool, int n_pages,
+                int page_rows, int min_page, tle::AppendArgs& a) {
     if (int rc = check_chunk_call(shape, plan, desc_dev, act_type, layer)) return rc;
     int shift = 0;
-    if (int rc = check_chunk_pool(shape, plan, key_pool, value_pool, n_pages, page_rows, pool_bf16 ? 64 : 16, &shift))
-        return rc;
+    if (int rc = check_chunk_pool(shape, plan, key_pool, value_pool, n_pages, page_rows, min_page, &shift)) return rc;
     if (flags & ~TLE_DECODE_ROTATE) return set_error(TLE_ERR_INVALID, "unknown flags 0x%x", flags);
-    if (plan->n_tokens == 0) return ok();
+    a.n_tokens = plan->n_tokens;
+    if (plan->n_tokens == 0) return 0;
     if ((q == nullptr) != (q_out == nullptr)) return set_error(TLE_ERR_INVALID, "q and q_out go together");
     if (q) {
         if (int rc = check_rows(q, q_stride, shape->n_head, "q")) return rc;
@@ -1690,11 +1692,9 @@ int append_common(const tle_shape_t* shape, const tle_chunk_plan_t* plan, const 
     }
     if (int rc = check_rows(k, k_stride, shape->n_head_kv, "k")) return rc;
     if (int rc = check_rows(v, v_stride, shape->n_head_kv, "v")) return rc;
-    tle::AppendArgs a{};
     a.d = tle::chunk_desc(desc_dev, plan->n_seqs, plan->n_segs, plan->n_merge,
                           static_cast<size_t>(plan->n_ctas) + plan->n_few_ctas);
     a.plan_id = tle::chunk_plan_id(*plan);
-    a.n_tokens = plan->n_tokens;
     a.q = q;
     a.k = k;
     a.v = v;
@@ -1702,29 +1702,154 @@ int append_common(const tle_shape_t* shape, const tle_chunk_plan_t* plan, const 
     a.q_stride = q_stride;
     a.k_stride = k_stride;
     a.v_stride = v_stride;
-    const size_t layer_bytes = static_cast<size_t>(n_pages) * page_rows * shape->n_head_kv * tle::kHeadDim * (pool_bf16 ? 2 : 4);
-    a.key_pool = static_cast<unsigned char*>(key_pool) + layer_bytes * layer;
-    a.value_pool = static_cast<unsigned char*>(value_pool) + layer_bytes * layer;
     a.pool_pages = n_pages;
     a.page_shift = shift;
     a.n_head = q ? shape->n_head : 0;
     a.n_head_kv = shape->n_head_kv;
     a.rotate = (flags & TLE_DECODE_ROTATE) ? 1 : 0;
-    if (a.rotate) {
-        // 32 powers, half a microsecond: kept for the thread's last base
-        thread_local float base = 0.f, table[tle::kHeadDim / 2];
-        if (base != shape->rope_freq_base) {
-            base = shape->rope_freq_base;
-            fill_inv_freq(table, tle::kHeadDim / 2, base);
-        }
-        std::copy(std::begin(table), std::end(table), a.inv_freq);
+    return 0;
+}
+
+// The frequencies of whole heads; 32 powers, half a microsecond: kept for the
+// thread's last base.
+void head_freq(float base_now, float* dst) {
+    thread_local float base = 0.f, table[tle::kHeadDim / 2];
+    if (base != base_now) {
+        base = base_now;
+        fill_inv_freq(table, tle::kHeadDim / 2, base);
     }
+    std::copy(std::begin(table), std::end(table), dst);
+}
+
+int append_common(const tle_shape_t* shape, const tle_chunk_plan_t* plan, const void* desc_dev, const void* q,
+                  int64_t q_stride, const void* k, int64_t k_stride, const void* v, int64_t v_stride, void* q_out,
+                  int act_type, int layer, int flags, void* key_pool, void* value_pool, int n_pages, int page_rows,
+                  bool pool_bf16, void* stream) {
+    tle::AppendArgs a{};
+    if (int rc = append_args(shape, plan, desc_dev, q, q_stride, k, k_stride, v, v_stride, q_out, act_type, layer, flags,
+                             key_pool, value_pool, n_pages, page_rows, pool_bf16 ? 64 : 16, a))
+        return rc;
+    if (a.n_tokens == 0) return ok();
+    const size_t layer_bytes = static_cast<size_t>(n_pages) * page_rows * shape->n_head_kv * tle::kHeadDim * (pool_bf16 ? 2 : 4);
+    a.key_pool = static_cast<unsigned char*>(key_pool) + layer_bytes * layer;
+    a.value_pool = static_cast<unsigned char*>(value_pool) + layer_bytes * layer;
+    if (a.rotate) head_freq(shape->rope_freq_base, a.inv_freq);
     cudaError_t e = tle::error_word(&a.err);
     if (e != cudaSuccess) return cuda_error(e, "device error word");
     e = tle::launch_append(a, act_type == TLE_ACT_BF16, pool_bf16, static_cast<cudaStream_t>(stream));
     if (e != cudaSuccess) return cuda_error(e, "append launch");
     return ok();
 }
+
+// An append by rules (NULL: the shape's rope, no norms) into pools of 1, 2 or
+// 4 bytes an element.
+int append_by_rules(const tle_shape_t* shape, const tle_chunk_plan_t* plan, const void* desc_dev, const void* q,
+                    int64_t q_stride, const void* k, int64_t k_stride, const void* v, int64_t v_stride, void* q_out,
+                    int act_type, int layer, int flags, void* key_pool, void* value_pool, uint8_t* key_scale,
+                    uint8_t* value_scale, int n_pages, int page_rows, int pool_bytes, const tle_append_rules_t* rules,
+                    void* stream) {
+    tle::AppendRulesArgs r{};
+    if (int rc = append_args(shape, plan, desc_dev, q, q_stride, k, k_stride, v, v_stride, q_out, act_type, layer, flags,
+                             key_pool, value_pool, n_pages, page_rows, pool_bytes == 4 ? 16 : 64, r.a))
+        return rc;
+    tle_append_rules_t own{};
+    own.rotary_dim = tle::kHeadDim;
+    own.rope_factor = 1.f;
+    if (!rules) rules = &own;
+    if (rules->layout != TLE_ROPE_INTERLEAVED && rules->layout != TLE_ROPE_HALF)
+        return set_error(TLE_ERR_INVALID, "unknown rope layout %d", rules->layout);
+    if (rules->rotary_dim < 16 || rules->rotary_dim > tle::kHeadDim || rules->rotary_dim % 16 != 0)
+        return set_error(TLE_ERR_UNSUPPORTED, "rotary_dim %d is not 16, 32, 48 or 64", rules->rotary_dim);
+    if (!(rules->norm_eps >= 0.f)) return set_error(TLE_ERR_INVALID, "norm_eps must be >= 0");
+    if ((reinterpret_cast<uintptr_t>(rules->q_norm) & 3u) || (reinterpret_cast<uintptr_t>(rules->k_norm) & 3u) ||
+        (reinterpret_cast<uintptr_t>(rules->inv_freq) & 3u))
+        return set_error(TLE_ERR_INVALID, "norm weights and frequencies must be 4-byte aligned");
+    if (r.a.n_tokens == 0) return ok();
+    const size_t layer_rows = static_cast<size_t>(n_pages) * page_rows * shape->n_head_kv;
+    r.a.key_pool = static_cast<unsigned char*>(key_pool) + layer_rows * layer * tle::kHeadDim * pool_bytes;
+    r.a.value_pool = static_cast<unsigned char*>(value_pool) + layer_rows * layer * tle::kHeadDim * pool_bytes;
+    if (key_scale) {
+        r.key_scale = key_scale + layer_rows * layer;
+        r.value_scale = value_scale + layer_rows * layer;
+    }
+    r.half = rules->rotary_dim / 2;
+    r.halves = rules->layout == TLE_ROPE_HALF;
+    r.factor = rules->rope_factor;
+    r.q_norm = r.a.n_head ? rules->q_norm : nullptr;
+    r.k_norm = rules->k_norm;
+    r.eps = rules->norm_eps;
+    if (r.a.rotate) {
+        if (rules->inv_freq) std::copy(rules->inv_freq, rules->inv_freq + r.half, r.a.inv_freq);
+        else if (rules->rotary_dim == tle::kHeadDim) head_freq(shape->rope_freq_base, r.a.inv_freq);
+        else fill_inv_freq(r.a.inv_freq, r.half, shape->rope_freq_base);
+    }
+    cudaError_t e = tle::error_word(&r.a.err);
+    if (e != cudaSuccess) return cuda_error(e, "device error word");
+    e = tle::launch_append_rules(r, act_type == TLE_ACT_BF16, pool_bytes, static_cast<cudaStream_t>(stream));
+    if (e != cudaSuccess) return cuda_error(e, "append launch");
+    return ok();
+}
+
+int check_scales(const tle_page_pool_q8_t* pool) {
+    if (!pool) return set_error(TLE_ERR_INVALID, "page pool and both pools must be non-null");
+    if (!pool->key_scale || !pool->value_scale || !aligned16(pool->key_scale) || !aligned16(pool->value_scale))
+        return set_error(TLE_ERR_INVALID, "the pools' scales must be non-null and 16-byte aligned");
+    return 0;
+}
+
+tle::Pool8 pool8(const tle_shape_t* shape, const tle_page_pool_q8_t* pool, int layer, int shift) {
+    const size_t rows = static_cast<size_t>(pool->n_pages) * pool->page_rows * shape->n_head_kv * layer;
+    return tle::Pool8{pool->key_codes + rows * tle::kHeadDim, pool->value_codes + rows * tle::kHeadDim, pool->key_scale + rows,
+                      pool->value_scale + rows, pool->n_pages, shift};
+}
+
+// The arguments of an attention over bf16 pages or 8-bit ones, but for the
+// pool's, whose pages have 2^shift rows; the calls' checks come first.
+void attention_args(const tle_shape_t* shape, const tle_chunk_plan_t* plan, const void* desc_dev, const void* q,
+                    int64_t q_stride, void* out, int64_t out_stride, void* workspace, tle::ChunkArgs& a) {
+    a.d = tle::chunk_desc(desc_dev, plan->n_seqs, plan->n_segs, plan->n_merge,
+                          static_cast<size_t>(plan->n_ctas) + plan->n_few_ctas);
+    a.plan_id = tle::chunk_plan_id(*plan);
+    a.n_ctas = plan->n_ctas;
+    a.n_few_ctas = plan->n_few_ctas;
+    a.n_merge = plan->n_merge;
+    a.merge_rows = plan->merge_rows;
+    a.q = q;
+    a.out = out;
+    a.q_stride = q_stride;
+    a.out_stride = out_stride;
+    a.n_head = shape->n_head;
+    a.n_head_kv = shape->n_head_kv;
+    a.group = shape->n_head / shape->n_head_kv;
+    if (a.group > 1) {
+        int bits = 1;
+        while ((1 << bits) < a.group) ++bits;
+        const uint64_t one = 1ull << (31 + bits);
+        a.group_mul = static_cast<uint32_t>((one + a.group - 1) / a.group);
+        a.group_shift = static_cast<uint32_t>(bits - 1);
+    }
+    a.part_o = static_cast<float*>(workspace);
+    a.part_lse = plan->part_rows > 0 ? a.part_o + static_cast<size_t>(plan->part_rows) * tle::kHeadDim : nullptr;
+}
+
+// The workspace of an attention over 8-bit pages: partial results | header and
+// records of the copied descriptor | staged K pages | staged V pages | their
+// page table.
+struct Stage8Room {
+    size_t records, pages, per_page;   // where they start; bytes of a page in K, V and the table
+    Stage8Room(const tle_shape_t* shape, const tle_chunk_plan_t* plan) {
+        auto up = [](size_t x) { return (x + 15) & ~static_cast<size_t>(15); };
+        records = up(tle_prefill_bf16_paged_workspace_bytes(plan));
+        pages = records;
+        per_page = 0;
+        if (plan->n_ctas == 0) return;
+        pages = up(records + tle::chunk_desc_bytes(0, plan->n_segs, 0, 0, static_cast<size_t>(plan->n_ctas) + plan->n_few_ctas));
+        per_page = 2 * page_bytes(shape) + sizeof(int32_t);
+    }
+    static size_t page_bytes(const tle_shape_t* shape) {
+        return static_cast<size_t>(tle::kStageRows) * shape->n_head_kv * tle::kHeadDim * sizeof(uint16_t);
+    }
+};
 
 }  // namespace
 
@@ -1872,38 +1997,200 @@ int tle_prefill_bf16_paged(const tle_shape_t* shape, const tle_page_pool_bf16_t*
         return set_error(TLE_ERR_WORKSPACE, "workspace %zu bytes < %zu needed", workspace_bytes, need);
     if (need && !aligned16(workspace)) return set_error(TLE_ERR_INVALID, "workspace must be 16-byte aligned");
     tle::ChunkArgs a{};
-    a.d = tle::chunk_desc(desc_dev, plan->n_seqs, plan->n_segs, plan->n_merge,
-                          static_cast<size_t>(plan->n_ctas) + plan->n_few_ctas);
-    a.plan_id = tle::chunk_plan_id(*plan);
-    a.n_ctas = plan->n_ctas;
-    a.n_few_ctas = plan->n_few_ctas;
-    a.n_merge = plan->n_merge;
-    a.merge_rows = plan->merge_rows;
-    a.q = q;
-    a.out = out;
-    a.q_stride = q_stride;
-    a.out_stride = out_stride;
+    attention_args(shape, plan, desc_dev, q, q_stride, out, out_stride, workspace, a);
     const size_t layer_halfs = static_cast<size_t>(pool->n_pages) * pool->page_rows * shape->n_head_kv * tle::kHeadDim;
     a.key_pool = static_cast<const uint16_t*>(pool->key_pool) + layer_halfs * layer;
     a.value_pool = static_cast<const uint16_t*>(pool->value_pool) + layer_halfs * layer;
     a.pool_pages = pool->n_pages;
     a.page_shift = shift;
-    a.n_head = shape->n_head;
-    a.n_head_kv = shape->n_head_kv;
-    a.group = shape->n_head / shape->n_head_kv;
-    if (a.group > 1) {
-        int bits = 1;
-        while ((1 << bits) < a.group) ++bits;
-        const uint64_t one = 1ull << (31 + bits);
-        a.group_mul = static_cast<uint32_t>((one + a.group - 1) / a.group);
-        a.group_shift = static_cast<uint32_t>(bits - 1);
-    }
-    a.part_o = static_cast<float*>(workspace);
-    a.part_lse = need ? a.part_o + static_cast<size_t>(plan->part_rows) * tle::kHeadDim : nullptr;
     cudaError_t e = tle::error_word(&a.err);
     if (e != cudaSuccess) return cuda_error(e, "device error word");
     e = tle::launch_chunk_attention(a, act_type == TLE_ACT_BF16, static_cast<cudaStream_t>(stream));
     if (e != cudaSuccess) return cuda_error(e, "chunk attention launch");
+    return ok();
+}
+
+// ===================== rules of an append, pages of 8 bits (tle_attn.h) =====================
+
+int tle_rope_frequencies(int kind, float base, int rotary_dim, float factor, int original_ctx, float* inv_freq,
+                         float* rope_factor) {
+    if (!inv_freq || !rope_factor) return set_error(TLE_ERR_INVALID, "inv_freq and rope_factor must be non-null");
+    if (kind < TLE_ROPE_SCALE_NONE || kind > TLE_ROPE_SCALE_YARN) return set_error(TLE_ERR_INVALID, "unknown scaling %d", kind);
+    if (rotary_dim < 16 || rotary_dim > tle::kHeadDim || rotary_dim % 16 != 0)
+        return set_error(TLE_ERR_UNSUPPORTED, "rotary_dim %d is not 16, 32, 48 or 64", rotary_dim);
+    if (!(base > 1.f) || !std::isfinite(base)) return set_error(TLE_ERR_INVALID, "base must be > 1");
+    if (kind != TLE_ROPE_SCALE_NONE && (!(factor >= 1.f) || !std::isfinite(factor)))
+        return set_error(TLE_ERR_INVALID, "factor must be >= 1");
+    if (kind == TLE_ROPE_SCALE_YARN && original_ctx <= 0) return set_error(TLE_ERR_INVALID, "original_ctx must be > 0");
+    const double d = rotary_dim;
+    double b = base, lo = 0, hi = 0;
+    if (kind == TLE_ROPE_SCALE_NTK) b *= std::pow(static_cast<double>(factor), d / (d - 2));
+    if (kind == TLE_ROPE_SCALE_YARN) {
+        // the pair (a real number) that turns `turns` times within original_ctx
+        auto pair_of = [&](double turns) {
+            return d * std::log(original_ctx / (turns * 2 * 3.14159265358979323846)) / (2 * std::log(b));
+        };
+        lo = std::max(std::floor(pair_of(32)), 0.0);
+        hi = std::min(std::ceil(pair_of(1)), d / 2 - 1);
+        if (hi <= lo) hi = lo + 0.001;
+    }
+    for (int i = 0; i < rotary_dim / 2; ++i) {
+        double f = std::pow(b, -2.0 * i / d);
+        if (kind == TLE_ROPE_SCALE_LINEAR) f /= factor;
+        if (kind == TLE_ROPE_SCALE_YARN) {
+            const double slow = std::min(std::max((i - lo) / (hi - lo), 0.0), 1.0);
+            f = f * (1 - slow) + f / factor * slow;
+        }
+        inv_freq[i] = static_cast<float>(f);
+    }
+    *rope_factor = kind == TLE_ROPE_SCALE_YARN ? static_cast<float>(1 + 0.1 * std::log(static_cast<double>(factor))) : 1.f;
+    return ok();
+}
+
+int tle_append_rules_paged(const tle_shape_t* shape, const tle_page_pool_t* pool, const tle_chunk_plan_t* plan,
+                           const void* desc_dev, const void* q, int64_t q_stride, const void* k, int64_t k_stride,
+                           const void* v, int64_t v_stride, void* q_out, int act_type, int layer, int flags,
+                           const tle_append_rules_t* rules, void* stream) {
+    if (!pool) return set_error(TLE_ERR_INVALID, "page pool and both pools must be non-null");
+    return append_by_rules(shape, plan, desc_dev, q, q_stride, k, k_stride, v, v_stride, q_out, act_type, layer, flags,
+                           pool->key_pool, pool->value_pool, nullptr, nullptr, pool->n_pages, pool->page_rows, 4, rules, stream);
+}
+
+int tle_append_rules_bf16_paged(const tle_shape_t* shape, const tle_page_pool_bf16_t* pool, const tle_chunk_plan_t* plan,
+                                const void* desc_dev, const void* q, int64_t q_stride, const void* k, int64_t k_stride,
+                                const void* v, int64_t v_stride, void* q_out, int act_type, int layer, int flags,
+                                const tle_append_rules_t* rules, void* stream) {
+    if (!pool) return set_error(TLE_ERR_INVALID, "page pool and both pools must be non-null");
+    return append_by_rules(shape, plan, desc_dev, q, q_stride, k, k_stride, v, v_stride, q_out, act_type, layer, flags,
+                           pool->key_pool, pool->value_pool, nullptr, nullptr, pool->n_pages, pool->page_rows, 2, rules, stream);
+}
+
+int tle_append_q8_paged(const tle_shape_t* shape, const tle_page_pool_q8_t* pool, const tle_chunk_plan_t* plan,
+                        const void* desc_dev, const void* q, int64_t q_stride, const void* k, int64_t k_stride,
+                        const void* v, int64_t v_stride, void* q_out, int act_type, int layer, int flags,
+                        const tle_append_rules_t* rules, void* stream) {
+    if (int rc = check_scales(pool)) return rc;
+    return append_by_rules(shape, plan, desc_dev, q, q_stride, k, k_stride, v, v_stride, q_out, act_type, layer, flags,
+                           pool->key_codes, pool->value_codes, pool->key_scale, pool->value_scale, pool->n_pages,
+                           pool->page_rows, 1, rules, stream);
+}
+
+int tle_read_q8_paged(const tle_shape_t* shape, const tle_page_pool_q8_t* pool, const tle_chunk_plan_t* plan,
+                      const void* desc_dev, void* k_out, int64_t k_stride, void* v_out, int64_t v_stride, int64_t n_rows,
+                      int out_type, int layer, int flags, void* stream) {
+    if (int rc = check_chunk_call(shape, plan, desc_dev, out_type, layer)) return rc;
+    if (int rc = check_scales(pool)) return rc;
+    int shift = 0;
+    if (int rc = check_chunk_pool(shape, plan, pool->key_codes, pool->value_codes, pool->n_pages, pool->page_rows, 64, &shift))
+        return rc;
+    if (flags & ~TLE_READ_NEW) return set_error(TLE_ERR_INVALID, "unknown flags 0x%x", flags);
+    if (n_rows < 0 || n_rows > (int64_t{1} << 40)) return set_error(TLE_ERR_INVALID, "n_rows %lld", static_cast<long long>(n_rows));
+    const bool new_only = (flags & TLE_READ_NEW) != 0;
+    if (new_only && n_rows != plan->n_tokens)
+        return set_error(TLE_ERR_INVALID, "n_rows %lld is not the plan's %d new tokens", static_cast<long long>(n_rows), plan->n_tokens);
+    if (n_rows == 0 || plan->n_tokens == 0) return ok();
+    if (k_out)
+        if (int rc = check_rows(k_out, k_stride, shape->n_head_kv, "k_out")) return rc;
+    if (v_out)
+        if (int rc = check_rows(v_out, v_stride, shape->n_head_kv, "v_out")) return rc;
+    if (!k_out && !v_out) return ok();
+    tle::Read8Args a{};
+    a.d = tle::chunk_desc(desc_dev, plan->n_seqs, plan->n_segs, plan->n_merge,
+                          static_cast<size_t>(plan->n_ctas) + plan->n_few_ctas);
+    a.plan_id = tle::chunk_plan_id(*plan);
+    a.pool = pool8(shape, pool, layer, shift);
+    a.n_seqs = plan->n_seqs;
+    a.n_tokens = plan->n_tokens;
+    a.n_head_kv = shape->n_head_kv;
+    a.n_rows = n_rows;
+    a.k = k_out;
+    a.v = v_out;
+    a.k_stride = k_stride;
+    a.v_stride = v_stride;
+    cudaError_t e = tle::error_word(&a.err);
+    if (e != cudaSuccess) return cuda_error(e, "device error word");
+    e = tle::launch_read8(a, out_type == TLE_ACT_BF16, new_only, static_cast<cudaStream_t>(stream));
+    if (e != cudaSuccess) return cuda_error(e, "8-bit read launch");
+    return ok();
+}
+
+size_t tle_prefill_q8_paged_workspace_bytes(const tle_shape_t* shape, const tle_paged_chunk_t* chunks, int n_seqs,
+                                            const tle_chunk_plan_t* plan) {
+    if (check_chunks(shape, 0, chunks, n_seqs)) return 0;
+    if (!plan || plan->n_head != shape->n_head || plan->n_head_kv != shape->n_head_kv || plan->n_seqs != n_seqs) {
+        set_error(TLE_ERR_INVALID, "the plan is not one of these chunks");
+        return 0;
+    }
+    const Stage8Room room(shape, plan);
+    const int64_t g = shape->n_head / shape->n_head_kv;
+    size_t pages = 0;
+    for (int s = 0; s < n_seqs; ++s)
+        if (chunks[s].n_tokens * g > tle::kChunkFewRows)
+            pages += (static_cast<size_t>(chunks[s].pos) + chunks[s].n_tokens + tle::kStageRows - 1) / tle::kStageRows;
+    ok();
+    return room.pages + pages * room.per_page;
+}
+
+int tle_prefill_q8_paged(const tle_shape_t* shape, const tle_page_pool_q8_t* pool, const tle_chunk_plan_t* plan,
+                         const void* desc_dev, const void* q, int64_t q_stride, void* out, int64_t out_stride, int act_type,
+                         int layer, void* workspace, size_t workspace_bytes, void* stream) {
+    if (int rc = check_chunk_call(shape, plan, desc_dev, act_type, layer)) return rc;
+    if (int rc = check_scales(pool)) return rc;
+    int shift = 0;
+    if (int rc = check_chunk_pool(shape, plan, pool->key_codes, pool->value_codes, pool->n_pages, pool->page_rows, 64, &shift))
+        return rc;
+    if (plan->n_tokens == 0) return ok();
+    if (int rc = check_rows(q, q_stride, shape->n_head, "q")) return rc;
+    if (int rc = check_rows(out, out_stride, shape->n_head, "out")) return rc;
+    if (out == q && out_stride != q_stride && plan->n_tokens > 1) return set_error(TLE_ERR_INVALID, "out is q, with another stride");
+    const Stage8Room room(shape, plan);
+    const size_t least = room.pages + room.per_page;   // a staged page at least
+    if (least && (!workspace || workspace_bytes < least))
+        return set_error(TLE_ERR_WORKSPACE, "workspace %zu bytes < %zu needed at least", workspace_bytes, least);
+    if (least && !aligned16(workspace)) return set_error(TLE_ERR_INVALID, "workspace must be 16-byte aligned");
+    const bool act_bf16 = act_type == TLE_ACT_BF16;
+    cudaStream_t s = static_cast<cudaStream_t>(stream);
+    tle::ChunkArgs a{};
+    attention_args(shape, plan, desc_dev, q, q_stride, out, out_stride, workspace, a);
+    const tle::Pool8 p8 = pool8(shape, pool, layer, shift);
+    cudaError_t e = tle::error_word(&a.err);
+    if (e != cudaSuccess) return cuda_error(e, "device error word");
+    if (a.n_few_ctas > 0) {
+        e = tle::launch_chunk_few8(a, p8, act_bf16, s);
+        if (e != cudaSuccess) return cuda_error(e, "8-bit attention launch");
+    }
+    if (a.n_ctas > 0) {
+        unsigned char* at = static_cast<unsigned char*>(workspace);
+        tle::Stage8Args st{};
+        st.d = a.d;
+        st.plan_id = a.plan_id;
+        st.pool = p8;
+        st.n_seqs = plan->n_seqs;
+        st.n_head_kv = shape->n_head_kv;
+        st.group = a.group;
+        st.n_ctas = plan->n_ctas + plan->n_few_ctas;
+        st.n_segs = plan->n_segs;
+        st.n_pages = static_cast<int64_t>(std::min<size_t>((workspace_bytes - room.pages) / room.per_page, (1u << 30) / tle::kStageRows));
+        st.hdr = reinterpret_cast<tle::ChunkHeader*>(at + room.records);
+        st.cta = reinterpret_cast<tle::ChunkSeg*>(st.hdr + 1);
+        st.k = reinterpret_cast<__nv_bfloat16*>(at + room.pages);
+        st.v = reinterpret_cast<__nv_bfloat16*>(at + room.pages + st.n_pages * Stage8Room::page_bytes(shape));
+        st.table = reinterpret_cast<int32_t*>(at + room.pages + 2 * st.n_pages * Stage8Room::page_bytes(shape));
+        st.err = a.err;
+        e = tle::launch_stage8(st, s);
+        if (e != cudaSuccess) return cuda_error(e, "8-bit attention: staging launch");
+        tle::ChunkArgs b = a;
+        b.d = tle::chunk_desc(st.hdr, 0, plan->n_segs, 0, st.n_ctas);
+        b.key_pool = reinterpret_cast<const uint16_t*>(st.k);
+        b.value_pool = reinterpret_cast<const uint16_t*>(st.v);
+        b.pool_pages = static_cast<int>(st.n_pages);
+        b.page_shift = 7;
+        static_assert(tle::kStageRows == 1 << 7, "rows of a staged page");
+        e = tle::launch_chunk_many(b, act_bf16, s);
+        if (e != cudaSuccess) return cuda_error(e, "8-bit attention launch");
+    }
+    e = tle::launch_chunk_merge(a, act_bf16, s);
+    if (e != cudaSuccess) return cuda_error(e, "8-bit attention: joining launch");
     return ok();
 }
 

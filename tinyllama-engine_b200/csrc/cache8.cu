@@ -1,0 +1,463 @@
+// cache8.cu -- append by rules (RMS norm of q and k heads, rope layouts) into
+// fp32, bf16 and 8-bit pages, and 8-bit pages read back.
+//
+// For a head x[0..63] of token position p:
+//   y = x / sqrt(mean(x^2) + eps) * w                              (norm, if given)
+//   (y'_a, y'_b) = (y_a c - y_b s, y_a s + y_b c),  c, s = factor (cos, sin)(fl32(p f_i))
+// for the pairs i < rotary_dim / 2, (a, b) = (2i, 2i + 1) or (i, i + rotary_dim / 2).
+//
+// 8-bit pages.  A head's row is 64 whole numbers n in -127..127 and a byte b:
+// the values n 2^(b - 127), with 2^(b - 127) the smallest power of two for
+// which max|y| <= 127 2^(b - 127) (1 <= b <= 248, so that n 2^(b - 127) is finite:
+// numbers above 127 2^121 become that) and n the nearest whole number, ties to even.  A power of two, because n 2^(b - 127) is then a bf16 number
+// exactly (8 bits): products with it are exact on the tensor cores, and rows
+// read back as bf16 or fp32 are the stored ones.  A scale of more bits would be
+// up to twice as fine (max|y| / 127 against 2^ceil(log2(max|y| / 127))), but every reader would
+// round its product.  Rows with an infinity or NaN: b = 255 and n = 0, which
+// is 0 * inf = NaN for every reader.
+#include <cuda_bf16.h>
+#include <math.h>
+#include <stdint.h>
+
+#include <algorithm>
+#include <type_traits>
+
+#include "chunk.cuh"
+#include "common.cuh"
+#include "kernels.h"
+
+namespace tle {
+
+namespace {
+
+// ---- append -----------------------------------------------------------------
+// As append_kernel (chunk.cu): a warp takes a token or a part of one, in
+// 16-byte pieces, 8 (bf16) or 16 (fp32) lanes per head, so the norm's sum and
+// the largest value of a head are reductions over those lanes, and a pair's
+// other half is in the lane itself (interleaved) or a fixed distance away.
+constexpr int kThreads = 64;
+constexpr int kPart = 4;            // pieces of the smallest part of a token
+constexpr int kWarps = 148 * 16;    // below so many tokens their heads are spread over several warps
+
+template <int LANES>
+__device__ __forceinline__ float sum_over(float x) {
+#pragma unroll
+    for (int d = LANES / 2; d > 0; d /= 2) x += __shfl_xor_sync(0xffffffffu, x, d);
+    return x;
+}
+template <int LANES>
+__device__ __forceinline__ float max_over(float x) {   // keeps a NaN
+#pragma unroll
+    for (int d = LANES / 2; d > 0; d /= 2) x = fmax3(x, __shfl_xor_sync(0xffffffffu, x, d), 0.f);
+    return x;
+}
+
+// The byte b of a row whose largest magnitude is `most`: 127 = 1.984375 * 2^6.
+__device__ __forceinline__ int scale_byte(float most) {
+    const uint32_t u = __float_as_uint(most);
+    const int b = static_cast<int>(u >> 23) - 6 + ((u & 0x7fffffu) > 0x7e0000u ? 1 : 0);
+    return (u >> 23) == 255u ? 255 : min(max(b, 1), 248);
+}
+
+template <int VE>
+__device__ __forceinline__ void store_codes(int8_t* p, const float (&y)[VE], float inv) {
+    uint32_t w[VE / 4];
+#pragma unroll
+    for (int i = 0; i < VE / 4; ++i) {
+        uint32_t u = 0;
+#pragma unroll
+        for (int e = 0; e < 4; ++e)   // the bounds cut the largest numbers of 32 bits only
+            u |= (static_cast<uint32_t>(__float2int_rn(fminf(fmaxf(y[4 * i + e] * inv, -127.f), 127.f))) & 0xffu) << (8 * e);
+        w[i] = u;
+    }
+    if constexpr (VE == 8) *reinterpret_cast<uint2*>(p) = make_uint2(w[0], w[1]);
+    else *reinterpret_cast<uint32_t*>(p) = w[0];
+}
+
+template <class Act, class Pool>
+__global__ void __launch_bounds__(kThreads) append_rules_kernel(const __grid_constant__ AppendRulesArgs R, int parts) {
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    constexpr bool kBits8 = sizeof(Pool) == 1;
+    constexpr int kBatch = sizeof(Act) == 4 ? 6 : 4;   // pieces in flight per lane
+    constexpr int VE = 16 / sizeof(Act);
+    constexpr int LPH = HD / VE;
+    constexpr int HPW = 32 / LPH;
+    const AppendArgs& A = R.a;
+    const int lane = threadIdx.x & 31;
+    const int64_t w = static_cast<int64_t>(blockIdx.x) * (kThreads / 32) + (threadIdx.x >> 5);
+    const int64_t tok = w / parts;
+    if (tok >= A.n_tokens) return;
+    const int part = static_cast<int>(w - tok * parts);
+    const int units = A.n_head + 2 * A.n_head_kv, kv0 = A.n_head, v0 = A.n_head + A.n_head_kv;
+    const int pieces = (units + HPW - 1) / HPW;
+    const int j_end = static_cast<int>(static_cast<int64_t>(part + 1) * pieces / parts);
+    // before its records: another plan's descriptor may end before this one's do
+    if (A.d.hdr->id != A.plan_id) {
+        if (lane == 0) record_error(A.err, kErrBadDesc);
+        return;
+    }
+    const ChunkTok tk = A.d.toks[tok];
+    const int d0 = lane % LPH * VE;
+    const Act* q = static_cast<const Act*>(A.q) + tok * A.q_stride + d0;
+    const Act* k = static_cast<const Act*>(A.k) + tok * A.k_stride + d0;
+    const Act* v = static_cast<const Act*>(A.v) + tok * A.v_stride + d0;
+    Act* qo = static_cast<Act*>(A.q_out) + tok * A.n_head * HD + d0;
+    // the token's row in the pools: its first head there, and from head to head
+    const int page_rows = 1 << A.page_shift, r_in = tk.pos & (page_rows - 1);
+    const size_t step = kBits8 ? static_cast<size_t>(page_rows) * HD : HD;
+    size_t row = 0;
+    bool have = false;
+    const int id = A.d.seqs[tk.seq].pages[tk.pos >> A.page_shift];
+    if (static_cast<unsigned>(id) < static_cast<unsigned>(A.pool_pages)) {
+        have = true;
+        row = kBits8 ? ((static_cast<size_t>(id) * A.n_head_kv) << A.page_shift) + r_in
+                     : ((static_cast<size_t>(id) << A.page_shift) + r_in) * A.n_head_kv;
+    } else if (lane == 0) {
+        record_error(A.err, kErrBadPage);
+    }
+    Pool* kr = static_cast<Pool*>(A.key_pool) + row * HD + d0;
+    Pool* vr = static_cast<Pool*>(A.value_pool) + row * HD + d0;
+    // y[e] = x[e] cs[e] + (the pair's other element) sn[e]
+    float cs[VE], sn[VE];
+    const bool turned = A.rotate && d0 < 2 * R.half;   // a multiple of 16: all of a lane's elements or none
+    const bool first = d0 < R.half;                    // half layout: the elements a of their pairs
+    const int other = R.halves ? (turned ? (first ? lane + R.half / VE : lane - R.half / VE) : lane) : lane;
+    if (A.rotate) {
+        float s1 = 0.f, c1 = 1.f;
+        if (lane < R.half) sincosf(static_cast<float>(tk.pos) * A.inv_freq[lane], &s1, &c1);
+        s1 *= R.factor;
+        c1 *= R.factor;
+#pragma unroll
+        for (int e = 0; e < VE; ++e) {
+            const int pair = (R.halves ? d0 + e - (first ? 0 : R.half) : (d0 + e) / 2) & 31;
+            cs[e] = __shfl_sync(0xffffffffu, c1, pair);
+            const float s = __shfl_sync(0xffffffffu, s1, pair);
+            sn[e] = (R.halves ? first : e % 2 == 0) ? -s : s;
+        }
+    }
+    float qw[VE], kw[VE];
+#pragma unroll
+    for (int e = 0; e < VE; ++e) {
+        qw[e] = R.q_norm ? R.q_norm[d0 + e] : 1.f;
+        kw[e] = R.k_norm ? R.k_norm[d0 + e] : 1.f;
+    }
+    for (int j0 = static_cast<int>(static_cast<int64_t>(part) * pieces / parts); j0 < j_end; j0 += kBatch) {
+        uint4 x[kBatch];
+#pragma unroll
+        for (int b = 0; b < kBatch; ++b) {
+            const int u = (j0 + b) * HPW + lane / LPH;
+            const Act* src = u < kv0 ? q + u * HD : u < v0 ? k + (u - kv0) * HD : v + (u - v0) * HD;
+            x[b] = j0 + b < j_end && u < units ? *reinterpret_cast<const uint4*>(src) : make_uint4(0, 0, 0, 0);
+        }
+#pragma unroll
+        for (int b = 0; b < kBatch; ++b) {
+            if (j0 + b >= j_end) break;   // the same in all lanes
+            const int u = (j0 + b) * HPW + lane / LPH;
+            float y[VE];
+            if constexpr (sizeof(Act) == 2) {
+                bf16x8(x[b], y);
+            } else {
+                y[0] = __uint_as_float(x[b].x);
+                y[1] = __uint_as_float(x[b].y);
+                y[2] = __uint_as_float(x[b].z);
+                y[3] = __uint_as_float(x[b].w);
+            }
+            if (R.q_norm || R.k_norm) {
+                float ss = 0.f;
+#pragma unroll
+                for (int e = 0; e < VE; ++e) ss = fmaf(y[e], y[e], ss);
+                ss = sum_over<LPH>(ss);
+                if (u < kv0 ? R.q_norm != nullptr : u < v0 && R.k_norm != nullptr) {
+                    const float f = 1.0f / sqrtf(ss * (1.0f / HD) + R.eps);
+#pragma unroll
+                    for (int e = 0; e < VE; ++e) y[e] = y[e] * f * (u < kv0 ? qw[e] : kw[e]);
+                }
+            }
+            if (A.rotate) {
+                float z[VE];
+#pragma unroll
+                for (int e = 0; e < VE; ++e) z[e] = R.halves ? __shfl_sync(0xffffffffu, y[e], other) : y[e ^ 1];
+                if (turned && u < v0) {
+#pragma unroll
+                    for (int e = 0; e < VE; ++e) y[e] = y[e] * cs[e] + z[e] * sn[e];
+                }
+            }
+            if constexpr (kBits8) {
+                float most = 0.f;
+#pragma unroll
+                for (int e = 0; e < VE; ++e) most = fmax3(most, fabsf(y[e]), 0.f);
+                most = max_over<LPH>(most);
+                if (u >= kv0 && u < units && have) {
+                    const int h = u < v0 ? u - kv0 : u - v0, sb = scale_byte(most);
+                    if (sb == 255) {
+#pragma unroll
+                        for (int e = 0; e < VE; ++e) y[e] = 0.f;
+                    }
+                    store_codes<VE>((u < v0 ? kr : vr) + h * step, y, __uint_as_float(static_cast<uint32_t>(254 - min(sb, 248)) << 23));
+                    if (d0 == 0) (u < v0 ? R.key_scale : R.value_scale)[row + (static_cast<size_t>(h) << A.page_shift)] = static_cast<uint8_t>(sb);
+                }
+            } else {
+                if (u >= kv0 && u < units && have) store_n<VE>(u < v0 ? kr + (u - kv0) * HD : vr + (u - v0) * HD, y);
+            }
+            if (u < kv0) store_n<VE>(qo + u * HD, y);
+        }
+    }
+}
+
+// ---- read -------------------------------------------------------------------
+// 16 codes and their row's byte to 16 numbers.
+__device__ __forceinline__ void from_codes(const uint4 c, uint8_t b, float (&f)[16]) {
+    const float s = __uint_as_float(static_cast<uint32_t>(b) << 23);   // 255: infinity, 0 * inf = NaN
+    const uint32_t u[4] = {c.x ^ 0x80808080u, c.y ^ 0x80808080u, c.z ^ 0x80808080u, c.w ^ 0x80808080u};
+#pragma unroll
+    for (int i = 0; i < 16; ++i)   // 2^23 + (n + 128), whose low byte is the code
+        f[i] = (__uint_as_float(__byte_perm(u[i / 4], 0x4B000000u, 0x7650 | (i % 4))) - 8388736.0f) * s;
+}
+__device__ __forceinline__ void store16(float* p, const float (&f)[16]) {
+#pragma unroll
+    for (int i = 0; i < 16; i += 4) store4(p + i, f + i);
+}
+__device__ __forceinline__ void store16(__nv_bfloat16* p, const float (&f)[16]) {
+    store8(p, f);
+    store8(p + 8, f + 8);
+}
+
+// Rows [r0, r0 + n) of one page of the 8-bit pools to rows of k and v
+// (either may be null), 16 elements a thread and step.
+template <class Out>
+__device__ __forceinline__ void read_rows(const Pool8& P, int n_head_kv, int id, int r0, int n, Out* k, int64_t k_stride, Out* v,
+                                          int64_t v_stride) {
+    const int per_row = n_head_kv * (HD / 16);
+    const bool ok = static_cast<unsigned>(id) < static_cast<unsigned>(P.n_pages);
+    for (int i = threadIdx.x; i < 2 * n * per_row; i += blockDim.x) {
+        const bool val = i >= n * per_row;
+        const int j = val ? i - n * per_row : i;
+        const int r = j / per_row, c = j - r * per_row;
+        Out* dst = val ? v : k;
+        if (!dst) continue;
+        float f[16];
+        if (ok) {
+            const size_t row = ((static_cast<size_t>(id) * n_head_kv + c / 4) << P.page_shift) + r0 + r;
+            from_codes(reinterpret_cast<const uint4*>((val ? P.value_codes : P.key_codes) + row * HD)[c % 4],
+                       (val ? P.value_scale : P.key_scale)[row], f);
+        } else {
+#pragma unroll
+            for (int e = 0; e < 16; ++e) f[e] = 0.f;
+        }
+        store16(dst + r * (val ? v_stride : k_stride) + c * 16, f);
+    }
+}
+
+constexpr int kReadThreads = 256;
+// The sequences in groups of kReadThreads: thread i of the group has the rows
+// and blocks of rows of its sequence, the shared arrays where they start.
+// f(sequence's ChunkSeq, block in the sequence, block in all, first row in all) for every
+// block b with b % gridDim.x == blockIdx.x; then g(first sequence of the group,
+// starts of its blocks).  Returns the blocks in all.
+struct WalkSmem {
+    int64_t block0[kReadThreads + 1], row0[kReadThreads + 1];
+    int64_t warp_sum[2][kReadThreads / 32];
+};
+template <class Rows, class F, class G>
+__device__ __forceinline__ int64_t walk(WalkSmem& S, const ChunkDesc& d, int n_seqs, int block_rows, Rows&& rows_of, F&& f, G&& g) {
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    int64_t blocks_so_far = 0, rows_so_far = 0;
+    for (int s0 = 0; s0 < n_seqs; s0 += kReadThreads) {
+        const int n = min(kReadThreads, n_seqs - s0);
+        int64_t x[2] = {0, 0};
+        if (tid < n) {
+            const int64_t rows = rows_of(d.seqs[s0 + tid]);
+            x[0] = (rows + block_rows - 1) / block_rows;
+            x[1] = rows;
+        }
+#pragma unroll
+        for (int q = 0; q < 2; ++q) {
+#pragma unroll
+            for (int o = 1; o < 32; o *= 2) {
+                const int64_t y = __shfl_up_sync(0xffffffffu, x[q], o);
+                if (lane >= o) x[q] += y;
+            }
+            if (lane == 31) S.warp_sum[q][warp] = x[q];
+        }
+        __syncthreads();
+#pragma unroll
+        for (int q = 0; q < 2; ++q)
+            for (int w = 0; w < warp; ++w) x[q] += S.warp_sum[q][w];
+        S.block0[tid + 1] = blocks_so_far + x[0];
+        S.row0[tid + 1] = rows_so_far + x[1];
+        if (tid == 0) {
+            S.block0[0] = blocks_so_far;
+            S.row0[0] = rows_so_far;
+        }
+        __syncthreads();
+        const int64_t end = S.block0[n];
+        int64_t b = blocks_so_far + (gridDim.x + blockIdx.x - blocks_so_far % gridDim.x) % gridDim.x;
+        for (int lo = 0; b < end; b += gridDim.x) {
+            int hi = n;   // the sequence with block0[lo] <= b < block0[lo + 1]
+            while (hi - lo > 1) {
+                const int mid = (lo + hi) / 2;
+                if (S.block0[mid] <= b) lo = mid;
+                else hi = mid;
+            }
+            f(d.seqs[s0 + lo], static_cast<int>(b - S.block0[lo]), b, S.row0[lo]);
+        }
+        g(s0, n, S.block0);
+        blocks_so_far = end;
+        rows_so_far = S.row0[n];
+        __syncthreads();
+    }
+    return blocks_so_far;
+}
+
+// All rows of all sequences, one sequence after another.  HBM-bound.
+constexpr int kReadRows = 64;   // the smallest page
+template <class Out>
+__global__ void __launch_bounds__(kReadThreads) read8_kernel(const __grid_constant__ Read8Args A) {
+    __shared__ WalkSmem S;
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    if (A.d.hdr->id != A.plan_id) {
+        if (threadIdx.x == 0) record_error(A.err, kErrBadDesc);
+        return;
+    }
+    walk(
+        S, A.d, A.n_seqs, kReadRows, [](const ChunkSeq& s) { return s.n_tokens > 0 ? static_cast<int64_t>(s.pos) + s.n_tokens : 0; },
+        [&](const ChunkSeq& s, int block, int64_t, int64_t row0) {
+            const int r = block * kReadRows;
+            const int64_t at = row0 + r;
+            const int n = static_cast<int>(min(static_cast<int64_t>(min(kReadRows, s.pos + s.n_tokens - r)), A.n_rows - at));
+            if (n < min(kReadRows, s.pos + s.n_tokens - r) && threadIdx.x == 0) record_error(A.err, kErrRoom);
+            if (n <= 0) return;
+            const int id = s.pages[r >> A.pool.page_shift];
+            if (threadIdx.x == 0 && static_cast<unsigned>(id) >= static_cast<unsigned>(A.pool.n_pages)) record_error(A.err, kErrBadPage);
+            read_rows(A.pool, A.n_head_kv, id, r & ((1 << A.pool.page_shift) - 1), n,
+                      A.k ? static_cast<Out*>(A.k) + at * A.k_stride : nullptr, A.k_stride,
+                      A.v ? static_cast<Out*>(A.v) + at * A.v_stride : nullptr, A.v_stride);
+        },
+        [](int, int, const int64_t*) {});
+}
+
+// The rows of the batch's new tokens, 16 elements a thread.
+template <class Out>
+__global__ void __launch_bounds__(kReadThreads) read8_new_kernel(const __grid_constant__ Read8Args A) {
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    if (A.d.hdr->id != A.plan_id) {
+        if (threadIdx.x == 0) record_error(A.err, kErrBadDesc);
+        return;
+    }
+    const int per_row = A.n_head_kv * (HD / 16);
+    const int64_t i = static_cast<int64_t>(blockIdx.x) * kReadThreads + threadIdx.x;
+    const int64_t tok = i / per_row;
+    if (tok >= A.n_tokens) return;
+    const int c = static_cast<int>(i - tok * per_row);
+    const ChunkTok tk = A.d.toks[tok];
+    const int id = A.d.seqs[tk.seq].pages[tk.pos >> A.pool.page_shift];
+    const bool ok = static_cast<unsigned>(id) < static_cast<unsigned>(A.pool.n_pages);
+    if (!ok) record_error(A.err, kErrBadPage);
+    const size_t row = ok ? ((static_cast<size_t>(id) * A.n_head_kv + c / 4) << A.pool.page_shift) +
+                                (tk.pos & ((1 << A.pool.page_shift) - 1)) : 0;
+    auto one = [&](const int8_t* codes, const uint8_t* scale, void* out, int64_t stride) {
+        if (!out) return;
+        float f[16];
+        from_codes(reinterpret_cast<const uint4*>(codes + row * HD)[c % 4], ok ? scale[row] : 0, f);
+        store16(static_cast<Out*>(out) + tok * stride + c * 16, f);
+    };
+    one(A.pool.key_codes, A.pool.key_scale, A.k, A.k_stride);
+    one(A.pool.value_codes, A.pool.value_scale, A.v, A.v_stride);
+}
+
+// The rows of the sequences of many rows (those that chunk_few8_kernel does
+// not take) as bf16 pages of kStageRows rows, and a copy of the descriptor's
+// first records with page tables that lead to them, for the attention over
+// bf16 pages.  Nothing is rounded: the stored values are bf16 numbers.
+__global__ void __launch_bounds__(kReadThreads) stage8_kernel(const __grid_constant__ Stage8Args A) {
+    __shared__ WalkSmem S;
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    const bool mine = A.d.hdr->id == A.plan_id;
+    if (!mine) {   // the attention will find the number of no plan
+        if (blockIdx.x == 0 && threadIdx.x == 0) {
+            record_error(A.err, kErrBadDesc);
+            A.hdr->id = 0;
+        }
+        return;
+    }
+    const size_t row_halfs = static_cast<size_t>(A.n_head_kv) * HD;
+    const int64_t total = walk(
+        S, A.d, A.n_seqs, kStageRows,
+        [&](const ChunkSeq& s) {
+            return static_cast<int64_t>(s.n_tokens) * A.group > kChunkFewRows ? static_cast<int64_t>(s.pos) + s.n_tokens : 0;
+        },
+        [&](const ChunkSeq& s, int block, int64_t at, int64_t) {
+            if (at >= A.n_pages) return;
+            if (threadIdx.x == 0) A.table[at] = static_cast<int32_t>(at);
+            for (int half = 0; half < kStageRows; half += kReadRows) {
+                const int r = block * kStageRows + half;
+                const int n = min(kReadRows, s.pos + s.n_tokens - r);
+                if (n <= 0) break;
+                const int id = s.pages[r >> A.pool.page_shift];
+                if (threadIdx.x == 0 && static_cast<unsigned>(id) >= static_cast<unsigned>(A.pool.n_pages)) record_error(A.err, kErrBadPage);
+                const size_t to = (static_cast<size_t>(at) * kStageRows + half) * row_halfs;
+                read_rows(A.pool, A.n_head_kv, id, r & ((1 << A.pool.page_shift) - 1), n, A.k + to, row_halfs, A.v + to, row_halfs);
+            }
+        },
+        [&](int s0, int n, const int64_t* block0) {
+            const int n_rec = A.n_ctas + A.n_segs;   // cta records and segments are one array
+            for (int i = blockIdx.x * kReadThreads + threadIdx.x; i < n_rec; i += gridDim.x * kReadThreads) {
+                ChunkSeg sg = A.d.cta[i];
+                if (sg.seq < s0 || sg.seq >= s0 + n) continue;
+                sg.pages = A.table + block0[sg.seq - s0];
+                A.cta[i] = sg;
+            }
+        });
+    if (blockIdx.x == 0 && threadIdx.x == 0) {
+        ChunkHeader h = *A.d.hdr;
+        if (total > A.n_pages) {
+            record_error(A.err, kErrRoom);
+            h.id = 0;
+        }
+        *A.hdr = h;
+    }
+}
+
+}  // namespace
+
+cudaError_t launch_append_rules(const AppendRulesArgs& a, bool act_bf16, int pool_bytes, cudaStream_t stream) {
+    const int per_piece = act_bf16 ? 4 : 2;   // heads
+    const int pieces = (a.a.n_head + 2 * a.a.n_head_kv + per_piece - 1) / per_piece;
+    const int most = (pieces + kPart - 1) / kPart;
+    const int parts = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(most, kWarps / a.a.n_tokens)));
+    const int64_t blocks = (static_cast<int64_t>(a.a.n_tokens) * parts * 32 + kThreads - 1) / kThreads;
+    if (blocks > 0x7fffffffLL) return cudaErrorInvalidConfiguration;
+    Launch L(dim3(static_cast<unsigned>(blocks)), kThreads, 0, stream);
+    if (act_bf16)
+        return pool_bytes == 1   ? cudaLaunchKernelEx(&L.cfg, append_rules_kernel<__nv_bfloat16, int8_t>, a, parts)
+               : pool_bytes == 2 ? cudaLaunchKernelEx(&L.cfg, append_rules_kernel<__nv_bfloat16, __nv_bfloat16>, a, parts)
+                                 : cudaLaunchKernelEx(&L.cfg, append_rules_kernel<__nv_bfloat16, float>, a, parts);
+    return pool_bytes == 1   ? cudaLaunchKernelEx(&L.cfg, append_rules_kernel<float, int8_t>, a, parts)
+           : pool_bytes == 2 ? cudaLaunchKernelEx(&L.cfg, append_rules_kernel<float, __nv_bfloat16>, a, parts)
+                             : cudaLaunchKernelEx(&L.cfg, append_rules_kernel<float, float>, a, parts);
+}
+
+cudaError_t launch_read8(const Read8Args& a, bool out_bf16, bool new_only, cudaStream_t stream) {
+    if (new_only) {
+        const int64_t blocks = (static_cast<int64_t>(a.n_tokens) * a.n_head_kv * (HD / 16) + kReadThreads - 1) / kReadThreads;
+        if (blocks > 0x7fffffffLL) return cudaErrorInvalidConfiguration;
+        Launch L(dim3(static_cast<unsigned>(blocks)), kReadThreads, 0, stream);
+        return out_bf16 ? cudaLaunchKernelEx(&L.cfg, read8_new_kernel<__nv_bfloat16>, a)
+                        : cudaLaunchKernelEx(&L.cfg, read8_new_kernel<float>, a);
+    }
+    const int64_t blocks = std::min<int64_t>(148 * 8, a.n_rows / kReadRows + a.n_seqs);
+    Launch L(dim3(static_cast<unsigned>(blocks)), kReadThreads, 0, stream);
+    return out_bf16 ? cudaLaunchKernelEx(&L.cfg, read8_kernel<__nv_bfloat16>, a) : cudaLaunchKernelEx(&L.cfg, read8_kernel<float>, a);
+}
+
+cudaError_t launch_stage8(const Stage8Args& a, cudaStream_t stream) {
+    const int64_t blocks = std::min<int64_t>(148 * 8, std::max<int64_t>(a.n_pages, 1));
+    Launch L(dim3(static_cast<unsigned>(blocks)), kReadThreads, 0, stream);
+    return cudaLaunchKernelEx(&L.cfg, stage8_kernel, a);
+}
+
+}  // namespace tle

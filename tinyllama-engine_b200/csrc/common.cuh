@@ -23,6 +23,7 @@ enum : uint32_t {
     kErrF16Range = 0x109,   // batched prompt: a finite value beyond fp16's range became inf
     kErrBadSeq = 0x10a,     // bf16 decode: a sequence record outside its cache or max_rows (skipped)
     kErrBadDesc = 0x10b,    // chunk calls: a descriptor of another plan than the launch (nothing done)
+    kErrRoom = 0x10c,       // 8-bit cache calls: more rows than the caller's buffer has room for (not written)
     kErrSelfTest = 0x1ff,   // tle_selftest_wait_timeout: the planted wait expired
 };
 

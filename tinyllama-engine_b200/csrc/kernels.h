@@ -1,6 +1,7 @@
 // kernels.h -- internal interface between the C ABI (abi.cu) and the kernels.
 #pragma once
 
+#include <cuda_bf16.h>
 #include <cuda_runtime.h>
 #include <stdint.h>
 
@@ -459,6 +460,61 @@ struct ChunkArgs {
     uint32_t* err;
 };
 cudaError_t launch_chunk_attention(const ChunkArgs& a, bool act_bf16, cudaStream_t stream);
+// Its parts, for the attention over 8-bit pages: the items of many rows, and
+// the joining of all partial results.
+cudaError_t launch_chunk_many(const ChunkArgs& a, bool act_bf16, cudaStream_t stream);
+cudaError_t launch_chunk_merge(const ChunkArgs& a, bool act_bf16, cudaStream_t stream);
+
+// ---- pages of 8 bits (cache8.cu, attend8.cu) ----
+struct Pool8 {                   // one layer
+    const int8_t* key_codes;     // [n_pages][n_head_kv][1 << page_shift][64]
+    const int8_t* value_codes;
+    const uint8_t* key_scale;    // [n_pages][n_head_kv][1 << page_shift]
+    const uint8_t* value_scale;
+    int n_pages, page_shift;
+};
+struct AppendRulesArgs {
+    AppendArgs a;                // inv_freq: the first `half` are used
+    int half, halves;            // pairs that are rotated; 1: pairs (i, i + half), 0: (2i, 2i + 1)
+    float factor;                // on sine and cosine
+    const float* q_norm;         // [64] or null
+    const float* k_norm;
+    float eps;
+    uint8_t* key_scale;          // 8-bit pools: the layer's scales
+    uint8_t* value_scale;
+};
+// pool_bytes: 1, 2 (bf16) or 4 (fp32) per element
+cudaError_t launch_append_rules(const AppendRulesArgs& a, bool act_bf16, int pool_bytes, cudaStream_t stream);
+struct Read8Args {
+    ChunkDesc d;
+    uint64_t plan_id;
+    Pool8 pool;
+    int n_seqs, n_tokens, n_head_kv;
+    int64_t n_rows;              // rows that k and v have room for
+    void* k;
+    void* v;
+    int64_t k_stride, v_stride;
+    uint32_t* err;
+};
+cudaError_t launch_read8(const Read8Args& a, bool out_bf16, bool new_only, cudaStream_t stream);
+constexpr int kStageRows = 128;  // rows of a staged bf16 page
+struct Stage8Args {
+    ChunkDesc d;
+    uint64_t plan_id;
+    Pool8 pool;
+    int n_seqs, n_head_kv, group, n_ctas, n_segs;   // n_ctas: of both kernels
+    int64_t n_pages;             // staged pages that there is room for
+    ChunkHeader* hdr;            // the copied records
+    ChunkSeg* cta;
+    int32_t* table;              // [n_pages]
+    __nv_bfloat16* k;            // [n_pages][kStageRows][n_head_kv * 64]
+    __nv_bfloat16* v;
+    uint32_t* err;
+};
+cudaError_t launch_stage8(const Stage8Args& a, cudaStream_t stream);
+// The items of few rows over 8-bit pages (a.key_pool, a.value_pool and the
+// pool's sizes are not read).
+cudaError_t launch_chunk_few8(const ChunkArgs& a, const Pool8& pool, bool act_bf16, cudaStream_t stream);
 // Logit rules (logits.cu): rules as in tle_forward.h, checked by the caller.
 struct LogitArgs {
     const float* logits;

@@ -10,8 +10,9 @@ Names follow the reference: ``rope`` (ops.h:175), ``attention`` (ops.h:204),
 ``rope_attention`` (forward.cpp:192-208 fused), ``DecodeBatch`` (attention()
 for many sequences), ``prefill`` (generate.cpp:56-59 as one causal kernel).
 Without a counterpart there: ``PagedChunkBatch`` (chunks of new tokens over a
-paged cache) and ``logits_adjust`` (penalties, biases and masks before a
-sampler).
+paged cache of fp32, bf16 or 8-bit rows), ``AppendRules`` (rope layouts, scaled
+positions, norms of heads) and ``logits_adjust`` (penalties, biases and masks
+before a sampler).
 """
 from __future__ import annotations
 
@@ -32,6 +33,8 @@ TLE_ERR_DEVICE = 5
 TLE_DECODE_ROTATE = 1
 TLE_ACT_F32, TLE_ACT_BF16 = 0, 1
 TLE_DECODE_KV_READY = 2
+TLE_ROPE_INTERLEAVED, TLE_ROPE_HALF = 0, 1
+TLE_READ_NEW = 1
 
 
 def _decode_flags(rotate: bool, kv_ready: bool) -> int:
@@ -54,6 +57,9 @@ EXPORTED = (
     # chunks over a paged cache, logit rules
     "tle_chunk_desc_bytes", "tle_chunk_desc_paged", "tle_append_paged", "tle_append_bf16_paged",
     "tle_prefill_bf16_paged_workspace_bytes", "tle_prefill_bf16_paged", "tle_logits_adjust",
+    # rules of an append, pages of 8 bits
+    "tle_rope_frequencies", "tle_append_rules_paged", "tle_append_rules_bf16_paged", "tle_append_q8_paged",
+    "tle_read_q8_paged", "tle_prefill_q8_paged_workspace_bytes", "tle_prefill_q8_paged",
 )
 
 
@@ -117,6 +123,19 @@ class ChunkPlan(ctypes.Structure):
     _fields_ = [(n, ctypes.c_int32) for n in ("n_seqs", "n_tokens", "n_head", "n_head_kv", "page_rows",
                                                "n_ctas", "n_few_ctas", "n_segs", "n_merge", "merge_rows")] + \
                [("part_rows", ctypes.c_int64), ("desc_bytes", ctypes.c_int64)]
+
+
+class PagePoolQ8(ctypes.Structure):
+    """tle_page_pool_q8_t: page pools of 8 bits."""
+    _fields_ = [(n, ctypes.c_void_p) for n in ("key_codes", "value_codes", "key_scale", "value_scale")] + \
+               [("n_pages", ctypes.c_int32), ("page_rows", ctypes.c_int32)]
+
+
+class AppendRulesDesc(ctypes.Structure):
+    """tle_append_rules_t: rope layout and norms of an append."""
+    _fields_ = [("layout", ctypes.c_int32), ("rotary_dim", ctypes.c_int32), ("inv_freq", ctypes.c_void_p),
+                ("rope_factor", ctypes.c_float), ("norm_eps", ctypes.c_float), ("q_norm", ctypes.c_void_p),
+                ("k_norm", ctypes.c_void_p)]
 
 
 class LogitRulesDesc(ctypes.Structure):
@@ -232,6 +251,14 @@ def lib() -> ctypes.CDLL:
         L.tle_prefill_bf16_paged_workspace_bytes.restype = sz
         L.tle_prefill_bf16_paged.argtypes = [P(Shape), vp, P(ChunkPlan), vp, vp, i64, vp, i64, i, i, vp, sz,
                                              vp]
+        L.tle_rope_frequencies.argtypes = [i, f, i, f, i, P(ctypes.c_float), P(ctypes.c_float)]
+        for name in ("tle_append_rules_paged", "tle_append_rules_bf16_paged", "tle_append_q8_paged"):
+            getattr(L, name).argtypes = [P(Shape), vp, P(ChunkPlan), vp, vp, i64, vp, i64, vp, i64, vp, i,
+                                         i, i, vp, vp]
+        L.tle_read_q8_paged.argtypes = [P(Shape), vp, P(ChunkPlan), vp, vp, i64, vp, i64, i64, i, i, i, vp]
+        L.tle_prefill_q8_paged_workspace_bytes.argtypes = [P(Shape), P(PagedChunk), i, P(ChunkPlan)]
+        L.tle_prefill_q8_paged_workspace_bytes.restype = sz
+        L.tle_prefill_q8_paged.argtypes = [P(Shape), vp, P(ChunkPlan), vp, vp, i64, vp, i64, i, i, vp, sz, vp]
         L.tle_logits_adjust.argtypes = [vp, i64, vp, i64, i, i, P(LogitRulesDesc), vp]
         _lib = L
     return _lib
@@ -554,6 +581,9 @@ class PagedKVCache:
 
     The pools are [n_layers][n_pages][page_rows][256] fp32 (256 = n_head_kv *
     head_dim of the shape), made here or given as ``pools`` = (keys, values);
+    dtype torch.int8: [n_layers][n_pages][n_head_kv][page_rows][64] codes, and
+    their rows' scales, uint8 [n_layers][n_pages][n_head_kv][page_rows]
+    (tle_page_pool_q8_t; pools = (keys, values, key scales, value scales));
     a sequence's row r lives in row r % page_rows of page ``table[r // page_rows]``.  Page ids
     are handed out from a free list (``alloc`` / ``free``); the page tables
     are int32 CUDA tensors the caller keeps per sequence.  The reference keeps
@@ -568,19 +598,28 @@ class PagedKVCache:
         self.page_rows = int(page_rows)
         self.dtype = dtype or torch.float32   # torch.bfloat16: pools for PagedDecodeBatchBf16
         dims = (self.shape.n_layers, self.n_pages, self.page_rows, self.shape.n_head_kv * self.shape.head_dim)
+        kinds = ((dims, self.dtype),) * 2
+        if self.dtype == torch.int8:
+            scales = (self.shape.n_layers, self.n_pages, self.shape.n_head_kv, self.page_rows)
+            kinds = ((scales + (self.shape.head_dim,), torch.int8),) * 2 + ((scales, torch.uint8),) * 2
         if pools is not None:
-            self.key_pool, self.value_pool = pools
-            for t in pools:
-                if tuple(t.shape) != dims or t.dtype != self.dtype or not t.is_contiguous() or \
-                        t.device != pools[0].device:
-                    raise ValueError(f"pools: need two contiguous {self.dtype} tensors of shape {dims}")
+            pools = tuple(pools)
+            if len(pools) != len(kinds):
+                raise ValueError(f"pools: need {len(kinds)} tensors, got {len(pools)}")
+            for t, (shape_, dt) in zip(pools, kinds):
+                if tuple(t.shape) != shape_ or t.dtype != dt or not t.is_contiguous() or t.device != pools[0].device:
+                    raise ValueError(f"pools: need a contiguous {dt} tensor of shape {shape_} on {pools[0].device}")
         else:
-            self.key_pool = torch.zeros(dims, dtype=self.dtype, device=device)
-            self.value_pool = torch.zeros(dims, dtype=self.dtype, device=device)
+            pools = tuple(torch.zeros(shape_, dtype=dt, device=device) for shape_, dt in kinds)
+        self.key_pool, self.value_pool = pools[:2]
+        self.key_scale, self.value_scale = pools[2:] if len(pools) == 4 else (None, None)
         self._free = list(range(self.n_pages - 1, -1, -1))
 
     def pool(self):
         import torch
+        if self.dtype == torch.int8:
+            return PagePoolQ8(_ptr(self.key_pool), _ptr(self.value_pool), _ptr(self.key_scale), _ptr(self.value_scale),
+                              self.n_pages, self.page_rows)
         if self.dtype != torch.float32:
             return PagePoolBf16(_ptr(self.key_pool), _ptr(self.value_pool), self.n_pages, self.page_rows)
         return PagePool(_ptr(self.key_pool), _ptr(self.value_pool), self.n_pages, self.page_rows)
@@ -664,6 +703,62 @@ class PagedDecodeBatch:
 
 
 # ------------------------------------------------- chunks over a paged cache
+_ROPE_SCALES = ("none", "linear", "ntk", "yarn")
+
+
+def rope_frequencies(rotary_dim: int = 64, base: float = 10000.0, scaling: str = "none", factor: float = 1.0,
+                     original_ctx: int = 2048):
+    """(inv_freq, rope_factor) for AppendRules: the frequencies of rotary_dim / 2
+    pairs for contexts `factor` times as long as original_ctx rows
+    (tle_rope_frequencies); scaling "none", "linear", "ntk" or "yarn"."""
+    if scaling not in _ROPE_SCALES:
+        raise ValueError(f"scaling: one of {_ROPE_SCALES}, got {scaling!r}")
+    freq, mul = (ctypes.c_float * 32)(), ctypes.c_float(1.0)
+    _check(lib().tle_rope_frequencies(_ROPE_SCALES.index(scaling), base, rotary_dim, factor, original_ctx, freq,
+                                      ctypes.byref(mul)))
+    return list(freq[:rotary_dim // 2]), mul.value
+
+
+class AppendRules:
+    """What PagedChunkBatch.append does to q and k heads (tle_append_rules_t):
+
+    layout       "interleaved": pairs (2i, 2i + 1); "half": (i, i + rotary_dim / 2);
+    rotary_dim   elements of a head that are rotated (16, 32, 48 or 64); None:
+        twice the frequencies given, or 64;
+    inv_freq     frequencies of the pairs (numbers; None: the shape's base), see
+        rope_frequencies; rope_factor: on sine and cosine;
+    q_norm, k_norm  float32 CUDA [64] or None: heads become
+        x / sqrt(mean(x^2) + eps) * norm before they are rotated.
+    """
+
+    def __init__(self, layout: str = "interleaved", rotary_dim: Optional[int] = None, inv_freq=None, rope_factor: float = 1.0,
+                 q_norm=None, k_norm=None, eps: float = 1e-5):
+        import torch
+        layouts = {"interleaved": TLE_ROPE_INTERLEAVED, "half": TLE_ROPE_HALF}
+        if layout not in layouts:
+            raise ValueError(f"layout: 'interleaved' or 'half', got {layout!r}")
+        freq = None if inv_freq is None else [float(x) for x in inv_freq]
+        if rotary_dim is None:
+            rotary_dim = 64 if freq is None else 2 * len(freq)
+        if freq is not None and len(freq) != rotary_dim // 2:
+            raise ValueError(f"inv_freq: need {rotary_dim // 2} numbers, got {len(freq)}")
+        self.index = None
+        for t, name in ((q_norm, "q_norm"), (k_norm, "k_norm")):
+            if t is None:
+                continue
+            if t.dtype != torch.float32 or not t.is_cuda or not t.is_contiguous() or t.numel() != 64:
+                raise ValueError(f"{name}: need a contiguous float32 CUDA tensor of 64")
+            if self.index not in (None, t.get_device()):
+                raise ValueError(f"{name}: is on {t.device}, the other norm on cuda:{self.index}")
+            self.index = t.get_device()
+        self.freq = None if freq is None else (ctypes.c_float * len(freq))(*freq)
+        self.keep = (q_norm, k_norm)
+        self.desc = AppendRulesDesc(layouts[layout], rotary_dim, None if freq is None else ctypes.addressof(self.freq),
+                                    rope_factor, eps, None if q_norm is None else q_norm.data_ptr(),
+                                    None if k_norm is None else k_norm.data_ptr())
+        self.desc_at = ctypes.addressof(self.desc)
+
+
 class PagedChunkBatch:
     """One chunk of new tokens per sequence over a PagedKVCache: ``lengths[s]``
     tokens (>= 0; 1 is a decode step) behind ``positions[s]`` cached rows,
@@ -672,8 +767,9 @@ class PagedChunkBatch:
     The tokens of all chunks are packed in sequence order: q and out
     [tokens][n_head*64], k and v [tokens][n_head_kv*64], all float32 or all
     bfloat16, rows contiguous and any row stride that is a multiple of 8.
-    ``append`` rotates q and k and stores k and v (fp32 or bf16 cache),
-    ``attend`` is the causal attention over a bf16 cache, ``run`` does both.
+    ``append`` rotates q and k and stores k and v (fp32, bf16 or 8-bit cache),
+    ``attend`` is the causal attention over a bf16 or 8-bit cache, ``run`` does
+    both, ``read`` gives rows of an 8-bit cache as numbers.
     ``set_positions`` re-plans on the host and uploads the descriptor (one H2D
     copy), once per step of all layers, not in a graph capture.  Calls of one batch share its
     descriptor and workspace: they must not overlap on the GPU, nor
@@ -697,9 +793,10 @@ class PagedChunkBatch:
         self._shape_ref = ctypes.byref(self.shape)
         self._widths = (self.shape.n_head * self.shape.head_dim, self.shape.n_head_kv * self.shape.head_dim)
         self._bf16 = cache.dtype == torch.bfloat16
+        self._q8 = cache.dtype == torch.int8
         self._acts = {torch.float32: TLE_ACT_F32, torch.bfloat16: TLE_ACT_BF16}
-        if not self._bf16 and cache.dtype != torch.float32:
-            raise ValueError(f"a float32 or bfloat16 PagedKVCache expected, got {cache.dtype}")
+        if not self._bf16 and not self._q8 and cache.dtype != torch.float32:
+            raise ValueError(f"a float32, bfloat16 or int8 PagedKVCache expected, got {cache.dtype}")
         self.max_ctas = max_ctas
         self.tables = list(tables)
         self.n = len(self.tables)
@@ -730,7 +827,11 @@ class PagedChunkBatch:
         plan = ChunkPlan()
         _check(L.tle_chunk_desc_paged(ctypes.byref(self.shape), self.cache.page_rows, chunks, self.n,
                                       self.max_ctas, host.data_ptr(), nbytes, ctypes.byref(plan)))
-        self.plan = plan
+        if self._q8:
+            nbytes = L.tle_prefill_q8_paged_workspace_bytes(ctypes.byref(self.shape), chunks, self.n, ctypes.byref(plan))
+        else:
+            nbytes = L.tle_prefill_bf16_paged_workspace_bytes(ctypes.byref(plan))
+        self.plan, self._ws_bytes = plan, nbytes
         return host[:plan.desc_bytes]
 
     def set_positions(self, positions: Sequence[int], lengths: Sequence[int], stream=None) -> None:
@@ -743,9 +844,9 @@ class PagedChunkBatch:
                     raise RuntimeError("a plan is made and uploaded outside of a graph capture: a replay would upload "
                                        "from a host buffer that is long given back")
                 host = self.build_host(positions, lengths)   # a new one: the last upload may be pending
-                nbytes = lib().tle_prefill_bf16_paged_workspace_bytes(ctypes.byref(self.plan))
+                nbytes = self._ws_bytes
                 if self.workspace is None or self.workspace.numel() * 4 < nbytes:
-                    self.workspace = torch.empty(self._room(max(nbytes // 4, 4), self.workspace), dtype=torch.float32,
+                    self.workspace = torch.empty(self._room(max(-(-nbytes // 4), 4), self.workspace), dtype=torch.float32,
                                                  device=self.device)
                     self._streams.clear()
                 if self._desc_dev is None or self._desc_dev.numel() < host.numel():
@@ -761,6 +862,8 @@ class PagedChunkBatch:
                         d[:8].zero_()   # the number of no plan: a captured call does nothing
         self.positions = [int(p) for p in positions]
         self.lengths = [int(x) for x in lengths]
+        # rows of the sequences with new tokens, as read() gives them
+        self.n_rows = sum(p + m for p, m in zip(self.positions, self.lengths) if m > 0)
 
     def _room(self, n: int, old) -> int:
         """Rows of the buffer that replaces `old` where n are needed: half as much
@@ -771,15 +874,17 @@ class PagedChunkBatch:
         self._old.append(old)
         return max(n, old.shape[0] * 3 // 2)
 
-    def _rows(self, t, w: int, name: str, dtype):
-        """Pointer and row stride of an activation tensor of rows of w."""
+    def _rows(self, t, w: int, name: str, dtype, n: Optional[int] = None):
+        """Pointer and row stride of an activation tensor of at least n rows of
+        w (None: the plan's tokens)."""
         shape, strides = t.shape, t.stride()
+        n = self.plan.n_tokens if n is None else n
         if t.dtype is not dtype:
             raise ValueError(f"{name}: activations are all float32 or all bfloat16, got {t.dtype}")
         if t.get_device() != self._index:
             raise ValueError(f"{name}: is on {t.device}, the cache on {self.device}")
-        if len(shape) != 2 or shape[1] != w or shape[0] < self.plan.n_tokens or strides[1] != 1:
-            raise ValueError(f"{name}: need [{self.plan.n_tokens}][{w}] with contiguous rows, got "
+        if len(shape) != 2 or shape[1] != w or shape[0] < n or strides[1] != 1:
+            raise ValueError(f"{name}: need [{n}][{w}] with contiguous rows, got "
                              f"{tuple(shape)} with strides {strides}")
         return t.data_ptr(), (strides[0] if shape[0] > 1 else w)
 
@@ -796,6 +901,10 @@ class PagedChunkBatch:
         c, pool = self.cache, self._pool_made
         if pool is None:
             pool = self._pool_made = c.pool()
+        if self._q8:
+            pool.key_codes, pool.value_codes = c.key_pool.data_ptr(), c.value_pool.data_ptr()
+            pool.key_scale, pool.value_scale = c.key_scale.data_ptr(), c.value_scale.data_ptr()
+            return pool
         pool.key_pool = c.key_pool.data_ptr()
         pool.value_pool = c.value_pool.data_ptr()
         return pool
@@ -812,10 +921,12 @@ class PagedChunkBatch:
             self._streams.add(raw)
         return raw
 
-    def append(self, q, k, v, layer: int, rotate: bool = True, q_out=None, stream=None) -> None:
+    def append(self, q, k, v, layer: int, rotate: bool = True, q_out=None, stream=None,
+               rules: Optional["AppendRules"] = None) -> None:
         """rope(q, k) at each token's position (rotate), k and v stored in
         their rows of the cache, q written to q_out (contiguous, the type of
-        q; may be q; q and q_out both None: keys and values only)."""
+        q; may be q; q and q_out both None: keys and values only).  rules:
+        another rope than the shape's, norms of q and k heads."""
         act, dt = self._act(k, "k"), k.dtype
         wq, wkv = self._widths
         kp, ks = self._rows(k, wkv, "k", dt)
@@ -833,31 +944,60 @@ class PagedChunkBatch:
             raise ValueError("q_out without q")
         L = lib()
         pool = self._pool()
+        if rules is not None or self._q8:
+            if rules is not None and rules.index not in (None, self._index):
+                raise ValueError(f"rules: are on cuda:{rules.index}, the cache on {self.device}")
+            fn = L.tle_append_q8_paged if self._q8 else L.tle_append_rules_bf16_paged if self._bf16 else L.tle_append_rules_paged
+            _on_device(self._index, fn, self._shape_ref, ctypes.addressof(pool), ctypes.byref(self.plan),
+                       self._desc_dev.data_ptr(), qp, qs, kp, ks, vp, vs, qo, act, layer,
+                       TLE_DECODE_ROTATE if rotate else 0, None if rules is None else rules.desc_at, self._on(stream))
+            return
         _on_device(self._index, L.tle_append_bf16_paged if self._bf16 else L.tle_append_paged, self._shape_ref,
                    ctypes.addressof(pool), ctypes.byref(self.plan), self._desc_dev.data_ptr(), qp, qs, kp, ks, vp, vs,
                    qo, act, layer, TLE_DECODE_ROTATE if rotate else 0, self._on(stream))
 
     def attend(self, q, out, layer: int, stream=None) -> None:
-        """Causal attention of the chunks (q already rotated) over a bf16
-        cache; rows of out behind the last token are left as they are.  out
-        may be q."""
-        if not self._bf16:
-            raise ValueError("attend: a bfloat16 PagedKVCache expected")
+        """Causal attention of the chunks (q already rotated) over a bf16 or
+        8-bit cache; rows of out behind the last token are left as they are.
+        out may be q."""
+        if not self._bf16 and not self._q8:
+            raise ValueError("attend: a bfloat16 or int8 PagedKVCache expected")
         act = self._act(q, "q")
         qp, qs = self._rows(q, self._widths[0], "q", q.dtype)
         op, os = self._rows(out, self._widths[0], "out", q.dtype)
         pool = self._pool()
-        _on_device(self._index, lib().tle_prefill_bf16_paged, self._shape_ref, ctypes.addressof(pool),
-                   ctypes.byref(self.plan), self._desc_dev.data_ptr(), qp, qs, op, os, act, layer,
+        _on_device(self._index, lib().tle_prefill_q8_paged if self._q8 else lib().tle_prefill_bf16_paged, self._shape_ref,
+                   ctypes.addressof(pool), ctypes.byref(self.plan), self._desc_dev.data_ptr(), qp, qs, op, os, act, layer,
                    self.workspace.data_ptr(), self.workspace.numel() * 4, self._on(stream))
 
-    def run(self, q, k, v, out, layer: int, rotate: bool = True, stream=None) -> None:
+    def read(self, k_out, v_out, layer: int, new_only: bool = False, stream=None) -> None:
+        """The rows of an 8-bit cache as numbers (tle_read_q8_paged), exactly:
+        rows 0 .. position + length - 1 of every sequence with new tokens, one
+        sequence after another (n_rows in all), or with new_only the rows of
+        the new tokens.  k_out and v_out [rows][n_head_kv*64], both float32 or
+        both bfloat16, any row stride that is a multiple of 8; either may be None."""
+        if not self._q8:
+            raise ValueError("read: an int8 PagedKVCache expected")
+        n = self.plan.n_tokens if new_only else self.n_rows
+        given = [t for t in (k_out, v_out) if t is not None]
+        if not given:
+            raise ValueError("read: k_out, v_out or both")
+        act, w = self._act(given[0], "k_out or v_out"), self._widths[1]
+        kp, ks = (None, 0) if k_out is None else self._rows(k_out, w, "k_out", given[0].dtype, n)
+        vp, vs = (None, 0) if v_out is None else self._rows(v_out, w, "v_out", given[0].dtype, n)
+        pool = self._pool()
+        _on_device(self._index, lib().tle_read_q8_paged, self._shape_ref, ctypes.addressof(pool), ctypes.byref(self.plan),
+                   self._desc_dev.data_ptr(), kp, ks, vp, vs, n, act, layer, TLE_READ_NEW if new_only else 0,
+                   self._on(stream))
+
+    def run(self, q, k, v, out, layer: int, rotate: bool = True, stream=None,
+            rules: Optional["AppendRules"] = None) -> None:
         """append, then attend: the attention block of one layer for every
         chunk.  q is left as it is (the rotated q goes through a buffer of
         the batch)."""
         import torch
-        if not rotate:
-            self.append(None, k, v, layer, rotate=False, stream=stream)
+        if not rotate and (rules is None or rules.desc.q_norm is None):
+            self.append(None, k, v, layer, rotate=False, stream=stream, rules=rules)
             self.attend(q, out, layer, stream=stream)
             return
         buf = self._q.get(q.dtype)
@@ -866,7 +1006,7 @@ class PagedChunkBatch:
                 buf = self._q[q.dtype] = torch.empty((self._room(self.plan.n_tokens, buf), self._widths[0]), dtype=q.dtype,
                                                      device=self.device)
             self._streams.clear()
-        self.append(q, k, v, layer, rotate=True, q_out=buf, stream=stream)
+        self.append(q, k, v, layer, rotate=rotate, q_out=buf, stream=stream, rules=rules)
         self.attend(buf, out, layer, stream=stream)
 
 
