@@ -117,6 +117,32 @@ typedef struct {
 int tle_logits_adjust(float* out, int64_t out_stride, const float* logits, int64_t logits_stride,
                       int n_rows, int n_vocab, const tle_logit_rules_t* rules, void* stream);
 
+/* How tle_sample_rows chooses among the tokens of each row; device pointers to
+ * [n_rows] numbers, NULL: off for all rows.  Off are also a top_k <= 0 or >=
+ * n_vocab, a top_p >= 1 and a min_p <= 0; NaN is off. */
+typedef struct {
+    const float* temperature;   /* NULL: 1; <= 0 or NaN: the largest logit's token */
+    const int32_t* top_k;
+    const float* top_p;         /* <= 0: the first token of the ranking       */
+    const float* min_p;         /* above 1 counts as 1                        */
+} tle_sample_rules_t;
+
+/* A token for each of n_rows rows of n_vocab logits (row r at r * logits_stride
+ * elements, left as they are), drawn with uniform[r] in [0, 1); the reference's
+ * samplers (ops.h:262-278) for a batch, in one launch.  The tokens of a row are
+ * ranked by their logits (equal ones: lower index first) and weigh exp((x - max)
+ * / temperature); kept are the first top_k, of these the ones of at least min_p
+ * times the largest weight, of these the first ones until their weights reach
+ * top_p of the sum.  The token is the first, by index, at which the running sum of the kept
+ * weights exceeds uniform[r] times their sum.  (tle_sample_top_p walks the
+ * nucleus by rank instead: the same probabilities, other tokens for the same number.)
+ * Weights are whole numbers of 2^-40 of the largest: the choice does not depend
+ * on the launch, and a token below 2^-41 of the likeliest is never drawn.  NaN
+ * logits count as -inf; of +inf logits each weighs 1 and all others nothing.  A row of -inf
+ * only gets the token -1.  n_vocab <= 393216; 4-byte aligned pointers. */
+int tle_sample_rows(int32_t* tokens, const float* logits, int64_t logits_stride, int n_rows, int n_vocab,
+                    const tle_sample_rules_t* rules, const float* uniform, void* stream);
+
 /* ---- forward() ---- */
 
 typedef struct {

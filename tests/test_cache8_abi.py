@@ -116,3 +116,15 @@ def test_rope_frequencies():
                dict(scaling="linear", factor=float("nan")), dict(scaling="yarn", factor=2.0, original_ctx=0)):
         with pytest.raises(tle.TleError):
             tle.rope_frequencies(**kw)
+
+
+def test_sampling_refuses_bad_arguments():
+    def go(out=P, x=P, xs=100, n=2, V=100, u=P, rules=True, **kw):
+        r = tle.SampleRulesDesc(**kw)
+        return tle.lib().tle_sample_rows(out, x, xs, n, V, ctypes.byref(r) if rules else None, u, None)
+    assert go(out=None) == BAD and go(x=None) == BAD and go(u=None) == BAD and go(rules=False) == BAD
+    assert go(n=0) == BAD and go(n=65536) == BAD and go(V=0) == BAD and go(xs=99) == BAD and go(xs=-100) == BAD
+    assert go(out=P + 2) == BAD and go(x=P + 1) == BAD and go(u=P + 2) == BAD
+    for name in ("temperature", "top_k", "top_p", "min_p"):
+        assert go(**{name: P + 2}) == BAD
+    assert go(V=393217, xs=393217) == tle.TLE_ERR_UNSUPPORTED

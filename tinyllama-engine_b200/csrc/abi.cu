@@ -2254,4 +2254,34 @@ int tle_logits_adjust(float* out, int64_t out_stride, const float* logits, int64
     return ok();
 }
 
+// ===================== sampling of rows (tle_forward.h) =====================
+
+int tle_sample_rows(int32_t* tokens, const float* logits, int64_t logits_stride, int n_rows, int n_vocab,
+                    const tle_sample_rules_t* rules, const float* uniform, void* stream) {
+    if (!tokens || !logits || !rules || !uniform) return set_error(TLE_ERR_INVALID, "null pointer argument");
+    if (n_rows <= 0 || n_rows > 65535 || n_vocab <= 0)
+        return set_error(TLE_ERR_INVALID, "n_rows %d outside [1, 65535] or n_vocab %d <= 0", n_rows, n_vocab);
+    if (n_vocab > tle::kSampleRowsVocab)
+        return set_error(TLE_ERR_UNSUPPORTED, "n_vocab %d > %d", n_vocab, tle::kSampleRowsVocab);
+    if (logits_stride < n_vocab)
+        return set_error(TLE_ERR_INVALID, "logits_stride %lld < n_vocab", static_cast<long long>(logits_stride));
+    for (const void* p : {static_cast<const void*>(tokens), static_cast<const void*>(logits), static_cast<const void*>(uniform),
+                          static_cast<const void*>(rules->temperature), static_cast<const void*>(rules->top_k),
+                          static_cast<const void*>(rules->top_p), static_cast<const void*>(rules->min_p)})
+        if ((reinterpret_cast<uintptr_t>(p) & 3u) != 0) return set_error(TLE_ERR_INVALID, "pointers must be 4-byte aligned");
+    tle::SampleRowsArgs a{};
+    a.logits = logits;
+    a.stride = logits_stride;
+    a.n_vocab = n_vocab;
+    a.temperature = rules->temperature;
+    a.top_k = rules->top_k;
+    a.top_p = rules->top_p;
+    a.min_p = rules->min_p;
+    a.uniform = uniform;
+    a.tokens = tokens;
+    cudaError_t e = tle::launch_sample_rows(a, n_rows, static_cast<cudaStream_t>(stream));
+    if (e != cudaSuccess) return cuda_error(e, "sampling launch");
+    return ok();
+}
+
 }  // extern "C"

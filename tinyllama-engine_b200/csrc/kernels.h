@@ -535,6 +535,22 @@ struct LogitArgs {
     uint32_t* err;
 };
 cudaError_t launch_logits_adjust(const LogitArgs& a, int n_rows, cudaStream_t stream);
+// Sampling of rows (sample.cu).  A cluster of up to 8 CTAs holds a row.
+constexpr int kSampleSlice = 49152;                   // logits that a CTA has room for
+constexpr int kSampleRowsVocab = 8 * kSampleSlice;
+struct SampleRowsArgs {
+    const float* logits;
+    int64_t stride;
+    int n_vocab;
+    const float* temperature;    // [n_rows] each, or null: 1, no top-k, 1, 0
+    const int32_t* top_k;
+    const float* top_p;
+    const float* min_p;
+    const float* uniform;        // [n_rows]
+    int32_t* tokens;             // [n_rows]
+    int slice, per_thread;       // (set by launch_sample_rows) logits of a CTA and of a thread
+};
+cudaError_t launch_sample_rows(SampleRowsArgs a, int n_rows, cudaStream_t stream);
 
 constexpr int kMaxDevices = 64;
 struct PerDeviceOnce {

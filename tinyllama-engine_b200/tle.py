@@ -11,8 +11,8 @@ Names follow the reference: ``rope`` (ops.h:175), ``attention`` (ops.h:204),
 for many sequences), ``prefill`` (generate.cpp:56-59 as one causal kernel).
 Without a counterpart there: ``PagedChunkBatch`` (chunks of new tokens over a
 paged cache of fp32, bf16 or 8-bit rows), ``AppendRules`` (rope layouts, scaled
-positions, norms of heads) and ``logits_adjust`` (penalties, biases and masks
-before a sampler).
+positions, norms of heads), ``logits_adjust`` (penalties, biases and masks
+before a sampler) and ``sample_rows`` (a token for each row of a batch).
 """
 from __future__ import annotations
 
@@ -60,6 +60,8 @@ EXPORTED = (
     # rules of an append, pages of 8 bits
     "tle_rope_frequencies", "tle_append_rules_paged", "tle_append_rules_bf16_paged", "tle_append_q8_paged",
     "tle_read_q8_paged", "tle_prefill_q8_paged_workspace_bytes", "tle_prefill_q8_paged",
+    # sampling of rows
+    "tle_sample_rows",
 )
 
 
@@ -145,6 +147,11 @@ class LogitRulesDesc(ctypes.Structure):
                                                 "bias_start", "allowed")] + \
                [("allowed_stride", ctypes.c_int64), ("n_tokens", ctypes.c_int32),
                 ("n_biases", ctypes.c_int32)]
+
+
+class SampleRulesDesc(ctypes.Structure):
+    """tle_sample_rules_t: how tle_sample_rows chooses (device pointers)."""
+    _fields_ = [(n, ctypes.c_void_p) for n in ("temperature", "top_k", "top_p", "min_p")]
 
 
 class Weight(ctypes.Structure):
@@ -259,6 +266,7 @@ def lib() -> ctypes.CDLL:
         L.tle_prefill_q8_paged_workspace_bytes.argtypes = [P(Shape), P(PagedChunk), i, P(ChunkPlan)]
         L.tle_prefill_q8_paged_workspace_bytes.restype = sz
         L.tle_prefill_q8_paged.argtypes = [P(Shape), vp, P(ChunkPlan), vp, vp, i64, vp, i64, i, i, vp, sz, vp]
+        L.tle_sample_rows.argtypes = [vp, vp, i64, i, i, P(SampleRulesDesc), vp, vp]
         L.tle_logits_adjust.argtypes = [vp, i64, vp, i64, i, i, P(LogitRulesDesc), vp]
         _lib = L
     return _lib
@@ -1229,6 +1237,60 @@ def logits_adjust(out, logits, rules: LogitRules, stream=None) -> None:
     op, os = rules._rows(out, index, "out")
     lp, ls = rules._rows(logits, index, "logits")
     _on_device(index, lib().tle_logits_adjust, op, os, lp, ls, rules.n_rows, rules.n_vocab, rules.desc_ref,
+               _raw_stream(stream, index))
+
+
+class SampleRules:
+    """How sample_rows chooses for ``n_rows`` rows of ``n_vocab`` logits
+    (tle_sample_rules_t): contiguous CUDA tensors [n_rows], or None (off).
+
+    temperature  float32; 0: the largest logit's token (None: 1);
+    top_k        int32: the first top_k tokens of the ranking (0: all);
+    min_p        float32: tokens of at least min_p times the largest probability;
+    top_p        float32: the first tokens whose probabilities reach top_p.
+    """
+
+    def __init__(self, n_rows: int, n_vocab: int, temperature=None, top_k=None, top_p=None, min_p=None):
+        import torch
+        self.n_rows, self.n_vocab = int(n_rows), int(n_vocab)
+        self.device = None
+        self._f32, self._i32 = torch.float32, torch.int32
+        self.keep = (temperature, top_k, top_p, min_p)
+        for t, name in zip(self.keep, ("temperature", "top_k", "top_p", "min_p")):
+            if t is None:
+                continue
+            dt = torch.int32 if name == "top_k" else torch.float32
+            if t.dtype != dt or not t.is_cuda or not t.is_contiguous() or t.numel() != self.n_rows:
+                raise ValueError(f"{name}: need a contiguous {dt} CUDA tensor of {self.n_rows}")
+            self.device = self.device or t.device
+            if t.device != self.device:
+                raise ValueError(f"{name}: is on {t.device}, the other rules on {self.device}")
+        self.index = None if self.device is None else self.device.index
+        self.desc = SampleRulesDesc(*[None if t is None else t.data_ptr() for t in self.keep])
+        self.desc_ref = ctypes.byref(self.desc)
+
+    def _row_numbers(self, t, index: int, name: str, dtype) -> int:
+        if t.dtype is not dtype or t.numel() != self.n_rows or not t.is_contiguous():
+            raise ValueError(f"{name}: need a contiguous {dtype} CUDA tensor of {self.n_rows}")
+        if index < 0 or t.get_device() != index:
+            raise ValueError(f"{name}: is on {t.device}, need " + (f"cuda:{index}" if index >= 0 else "a CUDA device"))
+        return t.data_ptr()
+
+
+def sample_rows(tokens_out, logits, rules: SampleRules, uniform, stream=None) -> None:
+    """A token for every row of logits (tle_sample_rows): float32 CUDA [n_rows][n_vocab]
+    with contiguous rows and any row stride, left as they are; uniform
+    float32 [n_rows] numbers in [0, 1), tokens_out int32 [n_rows] (-1 for a row of -inf only)."""
+    index = rules.index if rules.index is not None else logits.get_device()
+    n, v = rules.n_rows, rules.n_vocab
+    strides = logits.stride()
+    if logits.dtype is not rules._f32 or tuple(logits.shape) != (n, v) or (v > 1 and strides[1] != 1):
+        raise ValueError(f"logits: need float32 CUDA [{n}][{v}], rows contiguous")
+    if index < 0 or logits.get_device() != index:
+        raise ValueError(f"logits: is on {logits.device}, need " + (f"cuda:{index}" if index >= 0 else "a CUDA device"))
+    tp = rules._row_numbers(tokens_out, index, "tokens_out", rules._i32)
+    up = rules._row_numbers(uniform, index, "uniform", rules._f32)
+    _on_device(index, lib().tle_sample_rows, tp, logits.data_ptr(), strides[0] if n > 1 else v, n, v, rules.desc_ref, up,
                _raw_stream(stream, index))
 
 
