@@ -50,7 +50,7 @@ def oracle(x, T, k, p, m, u):
 
 def dev(a):
     import torch
-    return torch.from_numpy(np.ascontiguousarray(a)).cuda()
+    return torch.from_numpy(np.array(a)).cuda()
 
 
 def run(x, T=None, k=None, p=None, m=None, u=None, stream=None, xs=None):

@@ -42,13 +42,16 @@ namespace cg = cooperative_groups;
 
 constexpr int kThreads = 512;
 constexpr int kWarps = kThreads / 32;
-constexpr int kBins = 2048;
+constexpr int kBins = 2048;                // of a level of a search; in kGroups groups of 32
+constexpr int kGroups = kBins / 32;
 constexpr int kRowCtas = 8;
+constexpr int kList = kThreads;            // tokens of a bin that are ranked one by one
 constexpr uint64_t kOne = 1ull << 40;      // the largest weight
 constexpr float kReach = 28.6f;            // exp(-kReach) < 2^-41: weights beyond it are 0
 // A weight in three limbs of 14, 13 and 13 bits, so that a bin's sums of 32 bits
 // hold any slice (2^15.6 tokens).
 constexpr uint32_t kLimb0 = 14, kLimb1 = 13;
+static_assert(kGroups * kRowCtas == kThreads && kBins == 4 * kThreads, "a group of a CTA, and 4 bins, per thread");
 
 __device__ __forceinline__ uint32_t key_of(float x) {
     const uint32_t u = __float_as_uint(x);
@@ -92,16 +95,26 @@ struct RowRules {
     }
 };
 
-struct Shared {
-    uint32_t hist[3][kBins];
-    uint64_t slot[2][3][kRowCtas];   // what the CTAs of the cluster told each other, by turns
+struct alignas(16) Shared {                // the slice lies behind it
+    union {
+        uint32_t hist[3][kBins];
+        struct {                           // once nobody reads the bins any more:
+            uint64_t weight[kList];        // the weights and keys of the bin's tokens, of all CTAs
+            uint32_t key[kList];
+        };
+    };
+    uint64_t group[kRowCtas][kGroups];     // sums of 32 bins, of each CTA of the cluster
+    uint32_t fine[3 * kRowCtas][32];       // the bins of one group
+    uint32_t list[kList];                  // this CTA's keys of the bin in question
+    uint32_t count[kRowCtas], mine;        // how many each has; and this one
+    uint64_t slot[2][3][kRowCtas];         // what the CTAs of the cluster told each other, by turns
     uint64_t warp_sum[kWarps];
-    uint64_t found[2];
-    uint32_t warp_u32[kWarps];
-    int warp_arg[kWarps];
+    uint64_t found;
+    uint32_t found_key;
+    float warp_max[kWarps];
 };
 
-// The CTA's part of the exchanges: three numbers from each CTA to all.
+// The CTA's part of the exchanges.
 struct Cluster {
     cg::cluster_group g;
     Shared& S;
@@ -125,14 +138,19 @@ struct Cluster {
     }
 };
 
-// Inclusive scan over the block; returns the thread's sum, total the block's.
-__device__ __forceinline__ uint64_t block_scan(Shared& S, uint64_t x, uint64_t& total) {
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+__device__ __forceinline__ uint64_t warp_scan(uint64_t x) {
+    const int lane = threadIdx.x & 31;
 #pragma unroll
     for (int d = 1; d < 32; d *= 2) {
         const uint64_t y = __shfl_up_sync(0xffffffffu, x, d);
         if (lane >= d) x += y;
     }
+    return x;
+}
+// Inclusive scan over the block; returns the thread's sum, total the block's.
+__device__ __forceinline__ uint64_t block_scan(Shared& S, uint64_t x, uint64_t& total) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    x = warp_scan(x);
     __syncthreads();
     if (lane == 31) S.warp_sum[warp] = x;
     __syncthreads();
@@ -152,10 +170,9 @@ struct Cut {
     uint64_t ties;
 };
 
-__global__ void __launch_bounds__(kThreads) sample_kernel(const __grid_constant__ SampleRowsArgs A) {
+__global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_constant__ SampleRowsArgs A) {
     extern __shared__ __align__(16) unsigned char smem_raw[];
     Shared& S = *reinterpret_cast<Shared*>(smem_raw);
-    float* xs = reinterpret_cast<float*>(smem_raw + sizeof(Shared));
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     // the CTAs of the cluster run: their shared memory may be written to behind the wait below
     asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
@@ -165,149 +182,204 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const __grid_constant_
     const int64_t row = blockIdx.x / cl.n;
     const int v0 = cl.rank * A.slice, n = max(0, min(A.slice, A.n_vocab - v0));
     // ---- the slice into shared memory, its largest logit ----
-    float mx = -INFINITY;
-    int arg = INT32_MAX;
     const float* src = A.logits + row * A.stride + v0;
-    for (int i = tid; i < n; i += kThreads) {
-        float x = src[i] + 0.0f;               // -0 is 0
-        if (x != x) x = -INFINITY;
-        xs[i] = x;
-        if (x > mx) {
-            mx = x;
-            arg = v0 + i;
-        }
-    }
-#pragma unroll
-    for (int d = 16; d > 0; d /= 2) {
-        const float y = __shfl_xor_sync(0xffffffffu, mx, d);
-        const int b = __shfl_xor_sync(0xffffffffu, arg, d);
-        if (y > mx || (y == mx && b < arg)) {
-            mx = y;
-            arg = b;
-        }
-    }
-    if (lane == 0) {
-        S.warp_u32[warp] = __float_as_uint(mx);
-        S.warp_arg[warp] = arg;
-    }
-    __syncthreads();
-    if (tid == 0)
-        for (int w = 1; w < kWarps; ++w) {
-            const float y = __uint_as_float(S.warp_u32[w]);
-            if (y > mx || (y == mx && S.warp_arg[w] < arg)) {
-                mx = y;
-                arg = S.warp_arg[w];
-            }
-        }
-    asm volatile("barrier.cluster.wait.aligned;" ::: "memory");
+    const int head = min(n, static_cast<int>((-(reinterpret_cast<uintptr_t>(src) >> 2)) & 3u));   // before the first 16-byte boundary
+    float* xs = reinterpret_cast<float*>(smem_raw + sizeof(Shared)) + ((4 - head) & 3);              // aligned as the row is
+    float mx = -INFINITY;
+    auto take = [&](float x) {
+        x = x + 0.0f;                          // -0 is 0
+        x = x == x ? x : -INFINITY;
+        mx = fmaxf(mx, x);
+        return x;
+    };
     {
-        const auto s = cl.tell(tid == 0, __float_as_uint(mx), static_cast<uint64_t>(static_cast<uint32_t>(arg)));
-        mx = __uint_as_float(static_cast<uint32_t>(s[0][0]));
-        arg = static_cast<int>(s[1][0]);
-        for (int i = 1; i < cl.n; ++i) {
-            const float y = __uint_as_float(static_cast<uint32_t>(s[0][i]));
-            if (y > mx) {                      // equal: the earlier slice has the lower index
-                mx = y;
-                arg = static_cast<int>(s[1][i]);
-            }
+        const int body = (n - head) / 4;
+        const float4* from = reinterpret_cast<const float4*>(src + head);
+        float4* to = reinterpret_cast<float4*>(xs + head);
+        constexpr int kAhead = 8;
+        for (int i0 = tid; i0 < body; i0 += kAhead * kThreads) {
+            float4 x[kAhead];
+#pragma unroll
+            for (int q = 0; q < kAhead; ++q)
+                if (i0 + q * kThreads < body) x[q] = from[i0 + q * kThreads];
+#pragma unroll
+            for (int q = 0; q < kAhead; ++q)
+                if (i0 + q * kThreads < body) to[i0 + q * kThreads] = make_float4(take(x[q].x), take(x[q].y), take(x[q].z), take(x[q].w));
         }
+        if (tid < head) xs[tid] = take(src[tid]);
+        const int tail = head + 4 * body;
+        if (tail + tid < n && tid < 4) xs[tail + tid] = take(src[tail + tid]);
     }
     const float T = A.temperature ? A.temperature[row] : 1.0f;
-    if (mx == -INFINITY || !(T > 0.f)) {       // the same in all CTAs; nobody's memory is read from here on
-        if (cl.rank == 0 && tid == 0) A.tokens[row] = mx == -INFINITY ? -1 : arg;
-        cl.g.sync();
-        return;
-    }
     int k = A.top_k ? A.top_k[row] : 0;
-    if (k < 0 || k >= A.n_vocab) k = 0;
+    if (k >= A.n_vocab) k = 0;
     const float top_p = A.top_p ? A.top_p[row] : 1.0f;
     float min_p = A.min_p ? A.min_p[row] : 0.0f;
     min_p = min_p > 0.f ? fminf(min_p, 1.0f) : 0.f;
+    const float u = A.uniform[row];
+#pragma unroll
+    for (int d = 16; d > 0; d /= 2) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, d));
+    if (lane == 0) S.warp_max[warp] = mx;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) mx = fmaxf(mx, S.warp_max[w]);
+    asm volatile("barrier.cluster.wait.aligned;" ::: "memory");
+    {
+        const auto s = cl.tell(tid == 0, __float_as_uint(mx));
+        for (int i = 0; i < cl.n; ++i) mx = fmaxf(mx, __uint_as_float(static_cast<uint32_t>(s[0][i])));
+    }
+    const int L = A.per_thread, i0 = min(n, tid * L), i1 = min(n, i0 + L);   // this thread's tokens
+    if (mx == -INFINITY) {                     // the same in all CTAs
+        if (cl.rank == 0 && tid == 0) A.tokens[row] = -1;
+        return;
+    }
+    if (!(T > 0.f)) {                          // the first of the largest
+        int at = INT32_MAX;
+        for (int i = i1 - 1; i >= i0; --i)
+            if (xs[i] == mx) at = v0 + i;
+        at = __reduce_min_sync(0xffffffffu, at);
+        if (lane == 0) S.warp_sum[warp] = at;
+        __syncthreads();
+        for (int w = 0; w < kWarps; ++w) at = min(at, static_cast<int>(S.warp_sum[w]));
+        const auto s = cl.tell(tid == 0, at);
+        for (int i = 0; i < cl.n; ++i) at = min(at, static_cast<int>(s[0][i]));
+        if (cl.rank == 0 && tid == 0) A.tokens[row] = at;
+        return;
+    }
     RowRules R;
     R.mx = mx;
     R.inv_t = 1.0 / static_cast<double>(T);
     R.least = static_cast<double>(min_p) * static_cast<double>(kOne);
     R.reach = (min_p > 0.f ? fminf(kReach, -logf(min_p) + 0.01f) : kReach) * T;
-    const int L = A.per_thread, i0 = min(n, tid * L), i1 = min(n, i0 + L);   // this thread's tokens
-    // The cut at which the ranking's count (WEIGHT: sum of weights, without the
-    // tokens at or below `from`) first reaches `want`, which it does.
-    auto search = [&]<bool WEIGHT>(uint64_t want, uint32_t from) -> Cut {
+    // The cut at which the ranking's count (WEIGHT: sum of weights) of the tokens with a
+    // key above `from` first reaches want(its sum over all of them), among the tokens within reach: the others weigh
+    // nothing.  A want of 0, or of more than there is: no cut.  `left`: what is to be reached among the ties.
+    auto search = [&]<bool WEIGHT>(uint32_t from, auto&& want_of, Cut& cut) -> bool {
         constexpr int kLimbs = WEIGHT ? 3 : 1;
         uint32_t lo = from + 1, hi = key_of(mx);   // the keys in question
-        const float per = R.reach > 0.f ? (kBins - 1) / R.reach : 0.f;
-        bool by_logit = true;                      // bins of equal width in logits, then in keys
+        const float per = R.reach > 0.f ? kBins / R.reach : 0.f;
+        uint64_t want = 0;
         int shift = 0;
-        auto bin_of = [&](uint32_t key) {
-            if (!by_logit) return static_cast<int>((hi - key) >> shift);
-            const float d = (mx - of_key(key)) * per;   // falls with the key; inf * 0 and inf - inf: the last, the first
-            return d < kBins - 1 ? static_cast<int>(d) : key == key_of(mx) ? 0 : kBins - 1;
+        // level 0: bins of equal width in logits; then of keys.  Falls with the key;
+        // inf - inf and inf * 0 are the largest logit's.
+        auto by_logit = [&](float x) {
+            const float d = (mx - x) * per;
+            return d < kBins ? static_cast<int>(d) : x == mx ? 0 : kBins - 1;
         };
-        for (;;) {
+        for (int level = 0;; ++level) {
+            auto in = [&](float x, uint32_t key) { return key >= lo && key <= hi && (x == mx || mx - x < R.reach); };
+            auto bin_of = [&](float x, uint32_t key) { return level == 0 ? by_logit(x) : static_cast<int>((hi - key) >> shift); };
             for (int i = tid; i < kLimbs * kBins; i += kThreads) (&S.hist[0][0])[i] = 0;
+            if (tid == 0) S.mine = 0;
             __syncthreads();
             for (int i = i0; i < i1; ++i) {
                 const float x = xs[i];
                 const uint32_t key = key_of(x);
-                if (key < lo || key > hi) continue;
+                if (!in(x, key)) continue;
+                const int b = bin_of(x, key);
                 if constexpr (WEIGHT) {
                     const uint64_t w = R.weight(x);
                     if (w == 0) continue;
-                    const int b = bin_of(key);
                     atomicAdd(&S.hist[0][b], static_cast<uint32_t>(w) & ((1u << kLimb0) - 1));
                     atomicAdd(&S.hist[1][b], static_cast<uint32_t>(w >> kLimb0) & ((1u << kLimb1) - 1));
                     atomicAdd(&S.hist[2][b], static_cast<uint32_t>(w >> (kLimb0 + kLimb1)));
                 } else {
-                    atomicAdd(&S.hist[0][bin_of(key)], 1u);
+                    atomicAdd(&S.hist[0][b], 1u);
                 }
             }
+            __syncthreads();
+            auto limbs = [&](uint32_t a, uint32_t b, uint32_t c) {
+                return WEIGHT ? a + (static_cast<uint64_t>(b) << kLimb0) + (static_cast<uint64_t>(c) << (kLimb0 + kLimb1)) : a;
+            };
+            // groups of 32 bins: 8 threads each, to all CTAs
+            uint64_t sum = 0;
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                const int b = tid / 8 * 32 + tid % 8 + 8 * q;
+                sum += WEIGHT ? limbs(S.hist[0][b], S.hist[1][b], S.hist[2][b]) : S.hist[0][b];
+            }
+#pragma unroll
+            for (int d = 1; d < 8; d *= 2) sum += __shfl_xor_sync(0xffffffffu, sum, d);
+            if (lane % 8 < cl.n) *cl.g.map_shared_rank(&S.group[cl.rank][tid / 8], lane % 8) = sum;
             cl.g.sync();
-            // this CTA's bins, of all CTAs
-            const int per_cta = kBins / cl.n, per_t = (per_cta + kThreads - 1) / kThreads;
-            uint64_t mine[kBins / kThreads], sum = 0;
-#pragma unroll
-            for (int q = 0; q < kBins / kThreads; ++q) {
-                mine[q] = 0;
-                const int at = tid * per_t + q;
-                if (q < per_t && at < per_cta) {
-                    const int b = cl.rank * per_cta + at;
-                    for (int c = 0; c < cl.n; ++c) {
-                        mine[q] += *cl.g.map_shared_rank(&S.hist[0][b], c);
-                        if constexpr (WEIGHT) {
-                            mine[q] += static_cast<uint64_t>(*cl.g.map_shared_rank(&S.hist[1][b], c)) << kLimb0;
-                            mine[q] += static_cast<uint64_t>(*cl.g.map_shared_rank(&S.hist[2][b], c)) << (kLimb0 + kLimb1);
-                        }
-                    }
-                    sum += mine[q];
+            // the group in which want is reached, by every warp for itself
+            uint64_t g0 = 0, g1 = 0;
+            for (int c = 0; c < cl.n; ++c) {
+                g0 += S.group[c][2 * lane];
+                g1 += S.group[c][2 * lane + 1];
+            }
+            const uint64_t upto = warp_scan(g0 + g1);
+            if (level == 0) {
+                const uint64_t all = __shfl_sync(0xffffffffu, upto, 31);
+                want = want_of(all);
+                if (want == 0 || want > all) {
+                    cl.g.sync();               // all have read the groups
+                    return false;
                 }
             }
-            uint64_t total;
-            uint64_t before = block_scan(S, sum, total) - sum;
-            const auto s = cl.tell(tid == 0, total);
-            uint64_t base = 0;
-            for (int i = 0; i < cl.rank; ++i) base += s[0][i];
-            before += base;
-            // one thread of one CTA has the bin
-            if (tid == 0) S.found[0] = ~0ull;
+            const int first = __ffs(__ballot_sync(0xffffffffu, upto >= want)) - 1;
+            const uint64_t before2 = __shfl_sync(0xffffffffu, upto - g0 - g1, first), half = __shfl_sync(0xffffffffu, g0, first);
+            const bool second = before2 + half < want;
+            const int group = 2 * first + second;
+            uint64_t before = before2 + (second ? half : 0);
+            for (int e = warp; e < kLimbs * cl.n; e += kWarps)
+                S.fine[e][lane] = *cl.g.map_shared_rank(&S.hist[e % kLimbs][32 * group + lane], e / kLimbs);
             __syncthreads();
-#pragma unroll
-            for (int q = 0; q < kBins / kThreads; ++q) {
-                if (q < per_t && before < want && before + mine[q] >= want) {
-                    S.found[0] = cl.rank * per_cta + tid * per_t + q;
-                    S.found[1] = before;
+            uint64_t f = 0;
+            for (int c = 0; c < cl.n; ++c)
+                f += WEIGHT ? limbs(S.fine[3 * c][lane], S.fine[3 * c + 1][lane], S.fine[3 * c + 2][lane]) : S.fine[c][lane];
+            const uint64_t fine_upto = before + warp_scan(f);
+            const int at = __ffs(__ballot_sync(0xffffffffu, fine_upto >= want)) - 1;
+            want -= __shfl_sync(0xffffffffu, fine_upto - f, at);
+            const int bin = 32 * group + at;
+            if (level > 0) {
+                const uint32_t h = hi - (static_cast<uint32_t>(bin) << shift);
+                lo = max(lo, h - ((1u << shift) - 1));
+                hi = h;
+                if (lo == hi) {
+                    cl.g.sync();               // all have read the bins
+                    cut = Cut{hi, want};
+                    return true;
                 }
-                before += mine[q];
+            }
+            // ---- the bin's tokens, if they are few, ranked one by one ----
+            for (int i = i0; i < i1; ++i) {
+                const float x = xs[i];
+                const uint32_t key = key_of(x);
+                if (!in(x, key) || (level == 0 && by_logit(x) != bin)) continue;
+                const uint32_t to = atomicAdd(&S.mine, 1u);
+                if (to < kList) S.list[to] = key;
             }
             __syncthreads();
-            const auto f = cl.tell(tid == 0, S.found[0], S.found[1]);
-            int bin = 0;
-            uint64_t so_far = 0;
-            for (int i = 0; i < cl.n; ++i)
-                if (f[0][i] != ~0ull) {
-                    bin = static_cast<int>(f[0][i]);
-                    so_far = f[1][i];
+            if (tid < cl.n) *cl.g.map_shared_rank(&S.count[cl.rank], tid) = S.mine;
+            cl.g.sync();
+            const uint32_t me = tid;
+            uint32_t have = 0, key = 0;
+            for (int c = 0; c < cl.n; ++c) {
+                const uint32_t m = S.count[c];
+                if (me >= have && me - have < min(m, static_cast<uint32_t>(kList))) key = *cl.g.map_shared_rank(&S.list[me - have], c);
+                have += m;
+            }
+            if (have <= kList) {
+                S.key[tid] = key;
+                S.weight[tid] = !WEIGHT ? 1 : me < have ? R.weight(of_key(key)) : 0;
+                __syncthreads();
+                uint64_t above = 0, with = 0;
+                for (uint32_t j = 0; j < have; ++j) {
+                    const uint32_t kj = S.key[j];
+                    const uint64_t w = S.weight[j];
+                    above += kj > key ? w : 0;
+                    with += kj >= key ? w : 0;
                 }
-            want -= so_far;
-            if (by_logit) {
+                if (me < have && above < want && with >= want) {   // tokens of one key: they write the same
+                    S.found = want - above;
+                    S.found_key = key;
+                }
+                __syncthreads();
+                cut = Cut{S.found_key, S.found};
+                return true;
+            }
+            if (level == 0) {
                 // the keys of that bin: the largest one, and the smallest, by 32 probes at a time
                 auto last_with = [&](auto&& holds, uint32_t a, uint32_t b) {   // holds(a), holds falls: the largest key in [a, b]
                     while (a < b) {
@@ -320,95 +392,83 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const __grid_constant_
                     }
                     return a;
                 };
-                const uint32_t top = last_with([&](uint32_t key) { return bin_of(key) >= bin; }, lo, hi);
-                uint32_t bottom = lo;
-                if (bin < kBins - 1 && bin_of(lo) > bin) bottom = last_with([&](uint32_t key) { return bin_of(key) > bin; }, lo, top) + 1;
-                lo = bottom;
+                const uint32_t top = last_with([&](uint32_t q) { return by_logit(of_key(q)) >= bin; }, lo, hi);
+                if (by_logit(of_key(lo)) > bin) lo = last_with([&](uint32_t q) { return by_logit(of_key(q)) > bin; }, lo, top) + 1;
                 hi = top;
-                by_logit = false;
-            } else {
-                const uint32_t h = hi - (static_cast<uint32_t>(bin) << shift);
-                lo = max(lo, h - ((1u << shift) - 1));
-                hi = h;
             }
-            cl.g.sync();                            // all have read the others' bins
-            if (lo == hi) return Cut{hi, want};
             shift = max(0, 32 - __clz(hi - lo) - 11);   // (hi - lo) >> shift < kBins
         }
     };
     Cut cut{0, 0};
-    const bool ranked = k > 0;
-    if (ranked) cut = search.template operator()<false>(static_cast<uint64_t>(k), 0);
-    uint64_t tie_w = 0, ties_before = 0;            // weight of a tie; ties before this thread's tokens
-    // sum of this thread's kept weights
-    auto kept_sum = [&]() {
-        uint64_t sum = 0, ties = 0;
-        for (int i = i0; i < i1; ++i) {
-            const uint32_t key = key_of(xs[i]);
-            if (key > cut.key) sum += R.weight(xs[i]);
-            else if (key == cut.key) ++ties;
-        }
-        tie_w = cut.ties ? R.weight(of_key(cut.key)) : 0;
-        if (tie_w) {
-            uint64_t total;
-            ties_before = block_scan(S, ties, total) - ties;
-            const auto s = cl.tell(tid == 0, total);
-            for (int i = 0; i < cl.rank; ++i) ties_before += s[0][i];
-            if (ties_before < cut.ties) sum += min(ties, cut.ties - ties_before) * tie_w;
-        }
-        return sum;
-    };
-    uint64_t sum = kept_sum(), in_cta, upto = block_scan(S, sum, in_cta), base = 0, all = 0;
-    auto prefix = [&]() {
-        const auto s = cl.tell(tid == 0, in_cta);
-        base = all = 0;
-        for (int i = 0; i < cl.n; ++i) {
-            if (i < cl.rank) base += s[0][i];
-            all += s[0][i];
-        }
-    };
-    prefix();
+    if (k > 0) search.template operator()<false>(0, [&](uint64_t) { return static_cast<uint64_t>(k); }, cut);
     if (top_p < 1.0f) {
-        const double t = ceil(static_cast<double>(fmaxf(top_p, 0.f)) * static_cast<double>(all));
-        const uint64_t want = min(max(static_cast<uint64_t>(t), static_cast<uint64_t>(1)), all);
-        // above the ties of the cut so far, or among them
-        const uint64_t tied = cut.ties * tie_w;     // all tied and kept tokens' weight, if k was reached
-        const uint64_t above = all - tied;
-        if (want <= above) {
-            cut = search.template operator()<true>(want, cut.key);
-            const uint64_t w = R.weight(of_key(cut.key));
-            cut.ties = (cut.ties + w - 1) / w;      // so many of them reach what was left
+        const uint64_t tie_w = cut.ties ? R.weight(of_key(cut.key)) : 0, tied = cut.ties * tie_w;
+        uint64_t in_ties = 0;                       // what is left to be reached among the ties of the cut so far
+        Cut c2{0, 0};
+        const bool above = search.template operator()<true>(
+            cut.key,
+            [&](uint64_t above) -> uint64_t {
+                const uint64_t all = above + tied;
+                const double t = ceil(static_cast<double>(fmaxf(top_p, 0.f)) * static_cast<double>(all));
+                const uint64_t want = min(max(static_cast<uint64_t>(t), static_cast<uint64_t>(1)), all);
+                in_ties = want > above ? want - above : 0;
+                return want > above ? 0 : want;
+            },
+            c2);
+        if (above) {
+            const uint64_t w = R.weight(of_key(c2.key));
+            cut = Cut{c2.key, (c2.ties + w - 1) / w};   // so many of them reach what was left
         } else {
-            cut.ties = (want - above + tie_w - 1) / tie_w;
+            cut.ties = (in_ties + tie_w - 1) / tie_w;
         }
-        sum = kept_sum();
-        upto = block_scan(S, sum, in_cta);
-        prefix();
     }
-    const float u = A.uniform[row];
+    // ---- the running sum of kept weights, by index ----
+    const uint64_t tie_w = cut.ties ? R.weight(of_key(cut.key)) : 0;
+    uint64_t sum = 0, ties = 0;
+    for (int i = i0; i < i1; ++i) {
+        const uint32_t key = key_of(xs[i]);
+        if (key > cut.key) sum += R.weight(xs[i]);
+        else if (key == cut.key) ++ties;
+    }
+    uint64_t cta_sum, cta_ties;
+    const uint64_t sum_upto = block_scan(S, sum, cta_sum), ties_upto = block_scan(S, ties, cta_ties);
+    const auto s = cl.tell(tid == 0, cta_sum, cta_ties);
+    uint64_t base = 0, all = 0, ties_base = 0, ties_all = 0;
+    for (int i = 0; i < cl.n; ++i) {
+        if (i < cl.rank) {
+            base += s[0][i];
+            ties_base += s[1][i];
+        }
+        all += s[0][i];
+        ties_all += s[1][i];
+    }
+    all += min(ties_all, cut.ties) * tie_w;
     const uint64_t at = min(static_cast<uint64_t>(static_cast<double>(u > 0.f ? fminf(u, 1.0f) : 0.f) * static_cast<double>(all)), all - 1);
-    uint64_t run = base + upto - sum;
-    if (run <= at && at < run + sum) {
-        uint64_t ties = ties_before;
+    uint64_t tie = ties_base + ties_upto - ties;   // ties before this thread's tokens
+    uint64_t run = base + sum_upto - sum + min(tie, cut.ties) * tie_w;
+    const uint64_t end = base + sum_upto + min(tie + ties, cut.ties) * tie_w;
+    if (run <= at && at < end) {
         int i = i0;
         for (; i < i1; ++i) {
             const uint32_t key = key_of(xs[i]);
             if (key > cut.key) run += R.weight(xs[i]);
-            else if (key == cut.key && ties++ < cut.ties) run += tie_w;
+            else if (key == cut.key && tie++ < cut.ties) run += tie_w;
             if (run > at) break;
         }
         A.tokens[row] = v0 + i;
     }
-    cl.g.sync();                                    // the others may still read this CTA's memory
 }
 
 }  // namespace
 
 cudaError_t launch_sample_rows(SampleRowsArgs a, int n_rows, cudaStream_t stream) {
+    constexpr int kExtra = sizeof(Shared) + 16;     // and the alignment of a slice
+    static_assert(sizeof(Shared) % 16 == 0, "16-byte pieces of the slice");
+    static_assert(kExtra + kSampleSlice * sizeof(float) <= 232448, "shared memory of one SM");
     static PerDeviceOnce once;
     cudaError_t e = once.run([&](int) {
         return cudaFuncSetAttribute(sample_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                    static_cast<int>(sizeof(Shared) + kSampleSlice * sizeof(float)));
+                                    static_cast<int>(kExtra + kSampleSlice * sizeof(float)));
     });
     if (e != cudaSuccess) return e;
     int ctas = 1;
@@ -424,7 +484,7 @@ cudaError_t launch_sample_rows(SampleRowsArgs a, int n_rows, cudaStream_t stream
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3(static_cast<unsigned>(n_rows) * ctas);
     cfg.blockDim = dim3(kThreads);
-    cfg.dynamicSmemBytes = sizeof(Shared) + a.slice * sizeof(float);
+    cfg.dynamicSmemBytes = kExtra + a.slice * sizeof(float);
     cfg.stream = stream;
     cfg.attrs = attr;
     cfg.numAttrs = 2;
