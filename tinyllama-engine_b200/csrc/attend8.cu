@@ -6,6 +6,7 @@
 // the cache over CTAs are the chunk descriptor's: at most kChunkFewRows rows
 // an item, 128-row tiles, partial results joined by chunk_merge_kernel.  Items
 // of more rows go through chunk_attn_kernel over bf16 pages (stage8_kernel).
+#include <cuda.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <math.h>
@@ -22,57 +23,54 @@ namespace tle {
 
 namespace {
 
-// Bound by the K/V bytes, 130 a row and KV head.  Tiles come by 1-D bulk
-// copies (a head's rows of a page are contiguous) into a ring that a producer
-// warp keeps full across segments; 16 warps take 16-key steps of the tiles,
-// each with its own running maxima, sum and output, joined in shared memory at
-// the segment's end.
+// Bound by the K/V bytes, 130 a row and KV head.  Tiles of codes come by TMA (a
+// box is 64 rows of a page, 64-byte swizzle), their scales by bulk copies, into a ring that
+// a producer warp keeps full across segments; 16 warps take 16-key steps of the
+// tiles, each with its own running maximum, sum and output, joined in shared
+// memory at the segment's end.
 //
 // The codes become fp16 on their way from shared memory into the fragments of
-// m16n8k16 MMAs, exactly (the byte with its sign bit flipped, below the bits of
+// m16n8k16 MMAs, exactly (a byte with its sign bit flipped, below the bits of
 // 1024, less 1152), and K's and V's powers of two never meet an element: K's
-// multiply the scores, V's go into the exponent of the weights.  A tcgen05
-// tile would need the converted codes written back to shared memory, and 8
-// rows would leave it mostly empty.
-//
-// Which key is column c of a step's first or second 8 is free, and so is the
-// order of the 64 dimensions in a product over them: lane (g, t) takes
-// K's bytes 16 t .. 16 t + 15 of one key per 8 (one 16-byte load), and V's bytes
-// 8 g .. 8 g + 7 of the keys t, t + 4, t + 8, t + 12 of the step (columns 2 t, 2 t + 1
-// of either 8), so that no load has bank conflicts and neither K nor V is
-// transposed.
+// multiply the scores, V's the weights.  A tcgen05 tile would need the converted
+// codes written back to shared memory, and 8 rows would leave it mostly empty.
+// Matrices of 8 rows x 16 bytes are loaded as ones of 16-bit pairs, K as they lie
+// and V transposed, so that bytes 0 and 2, and 1 and 3, of a register are a
+// fragment's pair each: K's by a permutation of the 64 dimensions that q's
+// fragments share, V's by two dimensions in turn.
 //
 // Precision: q (times a power of two per row) and the weights enter as sums of
 // two fp16 numbers, 22 bits and rounding: within 2^-24 of the largest element,
 // as 32-bit arithmetic is.  The second terms are rows 8 to 15 of the A
 // fragments, so they cost no MMA.  Tensor cores cut their running sums off, so
-// the output is carried on in 32-bit registers every kFlush steps.
+// the output is carried on in 32-bit sums in shared memory every kFlush steps.
 //
-// The weights of the output are w_j = 2^(s_j + e_j - m2), e_j = bv_j - 127, with a
-// running maximum m2 of their own beside m for the sum of 2^(s_j - m): whatever
-// V's scales, the largest contribution has the largest weight.  Both maxima are whole
-// numbers, so that rescaling is exact, and move only when exceeded by more than
-// kMoveThreshold.
-constexpr int F8_WARPS = 16;
+// The output's weights are 2^(s_j - m) 2^(bv_j - 127) f with a power of two f per row
+// that keeps the largest one between 2^6 and 2^15, whatever V's scales are; m is a whole
+// number.  So all rescaling is exact; m moves when exceeded by more than
+// kMoveThreshold, f when a weight would be above 2^15.
+constexpr int F8_WARPS = 15;      // and the producer: 16 warps, so that a thread may have 128 registers
 constexpr int F8_THREADS = 32 * (F8_WARPS + 1);
 constexpr int F8_STAGES = 8;
+constexpr int kSteps = kTile / 16; // of a tile
+constexpr int kArrivals = 4 * kSteps;   // of a stage: a step of each of 1, 2 or 4 row groups arrives for 4, 2 or 1
 constexpr int kFlush = 8;          // steps of a warp whose MMAs are summed in a row
-constexpr int kBox8 = 64;          // rows of a bulk copy: the smallest page
-constexpr float kWeightBits = 7.f; // w <= 2^(kWeightBits + kMoveThreshold) = 2^15
+constexpr int kBox8 = 64;          // rows of a copy: the smallest page
 constexpr int kQBits = 12;         // the largest element of q in [2^12, 2^13)
+constexpr int kWeightBits = 15, kWeightStart = 6;
 
-struct Stage8 {
-    uint8_t k[kTile * HD];
-    uint8_t v[kTile * HD];
-    uint8_t ks[kTile];
-    uint8_t vs[kTile];
-};
 struct Few8Smem {
-    Stage8 st[F8_STAGES];
+    uint8_t k[F8_STAGES][kTile * HD];
+    uint8_t v[F8_STAGES][kTile * HD];
+    uint8_t ks[F8_STAGES][kTile];
+    uint8_t vs[F8_STAGES][kTile];
     float o[F8_WARPS][8][HD + 4];   // a warp's result, and its rows' maximum and sum
     float2 ml[F8_WARPS][8];
     uint64_t full[F8_STAGES], empty[F8_STAGES], work_full;
     Work work[kWorkCache];
+};
+struct Few8Tma {
+    CUtensorMap k, v;   // the layer's codes as [n_pages * n_head_kv][page rows][64], box {64, 64, 1}
 };
 
 __device__ __forceinline__ void mma_f16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
@@ -81,6 +79,35 @@ __device__ __forceinline__ void mma_f16(float (&d)[4], const uint32_t (&a)[4], u
         "{%0, %1, %2, %3};"
         : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void mma_f16_zero(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+        "{%10, %10, %10, %10};"
+        : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.f));
+}
+__device__ __forceinline__ void ldsm4_b(uint32_t addr, uint32_t (&r)[4]) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+                 : "r"(addr)
+                 : "memory");
+}
+__device__ __forceinline__ void ldsm4_bt(uint32_t addr, uint32_t (&r)[4]) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+                 : "r"(addr)
+                 : "memory");
+}
+__device__ __forceinline__ void tma_load_3d(void* dst, const CUtensorMap* map, int x, int y, int z, uint64_t* bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes "
+        "[%0], [%1, {%2, %3, %4}], [%5];" ::"r"(smem_u32(dst)),
+        "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(z), "r"(smem_u32(bar))
+        : "memory");
+}
+__device__ __forceinline__ void mbar_arrive_n(uint64_t* bar, uint32_t n) {
+    asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0], %1;" ::"r"(smem_u32(bar)), "r"(n) : "memory");
 }
 __device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
     uint32_t r;
@@ -100,26 +127,31 @@ __device__ __forceinline__ uint32_t codes_f16(uint32_t u) {
     asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(h), "r"(0x64806480u));   // - 1152
     return r;
 }
+// 2^e, -127 <= e <= 127
+__device__ __forceinline__ float pow2(int e) {
+    return e < -126 ? __uint_as_float(0x00400000u) : __uint_as_float(static_cast<uint32_t>(e + 127) << 23);
+}
 // 2^d for a whole number d <= 0 (or -inf).
 __device__ __forceinline__ float pow2_down(float d) {
     return d < -126.f ? 0.f : __uint_as_float(static_cast<uint32_t>(static_cast<int>(d) + 127) << 23);
 }
-__device__ __forceinline__ uint32_t byte_of(uint32_t w, int t) { return (w >> (8 * t)) & 0xffu; }
 
 template <class Act>
 __global__ void __launch_bounds__(F8_THREADS, 1)
-    chunk_few8_kernel(const __grid_constant__ ChunkArgs A, const __grid_constant__ Pool8 P) {
-    extern __shared__ __align__(128) unsigned char smem_raw[];
-    Few8Smem& S = *reinterpret_cast<Few8Smem*>(smem_raw);
+    chunk_few8_kernel(const __grid_constant__ ChunkArgs A, const __grid_constant__ Pool8 P, const __grid_constant__ Few8Tma M) {
+    extern __shared__ __align__(1024) unsigned char smem_raw[];
+    Few8Smem& S = *reinterpret_cast<Few8Smem*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     if (tid == 0) {
         for (int i = 0; i < F8_STAGES; ++i) {
             mbar_init(&S.full[i], 1);
-            mbar_init(&S.empty[i], F8_WARPS);
+            mbar_init(&S.empty[i], kArrivals);
         }
         mbar_init(&S.work_full, 1);
         fence_barrier_init();
+        prefetch_tmap(&M.k);
+        prefetch_tmap(&M.v);
     }
     asm volatile("griddepcontrol.wait;" ::: "memory");
     if (tid == 0) fetch_first(A, A.n_ctas + blockIdx.x, &S.work[0]);
@@ -159,19 +191,18 @@ __global__ void __launch_bounds__(F8_THREADS, 1)
                 wait_or_flag(&S.empty[st], ((ring / F8_STAGES) & 1) ^ 1, A.err, kErrWaitEmpty, failed);
                 failed = __any_sync(0xffffffffu, failed);
                 if (failed) break;
-                Stage8& T = S.st[st];
                 int boxes = 0;
 #pragma unroll
                 for (int b = 0; b < 2; ++b) {
                     boxes += ids[b] >= 0;
                     if (ids[b] != -2) continue;
                     for (int i = lane; i < kBox8 * HD / 16; i += 32) {   // its rows count as zeros
-                        reinterpret_cast<uint4*>(T.k + b * kBox8 * HD)[i] = make_uint4(0, 0, 0, 0);
-                        reinterpret_cast<uint4*>(T.v + b * kBox8 * HD)[i] = make_uint4(0, 0, 0, 0);
+                        reinterpret_cast<uint4*>(S.k[st] + b * kBox8 * HD)[i] = make_uint4(0, 0, 0, 0);
+                        reinterpret_cast<uint4*>(S.v[st] + b * kBox8 * HD)[i] = make_uint4(0, 0, 0, 0);
                     }
                     if (lane < kBox8 / 4) {
-                        reinterpret_cast<uint32_t*>(T.ks + b * kBox8)[lane] = 0x7f7f7f7fu;
-                        reinterpret_cast<uint32_t*>(T.vs + b * kBox8)[lane] = 0x7f7f7f7fu;
+                        reinterpret_cast<uint32_t*>(S.ks[st] + b * kBox8)[lane] = 0x7f7f7f7fu;
+                        reinterpret_cast<uint32_t*>(S.vs[st] + b * kBox8)[lane] = 0x7f7f7f7fu;
                     }
                     fence_proxy_async_smem();   // before the stage's next copy
                 }
@@ -181,12 +212,12 @@ __global__ void __launch_bounds__(F8_THREADS, 1)
 #pragma unroll
                     for (int b = 0; b < 2; ++b) {
                         if (ids[b] < 0) continue;
-                        const size_t row = ((static_cast<size_t>(ids[b]) * A.n_head_kv + w.kvh) << P.page_shift) +
-                                           (((2 * n + b) * kBox8) & ((1 << P.page_shift) - 1));
-                        bulk_g2s(T.k + b * kBox8 * HD, P.key_codes + row * HD, kBox8 * HD, &S.full[st], policy);
-                        bulk_g2s(T.ks + b * kBox8, P.key_scale + row, kBox8, &S.full[st], policy);
-                        bulk_g2s(T.v + b * kBox8 * HD, P.value_codes + row * HD, kBox8 * HD, &S.full[st], policy);
-                        bulk_g2s(T.vs + b * kBox8, P.value_scale + row, kBox8, &S.full[st], policy);
+                        const int z = ids[b] * A.n_head_kv + w.kvh, y = ((2 * n + b) * kBox8) & ((1 << P.page_shift) - 1);
+                        const size_t row = (static_cast<size_t>(z) << P.page_shift) + y;
+                        tma_load_3d(S.k[st] + b * kBox8 * HD, &M.k, 0, y, z, &S.full[st]);
+                        bulk_g2s(S.ks[st] + b * kBox8, P.key_scale + row, kBox8, &S.full[st], policy);
+                        tma_load_3d(S.v[st] + b * kBox8 * HD, &M.v, 0, y, z, &S.full[st]);
+                        bulk_g2s(S.vs[st] + b * kBox8, P.value_scale + row, kBox8, &S.full[st], policy);
                     }
                 }
                 __syncwarp();
@@ -199,47 +230,45 @@ __global__ void __launch_bounds__(F8_THREADS, 1)
             wait_or_flag(&S.full[u % F8_STAGES], (u / F8_STAGES) & 1, A.err, kErrDrain, late);
         return;
     }
-    const int g = lane >> 2, t = lane & 3;   // fragment row, and which quarter of it
-    static_assert(kChunkFewRows <= 32 && F8_WARPS % 4 == 0, "four row groups at most");
-    // row groups of 8 rows: 1, 2 or 4, each by F8_WARPS / groups warps
-    auto row_groups = [](int n_rows) { return n_rows <= 8 ? 1 : n_rows <= 16 ? 2 : 4; };
-    // This lane's 16 elements of row g of the warp's group, ahead of the segment.
-    constexpr int kRaw = 16 * sizeof(Act) / 16;
-    uint4 raw[kRaw];
+    const int g = lane >> 2, t = lane & 3;        // fragment row, and which quarter of it
+    const int mi = lane >> 3, li = lane & 7;      // ldmatrix: matrix and row of this lane's address
+    static_assert(kChunkFewRows <= 32 && F8_WARPS < 32, "four row groups at most");
+    // row groups of 8 rows: 1, 2 or 4 (as a power of two), the warps dealt out to them
+    auto group_bits = [](int n_rows) { return n_rows <= 8 ? 0 : n_rows <= 16 ? 1 : 2; };
+    auto workers = [](int gb, int rg) { return (F8_WARPS - rg + (1 << gb) - 1) >> gb; };   // warps of row group rg
+    // This lane's elements 16 c + 4 t .. + 3 of row g of the warp's group, ahead of the segment.
+    using Raw = std::conditional_t<sizeof(Act) == 4, uint4, uint2>;
+    Raw raw[HD / 16];
     auto load_q = [&](const Work& w) {
-        const int r = warp % row_groups(w.n_rows) * 8 + g;
+        const int r = (warp & ((1 << group_bits(w.n_rows)) - 1)) * 8 + g;
         const bool ok = r < w.n_rows;
         const int row = w.row0 + (ok ? r : 0), tok = row_token(A, row), h = row - tok * A.group;
-        const uint4* src = reinterpret_cast<const uint4*>(static_cast<const Act*>(A.q) +
-                                                          static_cast<int64_t>(w.first + tok) * A.q_stride +
-                                                          (w.kvh * A.group + h) * HD + 16 * t);
+        const Raw* src = reinterpret_cast<const Raw*>(static_cast<const Act*>(A.q) +
+                                                      static_cast<int64_t>(w.first + tok) * A.q_stride +
+                                                      (w.kvh * A.group + h) * HD) + t;
 #pragma unroll
-        for (int i = 0; i < kRaw; ++i) raw[i] = ok ? src[i] : make_uint4(0, 0, 0, 0);
+        for (int i = 0; i < HD / 16; ++i) raw[i] = ok ? src[4 * i] : Raw{};
     };
-    int ring = 0;
+    int ring0 = 0;   // tiles of the segments before
     auto segment = [&](const Work& w) {
-        const int rgroups = row_groups(w.n_rows), nkw = F8_WARPS / rgroups;
-        const int rg = warp % rgroups, kw = warp / rgroups;
+        const int gb = group_bits(w.n_rows), rg = warp & ((1 << gb) - 1), kw = warp >> gb;
         const int pos_r = w.pos + row_token(A, w.row0 + min(rg * 8 + g, w.n_rows - 1));
         uint32_t qf[HD / 16][4];   // A fragments: rows g the first terms, rows g + 8 the second
         float c;                   // of the row's scores: 2^e / 8 log2(e), q = 2^e (terms)
         {
             float x[16];
-            if constexpr (sizeof(Act) == 4) {
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
+            for (int i = 0; i < HD / 16; ++i) {
+                if constexpr (sizeof(Act) == 4) {
                     x[4 * i] = __uint_as_float(raw[i].x);
                     x[4 * i + 1] = __uint_as_float(raw[i].y);
                     x[4 * i + 2] = __uint_as_float(raw[i].z);
                     x[4 * i + 3] = __uint_as_float(raw[i].w);
-                }
-            } else {
-                float y[8];
-#pragma unroll
-                for (int i = 0; i < 2; ++i) {
-                    bf16x8(raw[i], y);
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) x[8 * i + e] = y[e];
+                } else {
+                    x[4 * i] = __uint_as_float(raw[i].x << 16);
+                    x[4 * i + 1] = __uint_as_float(raw[i].x & 0xffff0000u);
+                    x[4 * i + 2] = __uint_as_float(raw[i].y << 16);
+                    x[4 * i + 3] = __uint_as_float(raw[i].y & 0xffff0000u);
                 }
             }
             float most = 0.f;
@@ -248,171 +277,198 @@ __global__ void __launch_bounds__(F8_THREADS, 1)
             most = fmax3(most, __shfl_xor_sync(0xffffffffu, most, 1), 0.f);
             most = fmax3(most, __shfl_xor_sync(0xffffffffu, most, 2), 0.f);
             const bool fine = most <= 3.4028234e38f;   // otherwise every score is NaN
-            const int e = fine && most > 0.f ? ilogbf(most) - kQBits : 0;
-            c = fine ? ldexpf(kExpScale, e) : NAN;
+            // in two powers of two, neither of which leaves the range
+            const float pre = most < 0x1p-60f ? 0x1p64f : 1.f;
+            const int e = fine && most > 0.f ? static_cast<int>(__float_as_uint(most * pre) >> 23) - 127 - kQBits : 0;
+            const float up = fine ? pow2(-e) : 0.f;
+            c = fine ? kExpScale * pow2(e) * (1.f / pre) : NAN;
 #pragma unroll
-            for (int i = 0; i < 16; ++i) x[i] = fine ? ldexpf(x[i], -e) : 0.f;
+            for (int i = 0; i < 16; ++i) x[i] = fine ? x[i] * pre * up : 0.f;
 #pragma unroll
             for (int ks = 0; ks < HD / 16; ++ks) {
-                two_terms(x[4 * ks], x[4 * ks + 1], qf[ks][0], qf[ks][1]);
-                two_terms(x[4 * ks + 2], x[4 * ks + 3], qf[ks][2], qf[ks][3]);
+                two_terms(x[4 * ks], x[4 * ks + 2], qf[ks][0], qf[ks][1]);
+                two_terms(x[4 * ks + 1], x[4 * ks + 3], qf[ks][2], qf[ks][3]);
             }
         }
-        float m = -INFINITY, m2 = -INFINITY, l = 0.f;
-        float o[8][4], sum[8][2];   // sum: what o held before
+        float m = -INFINITY, l = 0.f;
+        int fe = 127;                             // f = 2^fe
+        float f = pow2(127), limit = pow2(kWeightBits - 127);
+        float o[8][4];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            o[j][0] = o[j][1] = o[j][2] = o[j][3] = 0.f;
-            sum[j][0] = sum[j][1] = 0.f;
-        }
+        for (int j = 0; j < 8; ++j) o[j][0] = o[j][1] = o[j][2] = o[j][3] = 0.f;
         int since = 0;
+        bool flushed = false;
+        // this lane's dimensions 16 c + 4 t .. + 3 of row g
+        auto held = [&](int i) -> float4& { return *reinterpret_cast<float4*>(&S.o[warp][g][16 * i + 4 * t]); };
         auto flush = [&]() {
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                sum[j][0] += o[j][0] + o[j][2];
-                sum[j][1] += o[j][1] + o[j][3];
-                o[j][0] = o[j][1] = o[j][2] = o[j][3] = 0.f;
+            for (int i = 0; i < HD / 16; ++i) {
+                float4 y = make_float4(o[2 * i][0] + o[2 * i][2], o[2 * i + 1][0] + o[2 * i + 1][2], o[2 * i][1] + o[2 * i][3],
+                                       o[2 * i + 1][1] + o[2 * i + 1][3]);
+                if (flushed) {
+                    const float4 z = held(i);
+                    y = make_float4(y.x + z.x, y.y + z.y, y.z + z.z, y.w + z.w);
+                }
+                held(i) = y;
             }
+#pragma unroll
+            for (int j = 0; j < 8; ++j) o[j][0] = o[j][1] = o[j][2] = o[j][3] = 0.f;
+            flushed = true;
             since = 0;
         };
-        // 16 keys from j0 of tile n in T; EDGE: some row does not attend to all of the tile.
-        auto step = [&]<bool EDGE>(const Stage8& T, int n, int j0) {
+        auto scale_o = [&](float by) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) o[j][e] *= by;
+            if (flushed)
+#pragma unroll
+                for (int i = 0; i < HD / 16; ++i) {
+                    const float4 z = held(i);
+                    held(i) = make_float4(z.x * by, z.y * by, z.z * by, z.w * by);
+                }
+        };
+        // 16 keys from j0 of tile n in stage st; EDGE: some row does not attend to all of the tile.
+        auto step = [&]<bool EDGE>(int st, int n, int j0) {
             const int key0 = n * kTile + j0;
             if (EDGE && key0 >= w.kv_len) return;
             if (++since > kFlush) flush();
-            // lane (g, t): of either 8 keys its column g is key (g / 2) + 4 (g % 2) + 8 b of the step
-            uint4 kr[2];
+            const uint32_t kb = smem_u32(S.k[st]), vb = smem_u32(S.v[st]);
+            // 16-byte chunk q of row r lies at q ^ (r / 2 % 4)
+            uint32_t kr[4][4];   // matrices: keys 0-7 and 8-15 of chunks 0, 1; then of 2, 3
 #pragma unroll
-            for (int b = 0; b < 2; ++b)
-                kr[b] = *reinterpret_cast<const uint4*>(T.k + (j0 + (g >> 1) + 4 * (g & 1) + 8 * b) * HD + 16 * t);
-            const uint4 ksc = *reinterpret_cast<const uint4*>(T.ks + j0), vsc = *reinterpret_cast<const uint4*>(T.vs + j0);
-            uint2 vr[4];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) vr[i] = *reinterpret_cast<const uint2*>(T.v + (j0 + t + 4 * i) * HD + 8 * g);
-            float sf[2][4];
+            for (int h = 0; h < 2; ++h) {
+                const int r = j0 + li + 8 * (mi & 1), q = 2 * h + (mi >> 1);
+                ldsm4_b(kb + r * HD + ((q ^ ((r >> 1) & 3)) << 4), kr[h]);
+                ldsm4_bt(vb + r * HD + ((q ^ ((r >> 1) & 3)) << 4), kr[2 + h]);
+            }
+            uint32_t ks2[2], vs2[2];   // the scales of keys 2 t, 2 t + 1 of either 8
 #pragma unroll
             for (int b = 0; b < 2; ++b) {
-                sf[b][0] = sf[b][1] = sf[b][2] = sf[b][3] = 0.f;
-                const uint32_t u[4] = {kr[b].x, kr[b].y, kr[b].z, kr[b].w};
-#pragma unroll
-                for (int ks = 0; ks < HD / 16; ++ks)
-                    mma_f16(sf[b], qf[ks], codes_f16(__byte_perm(u[ks], 0, 0x4140)), codes_f16(__byte_perm(u[ks], 0, 0x4342)));
+                ks2[b] = *reinterpret_cast<const uint16_t*>(&S.ks[st][j0 + 8 * b + 2 * t]);
+                vs2[b] = *reinterpret_cast<const uint16_t*>(&S.vs[st][j0 + 8 * b + 2 * t]);
             }
-            // key i of this lane: t + 4 i, columns 2 t + i % 2 of the 8 keys i / 2
-            const uint32_t kb[4] = {ksc.x, ksc.y, ksc.z, ksc.w}, vb[4] = {vsc.x, vsc.y, vsc.z, vsc.w};
-            float s[4], ev[4], su[4];
+            float sf[2][4];
+#pragma unroll
+            for (int ks = 0; ks < HD / 16; ++ks)
+#pragma unroll
+                for (int b = 0; b < 2; ++b) {
+                    const uint32_t u = kr[ks >> 1][2 * (ks & 1) + b];
+                    if (ks == 0) mma_f16_zero(sf[b], qf[ks], codes_f16(u), codes_f16(u >> 8));
+                    else mma_f16(sf[b], qf[ks], codes_f16(u), codes_f16(u >> 8));
+                }
+            float s[4], vsf[4];   // keys 2 t, 2 t + 1, 2 t + 8, 2 t + 9
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                s[i] = (sf[i >> 1][i & 1] + sf[i >> 1][2 + (i & 1)]) * c * __uint_as_float(byte_of(kb[i], t) << 23);
-                const uint32_t b = byte_of(vb[i], t);
-                ev[i] = b == 255u ? NAN : static_cast<float>(static_cast<int>(b) - 127);
-                if (EDGE && key0 + t + 4 * i > pos_r) {
+                const uint32_t kx = ks2[i >> 1], vx = vs2[i >> 1];
+                s[i] = (sf[i >> 1][i & 1] + sf[i >> 1][2 + (i & 1)]) * (__uint_as_float((i & 1 ? kx << 15 : kx << 23) & 0x7f800000u) * c);
+                vsf[i] = __uint_as_float((i & 1 ? vx << 15 : vx << 23) & 0x7f800000u);
+                if (EDGE && key0 + 8 * (i >> 1) + 2 * t + (i & 1) > pos_r) {
                     s[i] = -INFINITY;
-                    ev[i] = 0.f;
+                    vsf[i] = 0.f;
                 }
-                su[i] = s[i] + ev[i];
             }
-            float mt = fmax3(fmax3(s[0], s[1], s[2]), s[3], s[3]);
-            float mu = fmax3(fmax3(su[0], su[1], su[2]), su[3], su[3]);
-            const bool grow = (m == m && !(mt <= m + kMoveThreshold)) || (m2 == m2 && !(mu <= m2 + kMoveThreshold));
-            if (__any_sync(0xffffffffu, grow)) {
-                mt = fmax3(mt, __shfl_xor_sync(0xffffffffu, mt, 1), -INFINITY);
-                mt = fmax3(mt, __shfl_xor_sync(0xffffffffu, mt, 2), -INFINITY);
-                mu = fmax3(mu, __shfl_xor_sync(0xffffffffu, mu, 1), -INFINITY);
-                mu = fmax3(mu, __shfl_xor_sync(0xffffffffu, mu, 2), -INFINITY);
-                if (m == m && !(mt <= m + kMoveThreshold)) {
-                    const float to = ceilf(mt);
-                    l *= pow2_down(m - to);
+            const float mt = fmax3(fmax3(s[0], s[1], s[2]), s[3], s[3]);
+            if (__any_sync(0xffffffffu, m == m && !(mt <= m + kMoveThreshold))) {
+                float to = fmax3(mt, __shfl_xor_sync(0xffffffffu, mt, 1), -INFINITY);
+                to = fmax3(to, __shfl_xor_sync(0xffffffffu, to, 2), -INFINITY);
+                float by = 1.f;
+                if (m == m && !(to <= m + kMoveThreshold)) {
+                    to = ceilf(to);
+                    if (m != -INFINITY) {
+                        // weights of the new m are smaller by 2^(m - to): f makes up for it, as far as it goes
+                        l *= pow2_down(m - to);
+                        const float e = static_cast<float>(fe) + (to - m);
+                        by = pow2_down(fminf(127.f - e, 0.f));
+                        fe = static_cast<int>(fminf(e, 127.f));
+                        f = pow2(fe);
+                        limit = pow2(min(kWeightBits - fe, 127));
+                    }
                     m = to;
                 }
-                if (m2 == m2 && !(mu <= m2 + kMoveThreshold)) {
-                    const float to = ceilf(mu), f = pow2_down(m2 - to);
-                    m2 = to;
-#pragma unroll
-                    for (int j = 0; j < 8; ++j) {
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) o[j][e] *= f;
-                        sum[j][0] *= f;
-                        sum[j][1] *= f;
-                    }
-                }
+                if (__any_sync(0xffffffffu, by != 1.f)) scale_o(by);
             }
-            // nothing attended so far: all scores are -inf, and their weights 0
-            const float m_use = m == -INFINITY ? 0.f : m, shift = (m_use - (m2 == -INFINITY ? 0.f : m2)) + kWeightBits;
+            const float m_use = m == -INFINITY ? 0.f : m;   // nothing attended so far: the scores are -inf
             float wt[4];
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                const float d = s[i] - m_use;
-                l += ex2_sfu(d);
-                wt[i] = ex2_sfu(d + (ev[i] + shift));
+                const float p = ex2_sfu(s[i] - m_use);
+                l += p;
+                wt[i] = p * vsf[i];
+            }
+            const float wm = fmax3(fmax3(wt[0], wt[1], wt[2]), wt[3], wt[3]);
+            if (__any_sync(0xffffffffu, !(wm <= limit))) {
+                float to = fmax3(wm, __shfl_xor_sync(0xffffffffu, wm, 1), 0.f);
+                to = fmax3(to, __shfl_xor_sync(0xffffffffu, to, 2), 0.f);
+                float by = 1.f;
+                if (to > limit && to <= 3.4028234e38f) {
+                    const int e = max(kWeightStart + 127 - static_cast<int>(__float_as_uint(to) >> 23), -126);
+                    by = pow2_down(static_cast<float>(e - fe));
+                    fe = e;
+                    f = pow2(fe);
+                    limit = pow2(min(kWeightBits - fe, 127));
+                }
+                scale_o(by);
             }
             uint32_t pf[4];
-            two_terms(wt[0], wt[1], pf[0], pf[1]);
-            two_terms(wt[2], wt[3], pf[2], pf[3]);
+            two_terms(wt[0] * f, wt[1] * f, pf[0], pf[1]);
+            two_terms(wt[2] * f, wt[3] * f, pf[2], pf[3]);
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {   // 4 of the lane's 8 bytes: dimensions 8 g + 4 h ..
-                const uint32_t a = h ? vr[0].y : vr[0].x, b = h ? vr[1].y : vr[1].x;
-                const uint32_t cc = h ? vr[2].y : vr[2].x, d = h ? vr[3].y : vr[3].x;
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const uint32_t pick = e | ((4 + e) << 8);   // byte e of both, in bytes 0 and 2
-                    mma_f16(o[4 * h + e], pf, codes_f16(__byte_perm(a, b, pick)), codes_f16(__byte_perm(cc, d, pick)));
-                }
+            for (int q = 0; q < HD / 16; ++q) {   // chunk q: dimensions 16 q + 2 g (+1)
+                const uint32_t u0 = kr[2 + (q >> 1)][2 * (q & 1)], u1 = kr[2 + (q >> 1)][2 * (q & 1) + 1];
+                mma_f16(o[2 * q], pf, codes_f16(u0), codes_f16(u1));
+                mma_f16(o[2 * q + 1], pf, codes_f16(u0 >> 8), codes_f16(u1 >> 8));
             }
         };
-        for (int n = w.t0; n < w.t1; ++n, ++ring) {
-            const int st = ring % F8_STAGES;
+        // the steps of the segment, dealt out to the group's warps
+        const int n_steps = (w.t1 - w.t0) * kSteps, nkw = workers(gb, rg);
+        for (int i = kw; i < n_steps; i += nkw) {
+            const int n = w.t0 + i / kSteps, ring = ring0 + i / kSteps, st = ring % F8_STAGES;
             wait_or_flag(&S.full[st], (ring / F8_STAGES) & 1, A.err, kErrWaitFull, failed);
             __syncwarp();
-            const Stage8& T = S.st[st];
-            // the step s of the segment (8 a tile) is key worker s % nkw's
-            const int first = (n - w.t0) * (kTile / 16);
-            for (int j = (kw + nkw - first % nkw) % nkw; j < kTile / 16; j += nkw) {
-                if (w.edge(n)) step.template operator()<true>(T, n, 16 * j);
-                else step.template operator()<false>(T, n, 16 * j);
-            }
+            if (w.edge(n)) step.template operator()<true>(st, n, 16 * (i % kSteps));
+            else step.template operator()<false>(st, n, 16 * (i % kSteps));
             __syncwarp();
-            if (lane == 0) mbar_arrive(&S.empty[st]);
+            if (lane == 0) mbar_arrive_n(&S.empty[st], kArrivals / kSteps >> gb);
         }
+        ring0 += w.t1 - w.t0;
         flush();
         l += __shfl_xor_sync(0xffffffffu, l, 1);
         l += __shfl_xor_sync(0xffffffffu, l, 2);
         if (t == 0) S.ml[warp][g] = make_float2(m, l);
-        // with the weights 2^(s - m): the dimensions 16 t + j and 16 t + 8 + j
-        const float up = m2 - m - kWeightBits;
-        const int e = fabsf(up) < 4096.f ? static_cast<int>(up) : 0;   // 0: nothing attended, or NaN
+        const float back = pow2(-fe);   // to the weights 2^(s - m)
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            S.o[warp][g][16 * t + j] = ldexpf(sum[j][0], e);
-            S.o[warp][g][16 * t + 8 + j] = ldexpf(sum[j][1], e);
+        for (int i = 0; i < HD / 16; ++i) {
+            const float4 z = held(i);
+            held(i) = make_float4(z.x * back, z.y * back, z.z * back, z.w * back);
         }
     };
     if (seg0 < seg1) load_q(S.work[0]);
     if (warp == F8_WARPS - 1) fetch_work(A, seg0, seg1, S.work, &S.work_full);
     for (int sg = seg0; sg < seg1; ++sg) {
-        const Work w = work_of(sg);
+        const Work& w = work_of(sg);
         segment(w);
         if (sg + 1 < seg1) load_q(work_of(sg + 1));
         named_bar_sync(1, 32 * F8_WARPS);
         // ---- join the key workers: a row per warp, two columns per lane; lane q has the
         // weight of worker q ----
-        const int rgroups = row_groups(w.n_rows), nkw = F8_WARPS / rgroups;
+        const int gb = group_bits(w.n_rows);
         for (int r = warp; r < w.n_rows; r += F8_WARPS) {
-            const int w0 = r >> 3, rr = r & 7;
-            const float2 ml = lane < nkw ? S.ml[w0 + lane * rgroups][rr] : make_float2(-INFINITY, 0.f);
+            const int w0 = r >> 3, rr = r & 7, nkw = workers(gb, w0);
+            const float2 ml = lane < nkw ? S.ml[w0 + (lane << gb)][rr] : make_float2(-INFINITY, 0.f);
             float m_all = ml.x;
 #pragma unroll
-            for (int d = 1; d < F8_WARPS; d *= 2) m_all = fmaxf(m_all, __shfl_xor_sync(0xffffffffu, m_all, d));
-            const float f = ml.x == -INFINITY ? 0.f : ex2_sfu(ml.x - m_all);
-            float l_all = f == 0.f ? 0.f : f * ml.y;
+            for (int d = 1; d < 16; d *= 2) m_all = fmaxf(m_all, __shfl_xor_sync(0xffffffffu, m_all, d));
+            const float fw = ml.x == -INFINITY ? 0.f : ex2_sfu(ml.x - m_all);
+            float l_all = fw == 0.f ? 0.f : fw * ml.y;
 #pragma unroll
-            for (int d = 1; d < F8_WARPS; d *= 2) l_all += __shfl_xor_sync(0xffffffffu, l_all, d);
+            for (int d = 1; d < 16; d *= 2) l_all += __shfl_xor_sync(0xffffffffu, l_all, d);
             float2 acc = make_float2(0.f, 0.f);
 #pragma unroll
             for (int q = 0; q < F8_WARPS; ++q) {
-                const float fq = __shfl_sync(0xffffffffu, f, q);
+                const float fq = __shfl_sync(0xffffffffu, fw, q);
                 if (q < nkw && fq != 0.f) {
-                    const float2 x = *reinterpret_cast<const float2*>(&S.o[w0 + q * rgroups][rr][2 * lane]);
+                    const float2 x = *reinterpret_cast<const float2*>(&S.o[w0 + (q << gb)][rr][2 * lane]);
                     acc.x = fmaf(fq, x.x, acc.x);
                     acc.y = fmaf(fq, x.y, acc.y);
                 }
@@ -432,7 +488,13 @@ __global__ void __launch_bounds__(F8_THREADS, 1)
 
 template <class Act>
 cudaError_t launch_few8(const ChunkArgs& a, const Pool8& pool, cudaStream_t stream) {
-    constexpr size_t smem = sizeof(Few8Smem);
+    Few8Tma m;
+    const uint64_t heads = static_cast<uint64_t>(pool.n_pages) * a.n_head_kv, rows = uint64_t{1} << pool.page_shift;
+    cudaError_t me = make_tmap_3d_8b(&m.k, pool.key_codes, HD, rows, heads, kBox8);
+    if (me != cudaSuccess) return me;
+    me = make_tmap_3d_8b(&m.v, pool.value_codes, HD, rows, heads, kBox8);
+    if (me != cudaSuccess) return me;
+    constexpr size_t smem = sizeof(Few8Smem) + 1024;
     static_assert(smem <= 232448, "shared memory of one SM");
     static PerDeviceOnce once;
     cudaError_t e = once.run([&](int) {
@@ -440,7 +502,7 @@ cudaError_t launch_few8(const ChunkArgs& a, const Pool8& pool, cudaStream_t stre
     });
     if (e != cudaSuccess) return e;
     Launch L(dim3(a.n_few_ctas), F8_THREADS, smem, stream);
-    return cudaLaunchKernelEx(&L.cfg, chunk_few8_kernel<Act>, a, pool);
+    return cudaLaunchKernelEx(&L.cfg, chunk_few8_kernel<Act>, a, pool, m);
 }
 
 }  // namespace
