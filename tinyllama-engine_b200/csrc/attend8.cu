@@ -24,7 +24,7 @@ namespace tle {
 namespace {
 
 // Bound by the K/V bytes, 130 a row and KV head.  Tiles of codes come by TMA (a
-// box is 64 rows of a page, 64-byte swizzle), their scales by bulk copies, into a ring that
+// box is 64 or 128 rows of a page, 64-byte swizzle), their scales by bulk copies, into a ring that
 // a producer warp keeps full across segments; 16 warps take 16-key steps of the
 // tiles, each with its own running maximum, sum and output, joined in shared
 // memory at the segment's end.
@@ -55,9 +55,11 @@ constexpr int F8_STAGES = 8;
 constexpr int kSteps = kTile / 16; // of a tile
 constexpr int kArrivals = 4 * kSteps;   // of a stage: a step of each of 1, 2 or 4 row groups arrives for 4, 2 or 1
 constexpr int kFlush = 8;          // steps of a warp whose MMAs are summed in a row
-constexpr int kBox8 = 64;          // rows of a copy: the smallest page
 constexpr int kQBits = 12;         // the largest element of q in [2^12, 2^13)
 constexpr int kWeightBits = 15, kWeightStart = 6;
+
+// Rows of a copy: a tile, or two copies where a page is 64 rows.
+__host__ __device__ constexpr int box_of(int page_shift) { return page_shift >= 7 ? kTile : kTile / 2; }
 
 struct Few8Smem {
     uint8_t k[F8_STAGES][kTile * HD];
@@ -70,7 +72,7 @@ struct Few8Smem {
     Work work[kWorkCache];
 };
 struct Few8Tma {
-    CUtensorMap k, v;   // the layer's codes as [n_pages * n_head_kv][page rows][64], box {64, 64, 1}
+    CUtensorMap k, v;   // the layer's codes as [n_pages * n_head_kv][page rows][64], box {64, 64 or 128, 1}
 };
 
 __device__ __forceinline__ void mma_f16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
@@ -164,15 +166,17 @@ __global__ void __launch_bounds__(F8_THREADS, 1)
     };
     if (warp == F8_WARPS) {   // producer
         int ring = 0;
+        const int box_rows = box_of(P.page_shift);
         const uint64_t policy = l2_evict_first_policy();
         for (int sg = seg0; sg < seg1; ++sg) {
             const Work w = work_of(sg);
             // lane l has the page of box b0 + l: -1 behind the last row, -2 outside the pool
-            int b0 = 2 * w.t0, id = -1;
+            const int per_tile = kTile / box_rows;
+            int b0 = per_tile * w.t0, id = -1;
             auto refill = [&]() {
-                const int r = (b0 + lane) * kBox8;
+                const int r = (b0 + lane) * box_rows;
                 id = -1;
-                if (r < w.kv_len && b0 + lane < 2 * w.t1) {
+                if (r < w.kv_len && b0 + lane < per_tile * w.t1) {
                     id = w.pages[r >> P.page_shift];
                     if (static_cast<unsigned>(id) >= static_cast<unsigned>(P.n_pages)) {
                         record_error(A.err, kErrBadPage);
@@ -182,42 +186,40 @@ __global__ void __launch_bounds__(F8_THREADS, 1)
             };
             refill();
             for (int n = w.t0; n < w.t1; ++n, ++ring) {
-                if (2 * n - b0 >= 32) {
-                    b0 = 2 * n;
+                if (per_tile * n - b0 >= 32) {
+                    b0 = per_tile * n;
                     refill();
                 }
                 const int st = ring % F8_STAGES;
-                const int ids[2] = {__shfl_sync(0xffffffffu, id, 2 * n - b0), __shfl_sync(0xffffffffu, id, 2 * n - b0 + 1)};
+                const int id0 = __shfl_sync(0xffffffffu, id, per_tile * n - b0);
+                const int id1 = per_tile == 2 ? __shfl_sync(0xffffffffu, id, per_tile * n - b0 + 1) : -1;
                 wait_or_flag(&S.empty[st], ((ring / F8_STAGES) & 1) ^ 1, A.err, kErrWaitEmpty, failed);
                 failed = __any_sync(0xffffffffu, failed);
                 if (failed) break;
-                int boxes = 0;
-#pragma unroll
-                for (int b = 0; b < 2; ++b) {
-                    boxes += ids[b] >= 0;
-                    if (ids[b] != -2) continue;
-                    for (int i = lane; i < kBox8 * HD / 16; i += 32) {   // its rows count as zeros
-                        reinterpret_cast<uint4*>(S.k[st] + b * kBox8 * HD)[i] = make_uint4(0, 0, 0, 0);
-                        reinterpret_cast<uint4*>(S.v[st] + b * kBox8 * HD)[i] = make_uint4(0, 0, 0, 0);
+                for (int b = 0; b < per_tile; ++b) {
+                    if ((b ? id1 : id0) != -2) continue;
+                    for (int i = lane; i < box_rows * HD / 16; i += 32) {   // its rows count as zeros
+                        reinterpret_cast<uint4*>(S.k[st] + b * box_rows * HD)[i] = make_uint4(0, 0, 0, 0);
+                        reinterpret_cast<uint4*>(S.v[st] + b * box_rows * HD)[i] = make_uint4(0, 0, 0, 0);
                     }
-                    if (lane < kBox8 / 4) {
-                        reinterpret_cast<uint32_t*>(S.ks[st] + b * kBox8)[lane] = 0x7f7f7f7fu;
-                        reinterpret_cast<uint32_t*>(S.vs[st] + b * kBox8)[lane] = 0x7f7f7f7fu;
+                    if (lane < box_rows / 4) {
+                        reinterpret_cast<uint32_t*>(S.ks[st] + b * box_rows)[lane] = 0x7f7f7f7fu;
+                        reinterpret_cast<uint32_t*>(S.vs[st] + b * box_rows)[lane] = 0x7f7f7f7fu;
                     }
                     fence_proxy_async_smem();   // before the stage's next copy
                 }
                 __syncwarp();
                 if (lane == 0) {
-                    mbar_arrive_expect_tx(&S.full[st], boxes * 2 * (kBox8 * HD + kBox8));
-#pragma unroll
-                    for (int b = 0; b < 2; ++b) {
-                        if (ids[b] < 0) continue;
-                        const int z = ids[b] * A.n_head_kv + w.kvh, y = ((2 * n + b) * kBox8) & ((1 << P.page_shift) - 1);
+                    mbar_arrive_expect_tx(&S.full[st], ((id0 >= 0) + (id1 >= 0)) * 2 * box_rows * (HD + 1));
+                    for (int b = 0; b < per_tile; ++b) {
+                        const int page = b ? id1 : id0;
+                        if (page < 0) continue;
+                        const int z = page * A.n_head_kv + w.kvh, y = (n * kTile + b * box_rows) & ((1 << P.page_shift) - 1);
                         const size_t row = (static_cast<size_t>(z) << P.page_shift) + y;
-                        tma_load_3d(S.k[st] + b * kBox8 * HD, &M.k, 0, y, z, &S.full[st]);
-                        bulk_g2s(S.ks[st] + b * kBox8, P.key_scale + row, kBox8, &S.full[st], policy);
-                        tma_load_3d(S.v[st] + b * kBox8 * HD, &M.v, 0, y, z, &S.full[st]);
-                        bulk_g2s(S.vs[st] + b * kBox8, P.value_scale + row, kBox8, &S.full[st], policy);
+                        tma_load_3d(S.k[st] + b * box_rows * HD, &M.k, 0, y, z, &S.full[st]);
+                        bulk_g2s(S.ks[st] + b * box_rows, P.key_scale + row, box_rows, &S.full[st], policy);
+                        tma_load_3d(S.v[st] + b * box_rows * HD, &M.v, 0, y, z, &S.full[st]);
+                        bulk_g2s(S.vs[st] + b * box_rows, P.value_scale + row, box_rows, &S.full[st], policy);
                     }
                 }
                 __syncwarp();
@@ -490,9 +492,9 @@ template <class Act>
 cudaError_t launch_few8(const ChunkArgs& a, const Pool8& pool, cudaStream_t stream) {
     Few8Tma m;
     const uint64_t heads = static_cast<uint64_t>(pool.n_pages) * a.n_head_kv, rows = uint64_t{1} << pool.page_shift;
-    cudaError_t me = make_tmap_3d_8b(&m.k, pool.key_codes, HD, rows, heads, kBox8);
+    cudaError_t me = make_tmap_3d_8b(&m.k, pool.key_codes, HD, rows, heads, box_of(pool.page_shift));
     if (me != cudaSuccess) return me;
-    me = make_tmap_3d_8b(&m.v, pool.value_codes, HD, rows, heads, kBox8);
+    me = make_tmap_3d_8b(&m.v, pool.value_codes, HD, rows, heads, box_of(pool.page_shift));
     if (me != cudaSuccess) return me;
     constexpr size_t smem = sizeof(Few8Smem) + 1024;
     static_assert(smem <= 232448, "shared memory of one SM");
