@@ -24,7 +24,7 @@ namespace tle {
 namespace {
 
 // Bound by the K/V bytes, 130 a row and KV head.  Tiles of codes come by TMA (a
-// box is 64 or 128 rows of a page, 64-byte swizzle), their scales by bulk copies, into a ring that
+// box is 64 or 128 rows of a page, two rows a line, 128-byte swizzle), their scales by bulk copies, into a ring that
 // a producer warp keeps full across segments; 16 warps take 16-key steps of the
 // tiles, each with its own running maximum, sum and output, joined in shared
 // memory at the segment's end.
@@ -72,7 +72,7 @@ struct Few8Smem {
     Work work[kWorkCache];
 };
 struct Few8Tma {
-    CUtensorMap k, v;   // the layer's codes as [n_pages * n_head_kv][page rows][64], box {64, 64 or 128, 1}
+    CUtensorMap k, v;   // the layer's codes as [n_pages * n_head_kv][page rows / 2][128], box {128, 32 or 64, 1}
 };
 
 __device__ __forceinline__ void mma_f16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
@@ -216,9 +216,9 @@ __global__ void __launch_bounds__(F8_THREADS, 1)
                         if (page < 0) continue;
                         const int z = page * A.n_head_kv + w.kvh, y = (n * kTile + b * box_rows) & ((1 << P.page_shift) - 1);
                         const size_t row = (static_cast<size_t>(z) << P.page_shift) + y;
-                        tma_load_3d(S.k[st] + b * box_rows * HD, &M.k, 0, y, z, &S.full[st]);
+                        tma_load_3d(S.k[st] + b * box_rows * HD, &M.k, 0, y / 2, z, &S.full[st]);
                         bulk_g2s(S.ks[st] + b * box_rows, P.key_scale + row, box_rows, &S.full[st], policy);
-                        tma_load_3d(S.v[st] + b * box_rows * HD, &M.v, 0, y, z, &S.full[st]);
+                        tma_load_3d(S.v[st] + b * box_rows * HD, &M.v, 0, y / 2, z, &S.full[st]);
                         bulk_g2s(S.vs[st] + b * box_rows, P.value_scale + row, box_rows, &S.full[st], policy);
                     }
                 }
@@ -234,6 +234,14 @@ __global__ void __launch_bounds__(F8_THREADS, 1)
     }
     const int g = lane >> 2, t = lane & 3;        // fragment row, and which quarter of it
     const int mi = lane >> 3, li = lane & 7;      // ldmatrix: matrix and row of this lane's address
+    // Rows lie in pairs in lines of 128 bytes: chunk q of row r, 16 bytes, is 4 (r % 2) + q of line r / 2 and
+    // lies at that ^ (r / 2 % 8).  This lane's row of a step, chunks mi / 2 and mi / 2 + 2:
+    uint32_t piece[2];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        const int r = li + 8 * (mi & 1), line = r >> 1;
+        piece[h] = line * 2 * HD + ((((r & 1) * 4 + 2 * h + (mi >> 1)) ^ line) << 4);
+    }
     static_assert(kChunkFewRows <= 32 && F8_WARPS < 32, "four row groups at most");
     // row groups of 8 rows: 1, 2 or 4 (as a power of two), the warps dealt out to them
     auto group_bits = [](int n_rows) { return n_rows <= 8 ? 0 : n_rows <= 16 ? 1 : 2; };
@@ -336,13 +344,12 @@ __global__ void __launch_bounds__(F8_THREADS, 1)
             if (EDGE && key0 >= w.kv_len) return;
             if (++since > kFlush) flush();
             const uint32_t kb = smem_u32(S.k[st]), vb = smem_u32(S.v[st]);
-            // 16-byte chunk q of row r lies at q ^ (r / 2 % 4)
-            uint32_t kr[4][4];   // matrices: keys 0-7 and 8-15 of chunks 0, 1; then of 2, 3
+            // matrices: keys 0-7 and 8-15 of chunks 0, 1; then of 2, 3
+            uint32_t kr[4][4];
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-                const int r = j0 + li + 8 * (mi & 1), q = 2 * h + (mi >> 1);
-                ldsm4_b(kb + r * HD + ((q ^ ((r >> 1) & 3)) << 4), kr[h]);
-                ldsm4_bt(vb + r * HD + ((q ^ ((r >> 1) & 3)) << 4), kr[2 + h]);
+                ldsm4_b(kb + j0 * HD + piece[h], kr[h]);
+                ldsm4_bt(vb + j0 * HD + piece[h], kr[2 + h]);
             }
             uint32_t ks2[2], vs2[2];   // the scales of keys 2 t, 2 t + 1 of either 8
 #pragma unroll
@@ -492,9 +499,9 @@ template <class Act>
 cudaError_t launch_few8(const ChunkArgs& a, const Pool8& pool, cudaStream_t stream) {
     Few8Tma m;
     const uint64_t heads = static_cast<uint64_t>(pool.n_pages) * a.n_head_kv, rows = uint64_t{1} << pool.page_shift;
-    cudaError_t me = make_tmap_3d_8b(&m.k, pool.key_codes, HD, rows, heads, box_of(pool.page_shift));
+    cudaError_t me = make_tmap_3d_8b(&m.k, pool.key_codes, rows / 2, heads, box_of(pool.page_shift) / 2);
     if (me != cudaSuccess) return me;
-    me = make_tmap_3d_8b(&m.v, pool.value_codes, HD, rows, heads, box_of(pool.page_shift));
+    me = make_tmap_3d_8b(&m.v, pool.value_codes, rows / 2, heads, box_of(pool.page_shift) / 2);
     if (me != cudaSuccess) return me;
     constexpr size_t smem = sizeof(Few8Smem) + 1024;
     static_assert(smem <= 232448, "shared memory of one SM");

@@ -727,7 +727,8 @@ cudaError_t make_tmap_16b(CUtensorMap* m, void* base, uint64_t cols, uint64_t ro
     return make_map(m, base, cols, rows, box_rows, dtype);
 }
 
-cudaError_t make_tmap_3d_8b(CUtensorMap* m, const void* base, uint64_t cols, uint64_t rows, uint64_t blocks, uint32_t box_rows) {
+cudaError_t make_tmap_3d_8b(CUtensorMap* m, const void* base, uint64_t rows, uint64_t blocks, uint32_t box_rows) {
+    constexpr cuuint64_t cols = 128;
     EncodeTiledFn enc = nullptr;
     cudaError_t e = get_encoder(&enc);
     if (e != cudaSuccess) return e;
@@ -736,7 +737,7 @@ cudaError_t make_tmap_3d_8b(CUtensorMap* m, const void* base, uint64_t cols, uin
     const cuuint32_t box[3] = {static_cast<cuuint32_t>(cols), box_rows, 1};
     const cuuint32_t estr[3] = {1, 1, 1};
     CUresult r = enc(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, const_cast<void*>(base), dims, strides, box, estr,
-                     CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_64B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B,
+                     CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B,
                      CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     return r == CUDA_SUCCESS ? cudaSuccess : cudaErrorInvalidValue;
 }

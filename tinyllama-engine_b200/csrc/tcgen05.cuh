@@ -189,8 +189,8 @@ TLE_DEV void prefetch_tmap(const CUtensorMap* map) {
 // K-major SW128 layout), no out-of-bounds fill needed by the callers.
 cudaError_t make_tmap_16b(CUtensorMap* m, void* base, uint64_t cols, uint64_t rows, uint32_t box_rows,
                           CUtensorMapDataType dtype);
-// Host: 3-D tensor map over [blocks][rows][cols] bytes with cols = 64, box
-// {64, box_rows, 1}, 64-byte swizzle.
-cudaError_t make_tmap_3d_8b(CUtensorMap* m, const void* base, uint64_t cols, uint64_t rows, uint64_t blocks, uint32_t box_rows);
+// Host: 3-D tensor map over [blocks][rows][128] bytes, box {128, box_rows, 1},
+// 128-byte swizzle.
+cudaError_t make_tmap_3d_8b(CUtensorMap* m, const void* base, uint64_t rows, uint64_t blocks, uint32_t box_rows);
 
 }  // namespace tle
