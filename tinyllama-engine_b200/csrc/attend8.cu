@@ -25,7 +25,7 @@ namespace {
 
 // Bound by the K/V bytes, 130 a row and KV head.  Tiles of codes come by TMA (a
 // box is 64 or 128 rows of a page, two rows a line, 128-byte swizzle), their scales by bulk copies, into a ring that
-// a producer warp keeps full across segments; 16 warps take 16-key steps of the
+// a producer warp keeps full across segments; 15 warps take 32-key steps of the
 // tiles, each with its own running maximum, sum and output, joined in shared
 // memory at the segment's end.
 //
@@ -52,9 +52,10 @@ namespace {
 constexpr int F8_WARPS = 15;      // and the producer: 16 warps, so that a thread may have 128 registers
 constexpr int F8_THREADS = 32 * (F8_WARPS + 1);
 constexpr int F8_STAGES = 8;
-constexpr int kSteps = kTile / 16; // of a tile
+constexpr int kStep = 32;           // keys of a step
+constexpr int kSteps = kTile / kStep;
 constexpr int kArrivals = 4 * kSteps;   // of a stage: a step of each of 1, 2 or 4 row groups arrives for 4, 2 or 1
-constexpr int kFlush = 8;          // steps of a warp whose MMAs are summed in a row
+constexpr int kFlush = 4;          // steps of a warp whose MMAs are summed in a row
 constexpr int kQBits = 12;         // the largest element of q in [2^12, 2^13)
 constexpr int kWeightBits = 15, kWeightStart = 6;
 
@@ -122,10 +123,10 @@ __device__ __forceinline__ void two_terms(float lo, float hi, uint32_t& t0, uint
     const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&t0));
     t1 = pack_f16(lo - f.x, hi - f.y);
 }
-// The codes in bytes 0 and 2 of u as fp16 numbers.
+// The codes in bytes 0 and 2 of u as fp16 numbers: (u & 00ff00ff) ^ 64806480 is 1024 + (code + 128).
 __device__ __forceinline__ uint32_t codes_f16(uint32_t u) {
-    const uint32_t h = (u & 0x00ff00ffu) ^ 0x64806480u;   // 1024 + (code + 128)
-    uint32_t r;
+    uint32_t h, r;
+    asm("lop3.b32 %0, %1, %2, %3, 0x6a;" : "=r"(h) : "r"(u), "r"(0x00ff00ffu), "r"(0x64806480u));
     asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(h), "r"(0x64806480u));   // - 1152
     return r;
 }
@@ -338,46 +339,49 @@ __global__ void __launch_bounds__(F8_THREADS, 1)
                     held(i) = make_float4(z.x * by, z.y * by, z.z * by, z.w * by);
                 }
         };
-        // 16 keys from j0 of tile n in stage st; EDGE: some row does not attend to all of the tile.
+        // kStep keys from j0 of tile n in stage st; EDGE: some row does not attend to all of the tile.
         auto step = [&]<bool EDGE>(int st, int n, int j0) {
+            constexpr int B = kStep / 8, N = kStep / 4;   // blocks of 8 keys; keys of a lane: 2 t, 2 t + 1 of each
             const int key0 = n * kTile + j0;
             if (EDGE && key0 >= w.kv_len) return;
             if (++since > kFlush) flush();
-            const uint32_t kb = smem_u32(S.k[st]), vb = smem_u32(S.v[st]);
-            // matrices: keys 0-7 and 8-15 of chunks 0, 1; then of 2, 3
-            uint32_t kr[4][4];
+            const uint32_t kb = smem_u32(S.k[st]) + j0 * HD, vb = smem_u32(S.v[st]) + j0 * HD;
+            float sf[B][4];
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                ldsm4_b(kb + j0 * HD + piece[h], kr[h]);
-                ldsm4_bt(vb + j0 * HD + piece[h], kr[2 + h]);
+            for (int b2 = 0; b2 < B / 2; ++b2) {
+                // matrices: keys 0-7 and 8-15 of chunks 0, 1; then of 2, 3
+                uint32_t kr[2][4];
+#pragma unroll
+                for (int h = 0; h < 2; ++h) ldsm4_b(kb + 16 * b2 * HD + piece[h], kr[h]);
+#pragma unroll
+                for (int ks = 0; ks < HD / 16; ++ks)
+#pragma unroll
+                    for (int b = 0; b < 2; ++b) {
+                        const uint32_t u = kr[ks >> 1][2 * (ks & 1) + b];
+                        if (ks == 0) mma_f16_zero(sf[2 * b2 + b], qf[ks], codes_f16(u), codes_f16(u >> 8));
+                        else mma_f16(sf[2 * b2 + b], qf[ks], codes_f16(u), codes_f16(u >> 8));
+                    }
             }
-            uint32_t ks2[2], vs2[2];   // the scales of keys 2 t, 2 t + 1 of either 8
+            float s[N], vsf[N];
 #pragma unroll
-            for (int b = 0; b < 2; ++b) {
-                ks2[b] = *reinterpret_cast<const uint16_t*>(&S.ks[st][j0 + 8 * b + 2 * t]);
-                vs2[b] = *reinterpret_cast<const uint16_t*>(&S.vs[st][j0 + 8 * b + 2 * t]);
-            }
-            float sf[2][4];
+            for (int b = 0; b < B; ++b) {
+                const uint32_t kx = *reinterpret_cast<const uint16_t*>(&S.ks[st][j0 + 8 * b + 2 * t]);
+                const uint32_t vx = *reinterpret_cast<const uint16_t*>(&S.vs[st][j0 + 8 * b + 2 * t]);
 #pragma unroll
-            for (int ks = 0; ks < HD / 16; ++ks)
-#pragma unroll
-                for (int b = 0; b < 2; ++b) {
-                    const uint32_t u = kr[ks >> 1][2 * (ks & 1) + b];
-                    if (ks == 0) mma_f16_zero(sf[b], qf[ks], codes_f16(u), codes_f16(u >> 8));
-                    else mma_f16(sf[b], qf[ks], codes_f16(u), codes_f16(u >> 8));
+                for (int e = 0; e < 2; ++e) {
+                    const int i = 2 * b + e;
+                    s[i] = (sf[b][e] + sf[b][2 + e]) * (__uint_as_float((e ? kx << 15 : kx << 23) & 0x7f800000u) * c);
+                    vsf[i] = __uint_as_float((e ? vx << 15 : vx << 23) & 0x7f800000u);
+                    if (EDGE && key0 + 8 * b + 2 * t + e > pos_r) {
+                        s[i] = -INFINITY;
+                        vsf[i] = 0.f;
+                    }
                 }
-            float s[4], vsf[4];   // keys 2 t, 2 t + 1, 2 t + 8, 2 t + 9
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const uint32_t kx = ks2[i >> 1], vx = vs2[i >> 1];
-                s[i] = (sf[i >> 1][i & 1] + sf[i >> 1][2 + (i & 1)]) * (__uint_as_float((i & 1 ? kx << 15 : kx << 23) & 0x7f800000u) * c);
-                vsf[i] = __uint_as_float((i & 1 ? vx << 15 : vx << 23) & 0x7f800000u);
-                if (EDGE && key0 + 8 * (i >> 1) + 2 * t + (i & 1) > pos_r) {
-                    s[i] = -INFINITY;
-                    vsf[i] = 0.f;
-                }
             }
-            const float mt = fmax3(fmax3(s[0], s[1], s[2]), s[3], s[3]);
+            float mt = s[0];
+#pragma unroll
+            for (int i = 1; i + 1 < N; i += 2) mt = fmax3(mt, s[i], s[i + 1]);
+            mt = fmax3(mt, s[N - 1], s[N - 1]);
             if (__any_sync(0xffffffffu, m == m && !(mt <= m + kMoveThreshold))) {
                 float to = fmax3(mt, __shfl_xor_sync(0xffffffffu, mt, 1), -INFINITY);
                 to = fmax3(to, __shfl_xor_sync(0xffffffffu, to, 2), -INFINITY);
@@ -398,14 +402,17 @@ __global__ void __launch_bounds__(F8_THREADS, 1)
                 if (__any_sync(0xffffffffu, by != 1.f)) scale_o(by);
             }
             const float m_use = m == -INFINITY ? 0.f : m;   // nothing attended so far: the scores are -inf
-            float wt[4];
+            float wt[N];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
+            for (int i = 0; i < N; ++i) {
                 const float p = ex2_sfu(s[i] - m_use);
                 l += p;
                 wt[i] = p * vsf[i];
             }
-            const float wm = fmax3(fmax3(wt[0], wt[1], wt[2]), wt[3], wt[3]);
+            float wm = wt[0];
+#pragma unroll
+            for (int i = 1; i + 1 < N; i += 2) wm = fmax3(wm, wt[i], wt[i + 1]);
+            wm = fmax3(wm, wt[N - 1], wt[N - 1]);
             if (__any_sync(0xffffffffu, !(wm <= limit))) {
                 float to = fmax3(wm, __shfl_xor_sync(0xffffffffu, wm, 1), 0.f);
                 to = fmax3(to, __shfl_xor_sync(0xffffffffu, to, 2), 0.f);
@@ -419,14 +426,19 @@ __global__ void __launch_bounds__(F8_THREADS, 1)
                 }
                 scale_o(by);
             }
-            uint32_t pf[4];
-            two_terms(wt[0] * f, wt[1] * f, pf[0], pf[1]);
-            two_terms(wt[2] * f, wt[3] * f, pf[2], pf[3]);
 #pragma unroll
-            for (int q = 0; q < HD / 16; ++q) {   // chunk q: dimensions 16 q + 2 g (+1)
-                const uint32_t u0 = kr[2 + (q >> 1)][2 * (q & 1)], u1 = kr[2 + (q >> 1)][2 * (q & 1) + 1];
-                mma_f16(o[2 * q], pf, codes_f16(u0), codes_f16(u1));
-                mma_f16(o[2 * q + 1], pf, codes_f16(u0 >> 8), codes_f16(u1 >> 8));
+            for (int b2 = 0; b2 < B / 2; ++b2) {
+                uint32_t vr[2][4], pf[4];
+#pragma unroll
+                for (int h = 0; h < 2; ++h) ldsm4_bt(vb + 16 * b2 * HD + piece[h], vr[h]);
+                two_terms(wt[4 * b2] * f, wt[4 * b2 + 1] * f, pf[0], pf[1]);
+                two_terms(wt[4 * b2 + 2] * f, wt[4 * b2 + 3] * f, pf[2], pf[3]);
+#pragma unroll
+                for (int q = 0; q < HD / 16; ++q) {   // chunk q: dimensions 16 q + 2 g (+1)
+                    const uint32_t u0 = vr[q >> 1][2 * (q & 1)], u1 = vr[q >> 1][2 * (q & 1) + 1];
+                    mma_f16(o[2 * q], pf, codes_f16(u0), codes_f16(u1));
+                    mma_f16(o[2 * q + 1], pf, codes_f16(u0 >> 8), codes_f16(u1 >> 8));
+                }
             }
         };
         // the steps of the segment, dealt out to the group's warps
@@ -435,8 +447,8 @@ __global__ void __launch_bounds__(F8_THREADS, 1)
             const int n = w.t0 + i / kSteps, ring = ring0 + i / kSteps, st = ring % F8_STAGES;
             wait_or_flag(&S.full[st], (ring / F8_STAGES) & 1, A.err, kErrWaitFull, failed);
             __syncwarp();
-            if (w.edge(n)) step.template operator()<true>(st, n, 16 * (i % kSteps));
-            else step.template operator()<false>(st, n, 16 * (i % kSteps));
+            if (w.edge(n)) step.template operator()<true>(st, n, kStep * (i % kSteps));
+            else step.template operator()<false>(st, n, kStep * (i % kSteps));
             __syncwarp();
             if (lane == 0) mbar_arrive_n(&S.empty[st], kArrivals / kSteps >> gb);
         }
