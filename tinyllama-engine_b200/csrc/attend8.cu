@@ -51,7 +51,8 @@ namespace {
 // kMoveThreshold, f when a weight would be above 2^15.
 constexpr int F8_WARPS = 15;      // and the producer: 16 warps, so that a thread may have 128 registers
 constexpr int F8_THREADS = 32 * (F8_WARPS + 1);
-constexpr int F8_STAGES = 8;
+constexpr int F8_STAGES = 11;
+constexpr int kBatch = 3;          // tiles whose copies are issued at once
 constexpr int kStep = 32;           // keys of a step
 constexpr int kSteps = kTile / kStep;
 constexpr int kArrivals = 4 * kSteps;   // of a stage: a step of each of 1, 2 or 4 row groups arrives for 4, 2 or 1
@@ -186,31 +187,37 @@ __global__ void __launch_bounds__(F8_THREADS, 1)
                 }
             };
             refill();
-            for (int n = w.t0; n < w.t1; ++n, ++ring) {
-                if (per_tile * n - b0 >= 32) {
-                    b0 = per_tile * n;
+            // up to kBatch tiles at once, one a lane: a turn of this loop takes about as long as the tiles' copies do
+            for (int n0 = w.t0; n0 < w.t1; n0 += kBatch) {
+                const int count = min(kBatch, w.t1 - n0);
+                if (per_tile * (n0 + count) - b0 > 32) {
+                    b0 = per_tile * n0;
                     refill();
                 }
-                const int st = ring % F8_STAGES;
+                const int n = n0 + min(lane, count - 1), mine = ring + n - n0, st = mine % F8_STAGES;
                 const int id0 = __shfl_sync(0xffffffffu, id, per_tile * n - b0);
                 const int id1 = per_tile == 2 ? __shfl_sync(0xffffffffu, id, per_tile * n - b0 + 1) : -1;
-                wait_or_flag(&S.empty[st], ((ring / F8_STAGES) & 1) ^ 1, A.err, kErrWaitEmpty, failed);
+                wait_or_flag(&S.empty[st], ((mine / F8_STAGES) & 1) ^ 1, A.err, kErrWaitEmpty, failed);
                 failed = __any_sync(0xffffffffu, failed);
                 if (failed) break;
-                for (int b = 0; b < per_tile; ++b) {
-                    if ((b ? id1 : id0) != -2) continue;
-                    for (int i = lane; i < box_rows * HD / 16; i += 32) {   // its rows count as zeros
-                        reinterpret_cast<uint4*>(S.k[st] + b * box_rows * HD)[i] = make_uint4(0, 0, 0, 0);
-                        reinterpret_cast<uint4*>(S.v[st] + b * box_rows * HD)[i] = make_uint4(0, 0, 0, 0);
-                    }
-                    if (lane < box_rows / 4) {
-                        reinterpret_cast<uint32_t*>(S.ks[st] + b * box_rows)[lane] = 0x7f7f7f7fu;
-                        reinterpret_cast<uint32_t*>(S.vs[st] + b * box_rows)[lane] = 0x7f7f7f7fu;
+                ring += count;
+                if (__any_sync(0xffffffffu, id0 == -2 || id1 == -2)) {
+                    for (int e = 0; e < count * per_tile; ++e) {
+                        const int to = __shfl_sync(0xffffffffu, st, e / per_tile), b = e % per_tile;
+                        if (__shfl_sync(0xffffffffu, b ? id1 : id0, e / per_tile) != -2) continue;
+                        for (int i = lane; i < box_rows * HD / 16; i += 32) {   // its rows count as zeros
+                            reinterpret_cast<uint4*>(S.k[to] + b * box_rows * HD)[i] = make_uint4(0, 0, 0, 0);
+                            reinterpret_cast<uint4*>(S.v[to] + b * box_rows * HD)[i] = make_uint4(0, 0, 0, 0);
+                        }
+                        if (lane < box_rows / 4) {
+                            reinterpret_cast<uint32_t*>(S.ks[to] + b * box_rows)[lane] = 0x7f7f7f7fu;
+                            reinterpret_cast<uint32_t*>(S.vs[to] + b * box_rows)[lane] = 0x7f7f7f7fu;
+                        }
                     }
                     fence_proxy_async_smem();   // before the stage's next copy
                 }
                 __syncwarp();
-                if (lane == 0) {
+                if (lane < count) {
                     mbar_arrive_expect_tx(&S.full[st], ((id0 >= 0) + (id1 >= 0)) * 2 * box_rows * (HD + 1));
                     for (int b = 0; b < per_tile; ++b) {
                         const int page = b ? id1 : id0;
@@ -262,6 +269,8 @@ __global__ void __launch_bounds__(F8_THREADS, 1)
     };
     int ring0 = 0;   // tiles of the segments before
     auto segment = [&](const Work& w) {
+        // w may lie in either memory: what the steps need of it is held in registers
+        const int t0 = w.t0, pos_min = w.pos_min, kv_len = w.kv_len;
         const int gb = group_bits(w.n_rows), rg = warp & ((1 << gb) - 1), kw = warp >> gb;
         const int pos_r = w.pos + row_token(A, w.row0 + min(rg * 8 + g, w.n_rows - 1));
         uint32_t qf[HD / 16][4];   // A fragments: rows g the first terms, rows g + 8 the second
@@ -343,7 +352,7 @@ __global__ void __launch_bounds__(F8_THREADS, 1)
         auto step = [&]<bool EDGE>(int st, int n, int j0) {
             constexpr int B = kStep / 8, N = kStep / 4;   // blocks of 8 keys; keys of a lane: 2 t, 2 t + 1 of each
             const int key0 = n * kTile + j0;
-            if (EDGE && key0 >= w.kv_len) return;
+            if (EDGE && key0 >= kv_len) return;
             if (++since > kFlush) flush();
             const uint32_t kb = smem_u32(S.k[st]) + j0 * HD, vb = smem_u32(S.v[st]) + j0 * HD;
             float sf[B][4];
@@ -442,12 +451,12 @@ __global__ void __launch_bounds__(F8_THREADS, 1)
             }
         };
         // the steps of the segment, dealt out to the group's warps
-        const int n_steps = (w.t1 - w.t0) * kSteps, nkw = workers(gb, rg);
+        const int n_steps = (w.t1 - t0) * kSteps, nkw = workers(gb, rg);
         for (int i = kw; i < n_steps; i += nkw) {
-            const int n = w.t0 + i / kSteps, ring = ring0 + i / kSteps, st = ring % F8_STAGES;
+            const int n = t0 + i / kSteps, ring = ring0 + i / kSteps, st = ring % F8_STAGES;
             wait_or_flag(&S.full[st], (ring / F8_STAGES) & 1, A.err, kErrWaitFull, failed);
             __syncwarp();
-            if (w.edge(n)) step.template operator()<true>(st, n, kStep * (i % kSteps));
+            if (n * kTile + kTile - 1 > pos_min) step.template operator()<true>(st, n, kStep * (i % kSteps));
             else step.template operator()<false>(st, n, kStep * (i % kSteps));
             __syncwarp();
             if (lane == 0) mbar_arrive_n(&S.empty[st], kArrivals / kSteps >> gb);
