@@ -139,7 +139,7 @@ typedef struct {
  * Weights are whole numbers of 2^-40 of the largest: the choice does not depend
  * on the launch, and a token below 2^-41 of the likeliest is never drawn.  NaN
  * logits count as -inf; of +inf logits each weighs 1 and all others nothing.  A row of -inf
- * only gets the token -1.  n_vocab <= 393216; 4-byte aligned pointers. */
+ * only gets the token -1.  n_vocab <= 262144; 4-byte aligned pointers. */
 int tle_sample_rows(int32_t* tokens, const float* logits, int64_t logits_stride, int n_rows, int n_vocab,
                     const tle_sample_rules_t* rules, const float* uniform, void* stream);
 

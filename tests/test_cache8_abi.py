@@ -127,4 +127,4 @@ def test_sampling_refuses_bad_arguments():
     assert go(out=P + 2) == BAD and go(x=P + 1) == BAD and go(u=P + 2) == BAD
     for name in ("temperature", "top_k", "top_p", "min_p"):
         assert go(**{name: P + 2}) == BAD
-    assert go(V=393217, xs=393217) == tle.TLE_ERR_UNSUPPORTED
+    assert go(V=262145, xs=262145) == tle.TLE_ERR_UNSUPPORTED

@@ -536,7 +536,7 @@ struct LogitArgs {
 };
 cudaError_t launch_logits_adjust(const LogitArgs& a, int n_rows, cudaStream_t stream);
 // Sampling of rows (sample.cu).  A cluster of up to 8 CTAs holds a row.
-constexpr int kSampleSlice = 49152;                   // logits that a CTA has room for
+constexpr int kSampleSlice = 32768;                   // logits that a CTA has room for
 constexpr int kSampleRowsVocab = 8 * kSampleSlice;
 struct SampleRowsArgs {
     const float* logits;
@@ -548,7 +548,7 @@ struct SampleRowsArgs {
     const float* min_p;
     const float* uniform;        // [n_rows]
     int32_t* tokens;             // [n_rows]
-    int slice, per_thread;       // (set by launch_sample_rows) logits of a CTA and of a thread
+    int slice;                   // (set by launch_sample_rows) logits of a CTA
 };
 cudaError_t launch_sample_rows(SampleRowsArgs a, int n_rows, cudaStream_t stream);
 

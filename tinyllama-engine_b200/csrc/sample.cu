@@ -46,10 +46,11 @@ constexpr int kBins = 2048;                // of a level of a search; in kGroups
 constexpr int kGroups = kBins / 32;
 constexpr int kRowCtas = 8;
 constexpr int kList = kThreads;            // tokens of a bin that are ranked one by one
+constexpr uint64_t kFew = 128;             // so many tokens in all are ranked without bins
 constexpr uint64_t kOne = 1ull << 40;      // the largest weight
 constexpr float kReach = 28.6f;            // exp(-kReach) < 2^-41: weights beyond it are 0
 // A weight in three limbs of 14, 13 and 13 bits, so that a bin's sums of 32 bits
-// hold any slice (2^15.6 tokens).
+// hold any slice (2^15 tokens).
 constexpr uint32_t kLimb0 = 14, kLimb1 = 13;
 static_assert(kGroups * kRowCtas == kThreads && kBins == 4 * kThreads, "a group of a CTA, and 4 bins, per thread");
 
@@ -103,12 +104,16 @@ struct alignas(16) Shared {                // the slice lies behind it
             uint32_t key[kList];
         };
     };
-    uint64_t group[kRowCtas][kGroups];     // sums of 32 bins, of each CTA of the cluster
-    uint32_t fine[3 * kRowCtas][32];       // the bins of one group
-    uint32_t list[kList];                  // this CTA's keys of the bin in question
-    uint32_t count[kRowCtas], mine;        // how many each has; and this one
+    union {
+        uint64_t group[kRowCtas][kGroups]; // sums of 32 bins, of each CTA of the cluster
+        uint32_t fine[3 * kRowCtas][32];   // then the bins of one group
+    };
+    uint32_t list[2][kList];               // of two searches in turn: this CTA's keys of the bin in question
+    uint32_t count[2][kRowCtas];           // how many each CTA has
+    uint32_t mine;
     uint64_t slot[2][3][kRowCtas];         // what the CTAs of the cluster told each other, by turns
     uint64_t warp_sum[kWarps];
+    uint32_t warp_ties[kWarps];
     uint64_t found;
     uint32_t found_key;
     float warp_max[kWarps];
@@ -147,23 +152,6 @@ __device__ __forceinline__ uint64_t warp_scan(uint64_t x) {
     }
     return x;
 }
-// Inclusive scan over the block; returns the thread's sum, total the block's.
-__device__ __forceinline__ uint64_t block_scan(Shared& S, uint64_t x, uint64_t& total) {
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    x = warp_scan(x);
-    __syncthreads();
-    if (lane == 31) S.warp_sum[warp] = x;
-    __syncthreads();
-    uint64_t before = 0, all = 0;
-#pragma unroll
-    for (int w = 0; w < kWarps; ++w) {
-        if (w < warp) before += S.warp_sum[w];
-        all += S.warp_sum[w];
-    }
-    total = all;
-    return x + before;
-}
-
 // A cut of the ranking: the tokens with a key above `key`, and the first `ties` of those with it.
 struct Cut {
     uint32_t key;
@@ -187,8 +175,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
     float* xs = reinterpret_cast<float*>(smem_raw + sizeof(Shared)) + ((4 - head) & 3);              // aligned as the row is
     float mx = -INFINITY;
     auto take = [&](float x) {
-        x = x + 0.0f;                          // -0 is 0
-        x = x == x ? x : -INFINITY;
+        x = fmaxf(x + 0.0f, -INFINITY);        // -0 is 0, NaN -inf
         mx = fmaxf(mx, x);
         return x;
     };
@@ -228,15 +215,18 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
         const auto s = cl.tell(tid == 0, __float_as_uint(mx));
         for (int i = 0; i < cl.n; ++i) mx = fmaxf(mx, __uint_as_float(static_cast<uint32_t>(s[0][i])));
     }
-    const int L = A.per_thread, i0 = min(n, tid * L), i1 = min(n, i0 + L);   // this thread's tokens
     if (mx == -INFINITY) {                     // the same in all CTAs
         if (cl.rank == 0 && tid == 0) A.tokens[row] = -1;
         return;
     }
+    // a part of the slice for each warp, in order; `have` of its tokens are left in x and id
+    const int part = (A.slice + kWarps - 1) / kWarps, p0 = min(n, warp * part);
+    int have = min(n - p0, part);
+    float* x_of = xs + p0;
     if (!(T > 0.f)) {                          // the first of the largest
         int at = INT32_MAX;
-        for (int i = i1 - 1; i >= i0; --i)
-            if (xs[i] == mx) at = v0 + i;
+        for (int i = lane; i < have; i += 32)
+            if (x_of[i] == mx) at = min(at, v0 + p0 + i);
         at = __reduce_min_sync(0xffffffffu, at);
         if (lane == 0) S.warp_sum[warp] = at;
         __syncthreads();
@@ -251,11 +241,47 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
     R.inv_t = 1.0 / static_cast<double>(T);
     R.least = static_cast<double>(min_p) * static_cast<double>(kOne);
     R.reach = (min_p > 0.f ? fminf(kReach, -logf(min_p) + 0.01f) : kReach) * T;
-    // The cut at which the ranking's count (WEIGHT: sum of weights) of the tokens with a
-    // key above `from` first reaches want(its sum over all of them), among the tokens within reach: the others weigh
-    // nothing.  A want of 0, or of more than there is: no cut.  `left`: what is to be reached among the ties.
+    // ---- what is left of the warp's tokens, in place and in order ----
+    uint16_t* id_of = reinterpret_cast<uint16_t*>(smem_raw + sizeof(Shared) + 16 + A.slice * sizeof(float)) + p0;
+    auto keep = [&]<bool FIRST>(auto&& stays) {
+        int out = 0;
+        for (int i = 0; i < have; i += 32) {
+            const bool in = i + lane < have;
+            const float x = in ? x_of[i + lane] : 0.f;
+            const int id = FIRST ? i + lane : in ? id_of[i + lane] : 0;
+            const bool stay = in && stays(x);
+            const uint32_t set = __ballot_sync(0xffffffffu, stay);
+            if (stay) {
+                const int to = out + __popc(set & ((1u << lane) - 1));
+                x_of[to] = x;
+                id_of[to] = static_cast<uint16_t>(id);
+            }
+            out += __popc(set);
+            __syncwarp();
+        }
+        have = out;
+    };
+    // the tokens left in all CTAs; a barrier of the cluster
+    auto count_left = [&]() {
+        __syncthreads();
+        if (lane == 0) S.warp_sum[warp] = have;
+        __syncthreads();
+        uint64_t sum = 0;
+        for (int w = 0; w < kWarps; ++w) sum += S.warp_sum[w];
+        const auto s = cl.tell(tid == 0, sum);
+        uint64_t all = 0;
+        for (int i = 0; i < cl.n; ++i) all += s[0][i];
+        return all;
+    };
+    keep.template operator()<true>([&](float x) { return x == mx || mx - x < R.reach; });   // the others weigh nothing
+    uint64_t left = count_left();
+    int searches = 0;
+    // The cut at which the ranking's count (WEIGHT: sum of weights) of the tokens left with a key above `from` first
+    // reaches want_of(its sum over all of them).  A want of 0, or of more than there is: no cut.  Cut::ties is then
+    // what is to be reached among the tokens of Cut::key.  Tokens below the cut may be dropped.
     auto search = [&]<bool WEIGHT>(uint32_t from, auto&& want_of, Cut& cut) -> bool {
         constexpr int kLimbs = WEIGHT ? 3 : 1;
+        const int turn = searches++ & 1;
         uint32_t lo = from + 1, hi = key_of(mx);   // the keys in question
         const float per = R.reach > 0.f ? kBins / R.reach : 0.f;
         uint64_t want = 0;
@@ -266,16 +292,80 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
             const float d = (mx - x) * per;
             return d < kBins ? static_cast<int>(d) : x == mx ? 0 : kBins - 1;
         };
+        auto in = [&](uint32_t key) { return key >= lo && key <= hi; };
+        // this CTA's keys to list one by one: to all CTAs' knowledge, then those of all with their weights
+        // in S.key and S.weight; returns how many there are (more than kList: no list)
+        auto gather = [&]() {
+            __syncthreads();
+            if (tid < cl.n) *cl.g.map_shared_rank(&S.count[turn][cl.rank], tid) = S.mine;
+            cl.g.sync();
+            const uint32_t me = tid;
+            uint32_t all = 0, key = 0;
+            for (int c = 0; c < cl.n; ++c) {
+                const uint32_t m = S.count[turn][c];
+                if (me >= all && me - all < min(m, static_cast<uint32_t>(kList))) key = *cl.g.map_shared_rank(&S.list[turn][me - all], c);
+                all += m;
+            }
+            if (all <= kList) {
+                S.key[tid] = key;
+                S.weight[tid] = me >= all ? 0 : WEIGHT ? R.weight(of_key(key)) : 1;
+            }
+            __syncthreads();
+            return all;
+        };
+        // the listed key at which `want` is reached, by as many threads a key as there are
+        auto rank = [&](uint32_t all) {
+            const int bits = all <= 32 ? 4 : all <= 64 ? 3 : all <= 128 ? 2 : all <= 256 ? 1 : 0;
+            const uint32_t me = tid >> bits, key = me < all ? S.key[me] : 0;
+            uint64_t above = 0, with = 0;
+            for (uint32_t q = tid & ((1 << bits) - 1); q < all; q += 1 << bits) {
+                const uint32_t kq = S.key[q];
+                const uint64_t w = S.weight[q];
+                above += kq > key ? w : 0;
+                with += kq >= key ? w : 0;
+            }
+            for (int d = 1; d < 1 << bits; d *= 2) {
+                above += __shfl_xor_sync(0xffffffffu, above, d);
+                with += __shfl_xor_sync(0xffffffffu, with, d);
+            }
+            if (me < all && above < want && with >= want) {   // tokens of one key: they write the same
+                S.found = want - above;
+                S.found_key = key;
+            }
+            __syncthreads();
+            cut = Cut{S.found_key, S.found};
+        };
+        auto list_key = [&](uint32_t key) {
+            const uint32_t to = atomicAdd(&S.mine, 1u);
+            if (to < kList) S.list[turn][to] = key;
+        };
+        if (left <= kFew) {
+            __syncthreads();
+            if (tid == 0) S.mine = 0;
+            __syncthreads();
+            for (int i = lane; i < have; i += 32) {
+                const uint32_t key = key_of(x_of[i]);
+                if (in(key)) list_key(key);
+            }
+            const uint32_t all = gather();
+            uint64_t sum = 0;
+            for (uint32_t q = lane; q < all; q += 32) sum += S.weight[q];
+            for (int d = 1; d < 32; d *= 2) sum += __shfl_xor_sync(0xffffffffu, sum, d);
+            want = want_of(sum);
+            if (want == 0 || want > sum) return false;
+            rank(all);
+            return true;
+        }
         for (int level = 0;; ++level) {
-            auto in = [&](float x, uint32_t key) { return key >= lo && key <= hi && (x == mx || mx - x < R.reach); };
             auto bin_of = [&](float x, uint32_t key) { return level == 0 ? by_logit(x) : static_cast<int>((hi - key) >> shift); };
+            __syncthreads();
             for (int i = tid; i < kLimbs * kBins; i += kThreads) (&S.hist[0][0])[i] = 0;
             if (tid == 0) S.mine = 0;
             __syncthreads();
-            for (int i = i0; i < i1; ++i) {
-                const float x = xs[i];
+            for (int i = lane; i < have; i += 32) {
+                const float x = x_of[i];
                 const uint32_t key = key_of(x);
-                if (!in(x, key)) continue;
+                if (!in(key)) continue;
                 const int b = bin_of(x, key);
                 if constexpr (WEIGHT) {
                     const uint64_t w = R.weight(x);
@@ -309,6 +399,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
                 g1 += S.group[c][2 * lane + 1];
             }
             const uint64_t upto = warp_scan(g0 + g1);
+            __syncthreads();                   // read by all: its place is the group's bins'
             if (level == 0) {
                 const uint64_t all = __shfl_sync(0xffffffffu, upto, 31);
                 want = want_of(all);
@@ -342,41 +433,26 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
                     return true;
                 }
             }
-            // ---- the bin's tokens, if they are few, ranked one by one ----
-            for (int i = i0; i < i1; ++i) {
-                const float x = xs[i];
-                const uint32_t key = key_of(x);
-                if (!in(x, key) || (level == 0 && by_logit(x) != bin)) continue;
-                const uint32_t to = atomicAdd(&S.mine, 1u);
-                if (to < kList) S.list[to] = key;
-            }
-            __syncthreads();
-            if (tid < cl.n) *cl.g.map_shared_rank(&S.count[cl.rank], tid) = S.mine;
-            cl.g.sync();
-            const uint32_t me = tid;
-            uint32_t have = 0, key = 0;
-            for (int c = 0; c < cl.n; ++c) {
-                const uint32_t m = S.count[c];
-                if (me >= have && me - have < min(m, static_cast<uint32_t>(kList))) key = *cl.g.map_shared_rank(&S.list[me - have], c);
-                have += m;
-            }
-            if (have <= kList) {
-                S.key[tid] = key;
-                S.weight[tid] = !WEIGHT ? 1 : me < have ? R.weight(of_key(key)) : 0;
-                __syncthreads();
-                uint64_t above = 0, with = 0;
-                for (uint32_t j = 0; j < have; ++j) {
-                    const uint32_t kj = S.key[j];
-                    const uint64_t w = S.weight[j];
-                    above += kj > key ? w : 0;
-                    with += kj >= key ? w : 0;
+            // ---- the bin's tokens, if they are few, ranked one by one; those behind it dropped ----
+            if (level == 0) {
+                keep.template operator()<false>([&](float x) {
+                    const int b = by_logit(x);
+                    if (b == bin) {
+                        const uint32_t key = key_of(x);
+                        if (in(key)) list_key(key);
+                    }
+                    return b <= bin;
+                });
+            } else {
+                for (int i = lane; i < have; i += 32) {
+                    const uint32_t key = key_of(x_of[i]);
+                    if (in(key)) list_key(key);
                 }
-                if (me < have && above < want && with >= want) {   // tokens of one key: they write the same
-                    S.found = want - above;
-                    S.found_key = key;
-                }
-                __syncthreads();
-                cut = Cut{S.found_key, S.found};
+            }
+            const uint32_t all = gather();
+            if (all <= kList) {
+                rank(all);
+                left = ~0ull;                  // not known any more
                 return true;
             }
             if (level == 0) {
@@ -400,8 +476,9 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
         }
     };
     Cut cut{0, 0};
-    if (k > 0) search.template operator()<false>(0, [&](uint64_t) { return static_cast<uint64_t>(k); }, cut);
+    if (k > 0 && static_cast<uint64_t>(k) < left) search.template operator()<false>(0, [&](uint64_t) { return static_cast<uint64_t>(k); }, cut);
     if (top_p < 1.0f) {
+        if (left == ~0ull) left = count_left();
         const uint64_t tie_w = cut.ties ? R.weight(of_key(cut.key)) : 0, tied = cut.ties * tie_w;
         uint64_t in_ties = 0;                       // what is left to be reached among the ties of the cut so far
         Cut c2{0, 0};
@@ -422,40 +499,65 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
             cut.ties = (in_ties + tie_w - 1) / tie_w;
         }
     }
-    // ---- the running sum of kept weights, by index ----
+    // ---- the running sum of kept weights, by index: warps' sums, then the warp's in which the number lies ----
     const uint64_t tie_w = cut.ties ? R.weight(of_key(cut.key)) : 0;
-    uint64_t sum = 0, ties = 0;
-    for (int i = i0; i < i1; ++i) {
-        const uint32_t key = key_of(xs[i]);
-        if (key > cut.key) sum += R.weight(xs[i]);
+    uint64_t sum = 0;
+    uint32_t ties = 0;
+    for (int i = lane; i < have; i += 32) {
+        const float x = x_of[i];
+        const uint32_t key = key_of(x);
+        if (key > cut.key) sum += R.weight(x);
         else if (key == cut.key) ++ties;
     }
-    uint64_t cta_sum, cta_ties;
-    const uint64_t sum_upto = block_scan(S, sum, cta_sum), ties_upto = block_scan(S, ties, cta_ties);
+#pragma unroll
+    for (int d = 1; d < 32; d *= 2) sum += __shfl_xor_sync(0xffffffffu, sum, d);
+    ties = __reduce_add_sync(0xffffffffu, ties);
+    __syncthreads();
+    if (lane == 0) {
+        S.warp_sum[warp] = sum;
+        S.warp_ties[warp] = ties;
+    }
+    __syncthreads();
+    uint64_t cta_sum = 0, cta_ties = 0, run = 0, tie = 0;   // run, tie: before this warp's tokens
+    for (int w = 0; w < kWarps; ++w) {
+        if (w == warp) {
+            run = cta_sum;
+            tie = cta_ties;
+        }
+        cta_sum += S.warp_sum[w];
+        cta_ties += S.warp_ties[w];
+    }
     const auto s = cl.tell(tid == 0, cta_sum, cta_ties);
-    uint64_t base = 0, all = 0, ties_base = 0, ties_all = 0;
+    uint64_t all = 0, ties_all = 0;
     for (int i = 0; i < cl.n; ++i) {
         if (i < cl.rank) {
-            base += s[0][i];
-            ties_base += s[1][i];
+            run += s[0][i];
+            tie += s[1][i];
         }
         all += s[0][i];
         ties_all += s[1][i];
     }
     all += min(ties_all, cut.ties) * tie_w;
     const uint64_t at = min(static_cast<uint64_t>(static_cast<double>(u > 0.f ? fminf(u, 1.0f) : 0.f) * static_cast<double>(all)), all - 1);
-    uint64_t tie = ties_base + ties_upto - ties;   // ties before this thread's tokens
-    uint64_t run = base + sum_upto - sum + min(tie, cut.ties) * tie_w;
-    const uint64_t end = base + sum_upto + min(tie + ties, cut.ties) * tie_w;
-    if (run <= at && at < end) {
-        int i = i0;
-        for (; i < i1; ++i) {
-            const uint32_t key = key_of(xs[i]);
-            if (key > cut.key) run += R.weight(xs[i]);
-            else if (key == cut.key && tie++ < cut.ties) run += tie_w;
-            if (run > at) break;
+    const uint64_t end = run + sum + min(tie + ties, cut.ties) * tie_w;
+    run += min(tie, cut.ties) * tie_w;
+    if (run > at || at >= end) return;
+    for (int i = 0; i < have; i += 32) {
+        const float x = i + lane < have ? x_of[i + lane] : -INFINITY;
+        const uint32_t key = key_of(x);
+        const bool is_tie = i + lane < have && key == cut.key;
+        const uint32_t set = __ballot_sync(0xffffffffu, is_tie);
+        uint64_t w = 0;
+        if (i + lane < have && key > cut.key) w = R.weight(x);
+        if (is_tie && tie + __popc(set & ((1u << lane) - 1)) < cut.ties) w = tie_w;
+        tie += __popc(set);
+        const uint64_t upto = run + warp_scan(w);
+        const uint32_t over = __ballot_sync(0xffffffffu, upto > at);
+        if (over) {
+            if (lane == __ffs(over) - 1) A.tokens[row] = v0 + p0 + id_of[i + lane];
+            return;
         }
-        A.tokens[row] = v0 + i;
+        run = __shfl_sync(0xffffffffu, upto, 31);
     }
 }
 
@@ -463,18 +565,18 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
 
 cudaError_t launch_sample_rows(SampleRowsArgs a, int n_rows, cudaStream_t stream) {
     constexpr int kExtra = sizeof(Shared) + 16;     // and the alignment of a slice
+    constexpr int kToken = sizeof(float) + sizeof(uint16_t);
     static_assert(sizeof(Shared) % 16 == 0, "16-byte pieces of the slice");
-    static_assert(kExtra + kSampleSlice * sizeof(float) <= 232448, "shared memory of one SM");
+    static_assert(kExtra + kSampleSlice * kToken <= 232448, "shared memory of one SM");
     static PerDeviceOnce once;
     cudaError_t e = once.run([&](int) {
         return cudaFuncSetAttribute(sample_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                    static_cast<int>(kExtra + kSampleSlice * sizeof(float)));
+                                    kExtra + kSampleSlice * kToken);
     });
     if (e != cudaSuccess) return e;
     int ctas = 1;
     while (ctas < kRowCtas && (n_rows * ctas < 148 || (a.n_vocab + ctas - 1) / ctas > 12800)) ctas *= 2;
     a.slice = (a.n_vocab + ctas - 1) / ctas;
-    a.per_thread = ((a.slice + kThreads - 1) / kThreads) | 1;   // odd: no bank conflicts
     cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[0].val.programmaticStreamSerializationAllowed = 1;
@@ -484,7 +586,7 @@ cudaError_t launch_sample_rows(SampleRowsArgs a, int n_rows, cudaStream_t stream
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3(static_cast<unsigned>(n_rows) * ctas);
     cfg.blockDim = dim3(kThreads);
-    cfg.dynamicSmemBytes = kExtra + a.slice * sizeof(float);
+    cfg.dynamicSmemBytes = kExtra + a.slice * kToken;
     cfg.stream = stream;
     cfg.attrs = attr;
     cfg.numAttrs = 2;
