@@ -62,37 +62,45 @@ __device__ __forceinline__ float of_key(uint32_t k) {
     return __uint_as_float(k & 0x80000000u ? k & 0x7fffffffu : ~k);
 }
 
-// exp(z) 2^40 for -kReach - 1 < z <= 0: z = n ln 2 + r, |r| <= ln 2 / 2, and 12 terms
-// of r's power series (the next one is below 2^-47).
-__device__ __forceinline__ double exp_scaled(double z) {
-    const double n = rint(z * 1.4426950408889634);
-    double r = fma(n, -0.693147182464599609375, z);      // ln 2 in 24 bits: n times it is exact
-    r = fma(n, 1.904654299957768e-9, r);                 // and the rest
-    double p = 1.0 / 39916800;
-    p = fma(p, r, 1.0 / 3628800);
-    p = fma(p, r, 1.0 / 362880);
-    p = fma(p, r, 1.0 / 40320);
-    p = fma(p, r, 1.0 / 5040);
-    p = fma(p, r, 1.0 / 720);
-    p = fma(p, r, 1.0 / 120);
-    p = fma(p, r, 1.0 / 24);
-    p = fma(p, r, 1.0 / 6);
-    p = fma(p, r, 0.5);
-    p = fma(p, r, 1.0);
-    p = fma(p, r, 1.0);
-    return p * __longlong_as_double((static_cast<long long>(static_cast<int>(n) + 40 + 1023)) << 52);
-}
+// 2^(j / 64) 2^40, j < 64, by the power series of exp.
+struct Powers {
+    double v[64];
+    constexpr Powers() : v{} {
+        for (int j = 0; j < 64; ++j) {
+            double term = 1.0, sum = 0.0;
+            for (int k = 1; k < 24; ++k) {
+                sum += term;
+                term *= j * (0.69314718055994530942 / 64) / k;
+            }
+            v[j] = sum * 1099511627776.0;
+        }
+    }
+};
+__constant__ const Powers kPowers = Powers();
 
 struct RowRules {
-    float mx;          // the largest logit
-    float reach;       // logits at least so far below it weigh nothing
-    double inv_t;
-    double least;      // min_p 2^40
+    float mx;              // the largest logit
+    float reach;           // logits further below it weigh nothing
+    double c;              // 64 log2(e) / T
+    uint64_t least;        // min_p 2^40
+    const double* powers;  // Powers, in shared memory
+    // exp((x - mx) / T) 2^40 = 2^(n / 64) 2^40 e^s with a whole number n and |s| <= ln 2 / 128: four terms of e^s
+    // beyond 1 (the next is below 2^-44), the rounding to whole numbers by adding 1.5 * 2^52 and 2^52.
+    __device__ __forceinline__ bool in_reach(float x) const { return x - mx >= -reach; }
     __device__ __forceinline__ uint64_t weight(float x) const {
-        if (x == mx) return kOne;
-        if (!(mx - x < reach)) return 0;
-        const double w = exp_scaled((static_cast<double>(x) - static_cast<double>(mx)) * inv_t);
-        return w < least ? 0 : __double2ull_rn(w);
+        constexpr double kRound = 6755399441055744.0, kWhole = 4503599627370496.0, kUnit = 0.69314718055994530942 / 64;
+        const double d = static_cast<double>(x) - static_cast<double>(mx);
+        const double t = fma(d, c, kRound);
+        const int n = __double2loint(t);
+        const double s = fma(d, c, -(t - kRound));
+        double p = fma(s, kUnit * kUnit * kUnit * kUnit / 24, kUnit * kUnit * kUnit / 6);
+        p = fma(p, s, kUnit * kUnit / 2);
+        p = fma(p, s, kUnit);
+        p = fma(p, s, 1.0);
+        const double q = powers[n & 63];
+        const double w = fma(p, __hiloint2double(__double2hiint(q) + ((n >> 6) << 20), __double2loint(q)), kWhole);
+        const uint64_t whole = static_cast<uint64_t>(__double_as_longlong(w)) & 0xfffffffffffffull;
+        return in_reach(x) && whole >= least ? whole : 0;   // what is out of reach has come out as anything
     }
 };
 
@@ -112,6 +120,7 @@ struct alignas(16) Shared {                // the slice lies behind it
     uint32_t count[2][kRowCtas];           // how many each CTA has
     uint32_t mine;
     uint64_t slot[2][3][kRowCtas];         // what the CTAs of the cluster told each other, by turns
+    double powers[64];
     uint64_t warp_sum[kWarps];
     uint32_t warp_ties[kWarps];
     uint64_t found;
@@ -168,6 +177,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
     Cluster cl(S);
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int64_t row = blockIdx.x / cl.n;
+    if (tid < 64) S.powers[tid] = kPowers.v[tid];
     const int v0 = cl.rank * A.slice, n = max(0, min(A.slice, A.n_vocab - v0));
     // ---- the slice into shared memory, its largest logit ----
     const float* src = A.logits + row * A.stride + v0;
@@ -236,19 +246,26 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
         if (cl.rank == 0 && tid == 0) A.tokens[row] = at;
         return;
     }
+    if (mx == INFINITY) {                      // the ones of +inf are alike, and the others' weight is nothing
+        for (int i = lane; i < have; i += 32) x_of[i] = x_of[i] == INFINITY ? 0.f : -INFINITY;
+        mx = 0.f;
+        __syncwarp();
+    }
     RowRules R;
     R.mx = mx;
-    R.inv_t = 1.0 / static_cast<double>(T);
-    R.least = static_cast<double>(min_p) * static_cast<double>(kOne);
+    R.c = 64 * 1.4426950408889634 / static_cast<double>(T);
+    R.least = static_cast<uint64_t>(ceil(static_cast<double>(min_p) * static_cast<double>(kOne)));
+    R.powers = S.powers;
     R.reach = (min_p > 0.f ? fminf(kReach, -logf(min_p) + 0.01f) : kReach) * T;
-    // ---- what is left of the warp's tokens, in place and in order ----
+    // Drops tokens of the warp, the others stay in place and in order; id is a token's place in the warp's part.
     uint16_t* id_of = reinterpret_cast<uint16_t*>(smem_raw + sizeof(Shared) + 16 + A.slice * sizeof(float)) + p0;
-    auto keep = [&]<bool FIRST>(auto&& stays) {
+    bool whole = true;                         // nothing has been dropped: ids are not written yet
+    auto keep = [&](auto&& stays) {
         int out = 0;
         for (int i = 0; i < have; i += 32) {
             const bool in = i + lane < have;
             const float x = in ? x_of[i + lane] : 0.f;
-            const int id = FIRST ? i + lane : in ? id_of[i + lane] : 0;
+            const int id = whole ? i + lane : in ? id_of[i + lane] : 0;
             const bool stay = in && stays(x);
             const uint32_t set = __ballot_sync(0xffffffffu, stay);
             if (stay) {
@@ -260,9 +277,10 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
             __syncwarp();
         }
         have = out;
+        whole = false;
     };
-    // the tokens left in all CTAs; a barrier of the cluster
-    auto count_left = [&]() {
+    uint64_t left = ~0ull;                     // tokens left in all CTAs at most, once something was dropped
+    auto count_left = [&]() {                  // a barrier of the cluster
         __syncthreads();
         if (lane == 0) S.warp_sum[warp] = have;
         __syncthreads();
@@ -273,26 +291,23 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
         for (int i = 0; i < cl.n; ++i) all += s[0][i];
         return all;
     };
-    keep.template operator()<true>([&](float x) { return x == mx || mx - x < R.reach; });   // the others weigh nothing
-    uint64_t left = count_left();
     int searches = 0;
-    // The cut at which the ranking's count (WEIGHT: sum of weights) of the tokens left with a key above `from` first
-    // reaches want_of(its sum over all of them).  A want of 0, or of more than there is: no cut.  Cut::ties is then
+    // The cut at which the ranking's count (WEIGHT: sum of weights) within reach (the others weigh nothing) with a
+    // key above `from` first reaches want_of(its sum over all of them).  A want of 0, or of more than there is: no cut.  Cut::ties is then
     // what is to be reached among the tokens of Cut::key.  Tokens below the cut may be dropped.
     auto search = [&]<bool WEIGHT>(uint32_t from, auto&& want_of, Cut& cut) -> bool {
         constexpr int kLimbs = WEIGHT ? 3 : 1;
         const int turn = searches++ & 1;
         uint32_t lo = from + 1, hi = key_of(mx);   // the keys in question
-        const float per = R.reach > 0.f ? kBins / R.reach : 0.f;
+        const float per = R.reach > 0.f ? fminf(kBins / R.reach, 3e38f) : 0.f;   // finite: the largest logit's bin is 0
         uint64_t want = 0;
         int shift = 0;
-        // level 0: bins of equal width in logits; then of keys.  Falls with the key;
-        // inf - inf and inf * 0 are the largest logit's.
+        // level 0: bins of equal width in logits; then of keys.  Falls with the key.
         auto by_logit = [&](float x) {
             const float d = (mx - x) * per;
-            return d < kBins ? static_cast<int>(d) : x == mx ? 0 : kBins - 1;
+            return d < kBins ? static_cast<int>(d) : kBins - 1;
         };
-        auto in = [&](uint32_t key) { return key >= lo && key <= hi; };
+        auto in = [&](float x, uint32_t key) { return key >= lo && key <= hi && R.in_reach(x); };
         // this CTA's keys to list one by one: to all CTAs' knowledge, then those of all with their weights
         // in S.key and S.weight; returns how many there are (more than kList: no list)
         auto gather = [&]() {
@@ -344,8 +359,9 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
             if (tid == 0) S.mine = 0;
             __syncthreads();
             for (int i = lane; i < have; i += 32) {
-                const uint32_t key = key_of(x_of[i]);
-                if (in(key)) list_key(key);
+                const float x = x_of[i];
+                const uint32_t key = key_of(x);
+                if (in(x, key)) list_key(key);
             }
             const uint32_t all = gather();
             uint64_t sum = 0;
@@ -365,7 +381,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
             for (int i = lane; i < have; i += 32) {
                 const float x = x_of[i];
                 const uint32_t key = key_of(x);
-                if (!in(key)) continue;
+                if (!in(x, key)) continue;
                 const int b = bin_of(x, key);
                 if constexpr (WEIGHT) {
                     const uint64_t w = R.weight(x);
@@ -423,6 +439,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
             const int at = __ffs(__ballot_sync(0xffffffffu, fine_upto >= want)) - 1;
             want -= __shfl_sync(0xffffffffu, fine_upto - f, at);
             const int bin = 32 * group + at;
+            if (!WEIGHT && level == 0) left = __shfl_sync(0xffffffffu, fine_upto, at);   // up to and with the bin
             if (level > 0) {
                 const uint32_t h = hi - (static_cast<uint32_t>(bin) << shift);
                 lo = max(lo, h - ((1u << shift) - 1));
@@ -435,24 +452,24 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
             }
             // ---- the bin's tokens, if they are few, ranked one by one; those behind it dropped ----
             if (level == 0) {
-                keep.template operator()<false>([&](float x) {
+                keep([&](float x) {
                     const int b = by_logit(x);
                     if (b == bin) {
                         const uint32_t key = key_of(x);
-                        if (in(key)) list_key(key);
+                        if (in(x, key)) list_key(key);
                     }
-                    return b <= bin;
+                    return b <= bin && R.in_reach(x);
                 });
             } else {
                 for (int i = lane; i < have; i += 32) {
-                    const uint32_t key = key_of(x_of[i]);
-                    if (in(key)) list_key(key);
+                    const float x = x_of[i];
+                    const uint32_t key = key_of(x);
+                    if (in(x, key)) list_key(key);
                 }
             }
             const uint32_t all = gather();
             if (all <= kList) {
                 rank(all);
-                left = ~0ull;                  // not known any more
                 return true;
             }
             if (level == 0) {
@@ -475,10 +492,14 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
             shift = max(0, 32 - __clz(hi - lo) - 11);   // (hi - lo) >> shift < kBins
         }
     };
+    // where min-p leaves a narrow range, what is outside goes first
+    if (min_p > 0.f && (k > 0 || top_p < 1.0f)) {
+        keep([&](float x) { return R.in_reach(x); });
+        left = count_left();
+    }
     Cut cut{0, 0};
     if (k > 0 && static_cast<uint64_t>(k) < left) search.template operator()<false>(0, [&](uint64_t) { return static_cast<uint64_t>(k); }, cut);
     if (top_p < 1.0f) {
-        if (left == ~0ull) left = count_left();
         const uint64_t tie_w = cut.ties ? R.weight(of_key(cut.key)) : 0, tied = cut.ties * tie_w;
         uint64_t in_ties = 0;                       // what is left to be reached among the ties of the cut so far
         Cut c2{0, 0};
@@ -503,11 +524,16 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
     const uint64_t tie_w = cut.ties ? R.weight(of_key(cut.key)) : 0;
     uint64_t sum = 0;
     uint32_t ties = 0;
-    for (int i = lane; i < have; i += 32) {
-        const float x = x_of[i];
-        const uint32_t key = key_of(x);
-        if (key > cut.key) sum += R.weight(x);
-        else if (key == cut.key) ++ties;
+    if (cut.key == 0) {
+#pragma unroll 4
+        for (int i = lane; i < have; i += 32) sum += R.weight(x_of[i]);
+    } else {
+        for (int i = lane; i < have; i += 32) {
+            const float x = x_of[i];
+            const uint32_t key = key_of(x);
+            if (key > cut.key) sum += R.weight(x);
+            else if (key == cut.key) ++ties;
+        }
     }
 #pragma unroll
     for (int d = 1; d < 32; d *= 2) sum += __shfl_xor_sync(0xffffffffu, sum, d);
@@ -554,7 +580,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
         const uint64_t upto = run + warp_scan(w);
         const uint32_t over = __ballot_sync(0xffffffffu, upto > at);
         if (over) {
-            if (lane == __ffs(over) - 1) A.tokens[row] = v0 + p0 + id_of[i + lane];
+            if (lane == __ffs(over) - 1) A.tokens[row] = v0 + p0 + (whole ? i + lane : id_of[i + lane]);
             return;
         }
         run = __shfl_sync(0xffffffffu, upto, 31);
