@@ -121,7 +121,7 @@ int tle_logits_adjust(float* out, int64_t out_stride, const float* logits, int64
  * [n_rows] numbers, NULL: off for all rows.  Off are also a top_k <= 0 or >=
  * n_vocab, a top_p >= 1 and a min_p <= 0; NaN is off. */
 typedef struct {
-    const float* temperature;   /* NULL: 1; <= 0 or NaN: the largest logit's token */
+    const float* temperature;   /* NULL: 1; <= 0 or NaN: the largest logit's token; above 1e30: 1e30 */
     const int32_t* top_k;
     const float* top_p;         /* <= 0: the first token of the ranking       */
     const float* min_p;         /* above 1 counts as 1                        */
@@ -138,8 +138,8 @@ typedef struct {
  * nucleus by rank instead: the same probabilities, other tokens for the same number.)
  * Weights are whole numbers of 2^-40 of the largest: the choice does not depend
  * on the launch, and a token below 2^-41 of the likeliest is never drawn.  NaN
- * logits count as -inf; of +inf logits each weighs 1 and all others nothing.  A row of -inf
- * only gets the token -1.  n_vocab <= 262144; 4-byte aligned pointers. */
+ * logits count as -inf, +inf as the largest finite number.  A row of -inf only
+ * gets the token -1.  n_vocab <= 262144; 4-byte aligned pointers. */
 int tle_sample_rows(int32_t* tokens, const float* logits, int64_t logits_stride, int n_rows, int n_vocab,
                     const tle_sample_rules_t* rules, const float* uniform, void* stream);
 

@@ -158,6 +158,7 @@ def test_temperatures(cuda, T, rules):
     x = (5 * r.standard_normal((12, 2500))).astype(np.float32)
     x[3] *= 1e-20
     x[4] *= 1e20
+    x[5:8, ::2] = -np.inf                                   # masked tokens stay so at any temperature
     on = rules != "none"
     check(x, T, r.integers(2, 2500, 12) if on else 0, r.uniform(0.3, 1, 12) if on else 1.0, r.uniform(0, 0.01, 12) if on else 0.0, r.random(12))
 

@@ -119,7 +119,7 @@ struct alignas(16) Shared {                // the slice lies behind it
     uint32_t list[2][kList];               // of two searches in turn: this CTA's keys of the bin in question
     uint32_t count[2][kRowCtas];           // how many each CTA has
     uint32_t mine;
-    uint64_t slot[2][3][kRowCtas];         // what the CTAs of the cluster told each other, by turns
+    uint64_t slot[2][2][kRowCtas];         // what the CTAs of the cluster told each other, by turns
     double powers[64];
     uint64_t warp_sum[kWarps];
     uint32_t warp_ties[kWarps];
@@ -137,16 +137,14 @@ struct Cluster {
         rank = static_cast<int>(g.block_rank());
         n = static_cast<int>(g.num_blocks());
     }
-    // a, b, c of one thread (`by`) of every CTA, in slot[...] of all; a barrier of the cluster
-    __device__ __forceinline__ const uint64_t (*tell(bool by, uint64_t a, uint64_t b = 0, uint64_t c = 0))[kRowCtas] {
+    // a, b, the same in all threads of a CTA, to slot[..][this rank] of all CTAs; a barrier of the cluster
+    __device__ __forceinline__ const uint64_t (*tell(uint64_t a, uint64_t b = 0))[kRowCtas] {
         auto& s = S.slot[turn & 1];
         ++turn;
-        if (by)
-            for (int i = 0; i < n; ++i) {
-                *g.map_shared_rank(&s[0][rank], i) = a;
-                *g.map_shared_rank(&s[1][rank], i) = b;
-                *g.map_shared_rank(&s[2][rank], i) = c;
-            }
+        if (static_cast<int>(threadIdx.x) < n) {
+            *g.map_shared_rank(&s[0][rank], threadIdx.x) = a;
+            *g.map_shared_rank(&s[1][rank], threadIdx.x) = b;
+        }
         g.sync();
         return s;
     }
@@ -185,7 +183,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
     float* xs = reinterpret_cast<float*>(smem_raw + sizeof(Shared)) + ((4 - head) & 3);              // aligned as the row is
     float mx = -INFINITY;
     auto take = [&](float x) {
-        x = fmaxf(x + 0.0f, -INFINITY);        // -0 is 0, NaN -inf
+        x = fminf(fmaxf(x + 0.0f, -INFINITY), 3.4028234e38f);   // -0 is 0, NaN -inf, +inf the largest number
         mx = fmaxf(mx, x);
         return x;
     };
@@ -207,7 +205,8 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
         const int tail = head + 4 * body;
         if (tail + tid < n && tid < 4) xs[tail + tid] = take(src[tail + tid]);
     }
-    const float T = A.temperature ? A.temperature[row] : 1.0f;
+    float T = A.temperature ? A.temperature[row] : 1.0f;
+    T = T > 1e30f ? 1e30f : T;                 // so that differences of logits stay within reach or below it
     int k = A.top_k ? A.top_k[row] : 0;
     if (k >= A.n_vocab) k = 0;
     const float top_p = A.top_p ? A.top_p[row] : 1.0f;
@@ -222,7 +221,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
     for (int w = 0; w < kWarps; ++w) mx = fmaxf(mx, S.warp_max[w]);
     asm volatile("barrier.cluster.wait.aligned;" ::: "memory");
     {
-        const auto s = cl.tell(tid == 0, __float_as_uint(mx));
+        const auto s = cl.tell(__float_as_uint(mx));
         for (int i = 0; i < cl.n; ++i) mx = fmaxf(mx, __uint_as_float(static_cast<uint32_t>(s[0][i])));
     }
     if (mx == -INFINITY) {                     // the same in all CTAs
@@ -241,15 +240,10 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
         if (lane == 0) S.warp_sum[warp] = at;
         __syncthreads();
         for (int w = 0; w < kWarps; ++w) at = min(at, static_cast<int>(S.warp_sum[w]));
-        const auto s = cl.tell(tid == 0, at);
+        const auto s = cl.tell(at);
         for (int i = 0; i < cl.n; ++i) at = min(at, static_cast<int>(s[0][i]));
         if (cl.rank == 0 && tid == 0) A.tokens[row] = at;
         return;
-    }
-    if (mx == INFINITY) {                      // the ones of +inf are alike, and the others' weight is nothing
-        for (int i = lane; i < have; i += 32) x_of[i] = x_of[i] == INFINITY ? 0.f : -INFINITY;
-        mx = 0.f;
-        __syncwarp();
     }
     RowRules R;
     R.mx = mx;
@@ -286,7 +280,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
         __syncthreads();
         uint64_t sum = 0;
         for (int w = 0; w < kWarps; ++w) sum += S.warp_sum[w];
-        const auto s = cl.tell(tid == 0, sum);
+        const auto s = cl.tell(sum);
         uint64_t all = 0;
         for (int i = 0; i < cl.n; ++i) all += s[0][i];
         return all;
@@ -553,7 +547,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
         cta_sum += S.warp_sum[w];
         cta_ties += S.warp_ties[w];
     }
-    const auto s = cl.tell(tid == 0, cta_sum, cta_ties);
+    const auto s = cl.tell(cta_sum, cta_ties);
     uint64_t all = 0, ties_all = 0;
     for (int i = 0; i < cl.n; ++i) {
         if (i < cl.rank) {
