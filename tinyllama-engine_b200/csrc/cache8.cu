@@ -31,13 +31,17 @@ namespace tle {
 namespace {
 
 // ---- append -----------------------------------------------------------------
-// As append_kernel (chunk.cu): a warp takes a token or a part of one, in
-// 16-byte pieces, 8 (bf16) or 16 (fp32) lanes per head, so the norm's sum and
-// the largest value of a head are reductions over those lanes, and a pair's
-// other half is in the lane itself (interleaved) or a fixed distance away.
+// A warp takes a token, or an equal part of its pieces where there are few
+// tokens.  A piece is one load of a warp: as many q heads, k heads or v heads as
+// there are lanes for, 8 (bf16) or 16 (fp32) a head, each with two groups of 8
+// bytes -- with the half layout the two that its pairs lie in, otherwise two in
+// a row -- so that a pair's elements meet in a lane, and the norm's sum and the largest
+// value of a head are reductions over its lanes.  Sines and cosines are found once a token.
+// HBM-bound: kBatch pieces are in flight, the first ones while the token's place is looked up.
 constexpr int kThreads = 64;
 constexpr int kPart = 4;            // pieces of the smallest part of a token
 constexpr int kWarps = 148 * 16;    // below so many tokens their heads are spread over several warps
+constexpr int kBatch = 8;
 
 template <int LANES>
 __device__ __forceinline__ float sum_over(float x) {
@@ -59,50 +63,79 @@ __device__ __forceinline__ int scale_byte(float most) {
     return (u >> 23) == 255u ? 255 : min(max(b, 1), 248);
 }
 
-template <int VE>
-__device__ __forceinline__ void store_codes(int8_t* p, const float (&y)[VE], float inv) {
-    uint32_t w[VE / 4];
-#pragma unroll
-    for (int i = 0; i < VE / 4; ++i) {
-        uint32_t u = 0;
-#pragma unroll
-        for (int e = 0; e < 4; ++e)   // the bounds cut the largest numbers of 32 bits only
-            u |= (static_cast<uint32_t>(__float2int_rn(fminf(fmaxf(y[4 * i + e] * inv, -127.f), 127.f))) & 0xffu) << (8 * e);
-        w[i] = u;
-    }
-    if constexpr (VE == 8) *reinterpret_cast<uint2*>(p) = make_uint2(w[0], w[1]);
-    else *reinterpret_cast<uint32_t*>(p) = w[0];
+// A group of 8 bytes of activations as numbers.
+template <class Act>
+constexpr int kGroup = 8 / sizeof(Act);
+__device__ __forceinline__ void group_of(uint2 u, float (&f)[2]) {
+    f[0] = __uint_as_float(u.x);
+    f[1] = __uint_as_float(u.y);
+}
+__device__ __forceinline__ void group_of(uint2 u, float (&f)[4]) {
+    f[0] = __uint_as_float(u.x << 16);
+    f[1] = __uint_as_float(u.x & 0xffff0000u);
+    f[2] = __uint_as_float(u.y << 16);
+    f[3] = __uint_as_float(u.y & 0xffff0000u);
+}
+template <class T>
+__device__ __forceinline__ void store_group(T* p, const float (&f)[2]) { store_pair(p, make_float2(f[0], f[1])); }
+template <class T>
+__device__ __forceinline__ void store_group(T* p, const float (&f)[4]) { store4(p, f); }
+// Codes of a group; the bounds cut the largest numbers of 32 bits only.
+__device__ __forceinline__ uint32_t code_of(float y, float inv) {
+    return static_cast<uint32_t>(__float2int_rn(fminf(fmaxf(y * inv, -127.f), 127.f))) & 0xffu;
+}
+__device__ __forceinline__ void store_codes(int8_t* p, const float (&f)[2], float inv) {
+    *reinterpret_cast<uint16_t*>(p) = static_cast<uint16_t>(code_of(f[0], inv) | code_of(f[1], inv) << 8);
+}
+__device__ __forceinline__ void store_codes(int8_t* p, const float (&f)[4], float inv) {
+    *reinterpret_cast<uint32_t*>(p) =
+        code_of(f[0], inv) | code_of(f[1], inv) << 8 | code_of(f[2], inv) << 16 | code_of(f[3], inv) << 24;
 }
 
-template <class Act, class Pool>
+template <class Act, class Pool, bool HALF, bool NORM>
 __global__ void __launch_bounds__(kThreads) append_rules_kernel(const __grid_constant__ AppendRulesArgs R, int parts) {
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     asm volatile("griddepcontrol.wait;" ::: "memory");
     constexpr bool kBits8 = sizeof(Pool) == 1;
-    constexpr int kBatch = sizeof(Act) == 4 ? 6 : 4;   // pieces in flight per lane
-    constexpr int VE = 16 / sizeof(Act);
-    constexpr int LPH = HD / VE;
+    constexpr int GE = kGroup<Act>;
+    constexpr int LPH = HD / (2 * GE);
     constexpr int HPW = 32 / LPH;
     const AppendArgs& A = R.a;
-    const int lane = threadIdx.x & 31;
+    const int lane = threadIdx.x & 31, hl = lane % LPH, sub = lane / LPH;
     const int64_t w = static_cast<int64_t>(blockIdx.x) * (kThreads / 32) + (threadIdx.x >> 5);
     const int64_t tok = w / parts;
     if (tok >= A.n_tokens) return;
     const int part = static_cast<int>(w - tok * parts);
-    const int units = A.n_head + 2 * A.n_head_kv, kv0 = A.n_head, v0 = A.n_head + A.n_head_kv;
-    const int pieces = (units + HPW - 1) / HPW;
+    // this lane's two groups of a head: elements e1 .., e2 ..
+    const int hg = R.half / GE;
+    const int g1 = HALF ? (hl < hg ? hl : 2 * hl) : 2 * hl, g2 = HALF && hl < hg ? hl + hg : g1 + 1;
+    const int e1 = g1 * GE, e2 = g2 * GE;
+    const bool turned = A.rotate && (HALF ? hl < hg : e1 < 2 * R.half);
+    const int nq = (A.n_head + HPW - 1) / HPW, nk = (A.n_head_kv + HPW - 1) / HPW, pieces = nq + 2 * nk;
+    const int j_first = static_cast<int>(static_cast<int64_t>(part) * pieces / parts);
     const int j_end = static_cast<int>(static_cast<int64_t>(part + 1) * pieces / parts);
+    const Act* q = static_cast<const Act*>(A.q) + tok * A.q_stride;
+    const Act* k = static_cast<const Act*>(A.k) + tok * A.k_stride;
+    const Act* v = static_cast<const Act*>(A.v) + tok * A.v_stride;
+    uint2 x[kBatch][2];
+    auto load = [&](int j0) {
+#pragma unroll
+        for (int b = 0; b < kBatch; ++b) {
+            const int j = j0 + b, base = j < nq ? 0 : j < nq + nk ? nq : nq + nk;
+            const int h = (j - base) * HPW + sub;
+            const Act* src = (j < nq ? q : j < nq + nk ? k : v) + h * HD;
+            const bool in = j < j_end && h < (j < nq ? A.n_head : A.n_head_kv);
+            x[b][0] = in ? *reinterpret_cast<const uint2*>(src + e1) : make_uint2(0, 0);
+            x[b][1] = in ? *reinterpret_cast<const uint2*>(src + e2) : make_uint2(0, 0);
+        }
+    };
+    load(j_first);
     // before its records: another plan's descriptor may end before this one's do
     if (A.d.hdr->id != A.plan_id) {
         if (lane == 0) record_error(A.err, kErrBadDesc);
         return;
     }
     const ChunkTok tk = A.d.toks[tok];
-    const int d0 = lane % LPH * VE;
-    const Act* q = static_cast<const Act*>(A.q) + tok * A.q_stride + d0;
-    const Act* k = static_cast<const Act*>(A.k) + tok * A.k_stride + d0;
-    const Act* v = static_cast<const Act*>(A.v) + tok * A.v_stride + d0;
-    Act* qo = static_cast<Act*>(A.q_out) + tok * A.n_head * HD + d0;
     // the token's row in the pools: its first head there, and from head to head
     const int page_rows = 1 << A.page_shift, r_in = tk.pos & (page_rows - 1);
     const size_t step = kBits8 ? static_cast<size_t>(page_rows) * HD : HD;
@@ -116,92 +149,87 @@ __global__ void __launch_bounds__(kThreads) append_rules_kernel(const __grid_con
     } else if (lane == 0) {
         record_error(A.err, kErrBadPage);
     }
-    Pool* kr = static_cast<Pool*>(A.key_pool) + row * HD + d0;
-    Pool* vr = static_cast<Pool*>(A.value_pool) + row * HD + d0;
-    // y[e] = x[e] cs[e] + (the pair's other element) sn[e]
-    float cs[VE], sn[VE];
-    const bool turned = A.rotate && d0 < 2 * R.half;   // a multiple of 16: all of a lane's elements or none
-    const bool first = d0 < R.half;                    // half layout: the elements a of their pairs
-    const int other = R.halves ? (turned ? (first ? lane + R.half / VE : lane - R.half / VE) : lane) : lane;
+    float cs[GE], sn[GE];   // of this lane's pairs
     if (A.rotate) {
         float s1 = 0.f, c1 = 1.f;
         if (lane < R.half) sincosf(static_cast<float>(tk.pos) * A.inv_freq[lane], &s1, &c1);
         s1 *= R.factor;
         c1 *= R.factor;
 #pragma unroll
-        for (int e = 0; e < VE; ++e) {
-            const int pair = (R.halves ? d0 + e - (first ? 0 : R.half) : (d0 + e) / 2) & 31;
-            cs[e] = __shfl_sync(0xffffffffu, c1, pair);
-            const float s = __shfl_sync(0xffffffffu, s1, pair);
-            sn[e] = (R.halves ? first : e % 2 == 0) ? -s : s;
+        for (int e = 0; e < GE; ++e) {
+            cs[e] = __shfl_sync(0xffffffffu, c1, ((HALF ? e1 : e1 / 2) + e) & 31);
+            sn[e] = __shfl_sync(0xffffffffu, s1, ((HALF ? e1 : e1 / 2) + e) & 31);
         }
     }
-    float qw[VE], kw[VE];
-#pragma unroll
-    for (int e = 0; e < VE; ++e) {
-        qw[e] = R.q_norm ? R.q_norm[d0 + e] : 1.f;
-        kw[e] = R.k_norm ? R.k_norm[d0 + e] : 1.f;
-    }
-    for (int j0 = static_cast<int>(static_cast<int64_t>(part) * pieces / parts); j0 < j_end; j0 += kBatch) {
-        uint4 x[kBatch];
+    for (int j0 = j_first;;) {
 #pragma unroll
         for (int b = 0; b < kBatch; ++b) {
-            const int u = (j0 + b) * HPW + lane / LPH;
-            const Act* src = u < kv0 ? q + u * HD : u < v0 ? k + (u - kv0) * HD : v + (u - v0) * HD;
-            x[b] = j0 + b < j_end && u < units ? *reinterpret_cast<const uint4*>(src) : make_uint4(0, 0, 0, 0);
-        }
+            const int j = j0 + b;
+            if (j >= j_end) break;   // the same in all lanes, as what kind of heads it is
+            const bool is_q = j < nq, is_v = j >= nq + nk;
+            const int h = (j - (is_q ? 0 : is_v ? nq + nk : nq)) * HPW + sub;
+            const bool there = h < (is_q ? A.n_head : A.n_head_kv);
+            float y[GE], z[GE];
+            group_of(x[b][0], y);
+            group_of(x[b][1], z);
+            if (!is_v) {
+                if constexpr (NORM) {
+                    const float* norm = is_q ? R.q_norm : R.k_norm;
+                    if (norm) {
+                        float ss = 0.f;
 #pragma unroll
-        for (int b = 0; b < kBatch; ++b) {
-            if (j0 + b >= j_end) break;   // the same in all lanes
-            const int u = (j0 + b) * HPW + lane / LPH;
-            float y[VE];
-            if constexpr (sizeof(Act) == 2) {
-                bf16x8(x[b], y);
-            } else {
-                y[0] = __uint_as_float(x[b].x);
-                y[1] = __uint_as_float(x[b].y);
-                y[2] = __uint_as_float(x[b].z);
-                y[3] = __uint_as_float(x[b].w);
-            }
-            if (R.q_norm || R.k_norm) {
-                float ss = 0.f;
+                        for (int e = 0; e < GE; ++e) ss = fmaf(y[e], y[e], fmaf(z[e], z[e], ss));
+                        const float f = 1.0f / sqrtf(sum_over<LPH>(ss) * (1.0f / HD) + R.eps);
 #pragma unroll
-                for (int e = 0; e < VE; ++e) ss = fmaf(y[e], y[e], ss);
-                ss = sum_over<LPH>(ss);
-                if (u < kv0 ? R.q_norm != nullptr : u < v0 && R.k_norm != nullptr) {
-                    const float f = 1.0f / sqrtf(ss * (1.0f / HD) + R.eps);
+                        for (int e = 0; e < GE; ++e) {
+                            y[e] = y[e] * f * norm[e1 + e];
+                            z[e] = z[e] * f * norm[e2 + e];
+                        }
+                    }
+                }
+                if (turned) {
 #pragma unroll
-                    for (int e = 0; e < VE; ++e) y[e] = y[e] * f * (u < kv0 ? qw[e] : kw[e]);
+                    for (int e = 0; e < GE; ++e) {
+                        float& a = HALF ? y[e] : e < GE / 2 ? y[2 * e] : z[2 * e - GE];
+                        float& c = HALF ? z[e] : e < GE / 2 ? y[2 * e + 1] : z[2 * e - GE + 1];
+                        const float a0 = a, c0 = c;
+                        a = a0 * cs[e] - c0 * sn[e];
+                        c = a0 * sn[e] + c0 * cs[e];
+                    }
                 }
             }
-            if (A.rotate) {
-                float z[VE];
-#pragma unroll
-                for (int e = 0; e < VE; ++e) z[e] = R.halves ? __shfl_sync(0xffffffffu, y[e], other) : y[e ^ 1];
-                if (turned && u < v0) {
-#pragma unroll
-                    for (int e = 0; e < VE; ++e) y[e] = y[e] * cs[e] + z[e] * sn[e];
+            if (is_q) {
+                if (there) {
+                    Act* qo = static_cast<Act*>(A.q_out) + (tok * A.n_head + h) * HD;
+                    store_group(qo + e1, y);
+                    store_group(qo + e2, z);
                 }
+                continue;
             }
+            Pool* to = static_cast<Pool*>(is_v ? A.value_pool : A.key_pool) + row * HD + h * step;
             if constexpr (kBits8) {
                 float most = 0.f;
 #pragma unroll
-                for (int e = 0; e < VE; ++e) most = fmax3(most, fabsf(y[e]), 0.f);
-                most = max_over<LPH>(most);
-                if (u >= kv0 && u < units && have) {
-                    const int h = u < v0 ? u - kv0 : u - v0, sb = scale_byte(most);
+                for (int e = 0; e < GE; ++e) most = fmax3(most, fabsf(y[e]), fabsf(z[e]));
+                const int sb = scale_byte(max_over<LPH>(most));
+                if (there && have) {
                     if (sb == 255) {
 #pragma unroll
-                        for (int e = 0; e < VE; ++e) y[e] = 0.f;
+                        for (int e = 0; e < GE; ++e) y[e] = z[e] = 0.f;
                     }
-                    store_codes<VE>((u < v0 ? kr : vr) + h * step, y, __uint_as_float(static_cast<uint32_t>(254 - min(sb, 248)) << 23));
-                    if (d0 == 0) (u < v0 ? R.key_scale : R.value_scale)[row + (static_cast<size_t>(h) << A.page_shift)] = static_cast<uint8_t>(sb);
+                    const float inv = __uint_as_float(static_cast<uint32_t>(254 - min(sb, 248)) << 23);
+                    store_codes(to + e1, y, inv);
+                    store_codes(to + e2, z, inv);
+                    if (hl == 0) (is_v ? R.value_scale : R.key_scale)[row + (static_cast<size_t>(h) << A.page_shift)] = static_cast<uint8_t>(sb);
                 }
-            } else {
-                if (u >= kv0 && u < units && have) store_n<VE>(u < v0 ? kr + (u - kv0) * HD : vr + (u - v0) * HD, y);
+            } else if (there && have) {
+                store_group(to + e1, y);
+                store_group(to + e2, z);
             }
-            if (u < kv0) store_n<VE>(qo + u * HD, y);
         }
+        j0 += kBatch;
+        if (j0 >= j_end) break;
+        load(j0);
     }
 }
 
@@ -424,21 +452,30 @@ __global__ void __launch_bounds__(kReadThreads) stage8_kernel(const __grid_const
 
 }  // namespace
 
-cudaError_t launch_append_rules(const AppendRulesArgs& a, bool act_bf16, int pool_bytes, cudaStream_t stream) {
-    const int per_piece = act_bf16 ? 4 : 2;   // heads
-    const int pieces = (a.a.n_head + 2 * a.a.n_head_kv + per_piece - 1) / per_piece;
+template <class Act, class Pool>
+static cudaError_t launch_append(const AppendRulesArgs& a, cudaStream_t stream) {
+    constexpr int heads = 32 * 2 * kGroup<Act> / HD;   // of a piece
+    const int pieces = (a.a.n_head + heads - 1) / heads + 2 * ((a.a.n_head_kv + heads - 1) / heads);
     const int most = (pieces + kPart - 1) / kPart;
     const int parts = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(most, kWarps / a.a.n_tokens)));
     const int64_t blocks = (static_cast<int64_t>(a.a.n_tokens) * parts * 32 + kThreads - 1) / kThreads;
     if (blocks > 0x7fffffffLL) return cudaErrorInvalidConfiguration;
     Launch L(dim3(static_cast<unsigned>(blocks)), kThreads, 0, stream);
+    if (a.q_norm || a.k_norm)
+        return a.halves ? cudaLaunchKernelEx(&L.cfg, append_rules_kernel<Act, Pool, true, true>, a, parts)
+                        : cudaLaunchKernelEx(&L.cfg, append_rules_kernel<Act, Pool, false, true>, a, parts);
+    return a.halves ? cudaLaunchKernelEx(&L.cfg, append_rules_kernel<Act, Pool, true, false>, a, parts)
+                    : cudaLaunchKernelEx(&L.cfg, append_rules_kernel<Act, Pool, false, false>, a, parts);
+}
+
+cudaError_t launch_append_rules(const AppendRulesArgs& a, bool act_bf16, int pool_bytes, cudaStream_t stream) {
     if (act_bf16)
-        return pool_bytes == 1   ? cudaLaunchKernelEx(&L.cfg, append_rules_kernel<__nv_bfloat16, int8_t>, a, parts)
-               : pool_bytes == 2 ? cudaLaunchKernelEx(&L.cfg, append_rules_kernel<__nv_bfloat16, __nv_bfloat16>, a, parts)
-                                 : cudaLaunchKernelEx(&L.cfg, append_rules_kernel<__nv_bfloat16, float>, a, parts);
-    return pool_bytes == 1   ? cudaLaunchKernelEx(&L.cfg, append_rules_kernel<float, int8_t>, a, parts)
-           : pool_bytes == 2 ? cudaLaunchKernelEx(&L.cfg, append_rules_kernel<float, __nv_bfloat16>, a, parts)
-                             : cudaLaunchKernelEx(&L.cfg, append_rules_kernel<float, float>, a, parts);
+        return pool_bytes == 1   ? launch_append<__nv_bfloat16, int8_t>(a, stream)
+               : pool_bytes == 2 ? launch_append<__nv_bfloat16, __nv_bfloat16>(a, stream)
+                                 : launch_append<__nv_bfloat16, float>(a, stream);
+    return pool_bytes == 1   ? launch_append<float, int8_t>(a, stream)
+           : pool_bytes == 2 ? launch_append<float, __nv_bfloat16>(a, stream)
+                             : launch_append<float, float>(a, stream);
 }
 
 cudaError_t launch_read8(const Read8Args& a, bool out_bf16, bool new_only, cudaStream_t stream) {
