@@ -41,7 +41,7 @@ namespace {
 constexpr int kThreads = 64;
 constexpr int kPart = 4;            // pieces of the smallest part of a token
 constexpr int kWarps = 148 * 16;    // below so many tokens their heads are spread over several warps
-constexpr int kBatch = 8;
+constexpr int kBatch = 4;
 
 template <int LANES>
 __device__ __forceinline__ float sum_over(float x) {
@@ -76,20 +76,36 @@ __device__ __forceinline__ void group_of(uint2 u, float (&f)[4]) {
     f[2] = __uint_as_float(u.y << 16);
     f[3] = __uint_as_float(u.y & 0xffff0000u);
 }
+// (4-byte aligned)
+__device__ __forceinline__ void load_norm(const float* p, float (&f)[2]) {
+    f[0] = p[0];
+    f[1] = p[1];
+}
+__device__ __forceinline__ void load_norm(const float* p, float (&f)[4]) {
+    if ((reinterpret_cast<uintptr_t>(p) & 15u) == 0) {
+        const float4 x = *reinterpret_cast<const float4*>(p);
+        f[0] = x.x;
+        f[1] = x.y;
+        f[2] = x.z;
+        f[3] = x.w;
+    } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) f[e] = p[e];
+    }
+}
 template <class T>
 __device__ __forceinline__ void store_group(T* p, const float (&f)[2]) { store_pair(p, make_float2(f[0], f[1])); }
 template <class T>
 __device__ __forceinline__ void store_group(T* p, const float (&f)[4]) { store4(p, f); }
-// Codes of a group; the bounds cut the largest numbers of 32 bits only.
-__device__ __forceinline__ uint32_t code_of(float y, float inv) {
-    return static_cast<uint32_t>(__float2int_rn(fminf(fmaxf(y * inv, -127.f), 127.f))) & 0xffu;
-}
+// Codes of a group, |f| inv <= 127: adding 1.5 * 2^23 rounds to whole numbers, whose low bytes are the codes.
+__device__ __forceinline__ uint32_t code_bits(float y, float inv) { return __float_as_uint(fmaf(y, inv, 12582912.0f)); }
 __device__ __forceinline__ void store_codes(int8_t* p, const float (&f)[2], float inv) {
-    *reinterpret_cast<uint16_t*>(p) = static_cast<uint16_t>(code_of(f[0], inv) | code_of(f[1], inv) << 8);
+    *reinterpret_cast<uint16_t*>(p) = static_cast<uint16_t>(__byte_perm(code_bits(f[0], inv), code_bits(f[1], inv), 0x0040));
 }
 __device__ __forceinline__ void store_codes(int8_t* p, const float (&f)[4], float inv) {
     *reinterpret_cast<uint32_t*>(p) =
-        code_of(f[0], inv) | code_of(f[1], inv) << 8 | code_of(f[2], inv) << 16 | code_of(f[3], inv) << 24;
+        __byte_perm(__byte_perm(code_bits(f[0], inv), code_bits(f[1], inv), 0x0040),
+                    __byte_perm(code_bits(f[2], inv), code_bits(f[3], inv), 0x0040), 0x5410);
 }
 
 template <class Act, class Pool, bool HALF, bool NORM>
@@ -179,11 +195,14 @@ __global__ void __launch_bounds__(kThreads) append_rules_kernel(const __grid_con
                         float ss = 0.f;
 #pragma unroll
                         for (int e = 0; e < GE; ++e) ss = fmaf(y[e], y[e], fmaf(z[e], z[e], ss));
-                        const float f = 1.0f / sqrtf(sum_over<LPH>(ss) * (1.0f / HD) + R.eps);
+                        const float f = rsqrtf(sum_over<LPH>(ss) * (1.0f / HD) + R.eps);
+                        float ny[GE], nz[GE];
+                        load_norm(norm + e1, ny);
+                        load_norm(norm + e2, nz);
 #pragma unroll
                         for (int e = 0; e < GE; ++e) {
-                            y[e] = y[e] * f * norm[e1 + e];
-                            z[e] = z[e] * f * norm[e2 + e];
+                            y[e] = y[e] * f * ny[e];
+                            z[e] = z[e] * f * nz[e];
                         }
                     }
                 }
@@ -213,11 +232,14 @@ __global__ void __launch_bounds__(kThreads) append_rules_kernel(const __grid_con
                 for (int e = 0; e < GE; ++e) most = fmax3(most, fabsf(y[e]), fabsf(z[e]));
                 const int sb = scale_byte(max_over<LPH>(most));
                 if (there && have) {
-                    if (sb == 255) {
-#pragma unroll
-                        for (int e = 0; e < GE; ++e) y[e] = z[e] = 0.f;
-                    }
                     const float inv = __uint_as_float(static_cast<uint32_t>(254 - min(sb, 248)) << 23);
+                    if (sb >= 248) {   // no numbers, or some that may be too large for the largest power of two
+#pragma unroll
+                        for (int e = 0; e < GE; ++e) {
+                            y[e] = sb == 255 ? 0.f : fminf(fmaxf(y[e], -127 * 0x1p121f), 127 * 0x1p121f);
+                            z[e] = sb == 255 ? 0.f : fminf(fmaxf(z[e], -127 * 0x1p121f), 127 * 0x1p121f);
+                        }
+                    }
                     store_codes(to + e1, y, inv);
                     store_codes(to + e2, z, inv);
                     if (hl == 0) (is_v ? R.value_scale : R.key_scale)[row + (static_cast<size_t>(h) << A.page_shift)] = static_cast<uint8_t>(sb);
