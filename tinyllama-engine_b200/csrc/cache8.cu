@@ -274,42 +274,54 @@ __device__ __forceinline__ void store16(__nv_bfloat16* p, const float (&f)[16]) 
 }
 
 // Rows [r0, r0 + n) of one page of the 8-bit pools to rows of k and v
-// (either may be null), 16 elements a thread and step.
+// (either may be null), 16 elements a thread and turn, several turns' loads at once.
 template <class Out>
 __device__ __forceinline__ void read_rows(const Pool8& P, int n_head_kv, int id, int r0, int n, Out* k, int64_t k_stride, Out* v,
                                           int64_t v_stride) {
-    const int per_row = n_head_kv * (HD / 16);
+    constexpr int kTurns = 4;
+    const int per_row = n_head_kv * (HD / 16), total = 2 * n * per_row;
     const bool ok = static_cast<unsigned>(id) < static_cast<unsigned>(P.n_pages);
-    for (int i = threadIdx.x; i < 2 * n * per_row; i += blockDim.x) {
-        const bool val = i >= n * per_row;
-        const int j = val ? i - n * per_row : i;
-        const int r = j / per_row, c = j - r * per_row;
-        Out* dst = val ? v : k;
-        if (!dst) continue;
-        float f[16];
-        if (ok) {
-            const size_t row = ((static_cast<size_t>(id) * n_head_kv + c / 4) << P.page_shift) + r0 + r;
-            from_codes(reinterpret_cast<const uint4*>((val ? P.value_codes : P.key_codes) + row * HD)[c % 4],
-                       (val ? P.value_scale : P.key_scale)[row], f);
-        } else {
+    for (int i0 = threadIdx.x; i0 < total; i0 += kTurns * blockDim.x) {
+        uint4 codes[kTurns];
+        uint8_t scale[kTurns];
+        Out* dst[kTurns];
 #pragma unroll
-            for (int e = 0; e < 16; ++e) f[e] = 0.f;
+        for (int q = 0; q < kTurns; ++q) {
+            const int i = i0 + q * static_cast<int>(blockDim.x);
+            const bool val = i >= n * per_row;
+            const int j = val ? i - n * per_row : i;
+            const int r = j / per_row, c = j - r * per_row;
+            Out* to = i < total ? (val ? v : k) : nullptr;
+            dst[q] = to ? to + r * (val ? v_stride : k_stride) + c * 16 : nullptr;
+            codes[q] = make_uint4(0, 0, 0, 0);
+            scale[q] = 0;
+            if (to && ok) {
+                const size_t row = ((static_cast<size_t>(id) * n_head_kv + c / 4) << P.page_shift) + r0 + r;
+                codes[q] = reinterpret_cast<const uint4*>((val ? P.value_codes : P.key_codes) + row * HD)[c % 4];
+                scale[q] = (val ? P.value_scale : P.key_scale)[row];
+            }
         }
-        store16(dst + r * (val ? v_stride : k_stride) + c * 16, f);
+#pragma unroll
+        for (int q = 0; q < kTurns; ++q) {
+            if (!dst[q]) continue;
+            float f[16];
+            from_codes(codes[q], scale[q], f);
+            store16(dst[q], f);
+        }
     }
 }
 
 constexpr int kReadThreads = 256;
 // The sequences in groups of kReadThreads: thread i of the group has the rows
 // and blocks of rows of its sequence, the shared arrays where they start.
-// f(sequence's ChunkSeq, block in the sequence, block in all, first row in all) for every
-// block b with b % gridDim.x == blockIdx.x; then g(first sequence of the group,
-// starts of its blocks).  Returns the blocks in all.
+// f(sequence's ChunkSeq, block in the sequence, part of it, block in all, first row in all) for every
+// part p (block * PARTS + part of it) with p % gridDim.x == blockIdx.x; then g(first sequence of
+// the group, starts of its blocks).  Returns the blocks in all.
 struct WalkSmem {
     int64_t block0[kReadThreads + 1], row0[kReadThreads + 1];
     int64_t warp_sum[2][kReadThreads / 32];
 };
-template <class Rows, class F, class G>
+template <int PARTS, class Rows, class F, class G>
 __device__ __forceinline__ int64_t walk(WalkSmem& S, const ChunkDesc& d, int n_seqs, int block_rows, Rows&& rows_of, F&& f, G&& g) {
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     int64_t blocks_so_far = 0, rows_so_far = 0;
@@ -341,16 +353,17 @@ __device__ __forceinline__ int64_t walk(WalkSmem& S, const ChunkDesc& d, int n_s
             S.row0[0] = rows_so_far;
         }
         __syncthreads();
-        const int64_t end = S.block0[n];
-        int64_t b = blocks_so_far + (gridDim.x + blockIdx.x - blocks_so_far % gridDim.x) % gridDim.x;
-        for (int lo = 0; b < end; b += gridDim.x) {
+        const int64_t end = S.block0[n], p0 = blocks_so_far * PARTS;
+        int64_t p = p0 + (gridDim.x + blockIdx.x - p0 % gridDim.x) % gridDim.x;
+        for (int lo = 0; p < end * PARTS; p += gridDim.x) {
+            const int64_t b = p / PARTS;
             int hi = n;   // the sequence with block0[lo] <= b < block0[lo + 1]
             while (hi - lo > 1) {
                 const int mid = (lo + hi) / 2;
                 if (S.block0[mid] <= b) lo = mid;
                 else hi = mid;
             }
-            f(d.seqs[s0 + lo], static_cast<int>(b - S.block0[lo]), b, S.row0[lo]);
+            f(d.seqs[s0 + lo], static_cast<int>(b - S.block0[lo]), static_cast<int>(p % PARTS), b, S.row0[lo]);
         }
         g(s0, n, S.block0);
         blocks_so_far = end;
@@ -361,9 +374,14 @@ __device__ __forceinline__ int64_t walk(WalkSmem& S, const ChunkDesc& d, int n_s
 }
 
 // All rows of all sequences, one sequence after another.  HBM-bound.
-constexpr int kReadRows = 64;   // the smallest page
-template <class Out>
-__global__ void __launch_bounds__(kReadThreads) read8_kernel(const __grid_constant__ Read8Args A) {
+constexpr int kReadBlock = 64;       // the smallest page
+// Rows of a part of a block, the unit of a CTA's work: 16, so that small reads reach all SMs (700 rows READ16 us,
+// with 64 READ64 us), or whole blocks where there are several for every CTA (24 x 8000 READBIG).
+constexpr int kReadFew = 16, kReadMany = 64;
+constexpr int kReadCtas = 148 * 5;
+inline bool read_many(int64_t rows) { return rows > int64_t{2} * kReadCtas * kReadMany; }
+template <class Out, int ROWS>
+__global__ void __launch_bounds__(kReadThreads, 5) read8_kernel(const __grid_constant__ Read8Args A) {
     __shared__ WalkSmem S;
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     asm volatile("griddepcontrol.wait;" ::: "memory");
@@ -371,13 +389,14 @@ __global__ void __launch_bounds__(kReadThreads) read8_kernel(const __grid_consta
         if (threadIdx.x == 0) record_error(A.err, kErrBadDesc);
         return;
     }
-    walk(
-        S, A.d, A.n_seqs, kReadRows, [](const ChunkSeq& s) { return s.n_tokens > 0 ? static_cast<int64_t>(s.pos) + s.n_tokens : 0; },
-        [&](const ChunkSeq& s, int block, int64_t, int64_t row0) {
-            const int r = block * kReadRows;
+    walk<kReadBlock / ROWS>(
+        S, A.d, A.n_seqs, kReadBlock, [](const ChunkSeq& s) { return s.n_tokens > 0 ? static_cast<int64_t>(s.pos) + s.n_tokens : 0; },
+        [&](const ChunkSeq& s, int block, int part, int64_t, int64_t row0) {
+            const int r = block * kReadBlock + part * ROWS;
             const int64_t at = row0 + r;
-            const int n = static_cast<int>(min(static_cast<int64_t>(min(kReadRows, s.pos + s.n_tokens - r)), A.n_rows - at));
-            if (n < min(kReadRows, s.pos + s.n_tokens - r) && threadIdx.x == 0) record_error(A.err, kErrRoom);
+            const int there = min(ROWS, s.pos + s.n_tokens - r);
+            const int n = static_cast<int>(min(static_cast<int64_t>(there), A.n_rows - at));
+            if (n < there && threadIdx.x == 0) record_error(A.err, kErrRoom);
             if (n <= 0) return;
             const int id = s.pages[r >> A.pool.page_shift];
             if (threadIdx.x == 0 && static_cast<unsigned>(id) >= static_cast<unsigned>(A.pool.n_pages)) record_error(A.err, kErrBadPage);
@@ -422,7 +441,8 @@ __global__ void __launch_bounds__(kReadThreads) read8_new_kernel(const __grid_co
 // not take) as bf16 pages of kStageRows rows, and a copy of the descriptor's
 // first records with page tables that lead to them, for the attention over
 // bf16 pages.  Nothing is rounded: the stored values are bf16 numbers.
-__global__ void __launch_bounds__(kReadThreads) stage8_kernel(const __grid_constant__ Stage8Args A) {
+template <int ROWS>
+__global__ void __launch_bounds__(kReadThreads, 5) stage8_kernel(const __grid_constant__ Stage8Args A) {
     __shared__ WalkSmem S;
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     asm volatile("griddepcontrol.wait;" ::: "memory");
@@ -435,23 +455,20 @@ __global__ void __launch_bounds__(kReadThreads) stage8_kernel(const __grid_const
         return;
     }
     const size_t row_halfs = static_cast<size_t>(A.n_head_kv) * HD;
-    const int64_t total = walk(
+    const int64_t total = walk<kStageRows / ROWS>(
         S, A.d, A.n_seqs, kStageRows,
         [&](const ChunkSeq& s) {
             return static_cast<int64_t>(s.n_tokens) * A.group > kChunkFewRows ? static_cast<int64_t>(s.pos) + s.n_tokens : 0;
         },
-        [&](const ChunkSeq& s, int block, int64_t at, int64_t) {
+        [&](const ChunkSeq& s, int block, int part, int64_t at, int64_t) {
             if (at >= A.n_pages) return;
-            if (threadIdx.x == 0) A.table[at] = static_cast<int32_t>(at);
-            for (int half = 0; half < kStageRows; half += kReadRows) {
-                const int r = block * kStageRows + half;
-                const int n = min(kReadRows, s.pos + s.n_tokens - r);
-                if (n <= 0) break;
-                const int id = s.pages[r >> A.pool.page_shift];
-                if (threadIdx.x == 0 && static_cast<unsigned>(id) >= static_cast<unsigned>(A.pool.n_pages)) record_error(A.err, kErrBadPage);
-                const size_t to = (static_cast<size_t>(at) * kStageRows + half) * row_halfs;
-                read_rows(A.pool, A.n_head_kv, id, r & ((1 << A.pool.page_shift) - 1), n, A.k + to, row_halfs, A.v + to, row_halfs);
-            }
+            if (part == 0 && threadIdx.x == 0) A.table[at] = static_cast<int32_t>(at);
+            const int r = block * kStageRows + part * ROWS, n = min(ROWS, s.pos + s.n_tokens - r);
+            if (n <= 0) return;
+            const int id = s.pages[r >> A.pool.page_shift];
+            if (threadIdx.x == 0 && static_cast<unsigned>(id) >= static_cast<unsigned>(A.pool.n_pages)) record_error(A.err, kErrBadPage);
+            const size_t to = (static_cast<size_t>(at) * kStageRows + part * ROWS) * row_halfs;
+            read_rows(A.pool, A.n_head_kv, id, r & ((1 << A.pool.page_shift) - 1), n, A.k + to, row_halfs, A.v + to, row_halfs);
         },
         [&](int s0, int n, const int64_t* block0) {
             const int n_rec = A.n_ctas + A.n_segs;   // cta records and segments are one array
@@ -508,15 +525,23 @@ cudaError_t launch_read8(const Read8Args& a, bool out_bf16, bool new_only, cudaS
         return out_bf16 ? cudaLaunchKernelEx(&L.cfg, read8_new_kernel<__nv_bfloat16>, a)
                         : cudaLaunchKernelEx(&L.cfg, read8_new_kernel<float>, a);
     }
-    const int64_t blocks = std::min<int64_t>(148 * 8, a.n_rows / kReadRows + a.n_seqs);
-    Launch L(dim3(static_cast<unsigned>(blocks)), kReadThreads, 0, stream);
-    return out_bf16 ? cudaLaunchKernelEx(&L.cfg, read8_kernel<__nv_bfloat16>, a) : cudaLaunchKernelEx(&L.cfg, read8_kernel<float>, a);
+    auto go = [&](auto kernel, int rows) {
+        const int64_t blocks = std::min<int64_t>(kReadCtas, a.n_rows / rows + a.n_seqs);
+        Launch L(dim3(static_cast<unsigned>(blocks)), kReadThreads, 0, stream);
+        return cudaLaunchKernelEx(&L.cfg, kernel, a);
+    };
+    if (read_many(a.n_rows))
+        return out_bf16 ? go(read8_kernel<__nv_bfloat16, kReadMany>, kReadMany) : go(read8_kernel<float, kReadMany>, kReadMany);
+    return out_bf16 ? go(read8_kernel<__nv_bfloat16, kReadFew>, kReadFew) : go(read8_kernel<float, kReadFew>, kReadFew);
 }
 
 cudaError_t launch_stage8(const Stage8Args& a, cudaStream_t stream) {
-    const int64_t blocks = std::min<int64_t>(148 * 8, std::max<int64_t>(a.n_pages, 1));
-    Launch L(dim3(static_cast<unsigned>(blocks)), kReadThreads, 0, stream);
-    return cudaLaunchKernelEx(&L.cfg, stage8_kernel, a);
+    const int64_t rows = a.n_pages * kStageRows;   // at most: what the workspace has room for
+    auto go = [&](auto kernel, int per) {
+        Launch L(dim3(static_cast<unsigned>(std::min<int64_t>(kReadCtas, std::max<int64_t>(rows / per, 1)))), kReadThreads, 0, stream);
+        return cudaLaunchKernelEx(&L.cfg, kernel, a);
+    };
+    return read_many(rows) ? go(stage8_kernel<kReadMany>, kReadMany) : go(stage8_kernel<kReadFew>, kReadFew);
 }
 
 }  // namespace tle
