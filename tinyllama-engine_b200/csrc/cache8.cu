@@ -256,57 +256,72 @@ __global__ void __launch_bounds__(kThreads) append_rules_kernel(const __grid_con
 }
 
 // ---- read -------------------------------------------------------------------
-// 16 codes and their row's byte to 16 numbers.
-__device__ __forceinline__ void from_codes(const uint4 c, uint8_t b, float (&f)[16]) {
+// Codes and their row's byte to 16 bytes of numbers: 4 (fp32) or 8 (bf16).
+template <class Out>
+constexpr int kPer = 16 / sizeof(Out);
+__device__ __forceinline__ float number(uint32_t u, int i, float scale) {   // u: codes with their signs flipped
+    // 2^23 + (n + 128), whose low byte is the code
+    return (__uint_as_float(__byte_perm(u, 0x4B000000u, 0x7650 | i)) - 8388736.0f) * scale;
+}
+__device__ __forceinline__ void store_numbers(float* p, uint32_t c, uint8_t b) {
     const float s = __uint_as_float(static_cast<uint32_t>(b) << 23);   // 255: infinity, 0 * inf = NaN
-    const uint32_t u[4] = {c.x ^ 0x80808080u, c.y ^ 0x80808080u, c.z ^ 0x80808080u, c.w ^ 0x80808080u};
-#pragma unroll
-    for (int i = 0; i < 16; ++i)   // 2^23 + (n + 128), whose low byte is the code
-        f[i] = (__uint_as_float(__byte_perm(u[i / 4], 0x4B000000u, 0x7650 | (i % 4))) - 8388736.0f) * s;
+    const uint32_t u = c ^ 0x80808080u;
+    *reinterpret_cast<float4*>(p) = make_float4(number(u, 0, s), number(u, 1, s), number(u, 2, s), number(u, 3, s));
 }
-__device__ __forceinline__ void store16(float* p, const float (&f)[16]) {
-#pragma unroll
-    for (int i = 0; i < 16; i += 4) store4(p + i, f + i);
+__device__ __forceinline__ void store_numbers(__nv_bfloat16* p, uint2 c, uint8_t b) {
+    const float s = __uint_as_float(static_cast<uint32_t>(b) << 23);
+    const uint32_t u = c.x ^ 0x80808080u, w = c.y ^ 0x80808080u;
+    *reinterpret_cast<uint4*>(p) =
+        make_uint4(pack_bf16(number(u, 0, s), number(u, 1, s)), pack_bf16(number(u, 2, s), number(u, 3, s)),
+                   pack_bf16(number(w, 0, s), number(w, 1, s)), pack_bf16(number(w, 2, s), number(w, 3, s)));
 }
-__device__ __forceinline__ void store16(__nv_bfloat16* p, const float (&f)[16]) {
-    store8(p, f);
-    store8(p + 8, f + 8);
-}
+template <class Out>
+using Codes = std::conditional_t<sizeof(Out) == 4, uint32_t, uint2>;
 
-// Rows [r0, r0 + n) of one page of the 8-bit pools to rows of k and v
-// (either may be null), 16 elements a thread and turn, several turns' loads at once.
+// Rows [r0, r0 + n) of one page of the 8-bit pools to rows of k and v (either
+// may be null): whole rows are stored by consecutive lanes, K and V and several turns at once.
 template <class Out>
 __device__ __forceinline__ void read_rows(const Pool8& P, int n_head_kv, int id, int r0, int n, Out* k, int64_t k_stride, Out* v,
                                           int64_t v_stride) {
-    constexpr int kTurns = 4;
-    const int per_row = n_head_kv * (HD / 16), total = 2 * n * per_row;
+    constexpr int kTurns = 4, kHead = HD / kPer<Out>;   // pieces of a head
+    const int per_row = n_head_kv * kHead, threads = blockDim.x;
     const bool ok = static_cast<unsigned>(id) < static_cast<unsigned>(P.n_pages);
-    for (int i0 = threadIdx.x; i0 < total; i0 += kTurns * blockDim.x) {
-        uint4 codes[kTurns];
-        uint8_t scale[kTurns];
-        Out* dst[kTurns];
+    const size_t first = ((static_cast<size_t>(ok ? id : 0) * n_head_kv) << P.page_shift) + r0;
+    const int dr = threads / per_row, dc = threads - dr * per_row;
+    int r = threadIdx.x / per_row, c = threadIdx.x - r * per_row;
+    while (r < n) {
+        Codes<Out> kc[kTurns], vc[kTurns];
+        uint8_t ks[kTurns], vs[kTurns];
+        int rr[kTurns], cc[kTurns];
 #pragma unroll
         for (int q = 0; q < kTurns; ++q) {
-            const int i = i0 + q * static_cast<int>(blockDim.x);
-            const bool val = i >= n * per_row;
-            const int j = val ? i - n * per_row : i;
-            const int r = j / per_row, c = j - r * per_row;
-            Out* to = i < total ? (val ? v : k) : nullptr;
-            dst[q] = to ? to + r * (val ? v_stride : k_stride) + c * 16 : nullptr;
-            codes[q] = make_uint4(0, 0, 0, 0);
-            scale[q] = 0;
-            if (to && ok) {
-                const size_t row = ((static_cast<size_t>(id) * n_head_kv + c / 4) << P.page_shift) + r0 + r;
-                codes[q] = reinterpret_cast<const uint4*>((val ? P.value_codes : P.key_codes) + row * HD)[c % 4];
-                scale[q] = (val ? P.value_scale : P.key_scale)[row];
+            rr[q] = r;
+            cc[q] = c;
+            kc[q] = vc[q] = Codes<Out>{};
+            ks[q] = vs[q] = 0;
+            if (r < n && ok) {
+                const size_t row = first + (static_cast<size_t>(c / kHead) << P.page_shift) + r;
+                if (k) {
+                    kc[q] = reinterpret_cast<const Codes<Out>*>(P.key_codes + row * HD)[c % kHead];
+                    ks[q] = P.key_scale[row];
+                }
+                if (v) {
+                    vc[q] = reinterpret_cast<const Codes<Out>*>(P.value_codes + row * HD)[c % kHead];
+                    vs[q] = P.value_scale[row];
+                }
+            }
+            r += dr;
+            c += dc;
+            if (c >= per_row) {
+                c -= per_row;
+                ++r;
             }
         }
 #pragma unroll
         for (int q = 0; q < kTurns; ++q) {
-            if (!dst[q]) continue;
-            float f[16];
-            from_codes(codes[q], scale[q], f);
-            store16(dst[q], f);
+            if (rr[q] >= n) continue;
+            if (k) store_numbers(k + rr[q] * k_stride + cc[q] * kPer<Out>, kc[q], ks[q]);
+            if (v) store_numbers(v + rr[q] * v_stride + cc[q] * kPer<Out>, vc[q], vs[q]);
         }
     }
 }
@@ -407,7 +422,7 @@ __global__ void __launch_bounds__(kReadThreads, 5) read8_kernel(const __grid_con
         [](int, int, const int64_t*) {});
 }
 
-// The rows of the batch's new tokens, 16 elements a thread.
+// The rows of the batch's new tokens, 16 bytes of numbers a thread.
 template <class Out>
 __global__ void __launch_bounds__(kReadThreads) read8_new_kernel(const __grid_constant__ Read8Args A) {
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
@@ -416,25 +431,32 @@ __global__ void __launch_bounds__(kReadThreads) read8_new_kernel(const __grid_co
         if (threadIdx.x == 0) record_error(A.err, kErrBadDesc);
         return;
     }
-    const int per_row = A.n_head_kv * (HD / 16);
-    const int64_t i = static_cast<int64_t>(blockIdx.x) * kReadThreads + threadIdx.x;
-    const int64_t tok = i / per_row;
+    constexpr int kHead = HD / kPer<Out>;
+    const uint32_t per_row = A.n_head_kv * kHead;
+    const int64_t i0 = static_cast<int64_t>(blockIdx.x) * kReadThreads;
+    const int64_t tok0 = i0 / per_row;
+    const uint32_t in = static_cast<uint32_t>(i0 - tok0 * per_row) + threadIdx.x, more = in / per_row;
+    const int64_t tok = tok0 + more;
     if (tok >= A.n_tokens) return;
-    const int c = static_cast<int>(i - tok * per_row);
+    const uint32_t c = in - more * per_row;
     const ChunkTok tk = A.d.toks[tok];
     const int id = A.d.seqs[tk.seq].pages[tk.pos >> A.pool.page_shift];
     const bool ok = static_cast<unsigned>(id) < static_cast<unsigned>(A.pool.n_pages);
     if (!ok) record_error(A.err, kErrBadPage);
-    const size_t row = ok ? ((static_cast<size_t>(id) * A.n_head_kv + c / 4) << A.pool.page_shift) +
+    const size_t row = ok ? ((static_cast<size_t>(id) * A.n_head_kv + c / kHead) << A.pool.page_shift) +
                                 (tk.pos & ((1 << A.pool.page_shift) - 1)) : 0;
-    auto one = [&](const int8_t* codes, const uint8_t* scale, void* out, int64_t stride) {
-        if (!out) return;
-        float f[16];
-        from_codes(reinterpret_cast<const uint4*>(codes + row * HD)[c % 4], ok ? scale[row] : 0, f);
-        store16(static_cast<Out*>(out) + tok * stride + c * 16, f);
-    };
-    one(A.pool.key_codes, A.pool.key_scale, A.k, A.k_stride);
-    one(A.pool.value_codes, A.pool.value_scale, A.v, A.v_stride);
+    Codes<Out> kc{}, vc{};
+    uint8_t ks = 0, vs = 0;
+    if (ok && A.k) {
+        kc = reinterpret_cast<const Codes<Out>*>(A.pool.key_codes + row * HD)[c % kHead];
+        ks = A.pool.key_scale[row];
+    }
+    if (ok && A.v) {
+        vc = reinterpret_cast<const Codes<Out>*>(A.pool.value_codes + row * HD)[c % kHead];
+        vs = A.pool.value_scale[row];
+    }
+    if (A.k) store_numbers(static_cast<Out*>(A.k) + tok * A.k_stride + c * kPer<Out>, kc, ks);
+    if (A.v) store_numbers(static_cast<Out*>(A.v) + tok * A.v_stride + c * kPer<Out>, vc, vs);
 }
 
 // The rows of the sequences of many rows (those that chunk_few8_kernel does
@@ -519,7 +541,7 @@ cudaError_t launch_append_rules(const AppendRulesArgs& a, bool act_bf16, int poo
 
 cudaError_t launch_read8(const Read8Args& a, bool out_bf16, bool new_only, cudaStream_t stream) {
     if (new_only) {
-        const int64_t blocks = (static_cast<int64_t>(a.n_tokens) * a.n_head_kv * (HD / 16) + kReadThreads - 1) / kReadThreads;
+        const int64_t blocks = (static_cast<int64_t>(a.n_tokens) * a.n_head_kv * (HD / (out_bf16 ? 8 : 4)) + kReadThreads - 1) / kReadThreads;
         if (blocks > 0x7fffffffLL) return cudaErrorInvalidConfiguration;
         Launch L(dim3(static_cast<unsigned>(blocks)), kReadThreads, 0, stream);
         return out_bf16 ? cudaLaunchKernelEx(&L.cfg, read8_new_kernel<__nv_bfloat16>, a)
