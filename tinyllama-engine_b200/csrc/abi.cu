@@ -2140,6 +2140,8 @@ int tle_prefill_q8_paged(const tle_shape_t* shape, const tle_page_pool_q8_t* poo
     if (int rc = check_chunk_pool(shape, plan, pool->key_codes, pool->value_codes, pool->n_pages, pool->page_rows, 64, &shift))
         return rc;
     if (plan->n_tokens == 0) return ok();
+    if (static_cast<int64_t>(pool->n_pages) * shape->n_head_kv > INT32_MAX)
+        return set_error(TLE_ERR_UNSUPPORTED, "%d pages of %d KV heads: more than 2^31 in all", pool->n_pages, shape->n_head_kv);
     if (int rc = check_rows(q, q_stride, shape->n_head, "q")) return rc;
     if (int rc = check_rows(out, out_stride, shape->n_head, "out")) return rc;
     if (out == q && out_stride != q_stride && plan->n_tokens > 1) return set_error(TLE_ERR_INVALID, "out is q, with another stride");
