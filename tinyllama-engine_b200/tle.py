@@ -307,7 +307,7 @@ def _raw_stream(stream, index: int) -> int:
     return stream.cuda_stream
 
 
-def _on_device(index: int, fn, *args) -> None:
+def _on_device(index: int, fn, args) -> None:
     """fn(*args), checked, with device `index` current."""
     global _current_device
     if _current_device is None:
@@ -840,6 +840,7 @@ class PagedChunkBatch:
         else:
             nbytes = L.tle_prefill_bf16_paged_workspace_bytes(ctypes.byref(plan))
         self.plan, self._ws_bytes = plan, nbytes
+        self._plan_ref, self._n_tokens = ctypes.byref(plan), plan.n_tokens
         return host[:plan.desc_bytes]
 
     def set_positions(self, positions: Sequence[int], lengths: Sequence[int], stream=None) -> None:
@@ -856,6 +857,7 @@ class PagedChunkBatch:
                 if self.workspace is None or self.workspace.numel() * 4 < nbytes:
                     self.workspace = torch.empty(self._room(max(-(-nbytes // 4), 4), self.workspace), dtype=torch.float32,
                                                  device=self.device)
+                    self._room_bytes = self.workspace.numel() * 4
                     self._streams.clear()
                 if self._desc_dev is None or self._desc_dev.numel() < host.numel():
                     # with room for the plans of later positions; the old one may be in a graph
@@ -886,7 +888,8 @@ class PagedChunkBatch:
         """Pointer and row stride of an activation tensor of at least n rows of
         w (None: the plan's tokens)."""
         shape, strides = t.shape, t.stride()
-        n = self.plan.n_tokens if n is None else n
+        if n is None:
+            n = self._n_tokens
         if t.dtype is not dtype:
             raise ValueError(f"{name}: activations are all float32 or all bfloat16, got {t.dtype}")
         if t.get_device() != self._index:
@@ -904,18 +907,19 @@ class PagedChunkBatch:
         return act
 
     def _pool(self):
-        """The cache's tle_page_pool_t, one structure for all calls, with the
-        pools' places as they are now."""
+        """Address of the cache's tle_page_pool_t, one structure for all calls,
+        with the pools' places as they are now."""
         c, pool = self.cache, self._pool_made
         if pool is None:
             pool = self._pool_made = c.pool()
+            self._pool_at = ctypes.addressof(pool)
         if self._q8:
             pool.key_codes, pool.value_codes = c.key_pool.data_ptr(), c.value_pool.data_ptr()
             pool.key_scale, pool.value_scale = c.key_scale.data_ptr(), c.value_scale.data_ptr()
-            return pool
+            return self._pool_at
         pool.key_pool = c.key_pool.data_ptr()
         pool.value_pool = c.value_pool.data_ptr()
-        return pool
+        return self._pool_at
 
     def _on(self, stream) -> int:
         """Handle of the stream; the batch's buffers are kept from reuse until
@@ -952,17 +956,17 @@ class PagedChunkBatch:
             raise ValueError("q_out without q")
         L = lib()
         pool = self._pool()
+        flags = TLE_DECODE_ROTATE if rotate else 0
         if rules is not None or self._q8:
-            if rules is not None and rules.index not in (None, self._index):
+            if rules is not None and rules.index != self._index and rules.index is not None:
                 raise ValueError(f"rules: are on cuda:{rules.index}, the cache on {self.device}")
             fn = L.tle_append_q8_paged if self._q8 else L.tle_append_rules_bf16_paged if self._bf16 else L.tle_append_rules_paged
-            _on_device(self._index, fn, self._shape_ref, ctypes.addressof(pool), ctypes.byref(self.plan),
-                       self._desc_dev.data_ptr(), qp, qs, kp, ks, vp, vs, qo, act, layer,
-                       TLE_DECODE_ROTATE if rotate else 0, None if rules is None else rules.desc_at, self._on(stream))
+            _on_device(self._index, fn, (self._shape_ref, pool, self._plan_ref, self._desc_dev.data_ptr(), qp, qs, kp, ks, vp, vs,
+                                         qo, act, layer, flags, None if rules is None else rules.desc_at, self._on(stream)))
             return
-        _on_device(self._index, L.tle_append_bf16_paged if self._bf16 else L.tle_append_paged, self._shape_ref,
-                   ctypes.addressof(pool), ctypes.byref(self.plan), self._desc_dev.data_ptr(), qp, qs, kp, ks, vp, vs,
-                   qo, act, layer, TLE_DECODE_ROTATE if rotate else 0, self._on(stream))
+        _on_device(self._index, L.tle_append_bf16_paged if self._bf16 else L.tle_append_paged,
+                   (self._shape_ref, pool, self._plan_ref, self._desc_dev.data_ptr(), qp, qs, kp, ks, vp, vs, qo, act, layer, flags,
+                    self._on(stream)))
 
     def attend(self, q, out, layer: int, stream=None) -> None:
         """Causal attention of the chunks (q already rotated) over a bf16 or
@@ -974,9 +978,10 @@ class PagedChunkBatch:
         qp, qs = self._rows(q, self._widths[0], "q", q.dtype)
         op, os = self._rows(out, self._widths[0], "out", q.dtype)
         pool = self._pool()
-        _on_device(self._index, lib().tle_prefill_q8_paged if self._q8 else lib().tle_prefill_bf16_paged, self._shape_ref,
-                   ctypes.addressof(pool), ctypes.byref(self.plan), self._desc_dev.data_ptr(), qp, qs, op, os, act, layer,
-                   self.workspace.data_ptr(), self.workspace.numel() * 4, self._on(stream))
+        L = lib()
+        _on_device(self._index, L.tle_prefill_q8_paged if self._q8 else L.tle_prefill_bf16_paged,
+                   (self._shape_ref, pool, self._plan_ref, self._desc_dev.data_ptr(), qp, qs, op, os, act, layer,
+                    self.workspace.data_ptr(), self._room_bytes, self._on(stream)))
 
     def read(self, k_out, v_out, layer: int, new_only: bool = False, stream=None) -> None:
         """The rows of an 8-bit cache as numbers (tle_read_q8_paged), exactly:
@@ -986,7 +991,7 @@ class PagedChunkBatch:
         both bfloat16, any row stride that is a multiple of 8; either may be None."""
         if not self._q8:
             raise ValueError("read: an int8 PagedKVCache expected")
-        n = self.plan.n_tokens if new_only else self.n_rows
+        n = self._n_tokens if new_only else self.n_rows
         given = [t for t in (k_out, v_out) if t is not None]
         if not given:
             raise ValueError("read: k_out, v_out or both")
@@ -994,9 +999,9 @@ class PagedChunkBatch:
         kp, ks = (None, 0) if k_out is None else self._rows(k_out, w, "k_out", given[0].dtype, n)
         vp, vs = (None, 0) if v_out is None else self._rows(v_out, w, "v_out", given[0].dtype, n)
         pool = self._pool()
-        _on_device(self._index, lib().tle_read_q8_paged, self._shape_ref, ctypes.addressof(pool), ctypes.byref(self.plan),
-                   self._desc_dev.data_ptr(), kp, ks, vp, vs, n, act, layer, TLE_READ_NEW if new_only else 0,
-                   self._on(stream))
+        _on_device(self._index, lib().tle_read_q8_paged,
+                   (self._shape_ref, pool, self._plan_ref, self._desc_dev.data_ptr(), kp, ks, vp, vs, n, act, layer,
+                    TLE_READ_NEW if new_only else 0, self._on(stream)))
 
     def run(self, q, k, v, out, layer: int, rotate: bool = True, stream=None,
             rules: Optional["AppendRules"] = None) -> None:
@@ -1236,8 +1241,8 @@ def logits_adjust(out, logits, rules: LogitRules, stream=None) -> None:
     index = rules.index if rules.index is not None else logits.get_device()
     op, os = rules._rows(out, index, "out")
     lp, ls = rules._rows(logits, index, "logits")
-    _on_device(index, lib().tle_logits_adjust, op, os, lp, ls, rules.n_rows, rules.n_vocab, rules.desc_ref,
-               _raw_stream(stream, index))
+    _on_device(index, lib().tle_logits_adjust, (op, os, lp, ls, rules.n_rows, rules.n_vocab, rules.desc_ref,
+                                                _raw_stream(stream, index)))
 
 
 class SampleRules:
@@ -1290,8 +1295,8 @@ def sample_rows(tokens_out, logits, rules: SampleRules, uniform, stream=None) ->
         raise ValueError(f"logits: is on {logits.device}, need " + (f"cuda:{index}" if index >= 0 else "a CUDA device"))
     tp = rules._row_numbers(tokens_out, index, "tokens_out", rules._i32)
     up = rules._row_numbers(uniform, index, "uniform", rules._f32)
-    _on_device(index, lib().tle_sample_rows, tp, logits.data_ptr(), strides[0] if n > 1 else v, n, v, rules.desc_ref, up,
-               _raw_stream(stream, index))
+    _on_device(index, lib().tle_sample_rows, (tp, logits.data_ptr(), strides[0] if n > 1 else v, n, v, rules.desc_ref, up,
+                                              _raw_stream(stream, index)))
 
 
 class DeviceModel:
