@@ -119,6 +119,7 @@ struct alignas(16) Shared {                // the slice lies behind it
     uint32_t list[2][kList];               // of two searches in turn: this CTA's keys of the bin in question
     uint32_t count[2][kRowCtas];           // how many each CTA has
     uint32_t mine;
+    uint32_t n_last[2], last_key[kFew], last_at[kFew];   // rank 0: what is left of the row, if that is few
     uint64_t slot[2][2][kRowCtas];         // what the CTAs of the cluster told each other, by turns
     double powers[64];
     uint64_t warp_sum[kWarps];
@@ -176,6 +177,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int64_t row = blockIdx.x / cl.n;
     if (tid < 64) S.powers[tid] = kPowers.v[tid];
+    if (tid < 2) S.n_last[tid] = 0;
     const int v0 = cl.rank * A.slice, n = max(0, min(A.slice, A.n_vocab - v0));
     // ---- the slice into shared memory, its largest logit ----
     const float* src = A.logits + row * A.stride + v0;
@@ -228,6 +230,14 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
         if (cl.rank == 0 && tid == 0) A.tokens[row] = -1;
         return;
     }
+    // the weight that top-p asks for of a sum, and the place of the drawn number in one
+    auto want_of_p = [&](uint64_t all) {
+        const double t = ceil(static_cast<double>(fmaxf(top_p, 0.f)) * static_cast<double>(all));
+        return min(max(static_cast<uint64_t>(t), static_cast<uint64_t>(1)), all);
+    };
+    auto number_of = [&](uint64_t all) {
+        return min(static_cast<uint64_t>(static_cast<double>(u > 0.f ? fminf(u, 1.0f) : 0.f) * static_cast<double>(all)), all - 1);
+    };
     // a part of the slice for each warp, in order; `have` of its tokens are left in x and id
     const int part = (A.slice + kWarps - 1) / kWarps, p0 = min(n, warp * part);
     int have = min(n - p0, part);
@@ -274,16 +284,53 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
         whole = false;
     };
     uint64_t left = ~0ull;                     // tokens left in all CTAs at most, once something was dropped
-    auto count_left = [&]() {                  // a barrier of the cluster
+    // The tokens left to rank 0, as far as there is room (try 0 or 1), before a barrier of the cluster.
+    auto hand_over = [&](int turn) {
+        if (have == 0) return;
+        uint32_t to = 0;
+        if (lane == 0) to = atomicAdd(cl.g.map_shared_rank(&S.n_last[turn], 0), static_cast<uint32_t>(have));
+        to = __shfl_sync(0xffffffffu, to, 0);
+        for (int i = lane; i < have && to + i < kFew; i += 32) {
+            *cl.g.map_shared_rank(&S.last_key[to + i], 0) = key_of(x_of[i]);
+            *cl.g.map_shared_rank(&S.last_at[to + i], 0) = static_cast<uint32_t>(v0 + p0 + id_of[i]);
+        }
+    };
+    // The row's token from its last n <= kFew tokens, by rank 0: everything by comparing all pairs, four threads a token.
+    auto finish = [&](uint32_t n) {
+        static_assert(4 * kFew == kThreads, "four threads a token");
+        uint64_t* kept = S.weight;             // weights of the tokens that pass the filters so far
+        uint64_t* kept2 = S.weight + kFew;
+        const uint32_t i = tid >> 2, key = i < n ? S.last_key[i] : 0, at = i < n ? S.last_at[i] : 0;
+        const uint64_t w = i < n ? R.weight(of_key(key)) : 0;
+        auto sum4 = [](auto x) {
+            x += __shfl_xor_sync(0xffffffffu, x, 1);
+            return x + __shfl_xor_sync(0xffffffffu, x, 2);
+        };
+        auto before = [&](uint32_t j) { return S.last_key[j] > key || (S.last_key[j] == key && S.last_at[j] < at); };
+        uint32_t rank = 0;
+        for (uint32_t j = tid & 3; j < n; j += 4) rank += before(j);
+        rank = sum4(rank);
+        __syncthreads();                       // the weights' place may have held something else
+        if ((tid & 3) == 0) kept[i] = k == 0 || rank < static_cast<uint32_t>(k) ? w : 0;
         __syncthreads();
-        if (lane == 0) S.warp_sum[warp] = have;
+        uint64_t above = 0, all = 0;
+        for (uint32_t j = tid & 3; j < n; j += 4) {
+            above += before(j) ? kept[j] : 0;
+            all += kept[j];
+        }
+        above = sum4(above);
+        all = sum4(all);
+        if ((tid & 3) == 0) kept2[i] = top_p < 1.0f && above >= want_of_p(all) ? 0 : kept[i];
         __syncthreads();
-        uint64_t sum = 0;
-        for (int w = 0; w < kWarps; ++w) sum += S.warp_sum[w];
-        const auto s = cl.tell(sum);
-        uint64_t all = 0;
-        for (int i = 0; i < cl.n; ++i) all += s[0][i];
-        return all;
+        uint64_t run = 0, sum = 0;
+        for (uint32_t j = tid & 3; j < n; j += 4) {
+            run += S.last_at[j] < at ? kept2[j] : 0;
+            sum += kept2[j];
+        }
+        run = sum4(run);
+        sum = sum4(sum);
+        const uint64_t drawn = number_of(sum);
+        if ((tid & 3) == 0 && i < n && run <= drawn && drawn < run + kept2[i]) A.tokens[row] = static_cast<int32_t>(at);
     };
     int searches = 0;
     // The cut at which the ranking's count (WEIGHT: sum of weights) within reach (the others weigh nothing) with a
@@ -348,24 +395,6 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
             const uint32_t to = atomicAdd(&S.mine, 1u);
             if (to < kList) S.list[turn][to] = key;
         };
-        if (left <= kFew) {
-            __syncthreads();
-            if (tid == 0) S.mine = 0;
-            __syncthreads();
-            for (int i = lane; i < have; i += 32) {
-                const float x = x_of[i];
-                const uint32_t key = key_of(x);
-                if (in(x, key)) list_key(key);
-            }
-            const uint32_t all = gather();
-            uint64_t sum = 0;
-            for (uint32_t q = lane; q < all; q += 32) sum += S.weight[q];
-            for (int d = 1; d < 32; d *= 2) sum += __shfl_xor_sync(0xffffffffu, sum, d);
-            want = want_of(sum);
-            if (want == 0 || want > sum) return false;
-            rank(all);
-            return true;
-        }
         for (int level = 0;; ++level) {
             auto bin_of = [&](float x, uint32_t key) { return level == 0 ? by_logit(x) : static_cast<int>((hi - key) >> shift); };
             __syncthreads();
@@ -444,6 +473,12 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
                     return true;
                 }
             }
+            if (!WEIGHT && level == 0 && left <= kFew) {   // what the row's token will be one of
+                keep([&](float x) { return R.in_reach(x) && by_logit(x) <= bin; });
+                hand_over(1);
+                cl.g.sync();
+                return true;
+            }
             // ---- the bin's tokens, if they are few, ranked one by one; those behind it dropped ----
             if (level == 0) {
                 keep([&](float x) {
@@ -487,12 +522,31 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
         }
     };
     // where min-p leaves a narrow range, what is outside goes first
-    if (min_p > 0.f && (k > 0 || top_p < 1.0f)) {
+    if (min_p > 0.f) {
         keep([&](float x) { return R.in_reach(x); });
-        left = count_left();
+        hand_over(0);
+        __syncthreads();
+        if (lane == 0) S.warp_sum[warp] = have;
+        __syncthreads();
+        uint64_t mine = 0;
+        for (int w = 0; w < kWarps; ++w) mine += S.warp_sum[w];
+        const auto s = cl.tell(mine);
+        left = 0;
+        for (int i = 0; i < cl.n; ++i) left += s[0][i];
+        if (left <= kFew) {
+            if (cl.rank == 0) finish(static_cast<uint32_t>(left));
+            return;
+        }
     }
     Cut cut{0, 0};
-    if (k > 0 && static_cast<uint64_t>(k) < left) search.template operator()<false>(0, [&](uint64_t) { return static_cast<uint64_t>(k); }, cut);
+    if (k > 0 && static_cast<uint64_t>(k) < left) {
+        left = ~0ull;
+        search.template operator()<false>(0, [&](uint64_t) { return static_cast<uint64_t>(k); }, cut);
+        if (left <= kFew) {
+            if (cl.rank == 0) finish(static_cast<uint32_t>(left));
+            return;
+        }
+    }
     if (top_p < 1.0f) {
         const uint64_t tie_w = cut.ties ? R.weight(of_key(cut.key)) : 0, tied = cut.ties * tie_w;
         uint64_t in_ties = 0;                       // what is left to be reached among the ties of the cut so far
@@ -501,8 +555,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
             cut.key,
             [&](uint64_t above) -> uint64_t {
                 const uint64_t all = above + tied;
-                const double t = ceil(static_cast<double>(fmaxf(top_p, 0.f)) * static_cast<double>(all));
-                const uint64_t want = min(max(static_cast<uint64_t>(t), static_cast<uint64_t>(1)), all);
+                const uint64_t want = want_of_p(all);
                 in_ties = want > above ? want - above : 0;
                 return want > above ? 0 : want;
             },
@@ -558,7 +611,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
         ties_all += s[1][i];
     }
     all += min(ties_all, cut.ties) * tie_w;
-    const uint64_t at = min(static_cast<uint64_t>(static_cast<double>(u > 0.f ? fminf(u, 1.0f) : 0.f) * static_cast<double>(all)), all - 1);
+    const uint64_t at = number_of(all);
     const uint64_t end = run + sum + min(tie + ties, cut.ties) * tie_w;
     run += min(tie, cut.ties) * tie_w;
     if (run > at || at >= end) return;
