@@ -49,9 +49,15 @@ namespace {
 // that keeps the largest one between 2^6 and 2^15, whatever V's scales are; m is a whole
 // number.  So all rescaling is exact; m moves when exceeded by more than
 // kMoveThreshold, f when a weight would be above 2^15.
-constexpr int F8_WARPS = 15;      // and the producer: 16 warps, so that a thread may have 128 registers
+constexpr int F8_WARPS = 15;       // and the producer: 16 warps, so that a thread may have 128 registers
 constexpr int F8_THREADS = 32 * (F8_WARPS + 1);
 constexpr int F8_STAGES = 11;
+// Teams: a segment ends with its warps' results joined, so a CTA with several segments of few tiles has 3 teams of 5
+// warps, or 2 of 7, that work on segments in turn, each with its own barrier.  One team and as below: 100 x 1 behind 100
+// with 8 KV heads (1 tile) 22.3 and 11.7 us, 256 x 1 behind 500 (3) 33.3 and 28.1, 64 x 1 behind 800 with 8 KV heads (5)
+// 23.6 and 19.7, 256 x 1 behind 2000 (12) 59.9 and 58.3; behind 4000 (24 tiles) 2 teams 59.6 against 53.9: the ring
+// holds too few of them.  Where 4 row groups share 7 warps, 200 x 4 behind 1000 (8 tiles): 109 and 120, so one team.
+constexpr int kThreeTeams = 4, kTwoTeams = 16;   // below so many tiles a segment
 constexpr int kBatch = 3;          // tiles whose copies are issued at once
 constexpr int kStep = 32;           // keys of a step
 constexpr int kSteps = kTile / kStep;
@@ -71,6 +77,7 @@ struct Few8Smem {
     float o[F8_WARPS][8][HD + 4];   // a warp's result, and its rows' maximum and sum
     float2 ml[F8_WARPS][8];
     uint64_t full[F8_STAGES], empty[F8_STAGES], work_full;
+    int issued;                      // tiles that the producer has begun to copy
     Work work[kWorkCache];
 };
 struct Few8Tma {
@@ -153,6 +160,7 @@ __global__ void __launch_bounds__(F8_THREADS, 1)
             mbar_init(&S.empty[i], kArrivals);
         }
         mbar_init(&S.work_full, 1);
+        S.issued = 0;
         fence_barrier_init();
         prefetch_tmap(&M.k);
         prefetch_tmap(&M.v);
@@ -161,9 +169,12 @@ __global__ void __launch_bounds__(F8_THREADS, 1)
     if (tid == 0) fetch_first(A, A.n_ctas + blockIdx.x, &S.work[0]);
     __syncthreads();
     const int seg0 = S.work[0].seg0, seg1 = S.work[0].seg1;
-    bool failed = false;
+    bool failed = false, fetched = false;
     auto work_of = [&](int i) -> const Work& {
-        if (i == seg0 + 1) wait_or_flag(&S.work_full, 0, A.err, kErrWaitFull, failed);
+        if (i > seg0 && !fetched) {
+            wait_or_flag(&S.work_full, 0, A.err, kErrWaitFull, failed);
+            fetched = true;
+        }
         return i - seg0 < kWorkCache ? S.work[i - seg0] : *static_cast<const Work*>(A.d.segs + i);
     };
     if (warp == F8_WARPS) {   // producer
@@ -201,6 +212,7 @@ __global__ void __launch_bounds__(F8_THREADS, 1)
                 failed = __any_sync(0xffffffffu, failed);
                 if (failed) break;
                 ring += count;
+                if (lane == 0) *const_cast<volatile int*>(&S.issued) = ring;
                 if (__any_sync(0xffffffffu, id0 == -2 || id1 == -2)) {
                     for (int e = 0; e < count * per_tile; ++e) {
                         const int to = __shfl_sync(0xffffffffu, st, e / per_tile), b = e % per_tile;
@@ -240,280 +252,315 @@ __global__ void __launch_bounds__(F8_THREADS, 1)
             wait_or_flag(&S.full[u % F8_STAGES], (u / F8_STAGES) & 1, A.err, kErrDrain, late);
         return;
     }
-    const int g = lane >> 2, t = lane & 3;        // fragment row, and which quarter of it
-    const int mi = lane >> 3, li = lane & 7;      // ldmatrix: matrix and row of this lane's address
-    // Rows lie in pairs in lines of 128 bytes: chunk q of row r, 16 bytes, is 4 (r % 2) + q of line r / 2 and
-    // lies at that ^ (r / 2 % 8).  This lane's row of a step, chunks mi / 2 and mi / 2 + 2:
-    uint32_t piece[2];
+    auto consume = [&]<bool ONE>(int n_teams) {
+        const int in_team = ONE ? F8_WARPS : F8_WARPS / n_teams, team = ONE ? 0 : warp / in_team, tw = warp - team * in_team;
+        const int every = ONE ? 1 : n_teams;
+        if (!ONE && team >= n_teams) return;
+        const int g = lane >> 2, t = lane & 3;        // fragment row, and which quarter of it
+        const int mi = lane >> 3, li = lane & 7;      // ldmatrix: matrix and row of this lane's address
+        // Rows lie in pairs in lines of 128 bytes: chunk q of row r, 16 bytes, is 4 (r % 2) + q of line r / 2 and
+        // lies at that ^ (r / 2 % 8).  This lane's row of a step, chunks mi / 2 and mi / 2 + 2:
+        uint32_t piece[2];
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-        const int r = li + 8 * (mi & 1), line = r >> 1;
-        piece[h] = line * 2 * HD + ((((r & 1) * 4 + 2 * h + (mi >> 1)) ^ line) << 4);
-    }
-    static_assert(kChunkFewRows <= 32 && F8_WARPS < 32, "four row groups at most");
-    // row groups of 8 rows: 1, 2 or 4 (as a power of two), the warps dealt out to them
-    auto group_bits = [](int n_rows) { return n_rows <= 8 ? 0 : n_rows <= 16 ? 1 : 2; };
-    auto workers = [](int gb, int rg) { return (F8_WARPS - rg + (1 << gb) - 1) >> gb; };   // warps of row group rg
-    // This lane's elements 16 c + 4 t .. + 3 of row g of the warp's group, ahead of the segment.
-    using Raw = std::conditional_t<sizeof(Act) == 4, uint4, uint2>;
-    Raw raw[HD / 16];
-    auto load_q = [&](const Work& w) {
-        const int r = (warp & ((1 << group_bits(w.n_rows)) - 1)) * 8 + g;
-        const bool ok = r < w.n_rows;
-        const int row = w.row0 + (ok ? r : 0), tok = row_token(A, row), h = row - tok * A.group;
-        const Raw* src = reinterpret_cast<const Raw*>(static_cast<const Act*>(A.q) +
-                                                      static_cast<int64_t>(w.first + tok) * A.q_stride +
-                                                      (w.kvh * A.group + h) * HD) + t;
-#pragma unroll
-        for (int i = 0; i < HD / 16; ++i) raw[i] = ok ? src[4 * i] : Raw{};
-    };
-    int ring0 = 0;   // tiles of the segments before
-    auto segment = [&](const Work& w) {
-        // w may lie in either memory: what the steps need of it is held in registers
-        const int t0 = w.t0, pos_min = w.pos_min, kv_len = w.kv_len;
-        const int gb = group_bits(w.n_rows), rg = warp & ((1 << gb) - 1), kw = warp >> gb;
-        const int pos_r = w.pos + row_token(A, w.row0 + min(rg * 8 + g, w.n_rows - 1));
-        uint32_t qf[HD / 16][4];   // A fragments: rows g the first terms, rows g + 8 the second
-        float c;                   // of the row's scores: 2^e / 8 log2(e), q = 2^e (terms)
-        {
-            float x[16];
-#pragma unroll
-            for (int i = 0; i < HD / 16; ++i) {
-                if constexpr (sizeof(Act) == 4) {
-                    x[4 * i] = __uint_as_float(raw[i].x);
-                    x[4 * i + 1] = __uint_as_float(raw[i].y);
-                    x[4 * i + 2] = __uint_as_float(raw[i].z);
-                    x[4 * i + 3] = __uint_as_float(raw[i].w);
-                } else {
-                    x[4 * i] = __uint_as_float(raw[i].x << 16);
-                    x[4 * i + 1] = __uint_as_float(raw[i].x & 0xffff0000u);
-                    x[4 * i + 2] = __uint_as_float(raw[i].y << 16);
-                    x[4 * i + 3] = __uint_as_float(raw[i].y & 0xffff0000u);
-                }
-            }
-            float most = 0.f;
-#pragma unroll
-            for (int i = 0; i < 16; ++i) most = fmax3(most, fabsf(x[i]), 0.f);
-            most = fmax3(most, __shfl_xor_sync(0xffffffffu, most, 1), 0.f);
-            most = fmax3(most, __shfl_xor_sync(0xffffffffu, most, 2), 0.f);
-            const bool fine = most <= 3.4028234e38f;   // otherwise every score is NaN
-            // in two powers of two, neither of which leaves the range
-            const float pre = most < 0x1p-60f ? 0x1p64f : 1.f;
-            const int e = fine && most > 0.f ? static_cast<int>(__float_as_uint(most * pre) >> 23) - 127 - kQBits : 0;
-            const float up = fine ? pow2(-e) : 0.f;
-            c = fine ? kExpScale * pow2(e) * (1.f / pre) : NAN;
-#pragma unroll
-            for (int i = 0; i < 16; ++i) x[i] = fine ? x[i] * pre * up : 0.f;
-#pragma unroll
-            for (int ks = 0; ks < HD / 16; ++ks) {
-                two_terms(x[4 * ks], x[4 * ks + 2], qf[ks][0], qf[ks][1]);
-                two_terms(x[4 * ks + 1], x[4 * ks + 3], qf[ks][2], qf[ks][3]);
-            }
+        for (int h = 0; h < 2; ++h) {
+            const int r = li + 8 * (mi & 1), line = r >> 1;
+            piece[h] = line * 2 * HD + ((((r & 1) * 4 + 2 * h + (mi >> 1)) ^ line) << 4);
         }
-        float m = -INFINITY, l = 0.f;
-        int fe = 127;                             // f = 2^fe
-        float f = pow2(127), limit = pow2(kWeightBits - 127);
-        float o[8][4];
+        static_assert(kChunkFewRows <= 32 && F8_WARPS < 32, "four row groups at most");
+        // row groups of 8 rows: 1, 2 or 4 (as a power of two), the warps dealt out to them
+        auto group_bits = [](int n_rows) { return n_rows <= 8 ? 0 : n_rows <= 16 ? 1 : 2; };
+        auto workers = [&](int gb, int rg) { return (in_team - rg + (1 << gb) - 1) >> gb; };   // warps of row group rg
+        // This lane's elements 16 c + 4 t .. + 3 of row g of the warp's group, ahead of the segment.
+        using Raw = std::conditional_t<sizeof(Act) == 4, uint4, uint2>;
+        Raw raw[HD / 16];
+        auto load_q = [&](const Work& w) {
+            const int r = (tw & ((1 << group_bits(w.n_rows)) - 1)) * 8 + g;
+            const bool ok = r < w.n_rows;
+            const int row = w.row0 + (ok ? r : 0), tok = row_token(A, row), h = row - tok * A.group;
+            const Raw* src = reinterpret_cast<const Raw*>(static_cast<const Act*>(A.q) +
+                                                          static_cast<int64_t>(w.first + tok) * A.q_stride +
+                                                          (w.kvh * A.group + h) * HD) + t;
 #pragma unroll
-        for (int j = 0; j < 8; ++j) o[j][0] = o[j][1] = o[j][2] = o[j][3] = 0.f;
-        int since = 0;
-        bool flushed = false;
-        // this lane's dimensions 16 c + 4 t .. + 3 of row g
-        auto held = [&](int i) -> float4& { return *reinterpret_cast<float4*>(&S.o[warp][g][16 * i + 4 * t]); };
-        auto flush = [&]() {
-#pragma unroll
-            for (int i = 0; i < HD / 16; ++i) {
-                float4 y = make_float4(o[2 * i][0] + o[2 * i][2], o[2 * i + 1][0] + o[2 * i + 1][2], o[2 * i][1] + o[2 * i][3],
-                                       o[2 * i + 1][1] + o[2 * i + 1][3]);
-                if (flushed) {
-                    const float4 z = held(i);
-                    y = make_float4(y.x + z.x, y.y + z.y, y.z + z.z, y.w + z.w);
-                }
-                held(i) = y;
-            }
-#pragma unroll
-            for (int j = 0; j < 8; ++j) o[j][0] = o[j][1] = o[j][2] = o[j][3] = 0.f;
-            flushed = true;
-            since = 0;
+            for (int i = 0; i < HD / 16; ++i) raw[i] = ok ? src[4 * i] : Raw{};
         };
-        auto scale_o = [&](float by) {
-#pragma unroll
-            for (int j = 0; j < 8; ++j)
-#pragma unroll
-                for (int e = 0; e < 4; ++e) o[j][e] *= by;
-            if (flushed)
+        int ring0 = 0;   // tiles of the segments before
+        // A stage's barrier tells one lap of the ring from the next only: with several teams no warp looks for a
+        // tile before the producer has begun with it, which it does when the stage's last one has been used.
+        int issued = ONE ? INT32_MAX : 0;
+        auto begun = [&](int ring) {
+            if (ONE) return;
+            uint64_t t_first = 0;
+            for (int i = 1; issued <= ring && !failed; ++i) {
+                issued = *const_cast<volatile int*>(&S.issued);
+                if (i % 256 == 0) {
+                    const uint64_t now = globaltimer();
+                    if (t_first == 0) t_first = now;
+                    if (now - t_first > kWaitTimeoutNs) {
+                        record_error(A.err, kErrWaitFull);
+                        failed = true;
+                    }
+                }
+            }
+        };
+        auto segment = [&](const Work& w) {
+            // w may lie in either memory: what the steps need of it is held in registers
+            const int t0 = w.t0, pos_min = w.pos_min, kv_len = w.kv_len;
+            const int gb = group_bits(w.n_rows), rg = tw & ((1 << gb) - 1), kw = tw >> gb;
+            const int pos_r = w.pos + row_token(A, w.row0 + min(rg * 8 + g, w.n_rows - 1));
+            uint32_t qf[HD / 16][4];   // A fragments: rows g the first terms, rows g + 8 the second
+            float c;                   // of the row's scores: 2^e / 8 log2(e), q = 2^e (terms)
+            {
+                float x[16];
 #pragma unroll
                 for (int i = 0; i < HD / 16; ++i) {
-                    const float4 z = held(i);
-                    held(i) = make_float4(z.x * by, z.y * by, z.z * by, z.w * by);
-                }
-        };
-        // kStep keys from j0 of tile n in stage st; EDGE: some row does not attend to all of the tile.
-        auto step = [&]<bool EDGE>(int st, int n, int j0) {
-            constexpr int B = kStep / 8, N = kStep / 4;   // blocks of 8 keys; keys of a lane: 2 t, 2 t + 1 of each
-            const int key0 = n * kTile + j0;
-            if (EDGE && key0 >= kv_len) return;
-            if (++since > kFlush) flush();
-            const uint32_t kb = smem_u32(S.k[st]) + j0 * HD, vb = smem_u32(S.v[st]) + j0 * HD;
-            float sf[B][4];
-#pragma unroll
-            for (int b2 = 0; b2 < B / 2; ++b2) {
-                // matrices: keys 0-7 and 8-15 of chunks 0, 1; then of 2, 3
-                uint32_t kr[2][4];
-#pragma unroll
-                for (int h = 0; h < 2; ++h) ldsm4_b(kb + 16 * b2 * HD + piece[h], kr[h]);
-#pragma unroll
-                for (int ks = 0; ks < HD / 16; ++ks)
-#pragma unroll
-                    for (int b = 0; b < 2; ++b) {
-                        const uint32_t u = kr[ks >> 1][2 * (ks & 1) + b];
-                        if (ks == 0) mma_f16_zero(sf[2 * b2 + b], qf[ks], codes_f16(u), codes_f16(u >> 8));
-                        else mma_f16(sf[2 * b2 + b], qf[ks], codes_f16(u), codes_f16(u >> 8));
-                    }
-            }
-            float s[N], vsf[N];
-#pragma unroll
-            for (int b = 0; b < B; ++b) {
-                const uint32_t kx = *reinterpret_cast<const uint16_t*>(&S.ks[st][j0 + 8 * b + 2 * t]);
-                const uint32_t vx = *reinterpret_cast<const uint16_t*>(&S.vs[st][j0 + 8 * b + 2 * t]);
-#pragma unroll
-                for (int e = 0; e < 2; ++e) {
-                    const int i = 2 * b + e;
-                    s[i] = (sf[b][e] + sf[b][2 + e]) * (__uint_as_float((e ? kx << 15 : kx << 23) & 0x7f800000u) * c);
-                    vsf[i] = __uint_as_float((e ? vx << 15 : vx << 23) & 0x7f800000u);
-                    if (EDGE && key0 + 8 * b + 2 * t + e > pos_r) {
-                        s[i] = -INFINITY;
-                        vsf[i] = 0.f;
+                    if constexpr (sizeof(Act) == 4) {
+                        x[4 * i] = __uint_as_float(raw[i].x);
+                        x[4 * i + 1] = __uint_as_float(raw[i].y);
+                        x[4 * i + 2] = __uint_as_float(raw[i].z);
+                        x[4 * i + 3] = __uint_as_float(raw[i].w);
+                    } else {
+                        x[4 * i] = __uint_as_float(raw[i].x << 16);
+                        x[4 * i + 1] = __uint_as_float(raw[i].x & 0xffff0000u);
+                        x[4 * i + 2] = __uint_as_float(raw[i].y << 16);
+                        x[4 * i + 3] = __uint_as_float(raw[i].y & 0xffff0000u);
                     }
                 }
-            }
-            float mt = s[0];
+                float most = 0.f;
 #pragma unroll
-            for (int i = 1; i + 1 < N; i += 2) mt = fmax3(mt, s[i], s[i + 1]);
-            mt = fmax3(mt, s[N - 1], s[N - 1]);
-            if (__any_sync(0xffffffffu, m == m && !(mt <= m + kMoveThreshold))) {
-                float to = fmax3(mt, __shfl_xor_sync(0xffffffffu, mt, 1), -INFINITY);
-                to = fmax3(to, __shfl_xor_sync(0xffffffffu, to, 2), -INFINITY);
-                float by = 1.f;
-                if (m == m && !(to <= m + kMoveThreshold)) {
-                    to = ceilf(to);
-                    if (m != -INFINITY) {
-                        // weights of the new m are smaller by 2^(m - to): f makes up for it, as far as it goes
-                        l *= pow2_down(m - to);
-                        const float e = static_cast<float>(fe) + (to - m);
-                        by = pow2_down(fminf(127.f - e, 0.f));
-                        fe = static_cast<int>(fminf(e, 127.f));
+                for (int i = 0; i < 16; ++i) most = fmax3(most, fabsf(x[i]), 0.f);
+                most = fmax3(most, __shfl_xor_sync(0xffffffffu, most, 1), 0.f);
+                most = fmax3(most, __shfl_xor_sync(0xffffffffu, most, 2), 0.f);
+                const bool fine = most <= 3.4028234e38f;   // otherwise every score is NaN
+                // in two powers of two, neither of which leaves the range
+                const float pre = most < 0x1p-60f ? 0x1p64f : 1.f;
+                const int e = fine && most > 0.f ? static_cast<int>(__float_as_uint(most * pre) >> 23) - 127 - kQBits : 0;
+                const float up = fine ? pow2(-e) : 0.f;
+                c = fine ? kExpScale * pow2(e) * (1.f / pre) : NAN;
+#pragma unroll
+                for (int i = 0; i < 16; ++i) x[i] = fine ? x[i] * pre * up : 0.f;
+#pragma unroll
+                for (int ks = 0; ks < HD / 16; ++ks) {
+                    two_terms(x[4 * ks], x[4 * ks + 2], qf[ks][0], qf[ks][1]);
+                    two_terms(x[4 * ks + 1], x[4 * ks + 3], qf[ks][2], qf[ks][3]);
+                }
+            }
+            float m = -INFINITY, l = 0.f;
+            int fe = 127;                             // f = 2^fe
+            float f = pow2(127), limit = pow2(kWeightBits - 127);
+            float o[8][4];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) o[j][0] = o[j][1] = o[j][2] = o[j][3] = 0.f;
+            int since = 0;
+            bool flushed = false;
+            // this lane's dimensions 16 c + 4 t .. + 3 of row g
+            auto held = [&](int i) -> float4& { return *reinterpret_cast<float4*>(&S.o[warp][g][16 * i + 4 * t]); };
+            auto flush = [&]() {
+#pragma unroll
+                for (int i = 0; i < HD / 16; ++i) {
+                    float4 y = make_float4(o[2 * i][0] + o[2 * i][2], o[2 * i + 1][0] + o[2 * i + 1][2], o[2 * i][1] + o[2 * i][3],
+                                           o[2 * i + 1][1] + o[2 * i + 1][3]);
+                    if (flushed) {
+                        const float4 z = held(i);
+                        y = make_float4(y.x + z.x, y.y + z.y, y.z + z.z, y.w + z.w);
+                    }
+                    held(i) = y;
+                }
+#pragma unroll
+                for (int j = 0; j < 8; ++j) o[j][0] = o[j][1] = o[j][2] = o[j][3] = 0.f;
+                flushed = true;
+                since = 0;
+            };
+            auto scale_o = [&](float by) {
+#pragma unroll
+                for (int j = 0; j < 8; ++j)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) o[j][e] *= by;
+                if (flushed)
+#pragma unroll
+                    for (int i = 0; i < HD / 16; ++i) {
+                        const float4 z = held(i);
+                        held(i) = make_float4(z.x * by, z.y * by, z.z * by, z.w * by);
+                    }
+            };
+            // kStep keys from j0 of tile n in stage st; EDGE: some row does not attend to all of the tile.
+            auto step = [&]<bool EDGE>(int st, int n, int j0) {
+                constexpr int B = kStep / 8, N = kStep / 4;   // blocks of 8 keys; keys of a lane: 2 t, 2 t + 1 of each
+                const int key0 = n * kTile + j0;
+                if (EDGE && key0 >= kv_len) return;
+                if (++since > kFlush) flush();
+                const uint32_t kb = smem_u32(S.k[st]) + j0 * HD, vb = smem_u32(S.v[st]) + j0 * HD;
+                float sf[B][4];
+#pragma unroll
+                for (int b2 = 0; b2 < B / 2; ++b2) {
+                    // matrices: keys 0-7 and 8-15 of chunks 0, 1; then of 2, 3
+                    uint32_t kr[2][4];
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) ldsm4_b(kb + 16 * b2 * HD + piece[h], kr[h]);
+#pragma unroll
+                    for (int ks = 0; ks < HD / 16; ++ks)
+#pragma unroll
+                        for (int b = 0; b < 2; ++b) {
+                            const uint32_t u = kr[ks >> 1][2 * (ks & 1) + b];
+                            if (ks == 0) mma_f16_zero(sf[2 * b2 + b], qf[ks], codes_f16(u), codes_f16(u >> 8));
+                            else mma_f16(sf[2 * b2 + b], qf[ks], codes_f16(u), codes_f16(u >> 8));
+                        }
+                }
+                float s[N], vsf[N];
+#pragma unroll
+                for (int b = 0; b < B; ++b) {
+                    const uint32_t kx = *reinterpret_cast<const uint16_t*>(&S.ks[st][j0 + 8 * b + 2 * t]);
+                    const uint32_t vx = *reinterpret_cast<const uint16_t*>(&S.vs[st][j0 + 8 * b + 2 * t]);
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        const int i = 2 * b + e;
+                        s[i] = (sf[b][e] + sf[b][2 + e]) * (__uint_as_float((e ? kx << 15 : kx << 23) & 0x7f800000u) * c);
+                        vsf[i] = __uint_as_float((e ? vx << 15 : vx << 23) & 0x7f800000u);
+                        if (EDGE && key0 + 8 * b + 2 * t + e > pos_r) {
+                            s[i] = -INFINITY;
+                            vsf[i] = 0.f;
+                        }
+                    }
+                }
+                float mt = s[0];
+#pragma unroll
+                for (int i = 1; i + 1 < N; i += 2) mt = fmax3(mt, s[i], s[i + 1]);
+                mt = fmax3(mt, s[N - 1], s[N - 1]);
+                if (__any_sync(0xffffffffu, m == m && !(mt <= m + kMoveThreshold))) {
+                    float to = fmax3(mt, __shfl_xor_sync(0xffffffffu, mt, 1), -INFINITY);
+                    to = fmax3(to, __shfl_xor_sync(0xffffffffu, to, 2), -INFINITY);
+                    float by = 1.f;
+                    if (m == m && !(to <= m + kMoveThreshold)) {
+                        to = ceilf(to);
+                        if (m != -INFINITY) {
+                            // weights of the new m are smaller by 2^(m - to): f makes up for it, as far as it goes
+                            l *= pow2_down(m - to);
+                            const float e = static_cast<float>(fe) + (to - m);
+                            by = pow2_down(fminf(127.f - e, 0.f));
+                            fe = static_cast<int>(fminf(e, 127.f));
+                            f = pow2(fe);
+                            limit = pow2(min(kWeightBits - fe, 127));
+                        }
+                        m = to;
+                    }
+                    if (__any_sync(0xffffffffu, by != 1.f)) scale_o(by);
+                }
+                const float m_use = m == -INFINITY ? 0.f : m;   // nothing attended so far: the scores are -inf
+                float wt[N];
+#pragma unroll
+                for (int i = 0; i < N; ++i) {
+                    const float p = ex2_sfu(s[i] - m_use);
+                    l += p;
+                    wt[i] = p * vsf[i];
+                }
+                float wm = wt[0];
+#pragma unroll
+                for (int i = 1; i + 1 < N; i += 2) wm = fmax3(wm, wt[i], wt[i + 1]);
+                wm = fmax3(wm, wt[N - 1], wt[N - 1]);
+                if (__any_sync(0xffffffffu, !(wm <= limit))) {
+                    float to = fmax3(wm, __shfl_xor_sync(0xffffffffu, wm, 1), 0.f);
+                    to = fmax3(to, __shfl_xor_sync(0xffffffffu, to, 2), 0.f);
+                    float by = 1.f;
+                    if (to > limit && to <= 3.4028234e38f) {
+                        const int e = max(kWeightStart + 127 - static_cast<int>(__float_as_uint(to) >> 23), -126);
+                        by = pow2_down(static_cast<float>(e - fe));
+                        fe = e;
                         f = pow2(fe);
                         limit = pow2(min(kWeightBits - fe, 127));
                     }
-                    m = to;
+                    scale_o(by);
                 }
-                if (__any_sync(0xffffffffu, by != 1.f)) scale_o(by);
-            }
-            const float m_use = m == -INFINITY ? 0.f : m;   // nothing attended so far: the scores are -inf
-            float wt[N];
 #pragma unroll
-            for (int i = 0; i < N; ++i) {
-                const float p = ex2_sfu(s[i] - m_use);
-                l += p;
-                wt[i] = p * vsf[i];
-            }
-            float wm = wt[0];
+                for (int b2 = 0; b2 < B / 2; ++b2) {
+                    uint32_t vr[2][4], pf[4];
 #pragma unroll
-            for (int i = 1; i + 1 < N; i += 2) wm = fmax3(wm, wt[i], wt[i + 1]);
-            wm = fmax3(wm, wt[N - 1], wt[N - 1]);
-            if (__any_sync(0xffffffffu, !(wm <= limit))) {
-                float to = fmax3(wm, __shfl_xor_sync(0xffffffffu, wm, 1), 0.f);
-                to = fmax3(to, __shfl_xor_sync(0xffffffffu, to, 2), 0.f);
-                float by = 1.f;
-                if (to > limit && to <= 3.4028234e38f) {
-                    const int e = max(kWeightStart + 127 - static_cast<int>(__float_as_uint(to) >> 23), -126);
-                    by = pow2_down(static_cast<float>(e - fe));
-                    fe = e;
-                    f = pow2(fe);
-                    limit = pow2(min(kWeightBits - fe, 127));
+                    for (int h = 0; h < 2; ++h) ldsm4_bt(vb + 16 * b2 * HD + piece[h], vr[h]);
+                    two_terms(wt[4 * b2] * f, wt[4 * b2 + 1] * f, pf[0], pf[1]);
+                    two_terms(wt[4 * b2 + 2] * f, wt[4 * b2 + 3] * f, pf[2], pf[3]);
+#pragma unroll
+                    for (int q = 0; q < HD / 16; ++q) {   // chunk q: dimensions 16 q + 2 g (+1)
+                        const uint32_t u0 = vr[q >> 1][2 * (q & 1)], u1 = vr[q >> 1][2 * (q & 1) + 1];
+                        mma_f16(o[2 * q], pf, codes_f16(u0), codes_f16(u1));
+                        mma_f16(o[2 * q + 1], pf, codes_f16(u0 >> 8), codes_f16(u1 >> 8));
+                    }
                 }
-                scale_o(by);
+            };
+            // the steps of the segment, dealt out to the group's warps
+            const int n_steps = (w.t1 - t0) * kSteps, nkw = workers(gb, rg);
+            for (int i = kw; i < n_steps; i += nkw) {
+                const int n = t0 + i / kSteps, ring = ring0 + i / kSteps, st = ring % F8_STAGES;
+                begun(ring);
+                wait_or_flag(&S.full[st], (ring / F8_STAGES) & 1, A.err, kErrWaitFull, failed);
+                __syncwarp();
+                if (n * kTile + kTile - 1 > pos_min) step.template operator()<true>(st, n, kStep * (i % kSteps));
+                else step.template operator()<false>(st, n, kStep * (i % kSteps));
+                __syncwarp();
+                if (lane == 0) mbar_arrive_n(&S.empty[st], kArrivals / kSteps >> gb);
             }
+            flush();
+            l += __shfl_xor_sync(0xffffffffu, l, 1);
+            l += __shfl_xor_sync(0xffffffffu, l, 2);
+            if (t == 0) S.ml[warp][g] = make_float2(m, l);
+            const float back = pow2(-fe);   // to the weights 2^(s - m)
 #pragma unroll
-            for (int b2 = 0; b2 < B / 2; ++b2) {
-                uint32_t vr[2][4], pf[4];
-#pragma unroll
-                for (int h = 0; h < 2; ++h) ldsm4_bt(vb + 16 * b2 * HD + piece[h], vr[h]);
-                two_terms(wt[4 * b2] * f, wt[4 * b2 + 1] * f, pf[0], pf[1]);
-                two_terms(wt[4 * b2 + 2] * f, wt[4 * b2 + 3] * f, pf[2], pf[3]);
-#pragma unroll
-                for (int q = 0; q < HD / 16; ++q) {   // chunk q: dimensions 16 q + 2 g (+1)
-                    const uint32_t u0 = vr[q >> 1][2 * (q & 1)], u1 = vr[q >> 1][2 * (q & 1) + 1];
-                    mma_f16(o[2 * q], pf, codes_f16(u0), codes_f16(u1));
-                    mma_f16(o[2 * q + 1], pf, codes_f16(u0 >> 8), codes_f16(u1 >> 8));
-                }
+            for (int i = 0; i < HD / 16; ++i) {
+                const float4 z = held(i);
+                held(i) = make_float4(z.x * back, z.y * back, z.z * back, z.w * back);
             }
         };
-        // the steps of the segment, dealt out to the group's warps
-        const int n_steps = (w.t1 - t0) * kSteps, nkw = workers(gb, rg);
-        for (int i = kw; i < n_steps; i += nkw) {
-            const int n = t0 + i / kSteps, ring = ring0 + i / kSteps, st = ring % F8_STAGES;
-            wait_or_flag(&S.full[st], (ring / F8_STAGES) & 1, A.err, kErrWaitFull, failed);
-            __syncwarp();
-            if (n * kTile + kTile - 1 > pos_min) step.template operator()<true>(st, n, kStep * (i % kSteps));
-            else step.template operator()<false>(st, n, kStep * (i % kSteps));
-            __syncwarp();
-            if (lane == 0) mbar_arrive_n(&S.empty[st], kArrivals / kSteps >> gb);
-        }
-        ring0 += w.t1 - w.t0;
-        flush();
-        l += __shfl_xor_sync(0xffffffffu, l, 1);
-        l += __shfl_xor_sync(0xffffffffu, l, 2);
-        if (t == 0) S.ml[warp][g] = make_float2(m, l);
-        const float back = pow2(-fe);   // to the weights 2^(s - m)
+        if (ONE && seg0 < seg1) load_q(S.work[0]);
+        if (warp == (ONE ? F8_WARPS - 1 : 0)) fetch_work(A, seg0, seg1, S.work, &S.work_full);
+        if (!ONE && seg0 + team < seg1) load_q(work_of(seg0 + team));
+        for (int i = 0; i < team; ++i) ring0 += work_of(seg0 + i).t1 - work_of(seg0 + i).t0;
+        for (int sg = seg0 + team; sg < seg1; sg += every) {
+            const Work& w = work_of(sg);
+            segment(w);
+            if (sg + every < seg1) {
+                ring0 += w.t1 - w.t0;
+                if (!ONE)
+                    for (int i = sg + 1; i < sg + every; ++i) ring0 += work_of(i).t1 - work_of(i).t0;
+                load_q(work_of(sg + every));
+            }
+            named_bar_sync(1 + team, 32 * in_team);
+            // ---- join the key workers: a row per warp, two columns per lane; lane q has the
+            // weight of worker q ----
+            const int gb = group_bits(w.n_rows);
+            for (int r = tw; r < w.n_rows; r += in_team) {
+                const int w0 = r >> 3, rr = r & 7, nkw = workers(gb, w0);
+                const float2 ml = lane < nkw ? S.ml[team * in_team + w0 + (lane << gb)][rr] : make_float2(-INFINITY, 0.f);
+                float m_all = ml.x;
 #pragma unroll
-        for (int i = 0; i < HD / 16; ++i) {
-            const float4 z = held(i);
-            held(i) = make_float4(z.x * back, z.y * back, z.z * back, z.w * back);
+                for (int d = 1; d < 16; d *= 2) m_all = fmaxf(m_all, __shfl_xor_sync(0xffffffffu, m_all, d));
+                const float fw = ml.x == -INFINITY ? 0.f : ex2_sfu(ml.x - m_all);
+                float l_all = fw == 0.f ? 0.f : fw * ml.y;
+#pragma unroll
+                for (int d = 1; d < 16; d *= 2) l_all += __shfl_xor_sync(0xffffffffu, l_all, d);
+                float2 acc = make_float2(0.f, 0.f);
+#pragma unroll
+                for (int q = 0; q < F8_WARPS; ++q) {
+                    const float fq = __shfl_sync(0xffffffffu, fw, q);
+                    if (q < nkw && fq != 0.f) {
+                        const float2 x = *reinterpret_cast<const float2*>(&S.o[team * in_team + w0 + (q << gb)][rr][2 * lane]);
+                        acc.x = fmaf(fq, x.x, acc.x);
+                        acc.y = fmaf(fq, x.y, acc.y);
+                    }
+                }
+                const float l_row = __shfl_sync(0xffffffffu, l_all, 0), m_row = __shfl_sync(0xffffffffu, m_all, 0);
+                const bool empty = l_row == 0.f;   // no row of this segment has a weight
+                const float inv = empty ? 0.f : 1.0f / l_row;
+                acc = empty ? make_float2(no_weight(w), no_weight(w)) : make_float2(acc.x * inv, acc.y * inv);
+                const RowOut<Act> dst = row_out<Act>(A, w, r);
+                if (dst.out) store_pair(dst.out + 2 * lane, acc);
+                else store_pair(dst.part + 2 * lane, acc);
+                if (dst.lse && lane == 0) *dst.lse = empty ? -INFINITY : m_row + log2f(l_row);
+            }
+            named_bar_sync(1 + team, 32 * in_team);
         }
     };
-    if (seg0 < seg1) load_q(S.work[0]);
-    if (warp == F8_WARPS - 1) fetch_work(A, seg0, seg1, S.work, &S.work_full);
-    for (int sg = seg0; sg < seg1; ++sg) {
-        const Work& w = work_of(sg);
-        segment(w);
-        if (sg + 1 < seg1) load_q(work_of(sg + 1));
-        named_bar_sync(1, 32 * F8_WARPS);
-        // ---- join the key workers: a row per warp, two columns per lane; lane q has the
-        // weight of worker q ----
-        const int gb = group_bits(w.n_rows);
-        for (int r = warp; r < w.n_rows; r += F8_WARPS) {
-            const int w0 = r >> 3, rr = r & 7, nkw = workers(gb, w0);
-            const float2 ml = lane < nkw ? S.ml[w0 + (lane << gb)][rr] : make_float2(-INFINITY, 0.f);
-            float m_all = ml.x;
-#pragma unroll
-            for (int d = 1; d < 16; d *= 2) m_all = fmaxf(m_all, __shfl_xor_sync(0xffffffffu, m_all, d));
-            const float fw = ml.x == -INFINITY ? 0.f : ex2_sfu(ml.x - m_all);
-            float l_all = fw == 0.f ? 0.f : fw * ml.y;
-#pragma unroll
-            for (int d = 1; d < 16; d *= 2) l_all += __shfl_xor_sync(0xffffffffu, l_all, d);
-            float2 acc = make_float2(0.f, 0.f);
-#pragma unroll
-            for (int q = 0; q < F8_WARPS; ++q) {
-                const float fq = __shfl_sync(0xffffffffu, fw, q);
-                if (q < nkw && fq != 0.f) {
-                    const float2 x = *reinterpret_cast<const float2*>(&S.o[w0 + (q << gb)][rr][2 * lane]);
-                    acc.x = fmaf(fq, x.x, acc.x);
-                    acc.y = fmaf(fq, x.y, acc.y);
-                }
-            }
-            const float l_row = __shfl_sync(0xffffffffu, l_all, 0), m_row = __shfl_sync(0xffffffffu, m_all, 0);
-            const bool empty = l_row == 0.f;   // no row of this segment has a weight
-            const float inv = empty ? 0.f : 1.0f / l_row;
-            acc = empty ? make_float2(no_weight(w), no_weight(w)) : make_float2(acc.x * inv, acc.y * inv);
-            const RowOut<Act> dst = row_out<Act>(A, w, r);
-            if (dst.out) store_pair(dst.out + 2 * lane, acc);
-            else store_pair(dst.part + 2 * lane, acc);
-            if (dst.lse && lane == 0) *dst.lse = empty ? -INFINITY : m_row + log2f(l_row);
-        }
-        named_bar_sync(1, 32 * F8_WARPS);
-    }
+    const int n_segs = seg1 - seg0, each = n_segs > 0 ? (S.work[0].cta_tiles - 1) / n_segs : 0;
+    const bool two = each < kTwoTeams && n_segs > 2 && S.work[0].n_rows <= 16;
+    const int n_teams = each < kThreeTeams ? min(n_segs, 3) : two ? 2 : 1;
+    if (n_teams <= 1) consume.template operator()<true>(1);
+    else consume.template operator()<false>(n_teams);
 }
 
 template <class Act>
