@@ -1935,12 +1935,12 @@ int tle_chunk_desc_paged(const tle_shape_t* shape, int page_rows, const tle_page
     put(&hdr, sizeof hdr);
     for (const auto& st : start)
         for (size_t c = 0; c + 1 < st.size(); ++c) {
+            int64_t tiles = 0;
+            for (int32_t i = st[c]; i < st[c + 1]; ++i) tiles += segs[i].t1 - segs[i].t0;
+            if (st[c] < st[c + 1]) segs[st[c]].cta_tiles = static_cast<int32_t>(std::min<int64_t>(tiles, INT32_MAX));
             tle::ChunkSeg cta = st[c] < st[c + 1] ? segs[st[c]] : tle::ChunkSeg{};
             cta.seg0 = st[c];
             cta.seg1 = st[c + 1];
-            int64_t tiles = 0;
-            for (int32_t i = st[c]; i < st[c + 1]; ++i) tiles += segs[i].t1 - segs[i].t0;
-            cta.cta_tiles = static_cast<int32_t>(std::min<int64_t>(tiles, INT32_MAX));
             put(&cta, sizeof cta);
         }
     put(segs.data(), segs.size() * sizeof(tle::ChunkSeg));

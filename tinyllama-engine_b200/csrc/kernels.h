@@ -392,7 +392,7 @@ struct alignas(16) ChunkSeg {
     int32_t pos_min, kv_len;   // position of the item's first token; rows of its last token
     int32_t seg0, seg1;        // in cta: the CTA's segments [seg0, seg1)
     int32_t seq;
-    int32_t cta_tiles;         // in cta: tiles of all its segments
+    int32_t cta_tiles;         // in a CTA's first segment: tiles of all of its segments
 };
 struct ChunkMerge {          // an item whose results are in n_parts blocks of n_rows partial rows
     int32_t seq, kvh, row0, n_rows, part, n_parts;
