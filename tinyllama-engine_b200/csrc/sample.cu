@@ -178,6 +178,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
     const int64_t row = blockIdx.x / cl.n;
     if (tid < 64) S.powers[tid] = kPowers.v[tid];
     if (tid < 2) S.n_last[tid] = 0;
+    for (int i = tid; i < 3 * kBins / 4; i += kThreads) reinterpret_cast<uint4*>(S.hist)[i] = make_uint4(0, 0, 0, 0);
     const int v0 = cl.rank * A.slice, n = max(0, min(A.slice, A.n_vocab - v0));
     // ---- the slice into shared memory, its largest logit ----
     const float* src = A.logits + row * A.stride + v0;
@@ -262,22 +263,33 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
     R.powers = S.powers;
     R.reach = (min_p > 0.f ? fminf(kReach, -logf(min_p) + 0.01f) : kReach) * T;
     // Drops tokens of the warp, the others stay in place and in order; id is a token's place in the warp's part.
+    // stays(logit, whether there is one); four at a time: a row of 32000 with top-k 11.7 us, one at a time 12.0 us.
     uint16_t* id_of = reinterpret_cast<uint16_t*>(smem_raw + sizeof(Shared) + 16 + A.slice * sizeof(float)) + p0;
     bool whole = true;                         // nothing has been dropped: ids are not written yet
     auto keep = [&](auto&& stays) {
+        constexpr int kAhead = 4;
         int out = 0;
-        for (int i = 0; i < have; i += 32) {
-            const bool in = i + lane < have;
-            const float x = in ? x_of[i + lane] : 0.f;
-            const int id = whole ? i + lane : in ? id_of[i + lane] : 0;
-            const bool stay = in && stays(x);
-            const uint32_t set = __ballot_sync(0xffffffffu, stay);
-            if (stay) {
-                const int to = out + __popc(set & ((1u << lane) - 1));
-                x_of[to] = x;
-                id_of[to] = static_cast<uint16_t>(id);
+        for (int i0 = 0; i0 < have; i0 += 32 * kAhead) {
+            float x[kAhead];
+            int id[kAhead];
+            uint32_t set[kAhead];
+#pragma unroll
+            for (int q = 0; q < kAhead; ++q) {
+                const int i = i0 + 32 * q + lane;
+                x[q] = i < have ? x_of[i] : 0.f;
+                id[q] = whole ? i : i < have ? id_of[i] : 0;
             }
-            out += __popc(set);
+#pragma unroll
+            for (int q = 0; q < kAhead; ++q) set[q] = __ballot_sync(0xffffffffu, stays(x[q], i0 + 32 * q + lane < have));
+#pragma unroll
+            for (int q = 0; q < kAhead; ++q) {
+                if (set[q] >> lane & 1) {
+                    const int to = out + __popc(set[q] & ((1u << lane) - 1));
+                    x_of[to] = x[q];
+                    id_of[to] = static_cast<uint16_t>(id[q]);
+                }
+                out += __popc(set[q]);
+            }
             __syncwarp();
         }
         have = out;
@@ -333,6 +345,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
         if ((tid & 3) == 0 && i < n && run <= drawn && drawn < run + kept2[i]) A.tokens[row] = static_cast<int32_t>(at);
     };
     int searches = 0;
+    bool clean = true;                         // the bins are zeros
     // The cut at which the ranking's count (WEIGHT: sum of weights) within reach (the others weigh nothing) with a
     // key above `from` first reaches want_of(its sum over all of them).  A want of 0, or of more than there is: no cut.  Cut::ties is then
     // what is to be reached among the tokens of Cut::key.  Tokens below the cut may be dropped.
@@ -398,7 +411,9 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
         for (int level = 0;; ++level) {
             auto bin_of = [&](float x, uint32_t key) { return level == 0 ? by_logit(x) : static_cast<int>((hi - key) >> shift); };
             __syncthreads();
-            for (int i = tid; i < kLimbs * kBins; i += kThreads) (&S.hist[0][0])[i] = 0;
+            if (!clean)
+                for (int i = tid; i < kLimbs * kBins / 4; i += kThreads) reinterpret_cast<uint4*>(S.hist)[i] = make_uint4(0, 0, 0, 0);
+            clean = false;
             if (tid == 0) S.mine = 0;
             __syncthreads();
             for (int i = lane; i < have; i += 32) {
@@ -474,20 +489,21 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
                 }
             }
             if (!WEIGHT && level == 0 && left <= kFew) {   // what the row's token will be one of
-                keep([&](float x) { return R.in_reach(x) && by_logit(x) <= bin; });
+                keep([&](float x, bool there) { return there && R.in_reach(x) && by_logit(x) <= bin; });
                 hand_over(1);
                 cl.g.sync();
                 return true;
             }
             // ---- the bin's tokens, if they are few, ranked one by one; those behind it dropped ----
             if (level == 0) {
-                keep([&](float x) {
+                keep([&](float x, bool there) {
                     const int b = by_logit(x);
-                    if (b == bin) {
+                    const bool stays = there && b <= bin && R.in_reach(x);
+                    if (stays && b == bin) {
                         const uint32_t key = key_of(x);
                         if (in(x, key)) list_key(key);
                     }
-                    return b <= bin && R.in_reach(x);
+                    return stays;
                 });
             } else {
                 for (int i = lane; i < have; i += 32) {
@@ -523,7 +539,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
     };
     // where min-p leaves a narrow range, what is outside goes first
     if (min_p > 0.f) {
-        keep([&](float x) { return R.in_reach(x); });
+        keep([&](float x, bool there) { return there && R.in_reach(x); });
         hand_over(0);
         __syncthreads();
         if (lane == 0) S.warp_sum[warp] = have;
