@@ -23,11 +23,21 @@ namespace tle {
 
 namespace {
 
-// Bound by the K/V bytes, 130 a row and KV head.  Tiles of codes come by TMA (a
-// box is 64 or 128 rows of a page, two rows a line, 128-byte swizzle), their scales by bulk copies, into a ring that
-// a producer warp keeps full across segments; 15 warps take 32-key steps of the
-// tiles, each with its own running maximum, sum and output, joined in shared
-// memory at the segment's end.
+// Bound by the K/V bytes, 130 a row and KV head, where sequences are long; by a
+// segment's start and end (its q, the joining) where they are short.  Tiles of codes
+// come by TMA (a box is 64 or 128 rows of a page, two rows a line, 128-byte
+// swizzle), their scales by bulk copies, into a ring that a producer warp keeps
+// full across segments; 15 warps take 32-key steps of the tiles, each with its
+// own running maximum, sum and output, joined in shared memory at the segment's
+// end.
+//
+// Measured, 32 heads on 4 (us; bytes of K and V a second): 32 x 1 behind 8000 to 16000, bf16, 49.1,
+// 4.3 TB/s (the copies alone, no step taken, 40.4); 64 x 1 behind 1023 to 2047, fp32, 19.3, 2.6 TB/s
+// (13.6); 1 x 4 behind 700 10.7.  bf16 pages: 71.6, 25.1 and 11.  16 to 32 rows cost 2 or 4
+// such passes over the codes, one for 8 rows: 32 x 4 behind 2000, bf16, 33.6, where bf16 pages take 20.4.
+//
+// Tried: 8 to 11 stages, the same; two producers, scales by cp.async, q by copies and records
+// read ahead, joining by a warp of its own or one segment late, no gain; 16- and 64-key steps, slower.
 //
 // The codes become fp16 on their way from shared memory into the fragments of
 // m16n8k16 MMAs, exactly (a byte with its sign bit flipped, below the bits of

@@ -24,7 +24,15 @@
 //
 // A row is a cluster's: its logits are read once, into the shared memory of C
 // CTAs, C slices of the vocabulary; what they find out about a slice is
-// exchanged through distributed shared memory.
+// exchanged through distributed shared memory.  With slices of at most 12800
+// logits two CTAs fit on an SM, and one waits while the other counts; small batches are
+// spread over 8 CTAs a row for latency.
+//
+// Bound by latency: the load, three to six barriers of the cluster, and passes
+// over shared memory between them.  256 x 100003, mixed rules, 124 us, 0.8 TB/s of logits (issue 41 %, DRAM
+// 13 % busy; no filters 108, without the exponentials 71); 1 x 32000 11.7 us (no filters 6.9).
+// Tried: rereading logits from global memory instead of holding a row 279 us,
+// three CTAs an SM (42 registers a thread) 148, 4 CTAs a row 127; lists pulled by rank 0 instead of pushed to it, 130.
 #include <cooperative_groups.h>
 #include <math.h>
 #include <stdint.h>
@@ -663,8 +671,14 @@ cudaError_t launch_sample_rows(SampleRowsArgs a, int n_rows, cudaStream_t stream
                                     kExtra + kSampleSlice * kToken);
     });
     if (e != cudaSuccess) return e;
+    // Several CTAs a row while SMs are idle, as long as a slice is worth a barrier (1 x 32000 8 CTAs 11.7 us, 4 13.7, 1
+    // 27; 16 x 10000 4 CTAs 14.0 us, 8 15.9, 2 15.3), and so that two CTAs fit on an SM (256 x 100003 without filters
+    // 108 us, with slices of 25001 129; top-p alone 254 and 240).
     int ctas = 1;
-    while (ctas < kRowCtas && (n_rows * ctas < 148 || (a.n_vocab + ctas - 1) / ctas > 12800)) ctas *= 2;
+    for (; ctas < kRowCtas; ctas *= 2) {
+        const int slice = (a.n_vocab + ctas - 1) / ctas;
+        if (slice <= 12800 && (slice <= 3000 || n_rows * ctas >= 148)) break;
+    }
     a.slice = (a.n_vocab + ctas - 1) / ctas;
     cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
