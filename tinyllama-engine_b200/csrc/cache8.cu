@@ -443,13 +443,19 @@ __device__ __forceinline__ int64_t walk(WalkSmem& S, const ChunkDesc& d, int n_s
     return blocks_so_far;
 }
 
-// All rows of all sequences, one sequence after another.  HBM-bound: 24 x 8000 rows to bf16 49 us, 4.6 TB/s; 700 rows 3.9 us.
+// All rows of all sequences, one sequence after another.  HBM-bound: 24 x 8000 rows to bf16 44 us, 5.2 TB/s; 700 rows 3.8 us.
 constexpr int kReadBlock = 64;       // the smallest page
-// Rows of a part of a block, the unit of a CTA's work: 16, so that small reads reach all SMs (700 rows 3.8 us,
-// with 64 7.6 us), or whole blocks where there are several for every CTA (24 x 8000: 49 us, with 16 68 us).
-constexpr int kReadFew = 16, kReadMany = 64;
+// Rows of a part of a block, the unit of a CTA's work: 16, so that small reads reach all SMs (700 rows 3.8 us, with 32
+// 4.9, with 64 7.6; 4 x 4000 12.5, with 32 13.8), or 32 where every CTA has a part (16 x 4000 to bf16 22.0 us, with 16
+// 25.1; 60 x 8000 131, with 64 146).
+constexpr int kReadFew = 16, kReadMany = 32;
 constexpr int kReadCtas = 148 * 6;
-inline bool read_many(int64_t rows) { return rows > int64_t{2} * kReadCtas * kReadMany; }
+// go(rows of a part) for a read of so many rows
+template <class F>
+cudaError_t by_part(int64_t rows, F&& go) {
+    return rows > int64_t{1} * kReadCtas * kReadMany ? go(std::integral_constant<int, kReadMany>{})
+                                                     : go(std::integral_constant<int, kReadFew>{});
+}
 template <class Out, int ROWS>
 __global__ void __launch_bounds__(kReadThreads, 6) read8_kernel(const __grid_constant__ Read8Args A) {
     __shared__ WalkSmem S;
@@ -633,23 +639,20 @@ cudaError_t launch_read8(const Read8Args& a, bool out_bf16, bool new_only, cudaS
         return out_bf16 ? cudaLaunchKernelEx(&L.cfg, read8_new_kernel<__nv_bfloat16>, a)
                         : cudaLaunchKernelEx(&L.cfg, read8_new_kernel<float>, a);
     }
-    auto go = [&](auto kernel, int rows) {
-        const int64_t blocks = std::min<int64_t>(kReadCtas, a.n_rows / rows + a.n_seqs);
+    return by_part(a.n_rows, [&](auto part) {
+        const int64_t blocks = std::min<int64_t>(kReadCtas, a.n_rows / part + a.n_seqs);
         Launch L(dim3(static_cast<unsigned>(blocks)), kReadThreads, 0, stream);
-        return cudaLaunchKernelEx(&L.cfg, kernel, a);
-    };
-    if (read_many(a.n_rows))
-        return out_bf16 ? go(read8_kernel<__nv_bfloat16, kReadMany>, kReadMany) : go(read8_kernel<float, kReadMany>, kReadMany);
-    return out_bf16 ? go(read8_kernel<__nv_bfloat16, kReadFew>, kReadFew) : go(read8_kernel<float, kReadFew>, kReadFew);
+        return out_bf16 ? cudaLaunchKernelEx(&L.cfg, read8_kernel<__nv_bfloat16, decltype(part)::value>, a)
+                        : cudaLaunchKernelEx(&L.cfg, read8_kernel<float, decltype(part)::value>, a);
+    });
 }
 
 cudaError_t launch_stage8(const Stage8Args& a, cudaStream_t stream) {
     const int64_t rows = a.n_pages * kStageRows;   // at most: what the workspace has room for
-    auto go = [&](auto kernel, int per) {
-        Launch L(dim3(static_cast<unsigned>(std::min<int64_t>(kReadCtas, std::max<int64_t>(rows / per, 1)))), kReadThreads, 0, stream);
-        return cudaLaunchKernelEx(&L.cfg, kernel, a);
-    };
-    return read_many(rows) ? go(stage8_kernel<kReadMany>, kReadMany) : go(stage8_kernel<kReadFew>, kReadFew);
+    return by_part(rows, [&](auto part) {
+        Launch L(dim3(static_cast<unsigned>(std::min<int64_t>(kReadCtas, std::max<int64_t>(rows / part, 1)))), kReadThreads, 0, stream);
+        return cudaLaunchKernelEx(&L.cfg, stage8_kernel<decltype(part)::value>, a);
+    });
 }
 
 }  // namespace tle
