@@ -32,19 +32,18 @@ namespace {
 
 // ---- append -----------------------------------------------------------------
 // A warp takes a token, or an equal part of its pieces where there are few
-// tokens.  A piece is one load of a warp: as many q heads, k heads or v heads as
-// there are lanes for, 8 (bf16) or 16 (fp32) a head, each with two groups of 8
-// bytes -- with the half layout the two that its pairs lie in, otherwise two in
-// a row -- so that a pair's elements meet in a lane, and the norm's sum and the largest
+// tokens.  A piece is one load of a warp: four q heads, k heads or v heads, 8 lanes
+// a head, each with two groups of 4 elements
+// -- with the half layout the two that its pairs lie in, otherwise two in a
+// row -- so that a pair's elements meet in a lane, and the norm's sum and the largest
 // value of a head are reductions over its lanes.  Sines and cosines are found once a token.
 // HBM-bound: kBatch pieces are in flight, the first ones while the token's place is looked up.  Measured: 4096 tokens of 32 + 4 + 4
 // heads, bf16, into bf16 pages 9.9 us, 4.2 TB/s; 16 x 1501 of 16 + 8 + 8 heads, bf16, normed, into 8-bit pages 34.7 us,
-// 3.8 TB/s (a third of the instructions are the shuffles and roundings of norms and scales); 32 x 1 3.6 us, a launch.
+// 3.8 TB/s (a third of the instructions are the shuffles and roundings of norms and scales); 32 x 1 3.5 us, a launch.
 // Blocks of 32 threads, all of a token's pieces in flight, or parts of two pieces were slower.
 constexpr int kThreads = 64;
-constexpr int kPart = 4;            // pieces of the smallest part of a token
-// Below so many tokens their heads are spread over several warps: 1 x 600 5.6 us (one warp a token 8.2), 1 x 2000 fp32
-// 11.0 us (15.2); twice as many, 1 x 4096 bf16 10.7 us (9.8).
+// Below so many tokens their heads are spread over several warps: 1 x 600 5.4 us (one warp a token 8.2), 1 x 2000 fp32
+// 10.6 us (15.2); twice as many, 1 x 4096 bf16 10.7 us (9.8).
 constexpr int kWarps = 148 * 32;
 
 template <int LANES>
@@ -67,12 +66,15 @@ __device__ __forceinline__ int scale_byte(float most) {
     return (u >> 23) == 255u ? 255 : min(max(b, 1), 248);
 }
 
-// A group of 8 bytes of activations as numbers.
+// A group of 4 activations as numbers.
+constexpr int GE = 4;
 template <class Act>
-constexpr int kGroup = 8 / sizeof(Act);
-__device__ __forceinline__ void group_of(uint2 u, float (&f)[2]) {
+using Group = std::conditional_t<sizeof(Act) == 4, uint4, uint2>;
+__device__ __forceinline__ void group_of(uint4 u, float (&f)[4]) {
     f[0] = __uint_as_float(u.x);
     f[1] = __uint_as_float(u.y);
+    f[2] = __uint_as_float(u.z);
+    f[3] = __uint_as_float(u.w);
 }
 __device__ __forceinline__ void group_of(uint2 u, float (&f)[4]) {
     f[0] = __uint_as_float(u.x << 16);
@@ -81,10 +83,6 @@ __device__ __forceinline__ void group_of(uint2 u, float (&f)[4]) {
     f[3] = __uint_as_float(u.y & 0xffff0000u);
 }
 // (4-byte aligned)
-__device__ __forceinline__ void load_norm(const float* p, float (&f)[2]) {
-    f[0] = p[0];
-    f[1] = p[1];
-}
 __device__ __forceinline__ void load_norm(const float* p, float (&f)[4]) {
     if ((reinterpret_cast<uintptr_t>(p) & 15u) == 0) {
         const float4 x = *reinterpret_cast<const float4*>(p);
@@ -97,15 +95,8 @@ __device__ __forceinline__ void load_norm(const float* p, float (&f)[4]) {
         for (int e = 0; e < 4; ++e) f[e] = p[e];
     }
 }
-template <class T>
-__device__ __forceinline__ void store_group(T* p, const float (&f)[2]) { store_pair(p, make_float2(f[0], f[1])); }
-template <class T>
-__device__ __forceinline__ void store_group(T* p, const float (&f)[4]) { store4(p, f); }
 // Codes of a group, |f| inv <= 127: adding 1.5 * 2^23 rounds to whole numbers, whose low bytes are the codes.
 __device__ __forceinline__ uint32_t code_bits(float y, float inv) { return __float_as_uint(fmaf(y, inv, 12582912.0f)); }
-__device__ __forceinline__ void store_codes(int8_t* p, const float (&f)[2], float inv) {
-    *reinterpret_cast<uint16_t*>(p) = static_cast<uint16_t>(__byte_perm(code_bits(f[0], inv), code_bits(f[1], inv), 0x0040));
-}
 __device__ __forceinline__ void store_codes(int8_t* p, const float (&f)[4], float inv) {
     *reinterpret_cast<uint32_t*>(p) =
         __byte_perm(__byte_perm(code_bits(f[0], inv), code_bits(f[1], inv), 0x0040),
@@ -117,7 +108,6 @@ __global__ void __launch_bounds__(kThreads) append_rules_kernel(const __grid_con
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     asm volatile("griddepcontrol.wait;" ::: "memory");
     constexpr bool kBits8 = sizeof(Pool) == 1;
-    constexpr int GE = kGroup<Act>;
     constexpr int LPH = HD / (2 * GE);
     constexpr int HPW = 32 / LPH;
     const AppendArgs& A = R.a;
@@ -137,7 +127,7 @@ __global__ void __launch_bounds__(kThreads) append_rules_kernel(const __grid_con
     const Act* q = static_cast<const Act*>(A.q) + tok * A.q_stride;
     const Act* k = static_cast<const Act*>(A.k) + tok * A.k_stride;
     const Act* v = static_cast<const Act*>(A.v) + tok * A.v_stride;
-    uint2 x[kBatch][2];
+    Group<Act> x[kBatch][2];
     auto load = [&](int j0) {
 #pragma unroll
         for (int b = 0; b < kBatch; ++b) {
@@ -145,8 +135,8 @@ __global__ void __launch_bounds__(kThreads) append_rules_kernel(const __grid_con
             const int h = (j - base) * HPW + sub;
             const Act* src = (j < nq ? q : j < nq + nk ? k : v) + h * HD;
             const bool in = j < j_end && h < (j < nq ? A.n_head : A.n_head_kv);
-            x[b][0] = in ? *reinterpret_cast<const uint2*>(src + e1) : make_uint2(0, 0);
-            x[b][1] = in ? *reinterpret_cast<const uint2*>(src + e2) : make_uint2(0, 0);
+            x[b][0] = in ? *reinterpret_cast<const Group<Act>*>(src + e1) : Group<Act>{};
+            x[b][1] = in ? *reinterpret_cast<const Group<Act>*>(src + e2) : Group<Act>{};
         }
     };
     load(j_first);
@@ -224,8 +214,8 @@ __global__ void __launch_bounds__(kThreads) append_rules_kernel(const __grid_con
             if (is_q) {
                 if (there) {
                     Act* qo = static_cast<Act*>(A.q_out) + (tok * A.n_head + h) * HD;
-                    store_group(qo + e1, y);
-                    store_group(qo + e2, z);
+                    store4(qo + e1, y);
+                    store4(qo + e2, z);
                 }
                 continue;
             }
@@ -249,8 +239,8 @@ __global__ void __launch_bounds__(kThreads) append_rules_kernel(const __grid_con
                     if (hl == 0) (is_v ? R.value_scale : R.key_scale)[row + (static_cast<size_t>(h) << A.page_shift)] = static_cast<uint8_t>(sb);
                 }
             } else if (there && have) {
-                store_group(to + e1, y);
-                store_group(to + e2, z);
+                store4(to + e1, y);
+                store4(to + e2, z);
             }
         }
         j0 += kBatch;
@@ -607,17 +597,23 @@ static cudaError_t launch_append(const AppendRulesArgs& a, int parts, int64_t bl
 }
 template <class Act, class Pool>
 static cudaError_t launch_append(const AppendRulesArgs& a, cudaStream_t stream) {
-    constexpr int heads = 32 * 2 * kGroup<Act> / HD;   // of a piece
+    constexpr int heads = 32 * 2 * GE / HD;   // of a piece
     const int pieces = (a.a.n_head + heads - 1) / heads + 2 * ((a.a.n_head_kv + heads - 1) / heads);
-    const int most = (pieces + kPart - 1) / kPart;
+    constexpr int part = sizeof(Act) == 4 ? 3 : 4;   // pieces of the smallest part of a token: one turn
+    const int most = (pieces + part - 1) / part;
     const int parts = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(most, kWarps / a.a.n_tokens)));
     const int64_t blocks = (static_cast<int64_t>(a.a.n_tokens) * parts * 32 + kThreads - 1) / kThreads;
     if (blocks > 0x7fffffffLL / (kThreads / 32)) return cudaErrorInvalidConfiguration;
-    // four pieces in flight, or five where that saves a turn (8 pieces of 18 k tokens: 34.7 us with four, 39.5 with
-    // five, for registers; 10 pieces of 4096: 11.0 and 9.8 us)
-    const int mine = (pieces + parts - 1) / parts;
-    return (mine + 4) / 5 < (mine + 3) / 4 ? launch_append<Act, Pool, 5>(a, parts, blocks, stream)
-                                           : launch_append<Act, Pool, 4>(a, parts, blocks, stream);
+    if constexpr (sizeof(Act) == 4) {
+        // three pieces in flight: 1 x 4096 with norms 18.2 us, with two 18.7, with four or five 20.3
+        return launch_append<Act, Pool, 3>(a, parts, blocks, stream);
+    } else {
+        // four pieces in flight, or five where that saves a turn (8 pieces of 18 k tokens: 34.7 us with four, 39.5 with
+        // five, for registers; 10 pieces of 4096: 11.0 and 9.8 us)
+        const int mine = (pieces + parts - 1) / parts;
+        return (mine + 4) / 5 < (mine + 3) / 4 ? launch_append<Act, Pool, 5>(a, parts, blocks, stream)
+                                               : launch_append<Act, Pool, 4>(a, parts, blocks, stream);
+    }
 }
 
 cudaError_t launch_append_rules(const AppendRulesArgs& a, bool act_bf16, int pool_bytes, cudaStream_t stream) {
