@@ -34,8 +34,8 @@ namespace {
 // A warp takes a token, or an equal part of its pieces where there are few
 // tokens.  A piece is one load of a warp: four q heads, k heads or v heads, 8 lanes
 // a head, each with two groups of 4 elements
-// -- with the half layout the two that its pairs lie in, otherwise two in a
-// row -- so that a pair's elements meet in a lane, and the norm's sum and the largest
+// -- with the half layout the two that its pairs lie in, otherwise one of each
+// half of the head, so that a load is of whole sectors -- so that a pair's elements meet in a lane, and the norm's sum and the largest
 // value of a head are reductions over its lanes.  Sines and cosines are found once a token.
 // HBM-bound: kBatch pieces are in flight, the first ones while the token's place is looked up.  Measured: 4096 tokens of 32 + 4 + 4
 // heads, bf16, into bf16 pages 9.9 us, 4.2 TB/s; 16 x 1501 of 16 + 8 + 8 heads, bf16, normed, into 8-bit pages 34.7 us,
@@ -119,9 +119,13 @@ __global__ void __launch_bounds__(kThreads) append_rules_kernel(const __grid_con
     const int part = parts == 1 ? 0 : static_cast<int>(w % parts);
     // this lane's two groups of a head: elements e1 .., e2 ..
     const int hg = R.half / GE;
-    const int g1 = HALF ? (hl < hg ? hl : 2 * hl) : 2 * hl, g2 = HALF && hl < hg ? hl + hg : g1 + 1;
+    // those that are not turned: a head's rest in halves, or, of bf16, two in a row, which takes 8 registers less (16 x 1501
+    // normed into 8 bits and read back 46.1 and 49.1 us)
+    constexpr bool kNext = HALF && sizeof(Act) == 2;
+    const int g1 = HALF && hl >= hg ? (kNext ? 2 * hl : hl + hg) : hl, g2 = HALF && hl < hg ? hl + hg : kNext ? g1 + 1 : hl + LPH;
     const int e1 = g1 * GE, e2 = g2 * GE;
-    const bool turned = A.rotate && (HALF ? hl < hg : e1 < 2 * R.half);
+    const bool turned = A.rotate && (HALF ? hl < hg : e1 < 2 * R.half);   // the first group; the second one:
+    const bool turned2 = HALF ? turned : A.rotate && e2 < 2 * R.half;
     const int nq = (A.n_head + HPW - 1) / HPW, nk = (A.n_head_kv + HPW - 1) / HPW, pieces = nq + 2 * nk;
     const int j_first = parts == 1 ? 0 : part * pieces / parts, j_end = parts == 1 ? pieces : (part + 1) * pieces / parts;
     const Act* q = static_cast<const Act*>(A.q) + tok * A.q_stride;
@@ -167,8 +171,9 @@ __global__ void __launch_bounds__(kThreads) append_rules_kernel(const __grid_con
         c1 *= R.factor;
 #pragma unroll
         for (int e = 0; e < GE; ++e) {
-            cs[e] = __shfl_sync(0xffffffffu, c1, ((HALF ? e1 : e1 / 2) + e) & 31);
-            sn[e] = __shfl_sync(0xffffffffu, s1, ((HALF ? e1 : e1 / 2) + e) & 31);
+            const int i = HALF ? e1 + e : e < GE / 2 ? e1 / 2 + e : e2 / 2 + e - GE / 2;
+            cs[e] = __shfl_sync(0xffffffffu, c1, i & 31);
+            sn[e] = __shfl_sync(0xffffffffu, s1, i & 31);
         }
     }
     for (int j0 = j_first;;) {
@@ -203,6 +208,7 @@ __global__ void __launch_bounds__(kThreads) append_rules_kernel(const __grid_con
                 if (turned) {
 #pragma unroll
                     for (int e = 0; e < GE; ++e) {
+                        if (!HALF && e >= GE / 2 && !turned2) break;
                         float& a = HALF ? y[e] : e < GE / 2 ? y[2 * e] : z[2 * e - GE];
                         float& c = HALF ? z[e] : e < GE / 2 ? y[2 * e + 1] : z[2 * e - GE + 1];
                         const float a0 = a, c0 = c;
