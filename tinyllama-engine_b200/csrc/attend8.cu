@@ -33,8 +33,8 @@ namespace {
 //
 // Measured, 32 heads on 4 (us; bytes of K and V a second): 32 x 1 behind 8000 to 16000, bf16, 49.1,
 // 4.3 TB/s (the copies alone, no step taken, 40.4); 64 x 1 behind 1023 to 2047, fp32, 19.3, 2.6 TB/s
-// (13.6); 1 x 4 behind 700 10.7.  bf16 pages: 71.6, 25.1 and 11.  16 to 32 rows cost 2 or 4
-// such passes over the codes, one for 8 rows: 32 x 4 behind 2000, bf16, 33.6, where bf16 pages take 20.4.
+// (13.6); 1 x 4 behind 700 10.7.  bf16 pages: 71.2, 25.1 and 10.2.  16 to 32 rows cost 2 or 4
+// such passes over the codes, one for 8 rows: 32 x 4 behind 2000, bf16, 32.7, where bf16 pages take 20.3 (fp32 33.7 and 31.8).
 //
 // Tried: 8 to 11 stages, the same; two producers, scales by cp.async, q by copies and records
 // read ahead, joining by a warp of its own or one segment late, no gain; 16- and 64-key steps, slower.

@@ -541,7 +541,7 @@ __global__ void __launch_bounds__(kReadThreads) read8_new_kernel(const __grid_co
 // not take) as bf16 pages of kStageRows rows, and a copy of the descriptor's
 // first records with page tables that lead to them, for the attention over
 // bf16 pages.  Nothing is rounded: the stored values are bf16 numbers.  4 x 601
-// behind up to 2999 rows, 11 us of the call's 84 (over bf16 pages 73.5); 32 x 6 behind 2000, 48 rows a KV head, 30 of 53.
+// behind up to 2999 rows, 11 us of the call's 84 (over bf16 pages 73.5); 32 x 6 behind 2000, 48 rows a KV head, 27 of 50 (bf16 pages 23).
 template <int ROWS>
 __global__ void __launch_bounds__(kReadThreads, 6) stage8_kernel(const __grid_constant__ Stage8Args A) {
     __shared__ WalkSmem S;
