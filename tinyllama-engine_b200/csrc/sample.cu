@@ -29,8 +29,9 @@
 // spread over 8 CTAs a row for latency.
 //
 // Bound by latency: the load, three to six barriers of the cluster, and passes
-// over shared memory between them.  256 x 100003, mixed rules, 124 us, 0.8 TB/s of logits (issue 41 %, DRAM
-// 13 % busy; no filters 108, without the exponentials 71); 1 x 32000 11.7 us (no filters 6.9).
+// over shared memory between them.  256 x 100003, mixed rules, 122 us, 0.8 TB/s of logits (issue 41 %, DRAM
+// 13 % busy; no filters 108, without the exponentials 71); 1 x 32000 11.5 us (no filters 7.0).
+// Weights in bins by three additions of a third each, 124 and 11.7 us.
 // Tried: rereading logits from global memory instead of holding a row 279 us,
 // three CTAs an SM (42 registers a thread) 148, 4 CTAs a row 127; lists pulled by rank 0 instead of pushed to it, 130.
 #include <cooperative_groups.h>
@@ -57,9 +58,6 @@ constexpr int kList = kThreads;            // tokens of a bin that are ranked on
 constexpr uint64_t kFew = 128;             // so many tokens in all are ranked without bins
 constexpr uint64_t kOne = 1ull << 40;      // the largest weight
 constexpr float kReach = 28.6f;            // exp(-kReach) < 2^-41: weights beyond it are 0
-// A weight in three limbs of 14, 13 and 13 bits, so that a bin's sums of 32 bits
-// hold any slice (2^15 tokens).
-constexpr uint32_t kLimb0 = 14, kLimb1 = 13;
 static_assert(kGroups * kRowCtas == kThreads && kBins == 4 * kThreads, "a group of a CTA, and 4 bins, per thread");
 
 __device__ __forceinline__ uint32_t key_of(float x) {
@@ -114,7 +112,7 @@ struct RowRules {
 
 struct alignas(16) Shared {                // the slice lies behind it
     union {
-        uint32_t hist[3][kBins];
+        uint32_t hist[2][kBins];           // a bin's count; or its sum of weights, low and high 32 bits
         struct {                           // once nobody reads the bins any more:
             uint64_t weight[kList];        // the weights and keys of the bin's tokens, of all CTAs
             uint32_t key[kList];
@@ -122,7 +120,7 @@ struct alignas(16) Shared {                // the slice lies behind it
     };
     union {
         uint64_t group[kRowCtas][kGroups]; // sums of 32 bins, of each CTA of the cluster
-        uint32_t fine[3 * kRowCtas][32];   // then the bins of one group
+        uint32_t fine[2 * kRowCtas][32];   // then the bins of one group
     };
     uint32_t list[2][kList];               // of two searches in turn: this CTA's keys of the bin in question
     uint32_t count[2][kRowCtas];           // how many each CTA has
@@ -186,7 +184,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
     const int64_t row = blockIdx.x / cl.n;
     if (tid < 64) S.powers[tid] = kPowers.v[tid];
     if (tid < 2) S.n_last[tid] = 0;
-    for (int i = tid; i < 3 * kBins / 4; i += kThreads) reinterpret_cast<uint4*>(S.hist)[i] = make_uint4(0, 0, 0, 0);
+    for (int i = tid; i < 2 * kBins / 4; i += kThreads) reinterpret_cast<uint4*>(S.hist)[i] = make_uint4(0, 0, 0, 0);
     const int v0 = cl.rank * A.slice, n = max(0, min(A.slice, A.n_vocab - v0));
     // ---- the slice into shared memory, its largest logit ----
     const float* src = A.logits + row * A.stride + v0;
@@ -358,7 +356,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
     // key above `from` first reaches want_of(its sum over all of them).  A want of 0, or of more than there is: no cut.  Cut::ties is then
     // what is to be reached among the tokens of Cut::key.  Tokens below the cut may be dropped.
     auto search = [&]<bool WEIGHT>(uint32_t from, auto&& want_of, Cut& cut) -> bool {
-        constexpr int kLimbs = WEIGHT ? 3 : 1;
+        constexpr int kLimbs = WEIGHT ? 2 : 1;
         const int turn = searches++ & 1;
         uint32_t lo = from + 1, hi = key_of(mx);   // the keys in question
         const float per = R.reach > 0.f ? fminf(kBins / R.reach, 3e38f) : 0.f;   // finite: the largest logit's bin is 0
@@ -432,23 +430,22 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
                 if constexpr (WEIGHT) {
                     const uint64_t w = R.weight(x);
                     if (w == 0) continue;
-                    atomicAdd(&S.hist[0][b], static_cast<uint32_t>(w) & ((1u << kLimb0) - 1));
-                    atomicAdd(&S.hist[1][b], static_cast<uint32_t>(w >> kLimb0) & ((1u << kLimb1) - 1));
-                    atomicAdd(&S.hist[2][b], static_cast<uint32_t>(w >> (kLimb0 + kLimb1)));
+                    // most weights are below 2^32, 1 / 256 of the largest: one addition
+                    const uint32_t low = static_cast<uint32_t>(w), was = atomicAdd(&S.hist[0][b], low);
+                    const uint32_t high = static_cast<uint32_t>(w >> 32) + (was + low < low);
+                    if (high) atomicAdd(&S.hist[1][b], high);
                 } else {
                     atomicAdd(&S.hist[0][b], 1u);
                 }
             }
             __syncthreads();
-            auto limbs = [&](uint32_t a, uint32_t b, uint32_t c) {
-                return WEIGHT ? a + (static_cast<uint64_t>(b) << kLimb0) + (static_cast<uint64_t>(c) << (kLimb0 + kLimb1)) : a;
-            };
+            auto both = [](uint32_t low, uint32_t high) { return low + (static_cast<uint64_t>(high) << 32); };
             // groups of 32 bins: 8 threads each, to all CTAs
             uint64_t sum = 0;
 #pragma unroll
             for (int q = 0; q < 4; ++q) {
                 const int b = tid / 8 * 32 + tid % 8 + 8 * q;
-                sum += WEIGHT ? limbs(S.hist[0][b], S.hist[1][b], S.hist[2][b]) : S.hist[0][b];
+                sum += WEIGHT ? both(S.hist[0][b], S.hist[1][b]) : S.hist[0][b];
             }
 #pragma unroll
             for (int d = 1; d < 8; d *= 2) sum += __shfl_xor_sync(0xffffffffu, sum, d);
@@ -480,7 +477,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
             __syncthreads();
             uint64_t f = 0;
             for (int c = 0; c < cl.n; ++c)
-                f += WEIGHT ? limbs(S.fine[3 * c][lane], S.fine[3 * c + 1][lane], S.fine[3 * c + 2][lane]) : S.fine[c][lane];
+                f += WEIGHT ? both(S.fine[2 * c][lane], S.fine[2 * c + 1][lane]) : S.fine[c][lane];
             const uint64_t fine_upto = before + warp_scan(f);
             const int at = __ffs(__ballot_sync(0xffffffffu, fine_upto >= want)) - 1;
             want -= __shfl_sync(0xffffffffu, fine_upto - f, at);
@@ -671,7 +668,7 @@ cudaError_t launch_sample_rows(SampleRowsArgs a, int n_rows, cudaStream_t stream
                                     kExtra + kSampleSlice * kToken);
     });
     if (e != cudaSuccess) return e;
-    // Several CTAs a row while SMs are idle, as long as a slice is worth a barrier (1 x 32000 8 CTAs 11.7 us, 4 13.7, 1
+    // Several CTAs a row while SMs are idle, as long as a slice is worth a barrier (1 x 32000 8 CTAs 11.5 us, 4 13.7, 1
     // 27; 16 x 10000 4 CTAs 14.0 us, 8 15.9, 2 15.3), and so that two CTAs fit on an SM (256 x 100003 without filters
     // 108 us, with slices of 25001 129; top-p alone 254 and 240).
     int ctas = 1;
