@@ -27,7 +27,7 @@ all: $(LIB) oracle cpptest
 _build:
 	mkdir -p _build
 
-_build/%.o: $(CSRC)/%.cu $(CSRC)/common.cuh $(CSRC)/tcgen05.cuh $(CSRC)/chunk.cuh $(CSRC)/kernels.h include/tle_attn.h include/tle_forward.h | _build
+_build/%.o: $(CSRC)/%.cu $(CSRC)/common.cuh $(CSRC)/tcgen05.cuh $(CSRC)/chunk.cuh $(CSRC)/ring8.h $(CSRC)/kernels.h include/tle_attn.h include/tle_forward.h | _build
 	$(NVCC) $(NVFLAGS) -c $< -o $@
 
 _build/host_%.o: $(HOST)/%.cpp $(HOST)/ops_gpu.h include/tle_attn.h include/tle_forward.h | _build

@@ -17,6 +17,7 @@
 #include "chunk.cuh"
 #include "common.cuh"
 #include "kernels.h"
+#include "ring8.h"
 #include "tcgen05.cuh"
 
 namespace tle {
@@ -59,19 +60,8 @@ namespace {
 // that keeps the largest one between 2^6 and 2^15, whatever V's scales are; m is a whole
 // number.  So all rescaling is exact; m moves when exceeded by more than
 // kMoveThreshold, f when a weight would be above 2^15.
-constexpr int F8_WARPS = 15;       // and the producer: 16 warps, so that a thread may have 128 registers
 constexpr int F8_THREADS = 32 * (F8_WARPS + 1);
-constexpr int F8_STAGES = 11;
-// Teams: a segment ends with its warps' results joined, so a CTA with several segments of few tiles has 3 teams of 5
-// warps, or 2 of 7, that work on segments in turn, each with its own barrier.  One team and as below: 100 x 1 behind 100
-// with 8 KV heads (1 tile) 22.3 and 11.7 us, 256 x 1 behind 500 (3) 33.3 and 28.1, 64 x 1 behind 800 with 8 KV heads (5)
-// 23.6 and 19.7, 256 x 1 behind 2000 (12) 59.9 and 58.3; behind 4000 (24 tiles) 2 teams 59.6 against 53.9: the ring
-// holds too few of them.  Where 4 row groups share 7 warps, 200 x 4 behind 1000 (8 tiles): 109 and 120, so one team.
-constexpr int kThreeTeams = 4, kTwoTeams = 16;   // below so many tiles a segment
-constexpr int kBatch = 3;          // tiles whose copies are issued at once
-constexpr int kStep = 32;           // keys of a step
-constexpr int kSteps = kTile / kStep;
-constexpr int kArrivals = 4 * kSteps;   // of a stage: a step of each of 1, 2 or 4 row groups arrives for 4, 2 or 1
+static_assert(kRingTile == kTile, "the ring's tiles");
 constexpr int kFlush = 4;          // steps of a warp whose MMAs are summed in a row
 constexpr int kQBits = 12;         // the largest element of q in [2^12, 2^13)
 constexpr int kWeightBits = 15, kWeightStart = 6;
@@ -129,6 +119,15 @@ __device__ __forceinline__ void tma_load_3d(void* dst, const CUtensorMap* map, i
 }
 __device__ __forceinline__ void mbar_arrive_n(uint64_t* bar, uint32_t n) {
     asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0], %1;" ::"r"(smem_u32(bar)), "r"(n) : "memory");
+}
+// The count of begun tiles, between the producer and the warps: who reads it has seen what came before it.
+__device__ __forceinline__ int load_acquire(const int* p) {
+    int x;
+    asm volatile("ld.acquire.cta.shared::cta.b32 %0, [%1];" : "=r"(x) : "r"(smem_u32(p)) : "memory");
+    return x;
+}
+__device__ __forceinline__ void store_release(int* p, int x) {
+    asm volatile("st.release.cta.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(p)), "r"(x) : "memory");
 }
 __device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
     uint32_t r;
@@ -215,14 +214,14 @@ __global__ void __launch_bounds__(F8_THREADS, 1)
                     b0 = per_tile * n0;
                     refill();
                 }
-                const int n = n0 + min(lane, count - 1), mine = ring + n - n0, st = mine % F8_STAGES;
+                const int n = n0 + min(lane, count - 1), mine = ring + n - n0, st = ring_stage(mine);
                 const int id0 = __shfl_sync(0xffffffffu, id, per_tile * n - b0);
                 const int id1 = per_tile == 2 ? __shfl_sync(0xffffffffu, id, per_tile * n - b0 + 1) : -1;
-                wait_or_flag(&S.empty[st], ((mine / F8_STAGES) & 1) ^ 1, A.err, kErrWaitEmpty, failed);
+                wait_or_flag(&S.empty[st], ring_parity(mine) ^ 1, A.err, kErrWaitEmpty, failed);
                 failed = __any_sync(0xffffffffu, failed);
                 if (failed) break;
                 ring += count;
-                if (lane == 0) *const_cast<volatile int*>(&S.issued) = ring;
+                if (lane == 0) store_release(&S.issued, ring);
                 if (__any_sync(0xffffffffu, id0 == -2 || id1 == -2)) {
                     for (int e = 0; e < count * per_tile; ++e) {
                         const int to = __shfl_sync(0xffffffffu, st, e / per_tile), b = e % per_tile;
@@ -259,7 +258,7 @@ __global__ void __launch_bounds__(F8_THREADS, 1)
         // no copy may still be in flight when the CTA leaves, after a wait that expired neither
         bool late = false;
         for (int u = ring > F8_STAGES ? ring - F8_STAGES : 0; u < ring; ++u)
-            wait_or_flag(&S.full[u % F8_STAGES], (u / F8_STAGES) & 1, A.err, kErrDrain, late);
+            wait_or_flag(&S.full[ring_stage(u)], ring_parity(u), A.err, kErrDrain, late);
         return;
     }
     auto consume = [&]<bool ONE>(int n_teams) {
@@ -277,14 +276,11 @@ __global__ void __launch_bounds__(F8_THREADS, 1)
             piece[h] = line * 2 * HD + ((((r & 1) * 4 + 2 * h + (mi >> 1)) ^ line) << 4);
         }
         static_assert(kChunkFewRows <= 32 && F8_WARPS < 32, "four row groups at most");
-        // row groups of 8 rows: 1, 2 or 4 (as a power of two), the warps dealt out to them
-        auto group_bits = [](int n_rows) { return n_rows <= 8 ? 0 : n_rows <= 16 ? 1 : 2; };
-        auto workers = [&](int gb, int rg) { return (in_team - rg + (1 << gb) - 1) >> gb; };   // warps of row group rg
         // This lane's elements 16 c + 4 t .. + 3 of row g of the warp's group, ahead of the segment.
         using Raw = std::conditional_t<sizeof(Act) == 4, uint4, uint2>;
         Raw raw[HD / 16];
         auto load_q = [&](const Work& w) {
-            const int r = (tw & ((1 << group_bits(w.n_rows)) - 1)) * 8 + g;
+            const int r = (tw & ((1 << ring_group_bits(w.n_rows)) - 1)) * 8 + g;
             const bool ok = r < w.n_rows;
             const int row = w.row0 + (ok ? r : 0), tok = row_token(A, row), h = row - tok * A.group;
             const Raw* src = reinterpret_cast<const Raw*>(static_cast<const Act*>(A.q) +
@@ -294,14 +290,11 @@ __global__ void __launch_bounds__(F8_THREADS, 1)
             for (int i = 0; i < HD / 16; ++i) raw[i] = ok ? src[4 * i] : Raw{};
         };
         int ring0 = 0;   // tiles of the segments before
-        // A stage's barrier tells one lap of the ring from the next only: with several teams no warp looks for a
-        // tile before the producer has begun with it, which it does when the stage's last one has been used.
-        int issued = ONE ? INT32_MAX : 0;
+        int issued = 0;  // tiles that the producer is known to have begun to copy
         auto begun = [&](int ring) {
-            if (ONE) return;
             uint64_t t_first = 0;
             for (int i = 1; issued <= ring && !failed; ++i) {
-                issued = *const_cast<volatile int*>(&S.issued);
+                issued = load_acquire(&S.issued);
                 if (i % 256 == 0) {
                     const uint64_t now = globaltimer();
                     if (t_first == 0) t_first = now;
@@ -311,11 +304,16 @@ __global__ void __launch_bounds__(F8_THREADS, 1)
                     }
                 }
             }
+            return !failed;
+        };
+        auto full = [&](int st, uint32_t parity) {
+            wait_or_flag(&S.full[st], parity, A.err, kErrWaitFull, failed);
+            return !failed;
         };
         auto segment = [&](const Work& w) {
             // w may lie in either memory: what the steps need of it is held in registers
             const int t0 = w.t0, pos_min = w.pos_min, kv_len = w.kv_len;
-            const int gb = group_bits(w.n_rows), rg = tw & ((1 << gb) - 1), kw = tw >> gb;
+            const int gb = ring_group_bits(w.n_rows), rg = tw & ((1 << gb) - 1), kw = tw >> gb;
             const int pos_r = w.pos + row_token(A, w.row0 + min(rg * 8 + g, w.n_rows - 1));
             uint32_t qf[HD / 16][4];   // A fragments: rows g the first terms, rows g + 8 the second
             float c;                   // of the row's scores: 2^e / 8 log2(e), q = 2^e (terms)
@@ -495,11 +493,10 @@ __global__ void __launch_bounds__(F8_THREADS, 1)
                 }
             };
             // the steps of the segment, dealt out to the group's warps
-            const int n_steps = (w.t1 - t0) * kSteps, nkw = workers(gb, rg);
+            const int n_steps = (w.t1 - t0) * kSteps, nkw = ring_workers(in_team, gb, rg);
             for (int i = kw; i < n_steps; i += nkw) {
-                const int n = t0 + i / kSteps, ring = ring0 + i / kSteps, st = ring % F8_STAGES;
-                begun(ring);
-                wait_or_flag(&S.full[st], (ring / F8_STAGES) & 1, A.err, kErrWaitFull, failed);
+                const int n = t0 + i / kSteps, ring = ring0 + i / kSteps, st = ring_stage(ring);
+                ring_ready(ring, begun, full);   // after a wait that expired the warp goes on, in bounds
                 __syncwarp();
                 if (n * kTile + kTile - 1 > pos_min) step.template operator()<true>(st, n, kStep * (i % kSteps));
                 else step.template operator()<false>(st, n, kStep * (i % kSteps));
@@ -533,9 +530,9 @@ __global__ void __launch_bounds__(F8_THREADS, 1)
             named_bar_sync(1 + team, 32 * in_team);
             // ---- join the key workers: a row per warp, two columns per lane; lane q has the
             // weight of worker q ----
-            const int gb = group_bits(w.n_rows);
+            const int gb = ring_group_bits(w.n_rows);
             for (int r = tw; r < w.n_rows; r += in_team) {
-                const int w0 = r >> 3, rr = r & 7, nkw = workers(gb, w0);
+                const int w0 = r >> 3, rr = r & 7, nkw = ring_workers(in_team, gb, w0);
                 const float2 ml = lane < nkw ? S.ml[team * in_team + w0 + (lane << gb)][rr] : make_float2(-INFINITY, 0.f);
                 float m_all = ml.x;
 #pragma unroll
@@ -566,9 +563,8 @@ __global__ void __launch_bounds__(F8_THREADS, 1)
             named_bar_sync(1 + team, 32 * in_team);
         }
     };
-    const int n_segs = seg1 - seg0, each = n_segs > 0 ? (S.work[0].cta_tiles - 1) / n_segs : 0;
-    const bool two = each < kTwoTeams && n_segs > 2 && S.work[0].n_rows <= 16;
-    const int n_teams = each < kThreeTeams ? min(n_segs, 3) : two ? 2 : 1;
+    const int n_segs = seg1 - seg0;
+    const int n_teams = ring_teams(n_segs, n_segs > 0 ? S.work[0].cta_tiles : 0, n_segs > 0 ? S.work[0].n_rows : 0);
     if (n_teams <= 1) consume.template operator()<true>(1);
     else consume.template operator()<false>(n_teams);
 }
