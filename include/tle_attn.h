@@ -450,7 +450,9 @@ typedef struct {
  *   TLE_ROPE_SCALE_NTK     f_i with the base base * factor^(rotary_dim / (rotary_dim - 2))
  *   TLE_ROPE_SCALE_YARN    f_i where a pair turns more than 32 times within
  *                          original_ctx, f_i / factor where less than once, and
- *                          a linear ramp over the pairs in between;
+ *                          a linear ramp over the pairs in between (its ends
+ *                          are whole pairs, rounded away from the ramp, the
+ *                          first one not below 0);
  *                          *rope_factor = 1 + 0.1 ln(factor), otherwise 1. */
 enum { TLE_ROPE_SCALE_NONE = 0, TLE_ROPE_SCALE_LINEAR = 1, TLE_ROPE_SCALE_NTK = 2, TLE_ROPE_SCALE_YARN = 3 };
 int tle_rope_frequencies(int kind, float base, int rotary_dim, float factor, int original_ctx,

@@ -2033,15 +2033,15 @@ int tle_rope_frequencies(int kind, float base, int rotary_dim, float factor, int
         auto pair_of = [&](double turns) {
             return d * std::log(original_ctx / (turns * 2 * 3.14159265358979323846)) / (2 * std::log(b));
         };
+        // the ramp's ends, whole pairs: the last one may lie behind the head's, whose pairs then all turn more than once
         lo = std::max(std::floor(pair_of(32)), 0.0);
-        hi = std::min(std::ceil(pair_of(1)), d / 2 - 1);
-        if (hi <= lo) hi = lo + 0.001;
+        hi = std::ceil(pair_of(1));
     }
     for (int i = 0; i < rotary_dim / 2; ++i) {
         double f = std::pow(b, -2.0 * i / d);
         if (kind == TLE_ROPE_SCALE_LINEAR) f /= factor;
         if (kind == TLE_ROPE_SCALE_YARN) {
-            const double slow = std::min(std::max((i - lo) / (hi - lo), 0.0), 1.0);
+            const double slow = i >= hi ? 1.0 : i <= lo ? 0.0 : (i - lo) / (hi - lo);
             f = f * (1 - slow) + f / factor * slow;
         }
         inv_freq[i] = static_cast<float>(f);
