@@ -657,6 +657,8 @@ class PagedDecodeBatch:
     def __init__(self, cache: PagedKVCache, tables: Sequence, positions: Sequence[int],
                  max_ctas: int = 0):
         import torch
+        if cache.dtype != torch.float32:
+            raise ValueError(f"a float32 PagedKVCache expected, got {cache.dtype}")
         self.cache = cache
         self.shape = cache.shape
         self.tables = list(tables)
