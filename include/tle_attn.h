@@ -510,10 +510,14 @@ int tle_read_q8_paged(const tle_shape_t* shape, const tle_page_pool_q8_t* pool, 
                       int64_t n_rows, int out_type, int layer, int flags, void* stream);
 
 /* tle_prefill_bf16_paged over 8-bit pages, with the same descriptor and the
- * same contract; q and the softmax weights enter as sums of two fp16 numbers
- * (24 bits) where a chunk has at most 32 rows per KV head, and as for bf16 pages
- * otherwise.  Chunks of more rows are attended to over a bf16 copy of their
- * sequences' rows in the workspace, which nothing is rounded for. */
+ * same contract.  Where a chunk has at most 32 rows per KV head, q and the
+ * softmax weights enter as sums of two fp16 numbers (22 bits and rounding: within
+ * 2^-23 of a row's largest element; a row of q whose largest element is below
+ * 2^-111 counts with fewer bits).  Chunks of more rows are as over bf16 pages: with
+ * bf16 activations the weights are rounded to bf16, so that a result is off by
+ * 1.4 times what one rounding to bf16 leaves (root mean square).  They are attended to over a
+ * bf16 copy of their sequences' rows of the layer in the workspace, which nothing is
+ * rounded for: n_head_kv * 256 bytes a row, in whole pages of 128 rows. */
 size_t tle_prefill_q8_paged_workspace_bytes(const tle_shape_t* shape, const tle_paged_chunk_t* chunks, int n_seqs,
                                             const tle_chunk_plan_t* plan);
 /* workspace: 16-byte aligned, at least that many bytes.  Where a captured call

@@ -32,10 +32,10 @@ namespace {
 // own running maximum, sum and output, joined in shared memory at the segment's
 // end.
 //
-// Measured, 32 heads on 4 (us; bytes of K and V a second): 32 x 1 behind 8000 to 16000, bf16, 49.1,
-// 4.3 TB/s (the copies alone, no step taken, 40.4); 64 x 1 behind 1023 to 2047, fp32, 19.3, 2.6 TB/s
+// Measured, 32 heads on 4 (us; bytes of K and V a second): 32 x 1 behind 8000 to 16000, bf16, 49.8,
+// 4.3 TB/s (the copies alone, no step taken, 40.4); 64 x 1 behind 1023 to 2047, fp32, 19.5, 2.6 TB/s
 // (13.6); 1 x 4 behind 700 10.7.  bf16 pages: 71.2, 25.1 and 10.2.  16 to 32 rows cost 2 or 4
-// such passes over the codes, one for 8 rows: 32 x 4 behind 2000, bf16, 32.7, where bf16 pages take 20.3 (fp32 33.7 and 31.8).
+// such passes over the codes, one for 8 rows: 32 x 4 behind 2000, bf16, 34.2, where bf16 pages take 20.3 (fp32 34.5 and 31.8).
 //
 // Tried: 8 to 11 stages, the same; two producers, scales by cp.async, q by copies and records
 // read ahead, joining by a warp of its own or one segment late, no gain; 16- and 64-key steps, slower.
@@ -51,8 +51,9 @@ namespace {
 // fragments share, V's by two dimensions in turn.
 //
 // Precision: q (times a power of two per row) and the weights enter as sums of
-// two fp16 numbers, 22 bits and rounding: within 2^-24 of the largest element,
-// as 32-bit arithmetic is.  The second terms are rows 8 to 15 of the A
+// two fp16 numbers, 22 bits and rounding: within 2^-23 of a row's largest element,
+// twice a rounding to 32 bits (4096 + 1 + 2^-11 becomes 4097).  A row of q whose largest element is below 2^-111 has
+// fewer bits: its factor on the scores is then a subnormal number.  The second terms are rows 8 to 15 of the A
 // fragments, so they cost no MMA.  Tensor cores cut their running sums off, so
 // the output is carried on in 32-bit sums in shared memory every kFlush steps.
 //

@@ -18,9 +18,9 @@ constexpr int F8_WARPS = 15;       // and the producer: 16 warps, so that a thre
 constexpr int F8_STAGES = 11;
 // Teams: a segment ends with its warps' results joined, so a CTA with several segments of few tiles has 3 teams of 5
 // warps, or 2 of 7, that work on segments in turn, each with its own barrier.  One team and as below: 100 x 1 behind 100
-// with 8 KV heads (1 tile) 22.3 and 11.7 us, 256 x 1 behind 500 (3) 33.3 and 28.1, 64 x 1 behind 800 with 8 KV heads (5)
-// 23.6 and 19.7, 256 x 1 behind 2000 (12) 59.9 and 58.3; behind 4000 (24 tiles) 2 teams 59.6 against 53.9: the ring
-// holds too few of them.  Where 4 row groups share 7 warps, 200 x 4 behind 1000 (8 tiles): 109 and 120, so one team.
+// with 8 KV heads (1 tile) 22.3 and 11.9 us, 256 x 1 behind up to 500 (3) 34.3 and 28.0, 64 x 1 behind up to 800 with 8 KV
+// heads (5) 24.0 and 19.7, 256 x 1 behind up to 2000 (12) 60.9 and 58.6; behind up to 4000 (24 tiles) 93.7 and 104.8: the
+// ring holds too few of them.  Where 4 row groups share 7 warps, 200 x 4 behind 1000 (8 tiles): 113 and 128, so one team.
 constexpr int kThreeTeams = 4, kTwoTeams = 16;   // below so many tiles a segment
 constexpr int kBatch = 3;          // tiles whose copies are issued at once
 constexpr int kRingTile = 128;     // keys of a tile (kChunkTile)
