@@ -99,18 +99,6 @@ __device__ __forceinline__ void mma_f16_zero(float (&d)[4], const uint32_t (&a)[
         : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.f));
 }
-__device__ __forceinline__ void ldsm4_b(uint32_t addr, uint32_t (&r)[4]) {
-    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
-                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
-                 : "r"(addr)
-                 : "memory");
-}
-__device__ __forceinline__ void ldsm4_bt(uint32_t addr, uint32_t (&r)[4]) {
-    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
-                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
-                 : "r"(addr)
-                 : "memory");
-}
 __device__ __forceinline__ void tma_load_3d(void* dst, const CUtensorMap* map, int x, int y, int z, uint64_t* bar) {
     asm volatile(
         "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes "
@@ -403,7 +391,7 @@ __global__ void __launch_bounds__(F8_THREADS, 1)
                     // matrices: keys 0-7 and 8-15 of chunks 0, 1; then of 2, 3
                     uint32_t kr[2][4];
 #pragma unroll
-                    for (int h = 0; h < 2; ++h) ldsm4_b(kb + 16 * b2 * HD + piece[h], kr[h]);
+                    for (int h = 0; h < 2; ++h) ldsm4(kb + 16 * b2 * HD + piece[h], kr[h]);
 #pragma unroll
                     for (int ks = 0; ks < HD / 16; ++ks)
 #pragma unroll
@@ -481,7 +469,7 @@ __global__ void __launch_bounds__(F8_THREADS, 1)
                 for (int b2 = 0; b2 < B / 2; ++b2) {
                     uint32_t vr[2][4], pf[4];
 #pragma unroll
-                    for (int h = 0; h < 2; ++h) ldsm4_bt(vb + 16 * b2 * HD + piece[h], vr[h]);
+                    for (int h = 0; h < 2; ++h) ldsm4_t(vb + 16 * b2 * HD + piece[h], vr[h]);
                     two_terms(wt[4 * b2] * f, wt[4 * b2 + 1] * f, pf[0], pf[1]);
                     two_terms(wt[4 * b2 + 2] * f, wt[4 * b2 + 3] * f, pf[2], pf[3]);
 #pragma unroll
