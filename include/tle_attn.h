@@ -460,7 +460,8 @@ int tle_rope_frequencies(int kind, float base, int rotary_dim, float factor, int
 
 /* tle_append_paged / tle_append_bf16_paged by rules: q and k heads are normed,
  * then (flags & TLE_DECODE_ROTATE) rotated by angle fl32(p * inv_freq[i]), v is
- * stored as it is.  Everything in 32 bits, rounded once. */
+ * stored as it is.  Everything in 32 bits, rounded once; a norm's squares too, so
+ * that heads to be normed stay below 2^61, and with an eps of 0 above 2^-63. */
 int tle_append_rules_paged(const tle_shape_t* shape, const tle_page_pool_t* pool, const tle_chunk_plan_t* plan,
                            const void* desc_dev, const void* q, int64_t q_stride, const void* k,
                            int64_t k_stride, const void* v, int64_t v_stride, void* q_out, int act_type,

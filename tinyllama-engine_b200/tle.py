@@ -739,6 +739,9 @@ class AppendRules:
         rope_frequencies; rope_factor: on sine and cosine;
     q_norm, k_norm  float32 CUDA [64] or None: heads become
         x / sqrt(mean(x^2) + eps) * norm before they are rotated.
+
+    The norms stay with the object: it has to live until the calls that were
+    given it are done, on whatever stream, and as long as a graph that holds one.
     """
 
     def __init__(self, layout: str = "interleaved", rotary_dim: Optional[int] = None, inv_freq=None, rope_factor: float = 1.0,
@@ -1255,6 +1258,8 @@ class SampleRules:
     top_k        int32: the first top_k tokens of the ranking (0: all);
     min_p        float32: tokens of at least min_p times the largest probability;
     top_p        float32: the first tokens whose probabilities reach top_p.
+
+    The tensors stay with the object, which has to live as AppendRules.
     """
 
     def __init__(self, n_rows: int, n_vocab: int, temperature=None, top_k=None, top_p=None, min_p=None):
